@@ -383,6 +383,78 @@ int lq_sparse_row_add(const void* x, int dtype, int64_t M, int64_t K, int64_t N,
                       const int32_t* row_ptr, const int32_t* row_ids, int64_t n_rows,
                       const int32_t* cols, const float* vals, void* y, void* stream);
 
+/* ---- KV cache in 4 bits ---------------------------------------------------------
+ * No counterpart in the reference, whose caches keep a byte or more per code
+ * (kv_cache_quant.py:168-193).  Buffers of one layer, allocated by the caller
+ * and changed only by the calls below; cap is a multiple of 32, D is 64 or 128:
+ *   k_codes, v_codes [B, H, cap, D / 2] bytes: two codes per byte, in the
+ *       orders that lq_kv4.cuh describes;
+ *   params [B, H, cap] of two 32-bit words (K's, V's): scale as bf16 in the low
+ *       half, zero point as bf16 in the high half;
+ *   positions [B, H, cap] (-1: empty slot), mass [B, H, cap] attention weight
+ *       that a token has collected (0: empty slot);
+ *   state [2 B + 3]: tokens held and position of the next token of each
+ *       sequence, a ticket of the calls, tokens that found no room, and whether
+ *       anything was evicted (until then a token's slot is its position).
+ * A new cache has positions -1 and all of mass and state 0.  The lengths are
+ * the device's: no call reads them on the host, so a captured call sees the
+ * lengths of its replay.  Calls on one cache must not run at the same time,
+ * except lq_kv4_attention without `accumulate` and lq_kv4_dequant.
+ *
+ * value = (code - zero) * scale per token and head over its D values, in fp32:
+ * lo = min(0, min x), hi = max(0, max x), scale = bf16((hi - lo) / 15), zero =
+ * clamp(rint(-lo / scale), 0, 15), code = clamp(rint(x / scale) + zero, 0, 15).
+ * A range that is not finite reads as NaN, a scale below 2^-100 as zeros. */
+typedef struct {
+  void* k_codes;
+  void* v_codes;
+  void* params;
+  int32_t* positions;
+  float* mass;
+  int32_t* state;
+  int64_t B, H, cap, D;
+} lq_kv4_cache;
+
+/* Append S tokens: k, v [B, H, S, D] with element strides sb, sh, ss (multiples
+ * of 4, as are the base addresses) and D contiguous.  counts [B] (device, may
+ * be NULL: S): tokens of each sequence, from the front of the chunk; what lies
+ * behind them is padding and is not read.  Tokens past cap are dropped and
+ * counted in state. */
+int lq_kv4_append(const lq_kv4_cache* host_cache, const void* k, const void* v, int dtype, int64_t S,
+                  int64_t k_sb, int64_t k_sh, int64_t k_ss, int64_t v_sb, int64_t v_sh, int64_t v_ss,
+                  const int32_t* counts, void* stream);
+/* Values of the first n slots as k, v [B, H, n, D] (float dtype, rounded once);
+ * zeros past a sequence's length. */
+int lq_kv4_dequant(const lq_kv4_cache* host_cache, int64_t n, int dtype, void* k, void* v, void* stream);
+/* Cut every sequence back to at most `keep` tokens per head: the `recent` last
+ * positions and the positions below `sinks` stay, then the tokens with the
+ * greatest mass (NaN counts as greatest, equal mass from the lowest slot up).
+ * Tokens that stay and lie at or above slot `keep` move, in order, into the
+ * slots that came free below it. */
+size_t lq_kv4_evict_workspace_bytes(int64_t B, int64_t H, int64_t cap, int64_t keep);
+int lq_kv4_evict(const lq_kv4_cache* host_cache, int64_t keep, int64_t recent, int64_t sinks,
+                 void* workspace, size_t workspace_bytes, void* stream);
+/* softmax attention of q [B, Hq, Sq, D] (strides as above, query head h reads
+ * kv head h / (Hq / H)) over the cached tokens, out [B, Hq, Sq, D] contiguous
+ * in q's dtype.  The queries are the last tokens of their sequences: query i
+ * of sequence b has position next[b] - counts[b] + i (counts NULL: Sq); rows
+ * from counts[b] on are padding and come out as zeros, as do rows that see no
+ * token.  Score of a query at position p and a token at position t:
+ *   x = sm_scale * q.k;  softcap > 0: x = softcap * tanh(x / softcap);
+ *   slopes [Hq] not NULL: x -= slopes[h] * |p - t|
+ * and the query sees the token when
+ *   ((not causal or t <= p) and (window <= 0 or p - t < window))
+ *   or (prefix not NULL and t < prefix[b]).
+ * accumulate: mass of each token += the weights it got from all query rows.
+ * bound: tokens that the longest sequence is thought to hold (only the split
+ * of the work goes by it).  The workspace is for this call alone. */
+size_t lq_kv4_attention_workspace_bytes(const lq_kv4_cache* host_cache, int q_dtype, int64_t Hq, int64_t Sq,
+                                        int64_t bound, int accumulate);
+int lq_kv4_attention(const lq_kv4_cache* host_cache, const void* q, int q_dtype, int64_t Hq, int64_t Sq,
+                     int64_t q_sb, int64_t q_sh, int64_t q_ss, int64_t bound, const int32_t* counts,
+                     float sm_scale, int causal, float softcap, const float* slopes, int64_t window,
+                     const int32_t* prefix, int accumulate, void* out, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -78,6 +78,11 @@ _SIGS = {
                         _V, _I, _L, _V, _V, _L,
                         _V, _I, _L, _V, _V, _L,
                         _I, ctypes.c_float, _I, _V, _V, ctypes.c_size_t, _V],
+    "lq_kv4_append": [_V, _V, _V, _I, _L, _L, _L, _L, _L, _L, _L, _V, _V],
+    "lq_kv4_dequant": [_V, _L, _I, _V, _V, _V],
+    "lq_kv4_evict": [_V, _L, _L, _L, _V, ctypes.c_size_t, _V],
+    "lq_kv4_attention": [_V, _V, _I, _L, _L, _L, _L, _L, _L, _V, ctypes.c_float, _I, ctypes.c_float,
+                         _V, _L, _V, _I, _V, _V, ctypes.c_size_t, _V],
 }
 _SIZE_SIGS = {
     "lq_tensor_qparams_workspace_size": [_L],
@@ -85,7 +90,16 @@ _SIZE_SIGS = {
     "lq_w4a16_packed_bytes": [_L, _L, _L],
     "lq_nf4_linear_packed_bytes": [_L, _L],
     "lq_kv_attention_workspace_bytes": [_L, _L, _L, _L, _L, _L],
+    "lq_kv4_evict_workspace_bytes": [_L, _L, _L, _L],
+    "lq_kv4_attention_workspace_bytes": [_V, _I, _L, _L, _L, _I],
 }
+
+
+class KV4Cache(ctypes.Structure):
+    """lq_kv4_cache"""
+    _fields_ = [(n, _V) for n in ("k_codes", "v_codes", "params", "positions", "mass", "state")] + \
+               [(n, _L) for n in ("B", "H", "cap", "D")]
+
 
 _lib = None
 _lock = threading.Lock()

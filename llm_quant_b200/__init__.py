@@ -15,7 +15,10 @@ hand-written CUDA kernels in ``liblq_sm100.so`` on CUDA tensors:
   calibration helpers (eager PyTorch, off the hot path);
 * ``llm_quant_b200.qlora``: NF4 quantize / dequantize, double quantization,
   QLoRALinear (packed 4-bit storage), QLoRA;
-* ``llm_quant_b200.kv_cache_quant``: KV-cache quantizers and QuantizedKVCache.
+* ``llm_quant_b200.kv_cache_quant``: KV-cache quantizers and QuantizedKVCache;
+* ``llm_quant_b200.packed_kv_cache``: PackedKVCache, a KV cache held in 4 bits
+  with its attention, collected attention weights and eviction (beyond the
+  reference).
 
 ``install_as_llm_quant()`` registers these modules under the reference's
 import names (``llm_quant``, ``llm_quant.core.quantizer``, ...) for code
@@ -62,6 +65,7 @@ from .kv_cache_quant import (
     PerTokenKVCacheQuantizer, PerChannelKVCacheQuantizer,
     PerGroupKVCacheQuantizer, kv_cache_memory_ratio,
 )
+from .packed_kv_cache import PackedKVCache
 from .gptq import GPTQLinear
 from .spqr import SpQRLinear
 
@@ -82,6 +86,7 @@ __all__ = [
     "KVQuantGranularity", "KVCacheQuantizer", "QuantizedKVCache",
     "PerTokenKVCacheQuantizer", "PerChannelKVCacheQuantizer",
     "PerGroupKVCacheQuantizer", "kv_cache_memory_ratio",
+    "PackedKVCache",
     "GPTQLinear", "SpQRLinear",
     "install_as_llm_quant",
 ]

@@ -28,7 +28,8 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-I", INCLUDE,
           "--expt-relaxed-constexpr"]
 # sources whose arithmetic must not be contracted (bit-exact parity)
-EXACT = {"lq_group.cu", "lq_kv.cu", "lq_nf4.cu", "lq_hadamard.cu", "lq_affine.cu", "lq_api.cu"}
+EXACT = {"lq_group.cu", "lq_kv.cu", "lq_nf4.cu", "lq_hadamard.cu", "lq_affine.cu", "lq_api.cu",
+         "lq_kv4_store.cu"}
 
 
 def nvcc() -> str:

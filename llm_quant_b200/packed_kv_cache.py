@@ -1,0 +1,303 @@
+"""llm_quant_b200.packed_kv_cache -- a KV cache held in 4 bits a value.
+
+``QuantizedKVCache`` keeps a byte (or two) per code whatever the quantizer's
+width, one length for the whole batch, and rebuilds nothing but plain
+attention.  ``PackedKVCache`` stores two codes per byte (head dim 128: 136
+bytes per token and head for K and V, of 512 in 16 bits), gives each sequence
+of the batch a length of its own, attends single tokens and prompt chunks with
+the score forms that models use (tanh cap, distance bias, sliding window,
+prefix), collects the attention weight of each cached token, and evicts by it.
+
+Quantization, per token and kv head over the head dim, in fp32:
+
+    lo = min(0, min x)   hi = max(0, max x)   scale = bf16((hi - lo) / 15)
+    zero = clamp(rint(-lo / scale), 0, 15)    code = clamp(rint(x / scale) + zero, 0, 15)
+    value = (code - zero) * scale
+
+This is KVCacheQuantizer(4, symmetric=False, PER_TOKEN) (kv_cache_quant.py:102-139,
+168-193) but for three choices: the range always holds 0 (the reference clamps
+a zero point that falls outside, and saturates), arithmetic is in fp32 whatever
+the input's dtype (the reference rounds each operation to it, which turns an
+all-zero fp16 token into NaN), and the scale is kept in bf16.
+
+Lengths live on the device and nothing here reads them back, so every method
+can be captured into a CUDA graph and replayed: a replayed ``append`` goes on
+where the last one stopped.  The host keeps an upper bound of them
+(``seq_len``), which sizes what ``get``, ``positions`` and ``attention_mass``
+return; inside a capture, and from then on until ``reset``, it is the capacity.
+
+One cache is used by one stream at a time (``attend`` without ``accumulate``
+and ``get`` may overlap each other), as any tensor that is changed in place.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple, Union
+
+import torch
+import torch.nn as nn
+
+from . import _C
+
+
+class _LayerStore:
+    """Device buffers of one layer."""
+
+    def __init__(self, B: int, H: int, cap: int, D: int, device):
+        self.B, self.H, self.cap, self.D, self.device = B, H, cap, D, device
+
+        def new(fill, *shape, dtype=torch.int32):
+            return torch.full(shape, fill, dtype=dtype, device=device)
+
+        # codes are read in whole tiles, past the last token too: any code will do there
+        self.k_codes = torch.empty(B, H, cap, D // 2, dtype=torch.uint8, device=device)
+        self.v_codes = torch.empty_like(self.k_codes)
+        self.params = torch.empty(B, H, cap, 2, dtype=torch.int32, device=device)
+        self.positions = new(-1, B, H, cap)
+        self.mass = new(0.0, B, H, cap, dtype=torch.float32)
+        self.state = new(0, 2 * B + 3)
+        self.bound = 0        # no sequence holds more tokens, as far as the host knows
+        self.captured = False  # an append was captured: replays are not seen by the host
+        self.c = _C.KV4Cache(self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.params.data_ptr(),
+                             self.positions.data_ptr(), self.mass.data_ptr(), self.state.data_ptr(),
+                             B, H, cap, D)
+        self.ref = ctypes.byref(self.c)
+
+    def clear(self) -> None:
+        self.positions.fill_(-1)
+        self.mass.zero_()
+        self.state.zero_()
+        self.bound = 0
+        self.captured = False
+
+
+def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
+    """x with rows that the kernels can load: D contiguous, each row on a
+    multiple of 4 elements.  A transposed projection qualifies as it is."""
+    sb, sh, ss, sd = x.stride()
+    if sd == 1 and not (sb | sh | ss) & 3 and x.data_ptr() % (4 * x.element_size()) == 0:
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+class PackedKVCache(nn.Module):
+    """KV cache in 4 bits for inference (see the module's documentation).
+
+    ``max_seq_len`` tokens of room for each sequence are allocated per layer
+    at its first chunk, whose shape [B, H, S, D] and device the cache keeps
+    (head dim 64 or 128; float32, float16 or bfloat16 chunks)."""
+
+    def __init__(self, num_layers: int, max_seq_len: int):
+        super().__init__()
+        if num_layers < 0 or max_seq_len < 1:
+            raise ValueError("PackedKVCache: num_layers must not be negative and max_seq_len at least 1")
+        self.num_layers = num_layers
+        self.max_seq_len = max_seq_len
+        self._layers: list[Optional[_LayerStore]] = [None] * num_layers
+
+    # -- helpers ---------------------------------------------------------------
+    def _layer(self, layer_idx: int, what: str) -> _LayerStore:
+        st = self._layers[layer_idx]
+        if st is None:
+            raise RuntimeError(f"PackedKVCache.{what}: layer {layer_idx} is empty")
+        return st
+
+    @staticmethod
+    def _call(st: _LayerStore, name: str, *args) -> None:
+        """Call an entry point on the layer's device and its current stream."""
+        if st.device.index == torch.cuda.current_device():
+            _C.call(name, st.ref, *args, torch.cuda.current_stream(st.device).cuda_stream)
+        else:
+            with torch.cuda.device(st.device):
+                _C.call(name, st.ref, *args, torch.cuda.current_stream(st.device).cuda_stream)
+
+    @staticmethod
+    def _vector(x, n: int, dtype, st: _LayerStore, what: str) -> Optional[int]:
+        if x is None:
+            return None
+        if not isinstance(x, torch.Tensor) or x.dtype != dtype or x.shape != (n,) or x.device != st.device:
+            raise ValueError(f"PackedKVCache.{what} must be a {dtype} tensor of {n} values on {st.device}")
+        if not x.is_contiguous():
+            raise ValueError(f"PackedKVCache.{what} must be contiguous")
+        return x.data_ptr()
+
+    # -- writing -----------------------------------------------------------------
+    @torch.no_grad()
+    def append(self, layer_idx: int, key: torch.Tensor, value: torch.Tensor,
+               counts: Optional[torch.Tensor] = None) -> None:
+        """Quantize and store new K, V [B, H, S, D] behind what each sequence
+        holds.  ``counts`` (int32 [B], on the device) says how many of the S
+        tokens each sequence has, the rest being padding; default all.  Raises
+        ValueError when S tokens might not fit; what a replayed graph appends
+        past the room is dropped and counted (``dropped``)."""
+        _C.require_cuda(key, value, what="PackedKVCache.append")
+        _C.require_float(key, "PackedKVCache.append")
+        if key.ndim != 4 or key.shape != value.shape:
+            raise RuntimeError(f"PackedKVCache.append: key {list(key.shape)} and value {list(value.shape)} "
+                               "must both be [B, H, S, D]")
+        if key.dtype != value.dtype or key.device != value.device:
+            raise TypeError("PackedKVCache.append: key and value must share dtype and device")
+        B, H, S, D = key.shape
+        st = self._layers[layer_idx]
+        if st is None:
+            if D not in (64, 128):
+                raise ValueError(f"PackedKVCache: head dim {D}: 64 or 128 supported")
+            if B == 0 or H == 0:
+                raise ValueError("PackedKVCache: empty batch or no heads")
+            if B * H > 65535:
+                raise ValueError("PackedKVCache: more than 65535 (sequence, head) pairs")
+            st = _LayerStore(B, H, (self.max_seq_len + 31) // 32 * 32, D, key.device)
+            self._layers[layer_idx] = st
+        elif (B, H, D) != (st.B, st.H, st.D) or key.device != st.device:
+            raise RuntimeError(f"PackedKVCache.append: cache [{st.B}, {st.H}, *, {st.D}] on {st.device} vs new "
+                               f"{list(key.shape)} on {key.device}")
+        c = self._vector(counts, B, torch.int32, st, "append: counts")
+        if S == 0:
+            return
+        capturing = torch.cuda.is_current_stream_capturing()
+        if capturing:
+            st.captured = True
+        elif not st.captured and st.bound + S > self.max_seq_len:
+            raise ValueError(f"PackedKVCache.append: {S} more tokens than {st.bound} of {self.max_seq_len} "
+                             "do not fit (evict, or reset)")
+        k, v = _rows(key, "append"), _rows(value, "append")
+        ks, vs = k.stride(), v.stride()
+        self._call(st, "lq_kv4_append", k.data_ptr(), v.data_ptr(), _C.TORCH_TO_LQ[k.dtype], S, ks[0], ks[1], ks[2],
+                   vs[0], vs[1], vs[2], c)
+        st.bound = self.max_seq_len if st.captured else min(st.bound + S, self.max_seq_len)
+
+    def update(self, layer_idx: int, key: torch.Tensor, value: torch.Tensor,
+               counts: Optional[torch.Tensor] = None,
+               dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
+        """``append``, then all cached K and V as values (``get``)."""
+        self.append(layer_idx, key, value, counts)
+        return self.get(layer_idx, dtype)
+
+    # -- reading -----------------------------------------------------------------
+    @torch.no_grad()
+    def get(self, layer_idx: int, dtype: torch.dtype = torch.float32) -> Optional[Tuple[torch.Tensor, torch.Tensor]]:
+        """K, V [B, H, seq_len, D] as values in ``dtype``, zeros past a
+        sequence's length, or None if the layer is empty."""
+        st = self._layers[layer_idx]
+        if st is None:
+            return None
+        if dtype not in _C.FLOAT_TYPES:
+            raise TypeError(f"PackedKVCache.get: unsupported dtype {dtype} (float32, float16, bfloat16)")
+        k = torch.empty(st.B, st.H, st.bound, st.D, dtype=dtype, device=st.device)
+        v = torch.empty_like(k)
+        if st.bound:
+            self._call(st, "lq_kv4_dequant", st.bound, _C.TORCH_TO_LQ[dtype], k.data_ptr(), v.data_ptr())
+        return k, v
+
+    @torch.no_grad()
+    def attend(self, layer_idx: int, query: torch.Tensor, scale: Optional[float] = None, causal: bool = False, *,
+               counts: Optional[torch.Tensor] = None, softcap: float = 0.0,
+               slopes: Optional[torch.Tensor] = None, window: int = 0,
+               prefix: Optional[torch.Tensor] = None, accumulate: bool = False) -> torch.Tensor:
+        """softmax attention of query [B, Hq, Sq, D] over a layer's cached
+        tokens, computed from the 4-bit codes; [B, Hq, Sq, D] in query's dtype.
+
+        Hq is a multiple of the cached heads H (query head h reads kv head
+        h // (Hq // H)).  The queries belong to the last tokens of their
+        sequence: query i has position next - n + i, with n its sequence's
+        ``counts`` (int32 [B]; default Sq) and ``next`` the position of the
+        token that would be appended next.  Queries from n on are padding.
+        For a query at position p and a token at position t,
+
+            x = scale * q.k                      scale: default D ** -0.5
+            x = softcap * tanh(x / softcap)      if softcap > 0
+            x = x - slopes[h] * |p - t|          if slopes (float32 [Hq]) is given
+
+        and the query sees the token if ((not causal or t <= p) and (window == 0
+        or p - t < window)) or t < prefix[b] (int32 [B]).  A query that sees
+        nothing gives zeros, and so does padding.  ``accumulate`` adds the
+        weight that each token got from all queries to ``attention_mass``.
+
+        Inference only: no gradient is computed."""
+        st = self._layer(layer_idx, "attend")
+        _C.require_cuda(query, what="PackedKVCache.attend")
+        _C.require_float(query, "PackedKVCache.attend")
+        if query.ndim != 4 or query.shape[0] != st.B or query.shape[3] != st.D or query.shape[1] % st.H \
+                or query.shape[1] == 0 or query.device != st.device:
+            raise RuntimeError(f"PackedKVCache.attend: query {list(query.shape)} on {query.device} does not match "
+                               f"the cache [{st.B}, {st.H}*G, *, {st.D}] on {st.device}")
+        B, Hq, Sq, D = query.shape
+        if not 0.0 <= softcap < float("inf"):
+            raise ValueError(f"PackedKVCache.attend: softcap {softcap} must be finite and not negative")
+        if window < 0:
+            raise ValueError(f"PackedKVCache.attend: window {window} must not be negative")
+        cn = self._vector(counts, B, torch.int32, st, "attend: counts")
+        sl = self._vector(slopes, Hq, torch.float32, st, "attend: slopes")
+        pf = self._vector(prefix, B, torch.int32, st, "attend: prefix")
+        out = torch.empty((B, Hq, Sq, D), dtype=query.dtype, device=st.device)
+        if Sq == 0:
+            return out
+        q = _rows(query, "attend")
+        qs = q.stride()
+        dt = _C.TORCH_TO_LQ[q.dtype]
+        bound = st.cap if st.captured else st.bound
+        nbytes = _C.lib().lq_kv4_attention_workspace_bytes(st.ref, dt, Hq, Sq, bound, accumulate)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=st.device)
+        self._call(st, "lq_kv4_attention", q.data_ptr(), dt, Hq, Sq, qs[0], qs[1], qs[2], bound, cn,
+                   D ** -0.5 if scale is None else scale, causal, softcap, sl, window, pf, accumulate,
+                   out.data_ptr(), ws.data_ptr(), nbytes)
+        return out
+
+    # -- eviction ------------------------------------------------------------------
+    @torch.no_grad()
+    def evict(self, layer_idx: int, keep: int, recent: int = 0, sinks: int = 0) -> None:
+        """Cut every sequence back to ``keep`` tokens per kv head: the
+        ``recent`` last ones and those at positions below ``sinks`` stay, then
+        the ones with the greatest ``attention_mass`` (equal mass: from the
+        lowest slot up; NaN counts as greatest).  Heads keep tokens of their
+        own.  Sequences that hold no more than ``keep`` are left alone."""
+        st = self._layer(layer_idx, "evict")
+        if keep < 1 or recent < 0 or sinks < 0 or recent + sinks > keep:
+            raise ValueError(f"PackedKVCache.evict: keep {keep} must be positive and hold the {recent} recent and "
+                             f"{sinks} first tokens")
+        if keep >= st.cap or (not st.captured and keep >= st.bound):
+            return
+        nbytes = _C.lib().lq_kv4_evict_workspace_bytes(st.B, st.H, st.cap, keep)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=st.device)
+        self._call(st, "lq_kv4_evict", keep, recent, sinks, ws.data_ptr(), nbytes)
+        if torch.cuda.is_current_stream_capturing():
+            st.captured = True
+        if not st.captured:
+            st.bound = min(st.bound, keep)
+
+    # -- what the cache holds --------------------------------------------------------
+    def lengths(self, layer_idx: int) -> torch.Tensor:
+        """Tokens that each sequence holds: int32 [B] on the device (the cache's own)."""
+        st = self._layer(layer_idx, "lengths")
+        return st.state[:st.B]
+
+    def dropped(self, layer_idx: int) -> torch.Tensor:
+        """Tokens that replayed appends found no room for: int32 scalar on the device (the cache's own)."""
+        st = self._layer(layer_idx, "dropped")
+        return st.state[2 * st.B + 1]
+
+    def positions(self, layer_idx: int) -> torch.Tensor:
+        """Position of the token in each slot, -1 where it is empty: int32
+        [B, H, seq_len] (the cache's own).  Until something is evicted slot t
+        holds position t; then the order of slots means nothing."""
+        st = self._layer(layer_idx, "positions")
+        return st.positions[:, :, :st.bound]
+
+    def attention_mass(self, layer_idx: int) -> torch.Tensor:
+        """Attention weight that each slot's token collected (``attend`` with
+        ``accumulate``), 0 where it is empty: float32 [B, H, seq_len], the
+        cache's own, so it can be decayed or replaced in place."""
+        st = self._layer(layer_idx, "attention_mass")
+        return st.mass[:, :, :st.bound]
+
+    def reset(self, layer_idx: Optional[int] = None) -> None:
+        """Clear one layer, or all; the buffers stay."""
+        for st in self._layers if layer_idx is None else [self._layers[layer_idx]]:
+            if st is not None:
+                st.clear()
+
+    @property
+    def seq_len(self) -> int:
+        """Tokens cached in layer 0: the most that any sequence may hold."""
+        return 0 if not self.num_layers or self._layers[0] is None else self._layers[0].bound

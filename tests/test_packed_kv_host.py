@@ -1,0 +1,91 @@
+"""CPU-side checks of the 4-bit KV cache: what PackedKVCache and the lq_kv4_*
+entry points refuse before any launch (no GPU needed)."""
+
+import ctypes
+
+import pytest
+import torch
+
+import llm_quant_b200 as L
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from llm_quant_b200 import _C, build
+    build.build()
+    return _C.lib()
+
+
+def _cache(**kw):
+    """A cache struct whose pointers are aligned but lead nowhere: no call that is refused may follow them."""
+    from llm_quant_b200 import _C
+    f = dict(k_codes=4096, v_codes=4096, params=4096, positions=4096, mass=4096, state=4096, B=2, H=2, cap=64, D=64)
+    f.update(kw)
+    return _C.KV4Cache(*[f[n] for n, _ in _C.KV4Cache._fields_])
+
+
+BAD = [({"D": 96}, "head dim"), ({"cap": 40}, "multiple"), ({"B": 0}, "shape"), ({"H": -1}, "shape"),
+       ({"cap": 1 << 31}, "too large"), ({"B": 1000, "H": 1000}, "too large"), ({"params": None}, "NULL"),
+       ({"state": None}, "NULL"), ({"k_codes": 4097}, "aligned"), ({"params": 4104}, "aligned")]
+
+
+@pytest.mark.parametrize("kw,word", BAD)
+def test_bad_caches(lib, kw, word):
+    c = ctypes.byref(_cache(**kw))
+    calls = [lambda: lib.lq_kv4_append(c, 4096, 4096, 1, 1, 64, 64, 64, 64, 64, 64, None, None),
+             lambda: lib.lq_kv4_dequant(c, 1, 1, 4096, 4096, None),
+             lambda: lib.lq_kv4_evict(c, 4, 0, 0, 4096, 1 << 40, None),
+             lambda: lib.lq_kv4_attention(c, 4096, 1, 4, 1, 64, 64, 64, 64, None, 1.0, 0, 0.0, None, 0, None, 0,
+                                          4096, 4096, 1 << 40, None)]
+    for call in calls:
+        assert call() < 0
+        assert word.encode() in lib.lq_last_error()
+    assert lib.lq_kv4_attention_workspace_bytes(c, 1, 4, 1, 64, 0) == 0
+
+
+def test_bad_arguments(lib):
+    c = ctypes.byref(_cache())
+
+    def append(k=4096, v=4096, dt=1, S=1, st=(64,) * 6):
+        return lib.lq_kv4_append(c, k, v, dt, S, *st, None, None)
+
+    assert append(k=None) == -1 and append(dt=3) == -2 and append(S=-1) == -1
+    assert append(k=4100) == -5 and append(st=(64, 64, 63, 64, 64, 64)) == -5
+    assert append(S=0) == 0  # nothing to do
+    assert lib.lq_kv4_dequant(c, 65, 1, 4096, 4096, None) == -1
+    assert lib.lq_kv4_dequant(c, 4, 3, 4096, 4096, None) == -2
+    assert lib.lq_kv4_dequant(c, 4, 1, 4098, 4096, None) == -5
+    assert lib.lq_kv4_dequant(c, 0, 1, None, None, None) == 0
+    for keep, recent, sinks in ((0, 0, 0), (4, 5, 0), (4, 2, 3), (4, -1, 0)):
+        assert lib.lq_kv4_evict(c, keep, recent, sinks, 4096, 1 << 40, None) == -1
+    assert lib.lq_kv4_evict(c, 64, 0, 0, None, 0, None) == 0  # nothing can be over it
+    assert lib.lq_kv4_evict(c, 8, 0, 0, 4096, lib.lq_kv4_evict_workspace_bytes(2, 2, 64, 8) - 1, None) == -1
+
+    def attend(q=4096, dt=1, Hq=4, Sq=1, cap=0.0, window=0, out=4096, ws=4096, nbytes=1 << 40):
+        return lib.lq_kv4_attention(c, q, dt, Hq, Sq, 64, 64, 64, 64, None, 1.0, 0, cap, None, window, None, 0,
+                                    out, ws, nbytes, None)
+
+    assert attend(Hq=3) == -1 and attend(Hq=0) == -1 and attend(dt=3) == -2 and attend(cap=-1.0) == -1
+    assert attend(q=None) == -1 and attend(out=None) == -1 and attend(window=-1) == -1 and attend(Sq=-1) == -1
+    assert attend(ws=None) == -1 and attend(ws=4100) == -5
+    need = lib.lq_kv4_attention_workspace_bytes(c, 1, 4, 1, 64, 0)
+    assert need > 0 and attend(nbytes=need - 1) == -1
+    assert attend(Sq=0) == 0
+
+
+def test_python_layer_without_a_gpu():
+    with pytest.raises(ValueError):
+        L.PackedKVCache(1, 0)
+    with pytest.raises(ValueError):
+        L.PackedKVCache(-1, 5)
+    cache = L.PackedKVCache(2, 16)
+    x = torch.zeros(1, 1, 2, 64)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        cache.append(0, x, x)
+    with pytest.raises(RuntimeError, match="empty"):
+        cache.attend(1, x)
+    with pytest.raises(IndexError):
+        cache.get(2)
+    assert cache.get(0) is None and cache.seq_len == 0
+    cache.reset()
+    cache.reset(1)
