@@ -393,9 +393,11 @@ int lq_sparse_row_add(const void* x, int dtype, int64_t M, int64_t K, int64_t N,
  *       half, zero point as bf16 in the high half;
  *   positions [B, H, cap] (-1: empty slot), mass [B, H, cap] attention weight
  *       that a token has collected (0: empty slot);
- *   state [2 B + 3]: tokens held and position of the next token of each
- *       sequence, a ticket of the calls, tokens that found no room, and whether
- *       anything was evicted (until then a token's slot is its position).
+ *   state [2 B + 4]: tokens held and position of the next token of each
+ *       sequence, a ticket of the calls, tokens that found no room, whether
+ *       anything was evicted (until then a token's slot is its position), and
+ *       an lq_status: LQ_ETIMEOUT if a wait on the device ran out, whose call's
+ *       results are then incomplete.
  * A new cache has positions -1 and all of mass and state 0.  The lengths are
  * the device's: no call reads them on the host, so a captured call sees the
  * lengths of its replay.  Calls on one cache must not run at the same time,

@@ -40,7 +40,7 @@ struct Kv4 {
   float* mass;
   int32_t* len;   // [B] tokens held
   int32_t* next;  // [B] position of the next token
-  int32_t* sync;  // [0] ticket of the running call, [1] tokens dropped for want of room, [2] something was evicted
+  int32_t* sync;  // [0] ticket of the running call, [1] tokens dropped for want of room, [2] something was evicted, [3] a wait on the device ran out
   int B, H, cap, D;
 };
 

@@ -20,9 +20,8 @@
 // taken as f16 hi + lo (two MMAs, 22 bits), and P likewise; with 16-bit queries
 // P is rounded once to f16 (2^-11 of each probability, below the output's own
 // rounding), and the zero-point sum uses the rounded value.
-// P carries sv: p sv = exp2(x + log2 sv - m) with m the running maximum of
-// x + log2 sv, so that it is at most 1 whatever the scales (and times 2^15, so
-// that what is small beside it stays a normal f16); the denominator sums
+// P carries sv: p sv = exp2(x + log2 sv - m) with m a running reference of
+// x + log2 sv, so that it fits f16 whatever the scales; the denominator sums
 // exp2(x - m).
 //
 // Split: the 32-token units of all (sequence, kv head) pairs lie in one row,
@@ -34,6 +33,7 @@
 #include <algorithm>
 
 #include "lq_kv4.cuh"
+#include "lq_tma.cuh"
 
 namespace lq {
 namespace {
@@ -92,15 +92,26 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
-__device__ __forceinline__ float ld_q(const uint8_t* p, int64_t i, int dt) {
-  if (dt == LQ_F32) return reinterpret_cast<const float*>(p)[i];
-  if (dt == LQ_F16) return __half2float(reinterpret_cast<const __half*>(p)[i]);
-  return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
-}
 __device__ __forceinline__ void st_out(uint8_t* p, int64_t i, int dt, float v) {
   if (dt == LQ_F32) reinterpret_cast<float*>(p)[i] = v;
   else if (dt == LQ_F16) reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
   else reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+
+__device__ __forceinline__ void st_out4(uint8_t* p, int64_t i, int dt, float4 v, float f) {
+  if (dt == LQ_F32) {
+    *reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + i) = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+  } else if (dt == LQ_F16) {
+    *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(p) + i) = make_uint2(h2(v.x * f, v.y * f), h2(v.z * f, v.w * f));
+  } else {
+    union {
+      __nv_bfloat162 b[2];
+      uint2 u;
+    } r;
+    r.b[0] = __floats2bfloat162_rn(v.x * f, v.y * f);
+    r.b[1] = __floats2bfloat162_rn(v.z * f, v.w * f);
+    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p) + i) = r.u;
+  }
 }
 
 // Fragment registers from a word of codes: nibble n of both halves as f16.
@@ -147,15 +158,15 @@ __device__ __forceinline__ void ld_codes(const uint8_t* p, uint32_t* w) {
 struct Seq {
   int n, cnt, first;  // tokens held, new queries, position of the first of them
   int pre, gap, count;
-  bool ordered;  // nothing was evicted: slots are positions
+  int ordered;        // nothing was evicted: slots are positions
 };
 __device__ __forceinline__ Seq seq_of(const Attn& a, int b) {
   Seq s;
   s.n = min(a.kv.len[b], a.kv.cap);
   s.cnt = a.counts ? min(max(a.counts[b], 0), a.Sq) : a.Sq;
   s.first = a.kv.next[b] - s.cnt;
-  s.pre = s.gap = 0;
   s.ordered = a.kv.sync[2] == 0;
+  s.pre = s.gap = 0;
   s.count = s.cnt > 0 ? (s.n + kUnit - 1) / kUnit : 0;
   if (a.window > 0 && s.ordered && s.count > 0) {
     const int lo = min(max(s.first - a.window + 1, 0) / kUnit, s.count - 1);
@@ -167,310 +178,454 @@ __device__ __forceinline__ Seq seq_of(const Attn& a, int b) {
   return s;
 }
 
-// Units of all heads; every warp computes it for itself.
-__device__ __forceinline__ int64_t all_units(const Attn& a) {
-  int64_t u = 0;
-  for (int b = threadIdx.x & 31; b < a.kv.B; b += 32) u += seq_of(a, b).count;
+// The row of all heads' units, cut into equal stretches.  (A unit takes 32 D
+// bytes, so that their number fits an int on any GPU.)
+struct Cut {
+  int units, blocks, base, rem;
+  __device__ __forceinline__ void set(int u, int most) {
+    units = u;
+    blocks = max(min(u, most), 1);
+    base = units / blocks;
+    rem = units % blocks;
+  }
+  // units * cta / blocks, and the block that unit x falls to
+  __device__ __forceinline__ int begin(int cta) const { return cta * base + cta * rem / blocks; }
+  __device__ __forceinline__ int owner(int x) const { return (int)(((int64_t)(x + 1) * blocks - 1) / units); }
+};
+__device__ __forceinline__ int warp_sum(int u) {
 #pragma unroll
   for (int m = 16; m > 0; m >>= 1) u += __shfl_xor_sync(0xffffffffu, u, m);
-  return u * a.kv.H;
+  return u;
 }
-
-// Sequence that holds unit x of the row of units, and where it begins.
-__device__ __forceinline__ int seq_at(const Attn& a, int64_t x, int64_t& begin) {
+__device__ __forceinline__ int warp_scan(int u) {
   const int lane = threadIdx.x & 31;
-  int64_t base = 0;
-  for (int b0 = 0; b0 < a.kv.B; b0 += 32) {
-    const int b = b0 + lane;
-    int64_t inc = b < a.kv.B ? (int64_t)seq_of(a, b).count * a.kv.H : 0;
-    const int64_t own = inc;
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, inc, d);
-      if (lane >= d) inc += y;
-    }
-    const uint32_t hit = __ballot_sync(0xffffffffu, base + inc > x);
+  for (int d = 1; d < 32; d <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, u, d);
+    if (lane >= d) u += y;
+  }
+  return u;
+}
+// Units of the sequences before b, and of all; every warp computes it for itself.
+__device__ __forceinline__ int units_before(const Attn& a, int b, int& all) {
+  int before = 0, sum = 0;
+  for (int j = threadIdx.x & 31; j < a.kv.B; j += 32) {
+    const int u = seq_of(a, j).count;
+    sum += u;
+    if (j < b) before += u;
+  }
+  all = warp_sum(sum) * a.kv.H;
+  return warp_sum(before) * a.kv.H;
+}
+// Sequence that holds unit x, and the unit it begins at.
+__device__ __forceinline__ int seq_at(const Attn& a, int x, int& begin) {
+  const int lane = threadIdx.x & 31;
+  begin = 0;
+  for (int b0 = 0; b0 < a.kv.B; b0 += 32) {
+    const int own = b0 + lane < a.kv.B ? seq_of(a, b0 + lane).count * a.kv.H : 0;
+    const int inc = warp_scan(own);
+    const uint32_t hit = __ballot_sync(0xffffffffu, begin + inc > x);
     if (hit) {
       const int src = __ffs(hit) - 1;
-      begin = base + __shfl_sync(0xffffffffu, inc - own, src);
+      begin += __shfl_sync(0xffffffffu, inc - own, src);
       return b0 + src;
     }
-    base += __shfl_sync(0xffffffffu, inc, 31);
+    begin += __shfl_sync(0xffffffffu, inc, 31);
   }
-  begin = base;
   return a.kv.B;
 }
 
 // Queries of a block's rows as B fragments, and what each score column needs.
+// They are made once per head by the whole block, in shared memory.
+template <int D, int NQ, bool QLO>
+struct RowsShared {
+  static constexpr int NW = D / 8;  // words of a row
+  uint4 hi[8 * NQ][NW];             // nibble pairs (0, 4), (2, 6), (1, 5), (3, 7) of each word
+  uint4 lo[QLO ? 8 * NQ : 1][QLO ? NW : 1];
+  float sum[8 * NQ], fac[8 * NQ];
+};
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float* x) {  // p on a multiple of 4 elements
+  if constexpr (sizeof(T) == 4) {
+    const float4 u = __ldg(reinterpret_cast<const float4*>(p)), v = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
+  } else {
+    union {
+      uint2 u[2];
+      T t[8];
+    } v;
+    v.u[0] = __ldg(reinterpret_cast<const uint2*>(p));
+    v.u[1] = __ldg(reinterpret_cast<const uint2*>(p) + 1);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = Ty<T>::to_f(v.t[i]);
+  }
+}
+
 template <int D, int NQ, bool QLO>
 struct Rows {
-  static constexpr int W = D / 32;
-  uint32_t hi[NQ][W][4], lo[QLO ? NQ : 1][QLO ? W : 1][4];
-  float sum[NQ][2], fac[NQ][2];  // of columns 2c, 2c + 1: sum of q, factor that undoes the scaling
+  static constexpr int W = D / 32, NW = D / 8;
+  static constexpr float kUnitK = pow2(Nibbles<QLO ? kSix : kFour>::unit(0));
+  const RowsShared<D, NQ, QLO>* sh;
+  float sum[NQ][2], fac[NQ][2];  // of columns 2c, 2c + 1: -sum of q, factor that undoes the scaling
   float slope[NQ][2];
   int at[NQ][2];                 // position of the query; INT_MIN: no such row
 
-  __device__ __forceinline__ void load(const Attn& a, const Seq& s, int b, int h, int zb, bool gen) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-#pragma unroll
-    for (int nq = 0; nq < NQ; ++nq) {
-      const int r = zb * 8 * NQ + 8 * nq + g, i = r / a.G;
-      float x[8 * W];
-#pragma unroll
-      for (int d = 0; d < 8 * W; ++d) x[d] = 0.0f;
+  // NW neighbouring lanes make a row, 8 values each
+  __device__ __forceinline__ static void make(RowsShared<D, NQ, QLO>& sh, const Attn& a, const Seq& s, int b, int h,
+                                              int zb, int tid, int threads, bool gen) {
+    for (int j = tid; j < 8 * NQ * NW; j += threads) {
+      const int lr = j / NW, w = j % NW, r = zb * 8 * NQ + lr, i = r / a.G;
+      float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
       if (r < a.rows && i < s.cnt) {
-        const int64_t off = b * a.q_sb + (int64_t)(h * a.G + r % a.G) * a.q_sh + i * a.q_ss + c * (8 * W);
-#pragma unroll
-        for (int d = 0; d < 8 * W; ++d) x[d] = ld_q(a.q, off + d, a.q_dtype);
+        const int64_t off = b * a.q_sb + (int64_t)(h * a.G + r % a.G) * a.q_sh + i * a.q_ss + 8 * w;
+        if constexpr (QLO) load8(reinterpret_cast<const float*>(a.q) + off, x);
+        else if (a.q_dtype == LQ_F16) load8(reinterpret_cast<const __half*>(a.q) + off, x);
+        else load8(reinterpret_cast<const __nv_bfloat16*>(a.q) + off, x);
       }
-      float mx = 0.0f;
+      float mx = 0.0f, sum = 0.0f;
 #pragma unroll
-      for (int d = 0; d < 8 * W; ++d) mx = fmaxf(mx, fabsf(x[d]));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      for (int d = 0; d < 8; ++d) mx = fmaxf(mx, fabsf(x[d])), sum += x[d];
+#pragma unroll
+      for (int m = NW / 2; m > 0; m >>= 1) {
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, m));
+        sum += __shfl_xor_sync(0xffffffffu, sum, m);
+      }
       // 2^(14 - exponent of mx), kept a normal number
       const int e = (int)(__float_as_uint(mx) >> 23);
-      const int up = mx > 0.0f && e < 255 ? min(268 - e, 254) : 127;
-      const float f = __uint_as_float((uint32_t)max(up, 1) << 23);
-      float sum = 0.0f;
+      const int up = mx > 0.0f && e < 255 ? max(min(268 - e, 254), 1) : 127;
+      const float f = __uint_as_float((uint32_t)up << 23);
+      uint32_t p[4], q[4];
 #pragma unroll
-      for (int w = 0; w < W; ++w)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {  // register j: nibbles (n, n + 4), n = 0, 2, 1, 3
-          const int n = 8 * w + (j < 2 ? 2 * j : 2 * j - 3);
-          const float u = x[n] * f, v = x[n + 4] * f;
-          const uint32_t p = h2(u, v);
-          const float2 y = f2(p);
-          hi[nq][w][j] = p;
-          sum += y.x + y.y;
-          if constexpr (QLO) {
-            lo[nq][w][j] = h2(u - y.x, v - y.y);
-            const float2 y2 = f2(lo[nq][w][j]);
-            sum += y2.x + y2.y;
-          }
+      for (int k = 0; k < 4; ++k) {  // register k: nibbles (n, n + 4), n = 0, 2, 1, 3
+        const int n = k < 2 ? 2 * k : 2 * k - 3;
+        const float u = x[n] * f, v = x[n + 4] * f;
+        p[k] = h2(u, v);
+        if constexpr (QLO) {
+          const float2 y = f2(p[k]);
+          q[k] = h2(u - y.x, v - y.y);
         }
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      // the accumulators hold `unit` times the true sums
-      constexpr float unit = pow2(Nibbles<QLO ? kSix : kFour>::unit(0));
-      const float back = a.sm / f * (1.0f / unit);
+      }
+      sh.hi[lr][w] = make_uint4(p[0], p[1], p[2], p[3]);
+      if constexpr (QLO) sh.lo[lr][w] = make_uint4(q[0], q[1], q[2], q[3]);
+      if (w == 0) {
+        // the accumulators hold kUnitK * f times the true sums
+        sh.sum[lr] = -sum * f * kUnitK;
+        sh.fac[lr] = a.sm / f * (1.0f / kUnitK) * (gen && a.cap > 0.0f ? 1.0f / a.cap : kLog2e);
+      }
+    }
+  }
+  // fragment registers of word w: read where they are used, they are not worth 16 registers
+  __device__ __forceinline__ uint4 hi(int nq, int w) const {
+    const int lane = threadIdx.x & 31;
+    return sh->hi[8 * nq + (lane >> 2)][(lane & 3) * W + w];
+  }
+  __device__ __forceinline__ uint4 lo(int nq, int w) const {
+    const int lane = threadIdx.x & 31;
+    return sh->lo[8 * nq + (lane >> 2)][(lane & 3) * W + w];
+  }
+  __device__ __forceinline__ void load(const RowsShared<D, NQ, QLO>& sh, const Attn& a, const Seq& s, int h, int zb,
+                                       bool gen) {
+    const int c = threadIdx.x & 3;
+    this->sh = &sh;
 #pragma unroll
-      for (int e2 = 0; e2 < 2; ++e2) {
-        const int src = (2 * c + e2) * 4;
-        this->sum[nq][e2] = __shfl_sync(0xffffffffu, sum, src) * unit;
-        fac[nq][e2] = __shfl_sync(0xffffffffu, back, src) * (gen && a.cap > 0.0f ? 1.0f / a.cap : kLog2e);
-        const int rc = zb * 8 * NQ + 8 * nq + 2 * c + e2, ic = rc / a.G;
-        at[nq][e2] = rc < a.rows && ic < s.cnt ? s.first + ic : INT_MIN;
-        slope[nq][e2] = gen && a.slopes && rc < a.rows ? a.slopes[h * a.G + rc % a.G] * kLog2e : 0.0f;
+    for (int nq = 0; nq < NQ; ++nq) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        sum[nq][e] = sh.sum[8 * nq + 2 * c + e];
+        fac[nq][e] = sh.fac[8 * nq + 2 * c + e];
+        if (gen) {
+          const int r = zb * 8 * NQ + 8 * nq + 2 * c + e, i = r / a.G;
+          at[nq][e] = r < a.rows && i < s.cnt ? s.first + i : INT_MIN;
+          slope[nq][e] = a.slopes && r < a.rows ? a.slopes[h * a.G + r % a.G] * kLog2e : 0.0f;
+        }
       }
     }
   }
 };
 
-// Scores (in log2 units) of one 16-token tile: x[nq][0..3] = (token g, column
-// 2c), (g, 2c + 1), (g + 8, 2c), (g + 8, 2c + 1); -inf where the query does not see the token.
-template <int D, int NQ, bool QLO, bool GEN>
-__device__ __forceinline__ void tile_scores(const Attn& a, const Rows<D, NQ, QLO>& q, const uint32_t* k0,
-                                            const uint32_t* k1, const uint32_t* par, const int* tok, const int* pos,
-                                            int n, int pre, float (*x)[4]) {
-  constexpr int W = D / 32;
-  float s0[NQ][4], s1[NQ][4];
+// Products of N tiles of 16 tokens from the codes of rows k[2 N]: x[i][nq][0..3] =
+// (token g, column 2c), (g, 2c + 1), (g + 8, 2c), (g + 8, 2c + 1) of tile i, the
+// zero points' share taken off beforehand.
+template <int N, int D, int NQ, bool QLO>
+__device__ __forceinline__ void products(const Rows<D, NQ, QLO>& q, const uint32_t (*k)[D / 32], const uint32_t* par,
+                                         float (*x)[NQ][4]) {
 #pragma unroll
-  for (int nq = 0; nq < NQ; ++nq)
-#pragma unroll
-    for (int u = 0; u < 4; ++u) s0[nq][u] = s1[nq][u] = 0.0f;
-#pragma unroll
-  for (int w = 0; w < W; ++w) {
-    uint32_t ka[4], kb[4];
-    Nibbles<QLO ? kSix : kFour>::take(k0[w], ka);
-    Nibbles<QLO ? kSix : kFour>::take(k1[w], kb);
-#pragma unroll
-    for (int nq = 0; nq < NQ; ++nq) {
-      mma16(s0[nq], ka[0], kb[0], ka[2], kb[2], q.hi[nq][w][0], q.hi[nq][w][1]);
-      mma16(s1[nq], ka[1], kb[1], ka[3], kb[3], q.hi[nq][w][2], q.hi[nq][w][3]);
-      if constexpr (QLO) {
-        mma16(s0[nq], ka[0], kb[0], ka[2], kb[2], q.lo[nq][w][0], q.lo[nq][w][1]);
-        mma16(s1[nq], ka[1], kb[1], ka[3], kb[3], q.lo[nq][w][2], q.lo[nq][w][3]);
-      }
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const float sk = par_scale(par[j]), zk = par_zero(par[j]);
-    const bool in = tok[j] < n;
+  for (int i = 0; i < N; ++i)
 #pragma unroll
     for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int u = 2 * j + e;
-        float v = s0[nq][u] + s1[nq][u];
-        v = fmaf(-zk, q.sum[nq][e], v) * (sk * q.fac[nq][e]);
-        bool sees = in;
-        if constexpr (GEN) {
-          if (a.cap > 0.0f) v = tanh_exp(v) * (a.cap * kLog2e);
-          const int back = q.at[nq][e] - pos[j];
-          if (a.slopes) v = fmaf(-q.slope[nq][e], fabsf((float)back), v);
-          bool near = true;
-          if (a.causal) near = back >= 0;
-          if (a.window > 0) near = near && back < a.window;
-          sees = in && (near || pos[j] < pre) && q.at[nq][e] != INT_MIN;
+      for (int u = 0; u < 4; ++u) x[i][nq][u] = par_zero(par[2 * i + (u >> 1)]) * q.sum[nq][u & 1];
+#pragma unroll
+  for (int w = 0; w < D / 32; ++w) {
+    uint4 hi[NQ], lo[NQ];
+#pragma unroll
+    for (int nq = 0; nq < NQ; ++nq) {
+      hi[nq] = q.hi(nq, w);
+      if constexpr (QLO) lo[nq] = q.lo(nq, w);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      uint32_t ka[4], kb[4];
+      Nibbles<QLO ? kSix : kFour>::take(k[2 * i][w], ka);
+      Nibbles<QLO ? kSix : kFour>::take(k[2 * i + 1][w], kb);
+#pragma unroll
+      for (int nq = 0; nq < NQ; ++nq) {
+        mma16(x[i][nq], ka[0], kb[0], ka[2], kb[2], hi[nq].x, hi[nq].y);
+        mma16(x[i][nq], ka[1], kb[1], ka[3], kb[3], hi[nq].z, hi[nq].w);
+        if constexpr (QLO) {
+          mma16(x[i][nq], ka[0], kb[0], ka[2], kb[2], lo[nq].x, lo[nq].y);
+          mma16(x[i][nq], ka[1], kb[1], ka[3], kb[3], lo[nq].z, lo[nq].w);
         }
-        x[nq][u] = sees ? v : -INFINITY;
       }
+    }
   }
 }
 
+// Score (log2 units) from a product, with cap, bias and masks: -inf where the
+// query does not see the token.
+template <int D, int NQ, bool QLO>
+__device__ __forceinline__ float full_score(const Attn& a, const Rows<D, NQ, QLO>& q, int nq, int e, float v, bool in,
+                                            int pos, int pre) {
+  if (a.cap > 0.0f) v = tanh_exp(v) * (a.cap * kLog2e);
+  const int back = q.at[nq][e] - pos;
+  if (a.slopes) v = fmaf(-q.slope[nq][e], fabsf((float)back), v);
+  bool near = true;
+  if (a.causal) near = back >= 0;
+  if (a.window > 0) near = near && back < a.window;
+  return in && (near || pos < pre) && q.at[nq][e] != INT_MIN ? v : -INFINITY;
+}
+
 // Positions of a lane's tokens (general masks only).
-__device__ __forceinline__ void load_pos(const Attn& a, int64_t row, const int* tok, const Seq& s, int* pos, int count) {
+template <int N>
+__device__ __forceinline__ void load_pos(const Attn& a, int64_t row, const int* tok, const Seq& s, int* pos) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (j < count) pos[j] = s.ordered || tok[j] >= s.n ? tok[j] : a.kv.pos[row + tok[j]];
+  for (int j = 0; j < N; ++j) pos[j] = s.ordered || tok[j] >= s.n ? tok[j] : a.kv.pos[row + tok[j]];
+}
+
+// P is kept up to 2^kHead above 1 and scaled by 2^kHead: the running reference
+// of a row is raised only when a probability would pass 2^(2 kHead - 0.1), so
+// most units need no maximum across lanes and no rescaling.
+constexpr float kHead = 8.0f, kTop = 15.9f;
+constexpr float kNone = -1e30f;  // reference of a row that has seen nothing
+
+// Shared memory of a block: each warp has a ring of its own of kStages units,
+// filled by bulk copies that one lane issues, so that a unit's bytes are on
+// their way while the warp works on the one before and need no registers.
+constexpr int kStages = 2;
+template <int D>
+struct Stage {
+  uint32_t k[4][32][D / 32], v[4][32][D / 32];
+  uint2 par[kUnit];
+  static constexpr uint32_t bytes = kUnit * D + kUnit * 8;
+};
+template <int D, int NQ, bool QLO>
+struct alignas(128) AttnShared {
+  Stage<D> ring[kWarps][kStages];
+  float o[kWarps][8][D + 4];
+  RowsShared<D, NQ, QLO> q;
+  float2 ml[kWarps][8 * NQ];
+  uint64_t full[kWarps][kStages];
+};
+template <int W>
+__device__ __forceinline__ void lds_codes(const uint32_t* p, uint32_t* w) {
+  if constexpr (W == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x, w[1] = v.y;
+  }
 }
 
 template <int D, int NQ, bool QLO, bool GEN>
-__global__ void __launch_bounds__(32 * kWarps, NQ == 1 && !QLO && !GEN ? 4 : 2) kv4_attn_kernel(const Attn a) {
-  constexpr int W = D / 32, NR = 8 * NQ;
+__global__ void __launch_bounds__(32 * kWarps, NQ == 1 && !QLO ? 4 : NQ == 1 ? 2 : 1) kv4_attn_kernel(const Attn a) {
+  constexpr int W = D / 32;
   using VN = Nibbles<QLO ? kSix : kMixed>;
-  __shared__ float ob[kWarps][NR][D + 1];
-  __shared__ float2 mlb[kWarps][NR];
+  extern __shared__ __align__(128) uint8_t smem[];
+  AttnShared<D, NQ, QLO>& sh = *reinterpret_cast<AttnShared<D, NQ, QLO>*>(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int zb = blockIdx.y, cta = blockIdx.x;
-  const int64_t units = all_units(a);
-  const int64_t blocks = units < a.blocks ? units : a.blocks;
-  if (cta >= blocks) return;
-  int64_t x0 = cta * units / blocks;
-  const int64_t x1 = (cta + 1) * units / blocks;
-  int64_t seq_begin;
+  int all;
+  units_before(a, 0, all);
+  Cut cut;
+  cut.set(all, a.blocks);
+  if (all == 0 || cta >= cut.blocks) return;
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) mbar_init(&sh.full[warp][i], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  __syncwarp();
+  int fill = 0, take = 0;  // units that this warp has asked for, and used
+  int x0 = cut.begin(cta), seq_begin;
+  const int x1 = cut.begin(cta + 1);
   int b = seq_at(a, x0, seq_begin);
   Seq s = seq_of(a, b);
-
-  while (x0 < x1) {
-    while (x0 >= seq_begin + (int64_t)s.count * a.kv.H) {  // next sequence that has units
-      seq_begin += (int64_t)s.count * a.kv.H;
-      s = seq_of(a, ++b);
+  int h = (x0 - seq_begin) / max(s.count, 1), u0 = x0 - seq_begin - h * s.count;
+  int u1 = min(s.count, u0 + (x1 - x0));
+  auto token = [&](int u) { return GEN ? (u < s.pre ? u : u + s.gap) * kUnit : u * kUnit; };
+  auto ask = [&](int u) {  // every lane has read what the stage held
+    if (u < u1) {
+      if (lane == 0) {
+        Stage<D>& st = sh.ring[warp][fill % kStages];
+        uint64_t* bar = &sh.full[warp][fill % kStages];
+        const int64_t t = (int64_t)(b * a.kv.H + h) * a.kv.cap + token(u);
+        mbar_expect_tx(bar, Stage<D>::bytes);
+        bulk_load(st.k, a.kv.k + t * (D / 2), kUnit * (D / 2), bar);
+        bulk_load(st.v, a.kv.v + t * (D / 2), kUnit * (D / 2), bar);
+        bulk_load(st.par, a.kv.par + t, kUnit * 8, bar);
+      }
+      ++fill;
     }
-    const int h = (int)((x0 - seq_begin) / s.count);
-    const int u0 = (int)((x0 - seq_begin) % s.count);
-    const int u1 = (int)min((int64_t)s.count, u0 + (x1 - x0));
+  };
+#pragma unroll
+  for (int i = 0; i < kStages; ++i) ask(u0 + warp + i * kWarps);
+
+  while (true) {
     const int bh = b * a.kv.H + h;
     const int64_t row = (int64_t)bh * a.kv.cap;
-    const uint8_t* kc = a.kv.k + row * (D / 2);
-    const uint8_t* vc = a.kv.v + row * (D / 2);
     const int pre = GEN && a.prefix ? a.prefix[b] : 0;
+    int u = u0 + warp;
+    __syncthreads();  // the last head's queries have been read
+    Rows<D, NQ, QLO>::make(sh.q, a, s, b, h, zb, threadIdx.x, 32 * kWarps, GEN);
+    __syncthreads();
     Rows<D, NQ, QLO> q;
-    q.load(a, s, b, h, zb, GEN);
+    q.load(sh.q, a, s, h, zb, GEN);
 
     float m[NQ][2], l[NQ][2], z[NQ][2], O[NQ][2 * W][4];
 #pragma unroll
     for (int nq = 0; nq < NQ; ++nq) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) m[nq][e] = -INFINITY, l[nq][e] = z[nq][e] = 0.0f;
+      for (int e = 0; e < 2; ++e) m[nq][e] = kNone, l[nq][e] = z[nq][e] = 0.0f;
 #pragma unroll
       for (int e = 0; e < 2 * W; ++e)
 #pragma unroll
-        for (int u = 0; u < 4; ++u) O[nq][e][u] = 0.0f;
-    }
-    uint32_t kw[4][W], vw[4][W];
-    uint2 pw[4];
-    auto token = [&](int u) { return (u < s.pre ? u : u + s.gap) * kUnit; };
-    auto load_k = [&](int t0) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        ld_codes<W>(kc + (int64_t)(t0 + 8 * j) * (D / 2) + lane * (4 * W), kw[j]);
-        pw[j] = __ldg(a.kv.par + row + t0 + 8 * j + g);
-      }
-    };
-    auto load_v = [&](int t0) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) ld_codes<W>(vc + (int64_t)(t0 + 8 * j) * (D / 2) + lane * (4 * W), vw[j]);
-    };
-    int u = u0 + warp;
-    if (u < u1) {
-      load_k(token(u));
-      load_v(token(u));
+        for (int i = 0; i < 4; ++i) O[nq][e][i] = 0.0f;
     }
     for (; u < u1; u += kWarps) {
-      const int t0 = token(u), t_next = token(u + kWarps);
-      const bool more = u + kWarps < u1;
-      int tok[4], pos[4];
+      const int t0 = token(u);
+      const Stage<D>& st = sh.ring[warp][take % kStages];
+      if (!mbar_wait_warp(&sh.full[warp][take % kStages], (take / kStages) & 1)) {
+        // the copy never came (2 s): give up, so that the host learns of it
+        if (lane == 0) a.kv.sync[3] = LQ_ETIMEOUT;
+        take = fill;
+        break;
+      }
+      ++take;
       uint32_t kp[4], vp[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) tok[j] = t0 + 8 * j + g, kp[j] = pw[j].x, vp[j] = pw[j].y;
-      if constexpr (GEN) load_pos(a, row, tok, s, pos, 4);
-      float x[2][NQ][4];
+      for (int j = 0; j < 4; ++j) {
+        const uint2 p = st.par[8 * j + g];
+        kp[j] = p.x, vp[j] = p.y;
+      }
+      const bool tail = t0 + kUnit > s.n;
+      if (tail) {  // what lies past the end may be anything
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        tile_scores<D, NQ, QLO, GEN>(a, q, kw[2 * i], kw[2 * i + 1], kp + 2 * i, tok + 2 * i, pos + 2 * i, s.n, pre, x[i]);
-      if (more) load_k(t_next);
-
-      // log2 of the V scales; a scale of 0 has only zeros behind it
+        for (int j = 0; j < 4; ++j)
+          if (t0 + 8 * j + g >= s.n) kp[j] = vp[j] = 0u;
+      }
+      float x[2][NQ][4];
+      {
+        uint32_t k[4][W];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) lds_codes<W>(st.k[j][lane], k[j]);
+        products<2, D, NQ, QLO>(q, k, kp, x);
+      }
+      // scores
+      int tok[4], pos[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) tok[j] = t0 + 8 * j + g;
+      if constexpr (GEN) load_pos<4>(a, row, tok, s, pos);
       float lv[4], zv[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float sv = par_scale(vp[j]);
-        lv[j] = sv == 0.0f ? -100.0f : lg2(sv);
+        const float sk = par_scale(kp[j]), sv = par_scale(vp[j]);
+        lv[j] = (sv == 0.0f ? -100.0f : lg2(sv)) + kHead;  // a scale of 0 has only zeros behind it
         zv[j] = par_zero(vp[j]);
+#pragma unroll
+        for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float& v = x[j >> 1][nq][2 * (j & 1) + e];
+            v *= sk * q.fac[nq][e];
+            if constexpr (GEN) v = full_score<D, NQ, QLO>(a, q, nq, e, v, tok[j] < s.n, pos[j], pre);
+            else if (tail && tok[j] >= s.n) v = -INFINITY;
+          }
       }
       uint32_t pb[NQ][4], pl[QLO ? NQ : 1][4];
 #pragma unroll
       for (int nq = 0; nq < NQ; ++nq) {
-        float p[2][4], alpha[2];
+        // exponents of P, above the reference; a token that is not seen has none, whatever its scale
+        float w[4][2];
+        auto exponents = [&] {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float xs[4], w[4];
+          for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            xs[j] = x[j >> 1][nq][2 * (j & 1) + e];
-            w[j] = xs[j] == -INFINITY ? -INFINITY : xs[j] + lv[j];
+            for (int e = 0; e < 2; ++e) {
+              const float v = x[j >> 1][nq][2 * (j & 1) + e];
+              w[j][e] = (v - m[nq][e]) + lv[j];
+              if (GEN && v == -INFINITY) w[j][e] = -INFINITY;
+            }
+        };
+        exponents();
+        const float w0 = fmaxf(fmaxf(w[0][0], w[1][0]), fmaxf(w[2][0], w[3][0]));
+        const float w1 = fmaxf(fmaxf(w[0][1], w[1][1]), fmaxf(w[2][1], w[3][1]));
+        if (__any_sync(0xffffffffu, fmaxf(w0, w1) > kTop)) {
+          float alpha[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float mt = kNone;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float v = x[j >> 1][nq][2 * (j & 1) + e];
+              if (!GEN || v != -INFINITY) mt = fmaxf(mt, v + lv[j] - kHead);
+            }
+            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 4));
+            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 8));
+            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 16));
+            mt = fmaxf(m[nq][e], mt);
+            alpha[e] = ex2(m[nq][e] - mt);
+            m[nq][e] = mt;
+            l[nq][e] *= alpha[e];
+            z[nq][e] *= alpha[e];
           }
-          float mt = fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]));
-          mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 4));
-          mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 8));
-          mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 16));
-          const float mn = fmaxf(m[nq][e], mt), ref = mn == -INFINITY ? 0.0f : mn, ref15 = ref - 15.0f;
-          alpha[e] = ex2(m[nq][e] - ref);
-          m[nq][e] = mn;
-          l[nq][e] *= alpha[e];
-          z[nq][e] *= alpha[e];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            l[nq][e] += ex2(xs[j] - ref);
-            p[j >> 1][2 * (j & 1) + e] = ex2(w[j] - ref15);
-          }
-        }
-        if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
 #pragma unroll
           for (int d = 0; d < 2 * W; ++d)
 #pragma unroll
             for (int i = 0; i < 4; ++i) O[nq][d][i] *= alpha[i & 1];
+          exponents();
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float pa = p[j >> 1][2 * (j & 1)], pc = p[j >> 1][2 * (j & 1) + 1];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) l[nq][e] += ex2(x[j >> 1][nq][2 * (j & 1) + e] - m[nq][e]);
+          const float pa = ex2(w[j][0]), pc = ex2(w[j][1]);
           const uint32_t r = h2(pa, pc);
           const float2 rf = f2(r);
-          // tokens past the end have p = 0, but their zero point may be anything
-          const float zj = tok[j] < s.n ? zv[j] : 0.0f;
           if constexpr (QLO) {
             const uint32_t rl = h2(pa - rf.x, pc - rf.y);
             const float2 rlf = f2(rl);
             pl[nq][j] = transposed(rl);
-            z[nq][0] = fmaf(rf.x + rlf.x, zj, z[nq][0]);
-            z[nq][1] = fmaf(rf.y + rlf.y, zj, z[nq][1]);
+            z[nq][0] = fmaf(rf.x + rlf.x, zv[j], z[nq][0]);
+            z[nq][1] = fmaf(rf.y + rlf.y, zv[j], z[nq][1]);
           } else {
-            z[nq][0] = fmaf(rf.x, zj, z[nq][0]);
-            z[nq][1] = fmaf(rf.y, zj, z[nq][1]);
+            z[nq][0] = fmaf(rf.x, zv[j], z[nq][0]);
+            z[nq][1] = fmaf(rf.y, zv[j], z[nq][1]);
           }
           pb[nq][j] = transposed(r);
         }
       }
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 2; ++i) {
+        uint32_t v0[W], v1[W];
+        lds_codes<W>(st.v[2 * i][lane], v0);
+        lds_codes<W>(st.v[2 * i + 1][lane], v1);
 #pragma unroll
         for (int w = 0; w < W; ++w) {
           uint32_t va[4], vb[4];
-          VN::take(vw[2 * i][w], va);
-          VN::take(vw[2 * i + 1][w], vb);
+          VN::take(v0[w], va);
+          VN::take(v1[w], vb);
 #pragma unroll
           for (int nq = 0; nq < NQ; ++nq) {
             mma16(O[nq][2 * w], va[0], va[2], vb[0], vb[2], pb[nq][2 * i], pb[nq][2 * i + 1]);
@@ -481,12 +636,31 @@ __global__ void __launch_bounds__(32 * kWarps, NQ == 1 && !QLO && !GEN ? 4 : 2) 
             }
           }
         }
-      if (more) load_v(t_next);
+      }
+      __syncwarp();
+      ask(u + kStages * kWarps);
     }
 
     // ---- merge the warps: O in true units, minus the zero points' share ----
+    const bool whole = u0 == 0 && u1 == s.count;
+    const int b_done = b, h_done = h;
+    x0 += u1 - u0;
+    const bool more = x0 < x1;
+    if (more) {  // the next head's first units come while this one is merged
+      ++h;
+      while (h == a.kv.H || s.count == 0) {
+        s = seq_of(a, ++b);
+        h = 0;
+      }
+      u0 = 0;
+      u1 = min(s.count, x1 - x0);
+#pragma unroll
+      for (int i = 0; i < kStages; ++i) ask(warp + i * kWarps);
+    }
+    const int64_t slot = ((int64_t)cta + bh) * a.rows_pad;
 #pragma unroll
     for (int nq = 0; nq < NQ; ++nq) {
+      __syncthreads();  // the last round's O has been read
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
@@ -494,79 +668,94 @@ __global__ void __launch_bounds__(32 * kWarps, NQ == 1 && !QLO && !GEN ? 4 : 2) 
           l[nq][e] += __shfl_xor_sync(0xffffffffu, l[nq][e], k);
           z[nq][e] += __shfl_xor_sync(0xffffffffu, z[nq][e], k);
         }
-        if (g == 0) mlb[warp][8 * nq + 2 * c + e] = make_float2(m[nq][e], l[nq][e]);
+        if (g == 0) sh.ml[warp][8 * nq + 2 * c + e] = make_float2(m[nq][e], l[nq][e]);
       }
+      // d = 4 (g W + w) + n: nibble n of word w
 #pragma unroll
-      for (int d = 0; d < 2 * W; ++d)
+      for (int w = 0; w < W; ++w)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          ob[warp][8 * nq + 2 * c + (i & 1)][(g * W + d / 2) * 4 + (d & 1) + 2 * (i >> 1)] =
-              fmaf(O[nq][d][i], pow2(-VN::unit(d & 1)), -z[nq][i & 1]) * pow2(-15);
+        for (int e = 0; e < 2; ++e) {
+          float v[4];
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+            v[n] = fmaf(O[nq][2 * w + (n & 1)][e + 2 * (n >> 1)], pow2(-VN::unit(n & 1)), -z[nq][e]) * pow2(-(int)kHead);
+          *reinterpret_cast<float4*>(&sh.o[warp][2 * c + e][4 * (g * W + w)]) = make_float4(v[0], v[1], v[2], v[3]);
+        }
+      __syncthreads();
+      for (int i = threadIdx.x; i < 2 * D; i += 32 * kWarps) {
+        const int r = i / (D / 4), d = 4 * (i % (D / 4)), qr = zb * 8 * NQ + 8 * nq + r;
+        if (qr >= a.rows) break;
+        float M = kNone;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sh.ml[w][8 * nq + r].x);
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float2 ml = sh.ml[w][8 * nq + r];
+          const float f = ex2(ml.x - M);
+          const float4 v = *reinterpret_cast<const float4*>(&sh.o[w][r][d]);
+          o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
+          L = fmaf(f, ml.y, L);
+        }
+        if (whole) {
+          const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+          const int iq = qr / a.G, hq = h_done * a.G + qr % a.G;
+          st_out4(a.out, (((int64_t)b_done * a.Hq + hq) * a.Sq + iq) * D + d, a.q_dtype, o, inv);
+          if (a.lse && d == 0) a.lse[(int64_t)bh * a.rows_pad + qr] = L == 0.0f ? INFINITY : M + lg2(L);
+        } else {
+          *reinterpret_cast<float4*>(a.part + (slot + qr) * D + d) = o;
+          if (d == 0) a.ml[slot + qr] = make_float2(M, L);
+        }
+      }
     }
-    __syncthreads();
-    const bool whole = u0 == 0 && u1 == s.count;
-    const int64_t slot = ((int64_t)cta + bh) * a.rows_pad;
-    for (int i = threadIdx.x; i < NR * D; i += 32 * kWarps) {
-      const int r = i / D, d = i % D, qr = zb * NR + r;
-      if (qr >= a.rows) break;
-      float M = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) M = fmaxf(M, mlb[w][r].x);
-      const float ref = M == -INFINITY ? 0.0f : M;
-      float o = 0.0f, L = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float f = ex2(mlb[w][r].x - ref);
-        o = fmaf(f, ob[w][r][d], o);
-        L = fmaf(f, mlb[w][r].y, L);
-      }
-      if (whole) {
-        const int iq = qr / a.G, hq = h * a.G + qr % a.G;
-        st_out(a.out, (((int64_t)b * a.Hq + hq) * a.Sq + iq) * D + d, a.q_dtype, L == 0.0f ? 0.0f : o / L);
-        if (a.lse && d == 0) a.lse[(int64_t)bh * a.rows_pad + qr] = L == 0.0f ? INFINITY : ref + lg2(L);
-      } else {
-        a.part[(slot + qr) * D + d] = o;
-        if (d == 0) a.ml[slot + qr] = make_float2(M, L);
-      }
-    }
-    __syncthreads();
-    x0 += u1 - u0;
+    if (!more) break;
   }
   if (threadIdx.x == 0) pdl_trigger();
 }
 
-// One block per (row, head): merges the partial results of the blocks that
+// One warp per (row, head): merges the partial results of the blocks that
 // shared the head; zeros where there is nothing to see.  Heads that one block
-// covered are done already.
+// covered are done already.  The lengths are older than the kernel before this
+// one, so they are read while it still runs.
 __global__ void __launch_bounds__(128) kv4_combine_kernel(const Attn a) {
-  pdl_wait();
-  const int bh = blockIdx.y, b = bh / a.kv.H, h = bh % a.kv.H, qr = blockIdx.x, D = a.kv.D, d = threadIdx.x;
-  const int64_t units = all_units(a);
-  const int64_t blocks = units < a.blocks ? units : a.blocks;
+  const int item = blockIdx.x * 4 + threadIdx.x / 32, lane = threadIdx.x & 31, D = a.kv.D, V = D / 32;
+  if (item >= a.rows * a.kv.B * a.kv.H) return;
+  const int bh = item / a.rows, qr = item % a.rows, b = bh / a.kv.H, h = bh % a.kv.H;
   const Seq s = seq_of(a, b);
-  float o = 0.0f, L = 0.0f, ref = 0.0f;
-  if (s.count > 0) {
-    int64_t begin = 0;  // units of the sequences before b
-    for (int j = threadIdx.x & 31; j < b; j += 32) begin += seq_of(a, j).count;
+  int all;
+  int begin = units_before(a, b, all);
+  Cut cut;
+  cut.set(all, a.blocks);
+  begin += h * s.count;
+  const int c0 = s.count ? cut.owner(begin) : 0, c1 = s.count ? cut.owner(begin + s.count - 1) : -1;
+  if (s.count && c0 == c1) return;
+  pdl_wait();
+  float M = kNone, L = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  const int64_t first = (int64_t)(c0 + bh) * a.rows_pad + qr;
+  for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, a.ml[first + (int64_t)(c - c0) * a.rows_pad].x);
 #pragma unroll
-    for (int m = 16; m > 0; m >>= 1) begin += __shfl_xor_sync(0xffffffffu, begin, m);
-    begin = begin * a.kv.H + (int64_t)h * s.count;
-    const int64_t c0 = ((begin + 1) * blocks - 1) / units, c1 = ((begin + s.count) * blocks - 1) / units;
-    if (c0 == c1) return;
-    float M = -INFINITY;
-    for (int64_t c = c0; c <= c1; ++c) M = fmaxf(M, a.ml[(c + bh) * a.rows_pad + qr].x);
-    ref = M == -INFINITY ? 0.0f : M;
-    for (int64_t c = c0; c <= c1; ++c) {
-      const int64_t i = (c + bh) * a.rows_pad + qr;
-      const float2 ml = a.ml[i];
-      const float f = ex2(ml.x - ref);
-      o = fmaf(f, d < D ? a.part[i * D + d] : 0.0f, o);
-      L = fmaf(f, ml.y, L);
+  for (int m = 16; m > 0; m >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, m));
+#pragma unroll 4
+  for (int c = 0; c <= c1 - c0; ++c) {
+    const int64_t i = first + (int64_t)c * a.rows_pad;
+    const float2 ml = a.ml[i];
+    const float f = ex2(ml.x - M);
+    L = fmaf(f, ml.y, L);
+    const float* p = a.part + i * D + V * lane;
+    if (V == 4) {
+      const float4 v = *reinterpret_cast<const float4*>(p);
+      o[0] = fmaf(f, v.x, o[0]), o[1] = fmaf(f, v.y, o[1]), o[2] = fmaf(f, v.z, o[2]), o[3] = fmaf(f, v.w, o[3]);
+    } else {
+      const float2 v = *reinterpret_cast<const float2*>(p);
+      o[0] = fmaf(f, v.x, o[0]), o[1] = fmaf(f, v.y, o[1]);
     }
   }
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
   const int iq = qr / a.G, hq = h * a.G + qr % a.G;
-  if (d < D) st_out(a.out, (((int64_t)b * a.Hq + hq) * a.Sq + iq) * D + d, a.q_dtype, L == 0.0f ? 0.0f : o / L);
-  if (a.lse && d == 0) a.lse[(int64_t)bh * a.rows_pad + qr] = L == 0.0f ? INFINITY : ref + lg2(L);
+  const int64_t at = (((int64_t)b * a.Hq + hq) * a.Sq + iq) * D + V * lane;
+  for (int i = 0; i < V; ++i) st_out(a.out, at + i, a.q_dtype, o[i] * inv);
+  if (a.lse && lane == 0) a.lse[(int64_t)bh * a.rows_pad + qr] = L == 0.0f ? INFINITY : M + lg2(L);
 }
 
 // mass[t] += sum over the rows of exp2(x[r, t] - lse[r]).  A warp owns 16
@@ -575,34 +764,45 @@ __global__ void __launch_bounds__(128) kv4_combine_kernel(const Attn a) {
 template <int D, bool QLO, bool GEN>
 __global__ void __launch_bounds__(128) kv4_mass_kernel(const Attn a) {
   constexpr int W = D / 32;
+  __shared__ RowsShared<D, 1, QLO> sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int bh = blockIdx.y, b = bh / a.kv.H, h = bh % a.kv.H;
   const Seq s = seq_of(a, b);
   const int pre = GEN && a.prefix ? a.prefix[b] : 0;
   const int64_t row = (int64_t)bh * a.kv.cap;
-  for (int t0 = (blockIdx.x * 4 + warp) * 16; t0 < s.n && s.cnt > 0; t0 += gridDim.x * 64) {
-    uint32_t kw[2][W], kp[2];
-    int tok[2], pos[4];
+  if (s.cnt == 0) return;
+  for (int base = blockIdx.x * 64; base < s.n; base += gridDim.x * 64) {
+    const int t0 = base + warp * 16;  // within the capacity, a multiple of 32: the last warps of a block may find
+    const bool some = t0 < s.n;       // nothing there, but they help with the queries
+    uint32_t kw[2][W] = {}, kp[2] = {0u, 0u};
+    int tok[2], pos[2];
     float sum[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      ld_codes<W>(a.kv.k + (row + t0 + 8 * j) * (D / 2) + lane * (4 * W), kw[j]);
       tok[j] = t0 + 8 * j + g;
-      kp[j] = a.kv.par[row + tok[j]].x;
+      if (some) ld_codes<W>(a.kv.k + (row + t0 + 8 * j) * (D / 2) + lane * (4 * W), kw[j]);
+      if (tok[j] < s.n) kp[j] = a.kv.par[row + tok[j]].x;
     }
-    if constexpr (GEN) load_pos(a, row, tok, s, pos, 2);
+    if constexpr (GEN) load_pos<2>(a, row, tok, s, pos);
     for (int zb = 0; zb * 8 < a.rows; ++zb) {
+      __syncthreads();
+      Rows<D, 1, QLO>::make(sh, a, s, b, h, zb, threadIdx.x, 128, GEN);
+      __syncthreads();
       Rows<D, 1, QLO> q;
-      q.load(a, s, b, h, zb, GEN);
-      float x[1][4];
-      tile_scores<D, 1, QLO, GEN>(a, q, kw[0], kw[1], kp, tok, pos, s.n, pre, x);
+      q.load(sh, a, s, h, zb, GEN);
+      float x[1][1][4];
+      products<1, D, 1, QLO>(q, kw, kp, x);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int qr = zb * 8 + 2 * c + e;
         if (qr >= a.rows) continue;
         const float lse = a.lse[(int64_t)bh * a.rows_pad + qr];
-        sum[0] += ex2(x[0][e] - lse);
-        sum[1] += ex2(x[0][2 + e] - lse);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float v = x[0][0][2 * j + e] * (par_scale(kp[j]) * q.fac[0][e]);
+          if constexpr (GEN) v = full_score<D, 1, QLO>(a, q, 0, e, v, tok[j] < s.n, pos[j], pre);
+          sum[j] += ex2(v - lse);
+        }
       }
     }
 #pragma unroll
@@ -614,18 +814,22 @@ __global__ void __launch_bounds__(128) kv4_mass_kernel(const Attn a) {
   }
 }
 
-// Rows of a block, and blocks of the split: one wave of 4 blocks per SM over
+// Rows of a block, and blocks of the split: one wave of resident blocks over
 // all row blocks, and at least one unit per warp.
 struct Plan {
   int nq, row_blocks, rows_pad, blocks;
 };
-Plan plan_of(const Kv4& kv, int64_t rows, int64_t bound) {
+Plan plan_of(const Kv4& kv, int64_t rows, int64_t bound, bool qlo) {
   Plan p;
   p.nq = rows <= 8 ? 1 : 2;
   p.row_blocks = (int)((rows + 8 * p.nq - 1) / (8 * p.nq));
   p.rows_pad = p.row_blocks * 8 * p.nq;
   const int64_t units = (int64_t)kv.B * kv.H * ((std::max<int64_t>(bound, 1) + kUnit - 1) / kUnit);
-  const int64_t slots = std::max<int64_t>(1, (int64_t)num_sms() * 4 / p.row_blocks);
+  int64_t slots = std::max<int64_t>(1, (int64_t)num_sms() * (p.nq == 1 && !qlo ? 4 : p.nq == 1 ? 2 : 1) / p.row_blocks);
+  // the same number of blocks for every head, where that leaves few slots empty:
+  // with equal lengths no block then has to change heads
+  const int64_t heads = (int64_t)kv.B * kv.H;
+  if (slots >= heads && slots % heads * 10 <= slots) slots -= slots % heads;
   p.blocks = (int)std::max<int64_t>(1, std::min<int64_t>(slots, (units + kWarps - 1) / kWarps));
   return p;
 }
@@ -640,9 +844,13 @@ void spaces(const Kv4& kv, const Plan& p, bool weigh, size_t* bytes) {
 
 template <int D, int NQ, bool QLO, bool GEN>
 int run_attn(const Attn& a, const Plan& p, cudaStream_t st) {
-  kv4_attn_kernel<D, NQ, QLO, GEN><<<dim3(p.blocks, p.row_blocks), 32 * kWarps, 0, st>>>(a);
+  constexpr int smem = sizeof(AttnShared<D, NQ, QLO>);
+  auto kern = kv4_attn_kernel<D, NQ, QLO, GEN>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return launched("kv4_attn_kernel (attribute)");
+  kern<<<dim3(p.blocks, p.row_blocks), 32 * kWarps, smem, st>>>(a);
   LQ_TRY(launched("kv4_attn_kernel"));
-  launch_pdl(kv4_combine_kernel, dim3(a.rows, a.kv.B * a.kv.H), dim3(D), 0, st, a);
+  launch_pdl(kv4_combine_kernel, dim3((unsigned)(((int64_t)a.rows * a.kv.B * a.kv.H + 3) / 4)), dim3(128), 0, st, a);
   LQ_TRY(launched("kv4_combine_kernel"));
   if (a.lse) {
     kv4_mass_kernel<D, QLO, GEN><<<dim3((a.kv.cap + 63) / 64, a.kv.B * a.kv.H), 128, 0, st>>>(a);
@@ -666,11 +874,10 @@ int run_attn_d(const Attn& a, const Plan& p, bool gen, cudaStream_t st) {
 extern "C" size_t lq_kv4_attention_workspace_bytes(const lq_kv4_cache* cache, int q_dtype, int64_t Hq, int64_t Sq,
                                                    int64_t bound, int accumulate) {
   using namespace lq;
-  (void)q_dtype;
   if (kv4_check(cache) != LQ_OK || Hq <= 0 || Sq <= 0 || Hq % cache->H) return 0;
   const Kv4 kv = kv4_of(cache);
   size_t b[3];
-  spaces(kv, plan_of(kv, Hq / cache->H * Sq, bound), accumulate != 0, b);
+  spaces(kv, plan_of(kv, Hq / cache->H * Sq, bound, q_dtype == LQ_F32), accumulate != 0, b);
   return b[0] + b[1] + b[2];
 }
 
@@ -689,10 +896,10 @@ extern "C" int lq_kv4_attention(const lq_kv4_cache* cache, const void* q, int q_
   LQ_REQUIRE(window >= 0 && window <= INT32_MAX, LQ_EINVAL, "bad window");
   const int64_t rows = Hq / cache->H * Sq;
   if (rows == 0) return LQ_OK;
-  LQ_REQUIRE(rows <= 16 * 65535, LQ_ERANGE, "too many query rows");
+  LQ_REQUIRE(rows <= 16 * 65535 && rows * cache->B * cache->H <= INT32_MAX, LQ_ERANGE, "too many query rows");
   LQ_REQUIRE(q && out, LQ_EINVAL, "NULL pointer");
   const Kv4 kv = kv4_of(cache);
-  const Plan p = plan_of(kv, rows, bound);
+  const Plan p = plan_of(kv, rows, bound, q_dtype == LQ_F32);
   size_t bytes[3];
   spaces(kv, p, accumulate != 0, bytes);
   LQ_REQUIRE(workspace && workspace_bytes >= bytes[0] + bytes[1] + bytes[2], LQ_EINVAL, "workspace of %zu bytes needed",

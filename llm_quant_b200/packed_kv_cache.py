@@ -56,7 +56,7 @@ class _LayerStore:
         self.params = torch.empty(B, H, cap, 2, dtype=torch.int32, device=device)
         self.positions = new(-1, B, H, cap)
         self.mass = new(0.0, B, H, cap, dtype=torch.float32)
-        self.state = new(0, 2 * B + 3)
+        self.state = new(0, 2 * B + 4)
         self.bound = 0        # no sequence holds more tokens, as far as the host knows
         self.captured = False  # an append was captured: replays are not seen by the host
         self.c = _C.KV4Cache(self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.params.data_ptr(),
