@@ -449,13 +449,19 @@ int lq_kv4_evict(const lq_kv4_cache* host_cache, int64_t keep, int64_t recent, i
  *   or (prefix not NULL and t < prefix[b]).
  * accumulate: mass of each token += the weights it got from all query rows.
  * bound: tokens that the longest sequence is thought to hold (only the split
- * of the work goes by it).  The workspace is for this call alone. */
-size_t lq_kv4_attention_workspace_bytes(const lq_kv4_cache* host_cache, int q_dtype, int64_t Hq, int64_t Sq,
-                                        int64_t bound, int accumulate);
-int lq_kv4_attention(const lq_kv4_cache* host_cache, const void* q, int q_dtype, int64_t Hq, int64_t Sq,
-                     int64_t q_sb, int64_t q_sh, int64_t q_ss, int64_t bound, const int32_t* counts,
-                     float sm_scale, int causal, float softcap, const float* slopes, int64_t window,
-                     const int32_t* prefix, int accumulate, void* out, void* workspace, size_t workspace_bytes, void* stream);
+ * of the work goes by it).  The workspace, of lq_kv4_attention_workspace_bytes for
+ * the same form, is for this call alone. */
+typedef struct {
+  int64_t Hq, Sq, q_sb, q_sh, q_ss, bound, window;
+  float sm_scale, softcap;
+  int q_dtype, causal, accumulate;
+} lq_kv4_attn;
+size_t lq_kv4_attention_workspace_bytes(const lq_kv4_cache* host_cache, const lq_kv4_attn* host_form);
+int lq_kv4_attention(const lq_kv4_cache* host_cache, const lq_kv4_attn* host_form, const void* q,
+                     const int32_t* counts, const float* slopes, const int32_t* prefix, void* out,
+                     void* workspace, size_t workspace_bytes, void* stream);
+/* An empty cache again (device work on `stream`). */
+int lq_kv4_reset(const lq_kv4_cache* host_cache, void* stream);
 
 #ifdef __cplusplus
 }

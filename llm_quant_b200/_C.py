@@ -81,8 +81,8 @@ _SIGS = {
     "lq_kv4_append": [_V, _V, _V, _I, _L, _L, _L, _L, _L, _L, _L, _V, _V],
     "lq_kv4_dequant": [_V, _L, _I, _V, _V, _V],
     "lq_kv4_evict": [_V, _L, _L, _L, _V, ctypes.c_size_t, _V],
-    "lq_kv4_attention": [_V, _V, _I, _L, _L, _L, _L, _L, _L, _V, ctypes.c_float, _I, ctypes.c_float,
-                         _V, _L, _V, _I, _V, _V, ctypes.c_size_t, _V],
+    "lq_kv4_attention": [_V, _V, _V, _V, _V, _V, _V, _V, ctypes.c_size_t, _V],
+    "lq_kv4_reset": [_V, _V],
 }
 _SIZE_SIGS = {
     "lq_tensor_qparams_workspace_size": [_L],
@@ -91,7 +91,7 @@ _SIZE_SIGS = {
     "lq_nf4_linear_packed_bytes": [_L, _L],
     "lq_kv_attention_workspace_bytes": [_L, _L, _L, _L, _L, _L],
     "lq_kv4_evict_workspace_bytes": [_L, _L, _L, _L],
-    "lq_kv4_attention_workspace_bytes": [_V, _I, _L, _L, _L, _I],
+    "lq_kv4_attention_workspace_bytes": [_V, _V],
 }
 
 
@@ -99,6 +99,13 @@ class KV4Cache(ctypes.Structure):
     """lq_kv4_cache"""
     _fields_ = [(n, _V) for n in ("k_codes", "v_codes", "params", "positions", "mass", "state")] + \
                [(n, _L) for n in ("B", "H", "cap", "D")]
+
+
+class KV4Attn(ctypes.Structure):
+    """lq_kv4_attn"""
+    _fields_ = [(n, _L) for n in ("Hq", "Sq", "q_sb", "q_sh", "q_ss", "bound", "window")] + \
+               [(n, ctypes.c_float) for n in ("sm_scale", "softcap")] + \
+               [(n, _I) for n in ("q_dtype", "causal", "accumulate")]
 
 
 _lib = None
@@ -153,6 +160,11 @@ def launch_count() -> int:
 
 def stream_ptr(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def raw_stream(index: int) -> int:
+    """The current stream of device `index`, without the stream object."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def ptr(t: torch.Tensor | None):

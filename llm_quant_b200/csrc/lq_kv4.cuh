@@ -68,7 +68,9 @@ inline int kv4_check(const lq_kv4_cache* c) {
   LQ_REQUIRE(c->cap % kUnit == 0, LQ_EINVAL, "capacity %lld must be a multiple of %d", (long long)c->cap, kUnit);
   LQ_REQUIRE(c->cap <= (1LL << 30) && c->B * c->H <= 65535, LQ_ERANGE, "cache too large");
   LQ_REQUIRE(c->k_codes && c->v_codes && c->params && c->positions && c->mass && c->state, LQ_EINVAL, "NULL pointer");
-  LQ_REQUIRE(aligned16(c->k_codes) && aligned16(c->v_codes) && aligned16(c->params), LQ_EALIGN,
+  LQ_REQUIRE(aligned16(c->k_codes) && aligned16(c->v_codes) && aligned16(c->params) && aligned16(c->positions) &&
+                 aligned16(c->mass),
+             LQ_EALIGN,
              "cache buffers must be 16-byte aligned");
   return LQ_OK;
 }

@@ -871,58 +871,58 @@ int run_attn_d(const Attn& a, const Plan& p, bool gen, cudaStream_t st) {
 }  // namespace
 }  // namespace lq
 
-extern "C" size_t lq_kv4_attention_workspace_bytes(const lq_kv4_cache* cache, int q_dtype, int64_t Hq, int64_t Sq,
-                                                   int64_t bound, int accumulate) {
+extern "C" size_t lq_kv4_attention_workspace_bytes(const lq_kv4_cache* cache, const lq_kv4_attn* f) {
   using namespace lq;
-  if (kv4_check(cache) != LQ_OK || Hq <= 0 || Sq <= 0 || Hq % cache->H) return 0;
+  if (!f || kv4_check(cache) != LQ_OK || f->Hq <= 0 || f->Sq <= 0 || f->Hq % cache->H) return 0;
   const Kv4 kv = kv4_of(cache);
   size_t b[3];
-  spaces(kv, plan_of(kv, Hq / cache->H * Sq, bound, q_dtype == LQ_F32), accumulate != 0, b);
+  spaces(kv, plan_of(kv, f->Hq / cache->H * f->Sq, f->bound, f->q_dtype == LQ_F32), f->accumulate != 0, b);
   return b[0] + b[1] + b[2];
 }
 
-extern "C" int lq_kv4_attention(const lq_kv4_cache* cache, const void* q, int q_dtype, int64_t Hq, int64_t Sq,
-                                int64_t q_sb, int64_t q_sh, int64_t q_ss, int64_t bound, const int32_t* counts,
-                                float sm_scale, int causal, float softcap, const float* slopes, int64_t window,
-                                const int32_t* prefix, int accumulate, void* out, void* workspace,
+extern "C" int lq_kv4_attention(const lq_kv4_cache* cache, const lq_kv4_attn* f, const void* q, const int32_t* counts,
+                                const float* slopes, const int32_t* prefix, void* out, void* workspace,
                                 size_t workspace_bytes, void* stream) {
   using namespace lq;
   LQ_TRY(kv4_check(cache));
-  LQ_REQUIRE(is_float_dtype(q_dtype), LQ_EDTYPE, "float query required");
-  LQ_REQUIRE(Hq > 0 && Hq % cache->H == 0, LQ_EINVAL, "query heads %lld not a multiple of kv heads %lld",
-             (long long)Hq, (long long)cache->H);
-  LQ_REQUIRE(Sq >= 0 && bound >= 0, LQ_EINVAL, "bad shape");
-  LQ_REQUIRE(softcap >= 0.0f, LQ_EINVAL, "softcap must not be negative");
-  LQ_REQUIRE(window >= 0 && window <= INT32_MAX, LQ_EINVAL, "bad window");
-  const int64_t rows = Hq / cache->H * Sq;
+  LQ_REQUIRE(f, LQ_EINVAL, "NULL form");
+  LQ_REQUIRE(is_float_dtype(f->q_dtype), LQ_EDTYPE, "float query required");
+  LQ_REQUIRE(f->Hq > 0 && f->Hq % cache->H == 0, LQ_EINVAL, "query heads %lld not a multiple of kv heads %lld",
+             (long long)f->Hq, (long long)cache->H);
+  LQ_REQUIRE(f->Sq >= 0 && f->bound >= 0, LQ_EINVAL, "bad shape");
+  LQ_REQUIRE(f->softcap >= 0.0f, LQ_EINVAL, "softcap must not be negative");
+  LQ_REQUIRE(f->window >= 0 && f->window <= INT32_MAX, LQ_EINVAL, "bad window");
+  const int64_t rows = f->Hq / cache->H * f->Sq;
   if (rows == 0) return LQ_OK;
   LQ_REQUIRE(rows <= 16 * 65535 && rows * cache->B * cache->H <= INT32_MAX, LQ_ERANGE, "too many query rows");
   LQ_REQUIRE(q && out, LQ_EINVAL, "NULL pointer");
+  LQ_REQUIRE((uintptr_t)q % (4 * dtype_size(f->q_dtype)) == 0 && ((f->q_sb | f->q_sh | f->q_ss) & 3) == 0, LQ_EALIGN,
+             "query rows must start on multiples of 4 elements");
   const Kv4 kv = kv4_of(cache);
-  const Plan p = plan_of(kv, rows, bound, q_dtype == LQ_F32);
+  const Plan p = plan_of(kv, rows, f->bound, f->q_dtype == LQ_F32);
   size_t bytes[3];
-  spaces(kv, p, accumulate != 0, bytes);
+  spaces(kv, p, f->accumulate != 0, bytes);
   LQ_REQUIRE(workspace && workspace_bytes >= bytes[0] + bytes[1] + bytes[2], LQ_EINVAL, "workspace of %zu bytes needed",
              bytes[0] + bytes[1] + bytes[2]);
-  LQ_REQUIRE(aligned16(workspace), LQ_EALIGN, "workspace must be 16-byte aligned");
+  LQ_REQUIRE(aligned16(workspace) && aligned16(out), LQ_EALIGN, "output and workspace must be 16-byte aligned");
   Attn a;
   a.kv = kv;
   a.q = static_cast<const uint8_t*>(q);
-  a.q_dtype = q_dtype;
-  a.q_sb = q_sb, a.q_sh = q_sh, a.q_ss = q_ss;
-  a.Hq = (int)Hq, a.G = (int)(Hq / cache->H), a.Sq = (int)Sq, a.rows = (int)rows, a.rows_pad = p.rows_pad;
+  a.q_dtype = f->q_dtype;
+  a.q_sb = f->q_sb, a.q_sh = f->q_sh, a.q_ss = f->q_ss;
+  a.Hq = (int)f->Hq, a.G = (int)(f->Hq / cache->H), a.Sq = (int)f->Sq, a.rows = (int)rows, a.rows_pad = p.rows_pad;
   a.counts = counts;
-  a.sm = sm_scale, a.cap = softcap;
+  a.sm = f->sm_scale, a.cap = f->softcap;
   a.slopes = slopes, a.prefix = prefix;
-  a.causal = causal != 0, a.window = (int)window;
+  a.causal = f->causal != 0, a.window = (int)f->window;
   a.blocks = p.blocks;
   a.out = static_cast<uint8_t*>(out);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   a.part = reinterpret_cast<float*>(ws);
   a.ml = reinterpret_cast<float2*>(ws + bytes[0]);
-  a.lse = accumulate ? reinterpret_cast<float*>(ws + bytes[0] + bytes[1]) : nullptr;
+  a.lse = f->accumulate ? reinterpret_cast<float*>(ws + bytes[0] + bytes[1]) : nullptr;
   // a single query sees every token but for a window, a bias or a cap
-  const bool gen = (Sq > 1 && (causal || counts)) || softcap > 0.0f || slopes || window > 0;
+  const bool gen = (f->Sq > 1 && (f->causal || counts)) || f->softcap > 0.0f || slopes || f->window > 0;
   cudaStream_t st = as_stream(stream);
   return kv.D == 128 ? run_attn_d<128>(a, p, gen, st) : run_attn_d<64>(a, p, gen, st);
 }

@@ -316,6 +316,16 @@ __global__ void __launch_bounds__(kEvictThreads) kv4_evict_kernel(Kv4 kv, EvictA
       if (kv.len[j] > keep) kv.len[j] = keep, kv.sync[2] = 1;
 }
 
+__global__ void __launch_bounds__(256) kv4_reset_kernel(Kv4 kv) {
+  const int64_t n = (int64_t)kv.B * kv.H * kv.cap / 4, step = (int64_t)gridDim.x * blockDim.x;
+  const int64_t i0 = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  for (int64_t i = i0; i < n; i += step) {
+    reinterpret_cast<int4*>(kv.pos)[i] = make_int4(-1, -1, -1, -1);
+    reinterpret_cast<float4*>(kv.mass)[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
+  for (int64_t i = i0; i < 2 * kv.B + 4; i += step) kv.len[i] = 0;
+}
+
 template <typename T>
 int append_t(const Kv4& kv, const AppendArgs& a, cudaStream_t st) {
   const int tpb = kv.D == 128 ? 8 : 16;
@@ -398,4 +408,13 @@ extern "C" int lq_kv4_evict(const lq_kv4_cache* cache, int64_t keep, int64_t rec
   if (kv.D == 128) kv4_evict_kernel<128><<<kv.B * kv.H, kEvictThreads, 0, st>>>(kv, a);
   else kv4_evict_kernel<64><<<kv.B * kv.H, kEvictThreads, 0, st>>>(kv, a);
   return launched("kv4_evict_kernel");
+}
+
+extern "C" int lq_kv4_reset(const lq_kv4_cache* cache, void* stream) {
+  using namespace lq;
+  LQ_TRY(kv4_check(cache));
+  const Kv4 kv = kv4_of(cache);
+  const int64_t n = (int64_t)kv.B * kv.H * kv.cap / 4;
+  kv4_reset_kernel<<<resident_grid(kv4_reset_kernel, 256, 0, (n + 255) / 256), 256, 0, as_stream(stream)>>>(kv);
+  return launched("kv4_reset_kernel");
 }

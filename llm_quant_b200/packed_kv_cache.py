@@ -33,7 +33,7 @@ and ``get`` may overlap each other), as any tensor that is changed in place.
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Tuple, Union
+from typing import Optional, Tuple
 
 import torch
 import torch.nn as nn
@@ -63,11 +63,9 @@ class _LayerStore:
                              self.positions.data_ptr(), self.mass.data_ptr(), self.state.data_ptr(),
                              B, H, cap, D)
         self.ref = ctypes.byref(self.c)
+        self.forms: dict = {}  # attend's arguments as the entry point takes them
 
     def clear(self) -> None:
-        self.positions.fill_(-1)
-        self.mass.zero_()
-        self.state.zero_()
         self.bound = 0
         self.captured = False
 
@@ -78,7 +76,7 @@ def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
     sb, sh, ss, sd = x.stride()
     if sd == 1 and not (sb | sh | ss) & 3 and x.data_ptr() % (4 * x.element_size()) == 0:
         return x
-    return x.clone(memory_format=torch.contiguous_format)
+    return x.detach().clone(memory_format=torch.contiguous_format)
 
 
 class PackedKVCache(nn.Module):
@@ -106,16 +104,15 @@ class PackedKVCache(nn.Module):
     @staticmethod
     def _call(st: _LayerStore, name: str, *args) -> None:
         """Call an entry point on the layer's device and its current stream."""
-        if st.device.index == torch.cuda.current_device():
-            _C.call(name, st.ref, *args, torch.cuda.current_stream(st.device).cuda_stream)
+        index = st.device.index
+        if index == torch.cuda.current_device():
+            _C.call(name, st.ref, *args, _C.raw_stream(index))
         else:
-            with torch.cuda.device(st.device):
-                _C.call(name, st.ref, *args, torch.cuda.current_stream(st.device).cuda_stream)
+            with torch.cuda.device(index):
+                _C.call(name, st.ref, *args, _C.raw_stream(index))
 
     @staticmethod
-    def _vector(x, n: int, dtype, st: _LayerStore, what: str) -> Optional[int]:
-        if x is None:
-            return None
+    def _vector(x, n: int, dtype, st: _LayerStore, what: str) -> int:
         if not isinstance(x, torch.Tensor) or x.dtype != dtype or x.shape != (n,) or x.device != st.device:
             raise ValueError(f"PackedKVCache.{what} must be a {dtype} tensor of {n} values on {st.device}")
         if not x.is_contiguous():
@@ -123,7 +120,6 @@ class PackedKVCache(nn.Module):
         return x.data_ptr()
 
     # -- writing -----------------------------------------------------------------
-    @torch.no_grad()
     def append(self, layer_idx: int, key: torch.Tensor, value: torch.Tensor,
                counts: Optional[torch.Tensor] = None) -> None:
         """Quantize and store new K, V [B, H, S, D] behind what each sequence
@@ -152,7 +148,7 @@ class PackedKVCache(nn.Module):
         elif (B, H, D) != (st.B, st.H, st.D) or key.device != st.device:
             raise RuntimeError(f"PackedKVCache.append: cache [{st.B}, {st.H}, *, {st.D}] on {st.device} vs new "
                                f"{list(key.shape)} on {key.device}")
-        c = self._vector(counts, B, torch.int32, st, "append: counts")
+        c = None if counts is None else self._vector(counts, B, torch.int32, st, "append: counts")
         if S == 0:
             return
         capturing = torch.cuda.is_current_stream_capturing()
@@ -175,7 +171,6 @@ class PackedKVCache(nn.Module):
         return self.get(layer_idx, dtype)
 
     # -- reading -----------------------------------------------------------------
-    @torch.no_grad()
     def get(self, layer_idx: int, dtype: torch.dtype = torch.float32) -> Optional[Tuple[torch.Tensor, torch.Tensor]]:
         """K, V [B, H, seq_len, D] as values in ``dtype``, zeros past a
         sequence's length, or None if the layer is empty."""
@@ -190,7 +185,6 @@ class PackedKVCache(nn.Module):
             self._call(st, "lq_kv4_dequant", st.bound, _C.TORCH_TO_LQ[dtype], k.data_ptr(), v.data_ptr())
         return k, v
 
-    @torch.no_grad()
     def attend(self, layer_idx: int, query: torch.Tensor, scale: Optional[float] = None, causal: bool = False, *,
                counts: Optional[torch.Tensor] = None, softcap: float = 0.0,
                slopes: Optional[torch.Tensor] = None, window: int = 0,
@@ -216,36 +210,55 @@ class PackedKVCache(nn.Module):
 
         Inference only: no gradient is computed."""
         st = self._layer(layer_idx, "attend")
+        q = query if query.__class__ is torch.Tensor and query.ndim == 4 else self._query(st, query)
+        # 1/8 of an octave: the work is split by it, nothing else
+        bound = st.cap if st.captured else st.bound
+        step = 1 << max(5, bound.bit_length() - 4)
+        key = (q.dtype, q.shape, q.stride(), q.device, scale, causal, softcap, window, accumulate,
+               (bound + step - 1) // step)
+        form = st.forms.get(key)
+        if form is None or q.data_ptr() & 15:
+            q = _rows(self._query(st, query), "attend")
+            form = self._form(st, q, scale, causal, softcap, window, accumulate, min(bound + step, st.cap))
+            if q.data_ptr() == query.data_ptr():
+                if len(st.forms) >= 256:
+                    st.forms.clear()
+                st.forms[key] = form
+        ref, nbytes, _ = form
+        B, Hq, Sq, D = shape = q.shape
+        cn = None if counts is None else self._vector(counts, B, torch.int32, st, "attend: counts")
+        sl = None if slopes is None else self._vector(slopes, Hq, torch.float32, st, "attend: slopes")
+        pf = None if prefix is None else self._vector(prefix, B, torch.int32, st, "attend: prefix")
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        if Sq:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+            self._call(st, "lq_kv4_attention", ref, q.data_ptr(), cn, sl, pf, out.data_ptr(), ws.data_ptr(), nbytes)
+        return out
+
+    @staticmethod
+    def _query(st: _LayerStore, query: torch.Tensor) -> torch.Tensor:
         _C.require_cuda(query, what="PackedKVCache.attend")
         _C.require_float(query, "PackedKVCache.attend")
         if query.ndim != 4 or query.shape[0] != st.B or query.shape[3] != st.D or query.shape[1] % st.H \
                 or query.shape[1] == 0 or query.device != st.device:
             raise RuntimeError(f"PackedKVCache.attend: query {list(query.shape)} on {query.device} does not match "
                                f"the cache [{st.B}, {st.H}*G, *, {st.D}] on {st.device}")
-        B, Hq, Sq, D = query.shape
+        return query
+
+    @staticmethod
+    def _form(st: _LayerStore, q: torch.Tensor, scale, causal, softcap, window, accumulate, bound):
+        """The call's arguments but for the tensors: checked once for each form."""
         if not 0.0 <= softcap < float("inf"):
             raise ValueError(f"PackedKVCache.attend: softcap {softcap} must be finite and not negative")
-        if window < 0:
+        if not 0 <= window < 2 ** 31:
             raise ValueError(f"PackedKVCache.attend: window {window} must not be negative")
-        cn = self._vector(counts, B, torch.int32, st, "attend: counts")
-        sl = self._vector(slopes, Hq, torch.float32, st, "attend: slopes")
-        pf = self._vector(prefix, B, torch.int32, st, "attend: prefix")
-        out = torch.empty((B, Hq, Sq, D), dtype=query.dtype, device=st.device)
-        if Sq == 0:
-            return out
-        q = _rows(query, "attend")
-        qs = q.stride()
-        dt = _C.TORCH_TO_LQ[q.dtype]
-        bound = st.cap if st.captured else st.bound
-        nbytes = _C.lib().lq_kv4_attention_workspace_bytes(st.ref, dt, Hq, Sq, bound, accumulate)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=st.device)
-        self._call(st, "lq_kv4_attention", q.data_ptr(), dt, Hq, Sq, qs[0], qs[1], qs[2], bound, cn,
-                   D ** -0.5 if scale is None else scale, causal, softcap, sl, window, pf, accumulate,
-                   out.data_ptr(), ws.data_ptr(), nbytes)
-        return out
+        sb, sh, ss, _ = q.stride()
+        c = _C.KV4Attn(q.shape[1], q.shape[2], sb, sh, ss, bound, window,
+                       q.shape[3] ** -0.5 if scale is None else scale, softcap, _C.TORCH_TO_LQ[q.dtype], bool(causal),
+                       bool(accumulate))
+        return ctypes.byref(c), _C.lib().lq_kv4_attention_workspace_bytes(st.ref, ctypes.byref(c)), c
 
     # -- eviction ------------------------------------------------------------------
-    @torch.no_grad()
     def evict(self, layer_idx: int, keep: int, recent: int = 0, sinks: int = 0) -> None:
         """Cut every sequence back to ``keep`` tokens per kv head: the
         ``recent`` last ones and those at positions below ``sinks`` stay, then
@@ -296,6 +309,7 @@ class PackedKVCache(nn.Module):
         for st in self._layers if layer_idx is None else [self._layers[layer_idx]]:
             if st is not None:
                 st.clear()
+                self._call(st, "lq_kv4_reset")
 
     @property
     def seq_len(self) -> int:

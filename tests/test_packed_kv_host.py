@@ -24,6 +24,14 @@ def _cache(**kw):
     return _C.KV4Cache(*[f[n] for n, _ in _C.KV4Cache._fields_])
 
 
+def _form(**kw):
+    from llm_quant_b200 import _C
+    f = dict(Hq=4, Sq=1, q_sb=64, q_sh=64, q_ss=64, bound=64, window=0, sm_scale=1.0, softcap=0.0, q_dtype=1, causal=0,
+             accumulate=0)
+    f.update(kw)
+    return ctypes.byref(_C.KV4Attn(*[f[n] for n, _ in _C.KV4Attn._fields_]))
+
+
 BAD = [({"D": 96}, "head dim"), ({"cap": 40}, "multiple"), ({"B": 0}, "shape"), ({"H": -1}, "shape"),
        ({"cap": 1 << 31}, "too large"), ({"B": 1000, "H": 1000}, "too large"), ({"params": None}, "NULL"),
        ({"state": None}, "NULL"), ({"k_codes": 4097}, "aligned"), ({"params": 4104}, "aligned")]
@@ -35,12 +43,12 @@ def test_bad_caches(lib, kw, word):
     calls = [lambda: lib.lq_kv4_append(c, 4096, 4096, 1, 1, 64, 64, 64, 64, 64, 64, None, None),
              lambda: lib.lq_kv4_dequant(c, 1, 1, 4096, 4096, None),
              lambda: lib.lq_kv4_evict(c, 4, 0, 0, 4096, 1 << 40, None),
-             lambda: lib.lq_kv4_attention(c, 4096, 1, 4, 1, 64, 64, 64, 64, None, 1.0, 0, 0.0, None, 0, None, 0,
-                                          4096, 4096, 1 << 40, None)]
+             lambda: lib.lq_kv4_reset(c, None),
+             lambda: lib.lq_kv4_attention(c, _form(), 4096, None, None, None, 4096, 4096, 1 << 40, None)]
     for call in calls:
         assert call() < 0
         assert word.encode() in lib.lq_last_error()
-    assert lib.lq_kv4_attention_workspace_bytes(c, 1, 4, 1, 64, 0) == 0
+    assert lib.lq_kv4_attention_workspace_bytes(c, _form()) == 0
 
 
 def test_bad_arguments(lib):
@@ -61,14 +69,14 @@ def test_bad_arguments(lib):
     assert lib.lq_kv4_evict(c, 64, 0, 0, None, 0, None) == 0  # nothing can be over it
     assert lib.lq_kv4_evict(c, 8, 0, 0, 4096, lib.lq_kv4_evict_workspace_bytes(2, 2, 64, 8) - 1, None) == -1
 
-    def attend(q=4096, dt=1, Hq=4, Sq=1, cap=0.0, window=0, out=4096, ws=4096, nbytes=1 << 40):
-        return lib.lq_kv4_attention(c, q, dt, Hq, Sq, 64, 64, 64, 64, None, 1.0, 0, cap, None, window, None, 0,
-                                    out, ws, nbytes, None)
+    def attend(q=4096, out=4096, ws=4096, nbytes=1 << 40, **kw):
+        return lib.lq_kv4_attention(c, _form(**kw), q, None, None, None, out, ws, nbytes, None)
 
-    assert attend(Hq=3) == -1 and attend(Hq=0) == -1 and attend(dt=3) == -2 and attend(cap=-1.0) == -1
+    assert attend(Hq=3) == -1 and attend(Hq=0) == -1 and attend(q_dtype=3) == -2 and attend(softcap=-1.0) == -1
     assert attend(q=None) == -1 and attend(out=None) == -1 and attend(window=-1) == -1 and attend(Sq=-1) == -1
-    assert attend(ws=None) == -1 and attend(ws=4100) == -5
-    need = lib.lq_kv4_attention_workspace_bytes(c, 1, 4, 1, 64, 0)
+    assert attend(ws=None) == -1 and attend(ws=4100) == -5 and attend(q=4100) == -5 and attend(q_ss=66) == -5
+    assert lib.lq_kv4_attention(c, None, 4096, None, None, None, 4096, 4096, 1 << 40, None) == -1
+    need = lib.lq_kv4_attention_workspace_bytes(c, _form())
     assert need > 0 and attend(nbytes=need - 1) == -1
     assert attend(Sq=0) == 0
 
