@@ -28,9 +28,6 @@
 #include "lq_common.cuh"
 
 namespace lq {
-namespace {
-
-constexpr int kUnit = 32;  // tokens that a warp takes at a time (two tiles of 16)
 
 struct Kv4 {
   uint8_t* k;
@@ -43,6 +40,10 @@ struct Kv4 {
   int32_t* sync;  // [0] ticket of the running call, [1] tokens dropped for want of room, [2] something was evicted, [3] a wait on the device ran out
   int B, H, cap, D;
 };
+
+namespace {
+
+constexpr int kUnit = 32;  // tokens that a warp takes at a time (two tiles of 16)
 
 inline Kv4 kv4_of(const lq_kv4_cache* c) {
   Kv4 k;

@@ -32,53 +32,13 @@
 // kv4_combine_kernel, a programmatic dependent launch.
 #include <algorithm>
 
-#include "lq_kv4.cuh"
+#include "lq_kv4_attn.cuh"
 #include "lq_tma.cuh"
 
 namespace lq {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr float kLog2e = 1.4426950408889634f;
-
-struct Attn {
-  Kv4 kv;
-  const uint8_t* q;
-  int q_dtype;
-  int64_t q_sb, q_sh, q_ss;
-  int Hq, G, Sq, rows, rows_pad;
-  const int32_t* counts;
-  float sm, cap;  // softmax scale; cap 0: none
-  const float* slopes;
-  const int32_t* prefix;
-  int causal, window;
-  int blocks;     // blocks of the split (at most; never more than there are units)
-  uint8_t* out;
-  float* part;    // [blocks + B H][rows_pad][D] unnormalised O
-  float2* ml;     // [blocks + B H][rows_pad] running maximum and sum
-  float* lse;     // [B H][rows_pad] log2 of the softmax denominators (weights collected), or NULL
-};
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float lg2(float x) {
-  float y;
-  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// tanh from the exponential: the error is about 2^-23 absolute, which is what a
-// capped score needs (tanh.approx is only good to 2^-11)
-__device__ __forceinline__ float tanh_exp(float x) {
-  return 1.0f - __fdividef(2.0f, 1.0f + ex2(2.0f * kLog2e * x));
-}
-__device__ __forceinline__ uint32_t h2(float lo, float hi) {
-  __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&h);
-}
-__device__ __forceinline__ float2 f2(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
 __device__ __forceinline__ void mma16(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                       uint32_t b1) {
   asm volatile(
@@ -92,28 +52,6 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
-__device__ __forceinline__ void st_out(uint8_t* p, int64_t i, int dt, float v) {
-  if (dt == LQ_F32) reinterpret_cast<float*>(p)[i] = v;
-  else if (dt == LQ_F16) reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
-  else reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
-}
-
-__device__ __forceinline__ void st_out4(uint8_t* p, int64_t i, int dt, float4 v, float f) {
-  if (dt == LQ_F32) {
-    *reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + i) = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
-  } else if (dt == LQ_F16) {
-    *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(p) + i) = make_uint2(h2(v.x * f, v.y * f), h2(v.z * f, v.w * f));
-  } else {
-    union {
-      __nv_bfloat162 b[2];
-      uint2 u;
-    } r;
-    r.b[0] = __floats2bfloat162_rn(v.x * f, v.y * f);
-    r.b[1] = __floats2bfloat162_rn(v.z * f, v.w * f);
-    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p) + i) = r.u;
-  }
-}
-
 // Fragment registers from a word of codes: nibble n of both halves as f16.
 // The tensor cores align a subnormal's product by the exponent 2^-14 it would
 // have as a normal number, and cut below 24 bits: a code whose unit is 2^(b -
@@ -138,8 +76,6 @@ struct Nibbles {
     }
   }
 };
-constexpr float pow2(int e) { return e < 0 ? 1.0f / (float)(1u << -e) : (float)(1u << e); }
-
 // W aligned words (16 or 8 bytes) of codes
 template <int W>
 __device__ __forceinline__ void ld_codes(const uint8_t* p, uint32_t* w) {
@@ -152,60 +88,6 @@ __device__ __forceinline__ void ld_codes(const uint8_t* p, uint32_t* w) {
   }
 }
 
-// New queries of sequence b, and the units that they may see: units [0, pre)
-// and [pre + gap, pre + gap + ...), `count` in all.  Slots are positions when
-// nothing was evicted (ordered); only then can a window leave units out.
-struct Seq {
-  int n, cnt, first;  // tokens held, new queries, position of the first of them
-  int pre, gap, count;
-  int ordered;        // nothing was evicted: slots are positions
-};
-__device__ __forceinline__ Seq seq_of(const Attn& a, int b) {
-  Seq s;
-  s.n = min(a.kv.len[b], a.kv.cap);
-  s.cnt = a.counts ? min(max(a.counts[b], 0), a.Sq) : a.Sq;
-  s.first = a.kv.next[b] - s.cnt;
-  s.ordered = a.kv.sync[2] == 0;
-  s.pre = s.gap = 0;
-  s.count = s.cnt > 0 ? (s.n + kUnit - 1) / kUnit : 0;
-  if (a.window > 0 && s.ordered && s.count > 0) {
-    const int lo = min(max(s.first - a.window + 1, 0) / kUnit, s.count - 1);
-    const int pre = a.prefix ? min(max(a.prefix[b], 0), s.n) : 0;
-    s.pre = min((pre + kUnit - 1) / kUnit, lo);
-    s.gap = lo - s.pre;
-    s.count -= s.gap;
-  }
-  return s;
-}
-
-// The row of all heads' units, cut into equal stretches.  (A unit takes 32 D
-// bytes, so that their number fits an int on any GPU.)
-struct Cut {
-  int units, blocks, base, rem;
-  __device__ __forceinline__ void set(int u, int most) {
-    units = u;
-    blocks = max(min(u, most), 1);
-    base = units / blocks;
-    rem = units % blocks;
-  }
-  // units * cta / blocks, and the block that unit x falls to
-  __device__ __forceinline__ int begin(int cta) const { return cta * base + cta * rem / blocks; }
-  __device__ __forceinline__ int owner(int x) const { return (int)(((int64_t)(x + 1) * blocks - 1) / units); }
-};
-__device__ __forceinline__ int warp_sum(int u) {
-#pragma unroll
-  for (int m = 16; m > 0; m >>= 1) u += __shfl_xor_sync(0xffffffffu, u, m);
-  return u;
-}
-__device__ __forceinline__ int warp_scan(int u) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, u, d);
-    if (lane >= d) u += y;
-  }
-  return u;
-}
 // Units of the sequences before b, and of all; every warp computes it for itself.
 __device__ __forceinline__ int units_before(const Attn& a, int b, int& all) {
   int before = 0, sum = 0;
@@ -244,23 +126,6 @@ struct RowsShared {
   uint4 lo[QLO ? 8 * NQ : 1][QLO ? NW : 1];
   float sum[8 * NQ], fac[8 * NQ];
 };
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float* x) {  // p on a multiple of 4 elements
-  if constexpr (sizeof(T) == 4) {
-    const float4 u = __ldg(reinterpret_cast<const float4*>(p)), v = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
-  } else {
-    union {
-      uint2 u[2];
-      T t[8];
-    } v;
-    v.u[0] = __ldg(reinterpret_cast<const uint2*>(p));
-    v.u[1] = __ldg(reinterpret_cast<const uint2*>(p) + 1);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = Ty<T>::to_f(v.t[i]);
-  }
-}
-
 template <int D, int NQ, bool QLO>
 struct Rows {
   static constexpr int W = D / 32, NW = D / 8;
@@ -401,12 +266,6 @@ __device__ __forceinline__ void load_pos(const Attn& a, int64_t row, const int* 
 #pragma unroll
   for (int j = 0; j < N; ++j) pos[j] = s.ordered || tok[j] >= s.n ? tok[j] : a.kv.pos[row + tok[j]];
 }
-
-// P is kept up to 2^kHead above 1 and scaled by 2^kHead: the running reference
-// of a row is raised only when a probability would pass 2^(2 kHead - 0.1), so
-// most units need no maximum across lanes and no rescaling.
-constexpr float kHead = 8.0f, kTop = 15.9f;
-constexpr float kNone = -1e30f;  // reference of a row that has seen nothing
 
 // Shared memory of a block: each warp has a ring of its own of kStages units,
 // filled by bulk copies that one lane issues, so that a unit's bytes are on
@@ -818,9 +677,20 @@ __global__ void __launch_bounds__(128) kv4_mass_kernel(const Attn a) {
 // all row blocks, and at least one unit per warp.
 struct Plan {
   int nq, row_blocks, rows_pad, blocks;
+  int64_t slots;  // partial results, of rows_pad (prompt: kPromptRows) rows each
+  bool prompt;    // lq_kv4_prompt.cu's
 };
+constexpr int kFewRows = 16;  // up to here a row of the cache is read once by this file's kernel
 Plan plan_of(const Kv4& kv, int64_t rows, int64_t bound, bool qlo) {
   Plan p;
+  p.prompt = !qlo && rows > kFewRows;
+  if (p.prompt) {
+    p.nq = p.row_blocks = 0;
+    p.rows_pad = (int)((rows + kPromptRows - 1) / kPromptRows * kPromptRows);
+    p.blocks = num_sms();
+    p.slots = 2 * p.blocks;
+    return p;
+  }
   p.nq = rows <= 8 ? 1 : 2;
   p.row_blocks = (int)((rows + 8 * p.nq - 1) / (8 * p.nq));
   p.rows_pad = p.row_blocks * 8 * p.nq;
@@ -831,15 +701,22 @@ Plan plan_of(const Kv4& kv, int64_t rows, int64_t bound, bool qlo) {
   const int64_t heads = (int64_t)kv.B * kv.H;
   if (slots >= heads && slots % heads * 10 <= slots) slots -= slots % heads;
   p.blocks = (int)std::max<int64_t>(1, std::min<int64_t>(slots, (units + kWarps - 1) / kWarps));
+  p.slots = p.blocks + heads;
   return p;
 }
 
 // part, ml, lse
 void spaces(const Kv4& kv, const Plan& p, bool weigh, size_t* bytes) {
-  const size_t slots = (size_t)(p.blocks + kv.B * kv.H) * p.rows_pad;
-  bytes[0] = slots * kv.D * sizeof(float);
-  bytes[1] = slots * sizeof(float2);
+  const size_t rows = (size_t)p.slots * (p.prompt ? kPromptRows : p.rows_pad);
+  bytes[0] = rows * kv.D * sizeof(float);
+  bytes[1] = rows * sizeof(float2);
   bytes[2] = weigh ? (size_t)kv.B * kv.H * p.rows_pad * sizeof(float) : 0;
+}
+
+template <int D, bool QLO, bool GEN>
+int run_mass(const Attn& a, cudaStream_t st) {
+  kv4_mass_kernel<D, QLO, GEN><<<dim3((a.kv.cap + 63) / 64, a.kv.B * a.kv.H), 128, 0, st>>>(a);
+  return launched("kv4_mass_kernel");
 }
 
 template <int D, int NQ, bool QLO, bool GEN>
@@ -852,11 +729,7 @@ int run_attn(const Attn& a, const Plan& p, cudaStream_t st) {
   LQ_TRY(launched("kv4_attn_kernel"));
   launch_pdl(kv4_combine_kernel, dim3((unsigned)(((int64_t)a.rows * a.kv.B * a.kv.H + 3) / 4)), dim3(128), 0, st, a);
   LQ_TRY(launched("kv4_combine_kernel"));
-  if (a.lse) {
-    kv4_mass_kernel<D, QLO, GEN><<<dim3((a.kv.cap + 63) / 64, a.kv.B * a.kv.H), 128, 0, st>>>(a);
-    LQ_TRY(launched("kv4_mass_kernel"));
-  }
-  return LQ_OK;
+  return a.lse ? run_mass<D, QLO, GEN>(a, st) : LQ_OK;
 }
 template <int D, bool QLO, bool GEN>
 int run_attn_nq(const Attn& a, const Plan& p, cudaStream_t st) {
@@ -924,5 +797,11 @@ extern "C" int lq_kv4_attention(const lq_kv4_cache* cache, const lq_kv4_attn* f,
   // a single query sees every token but for a window, a bias or a cap
   const bool gen = (f->Sq > 1 && (f->causal || counts)) || f->softcap > 0.0f || slopes || f->window > 0;
   cudaStream_t st = as_stream(stream);
+  if (p.prompt) {
+    LQ_TRY(kv4_prompt(a, st));
+    if (!a.lse) return LQ_OK;
+    if (kv.D == 128) return gen ? run_mass<128, false, true>(a, st) : run_mass<128, false, false>(a, st);
+    return gen ? run_mass<64, false, true>(a, st) : run_mass<64, false, false>(a, st);
+  }
   return kv.D == 128 ? run_attn_d<128>(a, p, gen, st) : run_attn_d<64>(a, p, gen, st);
 }

@@ -1,0 +1,696 @@
+// lq_kv4_prompt.cu -- attention over the 4-bit KV cache for many query rows
+// (chunks of a prompt), on the 5th-generation tensor cores.  Formulas and
+// layouts: lq_kv4.cuh, lq_kv4_attn.cuh.
+//
+// A block works on 256 rows of one kv head (two tiles of 128; row r = i G +
+// head of the group) and goes over the cached tokens in tiles of 128:
+//   S = Q (C_k - Z_k)^T      kind::f16, Q and the bare integers of K in Q's type;
+//   O += P' (C_v - Z_v)      kind::f16 in f16, P' from tensor memory.
+// Code minus zero point is an integer of 5 bits, exact in either type, so the
+// products are exact; the scales stay in fp32 outside: K's times the softmax
+// scale multiplies a column of S, V's goes into P'.  P' = 2^(x + e - R + 8) sv /
+// 2^e with R the row's running reference and e the exponent of the tile's
+// largest sv: it fits f16 whatever the scales, and takes one exponential.  R is
+// raised only when an exponent passes 15.9 (then the row's O in tensor memory is
+// rescaled by the softmax threads themselves; it happens in the first tiles).
+//
+// Warps: 0-3 and 4-7 softmax of the two row tiles (a thread owns a row), 8-11
+// turn packed codes into the two operands in shared memory (swizzled, two
+// stages), 12 issues the MMAs.  Tensor memory: S0, S1 (P' lies over S), O0, O1.
+// The MMAs of one row tile run while the softmax of the other does.
+//
+// Bound: per 128 x 128 tile of scores the tensor cores need 1024 cycles (D =
+// 128) and the 16384 exponentials 1024 on the SM's special-function units; the
+// softmax is written with packed fp32 pairs (f32x2) so that its instructions
+// stay below that.
+//
+// Split: as in lq_kv4_attn.cu, the (row tile, token tile) pairs that have
+// anything to see lie in one row and each block takes an equal stretch;
+// kv4_prompt_combine_kernel merges row tiles that were cut.
+#include "lq_kv4_attn.cuh"
+#include "lq_tc.cuh"
+
+namespace lq {
+namespace {
+
+constexpr int kTok = 128;    // tokens of a tile
+constexpr int kTile = 128;   // rows of a tile
+constexpr int kItem = kPromptRows;  // rows of an item
+constexpr int kSoftmaxWarps = 8, kCodeWarps = 4;
+constexpr int kPromptThreads = 32 * (kSoftmaxWarps + kCodeWarps + 1);
+constexpr int kScaleStages = 4;
+
+// The token tiles that the rows of an item may see: tiles [0, pre) and [pre +
+// gap, ...), `count` in all.
+struct Tiles {
+  int n, cnt, first, ordered;
+  int pre, gap, count;
+};
+__device__ __forceinline__ Tiles tiles_of(const Attn& a, int b, int rt) {
+  const Seq s = seq_of(a, b);
+  Tiles t{s.n, s.cnt, s.first, s.ordered, 0, 0, 0};
+  const int i0 = rt * kItem / a.G, i1 = min((rt * kItem + kItem - 1) / a.G, s.cnt - 1);
+  if (i0 >= s.cnt || s.n == 0) return t;
+  int lo = 0, hi = s.n, pre = 0;
+  if (s.ordered) {
+    if (a.causal) hi = max(min(s.n, s.first + i1 + 1), 0);
+    if (a.window > 0) lo = min(max(s.first + i0 - a.window + 1, 0), hi);
+    if (a.prefix) pre = min(max(a.prefix[b], 0), s.n);
+  }
+  const int lo_t = lo / kTok, hi_t = hi > lo ? (hi + kTok - 1) / kTok : lo_t;
+  t.pre = (pre + kTok - 1) / kTok;
+  if (t.pre >= lo_t) {
+    t.pre = max(t.pre, hi_t);
+    t.count = t.pre;
+  } else {
+    t.gap = lo_t - t.pre;
+    t.count = t.pre + hi_t - lo_t;
+  }
+  return t;
+}
+
+// A block's way through the items (sequence, row tile, head) that its stretch
+// covers; every warp goes it for itself.
+struct Walk {
+  int x0, x1, j, h, u0, u1;
+  Tiles t;
+  __device__ __forceinline__ void piece() { u1 = min(t.count, u0 + (x1 - x0)); }
+  __device__ __forceinline__ bool next(const Attn& a) {  // to the next piece; false: done
+    const int rts = a.rows_pad / kItem;
+    x0 += u1 - u0;
+    if (x0 >= x1) return false;
+    ++h;
+    while (h == a.kv.H || t.count == 0) {
+      h = 0;
+      ++j;
+      t = tiles_of(a, j / rts, j % rts);
+    }
+    u0 = 0;
+    piece();
+    return true;
+  }
+};
+// Units of all items, and of those before item group j (a sequence's row tile, all heads).
+__device__ __forceinline__ int tiles_before(const Attn& a, int j, int& all) {
+  const int rts = a.rows_pad / kItem;
+  int before = 0, sum = 0;
+  for (int i = threadIdx.x & 31; i < a.kv.B * rts; i += 32) {
+    const int u = tiles_of(a, i / rts, i % rts).count;
+    sum += u;
+    if (i < j) before += u;
+  }
+  all = warp_sum(sum) * a.kv.H;
+  return warp_sum(before) * a.kv.H;
+}
+__device__ __forceinline__ bool walk_begin(const Attn& a, int cta, Walk& w) {
+  const int rts = a.rows_pad / kItem, lane = threadIdx.x & 31;
+  int all;
+  tiles_before(a, 0, all);
+  Cut cut;
+  cut.set(all, a.blocks);
+  if (all == 0 || cta >= cut.blocks) return false;
+  w.x0 = cut.begin(cta);
+  w.x1 = cut.begin(cta + 1);
+  int begin = 0;
+  for (int j0 = 0;; j0 += 32) {
+    const int own = j0 + lane < a.kv.B * rts ? tiles_of(a, (j0 + lane) / rts, (j0 + lane) % rts).count * a.kv.H : 0;
+    const int inc = warp_scan(own);
+    const uint32_t hit = __ballot_sync(0xffffffffu, begin + inc > w.x0);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      begin += __shfl_sync(0xffffffffu, inc - own, src);
+      w.j = j0 + src;
+      break;
+    }
+    begin += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  w.t = tiles_of(a, w.j / rts, w.j % rts);
+  w.h = (w.x0 - begin) / w.t.count;
+  w.u0 = (w.x0 - begin) % w.t.count;
+  w.piece();
+  return true;
+}
+__device__ __forceinline__ int tile_token(const Tiles& t, int u) { return (u < t.pre ? u : u + t.gap) * kTok; }
+
+template <int D>
+struct PromptShared {
+  static constexpr int kHalves = D / 64;             // 64-wide halves of the head dim
+  static constexpr int kQ = 2 * kHalves * 16384;     // [row tile][half][128 rows][128 bytes]
+  static constexpr int kK = kHalves * 16384;         // a stage: [half][128 tokens][128 bytes]
+  static constexpr int kV = 2 * D * 128;             // a stage: [token half][D values][128 bytes]
+  static constexpr int off_q = 0, off_k = kQ, off_v = off_k + 2 * kK, off_s = off_v + 2 * kV;
+  struct Scales {
+    float sk[kScaleStages][kTok], sv[kScaleStages][kTok];
+    int pos[kScaleStages][kTok];
+    float e[kScaleStages];
+    uint32_t zv[2][kTok / 2];   // V zero points as f16 pairs, biased
+    float top[2][kCodeWarps];
+    uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], t_full[2], s_full[2], p_full[2], o_full[2], drain;
+    uint32_t tmem;
+    int fail;
+  };
+  static constexpr int bytes = off_s + (int)sizeof(Scales) + 1024;  // and room to align
+};
+
+__device__ __forceinline__ void tc_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
+  tmem_st16(addr, r);
+  tmem_st16(addr + 16, r + 16);
+}
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t p) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// Integers of 4 bits as operands: bias + code is exact in the type, and so is
+// its difference from bias + zero point.
+template <typename T> struct Ints;
+template <> struct Ints<__half> {
+  static constexpr uint32_t bias = 0x64006400u;  // 1024
+  static constexpr int fmt = 0;
+  __device__ __forceinline__ static uint32_t sub(uint32_t x, uint32_t z) {
+    __half2 h = __hsub2(*reinterpret_cast<__half2*>(&x), *reinterpret_cast<__half2*>(&z));
+    return *reinterpret_cast<uint32_t*>(&h);
+  }
+};
+template <> struct Ints<__nv_bfloat16> {
+  static constexpr uint32_t bias = 0x43004300u;  // 128
+  static constexpr int fmt = 1;
+  __device__ __forceinline__ static uint32_t sub(uint32_t x, uint32_t z) {
+    __nv_bfloat162 h = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&x), *reinterpret_cast<__nv_bfloat162*>(&z));
+    return *reinterpret_cast<uint32_t*>(&h);
+  }
+};
+// The 8 values of a word: pairs (0, 4), (1, 5), (2, 6), (3, 7) less their zero points z.
+template <typename T>
+__device__ __forceinline__ void ints_of(uint32_t w, uint32_t z, uint32_t* r) {
+#pragma unroll
+  for (int n = 0; n < 4; ++n) r[n] = Ints<T>::sub(((w >> (4 * n)) & 0x000f000fu) | Ints<T>::bias, z);
+}
+
+// A tile of 128 query rows into shared memory as a K-major, 128-byte-swizzled
+// operand, the 8 values of a chunk in the order of ints_of.  128 threads.
+template <typename T, int D>
+__device__ __forceinline__ void stage_rows(uint8_t* dst, const Attn& a, int b, int h, int cnt, int r0, int tid) {
+  constexpr int CH = D / 8;
+  for (int idx = tid; idx < kTile * CH; idx += 128) {
+    const int lr = idx / CH, c = idx % CH, r = r0 + lr, i = r / a.G;
+    uint2 u = make_uint2(0u, 0u), v = u;
+    if (r < a.rows && i < cnt) {
+      const T* p = reinterpret_cast<const T*>(a.q) + b * a.q_sb + (int64_t)(h * a.G + r % a.G) * a.q_sh + i * a.q_ss + 8 * c;
+      u = __ldg(reinterpret_cast<const uint2*>(p));
+      v = __ldg(reinterpret_cast<const uint2*>(p) + 1);
+    }
+    const uint4 w = make_uint4(__byte_perm(u.x, v.x, 0x5410), __byte_perm(u.x, v.x, 0x7632),
+                               __byte_perm(u.y, v.y, 0x5410), __byte_perm(u.y, v.y, 0x7632));
+    *reinterpret_cast<uint4*>(dst + (c / 8) * 16384 + lr * 128 + (((c % 8) ^ (lr & 7)) << 4)) = w;
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Attn a) {
+  using L = PromptShared<D>;
+  constexpr int W = D / 32;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  typename L::Scales& sc = *reinterpret_cast<typename L::Scales*>(smem + L::off_s);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  Walk w;
+  if (!walk_begin(a, blockIdx.x, w)) return;
+  if (threadIdx.x == 0) {
+    sc.fail = 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sc.q_full[i], kTile);
+      mbar_init(&sc.k_full[i], kCodeWarps);
+      mbar_init(&sc.k_empty[i], 1);
+      mbar_init(&sc.v_full[i], kCodeWarps);
+      mbar_init(&sc.t_full[i], kCodeWarps);
+      mbar_init(&sc.v_empty[i], 1);
+      mbar_init(&sc.s_full[i], 1);
+      mbar_init(&sc.p_full[i], 4);
+      mbar_init(&sc.o_full[i], 1);
+    }
+    mbar_init(&sc.drain, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == kSoftmaxWarps + kCodeWarps) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sc.tmem)), "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sc.tmem;
+  // A wait that runs out (2 s) ends the block: every role leaves its loop, as
+  // every wait, this one's aside, is bounded too.  Whole warps agree on it.
+  volatile int* fail = &sc.fail;
+  auto gone = [&] { return __any_sync(0xffffffffu, *fail != 0); };
+  const int rts = a.rows_pad / kItem;
+
+  if (warp < kSoftmaxWarps) {
+    // ---------------- softmax: a thread owns a row of its tile ----------------
+    const int wg = warp >> 2, tid = threadIdx.x & 127;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t S = tmem + lanes + wg * 128, O = tmem + lanes + 256 + wg * 128;
+    int unit = 0, mine = 0;  // units of this block so far, and those of them that this tile had rows in
+    int items = 0;           // items that this tile had rows in
+    bool first_piece = true;
+    do {
+      const int b = w.j / rts, rt = w.j % rts;
+      const int r = rt * kItem + wg * kTile + tid, i = r / a.G;
+      const bool valid = r < a.rows && i < w.t.cnt;
+      const int at = w.t.first + i;
+      const bool active = rt * kItem + wg * kTile < a.rows;
+      if (!active) {
+        unit += w.u1 - w.u0;
+        first_piece = false;
+        continue;
+      }
+      stage_rows<T, D>(smem + L::off_q + wg * (L::kQ / 2), a, b, w.h, w.t.cnt, rt * kItem + wg * kTile, tid);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      mbar_arrive(&sc.q_full[wg]);
+      const float slope = a.slopes && r < a.rows ? a.slopes[w.h * a.G + r % a.G] * kLog2e : 0.0f;
+      const int pre = a.prefix ? a.prefix[b] : 0;
+      // positions of the tile's first and last row
+      const int qa = w.t.first + (rt * kItem + wg * kTile) / a.G, qb = w.t.first + (rt * kItem + wg * kTile + kTile - 1) / a.G;
+      float R = kNone, l = 0.0f;
+      for (int u = w.u0; u < w.u1; ++u, ++unit, ++mine) {
+        if (!mbar_wait_warp(&sc.s_full[wg], mine & 1)) *fail = 1;
+        if (gone()) break;
+        tc_fence_after();
+        const int t0 = tile_token(w.t, u), st = unit % kScaleStages;
+        const float* sk = sc.sk[st];
+        const float* sv = sc.sv[st];
+        const float e = sc.e[st];
+        const bool plain = a.cap == 0.0f && !a.slopes && t0 + kTok <= w.t.n &&
+                           ((!a.causal && a.window <= 0) ||
+                            (w.t.ordered && (!a.causal || t0 + kTok - 1 <= qa) && (a.window <= 0 || qb - t0 < a.window)));
+        // score (log2 units) of column c from its product, with cap, bias and masks
+        auto score = [&](float s, int c) {
+          float x = s * sk[c];
+          if (a.cap > 0.0f) x = tanh_exp(x) * (a.cap * kLog2e);
+          const int pos = w.t.ordered ? t0 + c : sc.pos[st][c], back = at - pos;
+          if (a.slopes) x = fmaf(-slope, fabsf((float)back), x);
+          bool near = true;
+          if (a.causal) near = back >= 0;
+          if (a.window > 0) near = near && back < a.window;
+          return valid && t0 + c < w.t.n && (near || pos < pre) ? x : -INFINITY;
+        };
+        uint32_t p[64];
+        float sum, top;
+        auto pass = [&] {
+          const float off = e + kHead - R;
+          top = -INFINITY;
+          if (plain) {
+            const uint64_t off2 = pair(off, off);
+            uint64_t s2 = pair(0.0f, 0.0f);
+#pragma unroll
+            for (int c = 0; c < kTok; c += 32) {
+              uint32_t x[32];
+              tmem_ld32(S + c, x);
+              tmem_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 32; k += 4) {
+                const float4 f = *reinterpret_cast<const float4*>(sk + c + k), v = *reinterpret_cast<const float4*>(sv + c + k);
+                const float2 y0 = unpair(fma2(pair(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), pair(f.x, f.y), off2));
+                const float2 y1 = unpair(fma2(pair(__uint_as_float(x[k + 2]), __uint_as_float(x[k + 3])), pair(f.z, f.w), off2));
+                top = fmaxf(fmaxf(top, fmaxf(y0.x, y0.y)), fmaxf(y1.x, y1.y));
+                const uint64_t q0 = pair(ex2(y0.x), ex2(y0.y)), q1 = pair(ex2(y1.x), ex2(y1.y));
+                s2 = add2(s2, add2(q0, q1));
+                const float2 p0 = unpair(mul2(q0, pair(v.x, v.y))), p1 = unpair(mul2(q1, pair(v.z, v.w)));
+                p[(c + k) / 2] = h2(p0.x, p0.y);
+                p[(c + k) / 2 + 1] = h2(p1.x, p1.y);
+              }
+            }
+            const float2 s = unpair(s2);
+            sum = s.x + s.y;
+          } else {
+            sum = 0.0f;
+#pragma unroll
+            for (int c = 0; c < kTok; c += 32) {
+              uint32_t x[32];
+              tmem_ld32(S + c, x);
+              tmem_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 32; k += 2) {
+                float y[2];
+#pragma unroll
+                for (int d = 0; d < 2; ++d) {
+                  const float v = score(__uint_as_float(x[k + d]), c + k + d), q = ex2(v + off);
+                  top = fmaxf(top, v + off);
+                  sum += q;
+                  y[d] = v == -INFINITY ? 0.0f : q * sv[c + k + d];  // whatever the scale of a token that is not seen
+                }
+                p[(c + k) / 2] = h2(y[0], y[1]);
+              }
+            }
+          }
+        };
+        bool redo = u == w.u0;
+        if (!redo) {
+          pass();
+          redo = __any_sync(0xffffffffu, top > kTop);
+        }
+        if (redo) {
+          float m = kNone;
+#pragma unroll 1
+          for (int c = 0; c < kTok; c += 32) {
+            uint32_t x[32];
+            tmem_ld32(S + c, x);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              m = fmaxf(m, plain ? __uint_as_float(x[k]) * sk[c + k] : score(__uint_as_float(x[k]), c + k));
+          }
+          m = fmaxf(R, m == kNone ? kNone : m + e);
+          const float alpha = ex2(R - m);
+          l *= alpha;
+          R = m;
+          if (u > w.u0) {  // the last PV is complete: its successor's S is
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              uint32_t x[32];
+              tmem_ld32(O + c, x);
+              tmem_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) * alpha);
+              tmem_st32(O + c, x);
+            }
+          }
+          pass();
+        }
+        l = fmaf(sum, ex2(-e - kHead), l);
+        tmem_st32(S, p);
+        tmem_st32(S + 32, p + 32);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sc.p_full[wg]);
+      }
+      if (gone()) break;
+      // ---- the item's rows, or this block's part of them ----
+      if (!mbar_wait_warp(&sc.o_full[wg], items & 1)) {
+        *fail = 1;
+        break;
+      }
+      ++items;
+      tc_fence_after();
+      const bool whole = w.u0 == 0 && w.u1 == w.t.count;
+      if (whole) {
+        const float inv = !valid || l == 0.0f ? 0.0f : pow2(-(int)kHead) / l;
+        T* out = reinterpret_cast<T*>(a.out) + (((int64_t)b * a.Hq + w.h * a.G + r % a.G) * a.Sq + i) * D;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t x[32];
+          tmem_ld32(O + c, x);
+          tmem_wait_ld();
+          if (r < a.rows) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 8) {
+              union {
+                T t[8];
+                uint4 v;
+              } y;
+#pragma unroll
+              for (int d = 0; d < 8; ++d) y.t[d] = Ty<T>::from_f(valid ? __uint_as_float(x[k + d]) * inv : 0.0f);
+              st_v4(out + c + k, y.v);
+            }
+          }
+        }
+        if (a.lse && r < a.rows)
+          a.lse[(int64_t)(b * a.kv.H + w.h) * a.rows_pad + r] = !valid || l == 0.0f ? INFINITY : R + lg2(l);
+      } else {
+        const int64_t row = (int64_t)(2 * blockIdx.x + (first_piece ? 0 : 1)) * kItem + wg * kTile + tid;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t x[32];
+          tmem_ld32(O + c, x);
+          tmem_wait_ld();
+          if (r < a.rows) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 4)
+              *reinterpret_cast<float4*>(a.part + row * D + c + k) =
+                  make_float4(__uint_as_float(x[k]), __uint_as_float(x[k + 1]), __uint_as_float(x[k + 2]), __uint_as_float(x[k + 3]));
+          }
+        }
+        if (r < a.rows) a.ml[row] = make_float2(R, valid ? l : 0.0f);
+      }
+      tc_fence_before();
+      first_piece = false;
+    } while (w.next(a));
+  } else if (warp < kSoftmaxWarps + kCodeWarps) {
+    // ---------------- codes to operands ----------------
+    const int tid = threadIdx.x - 32 * kSoftmaxWarps, cw = warp - kSoftmaxWarps;
+    const int g = tid >> 4, tg = tid & 15;  // V: 16 values (units g W ..) of 8 tokens
+    const float fk = a.sm * (a.cap > 0.0f ? 1.0f / a.cap : kLog2e);
+    uint32_t kr[2 * W][2], vr[4][W];
+    uint2 par = make_uint2(0u, 0u);
+    int unit = 0;
+    auto fetch = [&](const Walk& x, int u) {
+      const int t0 = tile_token(x.t, u), t = t0 + tid, tv = t0 + 8 * tg;
+      const int64_t row = (int64_t)(x.j / rts * a.kv.H + x.h) * a.kv.cap;
+      par = make_uint2(0u, 0u);
+      if (t < x.t.n) {
+        const uint2* p = reinterpret_cast<const uint2*>(a.kv.k + (row + t) * (D / 2));
+#pragma unroll
+        for (int i = 0; i < 2 * W; ++i) {
+          const uint2 v = __ldg(p + i);
+          kr[i][0] = v.x, kr[i][1] = v.y;
+        }
+        par = __ldg(a.kv.par + row + t);
+      }
+      if (tv < x.t.n) {
+        const uint8_t* p = a.kv.v + row * (D / 2) + (int64_t)(tv >> 4) * (W * 256) + ((tv >> 3) & 1) * (W * 128) + g * (W * 16);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < W; i += 2) {
+            const uint2 v = __ldg(reinterpret_cast<const uint2*>(p + c * (W * 4) + i * 4));
+            vr[c][i] = v.x, vr[c][i + 1] = v.y;
+          }
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < 2 * W; ++i) kr[i][0] = kr[i][1] = 0u;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int i = 0; i < W; ++i) vr[c][i] = 0u;
+    fetch(w, w.u0);
+    bool more = true;
+    int u = w.u0;
+    while (more) {
+      const int s2 = unit & 1, st = unit % kScaleStages, t0 = tile_token(w.t, u);
+      // where the next unit is
+      Walk nx = w;
+      int nu = u + 1;
+      if (nu >= w.u1) {
+        more = nx.next(a);
+        nu = nx.u0;
+      }
+      if (unit >= 2 && !mbar_wait_warp(&sc.k_empty[s2], ((unit >> 1) - 1) & 1)) *fail = 1;
+      if (gone()) break;
+      // ---- K, and the columns' scales ----
+      const uint32_t zk = (uint32_t)(int)par_zero(par.x) * 0x10001u + Ints<T>::bias;
+      uint8_t* kd = smem + L::off_k + s2 * L::kK + tid * 128;
+#pragma unroll
+      for (int i = 0; i < 4 * W; ++i) {
+        uint32_t r[4];
+        ints_of<T>(kr[i >> 1][i & 1], zk, r);
+        *reinterpret_cast<uint4*>(kd + (i / 8) * 16384 + (((i % 8) ^ (tid & 7)) << 4)) = make_uint4(r[0], r[1], r[2], r[3]);
+      }
+      const float sv = par_scale(par.y);
+      // a NaN scale (its token reads as NaN) is kept out of the tile's exponent
+      const uint32_t top = __reduce_max_sync(0xffffffffu, sv < INFINITY ? __float_as_uint(sv) : 0u);
+      if (lane == 0) sc.top[s2][cw] = __uint_as_float(top);
+      reinterpret_cast<uint16_t*>(sc.zv[s2])[tid] = (uint16_t)((uint32_t)(int)par_zero(par.y) + 0x6400u);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sc.t_full[s2]);
+      if (!mbar_wait_warp(&sc.t_full[s2], (unit >> 1) & 1)) *fail = 1;
+      if (gone()) break;
+      const float big = fmaxf(fmaxf(sc.top[s2][0], sc.top[s2][1]), fmaxf(sc.top[s2][2], sc.top[s2][3]));
+      const int e = big > 0.0f ? (int)(__float_as_uint(big) >> 23) - 126 : 0;  // big < 2^e
+      sc.sk[st][tid] = par_scale(par.x) * fk;
+      sc.sv[st][tid] = sv * __uint_as_float((uint32_t)(127 - e) << 23);
+      if (!w.t.ordered)
+        sc.pos[st][tid] = t0 + tid < w.t.n ? a.kv.pos[(int64_t)(w.j / rts * a.kv.H + w.h) * a.kv.cap + t0 + tid] : 0;
+      if (tid == 0) sc.e[st] = (float)e;
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sc.k_full[s2]);
+      // ---- V^T ----
+      if (unit >= 2 && !mbar_wait_warp(&sc.v_empty[s2], ((unit >> 1) - 1) & 1)) *fail = 1;
+      if (gone()) break;
+      const uint4 z = *reinterpret_cast<const uint4*>(&sc.zv[s2][4 * tg]);
+      uint8_t* vd = smem + L::off_v + s2 * L::kV + (tg >> 3) * (D * 128);
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        uint32_t r[4][4];
+        ints_of<__half>(vr[0][i], z.x, r[0]);
+        ints_of<__half>(vr[1][i], z.y, r[1]);
+        ints_of<__half>(vr[2][i], z.z, r[2]);
+        ints_of<__half>(vr[3][i], z.w, r[3]);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const int d = 4 * (g * W + i) + n;
+          *reinterpret_cast<uint4*>(vd + d * 128 + (((tg & 7) ^ (d & 7)) << 4)) = make_uint4(r[0][n], r[1][n], r[2][n], r[3][n]);
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sc.v_full[s2]);
+      if (more) {
+        w = nx;
+        u = nu;
+        fetch(w, u);
+      }
+      ++unit;
+    }
+  } else {
+    // ---------------- MMA issuer ----------------
+    if (lane == 0) {
+      constexpr uint32_t idesc_s = make_idesc(Ints<T>::fmt, kTok), idesc_o = make_idesc(0, D);
+      const uint32_t base = smem_u32(smem);
+      int unit = 0, items[2] = {0, 0}, done[2] = {0, 0};
+      auto mma_s = [&](int wg, int s2) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          tc_mma_ss(tmem + wg * 128, sw128_desc(base + L::off_q + wg * (L::kQ / 2) + (k >> 2) * 16384 + (k & 3) * 32),
+                    sw128_desc(base + L::off_k + s2 * L::kK + (k >> 2) * 16384 + (k & 3) * 32), idesc_s, k > 0);
+        tc_commit(&sc.s_full[wg]);
+      };
+      bool ok = true;
+      do {
+        const int tiles = (w.j % rts) * kItem + kTile < a.rows ? 2 : 1;
+        if (!mbar_wait(&sc.k_full[unit & 1], (unit >> 1) & 1)) { ok = false; break; }
+        for (int wg = 0; wg < tiles && ok; ++wg) {
+          ok = mbar_wait(&sc.q_full[wg], items[wg]++ & 1);
+          tc_fence_after();
+          if (ok) mma_s(wg, unit & 1);
+        }
+        if (!ok) break;
+        tc_commit(&sc.k_empty[unit & 1]);
+        for (int u = w.u0; u < w.u1 && ok; ++u, ++unit) {
+          const int s2 = unit & 1;
+          const bool more = u + 1 < w.u1;
+          if (more && !mbar_wait(&sc.k_full[s2 ^ 1], ((unit + 1) >> 1) & 1)) { ok = false; break; }
+          if (!mbar_wait(&sc.v_full[s2], (unit >> 1) & 1)) { ok = false; break; }
+          for (int wg = 0; wg < tiles; ++wg) {
+            if (!mbar_wait(&sc.p_full[wg], done[wg] & 1)) { ok = false; break; }
+            ++done[wg];
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < kTok / 16; ++k)
+              tc_mma(tmem + 256 + wg * 128, tmem + wg * 128 + 8 * k,
+                     sw128_desc(base + L::off_v + s2 * L::kV + (k >> 2) * (D * 128) + (k & 3) * 32), idesc_o,
+                     u > w.u0 || k > 0);
+            if (more) mma_s(wg, s2 ^ 1);
+            else tc_commit(&sc.o_full[wg]);
+          }
+          if (!ok) break;
+          tc_commit(&sc.v_empty[s2]);
+          if (more) tc_commit(&sc.k_empty[s2 ^ 1]);
+        }
+      } while (ok && w.next(a));
+      if (!ok) *fail = 1;
+      tc_commit(&sc.drain);  // nothing may be in flight when tensor memory is given back
+      if (!mbar_wait(&sc.drain, 0)) *fail = 1;
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (threadIdx.x == 0) {
+    if (*fail) a.kv.sync[3] = LQ_ETIMEOUT;
+    pdl_trigger();
+  }
+  if (warp == kSoftmaxWarps + kCodeWarps)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+}
+
+// One block per item: merges the parts of the blocks that shared it; zeros
+// where there is nothing to see.
+__global__ void __launch_bounds__(256) kv4_prompt_combine_kernel(const Attn a) {
+  const int rts = a.rows_pad / kItem, D = a.kv.D, V = D / 32;
+  const int j = blockIdx.x / a.kv.H, h = blockIdx.x % a.kv.H, b = j / rts, rt = j % rts;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Tiles t = tiles_of(a, b, rt);
+  int all;
+  const int begin = tiles_before(a, j, all) + h * t.count;
+  Cut cut;
+  cut.set(all, a.blocks);
+  const int c0 = t.count ? cut.owner(begin) : 0, c1 = t.count ? cut.owner(begin + t.count - 1) : -1;
+  if (t.count && c0 == c1) return;
+  pdl_wait();
+  for (int k = warp; k < kItem; k += 8) {
+    const int r = rt * kItem + k;
+    if (r >= a.rows) break;
+    float M = kNone, L = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto row_of = [&](int c) { return (int64_t)(2 * c + (cut.begin(c) >= begin ? 0 : 1)) * kItem + k; };
+    for (int c = c0; c <= c1; ++c) M = fmaxf(M, a.ml[row_of(c)].x);
+    for (int c = c0; c <= c1; ++c) {
+      const float2 ml = a.ml[row_of(c)];
+      const float f = ex2(ml.x - M);
+      L = fmaf(f, ml.y, L);
+      for (int d = 0; d < V; ++d) o[d] = fmaf(f, a.part[row_of(c) * D + V * lane + d], o[d]);
+    }
+    const float inv = L == 0.0f ? 0.0f : pow2(-(int)kHead) / L;
+    const int i = r / a.G, hq = h * a.G + r % a.G;
+    const int64_t at = (((int64_t)b * a.Hq + hq) * a.Sq + i) * D + V * lane;
+    for (int d = 0; d < V; ++d) st_out(a.out, at + d, a.q_dtype, L == 0.0f ? 0.0f : o[d] * inv);
+    if (a.lse && lane == 0) a.lse[(int64_t)(b * a.kv.H + h) * a.rows_pad + r] = L == 0.0f ? INFINITY : M + lg2(L);
+  }
+}
+
+template <typename T, int D>
+int run_prompt(const Attn& a, cudaStream_t st) {
+  constexpr int smem = PromptShared<D>::bytes;
+  static_assert(smem <= 227 * 1024, "shared memory per block");
+  auto kern = kv4_prompt_kernel<T, D>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return launched("kv4_prompt_kernel (attribute)");
+  kern<<<a.blocks, kPromptThreads, smem, st>>>(a);
+  LQ_TRY(launched("kv4_prompt_kernel"));
+  launch_pdl(kv4_prompt_combine_kernel, dim3((unsigned)(a.rows_pad / kItem * a.kv.B * a.kv.H)), dim3(256), 0, st, a);
+  return launched("kv4_prompt_combine_kernel");
+}
+
+}  // namespace
+
+int kv4_prompt(const Attn& a, cudaStream_t st) {
+  if (a.q_dtype == LQ_F16) return a.kv.D == 128 ? run_prompt<__half, 128>(a, st) : run_prompt<__half, 64>(a, st);
+  return a.kv.D == 128 ? run_prompt<__nv_bfloat16, 128>(a, st) : run_prompt<__nv_bfloat16, 64>(a, st);
+}
+
+}  // namespace lq
