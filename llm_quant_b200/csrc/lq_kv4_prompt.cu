@@ -143,6 +143,7 @@ struct PromptShared {
     float sk[kScaleStages][kTok], sv[kScaleStages][kTok];
     int pos[kScaleStages][kTok];
     float e[kScaleStages];
+    float one[32];              // 1: the scale of what is scaled already
     uint32_t zv[2][kTok / 2];   // V zero points as f16 pairs, biased
     float top[2][kCodeWarps];
     uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], t_full[2], s_full[2], p_full[2], o_full[2], drain;
@@ -161,9 +162,33 @@ __device__ __forceinline__ void tc_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
-  tmem_st16(addr, r);
-  tmem_st16(addr + 16, r + 16);
+// tcgen05.wait::ld that the loaded registers pass through, so that no use of
+// them moves ahead of it
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld32(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr)
+      : "memory");
 }
 __device__ __forceinline__ uint64_t pair(float x, float y) {
   uint64_t r;
@@ -246,6 +271,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   Walk w;
   if (!walk_begin(a, blockIdx.x, w)) return;
+  if (threadIdx.x < 32) sc.one[threadIdx.x] = 1.0f;
   if (threadIdx.x == 0) {
     sc.fail = 0;
     for (int i = 0; i < 2; ++i) {
@@ -315,103 +341,97 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
         const bool plain = a.cap == 0.0f && !a.slopes && t0 + kTok <= w.t.n &&
                            ((!a.causal && a.window <= 0) ||
                             (w.t.ordered && (!a.causal || t0 + kTok - 1 <= qa) && (a.window <= 0 || qb - t0 < a.window)));
-        // score (log2 units) of column c from its product, with cap, bias and masks
-        auto score = [&](float s, int c) {
-          float x = s * sk[c];
-          if (a.cap > 0.0f) x = tanh_exp(x) * (a.cap * kLog2e);
-          const int pos = w.t.ordered ? t0 + c : sc.pos[st][c], back = at - pos;
-          if (a.slopes) x = fmaf(-slope, fabsf((float)back), x);
-          bool near = true;
-          if (a.causal) near = back >= 0;
-          if (a.window > 0) near = near && back < a.window;
-          return valid && t0 + c < w.t.n && (near || pos < pre) ? x : -INFINITY;
+        // products to scores (log2 units), with cap, bias and masks
+        auto masked = [&](uint32_t* y, int c) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            float x = __uint_as_float(y[k]) * sk[c + k];
+            if (a.cap > 0.0f) x = tanh_exp(x) * (a.cap * kLog2e);
+            const int t = t0 + c + k, pos = w.t.ordered ? t : sc.pos[st][c + k], back = at - pos;
+            if (a.slopes) x = fmaf(-slope, fabsf((float)back), x);
+            bool near = !a.causal || back >= 0;
+            if (a.window > 0) near = near && back < a.window;
+            y[k] = __float_as_uint(valid && t < w.t.n && (near || pos < pre) ? x : -INFINITY);
+          }
         };
-        uint32_t p[64];
-        float sum, top;
-        auto pass = [&] {
+        float sum = 0.0f;
+        // One copy of this code: the instruction cache holds the roles of all
+        // warps at once (unrolled, fetching instructions was a fifth of the stalls).
+#pragma unroll 1
+        for (int c = 0; c < kTok; c += 32) {
+          uint32_t y[32], p[16];
+          tmem_ld32(S + c, y);
+          tmem_wait_ld32(y);
+          if (!plain) {  // scores in place of products
+            masked(y, c);
+          }
+          const float* f = plain ? sk + c : sc.one;
+          float m = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < 32; k += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(f + k);
+            const float2 y0 = unpair(mul2(pair(__uint_as_float(y[k]), __uint_as_float(y[k + 1])), pair(v.x, v.y)));
+            const float2 y1 = unpair(mul2(pair(__uint_as_float(y[k + 2]), __uint_as_float(y[k + 3])), pair(v.z, v.w)));
+            m = fmaxf(fmaxf(m, fmaxf(y0.x, y0.y)), fmaxf(y1.x, y1.y));
+            y[k] = __float_as_uint(y0.x), y[k + 1] = __float_as_uint(y0.y);
+            y[k + 2] = __float_as_uint(y1.x), y[k + 3] = __float_as_uint(y1.y);
+          }
+          if (__any_sync(0xffffffffu, m + (e + kHead - R) > kTop)) {
+            // raise the reference; P' of this tile so far and O are brought to it
+            m = fmaxf(R, m == -INFINITY ? kNone : m + e);
+            const float alpha = ex2(R - m);
+            l *= alpha;
+            sum *= alpha;
+            R = m;
+            const __half2 alpha2 = __float2half2_rn(alpha);
+#pragma unroll 1
+            for (int d = 0; d < c / 2; d += 16) {
+              tmem_ld16(S + d, p);
+              tmem_wait_ld16(p);
+#pragma unroll
+              for (int k = 0; k < 16; ++k) {
+                const __half2 v = __hmul2(*reinterpret_cast<__half2*>(&p[k]), alpha2);
+                p[k] = *reinterpret_cast<const uint32_t*>(&v);
+              }
+              tmem_st16(S + d, p);
+            }
+            if (u > w.u0) {  // the last PV is complete: its successor's S is
+#pragma unroll 1
+              for (int d = 0; d < D; d += 16) {
+                tmem_ld16(O + d, p);
+                tmem_wait_ld16(p);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) p[k] = __float_as_uint(__uint_as_float(p[k]) * alpha);
+                tmem_st16(O + d, p);
+              }
+            }
+          }
           const float off = e + kHead - R;
-          top = -INFINITY;
-          if (plain) {
-            const uint64_t off2 = pair(off, off);
-            uint64_t s2 = pair(0.0f, 0.0f);
+          const uint64_t off2 = pair(off, off);
+          uint64_t s2 = pair(sum, 0.0f);
 #pragma unroll
-            for (int c = 0; c < kTok; c += 32) {
-              uint32_t x[32];
-              tmem_ld32(S + c, x);
-              tmem_wait_ld();
+          for (int k = 0; k < 32; k += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(sv + c + k);
+            const float2 y0 = unpair(add2(pair(__uint_as_float(y[k]), __uint_as_float(y[k + 1])), off2));
+            const float2 y1 = unpair(add2(pair(__uint_as_float(y[k + 2]), __uint_as_float(y[k + 3])), off2));
+            const uint64_t q0 = pair(ex2(y0.x), ex2(y0.y)), q1 = pair(ex2(y1.x), ex2(y1.y));
+            s2 = add2(s2, add2(q0, q1));
+            const float2 p0 = unpair(mul2(q0, pair(v.x, v.y))), p1 = unpair(mul2(q1, pair(v.z, v.w)));
+            p[k / 2] = h2(p0.x, p0.y);
+            p[k / 2 + 1] = h2(p1.x, p1.y);
+          }
+          const float2 t = unpair(s2);
+          sum = t.x + t.y;
+          if (!plain) {  // a token that is not seen has no weight, whatever its scale
 #pragma unroll
-              for (int k = 0; k < 32; k += 4) {
-                const float4 f = *reinterpret_cast<const float4*>(sk + c + k), v = *reinterpret_cast<const float4*>(sv + c + k);
-                const float2 y0 = unpair(fma2(pair(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), pair(f.x, f.y), off2));
-                const float2 y1 = unpair(fma2(pair(__uint_as_float(x[k + 2]), __uint_as_float(x[k + 3])), pair(f.z, f.w), off2));
-                top = fmaxf(fmaxf(top, fmaxf(y0.x, y0.y)), fmaxf(y1.x, y1.y));
-                const uint64_t q0 = pair(ex2(y0.x), ex2(y0.y)), q1 = pair(ex2(y1.x), ex2(y1.y));
-                s2 = add2(s2, add2(q0, q1));
-                const float2 p0 = unpair(mul2(q0, pair(v.x, v.y))), p1 = unpair(mul2(q1, pair(v.z, v.w)));
-                p[(c + k) / 2] = h2(p0.x, p0.y);
-                p[(c + k) / 2 + 1] = h2(p1.x, p1.y);
-              }
-            }
-            const float2 s = unpair(s2);
-            sum = s.x + s.y;
-          } else {
-            sum = 0.0f;
-#pragma unroll
-            for (int c = 0; c < kTok; c += 32) {
-              uint32_t x[32];
-              tmem_ld32(S + c, x);
-              tmem_wait_ld();
-#pragma unroll
-              for (int k = 0; k < 32; k += 2) {
-                float y[2];
-#pragma unroll
-                for (int d = 0; d < 2; ++d) {
-                  const float v = score(__uint_as_float(x[k + d]), c + k + d), q = ex2(v + off);
-                  top = fmaxf(top, v + off);
-                  sum += q;
-                  y[d] = v == -INFINITY ? 0.0f : q * sv[c + k + d];  // whatever the scale of a token that is not seen
-                }
-                p[(c + k) / 2] = h2(y[0], y[1]);
-              }
+            for (int k = 0; k < 32; k += 2) {
+              if (y[k] == 0xff800000u) p[k / 2] &= 0xffff0000u;
+              if (y[k + 1] == 0xff800000u) p[k / 2] &= 0x0000ffffu;
             }
           }
-        };
-        bool redo = u == w.u0;
-        if (!redo) {
-          pass();
-          redo = __any_sync(0xffffffffu, top > kTop);
-        }
-        if (redo) {
-          float m = kNone;
-#pragma unroll 1
-          for (int c = 0; c < kTok; c += 32) {
-            uint32_t x[32];
-            tmem_ld32(S + c, x);
-            tmem_wait_ld();
-#pragma unroll
-            for (int k = 0; k < 32; ++k)
-              m = fmaxf(m, plain ? __uint_as_float(x[k]) * sk[c + k] : score(__uint_as_float(x[k]), c + k));
-          }
-          m = fmaxf(R, m == kNone ? kNone : m + e);
-          const float alpha = ex2(R - m);
-          l *= alpha;
-          R = m;
-          if (u > w.u0) {  // the last PV is complete: its successor's S is
-#pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-              uint32_t x[32];
-              tmem_ld32(O + c, x);
-              tmem_wait_ld();
-#pragma unroll
-              for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) * alpha);
-              tmem_st32(O + c, x);
-            }
-          }
-          pass();
+          tmem_st16(S + c / 2, p);  // over columns that have been read
         }
         l = fmaf(sum, ex2(-e - kHead), l);
-        tmem_st32(S, p);
-        tmem_st32(S + 32, p + 32);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -433,7 +453,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
         for (int c = 0; c < D; c += 32) {
           uint32_t x[32];
           tmem_ld32(O + c, x);
-          tmem_wait_ld();
+          tmem_wait_ld32(x);
           if (r < a.rows) {
 #pragma unroll
             for (int k = 0; k < 32; k += 8) {
@@ -455,7 +475,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
         for (int c = 0; c < D; c += 32) {
           uint32_t x[32];
           tmem_ld32(O + c, x);
-          tmem_wait_ld();
+          tmem_wait_ld32(x);
           if (r < a.rows) {
 #pragma unroll
             for (int k = 0; k < 32; k += 4)
@@ -639,12 +659,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
 }
 
-// One block per item: merges the parts of the blocks that shared it; zeros
-// where there is nothing to see.
-__global__ void __launch_bounds__(256) kv4_prompt_combine_kernel(const Attn a) {
-  const int rts = a.rows_pad / kItem, D = a.kv.D, V = D / 32;
-  const int j = blockIdx.x / a.kv.H, h = blockIdx.x % a.kv.H, b = j / rts, rt = j % rts;
+// A warp merges the parts of a row that blocks shared; zeros where there is
+// nothing to see.  kMergeRows rows of an item to a block.
+constexpr int kMergeRows = 16;
+template <int D>
+__global__ void __launch_bounds__(128) kv4_prompt_combine_kernel(const Attn a) {
+  constexpr int V = D / 32;
+  const int rts = a.rows_pad / kItem, item = blockIdx.x / (kItem / kMergeRows);
+  const int j = item / a.kv.H, h = item % a.kv.H, b = j / rts, rt = j % rts;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int k0 = blockIdx.x % (kItem / kMergeRows) * kMergeRows;
+  if (rt * kItem + k0 >= a.rows) return;
   const Tiles t = tiles_of(a, b, rt);
   int all;
   const int begin = tiles_before(a, j, all) + h * t.count;
@@ -653,21 +678,38 @@ __global__ void __launch_bounds__(256) kv4_prompt_combine_kernel(const Attn a) {
   const int c0 = t.count ? cut.owner(begin) : 0, c1 = t.count ? cut.owner(begin + t.count - 1) : -1;
   if (t.count && c0 == c1) return;
   pdl_wait();
-  for (int k = warp; k < kItem; k += 8) {
+#pragma unroll
+  for (int k = k0 + warp; k < k0 + kMergeRows; k += 4) {
     const int r = rt * kItem + k;
     if (r >= a.rows) break;
-    float M = kNone, L = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    float M = kNone, L = 0.0f, o[V];
+#pragma unroll
+    for (int d = 0; d < V; ++d) o[d] = 0.0f;
     auto row_of = [&](int c) { return (int64_t)(2 * c + (cut.begin(c) >= begin ? 0 : 1)) * kItem + k; };
-    for (int c = c0; c <= c1; ++c) M = fmaxf(M, a.ml[row_of(c)].x);
+    for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, a.ml[row_of(c)].x);
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, m));
+#pragma unroll 4
     for (int c = c0; c <= c1; ++c) {
-      const float2 ml = a.ml[row_of(c)];
+      const int64_t row = row_of(c);
+      const float2 ml = a.ml[row];
       const float f = ex2(ml.x - M);
+      float v[V];
+      if constexpr (V == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(a.part + row * D + V * lane);
+        v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+      } else {
+        const float2 x = *reinterpret_cast<const float2*>(a.part + row * D + V * lane);
+        v[0] = x.x, v[1] = x.y;
+      }
       L = fmaf(f, ml.y, L);
-      for (int d = 0; d < V; ++d) o[d] = fmaf(f, a.part[row_of(c) * D + V * lane + d], o[d]);
+#pragma unroll
+      for (int d = 0; d < V; ++d) o[d] = fmaf(f, v[d], o[d]);
     }
     const float inv = L == 0.0f ? 0.0f : pow2(-(int)kHead) / L;
     const int i = r / a.G, hq = h * a.G + r % a.G;
     const int64_t at = (((int64_t)b * a.Hq + hq) * a.Sq + i) * D + V * lane;
+#pragma unroll
     for (int d = 0; d < V; ++d) st_out(a.out, at + d, a.q_dtype, L == 0.0f ? 0.0f : o[d] * inv);
     if (a.lse && lane == 0) a.lse[(int64_t)(b * a.kv.H + h) * a.rows_pad + r] = L == 0.0f ? INFINITY : M + lg2(L);
   }
@@ -682,7 +724,7 @@ int run_prompt(const Attn& a, cudaStream_t st) {
     return launched("kv4_prompt_kernel (attribute)");
   kern<<<a.blocks, kPromptThreads, smem, st>>>(a);
   LQ_TRY(launched("kv4_prompt_kernel"));
-  launch_pdl(kv4_prompt_combine_kernel, dim3((unsigned)(a.rows_pad / kItem * a.kv.B * a.kv.H)), dim3(256), 0, st, a);
+  launch_pdl(kv4_prompt_combine_kernel<D>, dim3((unsigned)(a.rows_pad / kMergeRows * a.kv.B * a.kv.H)), dim3(128), 0, st, a);
   return launched("kv4_prompt_combine_kernel");
 }
 
