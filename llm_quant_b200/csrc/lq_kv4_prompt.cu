@@ -16,8 +16,9 @@
 //
 // Warps: 0-3 and 4-7 softmax of the two row tiles (a thread owns a row), 8-11
 // turn packed codes into the two operands in shared memory (swizzled, two
-// stages), 12 issues the MMAs.  Tensor memory: S0, S1 (P' lies over S), O0, O1.
-// The MMAs of one row tile run while the softmax of the other does.
+// stages), 12 issues the MMAs, 13 tells the others what to do next.  Tensor memory: S0, S1 (P' lies over S), O0, O1.
+// A row tile has two halves of S (64 tokens each): while one is turned into P'
+// in place, the MMAs fill the other.
 //
 // Bound: per 128 x 128 tile of scores the tensor cores need 1024 cycles (D =
 // 128) and the 16384 exponentials 1024 on the SM's special-function units; the
@@ -37,7 +38,13 @@ constexpr int kTok = 128;    // tokens of a tile
 constexpr int kTile = 128;   // rows of a tile
 constexpr int kItem = kPromptRows;  // rows of an item
 constexpr int kSoftmaxWarps = 8, kCodeWarps = 4;
-constexpr int kPromptThreads = 32 * (kSoftmaxWarps + kCodeWarps + 1);
+// 16 warps of 128 registers at launch; each group of four then takes what its
+// role needs: 2 x 168 + 96 + 80 = 4 x 128.
+constexpr int kPromptThreads = 512;
+template <int N>
+__device__ __forceinline__ void more_regs() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void fewer_regs() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 constexpr int kScaleStages = 4;
 
 // The token tiles that the rows of an item may see: tiles [0, pre) and [pre +
@@ -70,7 +77,7 @@ __device__ __forceinline__ Tiles tiles_of(const Attn& a, int b, int rt) {
 }
 
 // A block's way through the items (sequence, row tile, head) that its stretch
-// covers; every warp goes it for itself.
+// covers.
 struct Walk {
   int x0, x1, j, h, u0, u1;
   Tiles t;
@@ -130,7 +137,15 @@ __device__ __forceinline__ bool walk_begin(const Attn& a, int cta, Walk& w) {
   w.piece();
   return true;
 }
-__device__ __forceinline__ int tile_token(const Tiles& t, int u) { return (u < t.pre ? u : u + t.gap) * kTok; }
+
+// A part of an item, in shared memory: one warp goes the way, the others read
+// from here what they need (registers are short in all roles).
+struct Piece {
+  int some;  // 0: there is no more
+  int b, h, rt, u0, u1, n, cnt, first, ordered, pre, gap, whole;
+  __device__ __forceinline__ int token(int u) const { return (u < pre ? u : u + gap) * kTok; }
+};
+constexpr int kPieces = 4;
 
 template <int D>
 struct PromptShared {
@@ -143,10 +158,11 @@ struct PromptShared {
     float sk[kScaleStages][kTok], sv[kScaleStages][kTok];
     int pos[kScaleStages][kTok];
     float e[kScaleStages];
-    float one[32];              // 1: the scale of what is scaled already
     uint32_t zv[2][kTok / 2];   // V zero points as f16 pairs, biased
     float top[2][kCodeWarps];
-    uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], t_full[2], s_full[2], p_full[2], o_full[2], drain;
+    Piece piece[kPieces];
+    uint64_t piece_full[kPieces], piece_empty[kPieces];
+    uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], t_full[2], s_full[2][2], p_full[2][2], pv_done[2][2], drain;
     uint32_t tmem;
     int fail;
   };
@@ -265,15 +281,18 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Attn a) {
   using L = PromptShared<D>;
   constexpr int W = D / 32;
-  extern __shared__ uint8_t raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(16) uint8_t raw[];
+  // aligned without a cast to an integer, after which every access would be generic
+  uint8_t* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
   typename L::Scales& sc = *reinterpret_cast<typename L::Scales*>(smem + L::off_s);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  Walk w;
-  if (!walk_begin(a, blockIdx.x, w)) return;
-  if (threadIdx.x < 32) sc.one[threadIdx.x] = 1.0f;
+  const int rts = a.rows_pad / kItem;
   if (threadIdx.x == 0) {
     sc.fail = 0;
+    for (int i = 0; i < kPieces; ++i) {
+      mbar_init(&sc.piece_full[i], 1);
+      mbar_init(&sc.piece_empty[i], kSoftmaxWarps + kCodeWarps + 1);
+    }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sc.q_full[i], kTile);
       mbar_init(&sc.k_full[i], kCodeWarps);
@@ -281,9 +300,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
       mbar_init(&sc.v_full[i], kCodeWarps);
       mbar_init(&sc.t_full[i], kCodeWarps);
       mbar_init(&sc.v_empty[i], 1);
-      mbar_init(&sc.s_full[i], 1);
-      mbar_init(&sc.p_full[i], 4);
-      mbar_init(&sc.o_full[i], 1);
+      // one for each half of S: a row tile's softmax may be a step ahead of the
+      // MMAs, and a parity only tells neighbouring phases apart
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&sc.s_full[i][h], 1);
+        mbar_init(&sc.p_full[i][h], 4);
+        mbar_init(&sc.pv_done[i][h], 1);
+      }
     }
     mbar_init(&sc.drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -301,154 +324,199 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
   // every wait, this one's aside, is bounded too.  Whole warps agree on it.
   volatile int* fail = &sc.fail;
   auto gone = [&] { return __any_sync(0xffffffffu, *fail != 0); };
-  const int rts = a.rows_pad / kItem;
+  // the k-th piece; its warp's lanes return the slot together
+  auto next_piece = [&](int k) {
+    if (!mbar_wait_warp(&sc.piece_full[k % kPieces], (k / kPieces) & 1)) *fail = 1;
+  };
+  auto done_with = [&](int k) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sc.piece_empty[k % kPieces]);
+  };
 
   if (warp < kSoftmaxWarps) {
     // ---------------- softmax: a thread owns a row of its tile ----------------
+    more_regs<168>();
     const int wg = warp >> 2, tid = threadIdx.x & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t S = tmem + lanes + wg * 128, O = tmem + lanes + 256 + wg * 128;
-    int unit = 0, mine = 0;  // units of this block so far, and those of them that this tile had rows in
-    int items = 0;           // items that this tile had rows in
-    bool first_piece = true;
-    do {
-      const int b = w.j / rts, rt = w.j % rts;
-      const int r = rt * kItem + wg * kTile + tid, i = r / a.G;
-      const bool valid = r < a.rows && i < w.t.cnt;
-      const int at = w.t.first + i;
-      const bool active = rt * kItem + wg * kTile < a.rows;
-      if (!active) {
+    const uint32_t O = tmem + lanes + 256 + wg * 128;
+    int unit = 0;    // token tiles of this block so far
+    int steps = 0;   // half tiles that this row tile has worked on
+    for (int k = 0;; ++k) {
+      next_piece(k);
+      if (gone()) break;
+      const Piece& w = sc.piece[k % kPieces];
+      if (!w.some) break;
+      const int r0 = w.rt * kItem + wg * kTile;
+      if (r0 >= a.rows) {
         unit += w.u1 - w.u0;
-        first_piece = false;
+        done_with(k);
         continue;
       }
-      stage_rows<T, D>(smem + L::off_q + wg * (L::kQ / 2), a, b, w.h, w.t.cnt, rt * kItem + wg * kTile, tid);
+      const int r = r0 + tid, i = r / a.G;
+      const bool valid = r < a.rows && i < w.cnt;
+      const int at = w.first + i, n = w.n, n_steps = 2 * (w.u1 - w.u0), ordered = w.ordered;
+      stage_rows<T, D>(smem + L::off_q + wg * (L::kQ / 2), a, w.b, w.h, w.cnt, r0, tid);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(&sc.q_full[wg]);
       const float slope = a.slopes && r < a.rows ? a.slopes[w.h * a.G + r % a.G] * kLog2e : 0.0f;
-      const int pre = a.prefix ? a.prefix[b] : 0;
+      const int pre = a.prefix ? a.prefix[w.b] : 0;
       // positions of the tile's first and last row
-      const int qa = w.t.first + (rt * kItem + wg * kTile) / a.G, qb = w.t.first + (rt * kItem + wg * kTile + kTile - 1) / a.G;
+      const int qa = w.first + r0 / a.G, qb = w.first + (r0 + kTile - 1) / a.G;
       float R = kNone, l = 0.0f;
-      for (int u = w.u0; u < w.u1; ++u, ++unit, ++mine) {
-        if (!mbar_wait_warp(&sc.s_full[wg], mine & 1)) *fail = 1;
+      for (int j = 0; j < n_steps; ++j, ++steps) {
+        const int st = (unit + (j >> 1)) % kScaleStages, t0 = w.token(w.u0 + (j >> 1)) + 64 * (j & 1);
+        const float* sk = sc.sk[st] + 64 * (j & 1);
+        const float* sv = sc.sv[st] + 64 * (j & 1);
+        const bool plain = a.cap == 0.0f && !a.slopes && t0 + 64 <= n &&
+                           ((!a.causal && a.window <= 0) ||
+                            (ordered && (!a.causal || t0 + 63 <= qa) && (a.window <= 0 || qb - t0 < a.window)));
+        const uint32_t S = tmem + lanes + wg * 128 + 64 * (steps & 1);
+        if (!mbar_wait_warp(&sc.s_full[wg][steps & 1], (steps >> 1) & 1)) *fail = 1;
         if (gone()) break;
         tc_fence_after();
-        const int t0 = tile_token(w.t, u), st = unit % kScaleStages;
-        const float* sk = sc.sk[st];
-        const float* sv = sc.sv[st];
         const float e = sc.e[st];
-        const bool plain = a.cap == 0.0f && !a.slopes && t0 + kTok <= w.t.n &&
-                           ((!a.causal && a.window <= 0) ||
-                            (w.t.ordered && (!a.causal || t0 + kTok - 1 <= qa) && (a.window <= 0 || qb - t0 < a.window)));
         // products to scores (log2 units), with cap, bias and masks
         auto masked = [&](uint32_t* y, int c) {
 #pragma unroll
           for (int k = 0; k < 32; ++k) {
             float x = __uint_as_float(y[k]) * sk[c + k];
             if (a.cap > 0.0f) x = tanh_exp(x) * (a.cap * kLog2e);
-            const int t = t0 + c + k, pos = w.t.ordered ? t : sc.pos[st][c + k], back = at - pos;
+            const int t = t0 + c + k, pos = ordered ? t : sc.pos[st][64 * (j & 1) + c + k], back = at - pos;
             if (a.slopes) x = fmaf(-slope, fabsf((float)back), x);
             bool near = !a.causal || back >= 0;
             if (a.window > 0) near = near && back < a.window;
-            y[k] = __float_as_uint(valid && t < w.t.n && (near || pos < pre) ? x : -INFINITY);
+            y[k] = __float_as_uint(valid && t < n && (near || pos < pre) ? x : -INFINITY);
           }
         };
         float sum = 0.0f;
-        // One copy of this code: the instruction cache holds the roles of all
-        // warps at once (unrolled, fetching instructions was a fifth of the stalls).
+        // Raises the row's reference to the greatest score m, and brings O to
+        // it once the last PV is complete.
+        auto raise = [&](float m) {
+          m = fmaxf(R, m == -INFINITY ? kNone : m + e);
+          const float alpha = ex2(R - m);
+          l *= alpha;
+          sum *= alpha;
+          R = m;
+          if (j > 0) {
+            if (!mbar_wait_warp(&sc.pv_done[wg][(steps - 1) & 1], ((steps - 1) >> 1) & 1)) *fail = 1;
+            tc_fence_after();
+            uint32_t z[16];
 #pragma unroll 1
-        for (int c = 0; c < kTok; c += 32) {
-          uint32_t y[32], p[16];
-          tmem_ld32(S + c, y);
+            for (int d = 0; d < D; d += 16) {
+              tmem_ld16(O + d, z);
+              tmem_wait_ld16(z);
+#pragma unroll
+              for (int k = 0; k < 16; ++k) z[k] = __float_as_uint(__uint_as_float(z[k]) * alpha);
+              tmem_st16(O + d, z);
+            }
+          }
+        };
+        if (plain) {
+          uint32_t y[64], p[32];
+          float top[2];
+          auto exponents = [&] {
+            const float off = e + kHead - R;
+            const uint64_t off2 = pair(off, off);
+            top[0] = top[1] = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < 64; k += 4) {
+              const float4 f = *reinterpret_cast<const float4*>(sk + k);
+              const float2 y0 = unpair(fma2(pair(__uint_as_float(y[k]), __uint_as_float(y[k + 1])), pair(f.x, f.y), off2));
+              const float2 y1 = unpair(fma2(pair(__uint_as_float(y[k + 2]), __uint_as_float(y[k + 3])), pair(f.z, f.w), off2));
+              top[0] = fmaxf(top[0], fmaxf(y0.x, y0.y));
+              top[1] = fmaxf(top[1], fmaxf(y1.x, y1.y));
+              y[k] = __float_as_uint(ex2(y0.x)), y[k + 1] = __float_as_uint(ex2(y0.y));
+              y[k + 2] = __float_as_uint(ex2(y1.x)), y[k + 3] = __float_as_uint(ex2(y1.y));
+            }
+          };
+          tmem_ld32(S, y);
+          tmem_ld32(S + 32, y + 32);
           tmem_wait_ld32(y);
-          if (!plain) {  // scores in place of products
-            masked(y, c);
+          tmem_wait_ld32(y + 32);
+          exponents();
+          if (__any_sync(0xffffffffu, fmaxf(top[0], top[1]) > kTop)) {
+            float m = -INFINITY;
+            tmem_ld32(S, y);
+            tmem_ld32(S + 32, y + 32);
+            tmem_wait_ld32(y);
+            tmem_wait_ld32(y + 32);
+#pragma unroll
+            for (int k = 0; k < 64; ++k) m = fmaxf(m, __uint_as_float(y[k]) * sk[k]);
+            raise(m);
+            exponents();
           }
-          const float* f = plain ? sk + c : sc.one;
-          float m = -INFINITY;
+          uint64_t s2[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
 #pragma unroll
-          for (int k = 0; k < 32; k += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(f + k);
-            const float2 y0 = unpair(mul2(pair(__uint_as_float(y[k]), __uint_as_float(y[k + 1])), pair(v.x, v.y)));
-            const float2 y1 = unpair(mul2(pair(__uint_as_float(y[k + 2]), __uint_as_float(y[k + 3])), pair(v.z, v.w)));
-            m = fmaxf(fmaxf(m, fmaxf(y0.x, y0.y)), fmaxf(y1.x, y1.y));
-            y[k] = __float_as_uint(y0.x), y[k + 1] = __float_as_uint(y0.y);
-            y[k + 2] = __float_as_uint(y1.x), y[k + 3] = __float_as_uint(y1.y);
-          }
-          if (__any_sync(0xffffffffu, m + (e + kHead - R) > kTop)) {
-            // raise the reference; P' of this tile so far and O are brought to it
-            m = fmaxf(R, m == -INFINITY ? kNone : m + e);
-            const float alpha = ex2(R - m);
-            l *= alpha;
-            sum *= alpha;
-            R = m;
-            const __half2 alpha2 = __float2half2_rn(alpha);
-#pragma unroll 1
-            for (int d = 0; d < c / 2; d += 16) {
-              tmem_ld16(S + d, p);
-              tmem_wait_ld16(p);
-#pragma unroll
-              for (int k = 0; k < 16; ++k) {
-                const __half2 v = __hmul2(*reinterpret_cast<__half2*>(&p[k]), alpha2);
-                p[k] = *reinterpret_cast<const uint32_t*>(&v);
-              }
-              tmem_st16(S + d, p);
-            }
-            if (u > w.u0) {  // the last PV is complete: its successor's S is
-#pragma unroll 1
-              for (int d = 0; d < D; d += 16) {
-                tmem_ld16(O + d, p);
-                tmem_wait_ld16(p);
-#pragma unroll
-                for (int k = 0; k < 16; ++k) p[k] = __float_as_uint(__uint_as_float(p[k]) * alpha);
-                tmem_st16(O + d, p);
-              }
-            }
-          }
-          const float off = e + kHead - R;
-          const uint64_t off2 = pair(off, off);
-          uint64_t s2 = pair(sum, 0.0f);
-#pragma unroll
-          for (int k = 0; k < 32; k += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(sv + c + k);
-            const float2 y0 = unpair(add2(pair(__uint_as_float(y[k]), __uint_as_float(y[k + 1])), off2));
-            const float2 y1 = unpair(add2(pair(__uint_as_float(y[k + 2]), __uint_as_float(y[k + 3])), off2));
-            const uint64_t q0 = pair(ex2(y0.x), ex2(y0.y)), q1 = pair(ex2(y1.x), ex2(y1.y));
-            s2 = add2(s2, add2(q0, q1));
+          for (int k = 0; k < 64; k += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(sv + k);
+            const uint64_t q0 = pair(__uint_as_float(y[k]), __uint_as_float(y[k + 1]));
+            const uint64_t q1 = pair(__uint_as_float(y[k + 2]), __uint_as_float(y[k + 3]));
+            s2[0] = add2(s2[0], q0);
+            s2[1] = add2(s2[1], q1);
             const float2 p0 = unpair(mul2(q0, pair(v.x, v.y))), p1 = unpair(mul2(q1, pair(v.z, v.w)));
             p[k / 2] = h2(p0.x, p0.y);
             p[k / 2 + 1] = h2(p1.x, p1.y);
           }
-          const float2 t = unpair(s2);
-          sum = t.x + t.y;
-          if (!plain) {  // a token that is not seen has no weight, whatever its scale
+          tmem_st16(S, p);  // P' lies over S
+          tmem_st16(S + 16, p + 16);
+          const float2 x0 = unpair(s2[0]), x1 = unpair(s2[1]);
+          sum = (x0.x + x0.y) + (x1.x + x1.y);
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < 64; c += 32) {
+            uint32_t y[32], p[16];
+            tmem_ld32(S + c, y);
+            tmem_wait_ld32(y);
+            masked(y, c);
+            float m = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < 32; ++k) m = fmaxf(m, __uint_as_float(y[k]));
+            if (__any_sync(0xffffffffu, m + (e + kHead - R) > kTop)) {
+              const float before = R;
+              raise(m);
+              if (c) {  // the first half's P' is there already
+                const __half2 alpha = __float2half2_rn(ex2(before - R));
+                tmem_ld16(S, p);
+                tmem_wait_ld16(p);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                  const __half2 v = __hmul2(*reinterpret_cast<__half2*>(&p[k]), alpha);
+                  p[k] = *reinterpret_cast<const uint32_t*>(&v);
+                }
+                tmem_st16(S, p);
+              }
+            }
+            const float off = e + kHead - R;
 #pragma unroll
             for (int k = 0; k < 32; k += 2) {
-              if (y[k] == 0xff800000u) p[k / 2] &= 0xffff0000u;
-              if (y[k + 1] == 0xff800000u) p[k / 2] &= 0x0000ffffu;
+              float q[2];
+#pragma unroll
+              for (int d = 0; d < 2; ++d) {
+                const float v = __uint_as_float(y[k + d]);
+                q[d] = ex2(v + off);
+                sum += q[d];
+                q[d] = v == -INFINITY ? 0.0f : q[d] * sv[c + k + d];  // whatever the scale of a token that is not seen
+              }
+              p[k / 2] = h2(q[0], q[1]);
             }
+            tmem_st16(S + c / 2, p);
           }
-          tmem_st16(S + c / 2, p);  // over columns that have been read
         }
         l = fmaf(sum, ex2(-e - kHead), l);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sc.p_full[wg]);
+        if (lane == 0) mbar_arrive(&sc.p_full[wg][steps & 1]);
       }
+      unit += n_steps / 2;
       if (gone()) break;
       // ---- the item's rows, or this block's part of them ----
-      if (!mbar_wait_warp(&sc.o_full[wg], items & 1)) {
-        *fail = 1;
-        break;
-      }
-      ++items;
+      if (!mbar_wait_warp(&sc.pv_done[wg][(steps - 1) & 1], ((steps - 1) >> 1) & 1)) *fail = 1;
+      if (gone()) break;
       tc_fence_after();
-      const bool whole = w.u0 == 0 && w.u1 == w.t.count;
-      if (whole) {
+      if (w.whole) {
         const float inv = !valid || l == 0.0f ? 0.0f : pow2(-(int)kHead) / l;
-        T* out = reinterpret_cast<T*>(a.out) + (((int64_t)b * a.Hq + w.h * a.G + r % a.G) * a.Sq + i) * D;
+        T* out = reinterpret_cast<T*>(a.out) + (((int64_t)w.b * a.Hq + w.h * a.G + r % a.G) * a.Sq + i) * D;
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           uint32_t x[32];
@@ -468,9 +536,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
           }
         }
         if (a.lse && r < a.rows)
-          a.lse[(int64_t)(b * a.kv.H + w.h) * a.rows_pad + r] = !valid || l == 0.0f ? INFINITY : R + lg2(l);
+          a.lse[(int64_t)(w.b * a.kv.H + w.h) * a.rows_pad + r] = !valid || l == 0.0f ? INFINITY : R + lg2(l);
       } else {
-        const int64_t row = (int64_t)(2 * blockIdx.x + (first_piece ? 0 : 1)) * kItem + wg * kTile + tid;
+        const int64_t row = (int64_t)(2 * blockIdx.x + (k ? 1 : 0)) * kItem + wg * kTile + tid;
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           uint32_t x[32];
@@ -486,21 +554,22 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
         if (r < a.rows) a.ml[row] = make_float2(R, valid ? l : 0.0f);
       }
       tc_fence_before();
-      first_piece = false;
-    } while (w.next(a));
+      done_with(k);
+    }
   } else if (warp < kSoftmaxWarps + kCodeWarps) {
     // ---------------- codes to operands ----------------
+    fewer_regs<96>();
     const int tid = threadIdx.x - 32 * kSoftmaxWarps, cw = warp - kSoftmaxWarps;
     const int g = tid >> 4, tg = tid & 15;  // V: 16 values (units g W ..) of 8 tokens
     const float fk = a.sm * (a.cap > 0.0f ? 1.0f / a.cap : kLog2e);
     uint32_t kr[2 * W][2], vr[4][W];
     uint2 par = make_uint2(0u, 0u);
     int unit = 0;
-    auto fetch = [&](const Walk& x, int u) {
-      const int t0 = tile_token(x.t, u), t = t0 + tid, tv = t0 + 8 * tg;
-      const int64_t row = (int64_t)(x.j / rts * a.kv.H + x.h) * a.kv.cap;
+    auto fetch_k = [&](const Piece& x, int u) {
+      const int t = x.token(u) + tid;
+      const int64_t row = (int64_t)(x.b * a.kv.H + x.h) * a.kv.cap;
       par = make_uint2(0u, 0u);
-      if (t < x.t.n) {
+      if (t < x.n) {
         const uint2* p = reinterpret_cast<const uint2*>(a.kv.k + (row + t) * (D / 2));
 #pragma unroll
         for (int i = 0; i < 2 * W; ++i) {
@@ -509,8 +578,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
         }
         par = __ldg(a.kv.par + row + t);
       }
-      if (tv < x.t.n) {
-        const uint8_t* p = a.kv.v + row * (D / 2) + (int64_t)(tv >> 4) * (W * 256) + ((tv >> 3) & 1) * (W * 128) + g * (W * 16);
+    };
+    auto fetch_v = [&](const Piece& x, int u) {
+      const int t = x.token(u) + 8 * tg;
+      const int64_t row = (int64_t)(x.b * a.kv.H + x.h) * a.kv.cap;
+      if (t < x.n) {
+        const uint8_t* p = a.kv.v + row * (D / 2) + (int64_t)(t >> 4) * (W * 256) + ((t >> 3) & 1) * (W * 128) + g * (W * 16);
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -526,18 +599,26 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
     for (int c = 0; c < 4; ++c)
 #pragma unroll
       for (int i = 0; i < W; ++i) vr[c][i] = 0u;
-    fetch(w, w.u0);
-    bool more = true;
-    int u = w.u0;
+    int k = 0;
+    next_piece(0);
+    bool more = !gone() && sc.piece[0].some;
+    int u = sc.piece[0].u0;
+    if (more) {
+      fetch_k(sc.piece[0], u);
+      fetch_v(sc.piece[0], u);
+    }
     while (more) {
-      const int s2 = unit & 1, st = unit % kScaleStages, t0 = tile_token(w.t, u);
+      const Piece& w = sc.piece[k % kPieces];
+      const int s2 = unit & 1, st = unit % kScaleStages;
       // where the next unit is
-      Walk nx = w;
-      int nu = u + 1;
-      if (nu >= w.u1) {
-        more = nx.next(a);
-        nu = nx.u0;
+      int nk = k, nu = u + 1;
+      if (nu == w.u1) {
+        nk = k + 1;
+        next_piece(nk);
+        more = sc.piece[nk % kPieces].some;
+        nu = sc.piece[nk % kPieces].u0;
       }
+      const Piece& nx = sc.piece[nk % kPieces];
       if (unit >= 2 && !mbar_wait_warp(&sc.k_empty[s2], ((unit >> 1) - 1) & 1)) *fail = 1;
       if (gone()) break;
       // ---- K, and the columns' scales ----
@@ -562,12 +643,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
       const int e = big > 0.0f ? (int)(__float_as_uint(big) >> 23) - 126 : 0;  // big < 2^e
       sc.sk[st][tid] = par_scale(par.x) * fk;
       sc.sv[st][tid] = sv * __uint_as_float((uint32_t)(127 - e) << 23);
-      if (!w.t.ordered)
-        sc.pos[st][tid] = t0 + tid < w.t.n ? a.kv.pos[(int64_t)(w.j / rts * a.kv.H + w.h) * a.kv.cap + t0 + tid] : 0;
+      if (!w.ordered) {
+        const int t = w.token(u) + tid;
+        sc.pos[st][tid] = t < w.n ? a.kv.pos[(int64_t)(w.b * a.kv.H + w.h) * a.kv.cap + t] : 0;
+      }
       if (tid == 0) sc.e[st] = (float)e;
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(&sc.k_full[s2]);
+      if (more) fetch_k(nx, nu);
       // ---- V^T ----
       if (unit >= 2 && !mbar_wait_warp(&sc.v_empty[s2], ((unit >> 1) - 1) & 1)) *fail = 1;
       if (gone()) break;
@@ -589,59 +673,101 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(&sc.v_full[s2]);
-      if (more) {
-        w = nx;
-        u = nu;
-        fetch(w, u);
-      }
+      if (more) fetch_v(nx, nu);
+      if (nk != k) done_with(k);
+      k = nk;
+      u = nu;
       ++unit;
     }
   } else {
+    fewer_regs<80>();
+    if (warp == kSoftmaxWarps + kCodeWarps + 1) {
+      // ---------------- the way through the items ----------------
+      Walk w;
+      bool some = walk_begin(a, blockIdx.x, w);
+      for (int k = 0;; ++k) {
+        if (k >= kPieces && !mbar_wait_warp(&sc.piece_empty[k % kPieces], ((k / kPieces) - 1) & 1)) *fail = 1;
+        if (gone()) break;
+        if (lane == 0) {
+          Piece& p = sc.piece[k % kPieces];
+          p.some = some;
+          if (some) {
+            p.b = w.j / rts, p.rt = w.j % rts, p.h = w.h, p.u0 = w.u0, p.u1 = w.u1;
+            p.n = w.t.n, p.cnt = w.t.cnt, p.first = w.t.first, p.ordered = w.t.ordered, p.pre = w.t.pre, p.gap = w.t.gap;
+            p.whole = w.u0 == 0 && w.u1 == w.t.count;
+          }
+          mbar_arrive(&sc.piece_full[k % kPieces]);
+        }
+        if (!some) break;
+        some = w.next(a);
+      }
+    }
     // ---------------- MMA issuer ----------------
-    if (lane == 0) {
-      constexpr uint32_t idesc_s = make_idesc(Ints<T>::fmt, kTok), idesc_o = make_idesc(0, D);
+    if (warp == kSoftmaxWarps + kCodeWarps && lane == 0) {
+      constexpr uint32_t idesc_s = make_idesc(Ints<T>::fmt, 64), idesc_o = make_idesc(0, D);
       const uint32_t base = smem_u32(smem);
-      int unit = 0, items[2] = {0, 0}, done[2] = {0, 0};
-      auto mma_s = [&](int wg, int s2) {
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          tc_mma_ss(tmem + wg * 128, sw128_desc(base + L::off_q + wg * (L::kQ / 2) + (k >> 2) * 16384 + (k & 3) * 32),
-                    sw128_desc(base + L::off_k + s2 * L::kK + (k >> 2) * 16384 + (k & 3) * 32), idesc_s, k > 0);
-        tc_commit(&sc.s_full[wg]);
+      int unit = 0, items[2] = {0, 0}, steps[2] = {0, 0};
+      // The loops are short: unrolled, the MMAs of a tile (and the code of the
+      // other roles) did not fit the instruction cache, and an MMA took 200
+      // cycles to issue instead of 64.
+      // S of half tile j of this piece; x: half tiles of row tile wg so far.  A
+      // step of 16 along K is 32 bytes of the swizzled rows, 64 are a half.
+      auto mma_s = [&](int wg, int j, int x) {
+        const uint64_t dq = sw128_desc(base + L::off_q + wg * (L::kQ / 2));
+        const uint64_t dk = sw128_desc(base + L::off_k + ((unit + (j >> 1)) & 1) * L::kK + (j & 1) * 8192);
+#pragma unroll 4
+        for (int k = 0; k < D / 16; ++k) {
+          const uint64_t step = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
+          tc_mma_ss(tmem + wg * 128 + 64 * (x & 1), dq + step, dk + step, idesc_s, k > 0);
+        }
+        tc_commit(&sc.s_full[wg][x & 1]);
       };
       bool ok = true;
-      do {
-        const int tiles = (w.j % rts) * kItem + kTile < a.rows ? 2 : 1;
+      for (int k = 0;; ++k) {
+        ok = mbar_wait(&sc.piece_full[k % kPieces], (k / kPieces) & 1);
+        const Piece& w = sc.piece[k % kPieces];
+        if (!ok || !w.some) break;
+        const int tiles = w.rt * kItem + kTile < a.rows ? 2 : 1, n_steps = 2 * (w.u1 - w.u0);
         if (!mbar_wait(&sc.k_full[unit & 1], (unit >> 1) & 1)) { ok = false; break; }
         for (int wg = 0; wg < tiles && ok; ++wg) {
           ok = mbar_wait(&sc.q_full[wg], items[wg]++ & 1);
           tc_fence_after();
-          if (ok) mma_s(wg, unit & 1);
+          if (ok) mma_s(wg, 0, steps[wg]);
         }
+        for (int wg = 0; wg < tiles && ok; ++wg) mma_s(wg, 1, steps[wg] + 1);
         if (!ok) break;
         tc_commit(&sc.k_empty[unit & 1]);
-        for (int u = w.u0; u < w.u1 && ok; ++u, ++unit) {
-          const int s2 = unit & 1;
-          const bool more = u + 1 < w.u1;
-          if (more && !mbar_wait(&sc.k_full[s2 ^ 1], ((unit + 1) >> 1) & 1)) { ok = false; break; }
-          if (!mbar_wait(&sc.v_full[s2], (unit >> 1) & 1)) { ok = false; break; }
+#pragma unroll 1
+        for (int j = 0; j < n_steps && ok; ++j) {
+          const int u = unit + (j >> 1), un = unit + ((j + 2) >> 1);
+          const bool more = j + 2 < n_steps;
+          if (!(j & 1) && ((more && !mbar_wait(&sc.k_full[un & 1], (un >> 1) & 1)) || !mbar_wait(&sc.v_full[u & 1], (u >> 1) & 1))) {
+            ok = false;
+            break;
+          }
+#pragma unroll 1
           for (int wg = 0; wg < tiles; ++wg) {
-            if (!mbar_wait(&sc.p_full[wg], done[wg] & 1)) { ok = false; break; }
-            ++done[wg];
+            if (!mbar_wait(&sc.p_full[wg][steps[wg] & 1], (steps[wg] >> 1) & 1)) { ok = false; break; }
             tc_fence_after();
+            const uint64_t dv = sw128_desc(base + L::off_v + (u & 1) * L::kV + (j & 1) * (D * 128));
 #pragma unroll
-            for (int k = 0; k < kTok / 16; ++k)
-              tc_mma(tmem + 256 + wg * 128, tmem + wg * 128 + 8 * k,
-                     sw128_desc(base + L::off_v + s2 * L::kV + (k >> 2) * (D * 128) + (k & 3) * 32), idesc_o,
-                     u > w.u0 || k > 0);
-            if (more) mma_s(wg, s2 ^ 1);
-            else tc_commit(&sc.o_full[wg]);
+            for (int k = 0; k < 4; ++k)
+              tc_mma(tmem + 256 + wg * 128, tmem + wg * 128 + 64 * (steps[wg] & 1) + 8 * k, dv + ((k * 32) >> 4), idesc_o,
+                     j > 0 || k > 0);
+            tc_commit(&sc.pv_done[wg][steps[wg] & 1]);
+            if (more) mma_s(wg, j + 2, steps[wg] + 2);
+            ++steps[wg];
           }
           if (!ok) break;
-          tc_commit(&sc.v_empty[s2]);
-          if (more) tc_commit(&sc.k_empty[s2 ^ 1]);
+          if (j & 1) {
+            tc_commit(&sc.v_empty[u & 1]);
+            if (more) tc_commit(&sc.k_empty[un & 1]);
+          }
         }
-      } while (ok && w.next(a));
+        if (!ok) break;
+        unit += n_steps / 2;
+        mbar_arrive(&sc.piece_empty[k % kPieces]);
+      }
       if (!ok) *fail = 1;
       tc_commit(&sc.drain);  // nothing may be in flight when tensor memory is given back
       if (!mbar_wait(&sc.drain, 0)) *fail = 1;

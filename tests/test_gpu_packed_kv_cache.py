@@ -140,6 +140,7 @@ def check(L, cache, q, layer=0, **kw):
     assert torch.equal(cache.attention_mass(layer).double(), before)
     out2 = cache.attend(layer, q, accumulate=True, **kw)
     assert torch.equal(out2, out)
+    assert cache._layers[layer].state[-1].item() == 0  # no wait on the device ran out
     got = cache.attention_mass(layer).double() - before
     err = (got - m).abs()
     mb = mb + before.abs() * 2.0 ** -23 + m * 2.0 ** -23
