@@ -91,6 +91,7 @@ __device__ __forceinline__ void ld_codes(const uint8_t* p, uint32_t* w) {
 // Units of the sequences before b, and of all; every warp computes it for itself.
 __device__ __forceinline__ int units_before(const Attn& a, int b, int& all) {
   int before = 0, sum = 0;
+#pragma unroll 1
   for (int j = threadIdx.x & 31; j < a.kv.B; j += 32) {
     const int u = seq_of(a, j).count;
     sum += u;
@@ -103,6 +104,7 @@ __device__ __forceinline__ int units_before(const Attn& a, int b, int& all) {
 __device__ __forceinline__ int seq_at(const Attn& a, int x, int& begin) {
   const int lane = threadIdx.x & 31;
   begin = 0;
+#pragma unroll 1
   for (int b0 = 0; b0 < a.kv.B; b0 += 32) {
     const int own = b0 + lane < a.kv.B ? seq_of(a, b0 + lane).count * a.kv.H : 0;
     const int inc = warp_scan(own);

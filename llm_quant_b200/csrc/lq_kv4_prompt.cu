@@ -87,6 +87,7 @@ struct Walk {
     x0 += u1 - u0;
     if (x0 >= x1) return false;
     ++h;
+#pragma unroll 1
     while (h == a.kv.H || t.count == 0) {
       h = 0;
       ++j;
@@ -101,6 +102,7 @@ struct Walk {
 __device__ __forceinline__ int tiles_before(const Attn& a, int j, int& all) {
   const int rts = a.rows_pad / kItem;
   int before = 0, sum = 0;
+#pragma unroll 1
   for (int i = threadIdx.x & 31; i < a.kv.B * rts; i += 32) {
     const int u = tiles_of(a, i / rts, i % rts).count;
     sum += u;
@@ -119,6 +121,7 @@ __device__ __forceinline__ bool walk_begin(const Attn& a, int cta, Walk& w) {
   w.x0 = cut.begin(cta);
   w.x1 = cut.begin(cta + 1);
   int begin = 0;
+#pragma unroll 1
   for (int j0 = 0;; j0 += 32) {
     const int own = j0 + lane < a.kv.B * rts ? tiles_of(a, (j0 + lane) / rts, (j0 + lane) % rts).count * a.kv.H : 0;
     const int inc = warp_scan(own);
@@ -169,13 +172,39 @@ struct PromptShared {
   static constexpr int bytes = off_s + (int)sizeof(Scales) + 1024;  // and room to align
 };
 
-__device__ __forceinline__ void tc_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                          uint32_t accumulate) {
+// tcgen05.mma and tcgen05.commit by one elected lane of a converged warp
+__device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u)
+      : "memory");
+}
+// A bounded wait of a whole warp in few instructions (there are many, and the
+// instruction cache is small): up to 2^20 tries, each of which sleeps for up to
+// 10 us, so that it gives up after some seconds.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) {
+  bool ok = false;
+#pragma unroll 1
+  for (int i = 0; i < (1 << 20) && !ok; ++i) ok = mbar_try_sleep(bar, parity, 10000u);
+  return __all_sync(0xffffffffu, ok);
+}
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
       : "memory");
 }
 // tcgen05.wait::ld that the loaded registers pass through, so that no use of
@@ -205,6 +234,20 @@ __device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* r) {
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(addr)
       : "memory");
+}
+// with its wait
+__device__ __forceinline__ void tmem_ld8(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 __device__ __forceinline__ uint64_t pair(float x, float y) {
   uint64_t r;
@@ -263,6 +306,7 @@ __device__ __forceinline__ void ints_of(uint32_t w, uint32_t z, uint32_t* r) {
 template <typename T, int D>
 __device__ __forceinline__ void stage_rows(uint8_t* dst, const Attn& a, int b, int h, int cnt, int r0, int tid) {
   constexpr int CH = D / 8;
+#pragma unroll 4
   for (int idx = tid; idx < kTile * CH; idx += 128) {
     const int lr = idx / CH, c = idx % CH, r = r0 + lr, i = r / a.G;
     uint2 u = make_uint2(0u, 0u), v = u;
@@ -320,13 +364,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sc.tmem;
-  // A wait that runs out (2 s) ends the block: every role leaves its loop, as
+  // A wait that runs out ends the block: every role leaves its loop, as
   // every wait, this one's aside, is bounded too.  Whole warps agree on it.
   volatile int* fail = &sc.fail;
   auto gone = [&] { return __any_sync(0xffffffffu, *fail != 0); };
   // the k-th piece; its warp's lanes return the slot together
   auto next_piece = [&](int k) {
-    if (!mbar_wait_warp(&sc.piece_full[k % kPieces], (k / kPieces) & 1)) *fail = 1;
+    if (!wait_warp(&sc.piece_full[k % kPieces], (k / kPieces) & 1)) *fail = 1;
   };
   auto done_with = [&](int k) {
     __syncwarp();
@@ -355,6 +399,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
       const int r = r0 + tid, i = r / a.G;
       const bool valid = r < a.rows && i < w.cnt;
       const int at = w.first + i, n = w.n, n_steps = 2 * (w.u1 - w.u0), ordered = w.ordered;
+      const int first_tile = w.u0, pre_tiles = w.pre, gap = w.gap;
       stage_rows<T, D>(smem + L::off_q + wg * (L::kQ / 2), a, w.b, w.h, w.cnt, r0, tid);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(&sc.q_full[wg]);
@@ -362,32 +407,27 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
       const int pre = a.prefix ? a.prefix[w.b] : 0;
       // positions of the tile's first and last row
       const int qa = w.first + r0 / a.G, qb = w.first + (r0 + kTile - 1) / a.G;
+      // half tiles that begin in here need no masks
+      int plain_from = 0, plain_to = n - 64;
+      if (a.cap != 0.0f || a.slopes || (!ordered && (a.causal || a.window > 0))) plain_to = -1;
+      else {
+        if (a.causal) plain_to = min(plain_to, qa - 63);
+        if (a.window > 0) plain_from = max(qb - a.window + 1, 0);
+      }
       float R = kNone, l = 0.0f;
       for (int j = 0; j < n_steps; ++j, ++steps) {
-        const int st = (unit + (j >> 1)) % kScaleStages, t0 = w.token(w.u0 + (j >> 1)) + 64 * (j & 1);
+        const int st = (unit + (j >> 1)) % kScaleStages, u = first_tile + (j >> 1);
+        const int t0 = (u < pre_tiles ? u : u + gap) * kTok + 64 * (j & 1);
         const float* sk = sc.sk[st] + 64 * (j & 1);
         const float* sv = sc.sv[st] + 64 * (j & 1);
-        const bool plain = a.cap == 0.0f && !a.slopes && t0 + 64 <= n &&
-                           ((!a.causal && a.window <= 0) ||
-                            (ordered && (!a.causal || t0 + 63 <= qa) && (a.window <= 0 || qb - t0 < a.window)));
+        const bool plain = t0 >= plain_from && t0 <= plain_to;
         const uint32_t S = tmem + lanes + wg * 128 + 64 * (steps & 1);
-        if (!mbar_wait_warp(&sc.s_full[wg][steps & 1], (steps >> 1) & 1)) *fail = 1;
-        if (gone()) break;
+        if (!wait_warp(&sc.s_full[wg][steps & 1], (steps >> 1) & 1)) {
+          *fail = 1;
+          break;
+        }
         tc_fence_after();
         const float e = sc.e[st];
-        // products to scores (log2 units), with cap, bias and masks
-        auto masked = [&](uint32_t* y, int c) {
-#pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            float x = __uint_as_float(y[k]) * sk[c + k];
-            if (a.cap > 0.0f) x = tanh_exp(x) * (a.cap * kLog2e);
-            const int t = t0 + c + k, pos = ordered ? t : sc.pos[st][64 * (j & 1) + c + k], back = at - pos;
-            if (a.slopes) x = fmaf(-slope, fabsf((float)back), x);
-            bool near = !a.causal || back >= 0;
-            if (a.window > 0) near = near && back < a.window;
-            y[k] = __float_as_uint(valid && t < n && (near || pos < pre) ? x : -INFINITY);
-          }
-        };
         float sum = 0.0f;
         // Raises the row's reference to the greatest score m, and brings O to
         // it once the last PV is complete.
@@ -398,7 +438,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
           sum *= alpha;
           R = m;
           if (j > 0) {
-            if (!mbar_wait_warp(&sc.pv_done[wg][(steps - 1) & 1], ((steps - 1) >> 1) & 1)) *fail = 1;
+            if (!wait_warp(&sc.pv_done[wg][(steps - 1) & 1], ((steps - 1) >> 1) & 1)) *fail = 1;
             tc_fence_after();
             uint32_t z[16];
 #pragma unroll 1
@@ -413,82 +453,83 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
         };
         if (plain) {
           uint32_t y[64], p[32];
-          float top[2];
-          auto exponents = [&] {
-            const float off = e + kHead - R;
-            const uint64_t off2 = pair(off, off);
-            top[0] = top[1] = -INFINITY;
-#pragma unroll
-            for (int k = 0; k < 64; k += 4) {
-              const float4 f = *reinterpret_cast<const float4*>(sk + k);
-              const float2 y0 = unpair(fma2(pair(__uint_as_float(y[k]), __uint_as_float(y[k + 1])), pair(f.x, f.y), off2));
-              const float2 y1 = unpair(fma2(pair(__uint_as_float(y[k + 2]), __uint_as_float(y[k + 3])), pair(f.z, f.w), off2));
-              top[0] = fmaxf(top[0], fmaxf(y0.x, y0.y));
-              top[1] = fmaxf(top[1], fmaxf(y1.x, y1.y));
-              y[k] = __float_as_uint(ex2(y0.x)), y[k + 1] = __float_as_uint(ex2(y0.y));
-              y[k + 2] = __float_as_uint(ex2(y1.x)), y[k + 3] = __float_as_uint(ex2(y1.y));
-            }
-          };
-          tmem_ld32(S, y);
-          tmem_ld32(S + 32, y + 32);
-          tmem_wait_ld32(y);
-          tmem_wait_ld32(y + 32);
-          exponents();
-          if (__any_sync(0xffffffffu, fmaxf(top[0], top[1]) > kTop)) {
-            float m = -INFINITY;
+          // twice where the reference has to be raised first; one copy of the code
+#pragma unroll 1
+          for (int pass = 0; pass < 2; ++pass) {
             tmem_ld32(S, y);
             tmem_ld32(S + 32, y + 32);
             tmem_wait_ld32(y);
             tmem_wait_ld32(y + 32);
+            if (pass) {
+              float m = -INFINITY;
 #pragma unroll
-            for (int k = 0; k < 64; ++k) m = fmaxf(m, __uint_as_float(y[k]) * sk[k]);
-            raise(m);
-            exponents();
-          }
-          uint64_t s2[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
+              for (int k = 0; k < 64; ++k) m = fmaxf(m, __uint_as_float(y[k]) * sk[k]);
+              raise(m);
+            }
+            const float off = e + kHead - R;
+            const uint64_t off2 = pair(off, off);
+            float top[2] = {-INFINITY, -INFINITY};
+            uint64_t s2[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
+            // exponentials, sums and conversions in one block, so that the
+            // special-function unit is fed while the rest goes on
 #pragma unroll
-          for (int k = 0; k < 64; k += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(sv + k);
-            const uint64_t q0 = pair(__uint_as_float(y[k]), __uint_as_float(y[k + 1]));
-            const uint64_t q1 = pair(__uint_as_float(y[k + 2]), __uint_as_float(y[k + 3]));
-            s2[0] = add2(s2[0], q0);
-            s2[1] = add2(s2[1], q1);
-            const float2 p0 = unpair(mul2(q0, pair(v.x, v.y))), p1 = unpair(mul2(q1, pair(v.z, v.w)));
-            p[k / 2] = h2(p0.x, p0.y);
-            p[k / 2 + 1] = h2(p1.x, p1.y);
+            for (int k = 0; k < 64; k += 4) {
+              const float4 f = *reinterpret_cast<const float4*>(sk + k), v = *reinterpret_cast<const float4*>(sv + k);
+              const float2 y0 = unpair(fma2(pair(__uint_as_float(y[k]), __uint_as_float(y[k + 1])), pair(f.x, f.y), off2));
+              const float2 y1 = unpair(fma2(pair(__uint_as_float(y[k + 2]), __uint_as_float(y[k + 3])), pair(f.z, f.w), off2));
+              top[0] = fmaxf(top[0], fmaxf(y0.x, y0.y));
+              top[1] = fmaxf(top[1], fmaxf(y1.x, y1.y));
+              const uint64_t q0 = pair(ex2(y0.x), ex2(y0.y)), q1 = pair(ex2(y1.x), ex2(y1.y));
+              s2[0] = add2(s2[0], q0);
+              s2[1] = add2(s2[1], q1);
+              const float2 p0 = unpair(mul2(q0, pair(v.x, v.y))), p1 = unpair(mul2(q1, pair(v.z, v.w)));
+              p[k / 2] = h2(p0.x, p0.y);
+              p[k / 2 + 1] = h2(p1.x, p1.y);
+            }
+            const float2 x0 = unpair(s2[0]), x1 = unpair(s2[1]);
+            sum = (x0.x + x0.y) + (x1.x + x1.y);
+            if (!__any_sync(0xffffffffu, fmaxf(top[0], top[1]) > kTop)) break;
           }
           tmem_st16(S, p);  // P' lies over S
           tmem_st16(S + 16, p + 16);
-          const float2 x0 = unpair(s2[0]), x1 = unpair(s2[1]);
-          sum = (x0.x + x0.y) + (x1.x + x1.y);
         } else {
 #pragma unroll 1
-          for (int c = 0; c < 64; c += 32) {
-            uint32_t y[32], p[16];
-            tmem_ld32(S + c, y);
-            tmem_wait_ld32(y);
-            masked(y, c);
+          for (int c = 0; c < 64; c += 16) {
+            uint32_t y[16], p[8];
+            tmem_ld16(S + c, y);
+            tmem_wait_ld16(y);
             float m = -INFINITY;
 #pragma unroll
-            for (int k = 0; k < 32; ++k) m = fmaxf(m, __uint_as_float(y[k]));
+            for (int k = 0; k < 16; ++k) {
+              float x = __uint_as_float(y[k]) * sk[c + k];
+              if (a.cap > 0.0f) x = tanh_exp(x) * (a.cap * kLog2e);
+              const int t = t0 + c + k, pos = ordered ? t : sc.pos[st][64 * (j & 1) + c + k], back = at - pos;
+              if (a.slopes) x = fmaf(-slope, fabsf((float)back), x);
+              bool near = !a.causal || back >= 0;
+              if (a.window > 0) near = near && back < a.window;
+              x = valid && t < n && (near || pos < pre) ? x : -INFINITY;
+              y[k] = __float_as_uint(x);
+              m = fmaxf(m, x);
+            }
             if (__any_sync(0xffffffffu, m + (e + kHead - R) > kTop)) {
               const float before = R;
               raise(m);
-              if (c) {  // the first half's P' is there already
-                const __half2 alpha = __float2half2_rn(ex2(before - R));
-                tmem_ld16(S, p);
-                tmem_wait_ld16(p);
+              // what is there already of this half tile's P'
+              const __half2 alpha = __float2half2_rn(ex2(before - R));
+#pragma unroll 1
+              for (int d = 0; d < c / 2; d += 8) {
+                tmem_ld8(S + d, p);
 #pragma unroll
-                for (int k = 0; k < 16; ++k) {
+                for (int k = 0; k < 8; ++k) {
                   const __half2 v = __hmul2(*reinterpret_cast<__half2*>(&p[k]), alpha);
                   p[k] = *reinterpret_cast<const uint32_t*>(&v);
                 }
-                tmem_st16(S, p);
+                tmem_st8(S + d, p);
               }
             }
             const float off = e + kHead - R;
 #pragma unroll
-            for (int k = 0; k < 32; k += 2) {
+            for (int k = 0; k < 16; k += 2) {
               float q[2];
 #pragma unroll
               for (int d = 0; d < 2; ++d) {
@@ -499,7 +540,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
               }
               p[k / 2] = h2(q[0], q[1]);
             }
-            tmem_st16(S + c / 2, p);
+            tmem_st8(S + c / 2, p);
           }
         }
         l = fmaf(sum, ex2(-e - kHead), l);
@@ -511,7 +552,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
       unit += n_steps / 2;
       if (gone()) break;
       // ---- the item's rows, or this block's part of them ----
-      if (!mbar_wait_warp(&sc.pv_done[wg][(steps - 1) & 1], ((steps - 1) >> 1) & 1)) *fail = 1;
+      if (!wait_warp(&sc.pv_done[wg][(steps - 1) & 1], ((steps - 1) >> 1) & 1)) *fail = 1;
       if (gone()) break;
       tc_fence_after();
       if (w.whole) {
@@ -619,7 +660,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
         nu = sc.piece[nk % kPieces].u0;
       }
       const Piece& nx = sc.piece[nk % kPieces];
-      if (unit >= 2 && !mbar_wait_warp(&sc.k_empty[s2], ((unit >> 1) - 1) & 1)) *fail = 1;
+      if (unit >= 2 && !wait_warp(&sc.k_empty[s2], ((unit >> 1) - 1) & 1)) *fail = 1;
       if (gone()) break;
       // ---- K, and the columns' scales ----
       const uint32_t zk = (uint32_t)(int)par_zero(par.x) * 0x10001u + Ints<T>::bias;
@@ -637,7 +678,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
       reinterpret_cast<uint16_t*>(sc.zv[s2])[tid] = (uint16_t)((uint32_t)(int)par_zero(par.y) + 0x6400u);
       __syncwarp();
       if (lane == 0) mbar_arrive(&sc.t_full[s2]);
-      if (!mbar_wait_warp(&sc.t_full[s2], (unit >> 1) & 1)) *fail = 1;
+      if (!wait_warp(&sc.t_full[s2], (unit >> 1) & 1)) *fail = 1;
       if (gone()) break;
       const float big = fmaxf(fmaxf(sc.top[s2][0], sc.top[s2][1]), fmaxf(sc.top[s2][2], sc.top[s2][3]));
       const int e = big > 0.0f ? (int)(__float_as_uint(big) >> 23) - 126 : 0;  // big < 2^e
@@ -653,7 +694,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
       if (lane == 0) mbar_arrive(&sc.k_full[s2]);
       if (more) fetch_k(nx, nu);
       // ---- V^T ----
-      if (unit >= 2 && !mbar_wait_warp(&sc.v_empty[s2], ((unit >> 1) - 1) & 1)) *fail = 1;
+      if (unit >= 2 && !wait_warp(&sc.v_empty[s2], ((unit >> 1) - 1) & 1)) *fail = 1;
       if (gone()) break;
       const uint4 z = *reinterpret_cast<const uint4*>(&sc.zv[s2][4 * tg]);
       uint8_t* vd = smem + L::off_v + s2 * L::kV + (tg >> 3) * (D * 128);
@@ -686,7 +727,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
       Walk w;
       bool some = walk_begin(a, blockIdx.x, w);
       for (int k = 0;; ++k) {
-        if (k >= kPieces && !mbar_wait_warp(&sc.piece_empty[k % kPieces], ((k / kPieces) - 1) & 1)) *fail = 1;
+        if (k >= kPieces && !wait_warp(&sc.piece_empty[k % kPieces], ((k / kPieces) - 1) & 1)) *fail = 1;
         if (gone()) break;
         if (lane == 0) {
           Piece& p = sc.piece[k % kPieces];
@@ -703,74 +744,67 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
       }
     }
     // ---------------- MMA issuer ----------------
-    if (warp == kSoftmaxWarps + kCodeWarps && lane == 0) {
+    if (warp == kSoftmaxWarps + kCodeWarps) {
+      // The whole warp goes the way together and elects the lane that issues, so
+      // that descriptors and addresses are warp-uniform values.
       constexpr uint32_t idesc_s = make_idesc(Ints<T>::fmt, 64), idesc_o = make_idesc(0, D);
-      const uint32_t base = smem_u32(smem);
+      const uint32_t base = __reduce_max_sync(0xffffffffu, smem_u32(smem)), tm = __reduce_max_sync(0xffffffffu, tmem);
       int unit = 0, items[2] = {0, 0}, steps[2] = {0, 0};
-      // The loops are short: unrolled, the MMAs of a tile (and the code of the
-      // other roles) did not fit the instruction cache, and an MMA took 200
-      // cycles to issue instead of 64.
-      // S of half tile j of this piece; x: half tiles of row tile wg so far.  A
-      // step of 16 along K is 32 bytes of the swizzled rows, 64 are a half.
-      auto mma_s = [&](int wg, int j, int x) {
-        const uint64_t dq = sw128_desc(base + L::off_q + wg * (L::kQ / 2));
-        const uint64_t dk = sw128_desc(base + L::off_k + ((unit + (j >> 1)) & 1) * L::kK + (j & 1) * 8192);
-#pragma unroll 4
-        for (int k = 0; k < D / 16; ++k) {
-          const uint64_t step = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
-          tc_mma_ss(tmem + wg * 128 + 64 * (x & 1), dq + step, dk + step, idesc_s, k > 0);
-        }
-        tc_commit(&sc.s_full[wg][x & 1]);
-      };
       bool ok = true;
       for (int k = 0;; ++k) {
-        ok = mbar_wait(&sc.piece_full[k % kPieces], (k / kPieces) & 1);
+        ok = wait_warp(&sc.piece_full[k % kPieces], (k / kPieces) & 1);
         const Piece& w = sc.piece[k % kPieces];
         if (!ok || !w.some) break;
-        const int tiles = w.rt * kItem + kTile < a.rows ? 2 : 1, n_steps = 2 * (w.u1 - w.u0);
-        if (!mbar_wait(&sc.k_full[unit & 1], (unit >> 1) & 1)) { ok = false; break; }
-        for (int wg = 0; wg < tiles && ok; ++wg) {
-          ok = mbar_wait(&sc.q_full[wg], items[wg]++ & 1);
-          tc_fence_after();
-          if (ok) mma_s(wg, 0, steps[wg]);
-        }
-        for (int wg = 0; wg < tiles && ok; ++wg) mma_s(wg, 1, steps[wg] + 1);
-        if (!ok) break;
-        tc_commit(&sc.k_empty[unit & 1]);
+        const int two = __reduce_max_sync(0xffffffffu, w.rt * kItem + kTile < a.rows ? 1 : 0);
+        const int n_steps = 2 * __reduce_max_sync(0xffffffffu, w.u1 - w.u0);
+        // Slot i: PV of row tile i % 2, half tile i / 2, then S of the other row
+        // tile, which lies where the slot before last had its P' (the MMAs that
+        // read it are done by then).  The first three slots only have an S.  One
+        // copy of the code and short loops: unrolled, it did not fit the
+        // instruction cache, and an MMA took 200 cycles to issue instead of 64.
 #pragma unroll 1
-        for (int j = 0; j < n_steps && ok; ++j) {
-          const int u = unit + (j >> 1), un = unit + ((j + 2) >> 1);
-          const bool more = j + 2 < n_steps;
-          if (!(j & 1) && ((more && !mbar_wait(&sc.k_full[un & 1], (un >> 1) & 1)) || !mbar_wait(&sc.v_full[u & 1], (u >> 1) & 1))) {
-            ok = false;
-            break;
-          }
-#pragma unroll 1
-          for (int wg = 0; wg < tiles; ++wg) {
-            if (!mbar_wait(&sc.p_full[wg][steps[wg] & 1], (steps[wg] >> 1) & 1)) { ok = false; break; }
+        for (int i = -3; i < 2 * n_steps; ++i) {
+          const int wg = i & 1, j = i >> 1, u = unit + (j >> 1);
+          if (i >= 0 && (!wg || two)) {
+            const int x = steps[wg] + j;
+            if (!wg && !(j & 1)) ok = wait_warp(&sc.v_full[u & 1], (u >> 1) & 1);
+            if (!ok || !wait_warp(&sc.p_full[wg][x & 1], (x >> 1) & 1)) { ok = false; break; }
             tc_fence_after();
             const uint64_t dv = sw128_desc(base + L::off_v + (u & 1) * L::kV + (j & 1) * (D * 128));
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              tc_mma(tmem + 256 + wg * 128, tmem + wg * 128 + 64 * (steps[wg] & 1) + 8 * k, dv + ((k * 32) >> 4), idesc_o,
-                     j > 0 || k > 0);
-            tc_commit(&sc.pv_done[wg][steps[wg] & 1]);
-            if (more) mma_s(wg, j + 2, steps[wg] + 2);
-            ++steps[wg];
+              mma_ts(tm + 256 + wg * 128, tm + wg * 128 + 64 * (x & 1) + 8 * k, dv + ((k * 32) >> 4), idesc_o, j > 0 || k > 0);
+            commit(&sc.pv_done[wg][x & 1]);
+            if ((j & 1) && wg == two) commit(&sc.v_empty[u & 1]);
           }
-          if (!ok) break;
-          if (j & 1) {
-            tc_commit(&sc.v_empty[u & 1]);
-            if (more) tc_commit(&sc.k_empty[un & 1]);
+          const int sg = wg ^ 1, sj = j + 1 + wg, su = unit + (sj >> 1);
+          if (sj < n_steps && (!sg || two)) {
+            const int x = steps[sg] + sj;
+            if (!sg && !(sj & 1)) ok = wait_warp(&sc.k_full[su & 1], (su >> 1) & 1);
+            if (sj == 0) ok = ok && wait_warp(&sc.q_full[sg], items[sg]++ & 1);
+            if (!ok) break;
+            tc_fence_after();
+            // a step of 16 along K is 32 bytes of the swizzled rows, 64 are a half
+            const uint64_t dq = sw128_desc(base + L::off_q + sg * (L::kQ / 2));
+            const uint64_t dk = sw128_desc(base + L::off_k + (su & 1) * L::kK + (sj & 1) * 8192);
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+              const uint64_t step = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
+              mma_ss(tm + sg * 128 + 64 * (x & 1), dq + step, dk + step, idesc_s, k > 0);
+            }
+            commit(&sc.s_full[sg][x & 1]);
+            if ((sj & 1) && sg == two) commit(&sc.k_empty[su & 1]);
           }
         }
         if (!ok) break;
+        steps[0] += n_steps;
+        if (two) steps[1] += n_steps;
         unit += n_steps / 2;
-        mbar_arrive(&sc.piece_empty[k % kPieces]);
+        done_with(k);
       }
       if (!ok) *fail = 1;
-      tc_commit(&sc.drain);  // nothing may be in flight when tensor memory is given back
-      if (!mbar_wait(&sc.drain, 0)) *fail = 1;
+      commit(&sc.drain);  // nothing may be in flight when tensor memory is given back
+      if (!wait_warp(&sc.drain, 0)) *fail = 1;
     }
     __syncwarp();
   }
@@ -804,7 +838,7 @@ __global__ void __launch_bounds__(128) kv4_prompt_combine_kernel(const Attn a) {
   const int c0 = t.count ? cut.owner(begin) : 0, c1 = t.count ? cut.owner(begin + t.count - 1) : -1;
   if (t.count && c0 == c1) return;
   pdl_wait();
-#pragma unroll
+#pragma unroll 1
   for (int k = k0 + warp; k < k0 + kMergeRows; k += 4) {
     const int r = rt * kItem + k;
     if (r >= a.rows) break;
