@@ -800,10 +800,7 @@ extern "C" int lq_kv4_attention(const lq_kv4_cache* cache, const lq_kv4_attn* f,
   const bool gen = (f->Sq > 1 && (f->causal || counts)) || f->softcap > 0.0f || slopes || f->window > 0;
   cudaStream_t st = as_stream(stream);
   if (p.prompt) {
-    LQ_TRY(kv4_prompt(a, st));
-    if (!a.lse) return LQ_OK;
-    if (kv.D == 128) return gen ? run_mass<128, false, true>(a, st) : run_mass<128, false, false>(a, st);
-    return gen ? run_mass<64, false, true>(a, st) : run_mass<64, false, false>(a, st);
+    return kv4_prompt(a, st);
   }
   return kv.D == 128 ? run_attn_d<128>(a, p, gen, st) : run_attn_d<64>(a, p, gen, st);
 }

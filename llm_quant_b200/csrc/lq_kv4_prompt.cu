@@ -28,6 +28,8 @@
 // Split: as in lq_kv4_attn.cu, the (row tile, token tile) pairs that have
 // anything to see lie in one row and each block takes an equal stretch;
 // kv4_prompt_combine_kernel merges row tiles that were cut.
+#include <algorithm>
+
 #include "lq_kv4_attn.cuh"
 #include "lq_tc.cuh"
 
@@ -875,6 +877,268 @@ __global__ void __launch_bounds__(128) kv4_prompt_combine_kernel(const Attn a) {
   }
 }
 
+// ---------------------------------------------------------------------------
+// Collected weight: mass[t] += sum over the rows of exp2(x[r, t] - lse[r]).
+//   S^T = (C_k - Z_k) Q^T: 128 tokens (lanes) by 128 rows (columns)
+// so that a thread owns a token: it multiplies by its own scale, subtracts the
+// rows' log2 denominators and adds up what it has, in a fixed order and with no
+// exchange but one at the end between the two groups that take alternate row
+// tiles.  A block takes 128 tokens of a head at a time; heads' first tokens come
+// first, as with a causal mask they have the most rows.
+//
+// Warps: 0-3 and 4-7 sums of even and odd row tiles, 8-11 K's codes and the
+// query rows to operands, 12 the MMAs.  Bound: 16384 exponentials to a pair of
+// tiles, 1024 cycles, beside 512 of the tensor cores.
+// ---------------------------------------------------------------------------
+constexpr int kWeighThreads = 416;
+template <int D>
+struct WeighShared {
+  static constexpr int kOp = D / 64 * 16384;  // an operand of 128 rows
+  static constexpr int off_k = 0, off_q = kOp, off_s = off_q + 2 * kOp;
+  struct Rows {
+    float nl[4][kTile], slope[4][kTile];  // -lse, bias
+    int at[4][kTile];
+    float sk[2][kTok], half[2][kTok];
+    int pos[2][kTok];
+    uint64_t k_full, k_empty, q_full[2], q_empty[2], s_full[2], s_empty[2], half_full[2], drain;
+    uint32_t tmem;
+    int fail;
+  };
+  static constexpr int bytes = off_s + (int)sizeof(Rows) + 1024;
+};
+// Tokens t0 .. of head bh, and the row tiles [lo, hi) that may see any of them.
+struct WeighItem {
+  int b, h, t0, n, cnt, first, ordered, lo, hi;
+};
+__device__ __forceinline__ WeighItem weigh_item(const Attn& a, int idx) {
+  WeighItem w;
+  const int heads = a.kv.B * a.kv.H, bh = idx % heads;
+  w.b = bh / a.kv.H, w.h = bh % a.kv.H, w.t0 = idx / heads * kTok;
+  const Seq s = seq_of(a, w.b);
+  w.n = s.n, w.cnt = s.cnt, w.first = s.first, w.ordered = s.ordered;
+  w.lo = 0, w.hi = w.t0 < s.n ? (s.cnt * a.G + kTile - 1) / kTile : 0;
+  if (s.ordered && !(a.prefix && w.t0 < a.prefix[w.b])) {
+    if (a.causal) w.lo = (int)((int64_t)max(w.t0 - s.first, 0) * a.G / kTile);
+    if (a.window > 0) {
+      const int64_t i = (int64_t)w.t0 + kTok - 1 + a.window - s.first;  // queries from here on are past the window
+      w.hi = (int)min((int64_t)w.hi, i <= 0 ? 0 : (i * a.G + kTile - 1) / kTile);
+    }
+  }
+  return w;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kWeighThreads, 1) kv4_weigh_kernel(const Attn a, int items) {
+  using L = WeighShared<D>;
+  constexpr int W = D / 32;
+  extern __shared__ __align__(16) uint8_t raw[];
+  uint8_t* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+  typename L::Rows& sc = *reinterpret_cast<typename L::Rows*>(smem + L::off_s);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    sc.fail = 0;
+    mbar_init(&sc.k_full, 4);
+    mbar_init(&sc.k_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sc.q_full[i], 4);
+      mbar_init(&sc.q_empty[i], 1);
+      mbar_init(&sc.s_full[i], 1);
+      mbar_init(&sc.s_empty[i], 4);
+      mbar_init(&sc.half_full[i], 4);
+    }
+    mbar_init(&sc.drain, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sc.tmem)), "r"(256u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sc.tmem;
+  volatile int* fail = &sc.fail;
+  const float fk = a.sm * (a.cap > 0.0f ? 1.0f / a.cap : kLog2e);
+
+  if (warp < 8) {
+    const int wg = warp >> 2, tid = threadIdx.x & 127;
+    const uint32_t S = tmem + ((uint32_t)((warp & 3) * 32) << 16) + wg * 128;
+    int tile = 0, mine = 0, item = 0;  // row tiles so far, of this group, items with any
+    bool ok = true;
+    for (int idx = blockIdx.x; idx < items && ok; idx += gridDim.x) {
+      const WeighItem w = weigh_item(a, idx);
+      if (w.lo >= w.hi) continue;
+      const int t = w.t0 + tid, pre = a.prefix ? a.prefix[w.b] : 0, odd = (tile + wg) & 1;
+      float sum = 0.0f, sk = 0.0f;
+      int pos = t;
+      for (int rt = w.lo + odd; rt < w.hi; rt += 2, ++mine) {
+        const int st = (tile + rt - w.lo) & 3;
+        if (!wait_warp(&sc.s_full[wg], mine & 1)) { ok = false; break; }
+        tc_fence_after();
+        sk = sc.sk[item & 1][tid];
+        if (!w.ordered) pos = sc.pos[item & 1][tid];
+        const int q0 = w.first + rt * kTile / a.G, q1 = w.first + min((rt * kTile + kTile - 1) / a.G, w.cnt - 1);
+        const bool plain = a.cap == 0.0f && !a.slopes &&
+                           ((!a.causal && a.window <= 0) ||
+                            (w.ordered && (!a.causal || w.t0 + kTok - 1 <= q0) && (a.window <= 0 || q1 - w.t0 < a.window)));
+        if (plain) {
+          uint64_t s2[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
+          const uint64_t k2 = pair(sk, sk);
+#pragma unroll 1
+          for (int c = 0; c < kTile; c += 64) {
+            uint32_t y[64];
+            tmem_ld32(S + c, y);
+            tmem_ld32(S + c + 32, y + 32);
+            tmem_wait_ld32(y);
+            tmem_wait_ld32(y + 32);
+#pragma unroll
+            for (int k = 0; k < 64; k += 4) {
+              const float4 f = *reinterpret_cast<const float4*>(&sc.nl[st][c + k]);
+              const float2 y0 = unpair(fma2(pair(__uint_as_float(y[k]), __uint_as_float(y[k + 1])), k2, pair(f.x, f.y)));
+              const float2 y1 = unpair(fma2(pair(__uint_as_float(y[k + 2]), __uint_as_float(y[k + 3])), k2, pair(f.z, f.w)));
+              s2[0] = add2(s2[0], pair(ex2(y0.x), ex2(y0.y)));
+              s2[1] = add2(s2[1], pair(ex2(y1.x), ex2(y1.y)));
+            }
+          }
+          const float2 x0 = unpair(s2[0]), x1 = unpair(s2[1]);
+          sum += (x0.x + x0.y) + (x1.x + x1.y);
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < kTile; c += 16) {
+            uint32_t y[16];
+            tmem_ld16(S + c, y);
+            tmem_wait_ld16(y);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              float x = __uint_as_float(y[k]) * sk;
+              if (a.cap > 0.0f) x = tanh_exp(x) * (a.cap * kLog2e);
+              const int back = sc.at[st][c + k] - pos;
+              if (a.slopes) x = fmaf(-sc.slope[st][c + k], fabsf((float)back), x);
+              bool near = !a.causal || back >= 0;
+              if (a.window > 0) near = near && back < a.window;
+              const float p = ex2(x + sc.nl[st][c + k]);
+              if (near || pos < pre) sum += p;
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sc.s_empty[wg]);
+      }
+      if (!ok) break;
+      // the groups' sums, and what the token had
+      if (wg == 1) {
+        sc.half[item & 1][tid] = sum;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sc.half_full[item & 1]);
+      } else {
+        if (!wait_warp(&sc.half_full[item & 1], (item >> 1) & 1)) { ok = false; break; }
+        if (t < w.n) a.kv.mass[(int64_t)(w.b * a.kv.H + w.h) * a.kv.cap + t] += sum + sc.half[item & 1][tid];
+      }
+      ++item;
+      tile += w.hi - w.lo;
+    }
+    if (!ok) *fail = 1;
+  } else if (warp < 12) {
+    const int tid = threadIdx.x - 256;
+    int tile = 0, item = 0;
+    bool ok = true;
+    for (int idx = blockIdx.x; idx < items && ok; idx += gridDim.x) {
+      const WeighItem w = weigh_item(a, idx);
+      if (w.lo >= w.hi) continue;
+      // ---- K ----
+      const int t = w.t0 + tid;
+      const int64_t row = (int64_t)(w.b * a.kv.H + w.h) * a.kv.cap + t;
+      const bool in = t < w.n;
+      const uint32_t par = in ? a.kv.par[row].x : 0u;
+      if (item > 0 && !wait_warp(&sc.k_empty, (item - 1) & 1)) { ok = false; break; }
+      const uint32_t zk = (uint32_t)(int)par_zero(par) * 0x10001u + Ints<T>::bias;
+      uint8_t* kd = smem + L::off_k + tid * 128;
+#pragma unroll 2
+      for (int i = 0; i < 4 * W; i += 2) {
+        const uint2 v = in ? __ldg(reinterpret_cast<const uint2*>(a.kv.k + row * (D / 2)) + i / 2) : make_uint2(0u, 0u);
+        uint32_t r[4];
+        ints_of<T>(v.x, zk, r);
+        *reinterpret_cast<uint4*>(kd + (i / 8) * 16384 + (((i % 8) ^ (tid & 7)) << 4)) = make_uint4(r[0], r[1], r[2], r[3]);
+        ints_of<T>(v.y, zk, r);
+        *reinterpret_cast<uint4*>(kd + (i / 8) * 16384 + (((i % 8 + 1) ^ (tid & 7)) << 4)) = make_uint4(r[0], r[1], r[2], r[3]);
+      }
+      sc.sk[item & 1][tid] = par_scale(par) * fk;
+      if (!w.ordered) sc.pos[item & 1][tid] = in ? a.kv.pos[row] : 0;
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sc.k_full);
+      // ---- query rows ----
+      for (int rt = w.lo; rt < w.hi; ++rt, ++tile) {
+        const int s2 = tile & 1, st = tile & 3;
+        if (tile >= 2 && !wait_warp(&sc.q_empty[s2], ((tile >> 1) - 1) & 1)) { ok = false; break; }
+        const int r = rt * kTile + tid, i = r / a.G;
+        sc.nl[st][tid] = r < a.rows && i < w.cnt ? -a.lse[(int64_t)(w.b * a.kv.H + w.h) * a.rows_pad + r] : -INFINITY;
+        sc.at[st][tid] = w.first + i;
+        sc.slope[st][tid] = a.slopes && r < a.rows ? a.slopes[w.h * a.G + r % a.G] * kLog2e : 0.0f;
+        stage_rows<T, D>(smem + L::off_q + s2 * L::kOp, a, w.b, w.h, w.cnt, rt * kTile, tid);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sc.q_full[s2]);
+      }
+      ++item;
+    }
+    if (!ok) *fail = 1;
+  } else {
+    constexpr uint32_t idesc = make_idesc(Ints<T>::fmt, kTile);
+    const uint32_t base = __reduce_max_sync(0xffffffffu, smem_u32(smem)), tm = __reduce_max_sync(0xffffffffu, tmem);
+    int tile = 0, item = 0, used[2] = {0, 0};
+    bool ok = true;
+    for (int idx = blockIdx.x; idx < items && ok; idx += gridDim.x) {
+      const WeighItem w = weigh_item(a, idx);
+      const int tiles = __reduce_max_sync(0xffffffffu, max(w.hi - w.lo, 0));
+      if (tiles == 0) continue;
+      if (!wait_warp(&sc.k_full, item & 1)) { ok = false; break; }
+      // row tile `tile` goes to group tile % 2, whichever item it is of
+#pragma unroll 1
+      for (int i = 0; i < tiles; ++i, ++tile) {
+        const int s2 = tile & 1, wg = s2;
+        if (!wait_warp(&sc.q_full[s2], (tile >> 1) & 1)) { ok = false; break; }
+        if (used[wg] > 0 && !wait_warp(&sc.s_empty[wg], (used[wg] - 1) & 1)) { ok = false; break; }
+        ++used[wg];
+        tc_fence_after();
+        const uint64_t dk = sw128_desc(base + L::off_k), dq = sw128_desc(base + L::off_q + s2 * L::kOp);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint64_t step = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
+          mma_ss(tm + wg * 128, dk + step, dq + step, idesc, k > 0);
+        }
+        commit(&sc.s_full[wg]);
+        commit(&sc.q_empty[s2]);
+      }
+      commit(&sc.k_empty);
+      ++item;
+    }
+    if (!ok) *fail = 1;
+    commit(&sc.drain);
+    if (!wait_warp(&sc.drain, 0)) *fail = 1;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (threadIdx.x == 0 && *fail) a.kv.sync[3] = LQ_ETIMEOUT;
+  if (warp == 12)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u));
+}
+
+template <typename T, int D>
+int run_weigh(const Attn& a, cudaStream_t st) {
+  constexpr int smem = WeighShared<D>::bytes;
+  auto kern = kv4_weigh_kernel<T, D>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return launched("kv4_weigh_kernel (attribute)");
+  const int64_t items = (int64_t)((a.kv.cap + kTok - 1) / kTok) * a.kv.B * a.kv.H;
+  LQ_REQUIRE(items <= INT32_MAX, LQ_ERANGE, "cache too large to collect weights");
+  kern<<<(int)std::min<int64_t>(items, num_sms()), kWeighThreads, smem, st>>>(a, (int)items);
+  return launched("kv4_weigh_kernel");
+}
+
 template <typename T, int D>
 int run_prompt(const Attn& a, cudaStream_t st) {
   constexpr int smem = PromptShared<D>::bytes;
@@ -885,7 +1149,8 @@ int run_prompt(const Attn& a, cudaStream_t st) {
   kern<<<a.blocks, kPromptThreads, smem, st>>>(a);
   LQ_TRY(launched("kv4_prompt_kernel"));
   launch_pdl(kv4_prompt_combine_kernel<D>, dim3((unsigned)(a.rows_pad / kMergeRows * a.kv.B * a.kv.H)), dim3(128), 0, st, a);
-  return launched("kv4_prompt_combine_kernel");
+  LQ_TRY(launched("kv4_prompt_combine_kernel"));
+  return a.lse ? run_weigh<T, D>(a, st) : LQ_OK;
 }
 
 }  // namespace
