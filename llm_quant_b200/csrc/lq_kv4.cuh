@@ -7,8 +7,9 @@
 // become fp32 with one shift or mask.  The words of K and V of a token lie
 // side by side (uint2), [B, H, cap].
 //
-// K codes [B, H, cap, D / 2]: natural order, value d in nibble d % 8 (bits
-// 4 (d % 8) ..) of 32-bit word d / 8 of the token's row.
+// K codes [B, H, cap, D / 2]: value d in 32-bit word d / 8 of the token's row,
+// nibble (d % 8) / 2 of its low half for even d and of its high half for odd d:
+// a mask (after a shift by whole nibbles) leaves two neighbouring values.
 //
 // V codes [B, H, cap / 16, 8 D]: tiles of 16 tokens, laid out as the A
 // fragments of mma.m16n8k16 for O^T = V^T P^T: the 16-bit unit u of token t

@@ -124,7 +124,7 @@ __device__ __forceinline__ int seq_at(const Attn& a, int x, int& begin) {
 template <int D, int NQ, bool QLO>
 struct RowsShared {
   static constexpr int NW = D / 8;  // words of a row
-  uint4 hi[8 * NQ][NW];             // nibble pairs (0, 4), (2, 6), (1, 5), (3, 7) of each word
+  uint4 hi[8 * NQ][NW];             // values (0, 1), (4, 5), (2, 3), (6, 7) of each word
   uint4 lo[QLO ? 8 * NQ : 1][QLO ? NW : 1];
   float sum[8 * NQ], fac[8 * NQ];
 };
@@ -163,9 +163,9 @@ struct Rows {
       const float f = __uint_as_float((uint32_t)up << 23);
       uint32_t p[4], q[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {  // register k: nibbles (n, n + 4), n = 0, 2, 1, 3
+      for (int k = 0; k < 4; ++k) {  // register k: nibble n of both halves, n = 0, 2, 1, 3
         const int n = k < 2 ? 2 * k : 2 * k - 3;
-        const float u = x[n] * f, v = x[n + 4] * f;
+        const float u = x[2 * n] * f, v = x[2 * n + 1] * f;
         p[k] = h2(u, v);
         if constexpr (QLO) {
           const float2 y = f2(p[k]);
@@ -769,7 +769,7 @@ extern "C" int lq_kv4_attention(const lq_kv4_cache* cache, const lq_kv4_attn* f,
   LQ_REQUIRE(f->window >= 0 && f->window <= INT32_MAX, LQ_EINVAL, "bad window");
   const int64_t rows = f->Hq / cache->H * f->Sq;
   if (rows == 0) return LQ_OK;
-  LQ_REQUIRE(rows <= 16 * 65535 && rows * cache->B * cache->H <= INT32_MAX, LQ_ERANGE, "too many query rows");
+  LQ_REQUIRE(f->Hq / cache->H <= 4096 && rows <= 16 * 65535 && rows * cache->B * cache->H <= INT32_MAX, LQ_ERANGE, "too many query rows");
   LQ_REQUIRE(q && out, LQ_EINVAL, "NULL pointer");
   LQ_REQUIRE((uintptr_t)q % (4 * dtype_size(f->q_dtype)) == 0 && ((f->q_sb | f->q_sh | f->q_ss) & 3) == 0, LQ_EALIGN,
              "query rows must start on multiples of 4 elements");
@@ -790,6 +790,8 @@ extern "C" int lq_kv4_attention(const lq_kv4_cache* cache, const lq_kv4_attn* f,
   a.sm = f->sm_scale, a.cap = f->softcap;
   a.slopes = slopes, a.prefix = prefix;
   a.causal = f->causal != 0, a.window = (int)f->window;
+  a.g_mul = a.G == 1 ? 0u : (uint32_t)(0x100000000ull / a.G) + 1u;
+  a.q_wide = (uintptr_t)q % 16 == 0 && ((f->q_sb | f->q_sh | f->q_ss) * dtype_size(f->q_dtype)) % 16 == 0;
   a.blocks = p.blocks;
   a.out = static_cast<uint8_t*>(out);
   uint8_t* ws = static_cast<uint8_t*>(workspace);

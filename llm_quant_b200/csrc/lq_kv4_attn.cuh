@@ -18,6 +18,8 @@ struct Attn {
   const float* slopes;
   const int32_t* prefix;
   int causal, window;
+  uint32_t g_mul; // ceil(2^32 / G), 0 for G = 1
+  int q_wide;     // query rows start on multiples of 16 bytes
   int blocks;     // blocks of the split (at most; never more than there are units)
   uint8_t* out;
   float* part;    // [blocks + B H][rows_pad][D] unnormalised O
@@ -33,6 +35,9 @@ int kv4_prompt(const Attn& a, cudaStream_t st);
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+
+// r / G of a row: exact for r G < 2^32 (rows are fewer than 2^20, G at most 4096)
+__device__ __forceinline__ int div_g(const Attn& a, int r) { return a.g_mul ? (int)__umulhi((uint32_t)r, a.g_mul) : r; }
 
 __device__ __forceinline__ float ex2(float x) {
   float y;

@@ -296,31 +296,42 @@ template <> struct Ints<__nv_bfloat16> {
     return *reinterpret_cast<uint32_t*>(&h);
   }
 };
-// The 8 values of a word: pairs (0, 4), (1, 5), (2, 6), (3, 7) less their zero points z.
+// The 8 values of a word of K (or 4 of two tokens of V) less their zero points z.
 template <typename T>
 __device__ __forceinline__ void ints_of(uint32_t w, uint32_t z, uint32_t* r) {
 #pragma unroll
   for (int n = 0; n < 4; ++n) r[n] = Ints<T>::sub(((w >> (4 * n)) & 0x000f000fu) | Ints<T>::bias, z);
 }
 
-// A tile of 128 query rows into shared memory as a K-major, 128-byte-swizzled
-// operand, the 8 values of a chunk in the order of ints_of.  128 threads.
+// A tile of 128 query rows on its way into shared memory as a K-major,
+// 128-byte-swizzled operand; zeros for what is no row.  128 threads; each waits
+// for its own copies with staged().
 template <typename T, int D>
 __device__ __forceinline__ void stage_rows(uint8_t* dst, const Attn& a, int b, int h, int cnt, int r0, int tid) {
-  constexpr int CH = D / 8;
+  constexpr int CH = D / 8, STEP = 128 / CH;
+  const int c = tid % CH;
+  const T* q = reinterpret_cast<const T*>(a.q) + b * a.q_sb + 8 * c;
+  const uint32_t to = smem_u32(dst) + (c / 8) * 16384;
 #pragma unroll 4
-  for (int idx = tid; idx < kTile * CH; idx += 128) {
-    const int lr = idx / CH, c = idx % CH, r = r0 + lr, i = r / a.G;
-    uint2 u = make_uint2(0u, 0u), v = u;
-    if (r < a.rows && i < cnt) {
-      const T* p = reinterpret_cast<const T*>(a.q) + b * a.q_sb + (int64_t)(h * a.G + r % a.G) * a.q_sh + i * a.q_ss + 8 * c;
-      u = __ldg(reinterpret_cast<const uint2*>(p));
-      v = __ldg(reinterpret_cast<const uint2*>(p) + 1);
+  for (int lr = tid / CH; lr < kTile; lr += STEP) {
+    const int r = r0 + lr, i = div_g(a, r), g = r - i * a.G;
+    const bool in = r < a.rows && i < cnt;
+    const T* p = in ? q + (int64_t)(h * a.G + g) * a.q_sh + i * a.q_ss : q;
+    const uint32_t at = to + lr * 128 + (((c % 8) ^ (lr & 7)) << 4);
+    const int bytes = in ? 16 : 0;  // the rest is filled with zeros
+    if (a.q_wide) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(p), "r"(bytes) : "memory");
+    } else {
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(at), "l"(p), "r"(bytes / 2) : "memory");
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(at + 8), "l"(p + 4), "r"(bytes / 2) : "memory");
     }
-    const uint4 w = make_uint4(__byte_perm(u.x, v.x, 0x5410), __byte_perm(u.x, v.x, 0x7632),
-                               __byte_perm(u.y, v.y, 0x5410), __byte_perm(u.y, v.y, 0x7632));
-    *reinterpret_cast<uint4*>(dst + (c / 8) * 16384 + lr * 128 + (((c % 8) ^ (lr & 7)) << 4)) = w;
   }
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>  // all but the last N tiles are there, for the MMAs too
+__device__ __forceinline__ void staged() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
 template <typename T, int D>
@@ -403,7 +414,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
       const int at = w.first + i, n = w.n, n_steps = 2 * (w.u1 - w.u0), ordered = w.ordered;
       const int first_tile = w.u0, pre_tiles = w.pre, gap = w.gap;
       stage_rows<T, D>(smem + L::off_q + wg * (L::kQ / 2), a, w.b, w.h, w.cnt, r0, tid);
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      staged<0>();
       mbar_arrive(&sc.q_full[wg]);
       const float slope = a.slopes && r < a.rows ? a.slopes[w.h * a.G + r % a.G] * kLog2e : 0.0f;
       const int pre = a.prefix ? a.prefix[w.b] : 0;
@@ -1069,19 +1080,25 @@ __global__ void __launch_bounds__(kWeighThreads, 1) kv4_weigh_kernel(const Attn 
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(&sc.k_full);
-      // ---- query rows ----
+      // ---- query rows, the next tile on its way while this one arrives ----
       for (int rt = w.lo; rt < w.hi; ++rt, ++tile) {
         const int s2 = tile & 1, st = tile & 3;
         if (tile >= 2 && !wait_warp(&sc.q_empty[s2], ((tile >> 1) - 1) & 1)) { ok = false; break; }
-        const int r = rt * kTile + tid, i = r / a.G;
+        stage_rows<T, D>(smem + L::off_q + s2 * L::kOp, a, w.b, w.h, w.cnt, rt * kTile, tid);
+        const int r = rt * kTile + tid, i = div_g(a, r);
         sc.nl[st][tid] = r < a.rows && i < w.cnt ? -a.lse[(int64_t)(w.b * a.kv.H + w.h) * a.rows_pad + r] : -INFINITY;
         sc.at[st][tid] = w.first + i;
-        sc.slope[st][tid] = a.slopes && r < a.rows ? a.slopes[w.h * a.G + r % a.G] * kLog2e : 0.0f;
-        stage_rows<T, D>(smem + L::off_q + s2 * L::kOp, a, w.b, w.h, w.cnt, rt * kTile, tid);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sc.q_full[s2]);
+        sc.slope[st][tid] = a.slopes && r < a.rows ? a.slopes[w.h * a.G + r - i * a.G] * kLog2e : 0.0f;
+        if (rt > w.lo) {
+          staged<1>();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sc.q_full[s2 ^ 1]);
+        }
       }
+      if (!ok) break;
+      staged<0>();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sc.q_full[(tile - 1) & 1]);
       ++item;
     }
     if (!ok) *fail = 1;

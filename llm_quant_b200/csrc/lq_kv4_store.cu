@@ -91,9 +91,12 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4 kv, AppendArgs a) {
     if (live) load4(static_cast<const T*>(a.x[s]) + b * a.sb[s] + h * a.sh[s] + i * a.ss[s] + 4 * l, x);
     w[s] = quant4<LPT>(x, par[s]);
   }
+  // two lanes make a word of K: even values in its low half, odd ones in its high half
+  uint32_t kw = ((w[0] & 0xf) | ((w[0] >> 4) & 0xf0) | ((w[0] << 12) & 0xf0000) | ((w[0] << 8) & 0xf00000)) << (8 * (l & 1));
+  kw |= __shfl_xor_sync(0xffffffffu, kw, 1);
   if (live) {
     const int64_t row = (int64_t)bh * kv.cap;
-    *reinterpret_cast<uint16_t*>(kv.k + (row + t) * (D / 2) + 2 * l) = (uint16_t)w[0];
+    if (!(l & 1)) *reinterpret_cast<uint32_t*>(kv.k + (row + t) * (D / 2) + 2 * l) = kw;
     *reinterpret_cast<uint16_t*>(kv.v + row * (D / 2) + v_unit(t, l, W)) = (uint16_t)w[1];
     if (l == 0) {
       kv.par[row + t] = make_uint2(par[0], par[1]);
@@ -148,7 +151,7 @@ __global__ void __launch_bounds__(256) kv4_dequant_kernel(Kv4 kv, int n, T* ko, 
         float x[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          x[j] = t < len ? __fmul_rn((float)((p[i] >> (4 * j)) & 15) - par_zero(par), par_scale(par)) : 0.0f;
+          x[j] = t < len ? __fmul_rn((float)((p[i] >> (4 * (j >> 1) + 16 * (j & 1))) & 15) - par_zero(par), par_scale(par)) : 0.0f;
         store_n<T, 8>(ko + (bh * n + t) * D + (c * W + i) * 8, x);
       }
     }
