@@ -58,7 +58,7 @@ struct Tiles {
 __device__ __forceinline__ Tiles tiles_of(const Attn& a, int b, int rt) {
   const Seq s = seq_of(a, b);
   Tiles t{s.n, s.cnt, s.first, s.ordered, 0, 0, 0};
-  const int i0 = rt * kItem / a.G, i1 = min((rt * kItem + kItem - 1) / a.G, s.cnt - 1);
+  const int i0 = div_g(a, rt * kItem), i1 = min(div_g(a, rt * kItem + kItem - 1), s.cnt - 1);
   if (i0 >= s.cnt || s.n == 0) return t;
   int lo = 0, hi = s.n, pre = 0;
   if (s.ordered) {
@@ -308,23 +308,28 @@ __device__ __forceinline__ void ints_of(uint32_t w, uint32_t z, uint32_t* r) {
 // for its own copies with staged().
 template <typename T, int D>
 __device__ __forceinline__ void stage_rows(uint8_t* dst, const Attn& a, int b, int h, int cnt, int r0, int tid) {
-  constexpr int CH = D / 8, STEP = 128 / CH;
-  const int c = tid % CH;
-  const T* q = reinterpret_cast<const T*>(a.q) + b * a.q_sb + 8 * c;
-  const uint32_t to = smem_u32(dst) + (c / 8) * 16384;
+  constexpr int CH = D / 8, STEP = 128 / CH;  // 8 or 16 rows at a time: lr & 7 stays
+  const int c = tid % CH, lr = tid / CH;
+  uint32_t at = smem_u32(dst) + (c / 8) * 16384 + lr * 128 + (((c % 8) ^ (lr & 7)) << 4);
+  // row r = i G + g, and its address, are counted on: a step is di queries and dg heads
+  int r = r0 + lr, i = div_g(a, r), g = r - i * a.G;
+  const int di = div_g(a, STEP), dg = STEP - di * a.G;
+  const T* base = reinterpret_cast<const T*>(a.q) + b * a.q_sb + 8 * c;
+  const T* p = base + (int64_t)(h * a.G + g) * a.q_sh + i * a.q_ss;
+  const int64_t step = di * a.q_ss + dg * a.q_sh, carry = a.q_ss - a.G * a.q_sh;
 #pragma unroll 4
-  for (int lr = tid / CH; lr < kTile; lr += STEP) {
-    const int r = r0 + lr, i = div_g(a, r), g = r - i * a.G;
+  for (int k = 0; k < CH; ++k) {
     const bool in = r < a.rows && i < cnt;
-    const T* p = in ? q + (int64_t)(h * a.G + g) * a.q_sh + i * a.q_ss : q;
-    const uint32_t at = to + lr * 128 + (((c % 8) ^ (lr & 7)) << 4);
+    const T* from = in ? p : base;
     const int bytes = in ? 16 : 0;  // the rest is filled with zeros
     if (a.q_wide) {
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(p), "r"(bytes) : "memory");
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(from), "r"(bytes) : "memory");
     } else {
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(at), "l"(p), "r"(bytes / 2) : "memory");
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(at + 8), "l"(p + 4), "r"(bytes / 2) : "memory");
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(at), "l"(from), "r"(bytes / 2) : "memory");
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(at + 8), "l"(from + 4), "r"(bytes / 2) : "memory");
     }
+    r += STEP, at += STEP * 128, i += di, g += dg, p += step;
+    if (g >= a.G) g -= a.G, ++i, p += carry;
   }
   asm volatile("cp.async.commit_group;" ::: "memory");
 }
@@ -409,7 +414,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
         done_with(k);
         continue;
       }
-      const int r = r0 + tid, i = r / a.G;
+      const int r = r0 + tid, i = div_g(a, r);
       const bool valid = r < a.rows && i < w.cnt;
       const int at = w.first + i, n = w.n, n_steps = 2 * (w.u1 - w.u0), ordered = w.ordered;
       const int first_tile = w.u0, pre_tiles = w.pre, gap = w.gap;
@@ -419,7 +424,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
       const float slope = a.slopes && r < a.rows ? a.slopes[w.h * a.G + r % a.G] * kLog2e : 0.0f;
       const int pre = a.prefix ? a.prefix[w.b] : 0;
       // positions of the tile's first and last row
-      const int qa = w.first + r0 / a.G, qb = w.first + (r0 + kTile - 1) / a.G;
+      const int qa = w.first + div_g(a, r0), qb = w.first + div_g(a, r0 + kTile - 1);
       // half tiles that begin in here need no masks
       int plain_from = 0, plain_to = n - 64;
       if (a.cap != 0.0f || a.slopes || (!ordered && (a.causal || a.window > 0))) plain_to = -1;
@@ -989,7 +994,7 @@ __global__ void __launch_bounds__(kWeighThreads, 1) kv4_weigh_kernel(const Attn 
         tc_fence_after();
         sk = sc.sk[item & 1][tid];
         if (!w.ordered) pos = sc.pos[item & 1][tid];
-        const int q0 = w.first + rt * kTile / a.G, q1 = w.first + min((rt * kTile + kTile - 1) / a.G, w.cnt - 1);
+        const int q0 = w.first + div_g(a, rt * kTile), q1 = w.first + min(div_g(a, rt * kTile + kTile - 1), w.cnt - 1);
         const bool plain = a.cap == 0.0f && !a.slopes &&
                            ((!a.causal && a.window <= 0) ||
                             (w.ordered && (!a.causal || w.t0 + kTok - 1 <= q0) && (a.window <= 0 || q1 - w.t0 < a.window)));
@@ -1081,14 +1086,21 @@ __global__ void __launch_bounds__(kWeighThreads, 1) kv4_weigh_kernel(const Attn 
       __syncwarp();
       if (lane == 0) mbar_arrive(&sc.k_full);
       // ---- query rows, the next tile on its way while this one arrives ----
+      const float* lse = a.lse + (int64_t)(w.b * a.kv.H + w.h) * a.rows_pad;
+      auto lse_of = [&](int rt) {
+        const int r = rt * kTile + tid;
+        return r < a.rows && div_g(a, r) < w.cnt ? -__ldcg(lse + r) : -INFINITY;
+      };
+      float nl = lse_of(w.lo);
       for (int rt = w.lo; rt < w.hi; ++rt, ++tile) {
         const int s2 = tile & 1, st = tile & 3;
         if (tile >= 2 && !wait_warp(&sc.q_empty[s2], ((tile >> 1) - 1) & 1)) { ok = false; break; }
         stage_rows<T, D>(smem + L::off_q + s2 * L::kOp, a, w.b, w.h, w.cnt, rt * kTile, tid);
+        sc.nl[st][tid] = nl;
+        if (rt + 1 < w.hi) nl = lse_of(rt + 1);
         const int r = rt * kTile + tid, i = div_g(a, r);
-        sc.nl[st][tid] = r < a.rows && i < w.cnt ? -a.lse[(int64_t)(w.b * a.kv.H + w.h) * a.rows_pad + r] : -INFINITY;
         sc.at[st][tid] = w.first + i;
-        sc.slope[st][tid] = a.slopes && r < a.rows ? a.slopes[w.h * a.G + r - i * a.G] * kLog2e : 0.0f;
+        if (a.slopes) sc.slope[st][tid] = r < a.rows ? a.slopes[w.h * a.G + r - i * a.G] * kLog2e : 0.0f;
         if (rt > w.lo) {
           staged<1>();
           __syncwarp();
