@@ -425,8 +425,8 @@ typedef struct {
 int lq_kv4_append(const lq_kv4_cache* host_cache, const void* k, const void* v, int dtype, int64_t S,
                   int64_t k_sb, int64_t k_sh, int64_t k_ss, int64_t v_sb, int64_t v_sh, int64_t v_ss,
                   const int32_t* counts, void* stream);
-/* Values of the first n slots as k, v [B, H, n, D] (float dtype, rounded once);
- * zeros past a sequence's length. */
+/* Values of the first n slots as k, v [B, H, n, D] (float dtype, rounded once,
+ * 32-byte aligned); zeros past a sequence's length. */
 int lq_kv4_dequant(const lq_kv4_cache* host_cache, int64_t n, int dtype, void* k, void* v, void* stream);
 /* Cut every sequence back to at most `keep` tokens per head: the `recent` last
  * positions and the positions below `sinks` stay, then the tokens with the

@@ -75,36 +75,63 @@ __device__ __forceinline__ uint32_t quant4(const float* x, uint32_t& par) {
   return w;
 }
 
+// A group of D / 4 lanes takes the two tokens that share words of V (slots 2j,
+// 2j + 1), so that V is written in whole words too.  Blocks go over all pairs of
+// all heads in turn: few blocks, since each counts at the ticket (a block per 8
+// tokens spent most of its time there: 72 us for 64 heads x 2048 tokens).
 template <typename T, int D>
-__global__ void __launch_bounds__(256) kv4_append_kernel(Kv4 kv, AppendArgs a) {
-  constexpr int LPT = D / 4, TPB = 256 / LPT, W = D / 32;  // lanes per token, tokens per block
-  const int bh = blockIdx.y, b = bh / kv.H, h = bh % kv.H;
-  const int i = blockIdx.x * TPB + threadIdx.x / LPT, l = threadIdx.x % LPT;
-  const int cnt = a.counts ? min(max(a.counts[b], 0), a.S) : a.S;
-  const int len = kv.len[b];
-  const int64_t t = (int64_t)len + i;
-  const bool live = i < cnt && t < kv.cap;
-  uint32_t par[2], w[2];
+__global__ void __launch_bounds__(256) kv4_append_kernel(Kv4 kv, AppendArgs a, int groups) {
+  constexpr int LPT = D / 4, PPB = 256 / LPT, W = D / 32;  // lanes per token, pairs per block
+  const int l = threadIdx.x % LPT, pair = threadIdx.x / LPT;
+  const int64_t items = (int64_t)groups * kv.B * kv.H;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int bh = (int)(item / groups), b = bh / kv.H, h = bh % kv.H;
+    const int cnt = a.counts ? min(max(a.counts[b], 0), a.S) : a.S;
+    const int len = kv.len[b], next = kv.next[b];
+    const int i0 = 2 * ((int)(item % groups) * PPB + pair) - (len & 1);  // first token of the pair
+    if (i0 - 2 * pair >= cnt) continue;  // nothing for the whole block
+    uint32_t par[2][2], w[2][2];
+    bool live[2];
 #pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (live) load4(static_cast<const T*>(a.x[s]) + b * a.sb[s] + h * a.sh[s] + i * a.ss[s] + 4 * l, x);
-    w[s] = quant4<LPT>(x, par[s]);
-  }
-  // two lanes make a word of K: even values in its low half, odd ones in its high half
-  uint32_t kw = ((w[0] & 0xf) | ((w[0] >> 4) & 0xf0) | ((w[0] << 12) & 0xf0000) | ((w[0] << 8) & 0xf00000)) << (8 * (l & 1));
-  kw |= __shfl_xor_sync(0xffffffffu, kw, 1);
-  if (live) {
-    const int64_t row = (int64_t)bh * kv.cap;
-    if (!(l & 1)) *reinterpret_cast<uint32_t*>(kv.k + (row + t) * (D / 2) + 2 * l) = kw;
-    *reinterpret_cast<uint16_t*>(kv.v + row * (D / 2) + v_unit(t, l, W)) = (uint16_t)w[1];
-    if (l == 0) {
-      kv.par[row + t] = make_uint2(par[0], par[1]);
-      kv.pos[row + t] = kv.next[b] + i;
-      kv.mass[row + t] = 0.0f;
+    for (int e = 0; e < 2; ++e) {
+      const int i = i0 + e;
+      live[e] = i >= 0 && i < cnt && (int64_t)len + i < kv.cap;
     }
+    float x[2][2][4];
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+#pragma unroll
+        for (int d = 0; d < 4; ++d) x[e][s][d] = 0.0f;
+        if (live[e]) load4(static_cast<const T*>(a.x[s]) + b * a.sb[s] + h * a.sh[s] + (i0 + e) * a.ss[s] + 4 * l, x[e][s]);
+      }
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) w[e][s] = quant4<LPT>(x[e][s], par[e][s]);
+    const int64_t row = (int64_t)bh * kv.cap;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      // two lanes make a word of K: even values in its low half, odd ones in its high half
+      const uint32_t k = w[e][0];
+      uint32_t kw = ((k & 0xf) | ((k >> 4) & 0xf0) | ((k << 12) & 0xf0000) | ((k << 8) & 0xf00000)) << (8 * (l & 1));
+      kw |= __shfl_xor_sync(0xffffffffu, kw, 1);
+      if (!live[e]) continue;
+      const int64_t t = row + len + i0 + e;
+      if (!(l & 1)) *reinterpret_cast<uint32_t*>(kv.k + t * (D / 2) + 2 * l) = kw;
+      if (l == 0) {
+        kv.par[t] = make_uint2(par[e][0], par[e][1]);
+        kv.pos[t] = next + i0 + e;
+        kv.mass[t] = 0.0f;
+      }
+    }
+    uint8_t* v = kv.v + row * (D / 2) + v_unit((int64_t)len + i0, l, W);  // the pair's word
+    if (live[0] && live[1]) *reinterpret_cast<uint32_t*>(v) = w[0][1] | (w[1][1] << 16);
+    else if (live[0]) *reinterpret_cast<uint16_t*>(v) = (uint16_t)w[0][1];
+    else if (live[1]) *reinterpret_cast<uint16_t*>(v + 2) = (uint16_t)w[1][1];
   }
-  if (last_block(kv.sync, gridDim.x * gridDim.y)) {
+  if (last_block(kv.sync, gridDim.x)) {
     for (int j = threadIdx.x; j < kv.B; j += blockDim.x) {
       const int n = a.counts ? min(max(a.counts[j], 0), a.S) : a.S, room = kv.cap - kv.len[j];
       kv.len[j] += min(n, room);
@@ -116,59 +143,113 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4 kv, AppendArgs a) {
 
 // ---------------------------------------------------------------------------
 // Read out the first n slots of every head as values (zeros past a sequence's
-// length).
+// length).  A warp takes 16 tokens; code - zero is exact in 16 bits (bias + code
+// less bias + zero), its product with the scale is rounded once.  Bound by the
+// bytes written; each lane writes whole 32-byte sectors.
 // ---------------------------------------------------------------------------
-template <typename T, int N>
-__device__ __forceinline__ void store_n(T* p, const float* x) {
+template <typename T> struct Out;
+template <> struct Out<__nv_bfloat16> {
+  static constexpr uint32_t bias = 0x43004300u;  // 128
+  // the pair of values of a pair of codes; z: zero point, s: scale (bf16 pairs)
+  __device__ __forceinline__ static uint32_t value(uint32_t c, uint32_t z, uint32_t s) {
+    c |= bias;
+    __nv_bfloat162 v = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&c), *reinterpret_cast<__nv_bfloat162*>(&z));
+    v = __hmul2(v, *reinterpret_cast<__nv_bfloat162*>(&s));
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
+};
+__device__ __forceinline__ void st_v8(void* p, const uint32_t* r) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+// 16 values of a token from 8 pairs of codes: 32 bytes in 16 bits, 64 in 32
+template <typename T>
+__device__ __forceinline__ void put16(T* p, const uint32_t* c, uint32_t par, bool live) {
+  uint32_t r[16];
+  if constexpr (sizeof(T) == 2 && Ty<T>::code == LQ_BF16) {
+    const uint32_t z = (uint32_t)(int)par_zero(par) * 0x10001u + Out<T>::bias, s = (par & 0xffffu) * 0x10001u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = live ? Out<T>::value(c[i], z, s) : 0u;
+    st_v8(p, r);
+  } else {
+    const float z = par_zero(par), s = par_scale(par);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x = live ? __fmul_rn((float)(c[i] & 0xffffu) - z, s) : 0.0f;
+      const float y = live ? __fmul_rn((float)(c[i] >> 16) - z, s) : 0.0f;
+      if constexpr (sizeof(T) == 2) {
+        const __half2 v = __floats2half2_rn(x, y);
+        r[i] = *reinterpret_cast<const uint32_t*>(&v);
+      } else {
+        r[2 * i] = __float_as_uint(x), r[2 * i + 1] = __float_as_uint(y);
+      }
+    }
+    st_v8(p, r);
+    if constexpr (sizeof(T) == 4) st_v8(p + 8, r + 8);
+  }
+}
+
+template <typename T>  // 8 values, for head dim 64
+__device__ __forceinline__ void put8(T* p, const uint32_t* c, uint32_t par, bool live) {
+  const float z = par_zero(par), s = par_scale(par);
   union {
-    uint4 u[(N * sizeof(T) + 15) / 16];
-    T t[N];
-  } v;
+    T t[8];
+    uint4 u[sizeof(T) / 2];
+  } r;
 #pragma unroll
-  for (int i = 0; i < N; ++i) v.t[i] = Ty<T>::from_f(x[i]);
+  for (int i = 0; i < 8; ++i) r.t[i] = Ty<T>::from_f(live ? __fmul_rn((float)((c[i / 2] >> (16 * (i & 1))) & 0xffffu) - z, s) : 0.0f);
 #pragma unroll
-  for (int i = 0; i < (int)(N * sizeof(T)) / 16; ++i) st_v4(reinterpret_cast<uint4*>(p) + i, v.u[i]);
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) st_v4(reinterpret_cast<uint4*>(p) + i, r.u[i]);
 }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv4_dequant_kernel(Kv4 kv, int n, T* ko, T* vo) {
-  // one warp per tile of 16 tokens and head
   constexpr int W = D / 32;
   const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int64_t tiles = (n + 15) / 16, item = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
   if (item >= tiles * kv.B * kv.H) return;
   const int64_t bh = item / tiles, t0 = (item % tiles) * 16, row = bh * kv.cap;
   const int len = kv.len[bh / kv.H];
+  constexpr uint32_t m = 0x000f000fu;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
-    // K: token g of the half, words c W .. c W + W - 1
-    int64_t t = t0 + 8 * half + g;
+    // K: token g of the half, words c W .. c W + W - 1, 16 values to two words
+    const int64_t t = t0 + 8 * half + g;
     if (t < n) {
       const uint32_t* p = reinterpret_cast<const uint32_t*>(kv.k + (row + t) * (D / 2)) + c * W;
-      const uint32_t par = t < len ? kv.par[row + t].x : 0;
+      const uint32_t par = t < len ? kv.par[row + t].x : 0u;
 #pragma unroll
-      for (int i = 0; i < W; ++i) {
-        float x[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          x[j] = t < len ? __fmul_rn((float)((p[i] >> (4 * (j >> 1) + 16 * (j & 1))) & 15) - par_zero(par), par_scale(par)) : 0.0f;
-        store_n<T, 8>(ko + (bh * n + t) * D + (c * W + i) * 8, x);
+      for (int i = 0; i < W; i += 2) {
+        const uint2 w = *reinterpret_cast<const uint2*>(p + i);
+        const uint32_t x[8] = {w.x & m, (w.x >> 4) & m, (w.x >> 8) & m, (w.x >> 12) & m,
+                               w.y & m, (w.y >> 4) & m, (w.y >> 8) & m, (w.y >> 12) & m};
+        put16<T>(ko + (bh * n + t) * D + (c * W + i) * 8, x, par, t < len);
       }
     }
-    // V: tokens 2c, 2c + 1 of the half, units g W .. g W + W - 1
+    // V: tokens 2c, 2c + 1 of the half, units g W .. g W + W - 1, 4 values to a word
     const uint32_t* p = reinterpret_cast<const uint32_t*>(kv.v + row * (D / 2) + (t0 >> 4) * (W * 256) + half * (W * 128)) + lane * W;
+    uint32_t w[W];
+#pragma unroll
+    for (int i = 0; i < W; i += 2) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p + i);
+      w[i] = v.x, w[i + 1] = v.y;
+    }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      t = t0 + 8 * half + 2 * c + e;
-      if (t >= n) continue;
-      const uint32_t par = t < len ? kv.par[row + t].y : 0;
-      float x[4 * W];
+      const int64_t tv = t0 + 8 * half + 2 * c + e;
+      if (tv >= n) continue;
+      const uint32_t par = tv < len ? kv.par[row + tv].y : 0u;
+      uint32_t x[2 * W < 8 ? 8 : 2 * W];
 #pragma unroll
-      for (int i = 0; i < W; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          x[4 * i + j] = t < len ? __fmul_rn((float)((p[i] >> (16 * e + 4 * j)) & 15) - par_zero(par), par_scale(par)) : 0.0f;
-      store_n<T, 4 * W>(vo + (bh * n + t) * D + g * (4 * W), x);
+      for (int i = 0; i < W; ++i) {  // nibbles (0, 1) and (2, 3) of the token's half
+        const uint32_t u = (w[i] >> (16 * e)) & 0xffffu;
+        x[2 * i] = (u & 0xfu) | ((u & 0xf0u) << 12);
+        x[2 * i + 1] = ((u >> 8) & 0xfu) | ((u & 0xf000u) << 4);
+      }
+      T* out = vo + (bh * n + tv) * D + g * (4 * W);
+      if constexpr (W == 4) put16<T>(out, x, par, tv < len);
+      else put8<T>(out, x, par, tv < len);
     }
   }
 }
@@ -182,65 +263,83 @@ __global__ void __launch_bounds__(256) kv4_dequant_kernel(Kv4 kv, int n, T* ko, 
 // ---------------------------------------------------------------------------
 struct EvictArgs {
   int keep, recent, sinks;
+  int n_keys;      // keys that shared memory holds
   int32_t* moves;  // [B H, 2, n_moves]: holes, then the tokens that fill them
   int64_t n_moves;
 };
 
 constexpr int kEvictThreads = 1024;
+constexpr int kEvictKeys = 48 * 1024;  // 192 KB
 
 __device__ __forceinline__ uint32_t evict_key(const Kv4& kv, int64_t i, int from, int sinks) {
   const int p = kv.pos[i];
-  if (p >= from || p < sinks) return 0xffffffffu;
   const float m = kv.mass[i];
+  if (p >= from || p < sinks) return 0xffffffffu;
   return m != m ? 0x7fffffffu : __float_as_uint(fmaxf(m, 0.0f));
 }
 
-// Sum over the block of each thread's flag, before it and in all; two barriers.
-__device__ __forceinline__ int block_rank(bool f, int* scratch, int& total) {
+// Ranks of each thread's flags in the block, 10 bits and a total of 11 for each
+// of three; two barriers.
+__device__ __forceinline__ void block_ranks(const bool* f, uint64_t* scratch, int* before, int* total) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t m = __ballot_sync(0xffffffffu, f);
+  uint32_t m[3];
+#pragma unroll
+  for (int i = 0; i < 3; ++i) m[i] = __ballot_sync(0xffffffffu, f[i]);
   __syncthreads();
-  if (lane == 0) scratch[warp] = __popc(m);
+  if (lane == 0) scratch[warp] = (uint64_t)__popc(m[0]) | (uint64_t)__popc(m[1]) << 20 | (uint64_t)__popc(m[2]) << 40;
   __syncthreads();
-  int mine = scratch[lane], inc = mine;
+  const uint64_t mine = scratch[lane];
+  uint64_t inc = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, inc, d);
+    const uint64_t y = __shfl_up_sync(0xffffffffu, inc, d);
     if (lane >= d) inc += y;
   }
-  total = __shfl_sync(0xffffffffu, inc, 31);
-  const int before = __shfl_sync(0xffffffffu, inc - mine, warp);
-  return before + __popc(m & ((1u << lane) - 1));
+  const uint64_t all = __shfl_sync(0xffffffffu, inc, 31), base = __shfl_sync(0xffffffffu, inc - mine, warp);
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    before[i] = (int)((base >> (20 * i)) & 0xfffff) + __popc(m[i] & ((1u << lane) - 1));
+    total[i] = (int)((all >> (20 * i)) & 0xfffff);
+  }
 }
 
 template <int D>
 __global__ void __launch_bounds__(kEvictThreads) kv4_evict_kernel(Kv4 kv, EvictArgs a) {
+  extern __shared__ uint32_t keys[];
   __shared__ int hist[2048];
   __shared__ int scratch[32];
-  __shared__ int s_bin, s_above;
+  __shared__ uint64_t scratch3[32];
+  __shared__ int s_bin, s_above, s_inside;
   constexpr int W = D / 32;
-  const int bh = blockIdx.x, b = bh / kv.H, tid = threadIdx.x;
+  const int bh = blockIdx.x, b = bh / kv.H, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t row = (int64_t)bh * kv.cap;
   const int n = min(kv.len[b], kv.cap), keep = a.keep;
   if (n > keep) {
     const int from = kv.next[b] - a.recent;
+    auto key_of = [&](int t) { return t < a.n_keys ? keys[t] : evict_key(kv, row + t, from, a.sinks); };
     // the keep-th greatest key, 11 + 11 + 10 bits at a time
     uint32_t prefix = 0, mask = 0;
     int need = keep;  // of the keys that match the prefix so far
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
       const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
-      for (int i = tid; i < 2048; i += kEvictThreads) hist[i] = 0;
+      hist[tid] = hist[tid + 1024] = 0;
       __syncthreads();
+#pragma unroll 4
       for (int t = tid; t < n; t += kEvictThreads) {
-        const uint32_t k = evict_key(kv, row + t, from, a.sinks);
+        uint32_t k;
+        if (pass == 0) {
+          k = evict_key(kv, row + t, from, a.sinks);
+          if (t < a.n_keys) keys[t] = k;
+        } else {
+          k = key_of(t);
+        }
         if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1);
       }
       __syncthreads();
       // thread i sums the two bins from the top, 2047 - 2i and 2046 - 2i
       const int hi = hist[2047 - 2 * tid], lo = hist[2046 - 2 * tid];
       int inc = hi + lo;
-      const int warp = tid >> 5, lane = tid & 31;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, inc, d);
@@ -258,55 +357,64 @@ __global__ void __launch_bounds__(kEvictThreads) kv4_evict_kernel(Kv4 kv, EvictA
       if (base < need && base + hi >= need) {
         s_bin = 2047 - 2 * tid;
         s_above = base;
+        s_inside = hi;
       } else if (base + hi < need && base + hi + lo >= need) {
         s_bin = 2046 - 2 * tid;
         s_above = base + hi;
+        s_inside = lo;
       }
       __syncthreads();
       prefix |= (uint32_t)s_bin << shift;
       mask |= (uint32_t)(bins - 1) << shift;
       need -= s_above;
+      if (s_inside == need) break;  // all of the bin stay: what is below it does not matter
       __syncthreads();
     }
-    // slots in order: which keys equal to the threshold stay, the holes, the tokens that move
+    // Keys above the prefix stay, of those that match it the first `need`.  Slots
+    // in order: the holes, the tokens that move.
     int32_t* holes = a.moves + (int64_t)bh * 2 * a.n_moves;
     int32_t* late = holes + a.n_moves;
-    int equal = 0, n_holes = 0, n_late = 0;
+    int seen[3] = {0, 0, 0};  // keys that match, holes, tokens that move
 #pragma unroll 1
     for (int t0 = 0; t0 < n; t0 += kEvictThreads) {
       const int t = t0 + tid;
-      const uint32_t k = t < n ? evict_key(kv, row + t, from, a.sinks) : 0;
-      const bool eq = t < n && k == prefix;
-      int total;
-      const int er = equal + block_rank(eq, scratch, total);
-      equal += total;
-      const bool kept = t < n && (k > prefix || (eq && er < need));
-      const bool hole = t < keep && !kept, moves = t >= keep && kept;
-      const int hr = n_holes + block_rank(hole, scratch, total);
-      n_holes += total;
-      if (hole) holes[hr] = t;
-      const int lr = n_late + block_rank(moves, scratch, total);
-      n_late += total;
-      if (moves) late[lr] = t;
+      const uint32_t k = t < n ? key_of(t) & mask : 0u;
+      const bool eq = t < n && k == prefix, above = t < n && k > prefix;
+      // where a token's fate hangs on its rank, that comes first
+      int before[3], total[3];
+      bool kept = above || eq;
+      if (__syncthreads_count(eq) + seen[0] > need) {
+        const bool f[3] = {eq, false, false};
+        block_ranks(f, scratch3, before, total);
+        kept = above || (eq && seen[0] + before[0] < need);
+      }
+      const bool f[3] = {eq, t < keep && !kept, t >= keep && kept};
+      block_ranks(f, scratch3, before, total);
+      if (f[1]) holes[seen[1] + before[1]] = t;
+      if (f[2]) late[seen[2] + before[2]] = t;
+#pragma unroll
+      for (int i = 0; i < 3; ++i) seen[i] += total[i];
     }
     __threadfence_block();
     __syncthreads();
-    // n_late == n_holes: keep slots stay in all.  A warp moves a token.
-    const int lane = tid & 31;
-    for (int j = tid >> 5; j < n_late; j += kEvictThreads / 32) {
+    // As many move as there are holes: keep slots stay in all.  8 lanes move a token.
+    const int l8 = tid & 7;
+    uint8_t* kc = kv.k + row * (D / 2);
+    uint8_t* vc = kv.v + row * (D / 2);
+    for (int j = tid >> 3; j < seen[2]; j += kEvictThreads / 8) {
       const int src = late[j], dst = holes[j];
-      uint8_t* kc = kv.k + row * (D / 2);
-      uint8_t* vc = kv.v + row * (D / 2);
-      if (lane < D / 8) {
-        reinterpret_cast<uint32_t*>(kc + (int64_t)dst * (D / 2))[lane] = reinterpret_cast<const uint32_t*>(kc + (int64_t)src * (D / 2))[lane];
-      }
-      if (lane < D / 4)
-        *reinterpret_cast<uint16_t*>(vc + v_unit(dst, lane, W)) = *reinterpret_cast<const uint16_t*>(vc + v_unit(src, lane, W));
-      if (lane == 0) {
-        kv.par[row + dst] = kv.par[row + src];
-        kv.pos[row + dst] = kv.pos[row + src];
-        kv.mass[row + dst] = kv.mass[row + src];
-      }
+      if constexpr (D == 128)
+        reinterpret_cast<uint2*>(kc + (int64_t)dst * (D / 2))[l8] = reinterpret_cast<const uint2*>(kc + (int64_t)src * (D / 2))[l8];
+      else
+        reinterpret_cast<uint32_t*>(kc + (int64_t)dst * (D / 2))[l8] = reinterpret_cast<const uint32_t*>(kc + (int64_t)src * (D / 2))[l8];
+      uint16_t u[W];
+#pragma unroll
+      for (int i = 0; i < W; ++i) u[i] = *reinterpret_cast<const uint16_t*>(vc + v_unit(src, l8 * W + i, W));
+#pragma unroll
+      for (int i = 0; i < W; ++i) *reinterpret_cast<uint16_t*>(vc + v_unit(dst, l8 * W + i, W)) = u[i];
+      if (l8 == 0) kv.par[row + dst] = kv.par[row + src];
+      if (l8 == 1) kv.pos[row + dst] = kv.pos[row + src];
+      if (l8 == 2) kv.mass[row + dst] = kv.mass[row + src];
     }
     __syncthreads();
     for (int t = keep + tid; t < n; t += kEvictThreads) {
@@ -329,13 +437,17 @@ __global__ void __launch_bounds__(256) kv4_reset_kernel(Kv4 kv) {
   for (int64_t i = i0; i < 2 * kv.B + 4; i += step) kv.len[i] = 0;
 }
 
+template <typename T, int D>
+int append_td(const Kv4& kv, const AppendArgs& a, cudaStream_t st) {
+  constexpr int PPB = 1024 / D;                 // pairs per block
+  const int groups = (a.S / 2 + 1 + PPB - 1) / PPB;  // a chunk may begin at an odd slot
+  const int grid = resident_grid(kv4_append_kernel<T, D>, 256, 0, (int64_t)groups * kv.B * kv.H);
+  kv4_append_kernel<T, D><<<grid, 256, 0, st>>>(kv, a, groups);
+  return launched("kv4_append_kernel");
+}
 template <typename T>
 int append_t(const Kv4& kv, const AppendArgs& a, cudaStream_t st) {
-  const int tpb = kv.D == 128 ? 8 : 16;
-  const dim3 grid((unsigned)((a.S + tpb - 1) / tpb), kv.B * kv.H);
-  if (kv.D == 128) kv4_append_kernel<T, 128><<<grid, 256, 0, st>>>(kv, a);
-  else kv4_append_kernel<T, 64><<<grid, 256, 0, st>>>(kv, a);
-  return launched("kv4_append_kernel");
+  return kv.D == 128 ? append_td<T, 128>(kv, a, st) : append_td<T, 64>(kv, a, st);
 }
 
 template <typename T>
@@ -379,7 +491,7 @@ extern "C" int lq_kv4_dequant(const lq_kv4_cache* cache, int64_t n, int dtype, v
   LQ_REQUIRE(n >= 0 && n <= cache->cap, LQ_EINVAL, "%lld slots of %lld", (long long)n, (long long)cache->cap);
   if (n == 0) return LQ_OK;
   LQ_REQUIRE(k && v, LQ_EINVAL, "NULL pointer");
-  LQ_REQUIRE(aligned16(k) && aligned16(v), LQ_EALIGN, "outputs must be 16-byte aligned");
+  LQ_REQUIRE((((uintptr_t)k | (uintptr_t)v) & 31) == 0, LQ_EALIGN, "outputs must be 32-byte aligned");
   const Kv4 kv = kv4_of(cache);
   cudaStream_t st = as_stream(stream);
   switch (dtype) {
@@ -405,11 +517,14 @@ extern "C" int lq_kv4_evict(const lq_kv4_cache* cache, int64_t keep, int64_t rec
   const size_t need = lq_kv4_evict_workspace_bytes(cache->B, cache->H, cache->cap, keep);
   LQ_REQUIRE(workspace && workspace_bytes >= need, LQ_EINVAL, "workspace of %zu bytes needed", need);
   const Kv4 kv = kv4_of(cache);
-  const EvictArgs a{(int)keep, (int)recent, (int)sinks, static_cast<int32_t*>(workspace),
+  const int n_keys = (int)std::min<int64_t>(kv.cap, kEvictKeys);
+  const EvictArgs a{(int)keep, (int)recent, (int)sinks, n_keys, static_cast<int32_t*>(workspace),
                     std::min(keep, (int64_t)kv.cap - keep)};
   cudaStream_t st = as_stream(stream);
-  if (kv.D == 128) kv4_evict_kernel<128><<<kv.B * kv.H, kEvictThreads, 0, st>>>(kv, a);
-  else kv4_evict_kernel<64><<<kv.B * kv.H, kEvictThreads, 0, st>>>(kv, a);
+  auto kern = kv.D == 128 ? kv4_evict_kernel<128> : kv4_evict_kernel<64>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, n_keys * 4) != cudaSuccess)
+    return launched("kv4_evict_kernel (attribute)");
+  kern<<<kv.B * kv.H, kEvictThreads, n_keys * 4, st>>>(kv, a);
   return launched("kv4_evict_kernel");
 }
 
