@@ -42,20 +42,38 @@ __device__ __forceinline__ void load4(const T* p, float* x) {
   }
 }
 
+// x / y, correctly rounded, from inv = 1 / y correctly rounded: a quotient within
+// an ulp, its remainder (exact by fma), and one correction (Markstein); for
+// quotients, remainders and y far from over- and underflow.
+__device__ __forceinline__ float quotient(float x, float y, float inv) {
+  const float q = __fmul_rn(x, inv);
+  return __fmaf_rn(__fmaf_rn(-q, y, x), inv, q);
+}
+// Greatest and least value of a group of LPT neighbouring lanes, NaN if there is one.
+template <int LPT>
+__device__ __forceinline__ void group_range(float& lo, float& hi) {
+  if constexpr (LPT == 32) {
+    asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(hi) : "f"(hi));
+    asm("redux.sync.min.NaN.f32 %0, %1, 0xffffffff;" : "=f"(lo) : "f"(lo));
+  } else {
+#pragma unroll
+    for (int m = LPT / 2; m > 0; m >>= 1) {
+      lo = fmin_nan(lo, __shfl_xor_sync(0xffffffffu, lo, m));
+      hi = fmax_nan(hi, __shfl_xor_sync(0xffffffffu, hi, m));
+    }
+  }
+}
+
 // Codes (4 nibbles, the first lowest) and parameter word of a token from the
 // 4 values of each of its LPT lanes.
 template <int LPT>
 __device__ __forceinline__ uint32_t quant4(const float* x, uint32_t& par) {
   float lo = fmin_nan(fmin_nan(x[0], x[1]), fmin_nan(x[2], x[3]));
   float hi = fmax_nan(fmax_nan(x[0], x[1]), fmax_nan(x[2], x[3]));
-#pragma unroll
-  for (int m = LPT / 2; m > 0; m >>= 1) {
-    lo = fmin_nan(lo, __shfl_xor_sync(0xffffffffu, lo, m));
-    hi = fmax_nan(hi, __shfl_xor_sync(0xffffffffu, hi, m));
-  }
+  group_range<LPT>(lo, hi);
   lo = fmin_nan(lo, 0.0f);
   hi = fmax_nan(hi, 0.0f);
-  const float s = Ty<__nv_bfloat16>::round(__fdiv_rn(__fsub_rn(hi, lo), 15.0f));
+  const float s = Ty<__nv_bfloat16>::round(quotient(__fsub_rn(hi, lo), 15.0f, 0.066666667f));
   if (!(s < INFINITY)) {  // NaN or infinite
     par = 0x7fc0u;
     return 0;
@@ -64,32 +82,33 @@ __device__ __forceinline__ uint32_t quant4(const float* x, uint32_t& par) {
     par = 0;
     return 0;
   }
-  const float z = fminf(rintf(__fdiv_rn(-lo, s)), 15.0f);
+  // rint by adding 1.5 * 2^23, whose last mantissa bit is 1; codes are not below
+  // 0, since the zero point is the least value's, but the greatest may reach 16
+  const float inv = __frcp_rn(s), magic = 12582912.0f;
+  const float z = fminf(__fsub_rn(__fadd_rn(quotient(-lo, s, inv), magic), magic), 15.0f);
   par = __float_as_uint(z) | (__float_as_uint(s) >> 16);
+  const int off = (int)z - 0x4b400000;
   uint32_t w = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float c = fminf(fmaxf(__fadd_rn(rintf(__fdiv_rn(x[i], s)), z), 0.0f), 15.0f);
-    w |= (uint32_t)c << (4 * i);
-  }
+  for (int i = 0; i < 4; ++i)
+    w |= (uint32_t)min(__float_as_int(__fadd_rn(quotient(x[i], s, inv), magic)) + off, 15) << (4 * i);
   return w;
 }
 
 // A group of D / 4 lanes takes the two tokens that share words of V (slots 2j,
-// 2j + 1), so that V is written in whole words too.  Blocks go over all pairs of
-// all heads in turn: few blocks, since each counts at the ticket (a block per 8
-// tokens spent most of its time there: 72 us for 64 heads x 2048 tokens).
+// 2j + 1), so that V is written in whole words too.  The blocks
+// of a head go over its pairs in turn: about as many blocks as the GPU holds, since
+// each counts at the ticket.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4 kv, AppendArgs a, int groups) {
   constexpr int LPT = D / 4, PPB = 256 / LPT, W = D / 32;  // lanes per token, pairs per block
   const int l = threadIdx.x % LPT, pair = threadIdx.x / LPT;
-  const int64_t items = (int64_t)groups * kv.B * kv.H;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int bh = (int)(item / groups), b = bh / kv.H, h = bh % kv.H;
-    const int cnt = a.counts ? min(max(a.counts[b], 0), a.S) : a.S;
-    const int len = kv.len[b], next = kv.next[b];
-    const int i0 = 2 * ((int)(item % groups) * PPB + pair) - (len & 1);  // first token of the pair
-    if (i0 - 2 * pair >= cnt) continue;  // nothing for the whole block
+  const int bh = blockIdx.y, b = bh / kv.H, h = bh % kv.H;
+  const int cnt = a.counts ? min(max(a.counts[b], 0), a.S) : a.S;
+  const int len = kv.len[b], next = kv.next[b];
+  for (int group = blockIdx.x; group < groups; group += gridDim.x) {
+    const int i0 = 2 * (group * PPB + pair) - (len & 1);  // first token of the pair
+    if (i0 - 2 * pair >= cnt) break;  // nothing for the whole block any more
     uint32_t par[2][2], w[2][2];
     bool live[2];
 #pragma unroll
@@ -131,7 +150,7 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4 kv, AppendArgs a, i
     else if (live[0]) *reinterpret_cast<uint16_t*>(v) = (uint16_t)w[0][1];
     else if (live[1]) *reinterpret_cast<uint16_t*>(v + 2) = (uint16_t)w[1][1];
   }
-  if (last_block(kv.sync, gridDim.x)) {
+  if (last_block(kv.sync, gridDim.x * gridDim.y)) {
     for (int j = threadIdx.x; j < kv.B; j += blockDim.x) {
       const int n = a.counts ? min(max(a.counts[j], 0), a.S) : a.S, room = kv.cap - kv.len[j];
       kv.len[j] += min(n, room);
@@ -264,6 +283,7 @@ __global__ void __launch_bounds__(256) kv4_dequant_kernel(Kv4 kv, int n, T* ko, 
 struct EvictArgs {
   int keep, recent, sinks;
   int n_keys;      // keys that shared memory holds
+  int lists;       // and it holds the lists of the moves too
   int32_t* moves;  // [B H, 2, n_moves]: holes, then the tokens that fill them
   int64_t n_moves;
 };
@@ -303,6 +323,17 @@ __device__ __forceinline__ void block_ranks(const bool* f, uint64_t* scratch, in
   }
 }
 
+template <int W>
+__device__ __forceinline__ void ld_vec(const uint8_t* p, uint32_t* w) {
+  if constexpr (W == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x, w[1] = v.y;
+  }
+}
+
 template <int D>
 __global__ void __launch_bounds__(kEvictThreads) kv4_evict_kernel(Kv4 kv, EvictArgs a) {
   extern __shared__ uint32_t keys[];
@@ -317,7 +348,10 @@ __global__ void __launch_bounds__(kEvictThreads) kv4_evict_kernel(Kv4 kv, EvictA
   if (n > keep) {
     const int from = kv.next[b] - a.recent;
     auto key_of = [&](int t) { return t < a.n_keys ? keys[t] : evict_key(kv, row + t, from, a.sinks); };
-    // the keep-th greatest key, 11 + 11 + 10 bits at a time
+#pragma unroll 4
+    for (int t = tid; t < min(n, a.n_keys); t += kEvictThreads) keys[t] = evict_key(kv, row + t, from, a.sinks);
+    // the keep-th greatest key, 11 + 11 + 10 bits at a time (a thread reads back
+    // the keys that it wrote)
     uint32_t prefix = 0, mask = 0;
     int need = keep;  // of the keys that match the prefix so far
 #pragma unroll 1
@@ -325,16 +359,22 @@ __global__ void __launch_bounds__(kEvictThreads) kv4_evict_kernel(Kv4 kv, EvictA
       const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
       hist[tid] = hist[tid + 1024] = 0;
       __syncthreads();
-#pragma unroll 4
-      for (int t = tid; t < n; t += kEvictThreads) {
-        uint32_t k;
-        if (pass == 0) {
-          k = evict_key(kv, row + t, from, a.sinks);
-          if (t < a.n_keys) keys[t] = k;
-        } else {
-          k = key_of(t);
+#pragma unroll 1
+      for (int t0 = 0; t0 < n; t0 += kEvictThreads) {
+        const int t = t0 + tid;
+        const bool in = t < n;
+        const uint32_t k = in ? key_of(t) : 0u;
+        const bool match = in && (k & mask) == prefix;
+        // protected tokens, and those that never got any weight, are many and
+        // lie together: one addition for all that a warp has of them
+        const uint32_t safe = __ballot_sync(0xffffffffu, match && k == 0xffffffffu);
+        const uint32_t none = __ballot_sync(0xffffffffu, match && k == 0u);
+        const int bin = (k >> shift) & (bins - 1);
+        if (match && k != 0u && k != 0xffffffffu) atomicAdd(&hist[bin], 1);
+        if (lane == 0) {
+          if (safe) atomicAdd(&hist[bins - 1], __popc(safe));
+          if (none) atomicAdd(&hist[0], __popc(none));
         }
-        if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1);
       }
       __syncthreads();
       // thread i sums the two bins from the top, 2047 - 2i and 2046 - 2i
@@ -372,7 +412,7 @@ __global__ void __launch_bounds__(kEvictThreads) kv4_evict_kernel(Kv4 kv, EvictA
     }
     // Keys above the prefix stay, of those that match it the first `need`.  Slots
     // in order: the holes, the tokens that move.
-    int32_t* holes = a.moves + (int64_t)bh * 2 * a.n_moves;
+    int32_t* holes = a.lists ? reinterpret_cast<int32_t*>(keys + a.n_keys) : a.moves + (int64_t)bh * 2 * a.n_moves;
     int32_t* late = holes + a.n_moves;
     int seen[3] = {0, 0, 0};  // keys that match, holes, tokens that move
 #pragma unroll 1
@@ -401,17 +441,34 @@ __global__ void __launch_bounds__(kEvictThreads) kv4_evict_kernel(Kv4 kv, EvictA
     const int l8 = tid & 7;
     uint8_t* kc = kv.k + row * (D / 2);
     uint8_t* vc = kv.v + row * (D / 2);
+#pragma unroll 2
     for (int j = tid >> 3; j < seen[2]; j += kEvictThreads / 8) {
       const int src = late[j], dst = holes[j];
       if constexpr (D == 128)
         reinterpret_cast<uint2*>(kc + (int64_t)dst * (D / 2))[l8] = reinterpret_cast<const uint2*>(kc + (int64_t)src * (D / 2))[l8];
       else
         reinterpret_cast<uint32_t*>(kc + (int64_t)dst * (D / 2))[l8] = reinterpret_cast<const uint32_t*>(kc + (int64_t)src * (D / 2))[l8];
-      uint16_t u[W];
+      // The lane's units of V lie in one vector, in one half of its words; the other
+      // half is the neighbouring slot's.  It is written whole (by halves, the
+      // stores were half of the kernel's time): with what the neighbour has, or,
+      // if that is a hole too, with what it gets, by the group of the even slot.
+      const bool odd = dst & 1;
+      const int jn = odd ? j - 1 : j + 1;
+      const bool both = jn >= 0 && jn < seen[2] && holes[jn] == (dst ^ 1);
+      if (!(both && odd)) {
+        const int near = both ? late[jn] : dst ^ 1;
+        uint32_t u[W], o[W];
+        ld_vec<W>(vc + (v_unit(src, l8 * W, W) & ~(int64_t)3), u);
+        ld_vec<W>(vc + (v_unit(near, l8 * W, W) & ~(int64_t)3), o);
 #pragma unroll
-      for (int i = 0; i < W; ++i) u[i] = *reinterpret_cast<const uint16_t*>(vc + v_unit(src, l8 * W + i, W));
-#pragma unroll
-      for (int i = 0; i < W; ++i) *reinterpret_cast<uint16_t*>(vc + v_unit(dst, l8 * W + i, W)) = u[i];
+        for (int i = 0; i < W; ++i) {
+          const uint32_t x = (u[i] >> (16 * (src & 1))) & 0xffffu, y = (o[i] >> (16 * (near & 1))) & 0xffffu;
+          u[i] = odd ? y | x << 16 : x | y << 16;
+        }
+        uint8_t* to = vc + (v_unit(dst, l8 * W, W) & ~(int64_t)3);
+        if constexpr (W == 4) *reinterpret_cast<uint4*>(to) = make_uint4(u[0], u[1], u[2], u[3]);
+        else *reinterpret_cast<uint2*>(to) = make_uint2(u[0], u[1]);
+      }
       if (l8 == 0) kv.par[row + dst] = kv.par[row + src];
       if (l8 == 1) kv.pos[row + dst] = kv.pos[row + src];
       if (l8 == 2) kv.mass[row + dst] = kv.mass[row + src];
@@ -441,8 +498,9 @@ template <typename T, int D>
 int append_td(const Kv4& kv, const AppendArgs& a, cudaStream_t st) {
   constexpr int PPB = 1024 / D;                 // pairs per block
   const int groups = (a.S / 2 + 1 + PPB - 1) / PPB;  // a chunk may begin at an odd slot
-  const int grid = resident_grid(kv4_append_kernel<T, D>, 256, 0, (int64_t)groups * kv.B * kv.H);
-  kv4_append_kernel<T, D><<<grid, 256, 0, st>>>(kv, a, groups);
+  const int heads = kv.B * kv.H;
+  const int grid = resident_grid(kv4_append_kernel<T, D>, 256, 0, (int64_t)groups * heads);
+  kv4_append_kernel<T, D><<<dim3(std::max(1, std::min(groups, grid / heads)), heads), 256, 0, st>>>(kv, a, groups);
   return launched("kv4_append_kernel");
 }
 template <typename T>
@@ -518,13 +576,15 @@ extern "C" int lq_kv4_evict(const lq_kv4_cache* cache, int64_t keep, int64_t rec
   LQ_REQUIRE(workspace && workspace_bytes >= need, LQ_EINVAL, "workspace of %zu bytes needed", need);
   const Kv4 kv = kv4_of(cache);
   const int n_keys = (int)std::min<int64_t>(kv.cap, kEvictKeys);
-  const EvictArgs a{(int)keep, (int)recent, (int)sinks, n_keys, static_cast<int32_t*>(workspace),
-                    std::min(keep, (int64_t)kv.cap - keep)};
+  const int64_t n_moves = std::min(keep, (int64_t)kv.cap - keep);
+  const int lists = n_keys + 2 * n_moves <= kEvictKeys;
+  const EvictArgs a{(int)keep, (int)recent, (int)sinks, n_keys, lists, static_cast<int32_t*>(workspace), n_moves};
+  const int smem = 4 * (n_keys + (lists ? 2 * (int)n_moves : 0));
   cudaStream_t st = as_stream(stream);
   auto kern = kv.D == 128 ? kv4_evict_kernel<128> : kv4_evict_kernel<64>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, n_keys * 4) != cudaSuccess)
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return launched("kv4_evict_kernel (attribute)");
-  kern<<<kv.B * kv.H, kEvictThreads, n_keys * 4, st>>>(kv, a);
+  kern<<<kv.B * kv.H, kEvictThreads, smem, st>>>(kv, a);
   return launched("kv4_evict_kernel");
 }
 
