@@ -306,11 +306,25 @@ __global__ void __launch_bounds__(32 * kWarps, NQ == 1 && !QLO ? 4 : NQ == 1 ? 2
   AttnShared<D, NQ, QLO>& sh = *reinterpret_cast<AttnShared<D, NQ, QLO>*>(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int zb = blockIdx.y, cta = blockIdx.x;
-  int all;
-  units_before(a, 0, all);
   Cut cut;
-  cut.set(all, a.blocks);
-  if (all == 0 || cta >= cut.blocks) return;
+  int x0, x1, b, seq_begin;
+  Seq s;
+  if (a.whole) {  // a block to a head
+    b = cta / a.kv.H;
+    s = seq_of(a, b);
+    seq_begin = 0;
+    x0 = cta % a.kv.H * s.count;
+    x1 = x0 + s.count;
+  } else {
+    int all;
+    units_before(a, 0, all);
+    cut.set(all, a.blocks);
+    if (all == 0 || cta >= cut.blocks) return;
+    x0 = cut.begin(cta);
+    x1 = cut.begin(cta + 1);
+    b = seq_at(a, x0, seq_begin);
+    s = seq_of(a, b);
+  }
   if (lane == 0) {
 #pragma unroll
     for (int i = 0; i < kStages; ++i) mbar_init(&sh.full[warp][i], 1);
@@ -319,11 +333,7 @@ __global__ void __launch_bounds__(32 * kWarps, NQ == 1 && !QLO ? 4 : NQ == 1 ? 2
   }
   __syncwarp();
   int fill = 0, take = 0;  // units that this warp has asked for, and used
-  int x0 = cut.begin(cta), seq_begin;
-  const int x1 = cut.begin(cta + 1);
-  int b = seq_at(a, x0, seq_begin);
-  Seq s = seq_of(a, b);
-  int h = (x0 - seq_begin) / max(s.count, 1), u0 = x0 - seq_begin - h * s.count;
+  int h = a.whole ? cta % a.kv.H : (x0 - seq_begin) / s.count, u0 = x0 - seq_begin - h * s.count;
   int u1 = min(s.count, u0 + (x1 - x0));
   auto token = [&](int u) { return GEN ? (u < s.pre ? u : u + s.gap) * kUnit : u * kUnit; };
   auto ask = [&](int u) {  // every lane has read what the stage held
@@ -343,7 +353,7 @@ __global__ void __launch_bounds__(32 * kWarps, NQ == 1 && !QLO ? 4 : NQ == 1 ? 2
 #pragma unroll
   for (int i = 0; i < kStages; ++i) ask(u0 + warp + i * kWarps);
 
-  while (true) {
+  while (true) {  // (a whole head with nothing to see goes through too, and gives zeros)
     const int bh = b * a.kv.H + h;
     const int64_t row = (int64_t)bh * a.kv.cap;
     const int pre = GEN && a.prefix ? a.prefix[b] : 0;
@@ -413,6 +423,15 @@ __global__ void __launch_bounds__(32 * kWarps, NQ == 1 && !QLO ? 4 : NQ == 1 ? 2
             if constexpr (GEN) v = full_score<D, NQ, QLO>(a, q, nq, e, v, tok[j] < s.n, pos[j], pre);
             else if (tail && tok[j] >= s.n) v = -INFINITY;
           }
+      }
+      if (a.scores) {
+#pragma unroll
+        for (int nq = 0; nq < NQ; ++nq)
+          if (8 * nq + 2 * c < a.pitch)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              *reinterpret_cast<float2*>(a.scores + (row + tok[j]) * a.pitch + 8 * nq + 2 * c) =
+                  make_float2(x[j >> 1][nq][2 * (j & 1)], x[j >> 1][nq][2 * (j & 1) + 1]);
       }
       uint32_t pb[NQ][4], pl[QLO ? NQ : 1][4];
 #pragma unroll
@@ -564,6 +583,7 @@ __global__ void __launch_bounds__(32 * kWarps, NQ == 1 && !QLO ? 4 : NQ == 1 ? 2
           const int iq = qr / a.G, hq = h_done * a.G + qr % a.G;
           st_out4(a.out, (((int64_t)b_done * a.Hq + hq) * a.Sq + iq) * D + d, a.q_dtype, o, inv);
           if (a.lse && d == 0) a.lse[(int64_t)bh * a.rows_pad + qr] = L == 0.0f ? INFINITY : M + lg2(L);
+          if (a.scores && d == 0) a.ml[slot + qr] = make_float2(M, L);
         } else {
           *reinterpret_cast<float4*>(a.part + (slot + qr) * D + d) = o;
           if (d == 0) a.ml[slot + qr] = make_float2(M, L);
@@ -575,31 +595,86 @@ __global__ void __launch_bounds__(32 * kWarps, NQ == 1 && !QLO ? 4 : NQ == 1 ? 2
   if (threadIdx.x == 0) pdl_trigger();
 }
 
-// One warp per (row, head): merges the partial results of the blocks that
-// shared the head; zeros where there is nothing to see.  Heads that one block
-// covered are done already.  The lengths are older than the kernel before this
-// one, so they are read while it still runs.
-__global__ void __launch_bounds__(128) kv4_combine_kernel(const Attn a) {
-  const int item = blockIdx.x * 4 + threadIdx.x / 32, lane = threadIdx.x & 31, D = a.kv.D, V = D / 32;
-  if (item >= a.rows * a.kv.B * a.kv.H) return;
-  const int bh = item / a.rows, qr = item % a.rows, b = bh / a.kv.H, h = bh % a.kv.H;
+// First out_blocks blocks, a warp per (row, head): merges the partial results of
+// the blocks that shared the head; zeros where there is nothing to see.  Heads
+// that one block covered are done already.
+// The blocks behind them, if weights are collected from the scores that the
+// attention kernel left: 256 tokens of a head each, mass[t] += sum over the rows
+// of exp2(x[r, t] - lse[r]), with lse from the same partial results.
+// The lengths are older than the kernel before this one, so they are read while
+// it still runs.
+__global__ void __launch_bounds__(128) kv4_combine_kernel(const Attn a, int out_blocks) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, D = a.kv.D, V = D / 32;
+  const bool spread = (int)blockIdx.x >= out_blocks;
+  const int heads = a.kv.B * a.kv.H;
+  int bh, qr = 0, t0 = 0;
+  if (spread) {
+    bh = (blockIdx.x - out_blocks) % heads;
+    t0 = (blockIdx.x - out_blocks) / heads * 256;
+  } else {
+    const int item = blockIdx.x * 4 + warp;
+    if (item >= a.rows * heads) return;
+    bh = item / a.rows, qr = item % a.rows;
+  }
+  const int b = bh / a.kv.H, h = bh % a.kv.H;
   const Seq s = seq_of(a, b);
-  int all;
-  int begin = units_before(a, b, all);
-  Cut cut;
-  cut.set(all, a.blocks);
-  begin += h * s.count;
-  const int c0 = s.count ? cut.owner(begin) : 0, c1 = s.count ? cut.owner(begin + s.count - 1) : -1;
-  if (s.count && c0 == c1) return;
+  if (spread && (s.count == 0 || t0 >= s.n)) return;
+  int c0 = bh, c1 = bh;  // the blocks that had a part of the head
+  if (!a.whole) {
+    int all;
+    const int begin = units_before(a, b, all) + h * s.count;
+    Cut cut;
+    cut.set(all, a.blocks);
+    c0 = s.count ? cut.owner(begin) : 0, c1 = s.count ? cut.owner(begin + s.count - 1) : -1;
+  }
+  if (!spread && s.count && c0 == c1) return;
   pdl_wait();
-  float M = kNone, L = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  const int64_t first = (int64_t)(c0 + bh) * a.rows_pad + qr;
-  for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, a.ml[first + (int64_t)(c - c0) * a.rows_pad].x);
+  const int64_t first = (int64_t)(c0 + bh) * a.rows_pad;
+  auto reference = [&](int r) {
+    float m = kNone;
+    for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, a.ml[first + r + (int64_t)(c - c0) * a.rows_pad].x);
 #pragma unroll
-  for (int m = 16; m > 0; m >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, m));
+    for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+    return m;
+  };
+  if (spread) {
+    __shared__ float lse[16];
+    for (int r = warp; r < a.rows; r += 4) {
+      const float M = reference(r);
+      float L = 0.0f;
+      for (int c = c0 + lane; c <= c1; c += 32) {
+        const float2 ml = a.ml[first + r + (int64_t)(c - c0) * a.rows_pad];
+        L = fmaf(ex2(ml.x - M), ml.y, L);
+      }
+#pragma unroll
+      for (int k = 16; k > 0; k >>= 1) L += __shfl_xor_sync(0xffffffffu, L, k);
+      if (lane == 0) lse[r] = L == 0.0f ? INFINITY : M + lg2(L);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int t = t0 + 128 * k + threadIdx.x;
+      if (t >= s.n) break;
+      const int u = t / kUnit;
+      if (u >= s.pre && u < s.pre + s.gap) continue;  // behind the window: no scores were made
+      const int64_t i = (int64_t)bh * a.kv.cap + t;
+      float sum = 0.0f;
+      for (int r = 0; r < a.rows; r += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(a.scores + i * a.pitch + r);
+        sum += ex2(x.x - lse[r]);
+        if (r + 1 < a.rows) sum += ex2(x.y - lse[r + 1]);
+        if (r + 2 < a.rows) sum += ex2(x.z - lse[r + 2]);
+        if (r + 3 < a.rows) sum += ex2(x.w - lse[r + 3]);
+      }
+      a.kv.mass[i] += sum;
+    }
+    return;
+  }
+  const float M = reference(qr);
+  float L = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
   for (int c = 0; c <= c1 - c0; ++c) {
-    const int64_t i = first + (int64_t)c * a.rows_pad;
+    const int64_t i = first + qr + (int64_t)c * a.rows_pad;
     const float2 ml = a.ml[i];
     const float f = ex2(ml.x - M);
     L = fmaf(f, ml.y, L);
@@ -613,7 +688,7 @@ __global__ void __launch_bounds__(128) kv4_combine_kernel(const Attn a) {
     }
   }
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-  const int iq = qr / a.G, hq = h * a.G + qr % a.G;
+  const int iq = div_g(a, qr), hq = h * a.G + qr - iq * a.G;
   const int64_t at = (((int64_t)b * a.Hq + hq) * a.Sq + iq) * D + V * lane;
   for (int i = 0; i < V; ++i) st_out(a.out, at + i, a.q_dtype, o[i] * inv);
   if (a.lse && lane == 0) a.lse[(int64_t)bh * a.rows_pad + qr] = L == 0.0f ? INFINITY : M + lg2(L);
@@ -681,10 +756,18 @@ struct Plan {
   int nq, row_blocks, rows_pad, blocks;
   int64_t slots;  // partial results, of rows_pad (prompt: kPromptRows) rows each
   bool prompt;    // lq_kv4_prompt.cu's
+  bool whole;     // a block to a head
+  int pitch;      // scores kept per token for the collected weight; 0: none are kept
 };
+// Up to so many units a head is left to one block, and nothing has to be merged
+// (B=1, 8 heads, 500 tokens: 10 us in two kernels, see below for one).
+constexpr int kWholeUnits = 16;
+constexpr int64_t kMostScores = 256 << 20;  // bytes of kept scores
 constexpr int kFewRows = 16;  // up to here a row of the cache is read once by this file's kernel
-Plan plan_of(const Kv4& kv, int64_t rows, int64_t bound, bool qlo) {
+Plan plan_of(const Kv4& kv, int64_t rows, int64_t bound, bool qlo, bool weigh) {
   Plan p;
+  p.whole = false;
+  p.pitch = 0;
   p.prompt = !qlo && rows > kFewRows;
   if (p.prompt) {
     p.nq = p.row_blocks = 0;
@@ -696,23 +779,32 @@ Plan plan_of(const Kv4& kv, int64_t rows, int64_t bound, bool qlo) {
   p.nq = rows <= 8 ? 1 : 2;
   p.row_blocks = (int)((rows + 8 * p.nq - 1) / (8 * p.nq));
   p.rows_pad = p.row_blocks * 8 * p.nq;
-  const int64_t units = (int64_t)kv.B * kv.H * ((std::max<int64_t>(bound, 1) + kUnit - 1) / kUnit);
+  const int64_t per_head = (std::max<int64_t>(bound, 1) + kUnit - 1) / kUnit, units = (int64_t)kv.B * kv.H * per_head;
+  if (weigh && p.row_blocks == 1) {
+    const int pitch = (int)(rows + 3) / 4 * 4;
+    if ((int64_t)kv.B * kv.H * kv.cap * pitch * 4 <= kMostScores) p.pitch = pitch;
+  }
   int64_t slots = std::max<int64_t>(1, (int64_t)num_sms() * (p.nq == 1 && !qlo ? 4 : p.nq == 1 ? 2 : 1) / p.row_blocks);
   // the same number of blocks for every head, where that leaves few slots empty:
   // with equal lengths no block then has to change heads
   const int64_t heads = (int64_t)kv.B * kv.H;
   if (slots >= heads && slots % heads * 10 <= slots) slots -= slots % heads;
   p.blocks = (int)std::max<int64_t>(1, std::min<int64_t>(slots, (units + kWarps - 1) / kWarps));
+  if (per_head <= kWholeUnits) {
+    p.whole = true;
+    p.blocks = (int)heads;
+  }
   p.slots = p.blocks + heads;
   return p;
 }
 
-// part, ml, lse
+// part, ml, and lse or scores
 void spaces(const Kv4& kv, const Plan& p, bool weigh, size_t* bytes) {
   const size_t rows = (size_t)p.slots * (p.prompt ? kPromptRows : p.rows_pad);
   bytes[0] = rows * kv.D * sizeof(float);
   bytes[1] = rows * sizeof(float2);
-  bytes[2] = weigh ? (size_t)kv.B * kv.H * p.rows_pad * sizeof(float) : 0;
+  const size_t heads = (size_t)kv.B * kv.H;
+  bytes[2] = !weigh ? 0 : p.pitch ? heads * kv.cap * p.pitch * sizeof(float) : heads * p.rows_pad * sizeof(float);
 }
 
 template <int D, bool QLO, bool GEN>
@@ -729,7 +821,11 @@ int run_attn(const Attn& a, const Plan& p, cudaStream_t st) {
     return launched("kv4_attn_kernel (attribute)");
   kern<<<dim3(p.blocks, p.row_blocks), 32 * kWarps, smem, st>>>(a);
   LQ_TRY(launched("kv4_attn_kernel"));
-  launch_pdl(kv4_combine_kernel, dim3((unsigned)(((int64_t)a.rows * a.kv.B * a.kv.H + 3) / 4)), dim3(128), 0, st, a);
+  const int heads = a.kv.B * a.kv.H;
+  const int out_blocks = a.whole ? 0 : (int)(((int64_t)a.rows * heads + 3) / 4);
+  const int64_t spread_blocks = a.scores ? (int64_t)(a.kv.cap + 255) / 256 * heads : 0;
+  if (out_blocks + spread_blocks == 0) return a.lse ? run_mass<D, QLO, GEN>(a, st) : LQ_OK;
+  launch_pdl(kv4_combine_kernel, dim3((unsigned)(out_blocks + spread_blocks)), dim3(128), 0, st, a, out_blocks);
   LQ_TRY(launched("kv4_combine_kernel"));
   return a.lse ? run_mass<D, QLO, GEN>(a, st) : LQ_OK;
 }
@@ -751,8 +847,8 @@ extern "C" size_t lq_kv4_attention_workspace_bytes(const lq_kv4_cache* cache, co
   if (!f || kv4_check(cache) != LQ_OK || f->Hq <= 0 || f->Sq <= 0 || f->Hq % cache->H) return 0;
   const Kv4 kv = kv4_of(cache);
   size_t b[3];
-  spaces(kv, plan_of(kv, f->Hq / cache->H * f->Sq, f->bound, f->q_dtype == LQ_F32), f->accumulate != 0, b);
-  return b[0] + b[1] + b[2];
+  spaces(kv, plan_of(kv, f->Hq / cache->H * f->Sq, f->bound, f->q_dtype == LQ_F32, f->accumulate != 0), f->accumulate != 0, b);
+  return b[0] + b[1] + b[2] + 16;
 }
 
 extern "C" int lq_kv4_attention(const lq_kv4_cache* cache, const lq_kv4_attn* f, const void* q, const int32_t* counts,
@@ -774,11 +870,11 @@ extern "C" int lq_kv4_attention(const lq_kv4_cache* cache, const lq_kv4_attn* f,
   LQ_REQUIRE((uintptr_t)q % (4 * dtype_size(f->q_dtype)) == 0 && ((f->q_sb | f->q_sh | f->q_ss) & 3) == 0, LQ_EALIGN,
              "query rows must start on multiples of 4 elements");
   const Kv4 kv = kv4_of(cache);
-  const Plan p = plan_of(kv, rows, f->bound, f->q_dtype == LQ_F32);
+  const Plan p = plan_of(kv, rows, f->bound, f->q_dtype == LQ_F32, f->accumulate != 0);
   size_t bytes[3];
   spaces(kv, p, f->accumulate != 0, bytes);
-  LQ_REQUIRE(workspace && workspace_bytes >= bytes[0] + bytes[1] + bytes[2], LQ_EINVAL, "workspace of %zu bytes needed",
-             bytes[0] + bytes[1] + bytes[2]);
+  LQ_REQUIRE(workspace && workspace_bytes >= bytes[0] + bytes[1] + bytes[2] + 16, LQ_EINVAL, "workspace of %zu bytes needed",
+             bytes[0] + bytes[1] + bytes[2] + 16);
   LQ_REQUIRE(aligned16(workspace) && aligned16(out), LQ_EALIGN, "output and workspace must be 16-byte aligned");
   Attn a;
   a.kv = kv;
@@ -797,7 +893,11 @@ extern "C" int lq_kv4_attention(const lq_kv4_cache* cache, const lq_kv4_attn* f,
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   a.part = reinterpret_cast<float*>(ws);
   a.ml = reinterpret_cast<float2*>(ws + bytes[0]);
-  a.lse = f->accumulate ? reinterpret_cast<float*>(ws + bytes[0] + bytes[1]) : nullptr;
+  float* extra = f->accumulate ? reinterpret_cast<float*>(ws + (bytes[0] + bytes[1] + 15) / 16 * 16) : nullptr;
+  a.lse = p.pitch ? nullptr : extra;
+  a.scores = p.pitch ? extra : nullptr;
+  a.pitch = p.pitch;
+  a.whole = p.whole;
   // a single query sees every token but for a window, a bias or a cap
   const bool gen = (f->Sq > 1 && (f->causal || counts)) || f->softcap > 0.0f || slopes || f->window > 0;
   cudaStream_t st = as_stream(stream);

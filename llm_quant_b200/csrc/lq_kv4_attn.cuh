@@ -24,7 +24,10 @@ struct Attn {
   uint8_t* out;
   float* part;    // [blocks + B H][rows_pad][D] unnormalised O
   float2* ml;     // [blocks + B H][rows_pad] running reference and sum
+  int whole;      // a block to a head: blocks = B H
   float* lse;     // [B H][rows_pad] log2 of the softmax denominators (weights collected), or NULL
+  float* scores;  // [B H][cap][pitch] scores, instead of lse, or NULL
+  int pitch;
 };
 
 constexpr int kPromptRows = 256;
@@ -122,7 +125,12 @@ struct Cut {
   }
   // units * cta / blocks, and the block that unit x falls to
   __device__ __forceinline__ int begin(int cta) const { return cta * base + cta * rem / blocks; }
-  __device__ __forceinline__ int owner(int x) const { return (int)(((int64_t)(x + 1) * blocks - 1) / units); }
+  __device__ __forceinline__ int owner(int x) const {
+    int c = min((int)__fdividef((x + 0.5f) * blocks, (float)units), blocks - 1);  // or a neighbour
+    while (begin(c) > x) --c;
+    while (begin(c + 1) <= x) ++c;
+    return c;
+  }
 };
 __device__ __forceinline__ int warp_sum(int u) {
 #pragma unroll
