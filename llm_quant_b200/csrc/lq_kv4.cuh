@@ -46,6 +46,26 @@ namespace {
 
 constexpr int kUnit = 32;  // tokens that a warp takes at a time (two tiles of 16)
 
+// Dynamic shared memory of a kernel, asked for once on each device (the call
+// takes as long as a small launch): one of these beside each kernel.
+struct DeviceOnce {
+  std::atomic<uint64_t> done{0};
+  int allow_smem(const void* kernel, int bytes, const char* what) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (done.load(std::memory_order_relaxed) & bit) return LQ_OK;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) {
+      set_error("%s: %d bytes of shared memory: %s", what, bytes, cudaGetErrorString(e));
+      cudaGetLastError();
+      return LQ_ECUDA;
+    }
+    if (dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
+    return LQ_OK;
+  }
+};
+
 inline Kv4 kv4_of(const lq_kv4_cache* c) {
   Kv4 k;
   k.k = static_cast<uint8_t*>(c->k_codes);

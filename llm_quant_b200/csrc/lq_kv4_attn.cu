@@ -794,7 +794,7 @@ Plan plan_of(const Kv4& kv, int64_t rows, int64_t bound, bool qlo, bool weigh) {
     p.whole = true;
     p.blocks = (int)heads;
   }
-  p.slots = p.blocks + heads;
+  p.slots = p.whole && !p.pitch ? 0 : p.blocks + heads;
   return p;
 }
 
@@ -802,7 +802,7 @@ Plan plan_of(const Kv4& kv, int64_t rows, int64_t bound, bool qlo, bool weigh) {
 void spaces(const Kv4& kv, const Plan& p, bool weigh, size_t* bytes) {
   const size_t rows = (size_t)p.slots * (p.prompt ? kPromptRows : p.rows_pad);
   bytes[0] = rows * kv.D * sizeof(float);
-  bytes[1] = rows * sizeof(float2);
+  bytes[1] = (rows * sizeof(float2) + 15) / 16 * 16;
   const size_t heads = (size_t)kv.B * kv.H;
   bytes[2] = !weigh ? 0 : p.pitch ? heads * kv.cap * p.pitch * sizeof(float) : heads * p.rows_pad * sizeof(float);
 }
@@ -817,8 +817,8 @@ template <int D, int NQ, bool QLO, bool GEN>
 int run_attn(const Attn& a, const Plan& p, cudaStream_t st) {
   constexpr int smem = sizeof(AttnShared<D, NQ, QLO>);
   auto kern = kv4_attn_kernel<D, NQ, QLO, GEN>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return launched("kv4_attn_kernel (attribute)");
+  static DeviceOnce once;
+  LQ_TRY(once.allow_smem((const void*)kern, smem, "kv4_attn_kernel"));
   kern<<<dim3(p.blocks, p.row_blocks), 32 * kWarps, smem, st>>>(a);
   LQ_TRY(launched("kv4_attn_kernel"));
   const int heads = a.kv.B * a.kv.H;
@@ -848,7 +848,7 @@ extern "C" size_t lq_kv4_attention_workspace_bytes(const lq_kv4_cache* cache, co
   const Kv4 kv = kv4_of(cache);
   size_t b[3];
   spaces(kv, plan_of(kv, f->Hq / cache->H * f->Sq, f->bound, f->q_dtype == LQ_F32, f->accumulate != 0), f->accumulate != 0, b);
-  return b[0] + b[1] + b[2] + 16;
+  return b[0] + b[1] + b[2];
 }
 
 extern "C" int lq_kv4_attention(const lq_kv4_cache* cache, const lq_kv4_attn* f, const void* q, const int32_t* counts,
@@ -873,8 +873,8 @@ extern "C" int lq_kv4_attention(const lq_kv4_cache* cache, const lq_kv4_attn* f,
   const Plan p = plan_of(kv, rows, f->bound, f->q_dtype == LQ_F32, f->accumulate != 0);
   size_t bytes[3];
   spaces(kv, p, f->accumulate != 0, bytes);
-  LQ_REQUIRE(workspace && workspace_bytes >= bytes[0] + bytes[1] + bytes[2] + 16, LQ_EINVAL, "workspace of %zu bytes needed",
-             bytes[0] + bytes[1] + bytes[2] + 16);
+  const size_t need = bytes[0] + bytes[1] + bytes[2];
+  LQ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), LQ_EINVAL, "workspace of %zu bytes needed", need);
   LQ_REQUIRE(aligned16(workspace) && aligned16(out), LQ_EALIGN, "output and workspace must be 16-byte aligned");
   Attn a;
   a.kv = kv;
@@ -893,7 +893,7 @@ extern "C" int lq_kv4_attention(const lq_kv4_cache* cache, const lq_kv4_attn* f,
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   a.part = reinterpret_cast<float*>(ws);
   a.ml = reinterpret_cast<float2*>(ws + bytes[0]);
-  float* extra = f->accumulate ? reinterpret_cast<float*>(ws + (bytes[0] + bytes[1] + 15) / 16 * 16) : nullptr;
+  float* extra = f->accumulate ? reinterpret_cast<float*>(ws + bytes[0] + bytes[1]) : nullptr;
   a.lse = p.pitch ? nullptr : extra;
   a.scores = p.pitch ? extra : nullptr;
   a.pitch = p.pitch;

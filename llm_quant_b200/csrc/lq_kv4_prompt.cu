@@ -1160,8 +1160,8 @@ template <typename T, int D>
 int run_weigh(const Attn& a, cudaStream_t st) {
   constexpr int smem = WeighShared<D>::bytes;
   auto kern = kv4_weigh_kernel<T, D>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return launched("kv4_weigh_kernel (attribute)");
+  static DeviceOnce once;
+  LQ_TRY(once.allow_smem((const void*)kern, smem, "kv4_weigh_kernel"));
   const int64_t items = (int64_t)((a.kv.cap + kTok - 1) / kTok) * a.kv.B * a.kv.H;
   LQ_REQUIRE(items <= INT32_MAX, LQ_ERANGE, "cache too large to collect weights");
   kern<<<(int)std::min<int64_t>(items, num_sms()), kWeighThreads, smem, st>>>(a, (int)items);
@@ -1173,8 +1173,8 @@ int run_prompt(const Attn& a, cudaStream_t st) {
   constexpr int smem = PromptShared<D>::bytes;
   static_assert(smem <= 227 * 1024, "shared memory per block");
   auto kern = kv4_prompt_kernel<T, D>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return launched("kv4_prompt_kernel (attribute)");
+  static DeviceOnce once;
+  LQ_TRY(once.allow_smem((const void*)kern, smem, "kv4_prompt_kernel"));
   kern<<<a.blocks, kPromptThreads, smem, st>>>(a);
   LQ_TRY(launched("kv4_prompt_kernel"));
   launch_pdl(kv4_prompt_combine_kernel<D>, dim3((unsigned)(a.rows_pad / kMergeRows * a.kv.B * a.kv.H)), dim3(128), 0, st, a);

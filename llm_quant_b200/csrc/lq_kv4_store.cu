@@ -64,34 +64,34 @@ __device__ __forceinline__ void group_range(float& lo, float& hi) {
   }
 }
 
-// Codes (4 nibbles, the first lowest) and parameter word of a token from the
-// 4 values of each of its LPT lanes.
-template <int LPT>
-__device__ __forceinline__ uint32_t quant4(const float* x, uint32_t& par) {
-  float lo = fmin_nan(fmin_nan(x[0], x[1]), fmin_nan(x[2], x[3]));
-  float hi = fmax_nan(fmax_nan(x[0], x[1]), fmax_nan(x[2], x[3]));
-  group_range<LPT>(lo, hi);
+// Scale, its reciprocal, zero point and parameter word from a token's range.
+struct Grid {
+  float s, inv;
+  int zero;
+  uint32_t par;
+};
+__device__ __forceinline__ Grid grid_of(float lo, float hi) {
   lo = fmin_nan(lo, 0.0f);
   hi = fmax_nan(hi, 0.0f);
-  const float s = Ty<__nv_bfloat16>::round(quotient(__fsub_rn(hi, lo), 15.0f, 0.066666667f));
-  if (!(s < INFINITY)) {  // NaN or infinite
-    par = 0x7fc0u;
-    return 0;
-  }
-  if (s < 7.888609052210118e-31f) {  // 2^-100
-    par = 0;
-    return 0;
-  }
-  // rint by adding 1.5 * 2^23, whose last mantissa bit is 1; codes are not below
-  // 0, since the zero point is the least value's, but the greatest may reach 16
-  const float inv = __frcp_rn(s), magic = 12582912.0f;
-  const float z = fminf(__fsub_rn(__fadd_rn(quotient(-lo, s, inv), magic), magic), 15.0f);
-  par = __float_as_uint(z) | (__float_as_uint(s) >> 16);
-  const int off = (int)z - 0x4b400000;
+  Grid g;
+  g.s = Ty<__nv_bfloat16>::round(quotient(__fsub_rn(hi, lo), 15.0f, 0.066666667f));
+  g.inv = __frcp_rn(g.s);
+  const bool real = g.s < INFINITY, some = g.s >= 7.888609052210118e-31f;  // not NaN or infinite; 2^-100 or more
+  // rint by adding 1.5 * 2^23, whose last mantissa bit is 1
+  const float z = fminf(__fsub_rn(__fadd_rn(quotient(-lo, g.s, g.inv), 12582912.0f), 12582912.0f), 15.0f);
+  g.par = !real ? 0x7fc0u : some ? __float_as_uint(z) | (__float_as_uint(g.s) >> 16) : 0u;
+  g.zero = real && some ? (int)z : 0;
+  if (!(real && some)) g.s = g.inv = 0.0f;  // codes 0 for finite values, and something for others
+  return g;
+}
+// Codes of 4 values, the first lowest.  They are not below 0, since the zero
+// point is the least value's, but the greatest may reach 16.
+__device__ __forceinline__ uint32_t codes4(const float* x, const Grid& g) {
+  const int off = g.zero - 0x4b400000;
   uint32_t w = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    w |= (uint32_t)min(__float_as_int(__fadd_rn(quotient(x[i], s, inv), magic)) + off, 15) << (4 * i);
+    w |= (uint32_t)(min(__float_as_int(__fadd_rn(quotient(x[i], g.s, g.inv), 12582912.0f)) + off, 15) & 15) << (4 * i);
   return w;
 }
 
@@ -125,10 +125,27 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4 kv, AppendArgs a, i
         for (int d = 0; d < 4; ++d) x[e][s][d] = 0.0f;
         if (live[e]) load4(static_cast<const T*>(a.x[s]) + b * a.sb[s] + h * a.sh[s] + (i0 + e) * a.ss[s] + 4 * l, x[e][s]);
       }
+    // the four ranges (token, K or V); a lane makes the grid of one of them
+    float lo = 0.0f, hi = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
+    for (int k = 0; k < 4; ++k) {
+      const float* y = x[k >> 1][k & 1];
+      float l4 = fmin_nan(fmin_nan(y[0], y[1]), fmin_nan(y[2], y[3]));
+      float h4 = fmax_nan(fmax_nan(y[0], y[1]), fmax_nan(y[2], y[3]));
+      group_range<LPT>(l4, h4);
+      if ((l & 3) == k) lo = l4, hi = h4;
+    }
+    const Grid mine = grid_of(lo, hi);
 #pragma unroll
-      for (int s = 0; s < 2; ++s) w[e][s] = quant4<LPT>(x[e][s], par[e][s]);
+    for (int k = 0; k < 4; ++k) {
+      const int src = (threadIdx.x & 31 & ~3) + k;
+      Grid g;
+      g.s = __shfl_sync(0xffffffffu, mine.s, src);
+      g.inv = __shfl_sync(0xffffffffu, mine.inv, src);
+      g.zero = __shfl_sync(0xffffffffu, mine.zero, src);
+      par[k >> 1][k & 1] = __shfl_sync(0xffffffffu, mine.par, src);
+      w[k >> 1][k & 1] = codes4(x[k >> 1][k & 1], g);
+    }
     const int64_t row = (int64_t)bh * kv.cap;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -582,8 +599,8 @@ extern "C" int lq_kv4_evict(const lq_kv4_cache* cache, int64_t keep, int64_t rec
   const int smem = 4 * (n_keys + (lists ? 2 * (int)n_moves : 0));
   cudaStream_t st = as_stream(stream);
   auto kern = kv.D == 128 ? kv4_evict_kernel<128> : kv4_evict_kernel<64>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return launched("kv4_evict_kernel (attribute)");
+  static DeviceOnce once[2];
+  LQ_TRY(once[kv.D == 128].allow_smem((const void*)kern, 4 * kEvictKeys, "kv4_evict_kernel"));
   kern<<<kv.B * kv.H, kEvictThreads, smem, st>>>(kv, a);
   return launched("kv4_evict_kernel");
 }

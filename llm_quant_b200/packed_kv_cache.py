@@ -214,6 +214,7 @@ class PackedKVCache(nn.Module):
         # 1/8 of an octave: the work is split by it, nothing else
         bound = st.cap if st.captured else st.bound
         step = 1 << max(5, bound.bit_length() - 4)
+        softcap = float(softcap)
         key = (q.dtype, q.shape, q.stride(), q.device, scale, causal, softcap, window, accumulate,
                (bound + step - 1) // step)
         form = st.forms.get(key)
@@ -225,14 +226,14 @@ class PackedKVCache(nn.Module):
                     st.forms.clear()
                 st.forms[key] = form
         ref, nbytes, _ = form
-        B, Hq, Sq, D = shape = q.shape
+        B, Hq, Sq, D = q.shape
         cn = None if counts is None else self._vector(counts, B, torch.int32, st, "attend: counts")
         sl = None if slopes is None else self._vector(slopes, Hq, torch.float32, st, "attend: slopes")
         pf = None if prefix is None else self._vector(prefix, B, torch.int32, st, "attend: prefix")
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         if Sq:
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-            self._call(st, "lq_kv4_attention", ref, q.data_ptr(), cn, sl, pf, out.data_ptr(), ws.data_ptr(), nbytes)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+            self._call(st, "lq_kv4_attention", ref, q.data_ptr(), cn, sl, pf, out.data_ptr(), _C.ptr(ws), nbytes)
         return out
 
     @staticmethod

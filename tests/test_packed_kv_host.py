@@ -19,20 +19,20 @@ def lib():
 def _cache(**kw):
     """A cache struct whose pointers are aligned but lead nowhere: no call that is refused may follow them."""
     from llm_quant_b200 import _C
-    f = dict(k_codes=4096, v_codes=4096, params=4096, positions=4096, mass=4096, state=4096, B=2, H=2, cap=64, D=64)
+    f = dict(k_codes=4096, v_codes=4096, params=4096, positions=4096, mass=4096, state=4096, B=2, H=2, cap=4096, D=64)
     f.update(kw)
     return _C.KV4Cache(*[f[n] for n, _ in _C.KV4Cache._fields_])
 
 
 def _form(**kw):
     from llm_quant_b200 import _C
-    f = dict(Hq=4, Sq=1, q_sb=64, q_sh=64, q_ss=64, bound=64, window=0, sm_scale=1.0, softcap=0.0, q_dtype=1, causal=0,
+    f = dict(Hq=4, Sq=1, q_sb=64, q_sh=64, q_ss=64, bound=4096, window=0, sm_scale=1.0, softcap=0.0, q_dtype=1, causal=0,
              accumulate=0)
     f.update(kw)
     return ctypes.byref(_C.KV4Attn(*[f[n] for n, _ in _C.KV4Attn._fields_]))
 
 
-BAD = [({"D": 96}, "head dim"), ({"cap": 40}, "multiple"), ({"B": 0}, "shape"), ({"H": -1}, "shape"),
+BAD = [({"D": 96}, "head dim"), ({"cap": 4040}, "multiple"), ({"B": 0}, "shape"), ({"H": -1}, "shape"),
        ({"cap": 1 << 31}, "too large"), ({"B": 1000, "H": 1000}, "too large"), ({"params": None}, "NULL"),
        ({"state": None}, "NULL"), ({"k_codes": 4097}, "aligned"), ({"params": 4104}, "aligned")]
 
@@ -60,14 +60,14 @@ def test_bad_arguments(lib):
     assert append(k=None) == -1 and append(dt=3) == -2 and append(S=-1) == -1
     assert append(k=4100) == -5 and append(st=(64, 64, 63, 64, 64, 64)) == -5
     assert append(S=0) == 0  # nothing to do
-    assert lib.lq_kv4_dequant(c, 65, 1, 4096, 4096, None) == -1
+    assert lib.lq_kv4_dequant(c, 4097, 1, 4096, 4096, None) == -1
     assert lib.lq_kv4_dequant(c, 4, 3, 4096, 4096, None) == -2
     assert lib.lq_kv4_dequant(c, 4, 1, 4098, 4096, None) == -5
     assert lib.lq_kv4_dequant(c, 0, 1, None, None, None) == 0
     for keep, recent, sinks in ((0, 0, 0), (4, 5, 0), (4, 2, 3), (4, -1, 0)):
         assert lib.lq_kv4_evict(c, keep, recent, sinks, 4096, 1 << 40, None) == -1
-    assert lib.lq_kv4_evict(c, 64, 0, 0, None, 0, None) == 0  # nothing can be over it
-    assert lib.lq_kv4_evict(c, 8, 0, 0, 4096, lib.lq_kv4_evict_workspace_bytes(2, 2, 64, 8) - 1, None) == -1
+    assert lib.lq_kv4_evict(c, 4096, 0, 0, None, 0, None) == 0  # nothing can be over it
+    assert lib.lq_kv4_evict(c, 8, 0, 0, 4096, lib.lq_kv4_evict_workspace_bytes(2, 2, 4096, 8) - 1, None) == -1
 
     def attend(q=4096, out=4096, ws=4096, nbytes=1 << 40, **kw):
         return lib.lq_kv4_attention(c, _form(**kw), q, None, None, None, out, ws, nbytes, None)
