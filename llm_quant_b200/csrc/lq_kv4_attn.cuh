@@ -52,6 +52,11 @@ __device__ __forceinline__ float lg2(float x) {
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 // tanh from the exponential: the error is about 2^-23 absolute, which is what a
 // capped score needs (tanh.approx is only good to 2^-11)
 __device__ __forceinline__ float tanh_exp(float x) {

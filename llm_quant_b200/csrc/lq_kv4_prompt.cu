@@ -277,6 +277,28 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
+// Bits lo .. hi - 1, as far as there are such.
+__device__ __forceinline__ uint32_t bits_of(int lo, int hi) {
+  lo = max(lo, 0);
+  hi = min(hi, 32);
+  return hi <= lo ? 0u : (0xffffffffu >> (32 - hi)) & (0xffffffffu << lo);
+}
+template <int N>  // products to scores
+__device__ __forceinline__ void scaled(uint32_t* y, const float* sk) {
+#pragma unroll
+  for (int k = 0; k < N; k += 4) {
+    const float4 f = *reinterpret_cast<const float4*>(sk + k);
+    y[k] = __float_as_uint(__uint_as_float(y[k]) * f.x), y[k + 1] = __float_as_uint(__uint_as_float(y[k + 1]) * f.y);
+    y[k + 2] = __float_as_uint(__uint_as_float(y[k + 2]) * f.z), y[k + 3] = __float_as_uint(__uint_as_float(y[k + 3]) * f.w);
+  }
+}
+template <int N>  // cap tanh(x) = cap - 2 cap / (1 + exp 2x): good to 2^-23 of the cap
+__device__ __forceinline__ void capped(uint32_t* y, float cap) {
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    y[k] = __float_as_uint(fmaf(-2.0f * cap, rcp(1.0f + ex2(2.0f * kLog2e * __uint_as_float(y[k]))), cap));
+}
+
 // Integers of 4 bits as operands: bias + code is exact in the type, and so is
 // its difference from bias + zero point.
 template <typename T> struct Ints;
@@ -512,53 +534,70 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
           tmem_st16(S + 16, p + 16);
         } else {
 #pragma unroll 1
-          for (int c = 0; c < 64; c += 16) {
-            uint32_t y[16], p[8];
-            tmem_ld16(S + c, y);
-            tmem_wait_ld16(y);
+          for (int c = 0; c < 64; c += 32) {
+            uint32_t y[32], p[16];
+            tmem_ld32(S + c, y);
+            tmem_wait_ld32(y);
+            // columns that the row sees: between two bounds, or before the prefix
+            uint32_t seen;
+            const int t = t0 + c;
+            if (ordered) {
+              seen = bits_of(a.window > 0 ? at - a.window + 1 - t : 0, a.causal ? at + 1 - t : 32) | bits_of(0, pre - t);
+            } else {
+              const int hi = a.causal ? at : INT_MAX, lo = a.window > 0 ? at - a.window + 1 : INT_MIN;
+              const int* pos = sc.pos[st] + 64 * (j & 1) + c;
+              seen = 0;
+#pragma unroll 8
+              for (int k = 0; k < 32; ++k) seen |= ((pos[k] <= hi && pos[k] >= lo) || pos[k] < pre ? 1u : 0u) << k;
+            }
+            seen &= valid ? bits_of(0, n - t) : 0u;
+            scaled<32>(y, sk + c);
+            if (a.cap > 0.0f) capped<32>(y, a.cap * kLog2e);
+            if (a.slopes) {
+              if (ordered) {
+                const float d = (float)(at - t);
+#pragma unroll
+                for (int k = 0; k < 32; ++k) y[k] = __float_as_uint(fmaf(-slope, fabsf(d - (float)k), __uint_as_float(y[k])));
+              } else {
+                const int* pos = sc.pos[st] + 64 * (j & 1) + c;
+#pragma unroll
+                for (int k = 0; k < 32; ++k) y[k] = __float_as_uint(fmaf(-slope, fabsf((float)(at - pos[k])), __uint_as_float(y[k])));
+              }
+            }
             float m = -INFINITY;
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              float x = __uint_as_float(y[k]) * sk[c + k];
-              if (a.cap > 0.0f) x = tanh_exp(x) * (a.cap * kLog2e);
-              const int t = t0 + c + k, pos = ordered ? t : sc.pos[st][64 * (j & 1) + c + k], back = at - pos;
-              if (a.slopes) x = fmaf(-slope, fabsf((float)back), x);
-              bool near = !a.causal || back >= 0;
-              if (a.window > 0) near = near && back < a.window;
-              x = valid && t < n && (near || pos < pre) ? x : -INFINITY;
-              y[k] = __float_as_uint(x);
-              m = fmaxf(m, x);
+            for (int k = 0; k < 32; ++k) {
+              if (!(seen >> k & 1)) y[k] = 0xff800000u;
+              m = fmaxf(m, __uint_as_float(y[k]));
             }
             if (__any_sync(0xffffffffu, m + (e + kHead - R) > kTop)) {
               const float before = R;
               raise(m);
-              // what is there already of this half tile's P'
-              const __half2 alpha = __float2half2_rn(ex2(before - R));
-#pragma unroll 1
-              for (int d = 0; d < c / 2; d += 8) {
-                tmem_ld8(S + d, p);
+              if (c) {  // the first half's P' is there already
+                const __half2 alpha = __float2half2_rn(ex2(before - R));
+                tmem_ld16(S, p);
+                tmem_wait_ld16(p);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
+                for (int k = 0; k < 16; ++k) {
                   const __half2 v = __hmul2(*reinterpret_cast<__half2*>(&p[k]), alpha);
                   p[k] = *reinterpret_cast<const uint32_t*>(&v);
                 }
-                tmem_st8(S + d, p);
+                tmem_st16(S, p);
               }
             }
             const float off = e + kHead - R;
+            float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int k = 0; k < 16; k += 2) {
-              float q[2];
-#pragma unroll
-              for (int d = 0; d < 2; ++d) {
-                const float v = __uint_as_float(y[k + d]);
-                q[d] = ex2(v + off);
-                sum += q[d];
-                q[d] = v == -INFINITY ? 0.0f : q[d] * sv[c + k + d];  // whatever the scale of a token that is not seen
-              }
-              p[k / 2] = h2(q[0], q[1]);
+            for (int k = 0; k < 32; k += 2) {
+              const float q0 = ex2(__uint_as_float(y[k]) + off), q1 = ex2(__uint_as_float(y[k + 1]) + off);
+              const float2 v = *reinterpret_cast<const float2*>(sv + c + k);
+              s4[k & 2] += q0;
+              s4[(k & 2) + 1] += q1;
+              // a token that is not seen has no weight, whatever its scale
+              p[k / 2] = h2(seen >> k & 1 ? q0 * v.x : 0.0f, seen >> (k + 1) & 1 ? q1 * v.y : 0.0f);
             }
-            tmem_st8(S + c / 2, p);
+            sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+            tmem_st16(S + c / 2, p);
           }
         }
         l = fmaf(sum, ex2(-e - kHead), l);
@@ -1020,22 +1059,32 @@ __global__ void __launch_bounds__(kWeighThreads, 1) kv4_weigh_kernel(const Attn 
           const float2 x0 = unpair(s2[0]), x1 = unpair(s2[1]);
           sum += (x0.x + x0.y) + (x1.x + x1.y);
         } else {
+          // rows that see the token: those between two, or all
+          const int64_t hi_r = a.window > 0 ? ((int64_t)pos + a.window - w.first) * a.G - rt * kTile : kTile;
+          const int64_t lo_r = a.causal ? ((int64_t)pos - w.first) * a.G - rt * kTile : 0;
+          const int lo = (int)max(min(lo_r, (int64_t)kTile), (int64_t)-1), hi = (int)max(min(hi_r, (int64_t)kTile), (int64_t)-1);
+          const float d = (float)pos;
 #pragma unroll 1
-          for (int c = 0; c < kTile; c += 16) {
-            uint32_t y[16];
-            tmem_ld16(S + c, y);
-            tmem_wait_ld16(y);
+          for (int c = 0; c < kTile; c += 32) {
+            uint32_t y[32];
+            tmem_ld32(S + c, y);
+            tmem_wait_ld32(y);
+            const uint32_t seen = pos < pre ? 0xffffffffu : bits_of(lo - c, hi - c);
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              float x = __uint_as_float(y[k]) * sk;
-              if (a.cap > 0.0f) x = tanh_exp(x) * (a.cap * kLog2e);
-              const int back = sc.at[st][c + k] - pos;
-              if (a.slopes) x = fmaf(-sc.slope[st][c + k], fabsf((float)back), x);
-              bool near = !a.causal || back >= 0;
-              if (a.window > 0) near = near && back < a.window;
-              const float p = ex2(x + sc.nl[st][c + k]);
-              if (near || pos < pre) sum += p;
+            for (int k = 0; k < 32; ++k) y[k] = __float_as_uint(__uint_as_float(y[k]) * sk);
+            if (a.cap > 0.0f) capped<32>(y, a.cap * kLog2e);
+            if (a.slopes) {
+#pragma unroll
+              for (int k = 0; k < 32; ++k)
+                y[k] = __float_as_uint(fmaf(-sc.slope[st][c + k], fabsf((float)sc.at[st][c + k] - d), __uint_as_float(y[k])));
             }
+            float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              const float p = ex2(__uint_as_float(y[k]) + sc.nl[st][c + k]);
+              s4[k & 3] += seen >> k & 1 ? p : 0.0f;
+            }
+            sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
           }
         }
         tc_fence_before();
