@@ -237,20 +237,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* r) {
       : "r"(addr)
       : "memory");
 }
-// with its wait
-__device__ __forceinline__ void tmem_ld8(uint32_t addr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-      : "r"(addr)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t* r) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(r[0]),
-               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
-}
 __device__ __forceinline__ uint64_t pair(float x, float y) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
@@ -876,60 +862,52 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
 }
 
-// A warp merges the parts of a row that blocks shared; zeros where there is
-// nothing to see.  kMergeRows rows of an item to a block.
+// 8 lanes merge the parts of a row that blocks shared, a block those of 16 rows;
+// zeros where there is nothing to see.
 constexpr int kMergeRows = 16;
 template <int D>
 __global__ void __launch_bounds__(128) kv4_prompt_combine_kernel(const Attn a) {
-  constexpr int V = D / 32;
+  constexpr int V = D / 32;  // vectors of 4 to a lane
   const int rts = a.rows_pad / kItem, item = blockIdx.x / (kItem / kMergeRows);
   const int j = item / a.kv.H, h = item % a.kv.H, b = j / rts, rt = j % rts;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int k0 = blockIdx.x % (kItem / kMergeRows) * kMergeRows;
-  if (rt * kItem + k0 >= a.rows) return;
+  const int k = blockIdx.x % (kItem / kMergeRows) * kMergeRows + threadIdx.x / 8, l8 = threadIdx.x & 7, r = rt * kItem + k;
   const Tiles t = tiles_of(a, b, rt);
   int all;
   const int begin = tiles_before(a, j, all) + h * t.count;
   Cut cut;
   cut.set(all, a.blocks);
   const int c0 = t.count ? cut.owner(begin) : 0, c1 = t.count ? cut.owner(begin + t.count - 1) : -1;
-  if (t.count && c0 == c1) return;
+  if ((t.count && c0 == c1) || r >= a.rows) return;
   pdl_wait();
-#pragma unroll 1
-  for (int k = k0 + warp; k < k0 + kMergeRows; k += 4) {
-    const int r = rt * kItem + k;
-    if (r >= a.rows) break;
-    float M = kNone, L = 0.0f, o[V];
+  float M = kNone, L = 0.0f;
+  float4 o[V];
 #pragma unroll
-    for (int d = 0; d < V; ++d) o[d] = 0.0f;
-    auto row_of = [&](int c) { return (int64_t)(2 * c + (cut.begin(c) >= begin ? 0 : 1)) * kItem + k; };
-    for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, a.ml[row_of(c)].x);
+  for (int d = 0; d < V; ++d) o[d] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 2
+  for (int c = c0; c <= c1; ++c) {
+    const int64_t row = (int64_t)(2 * c + (cut.begin(c) >= begin ? 0 : 1)) * kItem + k;
+    const float2 ml = a.ml[row];
+    float4 v[V];
 #pragma unroll
-    for (int m = 16; m > 0; m >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, m));
-#pragma unroll 4
-    for (int c = c0; c <= c1; ++c) {
-      const int64_t row = row_of(c);
-      const float2 ml = a.ml[row];
-      const float f = ex2(ml.x - M);
-      float v[V];
-      if constexpr (V == 4) {
-        const float4 x = *reinterpret_cast<const float4*>(a.part + row * D + V * lane);
-        v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
-      } else {
-        const float2 x = *reinterpret_cast<const float2*>(a.part + row * D + V * lane);
-        v[0] = x.x, v[1] = x.y;
-      }
-      L = fmaf(f, ml.y, L);
+    for (int d = 0; d < V; ++d) v[d] = *reinterpret_cast<const float4*>(a.part + row * D + 32 * d + 4 * l8);
+    const float m = fmaxf(M, ml.x), f = ex2(M - m), g = ex2(ml.x - m);
+    M = m;
+    L = fmaf(L, f, g * ml.y);
 #pragma unroll
-      for (int d = 0; d < V; ++d) o[d] = fmaf(f, v[d], o[d]);
+    for (int d = 0; d < V; ++d) {
+      o[d].x = fmaf(o[d].x, f, g * v[d].x), o[d].y = fmaf(o[d].y, f, g * v[d].y);
+      o[d].z = fmaf(o[d].z, f, g * v[d].z), o[d].w = fmaf(o[d].w, f, g * v[d].w);
     }
-    const float inv = L == 0.0f ? 0.0f : pow2(-(int)kHead) / L;
-    const int i = r / a.G, hq = h * a.G + r % a.G;
-    const int64_t at = (((int64_t)b * a.Hq + hq) * a.Sq + i) * D + V * lane;
-#pragma unroll
-    for (int d = 0; d < V; ++d) st_out(a.out, at + d, a.q_dtype, L == 0.0f ? 0.0f : o[d] * inv);
-    if (a.lse && lane == 0) a.lse[(int64_t)(b * a.kv.H + h) * a.rows_pad + r] = L == 0.0f ? INFINITY : M + lg2(L);
   }
+  const float inv = L == 0.0f ? 0.0f : pow2(-(int)kHead) / L;
+  const int i = div_g(a, r), hq = h * a.G + r - i * a.G;
+  const int64_t at = (((int64_t)b * a.Hq + hq) * a.Sq + i) * D;
+#pragma unroll
+  for (int d = 0; d < V; ++d) {
+    if (L == 0.0f) o[d] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // padding's O may be anything
+    st_out4(a.out, at + 32 * d + 4 * l8, a.q_dtype, o[d], inv);
+  }
+  if (a.lse && l8 == 0) a.lse[(int64_t)(b * a.kv.H + h) * a.rows_pad + r] = L == 0.0f ? INFINITY : M + lg2(L);
 }
 
 // ---------------------------------------------------------------------------
@@ -946,16 +924,17 @@ __global__ void __launch_bounds__(128) kv4_prompt_combine_kernel(const Attn a) {
 // tiles, 1024 cycles, beside 512 of the tensor cores.
 // ---------------------------------------------------------------------------
 constexpr int kWeighThreads = 416;
+constexpr int kQs = 4;  // stages of query rows; what belongs to rows is kept twice as long, for the sums
 template <int D>
 struct WeighShared {
   static constexpr int kOp = D / 64 * 16384;  // an operand of 128 rows
-  static constexpr int off_k = 0, off_q = kOp, off_s = off_q + 2 * kOp;
+  static constexpr int off_k = 0, off_q = kOp, off_s = off_q + kQs * kOp;
   struct Rows {
-    float nl[4][kTile], slope[4][kTile];  // -lse, bias
-    int at[4][kTile];
+    float nl[2 * kQs][kTile], slope[2 * kQs][kTile];  // -lse, bias
+    int at[2 * kQs][kTile];
     float sk[2][kTok], half[2][kTok];
     int pos[2][kTok];
-    uint64_t k_full, k_empty, q_full[2], q_empty[2], s_full[2], s_empty[2], half_full[2], drain;
+    uint64_t k_full, k_empty, q_full[kQs], q_empty[kQs], s_full[2], s_empty[2], half_full[2], drain;
     uint32_t tmem;
     int fail;
   };
@@ -994,9 +973,11 @@ __global__ void __launch_bounds__(kWeighThreads, 1) kv4_weigh_kernel(const Attn 
     sc.fail = 0;
     mbar_init(&sc.k_full, 4);
     mbar_init(&sc.k_empty, 1);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kQs; ++i) {
       mbar_init(&sc.q_full[i], 4);
       mbar_init(&sc.q_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&sc.s_full[i], 1);
       mbar_init(&sc.s_empty[i], 4);
       mbar_init(&sc.half_full[i], 4);
@@ -1028,7 +1009,7 @@ __global__ void __launch_bounds__(kWeighThreads, 1) kv4_weigh_kernel(const Attn 
       float sum = 0.0f, sk = 0.0f;
       int pos = t;
       for (int rt = w.lo + odd; rt < w.hi; rt += 2, ++mine) {
-        const int st = (tile + rt - w.lo) & 3;
+        const int st = (tile + rt - w.lo) % (2 * kQs);
         if (!wait_warp(&sc.s_full[wg], mine & 1)) { ok = false; break; }
         tc_fence_after();
         sk = sc.sk[item & 1][tid];
@@ -1134,7 +1115,7 @@ __global__ void __launch_bounds__(kWeighThreads, 1) kv4_weigh_kernel(const Attn 
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(&sc.k_full);
-      // ---- query rows, the next tile on its way while this one arrives ----
+      // ---- query rows, two tiles on their way while another arrives ----
       const float* lse = a.lse + (int64_t)(w.b * a.kv.H + w.h) * a.rows_pad;
       auto lse_of = [&](int rt) {
         const int r = rt * kTile + tid;
@@ -1142,24 +1123,29 @@ __global__ void __launch_bounds__(kWeighThreads, 1) kv4_weigh_kernel(const Attn 
       };
       float nl = lse_of(w.lo);
       for (int rt = w.lo; rt < w.hi; ++rt, ++tile) {
-        const int s2 = tile & 1, st = tile & 3;
-        if (tile >= 2 && !wait_warp(&sc.q_empty[s2], ((tile >> 1) - 1) & 1)) { ok = false; break; }
-        stage_rows<T, D>(smem + L::off_q + s2 * L::kOp, a, w.b, w.h, w.cnt, rt * kTile, tid);
+        const int qs = tile % kQs, st = tile % (2 * kQs);
+        if (tile >= kQs && !wait_warp(&sc.q_empty[qs], (tile / kQs - 1) & 1)) { ok = false; break; }
+        stage_rows<T, D>(smem + L::off_q + qs * L::kOp, a, w.b, w.h, w.cnt, rt * kTile, tid);
         sc.nl[st][tid] = nl;
         if (rt + 1 < w.hi) nl = lse_of(rt + 1);
         const int r = rt * kTile + tid, i = div_g(a, r);
         sc.at[st][tid] = w.first + i;
         if (a.slopes) sc.slope[st][tid] = r < a.rows ? a.slopes[w.h * a.G + r - i * a.G] * kLog2e : 0.0f;
-        if (rt > w.lo) {
-          staged<1>();
+        if (rt >= w.lo + 2) {
+          staged<2>();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&sc.q_full[s2 ^ 1]);
+          if (lane == 0) mbar_arrive(&sc.q_full[(tile - 2) % kQs]);
         }
       }
       if (!ok) break;
+      if (w.hi >= w.lo + 2) {
+        staged<1>();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sc.q_full[(tile - 2) % kQs]);
+      }
       staged<0>();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sc.q_full[(tile - 1) & 1]);
+      if (lane == 0) mbar_arrive(&sc.q_full[(tile - 1) % kQs]);
       ++item;
     }
     if (!ok) *fail = 1;
@@ -1176,19 +1162,19 @@ __global__ void __launch_bounds__(kWeighThreads, 1) kv4_weigh_kernel(const Attn 
       // row tile `tile` goes to group tile % 2, whichever item it is of
 #pragma unroll 1
       for (int i = 0; i < tiles; ++i, ++tile) {
-        const int s2 = tile & 1, wg = s2;
-        if (!wait_warp(&sc.q_full[s2], (tile >> 1) & 1)) { ok = false; break; }
+        const int qs = tile % kQs, wg = tile & 1;
+        if (!wait_warp(&sc.q_full[qs], (tile / kQs) & 1)) { ok = false; break; }
         if (used[wg] > 0 && !wait_warp(&sc.s_empty[wg], (used[wg] - 1) & 1)) { ok = false; break; }
         ++used[wg];
         tc_fence_after();
-        const uint64_t dk = sw128_desc(base + L::off_k), dq = sw128_desc(base + L::off_q + s2 * L::kOp);
+        const uint64_t dk = sw128_desc(base + L::off_k), dq = sw128_desc(base + L::off_q + qs * L::kOp);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const uint64_t step = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
           mma_ss(tm + wg * 128, dk + step, dq + step, idesc, k > 0);
         }
         commit(&sc.s_full[wg]);
-        commit(&sc.q_empty[s2]);
+        commit(&sc.q_empty[qs]);
       }
       commit(&sc.k_empty);
       ++item;
