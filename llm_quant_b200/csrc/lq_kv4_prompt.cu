@@ -800,44 +800,66 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
         if (!ok || !w.some) break;
         const int two = __reduce_max_sync(0xffffffffu, w.rt * kItem + kTile < a.rows ? 1 : 0);
         const int n_steps = 2 * __reduce_max_sync(0xffffffffu, w.u1 - w.u0);
-        // Slot i: PV of row tile i % 2, half tile i / 2, then S of the other row
-        // tile, which lies where the slot before last had its P' (the MMAs that
-        // read it are done by then).  The first three slots only have an S.  One
-        // copy of the code and short loops: unrolled, it did not fit the
+        // A slot is the PV of a row tile's half, then an S of the other row tile,
+        // which lies where the slot before last had its P' (the MMAs that read it
+        // are done by then).  Short code: unrolled further it did not fit the
         // instruction cache, and an MMA took 200 cycles to issue instead of 64.
+        auto pv = [&](int wg, int half, int vs, uint32_t fresh) {
+          const uint64_t dv = sw128_desc(base + L::off_v) + (uint32_t)((vs * L::kV + half * (D * 128)) >> 4);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mma_ts(tm + 256 + wg * 128, tm + wg * 128 + 64 * half + 8 * k, dv + ((k * 32) >> 4), idesc_o, k > 0 ? 1u : fresh);
+          commit(&sc.pv_done[wg][half]);
+        };
+        auto qk = [&](int wg, int half, int ks) {
+          // a step of 16 along K is 32 bytes of the swizzled rows, 64 are a half
+          const uint64_t dq = sw128_desc(base + L::off_q) + (uint32_t)((wg * (L::kQ / 2)) >> 4);
+          const uint64_t dk = sw128_desc(base + L::off_k) + (uint32_t)((ks * L::kK + half * 8192) >> 4);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint64_t step = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
+            mma_ss(tm + wg * 128 + 64 * half, dq + step, dk + step, idesc_s, k > 0);
+          }
+          commit(&sc.s_full[wg][half]);
+        };
+        // the first S of each half; whichever half comes first is half 0, since a piece has whole tiles
+        ok = wait_warp(&sc.k_full[unit & 1], (unit >> 1) & 1) && wait_warp(&sc.q_full[0], items[0]++ & 1);
+        if (ok && two) ok = wait_warp(&sc.q_full[1], items[1]++ & 1);
+        if (!ok) break;
+        tc_fence_after();
+        qk(0, 0, unit & 1);
+        if (two) qk(1, 0, unit & 1);
+        qk(0, 1, unit & 1);
 #pragma unroll 1
-        for (int i = -3; i < 2 * n_steps; ++i) {
-          const int wg = i & 1, j = i >> 1, u = unit + (j >> 1);
-          if (i >= 0 && (!wg || two)) {
-            const int x = steps[wg] + j;
-            if (!wg && !(j & 1)) ok = wait_warp(&sc.v_full[u & 1], (u >> 1) & 1);
-            if (!ok || !wait_warp(&sc.p_full[wg][x & 1], (x >> 1) & 1)) { ok = false; break; }
+        for (int t = 0; t < n_steps / 2; ++t) {
+          const int u = unit + t, s2 = u & 1, p0 = ((steps[0] >> 1) + t) & 1, p1 = ((steps[1] >> 1) + t) & 1;
+          const bool more = t + 1 < n_steps / 2;
+          if (!wait_warp(&sc.v_full[s2], (u >> 1) & 1) || !wait_warp(&sc.p_full[0][0], p0)) { ok = false; break; }
+          tc_fence_after();
+          pv(0, 0, s2, t > 0);
+          if (two) qk(1, 1, s2);
+          commit(&sc.k_empty[s2]);
+          if (two) {
+            if (!wait_warp(&sc.p_full[1][0], p1)) { ok = false; break; }
             tc_fence_after();
-            const uint64_t dv = sw128_desc(base + L::off_v + (u & 1) * L::kV + (j & 1) * (D * 128));
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              mma_ts(tm + 256 + wg * 128, tm + wg * 128 + 64 * (x & 1) + 8 * k, dv + ((k * 32) >> 4), idesc_o, j > 0 || k > 0);
-            commit(&sc.pv_done[wg][x & 1]);
-            if ((j & 1) && wg == two) commit(&sc.v_empty[u & 1]);
+            pv(1, 0, s2, t > 0);
           }
-          const int sg = wg ^ 1, sj = j + 1 + wg, su = unit + (sj >> 1);
-          if (sj < n_steps && (!sg || two)) {
-            const int x = steps[sg] + sj;
-            if (!sg && !(sj & 1)) ok = wait_warp(&sc.k_full[su & 1], (su >> 1) & 1);
-            if (sj == 0) ok = ok && wait_warp(&sc.q_full[sg], items[sg]++ & 1);
-            if (!ok) break;
+          if (more) {
+            if (!wait_warp(&sc.k_full[s2 ^ 1], ((u + 1) >> 1) & 1)) { ok = false; break; }
             tc_fence_after();
-            // a step of 16 along K is 32 bytes of the swizzled rows, 64 are a half
-            const uint64_t dq = sw128_desc(base + L::off_q + sg * (L::kQ / 2));
-            const uint64_t dk = sw128_desc(base + L::off_k + (su & 1) * L::kK + (sj & 1) * 8192);
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-              const uint64_t step = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
-              mma_ss(tm + sg * 128 + 64 * (x & 1), dq + step, dk + step, idesc_s, k > 0);
-            }
-            commit(&sc.s_full[sg][x & 1]);
-            if ((sj & 1) && sg == two) commit(&sc.k_empty[su & 1]);
+            qk(0, 0, s2 ^ 1);
           }
+          if (!wait_warp(&sc.p_full[0][1], p0)) { ok = false; break; }
+          tc_fence_after();
+          pv(0, 1, s2, 1);
+          if (two) {
+            if (more) qk(1, 0, s2 ^ 1);
+            if (!wait_warp(&sc.p_full[1][1], p1)) { ok = false; break; }
+            tc_fence_after();
+            pv(1, 1, s2, 1);
+          }
+          commit(&sc.v_empty[s2]);
+          if (more) qk(0, 1, s2 ^ 1);
         }
         if (!ok) break;
         steps[0] += n_steps;
