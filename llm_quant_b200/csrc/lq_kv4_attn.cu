@@ -862,7 +862,7 @@ extern "C" int lq_kv4_attention(const lq_kv4_cache* cache, const lq_kv4_attn* f,
              (long long)f->Hq, (long long)cache->H);
   LQ_REQUIRE(f->Sq >= 0 && f->bound >= 0, LQ_EINVAL, "bad shape");
   LQ_REQUIRE(f->softcap >= 0.0f, LQ_EINVAL, "softcap must not be negative");
-  LQ_REQUIRE(f->window >= 0 && f->window <= INT32_MAX, LQ_EINVAL, "bad window");
+  LQ_REQUIRE(f->window >= 0 && f->window <= (1 << 30), LQ_EINVAL, "window %lld: 0 (none) to 2^30", (long long)f->window);
   const int64_t rows = f->Hq / cache->H * f->Sq;
   if (rows == 0) return LQ_OK;
   LQ_REQUIRE(f->Hq / cache->H <= 4096 && rows <= 16 * 65535 && rows * cache->B * cache->H <= INT32_MAX, LQ_ERANGE, "too many query rows");

@@ -141,6 +141,8 @@ class PackedKVCache(nn.Module):
                 raise ValueError(f"PackedKVCache: head dim {D}: 64 or 128 supported")
             if B == 0 or H == 0:
                 raise ValueError("PackedKVCache: empty batch or no heads")
+            if S > self.max_seq_len:
+                raise ValueError(f"PackedKVCache.append: {S} tokens do not fit into {self.max_seq_len}")
             if B * H > 65535:
                 raise ValueError("PackedKVCache: more than 65535 (sequence, head) pairs")
             st = _LayerStore(B, H, (self.max_seq_len + 31) // 32 * 32, D, key.device)
@@ -208,6 +210,11 @@ class PackedKVCache(nn.Module):
         nothing gives zeros, and so does padding.  ``accumulate`` adds the
         weight that each token got from all queries to ``attention_mass``.
 
+        Scores are summed in fp32 from exact products; with 16-bit queries each
+        probability is rounded once, to fp16 beside the greatest of its row,
+        before it meets the values.  Positions are int32, ``window`` is at most
+        2^30, a group has at most 4096 query heads.
+
         Inference only: no gradient is computed."""
         st = self._layer(layer_idx, "attend")
         q = query if query.__class__ is torch.Tensor and query.ndim == 4 else self._query(st, query)
@@ -249,10 +256,10 @@ class PackedKVCache(nn.Module):
     @staticmethod
     def _form(st: _LayerStore, q: torch.Tensor, scale, causal, softcap, window, accumulate, bound):
         """The call's arguments but for the tensors: checked once for each form."""
-        if not 0.0 <= softcap < float("inf"):
-            raise ValueError(f"PackedKVCache.attend: softcap {softcap} must be finite and not negative")
-        if not 0 <= window < 2 ** 31:
-            raise ValueError(f"PackedKVCache.attend: window {window} must not be negative")
+        if not (softcap == 0.0 or 1e-20 <= softcap < float("inf")):
+            raise ValueError(f"PackedKVCache.attend: softcap {softcap} must be finite and not negative (0: none)")
+        if not 0 <= window <= 2 ** 30:
+            raise ValueError(f"PackedKVCache.attend: window {window} must be 0 (none) to 2^30")
         sb, sh, ss, _ = q.stride()
         c = _C.KV4Attn(q.shape[1], q.shape[2], sb, sh, ss, bound, window,
                        q.shape[3] ** -0.5 if scale is None else scale, softcap, _C.TORCH_TO_LQ[q.dtype], bool(causal),
@@ -290,6 +297,14 @@ class PackedKVCache(nn.Module):
         """Tokens that replayed appends found no room for: int32 scalar on the device (the cache's own)."""
         st = self._layer(layer_idx, "dropped")
         return st.state[2 * st.B + 1]
+
+    def check(self, layer_idx: int) -> None:
+        """Wait for the layer's work and raise LQError if a kernel gave up a wait
+        on the device (its results are incomplete then)."""
+        st = self._layer(layer_idx, "check")
+        status = int(st.state[2 * st.B + 3])
+        if status:
+            raise _C.LQError("PackedKVCache", status, "a wait on the device ran out")
 
     def positions(self, layer_idx: int) -> torch.Tensor:
         """Position of the token in each slot, -1 where it is empty: int32

@@ -346,6 +346,35 @@ def test_prompt_chunks(L, dtype, B, H, G, D, T, S):
     check(L, cache, q, **_form("all", B, H * G))
 
 
+def test_scales_of_every_size_in_chunks(L):
+    """As for single tokens, but no scale differs by more than 2^16 within 128
+    tokens: P is kept beside the greatest V scale of a tile there."""
+    for dtype in (torch.float16, torch.bfloat16):
+        k, v = (x.clone() for x in _kv(1, 2, 700, 64, dtype, 8))
+        v *= torch.exp2(torch.randint(-6, 6, (1, 2, 700, 1), generator=_gen(1), device="cuda").float()).to(dtype)
+        k *= torch.exp2(torch.randint(-10, 2, (1, 2, 700, 1), generator=_gen(2), device="cuda").float()).to(dtype)
+        k[:, :, 10:20] = 0
+        v[:, :, 15:30] = 0
+        v[:, :, 256:400] = 0  # a whole tile of zeros
+        cache = L.PackedKVCache(1, 700)
+        cache.append(0, k, v)
+        q = _q(1, 4, 100, 64, dtype, 9)
+        check(L, cache, q, causal=True)
+        check(L, cache, q * 30, causal=True, scale=0.4)  # peaked: references are raised again and again
+        check(L, cache, q, softcap=5.0, window=300)
+
+
+def test_windows_and_prefixes_of_any_size(L):
+    cache = L.PackedKVCache(1, 300)
+    cache.append(0, *_kv(2, 2, 300, 64, torch.bfloat16, 8), counts=_ints(300, 77))
+    for S in (1, 50):
+        q = _q(2, 8, S, 64, torch.bfloat16, S)
+        for window in (1, 2, 64, 128, 299, 300, 2 ** 30):
+            for prefix in (None, _ints(0, -5), _ints(2 ** 31 - 1, 1), _ints(130, 64)):
+                for causal in (True, False):
+                    check(L, cache, q, causal=causal, window=window, prefix=prefix)
+
+
 def test_query_layouts_give_the_same(L):
     cache = L.PackedKVCache(1, 256)
     cache.append(0, *_kv(2, 2, 256, 64, torch.bfloat16, 1))
@@ -438,6 +467,15 @@ def test_evict_ties_and_odd_masses(L):
     check_evict(cache, 100, recent=50)
 
 
+def test_evict_more_tokens_than_shared_memory_holds(L):
+    T, keep = 60001, 55000
+    cache = L.PackedKVCache(1, T)
+    cache.append(0, *_kv(1, 1, T, 64, torch.float16, 1))
+    cache.attention_mass(0).copy_(torch.exp(3 * torch.randn(1, 1, T, generator=_gen(1), device="cuda")))
+    check_evict(cache, keep, recent=50, sinks=4)
+    check(L, cache, _q(1, 4, 30, 64, torch.float16, 2), causal=True, window=40000)
+
+
 def test_masks_go_by_position_after_eviction(L):
     for dtype in ALL:
         B, H, G, D = 2, 2, 4, 128
@@ -490,6 +528,7 @@ def test_decode_loop_with_a_budget(L):
             else:
                 cache.evict(layer, keep, recent=16, sinks=4)
     assert cache.lengths(1).tolist() == [96, 96] and cache.seq_len == 96
+    cache.check(0), cache.check(1)
     cache.reset()
     assert cache.seq_len == 0 and cache.lengths(0).tolist() == [0, 0]
     cache.append(0, *_kv(B, H, 5, D, torch.bfloat16, 1))
@@ -652,7 +691,7 @@ def test_refusals_on_the_device(L):
         cache.attend(0, q.long())
     with pytest.raises(RuntimeError, match="CUDA"):
         cache.attend(0, q.cpu())
-    for kw in ({"softcap": -1.0}, {"softcap": float("nan")}, {"softcap": float("inf")}, {"window": -1},
+    for kw in ({"softcap": -1.0}, {"softcap": float("nan")}, {"softcap": float("inf")}, {"softcap": 1e-30}, {"window": -1}, {"window": 2 ** 30 + 1},
                {"slopes": torch.ones(4, device="cuda", dtype=torch.float16)}, {"slopes": torch.ones(3, device="cuda")},
                {"slopes": torch.ones(8, device="cuda")[::2]}, {"prefix": torch.ones(2, device="cuda")},
                {"prefix": 4}, {"counts": [1, 1]}):
@@ -665,6 +704,8 @@ def test_refusals_on_the_device(L):
         cache.get(0, torch.int8)
     with pytest.raises(ValueError, match="head dim"):
         L.PackedKVCache(1, 8).append(0, torch.zeros(1, 1, 1, 96, device="cuda"), torch.zeros(1, 1, 1, 96, device="cuda"))
+    with pytest.raises(ValueError, match="fit"):
+        L.PackedKVCache(1, 8).append(0, k, v)
     assert cache.lengths(0).tolist() == [20, 20]
     # empty work is no work
     cache.append(0, k[:, :, :0], v[:, :, :0])

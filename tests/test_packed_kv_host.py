@@ -73,7 +73,7 @@ def test_bad_arguments(lib):
         return lib.lq_kv4_attention(c, _form(**kw), q, None, None, None, out, ws, nbytes, None)
 
     assert attend(Hq=3) == -1 and attend(Hq=0) == -1 and attend(q_dtype=3) == -2 and attend(softcap=-1.0) == -1
-    assert attend(q=None) == -1 and attend(out=None) == -1 and attend(window=-1) == -1 and attend(Sq=-1) == -1
+    assert attend(q=None) == -1 and attend(out=None) == -1 and attend(window=-1) == -1 and attend(window=1 << 31) == -1 and attend(Sq=-1) == -1
     assert attend(ws=None) == -1 and attend(ws=4100) == -5 and attend(q=4100) == -5 and attend(q_ss=66) == -5
     assert lib.lq_kv4_attention(c, None, 4096, None, None, None, 4096, 4096, 1 << 40, None) == -1
     need = lib.lq_kv4_attention_workspace_bytes(c, _form())
