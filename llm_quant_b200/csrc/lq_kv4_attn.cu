@@ -599,7 +599,7 @@ __global__ void __launch_bounds__(32 * kWarps, NQ == 1 && !QLO ? 4 : NQ == 1 ? 2
 // the blocks that shared the head; zeros where there is nothing to see.  Heads
 // that one block covered are done already.
 // The blocks behind them, if weights are collected from the scores that the
-// attention kernel left: 256 tokens of a head each, mass[t] += sum over the rows
+// attention kernel left: 256 tokens of a head at a time, mass[t] += sum over the rows
 // of exp2(x[r, t] - lse[r]), with lse from the same partial results.
 // The lengths are older than the kernel before this one, so they are read while
 // it still runs.
@@ -608,17 +608,18 @@ __global__ void __launch_bounds__(128) kv4_combine_kernel(const Attn a, int out_
   const bool spread = (int)blockIdx.x >= out_blocks;
   const int heads = a.kv.B * a.kv.H;
   int bh, qr = 0, t0 = 0;
+  bool idle = false;  // nothing to do, but no block ends before the kernel it waits for
   if (spread) {
     bh = (blockIdx.x - out_blocks) % heads;
     t0 = (blockIdx.x - out_blocks) / heads * 256;
   } else {
     const int item = blockIdx.x * 4 + warp;
-    if (item >= a.rows * heads) return;
-    bh = item / a.rows, qr = item % a.rows;
+    idle = item >= a.rows * heads;
+    bh = idle ? 0 : item / a.rows, qr = idle ? 0 : item % a.rows;
   }
   const int b = bh / a.kv.H, h = bh % a.kv.H;
   const Seq s = seq_of(a, b);
-  if (spread && (s.count == 0 || t0 >= s.n)) return;
+  if (spread) idle = s.count == 0 || t0 >= s.n;
   int c0 = bh, c1 = bh;  // the blocks that had a part of the head
   if (!a.whole) {
     int all;
@@ -627,8 +628,8 @@ __global__ void __launch_bounds__(128) kv4_combine_kernel(const Attn a, int out_
     cut.set(all, a.blocks);
     c0 = s.count ? cut.owner(begin) : 0, c1 = s.count ? cut.owner(begin + s.count - 1) : -1;
   }
-  if (!spread && s.count && c0 == c1) return;
   pdl_wait();
+  if (idle || (!spread && s.count && c0 == c1)) return;
   const int64_t first = (int64_t)(c0 + bh) * a.rows_pad;
   auto reference = [&](int r) {
     float m = kNone;
@@ -651,9 +652,10 @@ __global__ void __launch_bounds__(128) kv4_combine_kernel(const Attn a, int out_
       if (lane == 0) lse[r] = L == 0.0f ? INFINITY : M + lg2(L);
     }
     __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int t = t0 + 128 * k + threadIdx.x;
+    // from 256 tokens to the next that no other block has
+    const int step = ((int)gridDim.x - out_blocks) / heads * 256;
+    for (int64_t t2 = t0; t2 < s.n; t2 += (t2 & 128) ? step - 128 : 128) {
+      const int t = (int)t2 + threadIdx.x;
       if (t >= s.n) break;
       const int u = t / kUnit;
       if (u >= s.pre && u < s.pre + s.gap) continue;  // behind the window: no scores were made
@@ -760,7 +762,7 @@ struct Plan {
   int pitch;      // scores kept per token for the collected weight; 0: none are kept
 };
 // Up to so many units a head is left to one block, and nothing has to be merged
-// (B=1, 8 heads, 500 tokens: 10 us in two kernels, see below for one).
+// (B=1, 8 heads, 500 tokens: 6.7 us, 10 us in two kernels).
 constexpr int kWholeUnits = 16;
 constexpr int64_t kMostScores = 256 << 20;  // bytes of kept scores
 constexpr int kFewRows = 16;  // up to here a row of the cache is read once by this file's kernel
@@ -809,7 +811,7 @@ void spaces(const Kv4& kv, const Plan& p, bool weigh, size_t* bytes) {
 
 template <int D, bool QLO, bool GEN>
 int run_mass(const Attn& a, cudaStream_t st) {
-  kv4_mass_kernel<D, QLO, GEN><<<dim3((a.kv.cap + 63) / 64, a.kv.B * a.kv.H), 128, 0, st>>>(a);
+  kv4_mass_kernel<D, QLO, GEN><<<dim3((a.bound + 63) / 64, a.kv.B * a.kv.H), 128, 0, st>>>(a);
   return launched("kv4_mass_kernel");
 }
 
@@ -823,7 +825,7 @@ int run_attn(const Attn& a, const Plan& p, cudaStream_t st) {
   LQ_TRY(launched("kv4_attn_kernel"));
   const int heads = a.kv.B * a.kv.H;
   const int out_blocks = a.whole ? 0 : (int)(((int64_t)a.rows * heads + 3) / 4);
-  const int64_t spread_blocks = a.scores ? (int64_t)(a.kv.cap + 255) / 256 * heads : 0;
+  const int64_t spread_blocks = a.scores ? (int64_t)(a.bound + 255) / 256 * heads : 0;
   if (out_blocks + spread_blocks == 0) return a.lse ? run_mass<D, QLO, GEN>(a, st) : LQ_OK;
   launch_pdl(kv4_combine_kernel, dim3((unsigned)(out_blocks + spread_blocks)), dim3(128), 0, st, a, out_blocks);
   LQ_TRY(launched("kv4_combine_kernel"));
@@ -886,6 +888,7 @@ extern "C" int lq_kv4_attention(const lq_kv4_cache* cache, const lq_kv4_attn* f,
   a.sm = f->sm_scale, a.cap = f->softcap;
   a.slopes = slopes, a.prefix = prefix;
   a.causal = f->causal != 0, a.window = (int)f->window;
+  a.bound = (int)std::min<int64_t>(std::max<int64_t>(f->bound, 1), kv.cap);
   a.g_mul = a.G == 1 ? 0u : (uint32_t)(0x100000000ull / a.G) + 1u;
   a.q_wide = (uintptr_t)q % 16 == 0 && ((f->q_sb | f->q_sh | f->q_ss) * dtype_size(f->q_dtype)) % 16 == 0;
   a.blocks = p.blocks;
@@ -902,6 +905,8 @@ extern "C" int lq_kv4_attention(const lq_kv4_cache* cache, const lq_kv4_attn* f,
   const bool gen = (f->Sq > 1 && (f->causal || counts)) || f->softcap > 0.0f || slopes || f->window > 0;
   cudaStream_t st = as_stream(stream);
   if (p.prompt) {
+    LQ_REQUIRE((int64_t)p.rows_pad / kPromptRows * kv.B * kv.H <= INT32_MAX / ((kv.cap + 127) / 128), LQ_ERANGE,
+               "%lld query rows by %d tokens are too many for one call", (long long)rows, kv.cap);
     return kv4_prompt(a, st);
   }
   return kv.D == 128 ? run_attn_d<128>(a, p, gen, st) : run_attn_d<64>(a, p, gen, st);

@@ -18,6 +18,7 @@ struct Attn {
   const float* slopes;
   const int32_t* prefix;
   int causal, window;
+  int bound;      // tokens of the longest sequence as far as the host knows: for grids, nothing else
   uint32_t g_mul; // ceil(2^32 / G), 0 for G = 1
   int q_wide;     // query rows start on multiples of 16 bytes
   int blocks;     // blocks of the split (at most; never more than there are units)

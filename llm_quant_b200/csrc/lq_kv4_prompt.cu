@@ -899,8 +899,8 @@ __global__ void __launch_bounds__(128) kv4_prompt_combine_kernel(const Attn a) {
   Cut cut;
   cut.set(all, a.blocks);
   const int c0 = t.count ? cut.owner(begin) : 0, c1 = t.count ? cut.owner(begin + t.count - 1) : -1;
+  pdl_wait();  // no block ends before the kernel it waits for
   if ((t.count && c0 == c1) || r >= a.rows) return;
-  pdl_wait();
   float M = kNone, L = 0.0f;
   float4 o[V];
 #pragma unroll
@@ -984,7 +984,7 @@ __device__ __forceinline__ WeighItem weigh_item(const Attn& a, int idx) {
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kWeighThreads, 1) kv4_weigh_kernel(const Attn a, int items) {
+__global__ void __launch_bounds__(kWeighThreads, 1) kv4_weigh_kernel(const Attn a) {
   using L = WeighShared<D>;
   constexpr int W = D / 32;
   extern __shared__ __align__(16) uint8_t raw[];
@@ -1018,6 +1018,9 @@ __global__ void __launch_bounds__(kWeighThreads, 1) kv4_weigh_kernel(const Attn 
   const uint32_t tmem = sc.tmem;
   volatile int* fail = &sc.fail;
   const float fk = a.sm * (a.cap > 0.0f ? 1.0f / a.cap : kLog2e);
+  int longest = 0;
+  for (int b = lane; b < a.kv.B; b += 32) longest = max(longest, min(a.kv.len[b], a.kv.cap));
+  const int items = (__reduce_max_sync(0xffffffffu, longest) + kTok - 1) / kTok * a.kv.B * a.kv.H;
 
   if (warp < 8) {
     const int wg = warp >> 2, tid = threadIdx.x & 127;
@@ -1221,7 +1224,7 @@ int run_weigh(const Attn& a, cudaStream_t st) {
   LQ_TRY(once.allow_smem((const void*)kern, smem, "kv4_weigh_kernel"));
   const int64_t items = (int64_t)((a.kv.cap + kTok - 1) / kTok) * a.kv.B * a.kv.H;
   LQ_REQUIRE(items <= INT32_MAX, LQ_ERANGE, "cache too large to collect weights");
-  kern<<<(int)std::min<int64_t>(items, num_sms()), kWeighThreads, smem, st>>>(a, (int)items);
+  kern<<<(int)std::min<int64_t>(items, num_sms()), kWeighThreads, smem, st>>>(a);
   return launched("kv4_weigh_kernel");
 }
 

@@ -24,7 +24,8 @@ Lengths live on the device and nothing here reads them back, so every method
 can be captured into a CUDA graph and replayed: a replayed ``append`` goes on
 where the last one stopped.  The host keeps an upper bound of them
 (``seq_len``), which sizes what ``get``, ``positions`` and ``attention_mass``
-return; inside a capture, and from then on until ``reset``, it is the capacity.
+return; once an ``append`` or ``evict`` was captured, and until ``reset``, it is
+the capacity.
 
 One cache is used by one stream at a time (``attend`` without ``accumulate``
 and ``get`` may overlap each other), as any tensor that is changed in place.
@@ -212,7 +213,9 @@ class PackedKVCache(nn.Module):
 
         Scores are summed in fp32 from exact products; with 16-bit queries each
         probability is rounded once, to fp16 beside the greatest of its row,
-        before it meets the values.  Positions are int32, ``window`` is at most
+        before it meets the values.  More than 16 such queries to a kv head also
+        round it to 2^-24 of 2^8 and the greatest V scale among 128 slots: tokens
+        with a scale below 2^-20 of that lose bits.  Positions are int32, ``window`` is at most
         2^30, a group has at most 4096 query heads.
 
         Inference only: no gradient is computed."""
@@ -271,20 +274,22 @@ class PackedKVCache(nn.Module):
         """Cut every sequence back to ``keep`` tokens per kv head: the
         ``recent`` last ones and those at positions below ``sinks`` stay, then
         the ones with the greatest ``attention_mass`` (equal mass: from the
-        lowest slot up; NaN counts as greatest).  Heads keep tokens of their
+        lowest slot up; NaN counts as greatest, less than 0 as 0).  Heads keep tokens of their
         own.  Sequences that hold no more than ``keep`` are left alone."""
         st = self._layer(layer_idx, "evict")
         if keep < 1 or recent < 0 or sinks < 0 or recent + sinks > keep:
             raise ValueError(f"PackedKVCache.evict: keep {keep} must be positive and hold the {recent} recent and "
                              f"{sinks} first tokens")
-        if keep >= st.cap or (not st.captured and keep >= st.bound):
+        capturing = torch.cuda.is_current_stream_capturing()
+        if keep >= st.cap or (keep >= st.bound and not st.captured and not capturing):
             return
         nbytes = _C.lib().lq_kv4_evict_workspace_bytes(st.B, st.H, st.cap, keep)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=st.device)
         self._call(st, "lq_kv4_evict", keep, recent, sinks, ws.data_ptr(), nbytes)
-        if torch.cuda.is_current_stream_capturing():
+        if capturing:
             st.captured = True
-        if not st.captured:
+            st.bound = self.max_seq_len
+        elif not st.captured:
             st.bound = min(st.bound, keep)
 
     # -- what the cache holds --------------------------------------------------------

@@ -295,6 +295,20 @@ def test_nan_tokens_stay_behind_masks(L):
     nan = torch.isnan(out).all(-1)
     at = torch.arange(82, 90, device="cuda")
     assert torch.equal(nan[0, :2], (at - 40 < 46).expand(2, -1)) and torch.equal(nan[0, 2:], (at - 50 < 46).expand(2, -1))
+    # and in chunks
+    k, v = (x.clone() for x in _kv(1, 2, 400, 64, torch.bfloat16, 2))
+    k[:, 0, 140] = float("nan")
+    v[:, 1, 150] = float("-inf")
+    cache = L.PackedKVCache(1, 400)
+    cache.append(0, k, v)
+    q = _q(1, 4, 300, 64, torch.bfloat16, 3)
+    p = torch.arange(100, 400, device="cuda")
+    for window in (60, 0):
+        nan = torch.isnan(cache.attend(0, q, causal=True, window=window)).all(-1)
+        some = torch.isnan(cache.attend(0, q, causal=True, window=window)).any(-1)
+        for heads, t in ((slice(0, 2), 140), (slice(2, 4), 150)):
+            want = ((p >= t) & (p - t < (window or 1000))).expand(2, -1)
+            assert torch.equal(nan[0, heads], want) and torch.equal(some[0, heads], want)
 
 
 # ---- attention: chunks and score forms ---------------------------------------------------------------------------------
@@ -594,6 +608,65 @@ def test_replayed_appends_stop_at_the_room(L):
     out = cache.attend(0, _q(2, 2, 1, 64, torch.float16, 1))
     assert torch.isfinite(out).all()
     del graph
+
+
+def test_replayed_evictions_start_with_little(L):
+    """Captured while nothing had to go; the appends between replays are eager."""
+    cache = L.PackedKVCache(1, 64)
+    cache.append(0, *_kv(2, 1, 10, 64, torch.float16, 0))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.evict(0, 20, recent=20)
+    assert cache.seq_len == 64
+    for n in range(4):
+        cache.append(0, *_kv(2, 1, 9, 64, torch.float16, n))
+        graph.replay()
+        assert cache.lengths(0).tolist() == [min(20, 10 + 9 * (n + 1))] * 2
+    assert sorted(cache.positions(0)[1, 0, :20].tolist()) == list(range(26, 46))
+    cache.reset()
+    assert cache.seq_len == 0
+    del graph
+
+
+def test_replayed_attention_outgrows_its_capture(L):
+    """Captured with few tokens, replayed with many: grids are made for few."""
+    for S, dtype in ((1, torch.bfloat16), (30, torch.bfloat16), (30, torch.float32)):
+        cache, twin = L.PackedKVCache(1, 3000), L.PackedKVCache(1, 3000)
+        for c in (cache, twin):
+            c.append(0, *_kv(2, 2, 40, 64, dtype, 0), counts=_ints(40, 33))
+        q = _q(2, 4, S, 64, dtype, 1)
+        cache.attend(0, q, causal=True, accumulate=True)
+        torch.cuda.synchronize()
+        cache.attention_mass(0).zero_()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = cache.attend(0, q, causal=True, accumulate=True)
+        for c in (cache, twin):
+            c.append(0, *_kv(2, 2, 2900, 64, dtype, 2), counts=_ints(2900, 1700))
+        graph.replay()
+        ref, bound, m, mb, _ = reference(twin, 0, q, causal=True)
+        assert ((out.double() - ref).abs() <= bound).all()
+        assert ((cache.attention_mass(0).double() - m).abs() <= mb).all()
+        cache.check(0)
+        del graph
+
+
+def test_collected_weight_without_kept_scores(L):
+    """So much room that the scores of a call would take more than 256 MB."""
+    cache = L.PackedKVCache(1, 2 ** 22 + 64)
+    cache.append(0, *_kv(1, 1, 3000, 64, torch.bfloat16, 0))
+    for kw in ({}, dict(softcap=20.0, window=700)):
+        check(L, cache, _q(1, 16, 1, 64, torch.bfloat16, 1), **kw)
+
+
+def test_whole_heads_and_cut_ones(L):
+    """Lengths around those where a block takes a whole head, and scales of either sign."""
+    for T in (480, 511, 512, 513, 600, 1100):
+        cache = L.PackedKVCache(1, T)
+        cache.append(0, *_kv(2, 3, T, 128, torch.float16, T), counts=_ints(T, T // 2))
+        for scale in (None, 0.0, -0.1):
+            check(L, cache, _q(2, 6, 1, 128, torch.float16, 1), scale=scale)
+            check(L, cache, _q(2, 6, 40, 128, torch.float16, 1), scale=scale, causal=True)
 
 
 def test_two_calls_at_once_and_other_streams(L):
