@@ -603,23 +603,24 @@ __global__ void __launch_bounds__(32 * kWarps, NQ == 1 && !QLO ? 4 : NQ == 1 ? 2
 // of exp2(x[r, t] - lse[r]), with lse from the same partial results.
 // The lengths are older than the kernel before this one, so they are read while
 // it still runs.
+template <int D, bool WEIGH>
 __global__ void __launch_bounds__(128) kv4_combine_kernel(const Attn a, int out_blocks) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, D = a.kv.D, V = D / 32;
-  const bool spread = (int)blockIdx.x >= out_blocks;
+  constexpr int V = D / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+  const bool spread = WEIGH && (int)blockIdx.x >= out_blocks;
   const int heads = a.kv.B * a.kv.H;
   int bh, qr = 0, t0 = 0;
-  bool idle = false;  // nothing to do, but no block ends before the kernel it waits for
   if (spread) {
     bh = (blockIdx.x - out_blocks) % heads;
     t0 = (blockIdx.x - out_blocks) / heads * 256;
   } else {
     const int item = blockIdx.x * 4 + warp;
-    idle = item >= a.rows * heads;
-    bh = idle ? 0 : item / a.rows, qr = idle ? 0 : item % a.rows;
+    if (item >= a.rows * heads) return pdl_wait();  // no block ends before the kernel that it waits for
+    bh = item / a.rows, qr = item % a.rows;
   }
   const int b = bh / a.kv.H, h = bh % a.kv.H;
   const Seq s = seq_of(a, b);
-  if (spread) idle = s.count == 0 || t0 >= s.n;
+  if (spread && (s.count == 0 || t0 >= s.n)) return pdl_wait();
   int c0 = bh, c1 = bh;  // the blocks that had a part of the head
   if (!a.whole) {
     int all;
@@ -629,7 +630,7 @@ __global__ void __launch_bounds__(128) kv4_combine_kernel(const Attn a, int out_
     c0 = s.count ? cut.owner(begin) : 0, c1 = s.count ? cut.owner(begin + s.count - 1) : -1;
   }
   pdl_wait();
-  if (idle || (!spread && s.count && c0 == c1)) return;
+  if (!spread && s.count && c0 == c1) return;
   const int64_t first = (int64_t)(c0 + bh) * a.rows_pad;
   auto reference = [&](int r) {
     float m = kNone;
@@ -638,7 +639,7 @@ __global__ void __launch_bounds__(128) kv4_combine_kernel(const Attn a, int out_
     for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
     return m;
   };
-  if (spread) {
+  if constexpr (WEIGH) if (spread) {
     __shared__ float lse[16];
     for (int r = warp; r < a.rows; r += 4) {
       const float M = reference(r);
@@ -672,27 +673,48 @@ __global__ void __launch_bounds__(128) kv4_combine_kernel(const Attn a, int out_
     }
     return;
   }
+  // a lane has the factor of a part: loads of the parts wait for nothing but the wait above
   const float M = reference(qr);
   float L = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-  for (int c = 0; c <= c1 - c0; ++c) {
-    const int64_t i = first + qr + (int64_t)c * a.rows_pad;
-    const float2 ml = a.ml[i];
-    const float f = ex2(ml.x - M);
-    L = fmaf(f, ml.y, L);
+#pragma unroll 1
+  for (int base = 0; base <= c1 - c0; base += 32) {
+    const int64_t i = first + qr + (int64_t)base * a.rows_pad;
+    const int n = min(32, c1 - c0 + 1 - base);
+    float f = 0.0f;
+    if (lane < n) {
+      const float2 ml = a.ml[i + (int64_t)lane * a.rows_pad];
+      f = ex2(ml.x - M);
+      L = fmaf(f, ml.y, L);
+    }
     const float* p = a.part + i * D + V * lane;
-    if (V == 4) {
-      const float4 v = *reinterpret_cast<const float4*>(p);
-      o[0] = fmaf(f, v.x, o[0]), o[1] = fmaf(f, v.y, o[1]), o[2] = fmaf(f, v.z, o[2]), o[3] = fmaf(f, v.w, o[3]);
-    } else {
-      const float2 v = *reinterpret_cast<const float2*>(p);
-      o[0] = fmaf(f, v.x, o[0]), o[1] = fmaf(f, v.y, o[1]);
+#pragma unroll 1
+    for (int c = 0; c < n; c += 8) {  // behind the last part: that one again, with factor 0
+      float v[8][V];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float* from = p + (int64_t)min(c + k, n - 1) * a.rows_pad * D;
+        if constexpr (V == 4) *reinterpret_cast<float4*>(v[k]) = *reinterpret_cast<const float4*>(from);
+        else *reinterpret_cast<float2*>(v[k]) = *reinterpret_cast<const float2*>(from);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float fc = __shfl_sync(0xffffffffu, f, c + k);
+#pragma unroll
+        for (int d = 0; d < V; ++d) o[d] = fmaf(fc, v[k][d], o[d]);
+      }
     }
   }
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1) L += __shfl_xor_sync(0xffffffffu, L, k);
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
   const int iq = div_g(a, qr), hq = h * a.G + qr - iq * a.G;
   const int64_t at = (((int64_t)b * a.Hq + hq) * a.Sq + iq) * D + V * lane;
-  for (int i = 0; i < V; ++i) st_out(a.out, at + i, a.q_dtype, o[i] * inv);
+  if constexpr (V == 4) {
+    st_out4(a.out, at, a.q_dtype, make_float4(o[0], o[1], o[2], o[3]), inv);
+  } else {
+    st_out(a.out, at, a.q_dtype, o[0] * inv);
+    st_out(a.out, at + 1, a.q_dtype, o[1] * inv);
+  }
   if (a.lse && lane == 0) a.lse[(int64_t)bh * a.rows_pad + qr] = L == 0.0f ? INFINITY : M + lg2(L);
 }
 
@@ -827,7 +849,7 @@ int run_attn(const Attn& a, const Plan& p, cudaStream_t st) {
   const int out_blocks = a.whole ? 0 : (int)(((int64_t)a.rows * heads + 3) / 4);
   const int64_t spread_blocks = a.scores ? (int64_t)(a.bound + 255) / 256 * heads : 0;
   if (out_blocks + spread_blocks == 0) return a.lse ? run_mass<D, QLO, GEN>(a, st) : LQ_OK;
-  launch_pdl(kv4_combine_kernel, dim3((unsigned)(out_blocks + spread_blocks)), dim3(128), 0, st, a, out_blocks);
+  launch_pdl(a.scores ? kv4_combine_kernel<D, true> : kv4_combine_kernel<D, false>, dim3((unsigned)(out_blocks + spread_blocks)), dim3(128), 0, st, a, out_blocks);
   LQ_TRY(launched("kv4_combine_kernel"));
   return a.lse ? run_mass<D, QLO, GEN>(a, st) : LQ_OK;
 }
