@@ -2,6 +2,7 @@
 // (layout: lq_kv4.cuh).  Compiled without contraction: the quantization below
 // is a fixed sequence of fp32 operations.
 #include <algorithm>
+#include <type_traits>
 
 #include "lq_kv4.cuh"
 
@@ -27,20 +28,16 @@ struct AppendArgs {
 };
 
 template <typename T>
-__device__ __forceinline__ void load4(const T* p, float* x) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 v = __ldg(reinterpret_cast<const float4*>(p));
-    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-  } else {
-    union {
-      uint2 u;
-      T t[4];
-    } v;
-    v.u = __ldg(reinterpret_cast<const uint2*>(p));
+union Four {  // values as they are loaded
+  typename std::conditional<sizeof(T) == 4, uint4, uint2>::type u;
+  T t[4];
+  __device__ __forceinline__ Four() : u{} {}
+  __device__ __forceinline__ void load(const T* p) { u = __ldg(reinterpret_cast<const decltype(u)*>(p)); }
+  __device__ __forceinline__ void to(float* x) const {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = Ty<T>::to_f(v.t[i]);
+    for (int i = 0; i < 4; ++i) x[i] = Ty<T>::to_f(t[i]);
   }
-}
+};
 
 // x / y, correctly rounded, from inv = 1 / y correctly rounded: a quotient within
 // an ulp, its remainder (exact by fma), and one correction (Markstein); for
@@ -86,13 +83,23 @@ __device__ __forceinline__ Grid grid_of(float lo, float hi) {
 }
 // Codes of 4 values, the first lowest.  They are not below 0, since the zero
 // point is the least value's, but the greatest may reach 16.
+// 16-bit values have 11 bits at most and the scale has 8, so a quotient that is
+// no tie is 2^-12 or more away from one: both 2 x and (2 k + 1) s are multiples
+// of 2^-11 s there.  x / s rounded to 2^-13 (by adding 1.5 * 2^10; the
+// reciprocal is off by 2^-20 at most) then goes to the same integer as x / s
+// itself, ties included, and no exact quotient is needed.
+template <typename T>
 __device__ __forceinline__ uint32_t codes4(const float* x, const Grid& g) {
   const int off = g.zero - 0x4b400000;
   uint32_t w = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    w |= (uint32_t)(min(__float_as_int(__fadd_rn(quotient(x[i], g.s, g.inv), 12582912.0f)) + off, 15) & 15) << (4 * i);
-  return w;
+  for (int i = 3; i >= 0; --i) {
+    float y;  // 1.5 * 2^23 + rint(x / s)
+    if constexpr (sizeof(T) == 2) y = __fadd_rn(__fmaf_rn(x[i], g.inv, 1536.0f), 12582912.0f - 1536.0f);
+    else y = __fadd_rn(quotient(x[i], g.s, g.inv), 12582912.0f);
+    w = w * 16 + (uint32_t)__viaddmin_s32(__float_as_int(y), off, 15);
+  }
+  return w & 0xffffu;  // a token that is not finite keeps what it gets to itself
 }
 
 // A group of D / 4 lanes takes the two tokens that share words of V (slots 2j,
@@ -107,25 +114,33 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4 kv, AppendArgs a, i
   const int bh = blockIdx.y, b = bh / kv.H, h = bh % kv.H;
   const int cnt = a.counts ? min(max(a.counts[b], 0), a.S) : a.S;
   const int len = kv.len[b], next = kv.next[b];
+  const int most = min(cnt, kv.cap - len);  // tokens that find room
+  const T* from[2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s) from[s] = static_cast<const T*>(a.x[s]) + b * a.sb[s] + h * a.sh[s] + 4 * l;
+  Four<T> raw[2][2];
+  auto first_of = [&](int group) { return 2 * (group * PPB + pair) - (len & 1); };  // first token of the pair
+  auto fetch = [&](int group) {
+    const int i0 = first_of(group);
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (i0 + e >= 0 && i0 + e < most) raw[e][s].load(from[s] + (i0 + e) * a.ss[s]);
+  };
+  if ((int)blockIdx.x < groups) fetch(blockIdx.x);
   for (int group = blockIdx.x; group < groups; group += gridDim.x) {
-    const int i0 = 2 * (group * PPB + pair) - (len & 1);  // first token of the pair
+    const int i0 = first_of(group);
     if (i0 - 2 * pair >= cnt) break;  // nothing for the whole block any more
     uint32_t par[2][2], w[2][2];
-    bool live[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int i = i0 + e;
-      live[e] = i >= 0 && i < cnt && (int64_t)len + i < kv.cap;
-    }
+    const bool live[2] = {i0 >= 0 && i0 < most, i0 + 1 < most};
     float x[2][2][4];
 #pragma unroll
     for (int e = 0; e < 2; ++e)
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-#pragma unroll
-        for (int d = 0; d < 4; ++d) x[e][s][d] = 0.0f;
-        if (live[e]) load4(static_cast<const T*>(a.x[s]) + b * a.sb[s] + h * a.sh[s] + (i0 + e) * a.ss[s] + 4 * l, x[e][s]);
-      }
+      for (int s = 0; s < 2; ++s) raw[e][s].to(x[e][s]);
+    // the next pair's values arrive while this one's are worked on
+    if (group + (int)gridDim.x < groups) fetch(group + gridDim.x);
     // the four ranges (token, K or V); a lane makes the grid of one of them
     float lo = 0.0f, hi = 0.0f;
 #pragma unroll
@@ -145,7 +160,7 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4 kv, AppendArgs a, i
       g.inv = __shfl_sync(0xffffffffu, mine.inv, src);
       g.zero = __shfl_sync(0xffffffffu, mine.zero, src);
       par[k >> 1][k & 1] = __shfl_sync(0xffffffffu, mine.par, src);
-      w[k >> 1][k & 1] = codes4(x[k >> 1][k & 1], g);
+      w[k >> 1][k & 1] = codes4<T>(x[k >> 1][k & 1], g);
     }
     const int64_t row = (int64_t)bh * kv.cap;
 #pragma unroll

@@ -191,6 +191,29 @@ def test_counts_and_padding(L):
     assert cache.get(0) is None and cache.seq_len == 0
 
 
+@pytest.mark.parametrize("dtype", ALL)
+def test_values_halfway_between_codes(L, dtype):
+    """x / scale = k + 1/2 exactly, and the values beside those."""
+    toks = []
+    for m in range(4, 8) if dtype == torch.bfloat16 else range(16, 64):  # (2k + 1) m fits the type
+        s = m * 2.0 ** -7
+        for zero in (0, 3, 8):
+            x = torch.arange(64, dtype=torch.float64) % 15 + 0.5 - zero
+            x[0], x[1] = -zero, 15 - zero
+            x = (x * s).to(dtype)
+            assert torch.equal(x.double()[2:], ((torch.arange(64) % 15 + 0.5 - zero) * s).double()[2:])
+            toks.append(x)
+            up = x.float() * (1 + 2 * EPS[dtype])
+            up[:2] = x[:2].float()
+            toks += [up.to(dtype), (2 * x.float() - up).to(dtype)]
+    k = torch.stack(toks).cuda()[None, None]
+    cache = L.PackedKVCache(1, k.shape[2])
+    cache.append(0, k, k.flip(2))
+    a, b = cache.get(0)
+    ref, _ = quantized(k)
+    assert np.array_equal(a.cpu().numpy(), ref) and np.array_equal(b.flip(2).cpu().numpy(), ref)
+
+
 def test_unusual_tokens(L):
     """All equal, all zero, one-sided, tiny, huge, NaN and infinite tokens."""
     D = 64
