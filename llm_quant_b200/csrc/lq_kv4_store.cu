@@ -106,14 +106,18 @@ __device__ __forceinline__ uint32_t codes4(const float* x, const Grid& g) {
 // 2j + 1), so that V is written in whole words too.  The blocks
 // of a head go over its pairs in turn: twice as many blocks as the GPU holds, so that
 // heads of unequal lengths even out, and no more, since each counts at the ticket
-// (64 heads x up to 2048 tokens: 32, 27, 30, 38 us with 1, 2, 4, 8 times as many).
+// (64 heads x up to 2048 tokens: 21.6, 18.7, 20.8 us with 1, 2, 3 times as many).
+// 64 registers: 4 blocks per SM (20.3 us with 3).
+// Bound by instructions: some 300 to 512 values, a third of them for the codes;
+// 48 MB in 18.7 us are 2.6 TB/s.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) kv4_append_kernel(Kv4 kv, AppendArgs a, int groups) {
+__global__ void __launch_bounds__(256, 4) kv4_append_kernel(Kv4 kv, AppendArgs a, int groups) {
   constexpr int LPT = D / 4, PPB = 256 / LPT, W = D / 32;  // lanes per token, pairs per block
   const int l = threadIdx.x % LPT, pair = threadIdx.x / LPT;
   const int bh = blockIdx.y, b = bh / kv.H, h = bh % kv.H;
   const int cnt = a.counts ? min(max(a.counts[b], 0), a.S) : a.S;
   const int len = kv.len[b], next = kv.next[b];
+  const int64_t row = (int64_t)bh * kv.cap;
   const int most = min(cnt, kv.cap - len);  // tokens that find room
   const T* from[2];
 #pragma unroll
@@ -132,7 +136,7 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4 kv, AppendArgs a, i
   for (int group = blockIdx.x; group < groups; group += gridDim.x) {
     const int i0 = first_of(group);
     if (i0 - 2 * pair >= cnt) break;  // nothing for the whole block any more
-    uint32_t par[2][2], w[2][2];
+    uint32_t w[2][2];
     const bool live[2] = {i0 >= 0 && i0 < most, i0 + 1 < most};
     float x[2][2][4];
 #pragma unroll
@@ -155,29 +159,27 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4 kv, AppendArgs a, i
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int src = (threadIdx.x & 31 & ~3) + k;
-      Grid g;
-      g.s = __shfl_sync(0xffffffffu, mine.s, src);
+      Grid g = mine;
+      if constexpr (sizeof(T) == 4) g.s = __shfl_sync(0xffffffffu, mine.s, src);
       g.inv = __shfl_sync(0xffffffffu, mine.inv, src);
       g.zero = __shfl_sync(0xffffffffu, mine.zero, src);
-      par[k >> 1][k & 1] = __shfl_sync(0xffffffffu, mine.par, src);
       w[k >> 1][k & 1] = codes4<T>(x[k >> 1][k & 1], g);
     }
-    const int64_t row = (int64_t)bh * kv.cap;
+    // Two lanes make a word of K, even values in its low half, odd ones in its
+    // high half: the even lane the first token's, the odd lane the second's.
+    uint32_t kw[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      // two lanes make a word of K: even values in its low half, odd ones in its high half
       const uint32_t k = w[e][0];
-      uint32_t kw = ((k & 0xf) | ((k >> 4) & 0xf0) | ((k << 12) & 0xf0000) | ((k << 8) & 0xf00000)) << (8 * (l & 1));
-      kw |= __shfl_xor_sync(0xffffffffu, kw, 1);
-      if (!live[e]) continue;
-      const int64_t t = row + len + i0 + e;
-      if (!(l & 1)) *reinterpret_cast<uint32_t*>(kv.k + t * (D / 2) + 2 * l) = kw;
-      if (l == 0) {
-        kv.par[t] = make_uint2(par[e][0], par[e][1]);
-        kv.pos[t] = next + i0 + e;
-        kv.mass[t] = 0.0f;
-      }
+      kw[e] = ((k & 0xf) | ((k >> 4) & 0xf0) | ((k << 12) & 0xf0000) | ((k << 8) & 0xf00000)) << (8 * (l & 1));
     }
+    const uint32_t word = (l & 1 ? kw[1] : kw[0]) | __shfl_xor_sync(0xffffffffu, l & 1 ? kw[0] : kw[1], 1);
+    const int64_t t0 = row + len + i0;
+    if ((l & 1 ? live[1] : live[0])) *reinterpret_cast<uint32_t*>(kv.k + (t0 + (l & 1)) * (D / 2) + 2 * (l & ~1)) = word;
+    // lanes 0-3 have the parameters of both tokens' K and V; 4-7 set positions and weights
+    if (l < 4 && (l & 2 ? live[1] : live[0])) reinterpret_cast<uint32_t*>(kv.par + t0)[l] = mine.par;
+    if (l >= 4 && l < 8 && (l & 1 ? live[1] : live[0]))
+      (l < 6 ? kv.pos : reinterpret_cast<int32_t*>(kv.mass))[t0 + (l & 1)] = l < 6 ? next + i0 + (l & 1) : 0;
     uint8_t* v = kv.v + row * (D / 2) + v_unit((int64_t)len + i0, l, W);  // the pair's word
     if (live[0] && live[1]) *reinterpret_cast<uint32_t*>(v) = w[0][1] | (w[1][1] << 16);
     else if (live[0]) *reinterpret_cast<uint16_t*>(v) = (uint16_t)w[0][1];
