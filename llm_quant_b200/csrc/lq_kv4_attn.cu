@@ -30,6 +30,11 @@
 // fill the GPU alike.  The lengths are read on the device.  A head that one
 // block covers is finished there; partial results of the others are merged by
 // kv4_combine_kernel, a programmatic dependent launch.
+//
+// Bound and measured (D = 128): 8 sequences x 8 kv heads x 4 of 8192 tokens 21.6
+// us, merge 4.7 (71 MB, 3.3 TB/s); 16 of up to 20011 tokens, groups of 8, 47.2 us,
+// merge 5.3 (196 MB, 4.2 TB/s).  The copies alone take 15 and 35.6 us; the rest
+// is what mma.sync and the nibbles add (half of the MMAs taken out: -13 %).
 #include <algorithm>
 
 #include "lq_kv4_attn.cuh"
