@@ -316,14 +316,14 @@ class PackedKVCache(nn.Module):
         [B, H, seq_len] (the cache's own).  Until something is evicted slot t
         holds position t; then the order of slots means nothing."""
         st = self._layer(layer_idx, "positions")
-        return st.positions[:, :, :st.bound]
+        return st.positions.narrow(2, 0, st.bound)
 
     def attention_mass(self, layer_idx: int) -> torch.Tensor:
         """Attention weight that each slot's token collected (``attend`` with
         ``accumulate``), 0 where it is empty: float32 [B, H, seq_len], the
         cache's own, so it can be decayed or replaced in place."""
         st = self._layer(layer_idx, "attention_mass")
-        return st.mass[:, :, :st.bound]
+        return st.mass.narrow(2, 0, st.bound)
 
     def reset(self, layer_idx: Optional[int] = None) -> None:
         """Clear one layer, or all; the buffers stay."""
