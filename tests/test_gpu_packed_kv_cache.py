@@ -383,6 +383,27 @@ def test_prompt_chunks(L, dtype, B, H, G, D, T, S):
     check(L, cache, q, **_form("all", B, H * G))
 
 
+@pytest.mark.parametrize("dtype,D", [(torch.float16, 128), (torch.bfloat16, 64)])
+def test_chunks_with_rows_on_8_bytes(L, dtype, D):
+    """Rows that only 8-byte copies can load, and the same rows on 16 bytes."""
+    cache = L.PackedKVCache(1, 500)
+    cache.append(0, *_kv(2, 2, 500, D, dtype, 1), counts=_ints(500, 301))
+    wide = torch.randn(2, 6, 90, D + 4, generator=_gen(2), device="cuda").to(dtype)
+    q = wide[..., 4:]
+    assert q.data_ptr() % 16 == 8 and q.stride(2) % 8 == 4
+    out = check(L, cache, q, causal=True)
+    assert torch.equal(out, cache.attend(0, q.contiguous(), causal=True))
+
+
+@pytest.mark.parametrize("G,S", [(300, 1), (129, 3), (1000, 2), (17, 1), (7, 61)])
+def test_many_query_heads(L, G, S):
+    """Groups that are no power of two and larger than a tile."""
+    cache = L.PackedKVCache(1, 700)
+    cache.append(0, *_kv(1, 2, 700, 64, torch.float16, 3))
+    slopes = torch.rand(2 * G, generator=_gen(4), device="cuda") * 0.1
+    check(L, cache, _q(1, 2 * G, S, 64, torch.float16, 5), causal=True, slopes=slopes, window=333)
+
+
 def test_scales_of_every_size_in_chunks(L):
     """As for single tokens, but no scale differs by more than 2^16 within 128
     tokens: P is kept beside the greatest V scale of a tile there."""
