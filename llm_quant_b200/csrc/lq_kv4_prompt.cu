@@ -962,7 +962,10 @@ struct WeighShared {
     int at[2 * kQs][kTile];
     float sk[2][kTok], half[2][kTok];
     int pos[2][kTok];
-    uint64_t k_full, k_empty, q_full[kQs], q_empty[kQs], s_full[2], s_empty[2], half_full[2], drain;
+    // item_done: the eight warps of the sums are through with an item of this parity,
+    // whose half, sk and pos may then be another's.  An item of one row tile gives one group
+    // nothing to wait for, so that it could be two items ahead of the other.
+    uint64_t k_full, k_empty, q_full[kQs], q_empty[kQs], s_full[2], s_empty[2], half_full[2], item_done[2], drain;
     uint32_t tmem;
     int fail;
   };
@@ -1009,6 +1012,7 @@ __global__ void __launch_bounds__(kWeighThreads, 1) kv4_weigh_kernel(const Attn 
       mbar_init(&sc.s_full[i], 1);
       mbar_init(&sc.s_empty[i], 4);
       mbar_init(&sc.half_full[i], 4);
+      mbar_init(&sc.item_done[i], 8);
     }
     mbar_init(&sc.drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -1106,6 +1110,7 @@ __global__ void __launch_bounds__(kWeighThreads, 1) kv4_weigh_kernel(const Attn 
       if (!ok) break;
       // the groups' sums, and what the token had
       if (wg == 1) {
+        if (item >= 2 && !wait_warp(&sc.item_done[item & 1], ((item >> 1) - 1) & 1)) { ok = false; break; }
         sc.half[item & 1][tid] = sum;
         __syncwarp();
         if (lane == 0) mbar_arrive(&sc.half_full[item & 1]);
@@ -1113,6 +1118,8 @@ __global__ void __launch_bounds__(kWeighThreads, 1) kv4_weigh_kernel(const Attn 
         if (!wait_warp(&sc.half_full[item & 1], (item >> 1) & 1)) { ok = false; break; }
         if (t < w.n) a.kv.mass[(int64_t)(w.b * a.kv.H + w.h) * a.kv.cap + t] += sum + sc.half[item & 1][tid];
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sc.item_done[item & 1]);
       ++item;
       tile += w.hi - w.lo;
     }
@@ -1130,6 +1137,7 @@ __global__ void __launch_bounds__(kWeighThreads, 1) kv4_weigh_kernel(const Attn 
       const bool in = t < w.n;
       const uint32_t par = in ? a.kv.par[row].x : 0u;
       if (item > 0 && !wait_warp(&sc.k_empty, (item - 1) & 1)) { ok = false; break; }
+      if (item >= 2 && !wait_warp(&sc.item_done[item & 1], ((item >> 1) - 1) & 1)) { ok = false; break; }
       const uint32_t zk = (uint32_t)(int)par_zero(par) * 0x10001u + Ints<T>::bias;
       uint8_t* kd = smem + L::off_k + tid * 128;
 #pragma unroll 2

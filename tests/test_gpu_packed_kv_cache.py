@@ -703,6 +703,26 @@ def test_collected_weight_without_kept_scores(L):
         check(L, cache, _q(1, 16, 1, 64, torch.bfloat16, 1), **kw)
 
 
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("dtype,D", [(torch.float16, 64), (torch.bfloat16, 128)])
+def test_collected_weight_of_one_or_two_row_tiles(L, dtype, D, form):
+    """Chunks of one, two and three tiles of 128 rows side by side, more tiles
+    of tokens than SMs: a row tile's sums may run ahead of the other's."""
+    B, H, G, S, T = 6, 4, 4, 70, 3000
+    n = (20, 40, 5, 64, 70, 1)
+    cache = L.PackedKVCache(1, T)
+    cache.append(0, *_kv(B, H, T, D, dtype, 1), counts=_ints(T, 2500, 2999, 130, 1700, 2000))
+    q = _q(B, H * G, S, D, dtype, 2)
+    kw = dict(_form(form, B, H * G), counts=_ints(*n))
+    check(L, cache, q, **kw)
+    mass = []
+    for _ in range(4):
+        cache.attention_mass(0).zero_()
+        cache.attend(0, q, accumulate=True, **kw)
+        mass.append(cache.attention_mass(0).clone())
+    assert all(torch.equal(m, mass[0]) for m in mass)
+
+
 def test_whole_heads_and_cut_ones(L):
     """Lengths around those where a block takes a whole head, and scales of either sign."""
     for T in (480, 511, 512, 513, 600, 1100):
