@@ -480,6 +480,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
               for (int k = 0; k < 16; ++k) z[k] = __float_as_uint(__uint_as_float(z[k]) * alpha);
               tmem_st16(O + d, z);
             }
+            tmem_wait_st();  // the step's second half may raise it again
           }
         };
         if (plain) {
@@ -566,6 +567,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
               raise(m);
               if (c) {  // the first half's P' is there already
                 const __half2 alpha = __float2half2_rn(ex2(before - R));
+                tmem_wait_st();  // of P' itself
                 tmem_ld16(S, p);
                 tmem_wait_ld16(p);
 #pragma unroll

@@ -422,6 +422,37 @@ def test_scales_of_every_size_in_chunks(L):
         check(L, cache, q, softcap=5.0, window=300)
 
 
+@pytest.mark.parametrize("dtype,D", [(torch.float16, 128), (torch.bfloat16, 64)])
+def test_scores_that_rise_along_the_tokens(L, dtype, D):
+    """Each 32 tokens beat those before by more than a reference has room
+    for, so that both halves of every step raise it."""
+    T, S = 400, 70
+    k, v = (x.clone() for x in _kv(2, 2, T, D, dtype, 1))
+    up = (torch.arange(T, device="cuda") // 32).double() / 4
+    k = (torch.randn(D, generator=_gen(3), device="cuda") * up[:, None]).to(dtype).expand(2, 2, T, D)
+    cache = L.PackedKVCache(1, T)
+    cache.append(0, k, v, counts=_ints(T, 333))
+    q = _q(2, 8, S, D, dtype, 4)
+    for scale in (1.0, -1.0, 4.0):
+        for kw in ({}, {"causal": True}, {"causal": True, "window": 150}, {"softcap": 300.0}):
+            check(L, cache, q, scale=scale, **kw)
+    slopes = torch.linspace(0.3, 2.0, 8, device="cuda")
+    check(L, cache, q, causal=True, slopes=slopes, scale=0.1)
+    cache.evict(0, 200)
+    check(L, cache, q, causal=True, scale=1.0)
+    # the weight of the halves of one step: 32 tokens at 0, 32 a factor 2^9 .. 2^14 above, and so on
+    v = torch.ones(1, 1, T, D, device="cuda").to(dtype)
+    v[..., 1::2] *= ((torch.arange(T, device="cuda") // 32) % 2)[:, None].to(dtype)
+    k = torch.zeros(1, 1, T, D, device="cuda", dtype=dtype)
+    k[..., 0] = (torch.arange(T, device="cuda") // 32).to(dtype)
+    q = torch.zeros(1, 2, S, D, device="cuda", dtype=dtype)
+    q[..., 0] = torch.linspace(6.5, 9.5, 2 * S, device="cuda").view(1, 2, S).to(dtype)
+    cache = L.PackedKVCache(1, T)
+    cache.append(0, k, v)
+    for kw in ({}, {"causal": True}, {"softcap": 300.0}):  # the cap has every tile go the masked way
+        check(L, cache, q, scale=1.0, **kw)
+
+
 def test_windows_and_prefixes_of_any_size(L):
     cache = L.PackedKVCache(1, 300)
     cache.append(0, *_kv(2, 2, 300, 64, torch.bfloat16, 8), counts=_ints(300, 77))
