@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(32 * kWarps, NQ == 1 && !QLO ? 4 : NQ == 1 ? 2
   int u1 = min(s.count, u0 + (x1 - x0));
   auto token = [&](int u) { return GEN ? (u < s.pre ? u : u + s.gap) * kUnit : u * kUnit; };
   auto ask = [&](int u) {  // every lane has read what the stage held
-    if (u < u1) {
+    if (u < u1 && fill >= 0) {
       if (lane == 0) {
         Stage<D>& st = sh.ring[warp][fill % kStages];
         uint64_t* bar = &sh.full[warp][fill % kStages];
@@ -379,13 +379,15 @@ __global__ void __launch_bounds__(32 * kWarps, NQ == 1 && !QLO ? 4 : NQ == 1 ? 2
 #pragma unroll
         for (int i = 0; i < 4; ++i) O[nq][e][i] = 0.0f;
     }
-    for (; u < u1; u += kWarps) {
+    for (; u < u1 && fill >= 0; u += kWarps) {
       const int t0 = token(u);
       const Stage<D>& st = sh.ring[warp][take % kStages];
       if (!mbar_wait_warp(&sh.full[warp][take % kStages], (take / kStages) & 1)) {
-        // the copy never came (2 s): give up, so that the host learns of it
+        // The copy never came (2 s): give up, so that the host learns of it.  Nothing
+        // more is asked for (fill < 0), and the block does not end with copies on their way.
         if (lane == 0) a.kv.sync[3] = LQ_ETIMEOUT;
-        take = fill;
+        for (; take < fill; ++take) mbar_wait_warp(&sh.full[warp][take % kStages], (take / kStages) & 1);
+        fill = -1;
         break;
       }
       ++take;

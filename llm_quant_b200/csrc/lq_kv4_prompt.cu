@@ -1190,6 +1190,7 @@ __global__ void __launch_bounds__(kWeighThreads, 1) kv4_weigh_kernel(const Attn 
       ++item;
     }
     if (!ok) *fail = 1;
+    staged<0>();  // nothing on its way when the block ends, after a failed wait too
   } else {
     constexpr uint32_t idesc = make_idesc(Ints<T>::fmt, kTile);
     const uint32_t base = __reduce_max_sync(0xffffffffu, smem_u32(smem)), tm = __reduce_max_sync(0xffffffffu, tmem);

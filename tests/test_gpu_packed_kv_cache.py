@@ -825,6 +825,21 @@ def test_agrees_with_the_byte_cache(L):
 
 # ---- refusals ------------------------------------------------------------------------------------------------------------
 
+def test_check_reports_a_wait_that_ran_out(L):
+    """The status word as a kernel would leave it, set from the host."""
+    from llm_quant_b200 import _C
+    cache = L.PackedKVCache(1, 32)
+    cache.append(0, *_kv(2, 2, 20, 64, torch.float16, 0))
+    cache.check(0)
+    cache._layers[0].state[-1] = _C.ETIMEOUT
+    for _ in range(2):  # stays until the cache is emptied
+        with pytest.raises(_C.LQError, match="ran out") as e:
+            cache.check(0)
+        assert e.value.status == _C.ETIMEOUT
+    cache.reset()
+    cache.check(0)
+
+
 def test_refusals_on_the_device(L):
     cache = L.PackedKVCache(1, 32)
     k, v = _kv(2, 2, 20, 64, torch.float16, 0)
