@@ -24,8 +24,10 @@ Lengths live on the device and nothing here reads them back, so every method
 can be captured into a CUDA graph and replayed: a replayed ``append`` goes on
 where the last one stopped.  The host keeps an upper bound of them
 (``seq_len``), which sizes what ``get``, ``positions`` and ``attention_mass``
-return; once an ``append`` or ``evict`` was captured, and until ``reset``, it is
-the capacity.
+return.  Once an ``append``, ``evict`` or ``reset`` was captured it is the
+capacity for good, across ``reset`` too, since the host does not see replays;
+an ``append`` that does not fit then no longer raises, its tokens are dropped
+and counted (``dropped``).
 
 One cache is used by one stream at a time (``attend`` without ``accumulate``
 and ``get`` may overlap each other), as any tensor that is changed in place.
@@ -59,16 +61,18 @@ class _LayerStore:
         self.mass = new(0.0, B, H, cap, dtype=torch.float32)
         self.state = new(0, 2 * B + 4)
         self.bound = 0        # no sequence holds more tokens, as far as the host knows
-        self.captured = False  # an append was captured: replays are not seen by the host
+        self.captured = False  # a change of the lengths was captured: its replays are not seen by the host
+        self.emptied = False   # captured, and nothing but replays since the last reset
         self.c = _C.KV4Cache(self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.params.data_ptr(),
                              self.positions.data_ptr(), self.mass.data_ptr(), self.state.data_ptr(),
                              B, H, cap, D)
         self.ref = ctypes.byref(self.c)
         self.forms: dict = {}  # attend's arguments as the entry point takes them
 
-    def clear(self) -> None:
-        self.bound = 0
-        self.captured = False
+    def clear(self, capturing: bool, room: int) -> None:
+        self.captured |= capturing
+        self.bound = room if self.captured else 0
+        self.emptied = self.captured and not capturing
 
 
 def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
@@ -165,6 +169,7 @@ class PackedKVCache(nn.Module):
         self._call(st, "lq_kv4_append", k.data_ptr(), v.data_ptr(), _C.TORCH_TO_LQ[k.dtype], S, ks[0], ks[1], ks[2],
                    vs[0], vs[1], vs[2], c)
         st.bound = self.max_seq_len if st.captured else min(st.bound + S, self.max_seq_len)
+        st.emptied = False
 
     def update(self, layer_idx: int, key: torch.Tensor, value: torch.Tensor,
                counts: Optional[torch.Tensor] = None,
@@ -326,13 +331,18 @@ class PackedKVCache(nn.Module):
         return st.mass.narrow(2, 0, st.bound)
 
     def reset(self, layer_idx: Optional[int] = None) -> None:
-        """Clear one layer, or all; the buffers stay."""
+        """Clear one layer, or all; the buffers stay, and so do captured graphs."""
         for st in self._layers if layer_idx is None else [self._layers[layer_idx]]:
             if st is not None:
-                st.clear()
+                st.clear(torch.cuda.is_current_stream_capturing(), self.max_seq_len)
                 self._call(st, "lq_kv4_reset")
 
     @property
     def seq_len(self) -> int:
-        """Tokens cached in layer 0: the most that any sequence may hold."""
-        return 0 if not self.num_layers or self._layers[0] is None else self._layers[0].bound
+        """Tokens cached in layer 0: the most that any sequence may hold.  Only
+        where a graph was captured and nothing but replays may have come since
+        a ``reset`` does this wait for the device, to tell empty from not."""
+        st = self._layers[0] if self.num_layers else None
+        if st is None or st.emptied and not torch.cuda.is_current_stream_capturing() and not st.state[:st.B].any():
+            return 0
+        return st.bound

@@ -703,6 +703,56 @@ def test_replayed_evictions_start_with_little(L):
     del graph
 
 
+def test_replays_after_a_reset(L):
+    """A decode step captured once; each request resets, appends its prompt and replays."""
+    B, H, D, room, keep = 2, 2, 64, 160, 40
+    cache = L.PackedKVCache(1, room)
+    k, v = (x.clone() for x in _kv(B, H, 1, D, torch.float16, 0))
+    q = _q(B, 4, 1, D, torch.float16, 1)
+    cache.append(0, k, v)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.append(0, k, v)
+        cache.attend(0, q, causal=True, accumulate=True)
+    for request in range(2):
+        cache.reset()
+        assert cache.seq_len == 0
+        graph.replay()  # the host sees nothing of it
+        assert cache.seq_len == room and cache.lengths(0).tolist() == [1, 1]
+        cache.reset()
+        twin = L.PackedKVCache(1, room)
+        prompt, counts = _kv(B, H, 30, D, torch.float16, 10 + request), _ints(30, 17)
+        for c in (cache, twin):
+            c.append(0, *prompt, counts=counts)
+        for step in range(25):
+            new = _kv(B, H, 1, D, torch.float16, 100 * request + step)
+            k.copy_(new[0]), v.copy_(new[1])
+            graph.replay()
+            twin.append(0, *new)
+            twin.attend(0, q, causal=True, accumulate=True)
+        n = 55
+        assert cache.lengths(0).tolist() == twin.lengths(0).tolist() == [n, n - 13]
+        assert cache.seq_len == room
+        for a, b in zip(cache.get(0), twin.get(0)):
+            assert torch.equal(a[:, :, :n], b) and not a[:, :, n:].any()
+        assert torch.equal(cache.positions(0)[:, :, :n], twin.positions(0))
+        cache.attention_mass(0).mul_(0.5)  # reaches every token
+        assert (cache.attention_mass(0)[:, :, :n] > 0).sum().item() == 2 * (2 * n - 13)
+        check_evict(cache, keep, recent=4)
+        assert cache.lengths(0).tolist() == [keep, keep]
+        cache.append(0, *prompt, counts=counts)
+        check(L, cache, q, causal=True)
+    # a captured reset is the replay's
+    again = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(again):
+        cache.reset()
+    assert cache.seq_len == room and cache.lengths(0).tolist() != [0, 0]
+    assert cache.get(0)[0].any()
+    again.replay()
+    assert cache.lengths(0).tolist() == [0, 0] and not cache.get(0)[0].any()
+    del graph, again
+
+
 def test_replayed_attention_outgrows_its_capture(L):
     """Captured with few tokens, replayed with many: grids are made for few."""
     for S, dtype in ((1, torch.bfloat16), (30, torch.bfloat16), (30, torch.float32)):
