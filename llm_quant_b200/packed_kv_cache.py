@@ -21,7 +21,8 @@ the input's dtype (the reference rounds each operation to it, which turns an
 all-zero fp16 token into NaN), and the scale is kept in bf16.
 
 Lengths live on the device and nothing here reads them back, so every method
-can be captured into a CUDA graph and replayed: a replayed ``append`` goes on
+(but a layer's first ``append``, which makes its buffers, and ``check``) can be
+captured into a CUDA graph and replayed: a replayed ``append`` goes on
 where the last one stopped.  The host keeps an upper bound of them
 (``seq_len``), which sizes what ``get``, ``positions`` and ``attention_mass``
 return.  Once an ``append``, ``evict`` or ``reset`` was captured it is the
@@ -89,7 +90,8 @@ class PackedKVCache(nn.Module):
 
     ``max_seq_len`` tokens of room for each sequence are allocated per layer
     at its first chunk, whose shape [B, H, S, D] and device the cache keeps
-    (head dim 64 or 128; float32, float16 or bfloat16 chunks)."""
+    (head dim 64 or 128; float32, float16 or bfloat16 chunks).  That one cannot
+    be captured into a graph; it may be empty (S = 0)."""
 
     def __init__(self, num_layers: int, max_seq_len: int):
         super().__init__()
@@ -150,6 +152,10 @@ class PackedKVCache(nn.Module):
                 raise ValueError(f"PackedKVCache.append: {S} tokens do not fit into {self.max_seq_len}")
             if B * H > 65535:
                 raise ValueError("PackedKVCache: more than 65535 (sequence, head) pairs")
+            if torch.cuda.is_current_stream_capturing():
+                # a captured allocation would be filled, and so the cache emptied, by every replay
+                raise RuntimeError("PackedKVCache.append: a layer's first chunk (it may be empty, S = 0) must come "
+                                   "before the capture")
             st = _LayerStore(B, H, (self.max_seq_len + 31) // 32 * 32, D, key.device)
             self._layers[layer_idx] = st
         elif (B, H, D) != (st.B, st.H, st.D) or key.device != st.device:

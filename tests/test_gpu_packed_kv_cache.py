@@ -753,6 +753,27 @@ def test_replays_after_a_reset(L):
     del graph, again
 
 
+def test_first_chunk_is_not_captured(L):
+    """Its buffers would be made, and emptied, by every replay."""
+    cache = L.PackedKVCache(2, 64)
+    k, v = _kv(1, 1, 3, 64, torch.float16, 0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        k2 = k + 0
+        for n in (3, 0):
+            with pytest.raises(RuntimeError, match="capture"):
+                cache.append(0, k[:, :, :n], v[:, :, :n])
+    assert cache.get(0) is None
+    cache.append(0, k[:, :, :0], v[:, :, :0])  # makes room, as the message says
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.append(0, k, v)
+    for n in (3, 6):
+        graph.replay()
+        assert cache.lengths(0).tolist() == [n]
+    del graph, k2
+
+
 def test_replayed_attention_outgrows_its_capture(L):
     """Captured with few tokens, replayed with many: grids are made for few."""
     for S, dtype in ((1, torch.bfloat16), (30, torch.bfloat16), (30, torch.float32)):
