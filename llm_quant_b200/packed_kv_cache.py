@@ -70,9 +70,9 @@ class _LayerStore:
         self.ref = ctypes.byref(self.c)
         self.forms: dict = {}  # attend's arguments as the entry point takes them
 
-    def clear(self, capturing: bool, room: int) -> None:
+    def clear(self, capturing: bool) -> None:
         self.captured |= capturing
-        self.bound = room if self.captured else 0
+        self.bound = self.cap if self.captured else 0
         self.emptied = self.captured and not capturing
 
 
@@ -88,7 +88,8 @@ def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
 class PackedKVCache(nn.Module):
     """KV cache in 4 bits for inference (see the module's documentation).
 
-    ``max_seq_len`` tokens of room for each sequence are allocated per layer
+    ``max_seq_len`` tokens of room for each sequence, rounded up to a multiple
+    of 32 (the capacity, which replayed graphs may fill), are allocated per layer
     at its first chunk, whose shape [B, H, S, D] and device the cache keeps
     (head dim 64 or 128; float32, float16 or bfloat16 chunks).  That one cannot
     be captured into a graph; it may be empty (S = 0)."""
@@ -132,8 +133,9 @@ class PackedKVCache(nn.Module):
         """Quantize and store new K, V [B, H, S, D] behind what each sequence
         holds.  ``counts`` (int32 [B], on the device) says how many of the S
         tokens each sequence has, the rest being padding; default all.  Raises
-        ValueError when S tokens might not fit; what a replayed graph appends
-        past the room is dropped and counted (``dropped``)."""
+        ValueError when S tokens might not fit into max_seq_len; what a replayed
+        graph, or any call after a capture, appends past the capacity is dropped
+        and counted (``dropped``)."""
         _C.require_cuda(key, value, what="PackedKVCache.append")
         _C.require_float(key, "PackedKVCache.append")
         if key.ndim != 4 or key.shape != value.shape:
@@ -165,16 +167,17 @@ class PackedKVCache(nn.Module):
         if S == 0:
             return
         capturing = torch.cuda.is_current_stream_capturing()
-        if capturing:
-            st.captured = True
-        elif not st.captured and st.bound + S > self.max_seq_len:
+        if S > st.cap:
+            raise ValueError(f"PackedKVCache.append: {S} tokens do not fit into {st.cap}")
+        if not (capturing or st.captured) and st.bound + S > self.max_seq_len:
             raise ValueError(f"PackedKVCache.append: {S} more tokens than {st.bound} of {self.max_seq_len} "
                              "do not fit (evict, or reset)")
         k, v = _rows(key, "append"), _rows(value, "append")
         ks, vs = k.stride(), v.stride()
         self._call(st, "lq_kv4_append", k.data_ptr(), v.data_ptr(), _C.TORCH_TO_LQ[k.dtype], S, ks[0], ks[1], ks[2],
                    vs[0], vs[1], vs[2], c)
-        st.bound = self.max_seq_len if st.captured else min(st.bound + S, self.max_seq_len)
+        st.captured |= capturing
+        st.bound = st.cap if st.captured else st.bound + S
         st.emptied = False
 
     def update(self, layer_idx: int, key: torch.Tensor, value: torch.Tensor,
@@ -299,7 +302,7 @@ class PackedKVCache(nn.Module):
         self._call(st, "lq_kv4_evict", keep, recent, sinks, ws.data_ptr(), nbytes)
         if capturing:
             st.captured = True
-            st.bound = self.max_seq_len
+            st.bound = st.cap
         elif not st.captured:
             st.bound = min(st.bound, keep)
 
@@ -310,7 +313,8 @@ class PackedKVCache(nn.Module):
         return st.state[:st.B]
 
     def dropped(self, layer_idx: int) -> torch.Tensor:
-        """Tokens that replayed appends found no room for: int32 scalar on the device (the cache's own)."""
+        """Tokens that appends found no room for, replayed ones and those after
+        a capture: int32 scalar on the device (the cache's own)."""
         st = self._layer(layer_idx, "dropped")
         return st.state[2 * st.B + 1]
 
@@ -340,7 +344,7 @@ class PackedKVCache(nn.Module):
         """Clear one layer, or all; the buffers stay, and so do captured graphs."""
         for st in self._layers if layer_idx is None else [self._layers[layer_idx]]:
             if st is not None:
-                st.clear(torch.cuda.is_current_stream_capturing(), self.max_seq_len)
+                st.clear(torch.cuda.is_current_stream_capturing())
                 self._call(st, "lq_kv4_reset")
 
     @property

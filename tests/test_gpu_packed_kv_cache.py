@@ -774,6 +774,30 @@ def test_first_chunk_is_not_captured(L):
     del graph, k2
 
 
+def test_replayed_tokens_past_max_seq_len_can_be_read(L):
+    """The room is max_seq_len rounded up to 32; replays may fill all of it."""
+    cache, twin = L.PackedKVCache(1, 40), L.PackedKVCache(1, 70)
+    k, v = _kv(2, 1, 7, 64, torch.float16, 0)
+    cnt = _ints(7, 3)
+    for c in (cache, twin):
+        c.append(0, k, v, counts=cnt)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.append(0, k, v, counts=cnt)
+    for _ in range(8):
+        graph.replay()
+        twin.append(0, k, v, counts=cnt)
+    n = cache.lengths(0)
+    assert n.tolist() == [63, 27] and cache.seq_len >= 63
+    for a, b in zip((*cache.get(0), cache.positions(0)), (*twin.get(0), twin.positions(0))):
+        assert torch.equal(a[:, :, :63], b[:, :, :63])
+    cache.attend(0, _q(2, 2, 1, 64, torch.float16, 1), accumulate=True)
+    assert (cache.attention_mass(0) > 0).sum((1, 2)).tolist() == n.tolist()
+    with pytest.raises(ValueError, match="fit"):
+        cache.append(0, *_kv(2, 1, 65, 64, torch.float16, 0))
+    del graph
+
+
 def test_replayed_attention_outgrows_its_capture(L):
     """Captured with few tokens, replayed with many: grids are made for few."""
     for S, dtype in ((1, torch.bfloat16), (30, torch.bfloat16), (30, torch.float32)):
