@@ -235,16 +235,16 @@ class PackedKVCache(nn.Module):
         Inference only: no gradient is computed."""
         st = self._layer(layer_idx, "attend")
         q = query if query.__class__ is torch.Tensor and query.ndim == 4 else self._query(st, query)
-        # 1/8 of an octave: the work is split by it, nothing else
+        # rounded up by 1/8 of an octave at most: the work is split by it, nothing else
         bound = st.cap if st.captured else st.bound
         step = 1 << max(5, bound.bit_length() - 4)
+        bound = min((bound + step - 1) // step * step, st.cap)
         softcap = float(softcap)
-        key = (q.dtype, q.shape, q.stride(), q.device, scale, causal, softcap, window, accumulate,
-               (bound + step - 1) // step)
+        key = (q.dtype, q.shape, q.stride(), q.device, scale, causal, softcap, window, accumulate, bound)
         form = st.forms.get(key)
         if form is None or q.data_ptr() & 15:
             q = _rows(self._query(st, query), "attend")
-            form = self._form(st, q, scale, causal, softcap, window, accumulate, min(bound + step, st.cap))
+            form = self._form(st, q, scale, causal, softcap, window, accumulate, bound)
             if q.data_ptr() == query.data_ptr():
                 if len(st.forms) >= 256:
                     st.forms.clear()

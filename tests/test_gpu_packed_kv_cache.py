@@ -859,6 +859,23 @@ def test_whole_heads_and_cut_ones(L):
             check(L, cache, _q(2, 6, 40, 128, torch.float16, 1), scale=scale, causal=True)
 
 
+@pytest.mark.parametrize("dtype,S", [(torch.bfloat16, 1), (torch.float32, 5)])
+def test_split_follows_the_length(L, dtype, S):
+    """The work of a cache that grew is split as that of one that began as long."""
+    q = _q(1, 8, S, 64, dtype, 1)
+    grown = L.PackedKVCache(1, 9000)
+    for n, total in ((300, 300), (300, 600), (4200, 4800), (4000, 8800)):
+        grown.append(0, *_kv(1, 8, n, 64, dtype, total))
+        out = grown.attend(0, q, accumulate=True)
+        fresh = L.PackedKVCache(1, 9000)
+        fresh.append(0, *_kv(1, 8, total, 64, dtype, 0))
+        fresh.attend(0, q, accumulate=True)
+        (_, need, form), = fresh._layers[0].forms.values()
+        used = list(grown._layers[0].forms.values())[-1]
+        assert used[1] == need and used[2].bound == form.bound
+        assert torch.isfinite(out).all()
+
+
 def test_two_calls_at_once_and_other_streams(L):
     cache = L.PackedKVCache(1, 3000)
     cache.append(0, *_kv(4, 4, 3000, 128, torch.bfloat16, 0))
