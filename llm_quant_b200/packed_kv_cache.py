@@ -37,6 +37,7 @@ and ``get`` may overlap each other), as any tensor that is changed in place.
 from __future__ import annotations
 
 import ctypes
+import operator
 from typing import Optional, Tuple
 
 import torch
@@ -239,7 +240,9 @@ class PackedKVCache(nn.Module):
         bound = st.cap if st.captured else st.bound
         step = 1 << max(5, bound.bit_length() - 4)
         bound = min((bound + step - 1) // step * step, st.cap)
-        softcap = float(softcap)
+        # numbers, whatever holds them: a tensor may hold another one at the next call
+        softcap, window, causal, accumulate = float(softcap), operator.index(window), bool(causal), bool(accumulate)
+        scale = st.D ** -0.5 if scale is None else float(scale)
         key = (q.dtype, q.shape, q.stride(), q.device, scale, causal, softcap, window, accumulate, bound)
         form = st.forms.get(key)
         if form is None or q.data_ptr() & 15:
@@ -271,16 +274,16 @@ class PackedKVCache(nn.Module):
         return query
 
     @staticmethod
-    def _form(st: _LayerStore, q: torch.Tensor, scale, causal, softcap, window, accumulate, bound):
+    def _form(st: _LayerStore, q: torch.Tensor, scale: float, causal: bool, softcap: float, window: int,
+              accumulate: bool, bound: int):
         """The call's arguments but for the tensors: checked once for each form."""
         if not (softcap == 0.0 or 1e-20 <= softcap < float("inf")):
             raise ValueError(f"PackedKVCache.attend: softcap {softcap} must be finite and not negative (0: none)")
         if not 0 <= window <= 2 ** 30:
             raise ValueError(f"PackedKVCache.attend: window {window} must be 0 (none) to 2^30")
         sb, sh, ss, _ = q.stride()
-        c = _C.KV4Attn(q.shape[1], q.shape[2], sb, sh, ss, bound, window,
-                       q.shape[3] ** -0.5 if scale is None else scale, softcap, _C.TORCH_TO_LQ[q.dtype], bool(causal),
-                       bool(accumulate))
+        c = _C.KV4Attn(q.shape[1], q.shape[2], sb, sh, ss, bound, window, scale, softcap, _C.TORCH_TO_LQ[q.dtype],
+                       causal, accumulate)
         return ctypes.byref(c), _C.lib().lq_kv4_attention_workspace_bytes(st.ref, ctypes.byref(c)), c
 
     # -- eviction ------------------------------------------------------------------

@@ -876,6 +876,18 @@ def test_split_follows_the_length(L, dtype, S):
         assert torch.isfinite(out).all()
 
 
+def test_scale_as_a_tensor_is_read_at_each_call(L):
+    cache = L.PackedKVCache(1, 100)
+    cache.append(0, *_kv(1, 2, 100, 64, torch.float16, 0))
+    q = _q(1, 4, 1, 64, torch.float16, 1)
+    scale = torch.tensor(0.1)
+    a = cache.attend(0, q, scale=scale)
+    assert torch.equal(a, cache.attend(0, q, scale=scale.item()))
+    scale.fill_(0.3)
+    assert torch.equal(cache.attend(0, q, scale=scale), cache.attend(0, q, scale=scale.item()))
+    assert torch.equal(cache.attend(0, q, window=torch.tensor(7)), cache.attend(0, q, window=7))
+
+
 def test_two_calls_at_once_and_other_streams(L):
     cache = L.PackedKVCache(1, 3000)
     cache.append(0, *_kv(4, 4, 3000, 128, torch.bfloat16, 0))
