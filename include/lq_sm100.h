@@ -451,7 +451,8 @@ int lq_kv4_evict(const lq_kv4_cache* host_cache, int64_t keep, int64_t recent, i
  * bound: tokens that the longest sequence is thought to hold (only the split
  * of the work goes by it).  The workspace, of lq_kv4_attention_workspace_bytes for
  * the same form, is for this call alone. */
-/* window <= 2^30, Hq / H <= 4096; q and the strides as for lq_kv4_append's k. */
+/* window <= 2^30, Hq / H <= 4096, softcap 0 or 1e-20 to 1e30; q and the strides as
+ * for lq_kv4_append's k. */
 typedef struct {
   int64_t Hq, Sq, q_sb, q_sh, q_ss, bound, window;
   float sm_scale, softcap;

@@ -253,12 +253,11 @@ __device__ __forceinline__ void products(const Rows<D, NQ, QLO>& q, const uint32
   }
 }
 
-// Score (log2 units) from a product, with cap, bias and masks: -inf where the
-// query does not see the token.
+// Score (log2 units) from a scaled and capped product, with bias and masks: -inf
+// where the query does not see the token.
 template <int D, int NQ, bool QLO>
 __device__ __forceinline__ float full_score(const Attn& a, const Rows<D, NQ, QLO>& q, int nq, int e, float v, bool in,
                                             int pos, int pre) {
-  if (a.cap > 0.0f) v = tanh_exp(v) * (a.cap * kLog2e);
   const int back = q.at[nq][e] - pos;
   if (a.slopes) v = fmaf(-q.slope[nq][e], fabsf((float)back), v);
   bool near = true;
@@ -427,9 +426,20 @@ __global__ void __launch_bounds__(32 * kWarps, NQ == 1 && !QLO ? 4 : NQ == 1 ? 2
           for (int e = 0; e < 2; ++e) {
             float& v = x[j >> 1][nq][2 * (j & 1) + e];
             v *= sk * q.fac[nq][e];
-            if constexpr (GEN) v = full_score<D, NQ, QLO>(a, q, nq, e, v, tok[j] < s.n, pos[j], pre);
-            else if (tail && tok[j] >= s.n) v = -INFINITY;
+            if (!GEN && tail && tok[j] >= s.n) v = -INFINITY;
           }
+      }
+      if constexpr (GEN) {
+        if (a.cap > 0.0f) capped<8 * NQ>(&x[0][0][0], a.cap * kLog2e);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float& v = x[j >> 1][nq][2 * (j & 1) + e];
+              v = full_score<D, NQ, QLO>(a, q, nq, e, v, tok[j] < s.n, pos[j], pre);
+            }
       }
       if (a.scores) {
 #pragma unroll
@@ -760,13 +770,16 @@ __global__ void __launch_bounds__(128) kv4_mass_kernel(const Attn a) {
       float x[1][1][4];
       products<1, D, 1, QLO>(q, kw, kp, x);
 #pragma unroll
+      for (int i = 0; i < 4; ++i) x[0][0][i] *= par_scale(kp[i >> 1]) * q.fac[0][i & 1];
+      if (GEN && a.cap > 0.0f) capped<4>(&x[0][0][0], a.cap * kLog2e);
+#pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int qr = zb * 8 + 2 * c + e;
         if (qr >= a.rows) continue;
         const float lse = a.lse[(int64_t)bh * a.rows_pad + qr];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          float v = x[0][0][2 * j + e] * (par_scale(kp[j]) * q.fac[0][e]);
+          float v = x[0][0][2 * j + e];
           if constexpr (GEN) v = full_score<D, 1, QLO>(a, q, 0, e, v, tok[j] < s.n, pos[j], pre);
           sum[j] += ex2(v - lse);
         }
@@ -892,7 +905,8 @@ extern "C" int lq_kv4_attention(const lq_kv4_cache* cache, const lq_kv4_attn* f,
   LQ_REQUIRE(f->Hq > 0 && f->Hq % cache->H == 0, LQ_EINVAL, "query heads %lld not a multiple of kv heads %lld",
              (long long)f->Hq, (long long)cache->H);
   LQ_REQUIRE(f->Sq >= 0 && f->bound >= 0, LQ_EINVAL, "bad shape");
-  LQ_REQUIRE(f->softcap >= 0.0f, LQ_EINVAL, "softcap must not be negative");
+  LQ_REQUIRE(f->softcap == 0.0f || (f->softcap >= 1e-20f && f->softcap <= 1e30f), LQ_EINVAL,
+             "softcap %g: 0 (none) or 1e-20 to 1e30", (double)f->softcap);
   LQ_REQUIRE(f->window >= 0 && f->window <= (1 << 30), LQ_EINVAL, "window %lld: 0 (none) to 2^30", (long long)f->window);
   const int64_t rows = f->Hq / cache->H * f->Sq;
   if (rows == 0) return LQ_OK;

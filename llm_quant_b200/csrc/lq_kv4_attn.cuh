@@ -58,10 +58,35 @@ __device__ __forceinline__ float rcp(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// tanh from the exponential: the error is about 2^-23 absolute, which is what a
-// capped score needs (tanh.approx is only good to 2^-11)
-__device__ __forceinline__ float tanh_exp(float x) {
-  return 1.0f - __fdividef(2.0f, 1.0f + ex2(2.0f * kLog2e * x));
+// y = cap * tanh(x) of N scores of a thread (cap in log2 units); all lanes of a warp.
+// |x| <= 3/4: x + x u P(u), u = x^2, P of degree 4 with the least greatest relative
+// error of tanh (2^-24.9; fitted by Remez exchange, 2^-23.6 in fp32), so that a
+// score keeps its bits however large the cap.  Above: 1 - 2 / (1 + exp 2x), off by
+// 2^-22 of the cap or less, 2^-21 of the score (near 0 it would be 2^-22 of the cap
+// still, and a score nothing beside it).  The second form takes two of the
+// special-function unit's operations and is left out where the warp has no such score.
+__device__ __forceinline__ float f32_of(float x) { return x; }
+__device__ __forceinline__ float f32_of(uint32_t x) { return __uint_as_float(x); }
+__device__ __forceinline__ void put_f32(float& d, float x) { d = x; }
+__device__ __forceinline__ void put_f32(uint32_t& d, float x) { d = __float_as_uint(x); }
+template <int N, typename T>  // T: float, or its bits
+__device__ __forceinline__ void capped(T* v, float cap) {
+  constexpr float kSmall = 0.75f;
+  float top = 0.0f;
+#pragma unroll
+  for (int k = 0; k < N; ++k) top = fmaxf(top, fabsf(f32_of(v[k])));
+  const bool large = __any_sync(0xffffffffu, top > kSmall);
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const float x = f32_of(v[k]), u = x * x;
+    float p = fmaf(-0.0047694904f, u, 0.019664914f);
+    p = fmaf(p, u, -0.053390259f);
+    p = fmaf(p, u, 0.13326521f);
+    p = fmaf(p, u, -0.33333068f);
+    float y = cap * fmaf(x * u, p, x);
+    if (large && fabsf(x) > kSmall) y = fmaf(-2.0f * cap, rcp(1.0f + ex2(2.0f * kLog2e * x)), cap);
+    put_f32(v[k], y);
+  }
 }
 __device__ __forceinline__ uint32_t h2(float lo, float hi) {
   __half2 h = __floats2half2_rn(lo, hi);

@@ -283,12 +283,6 @@ __device__ __forceinline__ void scaled(uint32_t* y, const float* sk) {
     y[k + 2] = __float_as_uint(__uint_as_float(y[k + 2]) * f.z), y[k + 3] = __float_as_uint(__uint_as_float(y[k + 3]) * f.w);
   }
 }
-template <int N>  // cap tanh(x) = cap - 2 cap / (1 + exp 2x): good to 2^-23 of the cap
-__device__ __forceinline__ void capped(uint32_t* y, float cap) {
-#pragma unroll
-  for (int k = 0; k < N; ++k)
-    y[k] = __float_as_uint(fmaf(-2.0f * cap, rcp(1.0f + ex2(2.0f * kLog2e * __uint_as_float(y[k]))), cap));
-}
 
 // Integers of 4 bits as operands: bias + code is exact in the type, and so is
 // its difference from bias + zero point.

@@ -231,7 +231,7 @@ class PackedKVCache(nn.Module):
         before it meets the values.  More than 16 such queries to a kv head also
         round it to 2^-24 of 2^8 and the greatest V scale among 128 slots: tokens
         with a scale below 2^-20 of that lose bits.  Positions are int32, ``window`` is at most
-        2^30, a group has at most 4096 query heads.
+        2^30, a group has at most 4096 query heads, ``softcap`` is 0 or 1e-20 to 1e30.
 
         Inference only: no gradient is computed."""
         st = self._layer(layer_idx, "attend")
@@ -277,8 +277,8 @@ class PackedKVCache(nn.Module):
     def _form(st: _LayerStore, q: torch.Tensor, scale: float, causal: bool, softcap: float, window: int,
               accumulate: bool, bound: int):
         """The call's arguments but for the tensors: checked once for each form."""
-        if not (softcap == 0.0 or 1e-20 <= softcap < float("inf")):
-            raise ValueError(f"PackedKVCache.attend: softcap {softcap} must be finite and not negative (0: none)")
+        if not (softcap == 0.0 or 1e-20 <= softcap <= 1e30):
+            raise ValueError(f"PackedKVCache.attend: softcap {softcap} must be 0 (none) or 1e-20 to 1e30")
         if not 0 <= window <= 2 ** 30:
             raise ValueError(f"PackedKVCache.attend: window {window} must be 0 (none) to 2^30")
         sb, sh, ss, _ = q.stride()

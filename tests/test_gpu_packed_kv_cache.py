@@ -453,6 +453,30 @@ def test_scores_that_rise_along_the_tokens(L, dtype, D):
         check(L, cache, q, scale=1.0, **kw)
 
 
+@pytest.mark.parametrize("S", [1, 40])
+@pytest.mark.parametrize("dtype", ALL)
+def test_large_caps(L, dtype, S):
+    """A cap far above the scores changes them as its formula says, and loses
+    no bits of them: tanh of a small argument is good to 2^-23 of itself, a score x then to 2^-21 |x|
+    on top of dx = 12 * 2^-22 a, and |x| <= a: dx <= 14 / 12 of what it is
+    without a cap.  A cap of 1000 or more changes scores up to 20 by less than
+    20^3 / (3 * 1000^2) = 0.003, so probabilities in the bound by 0.6 %:
+    1.2 > 14 / 12 * 1.006 covers both."""
+    B, H, G, D, T = 2, 2, 4, 64, 700
+    cache = L.PackedKVCache(1, T)
+    cache.append(0, *_kv(B, H, T, D, dtype, 1), counts=_ints(T, 333))
+    q = _q(B, H * G, S, D, dtype, 2)
+    _, bound, _, mb, _ = reference(cache, 0, q, causal=True)
+    for cap in (1e3, 1e4, 1e5, 1e6, 1e7, 1e9, 1e15, 1e30):
+        ref, _, m, _, _ = reference(cache, 0, q, causal=True, softcap=cap)
+        cache.attention_mass(0).zero_()
+        out = cache.attend(0, q, causal=True, softcap=cap, accumulate=True)
+        err = (out.double() - ref).abs()
+        assert (err <= 1.2 * bound).all(), (cap, float((err / bound).max()))
+        err = (cache.attention_mass(0).double() - m).abs()
+        assert (err <= 1.2 * mb).all(), (cap, float((err / mb).max()))
+
+
 def test_windows_and_prefixes_of_any_size(L):
     cache = L.PackedKVCache(1, 300)
     cache.append(0, *_kv(2, 2, 300, 64, torch.bfloat16, 8), counts=_ints(300, 77))

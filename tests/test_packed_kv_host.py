@@ -81,6 +81,13 @@ def test_bad_arguments(lib):
     assert attend(Sq=0) == 0
 
 
+def test_caps_out_of_range(lib):
+    c = ctypes.byref(_cache())
+    for cap in (-1.0, 1e-21, 1e31, float("inf"), float("nan")):
+        assert lib.lq_kv4_attention(c, _form(softcap=cap), 4096, None, None, None, 4096, 4096, 1 << 40, None) == -1
+        assert b"softcap" in lib.lq_last_error()
+
+
 def test_python_layer_without_a_gpu():
     with pytest.raises(ValueError):
         L.PackedKVCache(1, 0)
