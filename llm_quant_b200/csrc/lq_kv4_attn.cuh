@@ -75,17 +75,23 @@ __device__ __forceinline__ void capped(T* v, float cap) {
   float top = 0.0f;
 #pragma unroll
   for (int k = 0; k < N; ++k) top = fmaxf(top, fabsf(f32_of(v[k])));
-  const bool large = __any_sync(0xffffffffu, top > kSmall);
-#pragma unroll
-  for (int k = 0; k < N; ++k) {
-    const float x = f32_of(v[k]), u = x * x;
+  auto small = [&](float x) {
+    const float u = x * x;
     float p = fmaf(-0.0047694904f, u, 0.019664914f);
     p = fmaf(p, u, -0.053390259f);
     p = fmaf(p, u, 0.13326521f);
     p = fmaf(p, u, -0.33333068f);
-    float y = cap * fmaf(x * u, p, x);
-    if (large && fabsf(x) > kSmall) y = fmaf(-2.0f * cap, rcp(1.0f + ex2(2.0f * kLog2e * x)), cap);
-    put_f32(v[k], y);
+    return cap * fmaf(x * u, p, x);
+  };
+  if (!__any_sync(0xffffffffu, top > kSmall)) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) put_f32(v[k], small(f32_of(v[k])));
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const float x = f32_of(v[k]), y = fmaf(-2.0f * cap, rcp(1.0f + ex2(2.0f * kLog2e * x)), cap);
+      put_f32(v[k], fabsf(x) > kSmall ? y : small(x));
+    }
   }
 }
 __device__ __forceinline__ uint32_t h2(float lo, float hi) {
