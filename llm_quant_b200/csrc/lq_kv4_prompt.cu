@@ -455,9 +455,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
         const float e = sc.e[st];
         float sum = 0.0f;
         // Raises the row's reference to the greatest score m, and brings O to
-        // it once the last PV is complete.
+        // it once the last PV is complete.  References are whole numbers, so that
+        // what is there already, P' in f16 too, is multiplied by powers of two.
         auto raise = [&](float m) {
-          m = fmaxf(R, m == -INFINITY ? kNone : m + e);
+          m = fmaxf(R, m == -INFINITY ? kNone : ceilf(m + e));
           const float alpha = ex2(R - m);
           l *= alpha;
           sum *= alpha;
@@ -560,14 +561,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
               const float before = R;
               raise(m);
               if (c) {  // the first half's P' is there already
-                const __half2 alpha = __float2half2_rn(ex2(before - R));
+                const float alpha = ex2(before - R);
                 tmem_wait_st();  // of P' itself
                 tmem_ld16(S, p);
                 tmem_wait_ld16(p);
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
-                  const __half2 v = __hmul2(*reinterpret_cast<__half2*>(&p[k]), alpha);
-                  p[k] = *reinterpret_cast<const uint32_t*>(&v);
+                  const float2 v = f2(p[k]);
+                  p[k] = h2(v.x * alpha, v.y * alpha);
                 }
                 tmem_st16(S, p);
               }

@@ -477,6 +477,31 @@ def test_large_caps(L, dtype, S):
         assert (err <= 1.2 * mb).all(), (cap, float((err / mb).max()))
 
 
+def test_probabilities_of_chunks_are_rounded_once(L):
+    """32 tokens, then one whose score passes the reference's headroom in the
+    same step: the first 32 keep one rounding each.  They have the same
+    probability p and the value 1, the rest the value 0, so out = 32 p: off by
+    2^-11 for P, 2^-11 for the output, and 2 (dx + 2^-20) with dx = 12 * 2^-22
+    times a score of at most 9.1."""
+    S, T, D = 256, 64, 64
+    k = torch.zeros(1, 1, T, D, device="cuda", dtype=torch.float16)
+    k[..., 32, :2] = 1
+    v = torch.zeros(1, 1, T, D, device="cuda", dtype=torch.float16)
+    v[..., :32, :] = 1
+    cache = L.PackedKVCache(1, T)
+    cache.append(0, k, v)
+    q = torch.zeros(1, 8, S, D, device="cuda", dtype=torch.float16)
+    q[..., 0] = torch.linspace(6.5, 8.9, 8 * S, device="cuda").view(1, 8, S)
+    q[..., 1] = torch.rand(1, 8, S, generator=_gen(1), device="cuda") * 0.1
+    kv, vv = (x.double() for x in cache.get(0))
+    x = torch.einsum("hsd,td->hst", q[0].double(), kv[0, 0])
+    assert 6.4 < x.amax(-1).min() and x.max() < 9.1
+    ref = torch.softmax(x, -1) @ vv[0, 0]
+    out = cache.attend(0, q, scale=1.0, slopes=torch.zeros(8, device="cuda"))[0].double()
+    err = ((out - ref) / ref).abs().max().item()
+    assert err <= 2 * 2.0 ** -11 + 2 * (12 * 2.0 ** -22 * 9.1 + 2.0 ** -20), err * 2.0 ** 11
+
+
 def test_windows_and_prefixes_of_any_size(L):
     cache = L.PackedKVCache(1, 300)
     cache.append(0, *_kv(2, 2, 300, 64, torch.bfloat16, 8), counts=_ints(300, 77))
