@@ -989,7 +989,8 @@ __device__ __forceinline__ WeighItem weigh_item(const Attn& a, int idx) {
   return w;
 }
 
-template <typename T, int D>
+// CAP apart: its code beside the rest costs calls without a cap 2 % (instruction cache).
+template <typename T, int D, bool CAP>
 __global__ void __launch_bounds__(kWeighThreads, 1) kv4_weigh_kernel(const Attn a) {
   using L = WeighShared<D>;
   constexpr int W = D / 32;
@@ -1024,7 +1025,7 @@ __global__ void __launch_bounds__(kWeighThreads, 1) kv4_weigh_kernel(const Attn 
   tc_fence_after();
   const uint32_t tmem = sc.tmem;
   volatile int* fail = &sc.fail;
-  const float fk = a.sm * (a.cap > 0.0f ? 1.0f / a.cap : kLog2e);
+  const float fk = a.sm * (CAP ? 1.0f / a.cap : kLog2e);
   int longest = 0;
   for (int b = lane; b < a.kv.B; b += 32) longest = max(longest, min(a.kv.len[b], a.kv.cap));
   const int items = (__reduce_max_sync(0xffffffffu, longest) + kTok - 1) / kTok * a.kv.B * a.kv.H;
@@ -1047,7 +1048,7 @@ __global__ void __launch_bounds__(kWeighThreads, 1) kv4_weigh_kernel(const Attn 
         sk = sc.sk[item & 1][tid];
         if (!w.ordered) pos = sc.pos[item & 1][tid];
         const int q0 = w.first + div_g(a, rt * kTile), q1 = w.first + min(div_g(a, rt * kTile + kTile - 1), w.cnt - 1);
-        const bool plain = a.cap == 0.0f && !a.slopes &&
+        const bool plain = !CAP && !a.slopes &&
                            ((!a.causal && a.window <= 0) ||
                             (w.ordered && (!a.causal || w.t0 + kTok - 1 <= q0) && (a.window <= 0 || q1 - w.t0 < a.window)));
         if (plain) {
@@ -1085,7 +1086,7 @@ __global__ void __launch_bounds__(kWeighThreads, 1) kv4_weigh_kernel(const Attn 
             const uint32_t seen = pos < pre ? 0xffffffffu : bits_of(lo - c, hi - c);
 #pragma unroll
             for (int k = 0; k < 32; ++k) y[k] = __float_as_uint(__uint_as_float(y[k]) * sk);
-            if (a.cap > 0.0f) capped<32>(y, a.cap * kLog2e);
+            if constexpr (CAP) capped<32>(y, a.cap * kLog2e);
             if (a.slopes) {
 #pragma unroll
               for (int k = 0; k < 32; ++k)
@@ -1228,10 +1229,10 @@ __global__ void __launch_bounds__(kWeighThreads, 1) kv4_weigh_kernel(const Attn 
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u));
 }
 
-template <typename T, int D>
+template <typename T, int D, bool CAP>
 int run_weigh(const Attn& a, cudaStream_t st) {
   constexpr int smem = WeighShared<D>::bytes;
-  auto kern = kv4_weigh_kernel<T, D>;
+  auto kern = kv4_weigh_kernel<T, D, CAP>;
   static DeviceOnce once;
   LQ_TRY(once.allow_smem((const void*)kern, smem, "kv4_weigh_kernel"));
   const int64_t items = (int64_t)((a.kv.cap + kTok - 1) / kTok) * a.kv.B * a.kv.H;
@@ -1251,7 +1252,8 @@ int run_prompt(const Attn& a, cudaStream_t st) {
   LQ_TRY(launched("kv4_prompt_kernel"));
   launch_pdl(kv4_prompt_combine_kernel<D>, dim3((unsigned)(a.rows_pad / kMergeRows * a.kv.B * a.kv.H)), dim3(128), 0, st, a);
   LQ_TRY(launched("kv4_prompt_combine_kernel"));
-  return a.lse ? run_weigh<T, D>(a, st) : LQ_OK;
+  if (!a.lse) return LQ_OK;
+  return a.cap > 0.0f ? run_weigh<T, D, true>(a, st) : run_weigh<T, D, false>(a, st);
 }
 
 }  // namespace
