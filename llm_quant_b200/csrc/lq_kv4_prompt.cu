@@ -1077,7 +1077,7 @@ __global__ void __launch_bounds__(kWeighThreads, 1) kv4_weigh_kernel(const Attn 
           const int64_t hi_r = a.window > 0 ? ((int64_t)pos + a.window - w.first) * a.G - rt * kTile : kTile;
           const int64_t lo_r = a.causal ? ((int64_t)pos - w.first) * a.G - rt * kTile : 0;
           const int lo = (int)max(min(lo_r, (int64_t)kTile), (int64_t)-1), hi = (int)max(min(hi_r, (int64_t)kTile), (int64_t)-1);
-          const float d = (float)pos;
+          const float d = (float)(pos - w.first);  // and the queries count from 0: positions may pass 2^24
 #pragma unroll 1
           for (int c = 0; c < kTile; c += 32) {
             uint32_t y[32];
@@ -1166,7 +1166,7 @@ __global__ void __launch_bounds__(kWeighThreads, 1) kv4_weigh_kernel(const Attn 
         sc.nl[st][tid] = nl;
         if (rt + 1 < w.hi) nl = lse_of(rt + 1);
         const int r = rt * kTile + tid, i = div_g(a, r);
-        sc.at[st][tid] = w.first + i;
+        sc.at[st][tid] = i;
         if (a.slopes) sc.slope[st][tid] = r < a.rows ? a.slopes[w.h * a.G + r - i * a.G] * kLog2e : 0.0f;
         if (rt >= w.lo + 2) {
           staged<2>();

@@ -629,6 +629,24 @@ def test_masks_go_by_position_after_eviction(L):
             check_evict(cache, 150, recent=S, sinks=4)
 
 
+def test_distances_at_far_positions(L):
+    """Positions past 2^24, where fp32 has no more odd numbers: as after
+    so many tokens through a cache that evicts."""
+    far = 2 ** 25 + 1
+    for dtype in ALL:
+        cache = L.PackedKVCache(1, 300)
+        cache.append(0, *_kv(2, 2, 300, 64, dtype, 1), counts=_ints(300, 133))
+        st = cache._layers[0]
+        st.state[2:4] += far
+        st.state[6] = 1  # slots are not positions any more
+        st.positions.add_(far * (st.positions >= 0))
+        slopes = torch.exp2(-torch.arange(1, 9, device="cuda").float())
+        for S in (1, 70):
+            q = _q(2, 8, S, 64, dtype, 2)
+            for kw in ({}, {"causal": True}, {"causal": True, "window": 77}, {"causal": True, "softcap": 20.0}):
+                check(L, cache, q, slopes=slopes, **kw)
+
+
 def test_row_that_sees_nothing_after_eviction(L):
     """Everything within the window was evicted: zeros, and no weight."""
     cache = L.PackedKVCache(1, 64)
