@@ -77,6 +77,14 @@ class _LayerStore:
         self.emptied = self.captured and not capturing
 
 
+def _capturing(device: torch.device) -> bool:
+    """Whether the stream that calls on `device` go to is being captured."""
+    if device.index == torch.cuda.current_device():
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device.index):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
     """x with rows that the kernels can load: D contiguous, each row on a
     multiple of 4 elements.  A transposed projection qualifies as it is."""
@@ -155,7 +163,7 @@ class PackedKVCache(nn.Module):
                 raise ValueError(f"PackedKVCache.append: {S} tokens do not fit into {self.max_seq_len}")
             if B * H > 65535:
                 raise ValueError("PackedKVCache: more than 65535 (sequence, head) pairs")
-            if torch.cuda.is_current_stream_capturing():
+            if _capturing(key.device):
                 # a captured allocation would be filled, and so the cache emptied, by every replay
                 raise RuntimeError("PackedKVCache.append: a layer's first chunk (it may be empty, S = 0) must come "
                                    "before the capture")
@@ -167,7 +175,7 @@ class PackedKVCache(nn.Module):
         c = None if counts is None else self._vector(counts, B, torch.int32, st, "append: counts")
         if S == 0:
             return
-        capturing = torch.cuda.is_current_stream_capturing()
+        capturing = _capturing(st.device)
         if S > st.cap:
             raise ValueError(f"PackedKVCache.append: {S} tokens do not fit into {st.cap}")
         if not (capturing or st.captured) and st.bound + S > self.max_seq_len:
@@ -297,7 +305,7 @@ class PackedKVCache(nn.Module):
         if keep < 1 or recent < 0 or sinks < 0 or recent + sinks > keep:
             raise ValueError(f"PackedKVCache.evict: keep {keep} must be positive and hold the {recent} recent and "
                              f"{sinks} first tokens")
-        capturing = torch.cuda.is_current_stream_capturing()
+        capturing = _capturing(st.device)
         if keep >= st.cap or (keep >= st.bound and not st.captured and not capturing):
             return
         nbytes = _C.lib().lq_kv4_evict_workspace_bytes(st.B, st.H, st.cap, keep)
@@ -347,7 +355,7 @@ class PackedKVCache(nn.Module):
         """Clear one layer, or all; the buffers stay, and so do captured graphs."""
         for st in self._layers if layer_idx is None else [self._layers[layer_idx]]:
             if st is not None:
-                st.clear(torch.cuda.is_current_stream_capturing())
+                st.clear(_capturing(st.device))
                 self._call(st, "lq_kv4_reset")
 
     @property
@@ -356,6 +364,6 @@ class PackedKVCache(nn.Module):
         where a graph was captured and nothing but replays may have come since
         a ``reset`` does this wait for the device, to tell empty from not."""
         st = self._layers[0] if self.num_layers else None
-        if st is None or st.emptied and not torch.cuda.is_current_stream_capturing() and not st.state[:st.B].any():
+        if st is None or st.emptied and not _capturing(st.device) and not st.state[:st.B].any():
             return 0
         return st.bound

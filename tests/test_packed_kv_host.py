@@ -88,6 +88,33 @@ def test_caps_out_of_range(lib):
         assert b"softcap" in lib.lq_last_error()
 
 
+def test_captures_are_looked_for_on_the_caches_device(monkeypatch):
+    from llm_quant_b200 import packed_kv_cache as P
+    now = [0]
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, now[0] = now[0], self.index
+
+        def __exit__(self, *exc):
+            now[0] = self.before
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now[0] == 1)
+    assert P._capturing(torch.device("cuda", 1)) and not P._capturing(torch.device("cuda", 0))
+    st = object.__new__(P._LayerStore)
+    st.device, st.B, st.cap, st.bound, st.captured = torch.device("cuda", 1), 1, 64, 5, False
+    cache = L.PackedKVCache(1, 64)
+    cache._layers[0] = st
+    monkeypatch.setattr(cache, "_call", lambda *a: None)
+    cache.reset()
+    assert st.captured and cache.seq_len == 64 and now == [0]
+
+
 def test_python_layer_without_a_gpu():
     with pytest.raises(ValueError):
         L.PackedKVCache(1, 0)
