@@ -85,7 +85,7 @@ def _capturing(device: torch.device) -> bool:
         return torch.cuda.is_current_stream_capturing()
 
 
-def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
+def _rows(x: torch.Tensor) -> torch.Tensor:
     """x with rows that the kernels can load: D contiguous, each row on a
     multiple of 4 elements.  A transposed projection qualifies as it is."""
     sb, sh, ss, sd = x.stride()
@@ -181,7 +181,7 @@ class PackedKVCache(nn.Module):
         if not (capturing or st.captured) and st.bound + S > self.max_seq_len:
             raise ValueError(f"PackedKVCache.append: {S} more tokens than {st.bound} of {self.max_seq_len} "
                              "do not fit (evict, or reset)")
-        k, v = _rows(key, "append"), _rows(value, "append")
+        k, v = _rows(key), _rows(value)
         ks, vs = k.stride(), v.stride()
         self._call(st, "lq_kv4_append", k.data_ptr(), v.data_ptr(), _C.TORCH_TO_LQ[k.dtype], S, ks[0], ks[1], ks[2],
                    vs[0], vs[1], vs[2], c)
@@ -254,7 +254,7 @@ class PackedKVCache(nn.Module):
         key = (q.dtype, q.shape, q.stride(), q.device, scale, causal, softcap, window, accumulate, bound)
         form = st.forms.get(key)
         if form is None or q.data_ptr() & 15:
-            q = _rows(self._query(st, query), "attend")
+            q = _rows(self._query(st, query))
             form = self._form(st, q, scale, causal, softcap, window, accumulate, bound)
             if q.data_ptr() == query.data_ptr():
                 if len(st.forms) >= 256:
