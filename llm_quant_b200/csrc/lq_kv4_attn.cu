@@ -31,9 +31,9 @@
 // block covers is finished there; partial results of the others are merged by
 // kv4_combine_kernel, a programmatic dependent launch.
 //
-// Bound and measured (D = 128): 8 sequences x 8 kv heads x 4 of 8192 tokens 21.6
-// us, merge 4.7 (71 MB, 3.3 TB/s); 16 of up to 20011 tokens, groups of 8, 47.2 us,
-// merge 5.3 (196 MB, 4.2 TB/s).  The copies alone take 15 and 35.6 us; the rest
+// Bound and measured (D = 128): 8 sequences x 8 kv heads x 4 of 8192 tokens 21.9
+// us, merge 4.8 (71 MB, 3.3 TB/s); 16 of up to 20011 tokens, groups of 8, 47.7 us,
+// merge 5.4 (196 MB, 4.1 TB/s).  The copies alone take 15 and 35.6 us; the rest
 // is what mma.sync and the nibbles add (half of the MMAs taken out: -13 %).
 #include <algorithm>
 
@@ -60,11 +60,15 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
 // Fragment registers from a word of codes: nibble n of both halves as f16.
 // The tensor cores align a subnormal's product by the exponent 2^-14 it would
 // have as a normal number, and cut below 24 bits: a code whose unit is 2^(b -
-// 24) loses what is under 2^(-14 - b) of that unit, times the largest factor it
-// meets.  That is nothing beside a 16-bit output, so V takes nibbles where they
-// are with a mask and one shift for two (b = 0 and 4: 5 instructions for 8
-// codes); scores decide collected weights in fp32, so K is shifted to b = 4 (7);
-// with fp32 queries K and V are shifted to b = 6 (8).
+// 24) loses what is under 2^(-14 - b) of that unit, times the largest factor that
+// it meets among the 16 of an MMA.  V takes nibbles where they are with a mask and
+// one shift for two (b = 0 and 4: 5 instructions for 8 codes): an output then loses
+// up to 16 * 2^-14 of the V scale times the probability, as much as P's rounding to
+// f16 costs a value of 2 scales.  With all of them at b = 4 (7 instructions) it is
+// 2^-14, at 28.7 us instead of 27.0 (8 x 8 heads of 8192 tokens, groups of 4) and
+// 55.6 instead of 53.6 (16 of up to 20011, groups of 8): not worth it beside values that
+// are off by up to half a scale.  Scores decide collected weights in fp32, so K is
+// shifted to b = 4 (7); with fp32 queries K and V are shifted to b = 6 (8).
 enum Place { kMixed, kFour, kSix };
 template <Place P>
 struct Nibbles {
@@ -803,11 +807,17 @@ struct Plan {
   bool whole;     // a block to a head
   int pitch;      // scores kept per token for the collected weight; 0: none are kept
 };
-// Up to so many units a head is left to one block, and nothing has to be merged
-// (B=1, 8 heads, 500 tokens: 6.7 us, 10 us in two kernels).
+// Up to so many units a head is left to one block, and nothing has to be merged.
+// One block to a head against cut heads, us (D = 128, groups of 4): 512 tokens 7.1 /
+// 8.4 with one head, 7.2 / 8.7 with 8, 7.3 / 11.0 with 128, 12.5 / 19.7 with 512;
+// 1024 tokens 10.7 / 8.4, 10.8 / 8.8, 11.0 / 15.2, 20.0 / 26.0.
 constexpr int kWholeUnits = 16;
 constexpr int64_t kMostScores = 256 << 20;  // bytes of kept scores
-constexpr int kFewRows = 16;  // up to here a row of the cache is read once by this file's kernel
+// Up to so many query rows a row of the cache is read once by this file's kernel;
+// beyond, once per 16 rows, against once per 256 by the prompt kernel.  This against
+// that, us (D = 128): 16 rows 17.3 / 26.3 on 8 heads of 8192 tokens, 57.8 / 80.8 on 64
+// heads, 26.8 / 34.5 on 128 heads of 1000; 24 rows 22.7 / 26.9, 101 / 81, 42.3 / 35.0.
+constexpr int kFewRows = 16;
 Plan plan_of(const Kv4& kv, int64_t rows, int64_t bound, bool qlo, bool weigh) {
   Plan p;
   p.whole = false;

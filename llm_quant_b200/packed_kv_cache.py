@@ -236,10 +236,12 @@ class PackedKVCache(nn.Module):
 
         Scores are summed in fp32 from exact products; with 16-bit queries each
         probability is rounded once, to fp16 beside the greatest of its row,
-        before it meets the values.  More than 16 such queries to a kv head also
-        round it to 2^-24 of 2^7 and the greatest V scale among 128 slots: tokens
-        with a scale below 2^-20 of that lose bits.  Positions are int32, ``window`` is at most
-        2^30, a group has at most 4096 query heads, ``softcap`` is 0 or 1e-20 to 1e30.
+        before it meets the values.  Up to 16 such queries to a kv head also cut
+        products below 2^-14 of a V scale times the probability (2^-10 at most for
+        16 tokens); more round probabilities to 2^-24 of 2^7 and the greatest V
+        scale among 128 slots: tokens with a scale below 2^-20 of that lose bits.
+        Positions are int32, ``window`` is at most 2^30, a group has at most 4096
+        query heads, ``softcap`` is 0 or 1e-20 to 1e30.
 
         Inference only: no gradient is computed."""
         st = self._layer(layer_idx, "attend")

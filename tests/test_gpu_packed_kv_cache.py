@@ -303,6 +303,29 @@ def test_scales_of_every_size(L):
         assert (check(L, cache, _q(1, 4, 1, 64, dtype, 9)) == 0).all()
 
 
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("T", [2, 3, 7, 16, 40])
+def test_few_tokens_whose_values_cancel(L, T, dtype):
+    """Few rows and few tokens, V scales 2^10 apart: outputs near 0 show what
+    an MMA cuts off.  With 16-bit queries half of V's codes are subnormals of
+    which 2^-14 of a unit times the greatest p s_v among the 16 tokens of an
+    MMA may be lost, in each of its 16 products: 2^-10 times the sum of those
+    greatest ones beside the bound that the module's text derives."""
+    for D, G, S, seed in ((64, 1, 1, 0), (128, 8, 2, 1), (64, 3, 1, 2), (128, 4, 4, 3)):
+        k, v = _kv(4, 2, T, D, dtype, seed)
+        v = v * torch.exp2(torch.randint(-5, 5, (4, 2, T, 1), generator=_gen(seed), device="cuda").float()).to(dtype)
+        cache = L.PackedKVCache(1, T)
+        cache.append(0, k, v)
+        q = _q(4, 2 * G, S, D, dtype, seed + 5)
+        ref, bound, _, _, _ = reference(cache, 0, q)
+        x = torch.einsum("bhgsd,bhtd->bhgst", q.double().unflatten(1, (2, G)), cache.get(0)[0].double()) * D ** -0.5
+        s_v = cache._layers[0].params[:, :, :T, 1].bitwise_left_shift(16).view(torch.float32).double()
+        ps = torch.nn.functional.pad(torch.softmax(x, -1) * s_v[:, :, None, None], (0, -T % 16))
+        cut = 2.0 ** -10 * ps.unflatten(-1, (-1, 16)).amax(-1).sum(-1) if dtype != torch.float32 else ps.sum(-1) * 0
+        err = (cache.attend(0, q).double() - ref).abs() - cut.flatten(1, 2)[..., None]
+        assert (err <= bound).all(), float((err / bound).max())
+
+
 def test_nan_tokens_stay_behind_masks(L):
     """A NaN token reaches the queries that see it and no others."""
     k, v = (x.clone() for x in _kv(1, 2, 90, 64, torch.float16, 2))
