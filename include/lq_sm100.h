@@ -445,7 +445,7 @@ int lq_kv4_evict(const lq_kv4_cache* host_cache, int64_t keep, int64_t recent, i
  *   x = sm_scale * q.k;  softcap > 0: x = softcap * tanh(x / softcap);
  *   slopes [Hq] not NULL: x -= slopes[h] * |p - t|
  * and the query sees the token when
- *   ((not causal or t <= p) and (window <= 0 or p - t < window))
+ *   ((not causal or t <= p) and (window == 0 or p - t < window))
  *   or (prefix not NULL and t < prefix[b]).
  * accumulate: mass of each token += the weights it got from all query rows.
  * bound: tokens that the longest sequence is thought to hold (only the split

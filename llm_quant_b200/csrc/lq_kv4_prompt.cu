@@ -25,10 +25,12 @@
 // softmax is written with packed fp32 pairs (f32x2) so that its instructions
 // stay below that.
 //
-// Measured: 2048 queries of 8 kv heads x 4 on 8192 tokens, D = 128, causal: 340
-// us, merge 16; 0.43 of the bf16 rate.  Issue slots are 44 % used, the tensor pipe
+// Measured: 2048 queries of 8 kv heads x 4 on 8192 tokens, D = 128, causal: 339
+// us, merge 16; 0.42 of the bf16 rate.  Issue slots are 43 % used, the tensor pipe
 // 34 %, the special-function units 35 %: what holds it is the chain of a half
 // tile (S, load, exponentials, store, PV) with two softmax warps to a scheduler.
+// (D = 128 spills 112 bytes a thread.)  With cap, window and prefix, 3 x up to 777
+// queries of 4 kv heads x 2 on 1500 tokens, D = 64: 30.5 us, merge 7.1.
 //
 // Split: as in lq_kv4_attn.cu, the (row tile, token tile) pairs that have
 // anything to see lie in one row and each block takes an equal stretch;
@@ -946,7 +948,8 @@ __global__ void __launch_bounds__(128) kv4_prompt_combine_kernel(const Attn a) {
 // Warps: 0-3 and 4-7 sums of even and odd row tiles, 8-11 K's codes and the
 // query rows to operands, 12 the MMAs.  Bound: 16384 exponentials to a pair of
 // tiles, 1024 cycles, beside 512 of the tensor cores.  Measured: 2 x 1024 queries
-// of 8 kv heads x 4 on 2048 tokens, D = 128, causal: 75 us.
+// of 8 kv heads x 4 on 2048 tokens, D = 128, causal: 74 us (special-function units
+// 41 % while an SM has work, which it has for 71 % of the time).
 // ---------------------------------------------------------------------------
 constexpr int kWeighThreads = 416;
 constexpr int kQs = 4;  // stages of query rows; what belongs to rows is kept twice as long, for the sums

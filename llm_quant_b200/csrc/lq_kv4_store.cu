@@ -108,8 +108,9 @@ __device__ __forceinline__ uint32_t codes4(const float* x, const Grid& g) {
 // heads of unequal lengths even out, and no more, since each counts at the ticket
 // (64 heads x up to 2048 tokens: 21.6, 18.7, 20.8 us with 1, 2, 3 times as many).
 // 64 registers: 4 blocks per SM (20.3 us with 3).
-// Bound by instructions: some 300 to 512 values, a third of them for the codes;
-// 48 MB in 18.7 us are 2.6 TB/s.
+// Bound by instructions (370 to 512 values; 76 % of the issue slots of SMs that have
+// work) and, in that case, by heads of unequal lengths (SMs have work for 76 % of the
+// time); 48 MB in 18.9 us are 2.5 TB/s.
 template <typename T, int D>
 __global__ void __launch_bounds__(256, 4) kv4_append_kernel(Kv4 kv, AppendArgs a, int groups) {
   constexpr int LPT = D / 4, PPB = 256 / LPT, W = D / 32;  // lanes per token, pairs per block
