@@ -465,6 +465,53 @@ int lq_kv4_attention(const lq_kv4_cache* host_cache, const lq_kv4_attn* host_for
 /* An empty cache again (device work on `stream`). */
 int lq_kv4_reset(const lq_kv4_cache* host_cache, void* stream);
 
+/* ---- adapters of many requests -------------------------------------------------
+ * Low-rank adapters beside one shared projection; no counterpart in the
+ * reference, whose QLoRALinear holds one (qlora.py:230-324).  Adapter l:
+ * A [R, K] and B [R, N] (lora_B transposed), scaling[l].  For token t with
+ * adapter i:  out_t = base_t + scaling[i] B_i^T (A_i x_t), else out_t = base_t.
+ * fp16 or bf16; K and N multiples of 8 up to 2^22, R up to 128, L up to 8192, up
+ * to 2^24 tokens.  Products are summed in fp32 or more, u is kept in fp32 and
+ * each output is rounded once. */
+typedef struct {
+  const void* a;        /* [L, R, K] */
+  const void* b;        /* [L, R, N] */
+  const float* scaling; /* [L] */
+  int64_t L, R, K, N;
+  int dtype;
+} lq_adapter_bank;
+
+/* Which tokens use which adapter, for n = n_ids * seq_len tokens: token t uses
+ * ids[t / seq_len] (int32 or int64; outside [0, L): none), or none where t %
+ * seq_len >= counts[t / seq_len] (counts may be NULL).  plan: 16-byte aligned,
+ * of lq_adapter_plan_bytes; read by the calls below until it is built again. */
+size_t lq_adapter_plan_bytes(int64_t n, int64_t L);
+int lq_adapter_plan(const void* ids, int ids_dtype, int64_t n_ids, int64_t seq_len, const int32_t* counts,
+                    int64_t L, void* plan, void* stream);
+/* out [n, N] = base [n, N] (NULL: 0; may be out itself) + the adapters' share of
+ * x [n, K].  Strides are of rows, in elements, multiples of 8, as the addresses
+ * are of 16 bytes.  u [n, R] fp32: scaling * A x of the tokens with an adapter. */
+int lq_adapter_forward(const lq_adapter_bank* host_bank, const void* plan, int64_t n, const void* x, int64_t x_stride,
+                       const void* base, int64_t base_stride, void* out, int64_t out_stride, float* u, void* stream);
+/* Gradients for dy [n, N], the gradient of out (base's is dy itself): dx [n, K],
+ * da [L, R, K], db [L, R, N] in grad_dtype (LQ_F32 or the bank's), all
+ * contiguous; a NULL one is not computed.  u is what the forward call left. */
+size_t lq_adapter_backward_workspace_bytes(const lq_adapter_bank* host_bank, int64_t n);
+int lq_adapter_backward(const lq_adapter_bank* host_bank, const void* plan, int64_t n, const void* x, int64_t x_stride,
+                        const void* dy, int64_t dy_stride, const float* u, void* dx, void* da, void* db,
+                        int grad_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- gradients -----------------------------------------------------------------
+ * norm = sqrt(sum of the squares of all values of `count` tensors together), out
+ * = in * min(1, max_norm / (norm + 1e-6)); no counterpart in the reference.  The
+ * host arrays give each tensor's address, its result's (host_out NULL: in
+ * place), its number of values, side by side, and its dtype (float types, mixed);
+ * they are read before the call returns.  Tensors must not overlap.  norm: one
+ * fp32 value on the device. */
+size_t lq_clip_workspace_bytes(int64_t count);
+int lq_clip_grad_norm(const void* const* host_in, void* const* host_out, const int64_t* host_n, const int* host_dtype,
+                      int64_t count, double max_norm, float* norm, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -83,6 +83,10 @@ _SIGS = {
     "lq_kv4_evict": [_V, _L, _L, _L, _V, ctypes.c_size_t, _V],
     "lq_kv4_attention": [_V, _V, _V, _V, _V, _V, _V, _V, ctypes.c_size_t, _V],
     "lq_kv4_reset": [_V, _V],
+    "lq_adapter_plan": [_V, _I, _L, _L, _V, _L, _V, _V],
+    "lq_adapter_forward": [_V, _V, _L, _V, _L, _V, _L, _V, _L, _V, _V],
+    "lq_adapter_backward": [_V, _V, _L, _V, _L, _V, _L, _V, _V, _V, _V, _I, _V, ctypes.c_size_t, _V],
+    "lq_clip_grad_norm": [_V, _V, _V, _V, _L, ctypes.c_double, _V, _V, ctypes.c_size_t, _V],
 }
 _SIZE_SIGS = {
     "lq_tensor_qparams_workspace_size": [_L],
@@ -92,6 +96,9 @@ _SIZE_SIGS = {
     "lq_kv_attention_workspace_bytes": [_L, _L, _L, _L, _L, _L],
     "lq_kv4_evict_workspace_bytes": [_L, _L, _L, _L],
     "lq_kv4_attention_workspace_bytes": [_V, _V],
+    "lq_clip_workspace_bytes": [_L],
+    "lq_adapter_plan_bytes": [_L, _L],
+    "lq_adapter_backward_workspace_bytes": [_V, _L],
 }
 
 
@@ -106,6 +113,11 @@ class KV4Attn(ctypes.Structure):
     _fields_ = [(n, _L) for n in ("Hq", "Sq", "q_sb", "q_sh", "q_ss", "bound", "window")] + \
                [(n, ctypes.c_float) for n in ("sm_scale", "softcap")] + \
                [(n, _I) for n in ("q_dtype", "causal", "accumulate")]
+
+
+class AdapterBank(ctypes.Structure):
+    """lq_adapter_bank"""
+    _fields_ = [(n, _V) for n in ("a", "b", "scaling")] + [(n, _L) for n in ("L", "R", "K", "N")] + [("dtype", _I)]
 
 
 _lib = None

@@ -18,7 +18,12 @@ hand-written CUDA kernels in ``liblq_sm100.so`` on CUDA tensors:
 * ``llm_quant_b200.kv_cache_quant``: KV-cache quantizers and QuantizedKVCache;
 * ``llm_quant_b200.packed_kv_cache``: PackedKVCache, a KV cache held in 4 bits
   with its attention, collected attention weights and eviction (beyond the
-  reference).
+  reference);
+* ``llm_quant_b200.adapters``: AdapterBank and AdapterBatch, low-rank adapters
+  of many requests beside one shared projection, with their gradients (beyond
+  the reference);
+* ``llm_quant_b200.grad_clip``: GradClipper and clip_grad_norm_, the norm of
+  many gradients together and their clipping (beyond the reference).
 
 ``install_as_llm_quant()`` registers these modules under the reference's
 import names (``llm_quant``, ``llm_quant.core.quantizer``, ...) for code
@@ -66,6 +71,8 @@ from .kv_cache_quant import (
     PerGroupKVCacheQuantizer, kv_cache_memory_ratio,
 )
 from .packed_kv_cache import PackedKVCache
+from .adapters import AdapterBank, AdapterBatch
+from .grad_clip import GradClipper, clip_grad_norm_
 from .gptq import GPTQLinear
 from .spqr import SpQRLinear
 
@@ -87,6 +94,8 @@ __all__ = [
     "PerTokenKVCacheQuantizer", "PerChannelKVCacheQuantizer",
     "PerGroupKVCacheQuantizer", "kv_cache_memory_ratio",
     "PackedKVCache",
+    "AdapterBank", "AdapterBatch",
+    "GradClipper", "clip_grad_norm_",
     "GPTQLinear", "SpQRLinear",
     "install_as_llm_quant",
 ]

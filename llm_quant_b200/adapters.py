@@ -1,0 +1,286 @@
+"""llm_quant_b200.adapters -- low-rank adapters of many requests beside one shared projection.
+
+``QLoRALinear`` holds one adapter.  An ``AdapterBank`` holds L of them for a
+projection from K to N features, an ``AdapterBatch`` says which of a batch's
+tokens use which, and one call adds each token's own share to what the shared
+projection gave:
+
+    y_t = base_t + scaling[i] * lora_B[i]^T (lora_A[i] x_t)     i: the adapter of token t
+    y_t = base_t                                                for a token without one
+
+and, in training, gives the gradients of x, of all lora_A and of all lora_B.
+The reference has no counterpart (its QLoRALinear.forward, qlora.py:306-312, is
+the case of one adapter).
+
+Activations are float16 or bfloat16.  Products are exact and summed in fp32,
+``scaling * lora_A x`` is kept in fp32, and each output is rounded once.
+Parameters may be float32 (a training run's master weights): they are rounded
+to the activations' dtype at each call and their gradients come in float32.
+Sums go in an order of their own: equal calls give equal bits.
+
+Nothing here reads the device on the host, so plans, calls and their backward
+passes can be captured into a CUDA graph and replayed (as for any module, with
+no eager graph of the same parameters alive while a backward pass is captured).
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Iterable, Optional
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import _C
+
+_HALF = (torch.float16, torch.bfloat16)
+MAX_RANK, MAX_ADAPTERS, MAX_TOKENS = 128, 8192, 1 << 24
+
+
+def _call(device: torch.device, name: str, *args) -> None:
+    """Call an entry point on `device` and its current stream."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        _C.call(name, *args, _C.raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            _C.call(name, *args, _C.raw_stream(index))
+
+
+def _changed(t: torch.Tensor) -> None:
+    """Tell autograd that a kernel wrote to t."""
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+
+
+class AdapterBatch:
+    """Which tokens of a batch use which adapter: built once for all
+    projections of a step, on the device.
+
+    ``ids`` (int32 or int64 [n], on the device) is the adapter of each request;
+    a value outside [0, num_adapters) (say -1) means none.  A request has
+    ``seq_len`` tokens: the batch is n * seq_len tokens, as the rows of x
+    [n, seq_len, K] or [n * seq_len, K].  ``counts`` (int32 [n], on the device)
+    says how many of them are tokens, the rest being padding, which uses no
+    adapter; default all.  ``ids`` of shape [n, seq_len] with ``seq_len`` left at
+    1 give every token an adapter of its own.
+
+    ``update`` writes the plan for new requests in place, so that a captured
+    call sees them when it is replayed."""
+
+    def __init__(self, ids: torch.Tensor, num_adapters: int, seq_len: int = 1,
+                 counts: Optional[torch.Tensor] = None):
+        _C.require_cuda(ids, what="AdapterBatch")
+        if not 1 <= num_adapters <= MAX_ADAPTERS:
+            raise ValueError(f"AdapterBatch: num_adapters {num_adapters} outside [1, {MAX_ADAPTERS}]")
+        if seq_len < 0 or ids.numel() * seq_len > MAX_TOKENS:
+            raise ValueError(f"AdapterBatch: {ids.numel()} requests of {seq_len} tokens outside [0, 2^24] tokens")
+        self.num_adapters, self.seq_len, self.requests = num_adapters, seq_len, ids.numel()
+        self.tokens = self.requests * seq_len
+        self.device = ids.device
+        self._plan = torch.empty(_C.lib().lq_adapter_plan_bytes(self.tokens, num_adapters), dtype=torch.uint8,
+                                 device=ids.device)
+        self.update(ids, counts)
+
+    def update(self, ids: torch.Tensor, counts: Optional[torch.Tensor] = None) -> None:
+        """The plan of other requests, as many and as long."""
+        if ids.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"AdapterBatch: ids must be int32 or int64, not {ids.dtype}")
+        if ids.device != self.device or ids.numel() != self.requests:
+            raise ValueError(f"AdapterBatch: {ids.numel()} ids on {ids.device}, expected {self.requests} on {self.device}")
+        if counts is not None and (counts.dtype != torch.int32 or counts.device != self.device
+                                   or counts.numel() != self.requests):
+            raise ValueError(f"AdapterBatch: counts must be {self.requests} int32 values on {self.device}")
+        if self.tokens == 0:
+            return
+        ids = ids.contiguous()
+        counts = None if counts is None else counts.contiguous()
+        _changed(self._plan)  # a backward pass of the old plan raises
+        _call(self.device, "lq_adapter_plan", ids.data_ptr(), _C.dt(ids), self.requests, self.seq_len, _C.ptr(counts),
+              self.num_adapters, self._plan.data_ptr())
+
+
+def _rows(x: torch.Tensor, width: int):
+    """x as rows of `width` values that the kernels can read, and their stride:
+    the values side by side, rows on 16 bytes."""
+    x2 = x if x.ndim == 2 else x.reshape(-1, width)
+    stride = x2.stride(0) if x2.shape[0] > 1 else width
+    if x2.stride(1) == 1 and stride >= 0 and stride % 8 == 0 and x2.data_ptr() % 16 == 0:
+        return x2, stride
+    return x2.contiguous() if not x2.is_contiguous() else x2.clone(), width
+
+
+class AdapterBank(nn.Module):
+    """L adapters of one projection (see the module's documentation).
+
+    ``lora_A`` [L, rank, in_features], ``lora_B`` [L, rank, out_features] (each
+    adapter's lora_B of QLoRALinear transposed; zeros at the start) and
+    ``scaling`` [L] (float32; alpha / rank).  in_features and out_features are
+    multiples of 8, rank is at most 128: a smaller adapter's rows are filled
+    up with zeros and stay so in training."""
+
+    def __init__(self, in_features: int, out_features: int, num_adapters: int, rank: int = 16, alpha: float = 16.0,
+                 *, dtype: torch.dtype = torch.bfloat16, device=None):
+        super().__init__()
+        for name, n in (("in_features", in_features), ("out_features", out_features)):
+            if n < 8 or n % 8 or n > 1 << 22:
+                raise ValueError(f"AdapterBank: {name} {n} must be a multiple of 8 up to 2^22")
+        if not 1 <= rank <= MAX_RANK:
+            raise ValueError(f"AdapterBank: rank {rank} outside [1, {MAX_RANK}]")
+        if not 1 <= num_adapters <= MAX_ADAPTERS:
+            raise ValueError(f"AdapterBank: num_adapters {num_adapters} outside [1, {MAX_ADAPTERS}]")
+        if dtype not in _C.FLOAT_TYPES:
+            raise TypeError(f"AdapterBank: unsupported dtype {dtype} (float32, float16, bfloat16)")
+        self.in_features, self.out_features = in_features, out_features
+        self.num_adapters, self.rank = num_adapters, rank
+        self.lora_A = nn.Parameter(torch.empty(num_adapters, rank, in_features, dtype=dtype, device=device))
+        self.lora_B = nn.Parameter(torch.zeros(num_adapters, rank, out_features, dtype=dtype, device=device))
+        self.register_buffer("scaling", torch.full((num_adapters,), alpha / rank, dtype=torch.float32, device=device))
+        bound = 1.0 / math.sqrt(in_features)  # as QLoRALinear's
+        nn.init.uniform_(self.lora_A, -bound, bound)
+        self._c = (None, None)  # the bank as the entry points take it, and its addresses
+
+    @classmethod
+    def from_layers(cls, layers: Iterable, *, dtype: torch.dtype = torch.bfloat16) -> "AdapterBank":
+        """The adapters of several QLoRALinear of one shape, as one bank."""
+        layers = list(layers)
+        if not layers:
+            raise ValueError("AdapterBank.from_layers: no layers")
+        bank = cls(layers[0].in_features, layers[0].out_features, len(layers), max(ql.rank for ql in layers),
+                   dtype=dtype, device=layers[0].lora_A.device)
+        for i, ql in enumerate(layers):
+            bank.load_adapter(i, ql.lora_A, ql.lora_B, ql.scaling)
+        return bank
+
+    @torch.no_grad()
+    def load_adapter(self, index: int, lora_A: torch.Tensor, lora_B: torch.Tensor, scaling: float) -> None:
+        """Adapter `index` from lora_A [r, in_features] and lora_B
+        [out_features, r], r up to the bank's rank."""
+        r = lora_A.shape[0]
+        if not 0 <= index < self.num_adapters:
+            raise IndexError(f"AdapterBank.load_adapter: {index} outside [0, {self.num_adapters})")
+        if lora_A.shape != (r, self.in_features) or lora_B.shape != (self.out_features, r) or r > self.rank:
+            raise ValueError(f"AdapterBank.load_adapter: lora_A {list(lora_A.shape)} and lora_B {list(lora_B.shape)} for "
+                             f"a bank of {self.in_features} to {self.out_features} features, rank {self.rank}")
+        self.lora_A[index, :r] = lora_A
+        self.lora_A[index, r:] = 0
+        self.lora_B[index, :r] = lora_B.t()
+        self.lora_B[index, r:] = 0
+        self.scaling[index] = scaling
+
+    # -- calls -------------------------------------------------------------------
+    def _struct(self, a: torch.Tensor, b: torch.Tensor, s: torch.Tensor):
+        key = (a.data_ptr(), b.data_ptr(), s.data_ptr(), a.dtype)
+        at, c = self._c
+        if at != key:
+            c = _C.AdapterBank(*key[:3], self.num_adapters, self.rank, self.in_features, self.out_features, _C.dt(a))
+            self._c = (key, c)  # the struct itself is never changed
+        return ctypes.byref(c)
+
+    def _check(self, x: torch.Tensor, batch: AdapterBatch, base: Optional[torch.Tensor]) -> None:
+        _C.require_cuda(x, what="AdapterBank")
+        if x.dtype not in _HALF:
+            raise TypeError(f"AdapterBank: unsupported dtype {x.dtype} (float16, bfloat16)")
+        if x.shape[-1:] != (self.in_features,) or x.numel() != batch.tokens * self.in_features:
+            raise RuntimeError(f"AdapterBank: x {list(x.shape)} is not {batch.tokens} tokens of {self.in_features} features")
+        if batch.num_adapters != self.num_adapters:
+            raise ValueError(f"AdapterBank: a batch for {batch.num_adapters} adapters, a bank of {self.num_adapters}")
+        dev = x.device
+        if self.lora_A.device != dev or self.lora_B.device != dev or self.scaling.device != dev or batch.device != dev:
+            raise RuntimeError(f"AdapterBank: x on {dev}, the bank on {self.lora_A.device}, the batch on {batch.device}")
+        if self.lora_A.dtype != self.lora_B.dtype:
+            raise TypeError(f"AdapterBank: lora_A is {self.lora_A.dtype}, lora_B {self.lora_B.dtype}")
+        if self.scaling.dtype != torch.float32:
+            raise TypeError(f"AdapterBank: scaling must stay float32, not {self.scaling.dtype}")
+        if base is not None and (base.dtype != x.dtype or base.device != dev
+                                 or base.shape != x.shape[:-1] + (self.out_features,)):
+            raise RuntimeError(f"AdapterBank: base {list(base.shape)} {base.dtype} on {base.device} for x {list(x.shape)} "
+                               f"{x.dtype} on {dev}")
+
+    def _weights(self, dtype: torch.dtype):
+        a, b = self.lora_A, self.lora_B
+        if a.dtype != dtype:
+            a = a.detach().to(dtype)
+        if b.dtype != dtype:
+            b = b.detach().to(dtype)
+        return a.contiguous(), b.contiguous()
+
+    def _forward(self, x: torch.Tensor, batch: AdapterBatch, base: Optional[torch.Tensor], out: Optional[torch.Tensor] = None):
+        """(out, u, a, b): out [..., out_features] is made here unless given as rows."""
+        n, dev = batch.tokens, x.device
+        x2, xs = _rows(x, self.in_features)
+        b2, bs = (None, 0) if base is None else _rows(base, self.out_features)
+        y, ys = (x.new_empty(x.shape[:-1] + (self.out_features,)), self.out_features) if out is None else (out, out.stride(0))
+        u = torch.empty(n, self.rank, dtype=torch.float32, device=dev)
+        a, b = self._weights(x.dtype)
+        if n:
+            _call(dev, "lq_adapter_forward", self._struct(a, b, self.scaling), batch._plan.data_ptr(), n, x2.data_ptr(), xs,
+                  None if b2 is None else b2.data_ptr(), bs, y.data_ptr(), ys, u.data_ptr())
+        return y, u, a, b
+
+    def forward(self, x: torch.Tensor, batch: AdapterBatch, base: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """base [..., out_features] (default zeros) plus each token's adapter of
+        x [..., in_features], whose leading dimensions are the batch's tokens."""
+        self._check(x, batch, base)
+        if torch.is_grad_enabled() and (x.requires_grad or self.lora_A.requires_grad or self.lora_B.requires_grad
+                                        or base is not None and base.requires_grad):
+            return _Adapters.apply(x, self.lora_A, self.lora_B, base, self, batch)
+        return self._forward(x, batch, base)[0]
+
+    def add_(self, y: torch.Tensor, x: torch.Tensor, batch: AdapterBatch) -> torch.Tensor:
+        """y += each token's adapter of x, in place; no gradient (call it under
+        ``torch.no_grad()``).  Rows of tokens without an adapter are not written."""
+        self._check(x, batch, y)
+        if torch.is_grad_enabled() and (x.requires_grad or y.requires_grad or self.lora_A.requires_grad
+                                        or self.lora_B.requires_grad):
+            raise RuntimeError("AdapterBank.add_: no gradient is computed here (use forward, or torch.no_grad())")
+        try:
+            y2 = y.view(-1, self.out_features)
+        except RuntimeError:
+            y2 = None
+        if y2 is None or y2.stride(1) != 1 or y2.data_ptr() % 16 \
+                or y2.shape[0] > 1 and (y2.stride(0) % 8 or y2.stride(0) < self.out_features):
+            raise ValueError(f"AdapterBank.add_: y {list(y.shape)} with strides {list(y.stride())} must be rows on 16 bytes")
+        if y2.shape[0] == 1:
+            y2 = y2.as_strided(y2.shape, (self.out_features, 1))
+        self._forward(x, batch, y2, out=y2)
+        _changed(y)
+        return y
+
+    def extra_repr(self) -> str:
+        return (f"in={self.in_features}, out={self.out_features}, adapters={self.num_adapters}, rank={self.rank}, "
+                f"dtype={self.lora_A.dtype}")
+
+
+class _Adapters(torch.autograd.Function):
+    """AdapterBank.forward with the gradients of x, lora_A, lora_B and base."""
+
+    @staticmethod
+    def forward(ctx, x, lora_A, lora_B, base, bank, batch):
+        y, u, a, b = bank._forward(x, batch, base)
+        # the weights as the call rounded them; scaling and the plan raise if they were changed since
+        ctx.save_for_backward(x, a, b, u, bank.scaling, batch._plan)
+        ctx.bank, ctx.tokens = bank, batch.tokens
+        ctx.dtype = lora_A.dtype
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, a, b, u, scaling, plan = ctx.saved_tensors
+        bank, n, dev = ctx.bank, ctx.tokens, x.device
+        want_x, want_a, want_b, want_base = ctx.needs_input_grad[:4]
+        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_x else None
+        da = torch.empty(a.shape, dtype=ctx.dtype, device=dev) if want_a else None
+        db = torch.empty(b.shape, dtype=ctx.dtype, device=dev) if want_b else None
+        if want_x or want_a or want_b:
+            x2, xs = _rows(x, bank.in_features)
+            d2, ds = _rows(dy, bank.out_features)
+            ref = bank._struct(a, b, scaling)
+            nbytes = _C.lib().lq_adapter_backward_workspace_bytes(ref, n)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            _call(dev, "lq_adapter_backward", ref, plan.data_ptr(), n, x2.data_ptr(), xs, d2.data_ptr(), ds, u.data_ptr(),
+                  _C.ptr(dx), _C.ptr(da), _C.ptr(db), _C.dt(ctx.dtype), ws.data_ptr(), nbytes)
+        return dx, da, db, dy if want_base else None, None, None

@@ -1,0 +1,298 @@
+// lq_adapters.cu -- low-rank adapters of many requests beside one shared
+// projection: y_t = base_t + s_i B_i^T (A_i x_t) with i the adapter of token t,
+// and the gradients of x, A and B.  A is [L, R, K], B is [L, R, N] (each
+// adapter's lora_B transposed), so that both directions are the same three
+// products: rows times a factor (u = s A x, v = s B dy), a low-rank row times a
+// factor (y = B^T u, dx = A^T v) and sums of outer products over an adapter's
+// tokens (dA = v x^T, dB = u dy^T).  u and v are kept in fp32.
+#include "lq_adapters.cuh"
+
+namespace lq {
+namespace {
+
+// ---------------------------------------------------------------------------
+// The plan.  A block to an adapter (block L: the tokens without one) counts all
+// tokens by adapter in shared memory (integers: no order of atomics shows), adds
+// up the counts below its own, and writes its tokens, in order, by ballots.
+// Every block counts for itself: T reads from L2 each, and no second launch.
+// ---------------------------------------------------------------------------
+constexpr int kPlanThreads = 512;
+
+template <typename I>
+__device__ __forceinline__ int owner_of(const I* ids, const int* counts, int64_t seq, int L, int64_t t) {
+  const int64_t b = seq == 1 ? t : t / seq;
+  if (counts && t - b * seq >= counts[b]) return L;
+  const int64_t i = static_cast<int64_t>(ids[b]);
+  return i >= 0 && i < L ? static_cast<int>(i) : L;
+}
+
+template <typename I>
+__global__ void __launch_bounds__(kPlanThreads) ad_plan_kernel(const I* __restrict__ ids, const int* __restrict__ counts,
+                                                               int64_t seq, int T, int L, AdPlan p) {
+  extern __shared__ int hist[];  // [L + 1]
+  __shared__ int part[2][kPlanThreads / 32];
+  __shared__ int base[2];
+  const int me = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  for (int i = tid; i <= L; i += kPlanThreads) hist[i] = 0;
+  __syncthreads();
+  for (int t = tid; t < T; t += kPlanThreads) {
+    const int o = owner_of(ids, counts, seq, L, t);
+    atomicAdd(&hist[o], 1);
+    if (me == L) p.owner[t] = o == L ? -1 : o;
+  }
+  __syncthreads();
+  int before = 0, tiles = 0;
+  for (int i = tid; i < me; i += kPlanThreads) before += hist[i], tiles += (hist[i] + kAdTile - 1) / kAdTile;
+#pragma unroll
+  for (int m = 16; m; m >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, m);
+    tiles += __shfl_xor_sync(0xffffffffu, tiles, m);
+  }
+  if (lane == 0) part[0][warp] = before, part[1][warp] = tiles;
+  __syncthreads();
+  if (tid < 2) {
+    int s = 0;
+    for (int w = 0; w < kPlanThreads / 32; ++w) s += part[tid][w];
+    base[tid] = s;
+  }
+  __syncthreads();
+  const int first = base[0], tile = base[1], n = hist[me], n_tiles = (n + kAdTile - 1) / kAdTile;
+  if (tid == 0) {
+    p.start[me] = first, p.tile_of[me] = tile;
+    if (me == L) p.start[L + 1] = first + n, p.tile_of[L + 1] = tile + n_tiles;
+  }
+  int at = first;
+  for (int t0 = 0; t0 < T && at < first + n; t0 += kPlanThreads) {
+    const int t = t0 + tid;
+    const bool mine = t < T && owner_of(ids, counts, seq, L, t) == me;
+    const unsigned m = __ballot_sync(0xffffffffu, mine);
+    __syncthreads();  // part was read
+    if (lane == 0) part[0][warp] = __popc(m);
+    __syncthreads();
+    int below = 0, all = 0;
+    for (int w = 0; w < kPlanThreads / 32; ++w) {
+      below += w < warp ? part[0][w] : 0;
+      all += part[0][w];
+    }
+    if (mine) p.order[at + below + __popc(m & ((1u << lane) - 1))] = t;
+    at += all;
+  }
+  __syncthreads();  // the block's own order, read back below
+  for (int i = tid; i < n_tiles; i += kPlanThreads) {
+    AdTile d;
+    d.owner = me == L ? -1 : me;
+    d.first = first + i * kAdTile;
+    d.rows = min(kAdTile, n - i * kAdTile);
+    const int a = p.order[d.first], z = p.order[d.first + d.rows - 1];
+    d.run = z - a == d.rows - 1 ? a : -1;
+    p.tiles[tile + i] = d;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// A block to a token: u[t][r] = s sum_k f[r][k] x[t][k], a warp to a rank row.
+// ---------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(256) ad_down_kernel(const T* __restrict__ x, int64_t stride, const T* __restrict__ f,
+                                                      const float* __restrict__ scaling, int R, int K,
+                                                      const int* __restrict__ owner, float* __restrict__ u) {
+  const int64_t t = blockIdx.x;
+  const int o = owner[t];
+  if (o < 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int r = warp; r < R; r += 8) {
+    const T* row = f + ((int64_t)o * R + r) * K;
+    float s = 0.0f;
+    for (int k = lane * 8; k < K; k += 256) {
+      Vec16<T> a, b;
+      a.u = *reinterpret_cast<const uint4*>(row + k);
+      b.u = *reinterpret_cast<const uint4*>(x + t * stride + k);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s = fmaf(Ty<T>::to_f(a.v[i]), Ty<T>::to_f(b.v[i]), s);
+    }
+#pragma unroll
+    for (int m = 16; m; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
+    if (lane == 0) u[t * R + r] = s * scaling[o];
+  }
+}
+
+// A block to a token and 2048 columns: out[t][c] = base[t][c] + sum_r u[t][r] f[r][c].
+template <typename T>
+__global__ void __launch_bounds__(256) ad_up_kernel(const float* __restrict__ u, const T* __restrict__ f, int R, int N,
+                                                    const int* __restrict__ owner, const T* base, int64_t base_stride,
+                                                    T* out, int64_t out_stride) {
+  const int64_t t = blockIdx.x;
+  const int c = (blockIdx.y * 256 + threadIdx.x) * 8;
+  if (c >= N) return;
+  const int o = owner[t];
+  float s[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s[i] = 0.0f;
+  for (int r = 0; r < (o < 0 ? 0 : R); ++r) {
+    Vec16<T> a;
+    a.u = *reinterpret_cast<const uint4*>(f + ((int64_t)o * R + r) * N + c);
+    const float w = u[t * R + r];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] = fmaf(w, Ty<T>::to_f(a.v[i]), s[i]);
+  }
+  Vec16<T> y;
+  y.u = base ? *reinterpret_cast<const uint4*>(base + t * base_stride + c) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y.v[i] = Ty<T>::from_f(Ty<T>::to_f(y.v[i]) + s[i]);
+  *reinterpret_cast<uint4*>(out + t * out_stride + c) = y.u;
+}
+
+// A block to an adapter, 256 columns and 16 ranks: g[l][r][c] = sum_t u[t][r] x[t][c].
+template <typename T, typename G>
+__global__ void __launch_bounds__(256) ad_outer_kernel(const float* __restrict__ u, const T* __restrict__ x, int64_t stride,
+                                                       int R, int K, AdPlan p, G* __restrict__ g) {
+  const int l = blockIdx.x, c = blockIdx.y * 256 + threadIdx.x, r0 = blockIdx.z * 16;
+  if (c >= K) return;
+  float s[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+  for (int j = p.start[l]; j < p.start[l + 1]; ++j) {
+    const int64_t t = p.order[j];
+    const float v = Ty<T>::to_f(x[t * stride + c]);
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (r0 + i < R) s[i] = fmaf(u[t * R + r0 + i], v, s[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (r0 + i < R) g[((int64_t)l * R + r0 + i) * K + c] = Ty<G>::from_f(s[i]);
+}
+
+template <typename T>
+int down(const lq_adapter_bank& b, const AdPlan& p, int64_t n, const void* x, int64_t stride, bool is_a, float* u,
+         cudaStream_t st) {
+  const int K = (int)(is_a ? b.K : b.N);
+  ad_down_kernel<T><<<(unsigned)n, 256, 0, st>>>(static_cast<const T*>(x), stride, static_cast<const T*>(is_a ? b.a : b.b),
+                                                 b.scaling, (int)b.R, K, p.owner, u);
+  return launched("ad_down_kernel");
+}
+template <typename T>
+int up(const lq_adapter_bank& b, const AdPlan& p, int64_t n, const float* u, bool is_a, const void* base, int64_t bs,
+       void* out, int64_t os, cudaStream_t st) {
+  const int N = (int)(is_a ? b.K : b.N);
+  ad_up_kernel<T><<<dim3((unsigned)n, (N + 2047) / 2048), 256, 0, st>>>(
+      u, static_cast<const T*>(is_a ? b.a : b.b), (int)b.R, N, p.owner, static_cast<const T*>(base), bs,
+      static_cast<T*>(out), os);
+  return launched("ad_up_kernel");
+}
+template <typename T>
+int outer(const lq_adapter_bank& b, const AdPlan& p, const float* u, const void* x, int64_t stride, bool is_a, void* g,
+          int grad_dtype, cudaStream_t st) {
+  const int K = (int)(is_a ? b.K : b.N);
+  const dim3 grid((unsigned)b.L, (K + 255) / 256, (unsigned)(b.R + 15) / 16);
+  if (grad_dtype == LQ_F32)
+    ad_outer_kernel<T, float><<<grid, 256, 0, st>>>(u, static_cast<const T*>(x), stride, (int)b.R, K, p, static_cast<float*>(g));
+  else
+    ad_outer_kernel<T, T><<<grid, 256, 0, st>>>(u, static_cast<const T*>(x), stride, (int)b.R, K, p, static_cast<T*>(g));
+  return launched("ad_outer_kernel");
+}
+
+int check_bank(const lq_adapter_bank* b, const void* plan, int64_t n) {
+  LQ_REQUIRE(b && b->a && b->b && b->scaling, LQ_EINVAL, "adapters: NULL bank");
+  LQ_REQUIRE(b->dtype == LQ_F16 || b->dtype == LQ_BF16, LQ_EDTYPE, "adapters: fp16 or bf16 (got dtype %d)", b->dtype);
+  LQ_REQUIRE(b->L >= 1 && b->L <= kAdMaxAdapters, LQ_ERANGE, "adapters: %lld adapters outside [1, %d]", (long long)b->L,
+             kAdMaxAdapters);
+  LQ_REQUIRE(b->R >= 1 && b->R <= kAdMaxRank, LQ_ERANGE, "adapters: rank %lld outside [1, %d]", (long long)b->R, kAdMaxRank);
+  LQ_REQUIRE(b->K >= 8 && b->N >= 8 && b->K <= (1 << 22) && b->N <= (1 << 22), LQ_ERANGE, "adapters: features outside [8, 2^22]");
+  LQ_REQUIRE(b->K % 8 == 0 && b->N % 8 == 0, LQ_EALIGN, "adapters: features must be multiples of 8");
+  LQ_REQUIRE(aligned16(b->a) && aligned16(b->b), LQ_EALIGN, "adapters: weights must be 16-byte aligned");
+  LQ_REQUIRE(n >= 0 && n <= (1 << 24), LQ_ERANGE, "adapters: %lld tokens outside [0, 2^24]", (long long)n);
+  LQ_REQUIRE(n == 0 || (plan && aligned16(plan)), LQ_EINVAL, "adapters: the plan is NULL or not 16-byte aligned");
+  return LQ_OK;
+}
+int check_rows(const char* what, const void* p, int64_t stride, int64_t width, bool wide) {
+  LQ_REQUIRE(p && aligned16(p) && stride % 8 == 0, LQ_EALIGN, "adapters: %s must be on 16 bytes, its rows too", what);
+  LQ_REQUIRE(stride >= (wide ? width : 0), LQ_EINVAL, "adapters: rows of %s overlap", what);
+  return LQ_OK;
+}
+
+}  // namespace
+}  // namespace lq
+
+using namespace lq;
+
+extern "C" size_t lq_adapter_plan_bytes(int64_t n, int64_t L) {
+  if (n < 0 || n > (1 << 24) || L < 1 || L > kAdMaxAdapters) return 0;
+  return 4 * (size_t)ad_plan_ints(n, L);
+}
+
+extern "C" int lq_adapter_plan(const void* ids, int ids_dtype, int64_t n_ids, int64_t seq_len, const int32_t* counts,
+                               int64_t L, void* plan, void* stream) {
+  LQ_REQUIRE(ids_dtype == LQ_I32 || ids_dtype == LQ_I64, LQ_EDTYPE, "adapters: ids must be int32 or int64");
+  LQ_REQUIRE(L >= 1 && L <= kAdMaxAdapters, LQ_ERANGE, "adapters: %lld adapters outside [1, %d]", (long long)L, kAdMaxAdapters);
+  LQ_REQUIRE(n_ids >= 0 && n_ids <= (1 << 24) && seq_len >= 0 && seq_len <= (1 << 24) && n_ids * seq_len <= (1 << 24),
+             LQ_ERANGE, "adapters: tokens outside [0, 2^24]");
+  const int64_t n = n_ids * seq_len;
+  LQ_REQUIRE(n == 0 || (ids && plan && aligned16(plan)), LQ_EINVAL, "adapters: NULL ids, or a plan not on 16 bytes");
+  if (n == 0) return LQ_OK;
+  const AdPlan p = ad_plan(plan, n, L);
+  const size_t smem = 4 * (size_t)(L + 1);
+  cudaStream_t st = as_stream(stream);
+  if (ids_dtype == LQ_I32)
+    ad_plan_kernel<int32_t><<<(unsigned)L + 1, kPlanThreads, smem, st>>>(static_cast<const int32_t*>(ids), counts, seq_len, (int)n, (int)L, p);
+  else
+    ad_plan_kernel<int64_t><<<(unsigned)L + 1, kPlanThreads, smem, st>>>(static_cast<const int64_t*>(ids), counts, seq_len, (int)n, (int)L, p);
+  return launched("ad_plan_kernel");
+}
+
+extern "C" int lq_adapter_forward(const lq_adapter_bank* bank, const void* plan, int64_t n, const void* x, int64_t x_stride,
+                                  const void* base, int64_t base_stride, void* out, int64_t out_stride, float* u,
+                                  void* stream) {
+  LQ_TRY(check_bank(bank, plan, n));
+  if (n == 0) return LQ_OK;
+  LQ_TRY(check_rows("x", x, x_stride, bank->K, false));
+  LQ_TRY(check_rows("out", out, out_stride, bank->N, n > 1));
+  if (base) LQ_TRY(check_rows("base", base, base_stride, bank->N, false));
+  LQ_REQUIRE(base != out || base_stride == out_stride, LQ_EINVAL, "adapters: out is base, with other rows");
+  LQ_REQUIRE(u, LQ_EINVAL, "adapters: NULL u");
+  const AdPlan p = ad_plan(const_cast<void*>(plan), n, bank->L);
+  cudaStream_t st = as_stream(stream);
+  if (bank->dtype == LQ_F16) {
+    LQ_TRY((down<__half>(*bank, p, n, x, x_stride, true, u, st)));
+    return up<__half>(*bank, p, n, u, false, base, base_stride, out, out_stride, st);
+  }
+  LQ_TRY((down<__nv_bfloat16>(*bank, p, n, x, x_stride, true, u, st)));
+  return up<__nv_bfloat16>(*bank, p, n, u, false, base, base_stride, out, out_stride, st);
+}
+
+extern "C" size_t lq_adapter_backward_workspace_bytes(const lq_adapter_bank* bank, int64_t n) {
+  if (!bank || n < 0 || n > (1 << 24)) return 0;
+  return 4 * (size_t)(n * bank->R);
+}
+
+extern "C" int lq_adapter_backward(const lq_adapter_bank* bank, const void* plan, int64_t n, const void* x, int64_t x_stride,
+                                   const void* dy, int64_t dy_stride, const float* u, void* dx, void* da, void* db,
+                                   int grad_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  LQ_TRY(check_bank(bank, plan, n));
+  LQ_REQUIRE(grad_dtype == LQ_F32 || grad_dtype == bank->dtype, LQ_EDTYPE, "adapters: gradients in fp32 or the bank's type");
+  cudaStream_t st = as_stream(stream);
+  if (n == 0) {
+    const size_t size = bank->L * bank->R * (grad_dtype == LQ_F32 ? 4 : 2);
+    LQ_REQUIRE(!da || cudaMemsetAsync(da, 0, size * bank->K, st) == cudaSuccess, LQ_ECUDA, "adapters: memset failed");
+    LQ_REQUIRE(!db || cudaMemsetAsync(db, 0, size * bank->N, st) == cudaSuccess, LQ_ECUDA, "adapters: memset failed");
+    return LQ_OK;
+  }
+  LQ_TRY(check_rows("dy", dy, dy_stride, bank->N, false));
+  if (da) LQ_TRY(check_rows("x", x, x_stride, bank->K, false));
+  LQ_REQUIRE(!dx || aligned16(dx), LQ_EALIGN, "adapters: dx must be 16-byte aligned");
+  LQ_REQUIRE(!db || u, LQ_EINVAL, "adapters: NULL u");
+  const size_t need = lq_adapter_backward_workspace_bytes(bank, n);
+  LQ_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need, LQ_EINVAL, "adapters: %zu bytes of workspace needed", need);
+  const AdPlan p = ad_plan(const_cast<void*>(plan), n, bank->L);
+  float* v = static_cast<float*>(workspace);
+  const bool half = bank->dtype == LQ_F16;
+  using H = __half;
+  using B = __nv_bfloat16;
+  if (dx || da) {
+    LQ_TRY((half ? down<H>(*bank, p, n, dy, dy_stride, false, v, st) : down<B>(*bank, p, n, dy, dy_stride, false, v, st)));
+  }
+  if (db) LQ_TRY((half ? outer<H>(*bank, p, u, dy, dy_stride, false, db, grad_dtype, st) : outer<B>(*bank, p, u, dy, dy_stride, false, db, grad_dtype, st)));
+  if (da) LQ_TRY((half ? outer<H>(*bank, p, v, x, x_stride, true, da, grad_dtype, st) : outer<B>(*bank, p, v, x, x_stride, true, da, grad_dtype, st)));
+  if (dx) LQ_TRY((half ? up<H>(*bank, p, n, v, true, nullptr, 0, dx, bank->K, st) : up<B>(*bank, p, n, v, true, nullptr, 0, dx, bank->K, st)));
+  return LQ_OK;
+}

@@ -21,6 +21,8 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _C
+from .adapters import AdapterBank, AdapterBatch
+from .grad_clip import clip_grad_norm_
 
 # 16-level NormalFloat table (qlora.py:43-59), float32.
 NF4_TABLE = torch.tensor([
@@ -276,12 +278,16 @@ class QLoRALinear(nn.Module):
                     out.data_ptr(), _C.stream_ptr(codes))
         return out
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
-        """qlora.py:306-312.  fp16 / bf16 activations of the base weight's dtype
+    def forward(self, x: torch.Tensor, adapters: Optional[AdapterBank] = None,
+                batch: Optional[AdapterBatch] = None) -> torch.Tensor:
+        """qlora.py:306-312.  With ``adapters`` and ``batch`` each token of x (fp16
+        or bf16) uses its own adapter of that bank in place of this layer's.  fp16 / bf16 activations of the base weight's dtype
         take the fused NF4 kernel for the base product (the reference fails
         there: its bias and LoRA factors stay fp32), with the LoRA path in the
         activations' dtype; other inputs follow the reference exactly."""
         from . import nf4_linear
+        if adapters is not None or batch is not None:
+            return self._forward_adapters(x, adapters, batch)
         if nf4_linear.eligible(self, x):
             if nf4_linear.lora_fusable(self, x):
                 # base product, bias and the rank-r LoRA term in one kernel
@@ -293,6 +299,26 @@ class QLoRALinear(nn.Module):
         out = F.linear(x, w_base, self.bias)
         out = out + F.linear(F.linear(x, self.lora_A), self.lora_B) * self.scaling
         return out
+
+    def _forward_adapters(self, x: torch.Tensor, adapters: Optional[AdapterBank],
+                          batch: Optional[AdapterBatch]) -> torch.Tensor:
+        """The base product plus each token's adapter."""
+        from . import nf4_linear
+        if adapters is None or batch is None:
+            raise ValueError("QLoRALinear.forward: adapters and batch go together")
+        if (adapters.in_features, adapters.out_features) != (self.in_features, self.out_features):
+            raise ValueError(f"QLoRALinear.forward: adapters of {adapters.in_features} to {adapters.out_features} features "
+                             f"beside {self.in_features} to {self.out_features}")
+        adapters._check(x, batch, None)
+        if nf4_linear.eligible(self, x):
+            base = nf4_linear.base_linear(self, x)
+        else:
+            bias = None if self.bias is None else self.bias.to(x.dtype)
+            base = F.linear(x, self._dequantize_base().to(x.dtype), bias)
+        if torch.is_grad_enabled() and (base.requires_grad or x.requires_grad or adapters.lora_A.requires_grad
+                                        or adapters.lora_B.requires_grad):
+            return adapters(x, batch, base)
+        return adapters.add_(base, x, batch)
 
     def merge_lora(self) -> torch.Tensor:
         """W_eff = W_base + scaling * B @ A (qlora.py:314-317): one kernel that
@@ -346,3 +372,8 @@ class QLoRA:
     def trainable_params(self, module: nn.Module) -> list[nn.Parameter]:
         """Only the trainable (LoRA) parameters."""
         return [p for p in module.parameters() if p.requires_grad]
+
+    def clip_gradients(self, module: nn.Module, max_norm: float) -> torch.Tensor:
+        """Clip the gradients of the trainable parameters to ``max_norm``
+        together, and return their norm before it (``clip_grad_norm_``)."""
+        return clip_grad_norm_(self.trainable_params(module), max_norm)

@@ -1,0 +1,112 @@
+"""CPU-side checks of the adapter bank and of gradient clipping: what the classes
+and the C entry points refuse before any launch (no GPU needed)."""
+
+import ctypes
+
+import pytest
+import torch
+
+import llm_quant_b200 as L
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from llm_quant_b200 import _C, build
+    build.build()
+    return _C.lib()
+
+
+def _bank(**kw):
+    """A bank whose pointers are aligned but lead nowhere: no call that is refused may follow them."""
+    from llm_quant_b200 import _C
+    f = dict(a=4096, b=4096, scaling=4096, L=4, R=16, K=64, N=128, dtype=2)
+    f.update(kw)
+    return ctypes.byref(_C.AdapterBank(*[f[n] for n, _ in _C.AdapterBank._fields_]))
+
+
+BAD = [({"a": None}, -1, "NULL"), ({"scaling": None}, -1, "NULL"), ({"dtype": 0}, -2, "fp16 or bf16"), ({"L": 0}, -6, "adapters"),
+       ({"L": 8193}, -6, "adapters"), ({"R": 0}, -6, "rank"), ({"R": 129}, -6, "rank"), ({"K": 68}, -5, "multiples of 8"),
+       ({"N": 4}, -6, "features"), ({"N": (1 << 22) + 8}, -6, "features"), ({"a": 4104}, -5, "aligned")]
+
+
+@pytest.mark.parametrize("kw,status,word", BAD)
+def test_bad_banks(lib, kw, status, word):
+    b = _bank(**kw)
+    for call in (lambda: lib.lq_adapter_forward(b, 4096, 4, 4096, 128, None, 0, 4096, 128, 4096, None),
+                 lambda: lib.lq_adapter_backward(b, 4096, 4, 4096, 128, 4096, 128, 4096, 4096, 4096, 4096, 2, 4096, 1 << 40, None)):
+        assert call() == status
+        assert word.encode() in lib.lq_last_error()
+
+
+def test_bad_calls(lib):
+    def forward(bank=None, plan=4096, n=4, x=4096, xs=64, base=None, bs=0, out=4096, os=128, u=4096):
+        return lib.lq_adapter_forward(bank or _bank(), plan, n, x, xs, base, bs, out, os, u, None)
+
+    assert forward(plan=None) == -1 and forward(plan=4104) == -1 and forward(n=-1) == -6 and forward(n=(1 << 24) + 1) == -6
+    assert forward(x=None) == -5 and forward(x=4098) == -5 and forward(xs=68) == -5 and forward(xs=-64) == -1
+    assert forward(out=None) == -5 and forward(os=64) == -1 and forward(base=4104) == -5
+    assert forward(base=4096, bs=136) == -1 and forward(u=None) == -1
+    assert forward(n=0, plan=None, x=None, out=None, u=None) == 0
+
+    def backward(x=4096, dy=4096, ds=128, u=4096, dx=4096, da=4096, db=4096, dt=2, ws=4096, nb=1 << 40):
+        return lib.lq_adapter_backward(_bank(), 4096, 4, x, 64, dy, ds, u, dx, da, db, dt, ws, nb, None)
+
+    assert backward(dt=1) == -2 and backward(dy=None) == -5 and backward(ds=100) == -5 and backward(u=None) == -1
+    assert backward(x=None) == -5 and backward(dx=4104) == -5 and backward(ws=None) == -1 and backward(nb=8) == -1
+    assert lib.lq_adapter_backward_workspace_bytes(None, 4) == 0 and lib.lq_adapter_backward_workspace_bytes(_bank(), -1) == 0
+
+
+def test_bad_plans(lib):
+    def plan(ids=4096, dt=5, n=4, seq=1, counts=None, num=4, p=4096):
+        return lib.lq_adapter_plan(ids, dt, n, seq, counts, num, p, None)
+
+    assert plan(dt=4) == -2 and plan(num=0) == -6 and plan(num=8193) == -6 and plan(n=-1) == -6 and plan(seq=1 << 23) == -6
+    assert plan(ids=None) == -1 and plan(p=None) == -1 and plan(p=4100) == -1 and plan(n=0, ids=None, p=None) == 0
+    assert lib.lq_adapter_plan_bytes(-1, 4) == 0 and lib.lq_adapter_plan_bytes(4, 0) == 0
+    assert lib.lq_adapter_plan_bytes(1000, 4) >= 4 * (2000 + 12 + 4 * 12)
+
+
+def test_bad_clips(lib):
+    V, I64, I = ctypes.c_void_p * 2, ctypes.c_int64 * 2, ctypes.c_int * 2
+
+    def clip(ptrs=(4096, 8192), out=None, n=(8, 8), dt=(0, 0), count=2, m=1.0, norm=4096, ws=4096, nb=1 << 40):
+        return lib.lq_clip_grad_norm(V(*ptrs), None if out is None else V(*out), I64(*n), I(*dt), count, m, norm, ws, nb, None)
+
+    assert clip(ptrs=(4096, None)) == -1 and clip(ptrs=(4098, 4096)) == -5 and clip(out=(4096, 4098)) == -5
+    assert clip(n=(8, -1)) == -1 and clip(dt=(0, 3)) == -2 and clip(count=-1) == -1 and clip(m=-1.0) == -1
+    assert clip(m=float("nan")) == -1 and clip(norm=None) == -1 and clip(ws=None) == -1 and clip(nb=8) == -1 and clip(ws=4100) == -1
+    assert lib.lq_clip_workspace_bytes(-1) == 0
+
+
+def test_refusals_without_a_device():
+    for kw, word in (({"in_features": 65}, "in_features"), ({"out_features": 0}, "out_features"), ({"rank": 0}, "rank"),
+                     ({"rank": 129}, "rank"), ({"num_adapters": 0}, "num_adapters"), ({"num_adapters": 8193}, "num_adapters")):
+        args = dict(in_features=64, out_features=128, num_adapters=2, rank=8)
+        args.update(kw)
+        with pytest.raises(ValueError, match=word):
+            L.AdapterBank(**args)
+    with pytest.raises(TypeError):
+        L.AdapterBank(64, 64, 2, dtype=torch.float64)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        L.AdapterBatch(torch.zeros(3, dtype=torch.int32), 2)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        L.GradClipper([torch.zeros(3)])
+    with pytest.raises(ValueError, match="no layers"):
+        L.AdapterBank.from_layers([])
+    assert L.clip_grad_norm_([torch.nn.Parameter(torch.zeros(3))], 1.0) == 0
+
+
+def test_a_bank_of_layers():
+    """Smaller ranks are filled up with zeros, lora_B is transposed."""
+    layers = [L.QLoRALinear(64, 128, rank=r, alpha=2.0) for r in (4, 8)]
+    for ql in layers:
+        torch.nn.init.normal_(ql.lora_B)
+    bank = L.AdapterBank.from_layers(layers, dtype=torch.float32)
+    assert bank.rank == 8 and bank.scaling.tolist() == [0.5, 0.25]
+    for i, ql in enumerate(layers):
+        assert torch.equal(bank.lora_A[i, :ql.rank], ql.lora_A) and torch.equal(bank.lora_B[i, :ql.rank], ql.lora_B.t())
+        assert not bank.lora_A[i, ql.rank:].any() and not bank.lora_B[i, ql.rank:].any()
+    with pytest.raises(IndexError):
+        bank.load_adapter(2, layers[0].lora_A, layers[0].lora_B, 1.0)
+    with pytest.raises(ValueError):
+        bank.load_adapter(0, layers[0].lora_A, layers[1].lora_B, 1.0)

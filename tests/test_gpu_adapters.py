@@ -1,0 +1,472 @@
+"""GPU tests of AdapterBank and AdapterBatch against the definition in 64 bits.
+
+Tolerances.  y is rounded once (half a step of its type), u = scaling * A x is a
+sum of K exact products in fp32, y a sum of R products more.  A sum of n terms
+is off by n steps of 2^-23 of the sum of their magnitudes at most (tensor cores
+cut instead of rounding), and a value of u that meets a 16-bit factor as two
+16-bit parts is off by 2^-16 of itself (bf16; half a step of half a step).  So
+with |Y| = |base| + sum_r |B_r| s sum_k |A_rk x_k|:
+
+    |y - exact| <= eps / 2 |exact| + ((K + R + 16) 2^-23 + 2^-16) |Y|
+
+and the gradients likewise, with the terms that their sums have."""
+
+import pytest
+import torch
+
+import llm_quant_b200 as L
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+def owners(ids, n, seq, num, counts=None):
+    own = ids.long().cpu().repeat_interleave(seq)
+    own[(own < 0) | (own >= num)] = -1
+    if counts is not None:
+        pos = torch.arange(n * seq) % max(seq, 1)
+        own[pos >= counts.cpu().repeat_interleave(seq)] = -1
+    return own
+
+
+def reference(x, base, a, b, s, own, dy=None):
+    """y and, with dy, dx, da, db in 64 bits, each with the sum of its terms' magnitudes."""
+    x, a, b, s = x.double(), a.double(), b.double(), s.double()
+    y = torch.zeros(x.shape[0], b.shape[2], dtype=torch.float64, device=x.device) if base is None else base.double().clone()
+    ya = y.abs()
+    out = [(y, ya)]
+    if dy is not None:
+        dy = dy.double()
+        out += [(torch.zeros_like(t), torch.zeros_like(t)) for t in (x, a, b)]
+    for i in range(a.shape[0]):
+        rows = (own == i).nonzero().flatten().to(x.device)
+        if not len(rows):
+            continue
+        xi = x[rows]
+        u, ua = s[i] * xi @ a[i].T, s[i].abs() * xi.abs() @ a[i].abs().T
+        y[rows] += u @ b[i]
+        ya[rows] += ua @ b[i].abs()
+        if dy is not None:
+            d = dy[rows]
+            v, va = s[i] * d @ b[i].T, s[i].abs() * d.abs() @ b[i].abs().T
+            for (t, m), p, q in ((out[1], v @ a[i], va @ a[i].abs()),):
+                t[rows], m[rows] = p, q
+            out[2][0][i], out[2][1][i] = v.T @ xi, va.T @ xi.abs()
+            out[3][0][i], out[3][1][i] = u.T @ d, ua.T @ d.abs()
+    return out
+
+
+def close(got, want, terms):
+    want, mag = want
+    eps = torch.finfo(got.dtype).eps
+    tiny = 2.0 ** -25 if got.dtype == torch.float16 else 2.0 ** -133
+    tol = eps / 2 * want.abs() + ((terms + 16) * 2.0 ** -23 + 2.0 ** -16) * mag + tiny
+    err = (got.double() - want).abs()
+    assert got.shape == want.shape
+    assert bool((err <= tol).all()), f"worst {float((err / tol.clamp(min=1e-300)).max())} of the tolerance"
+
+
+def make(n, seq, num, R, K, N, dt, seed=0, base=True, scale=1.0):
+    g = torch.Generator(DEV).manual_seed(seed)
+
+    def rand(*shape, scale=1.0):
+        return (torch.randn(shape, generator=g, device=DEV) * scale).to(dt)
+
+    bank = L.AdapterBank(K, N, num, R, dtype=dt, device=DEV).requires_grad_(False)
+    bank.lora_A.copy_(rand(num, R, K, scale=K ** -0.5))
+    bank.lora_B.copy_(rand(num, R, N, scale=0.1))
+    bank.scaling.copy_(torch.rand(num, generator=g, device=DEV) * 2 - 0.5)
+    x = rand(n * seq, K, scale=scale)
+    return bank, x, rand(n * seq, N) if base else None, rand(n * seq, N, scale=0.1)
+
+
+# requests, tokens of each, adapters, rank, in, out
+SHAPES = [
+    (1, 1, 1, 1, 8, 8), (1, 1, 8, 16, 4096, 4096), (2, 1, 3, 16, 64, 128), (7, 1, 4, 4, 200, 72), (16, 1, 16, 64, 1032, 520),
+    (33, 1, 5, 8, 264, 1288), (64, 1, 2, 24, 512, 256), (100, 1, 64, 33, 136, 2056), (200, 1, 7, 128, 256, 264),
+    (1, 127, 2, 16, 128, 128), (1, 128, 1, 16, 256, 384), (1, 129, 3, 8, 72, 520), (3, 100, 2, 32, 1032, 248),
+    (4, 333, 3, 64, 512, 1024), (2, 700, 1, 17, 264, 136), (5, 1, 8192, 2, 64, 64), (300, 3, 40, 16, 128, 1032),
+    (1, 2500, 2, 128, 192, 320), (6, 513, 4, 12, 2056, 1160), (20, 260, 2, 16, 320, 256),
+]
+
+
+def some_ids(n, num, seed, none):
+    g = torch.Generator().manual_seed(seed)
+    lo = -1 if none else 0
+    return torch.randint(lo, num, (n,), generator=g).to(torch.int32).to(DEV)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_forward(shape, dt):
+    n, seq, num, R, K, N = shape
+    bank, x, base, _ = make(n, seq, num, R, K, N, TYPES[dt])
+    ids = some_ids(n, num, n + seq, n % 2)
+    counts = torch.randint(0, seq + 1, (n,), dtype=torch.int32, generator=torch.Generator().manual_seed(5)).to(DEV) if seq > 2 else None
+    batch = L.AdapterBatch(ids, num, seq, counts)
+    own = owners(ids, n, seq, num, counts)
+    for b in (base, None):
+        y = bank(x, batch, b)
+        close(y, reference(x, b, bank.lora_A, bank.lora_B, bank.scaling, own)[0], K + R)
+        bare = (own < 0).to(DEV)
+        assert torch.equal(y[bare], (b if b is not None else torch.zeros_like(y))[bare])
+    kept = base.clone()
+    assert torch.equal(bank.add_(kept, x, batch), bank(x, batch, base))
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_backward(shape, dt):
+    n, seq, num, R, K, N = shape
+    bank, x, base, dy = make(n, seq, num, R, K, N, TYPES[dt], seed=1)
+    bank.requires_grad_(True)
+    ids = some_ids(n, num, n, n % 3 == 0)
+    counts = torch.randint(0, seq + 1, (n,), dtype=torch.int32, generator=torch.Generator().manual_seed(6)).to(DEV) if seq > 2 else None
+    batch = L.AdapterBatch(ids.long(), num, seq, counts)
+    own = owners(ids, n, seq, num, counts)
+    x.requires_grad_(True)
+    base.requires_grad_(True)
+    y = bank(x, batch, base)
+    dx, da, db, dbase = torch.autograd.grad(y, (x, bank.lora_A, bank.lora_B, base), dy)
+    with torch.no_grad():
+        ry, rx, ra, rb = reference(x, base, bank.lora_A, bank.lora_B, bank.scaling, own, dy)
+    most = max(int((own == i).sum()) for i in range(num))
+    close(y.detach(), ry, K + R)
+    close(dx, rx, N + R)
+    close(da, ra, N + most)
+    close(db, rb, K + most)
+    assert torch.equal(dbase, dy)
+    # equal calls, equal bits
+    again = torch.autograd.grad(bank(x, batch, base), (x, bank.lora_A, bank.lora_B), dy)
+    for p, q in zip((dx, da, db), again):
+        assert torch.equal(p, q)
+
+
+def test_gradients_against_differences():
+    """y is linear in x, in A and in B: a difference over any step is the
+    derivative, up to the rounding of the two outputs."""
+    dt = torch.float16
+    bank, x, base, dy = make(5, 40, 3, 16, 256, 128, dt, seed=3)
+    batch = L.AdapterBatch(some_ids(5, 3, 1, True), 3, 40)
+    bank.requires_grad_(True)
+    x.requires_grad_(True)
+    grads = torch.autograd.grad(bank(x, batch), (x, bank.lora_A, bank.lora_B), dy)
+    g = torch.Generator(DEV).manual_seed(9)
+    for t, grad in zip((x, bank.lora_A, bank.lora_B), grads):
+        step = torch.randn(t.shape, generator=g, device=DEV)
+        with torch.no_grad():
+            kept = t.detach().clone()
+            sides = []
+            moved = []
+            for sign in (1, -1):
+                t.copy_((kept.float() + sign * 0.5 * step * kept.float().std()).to(dt))
+                moved.append(t.detach().double().clone())
+                sides.append(bank(x, batch).double())
+            t.copy_(kept)
+        want = ((sides[0] - sides[1]) * dy.double()).sum()
+        d = moved[0] - moved[1]
+        got = (grad.double() * d).sum()
+        half = torch.finfo(dt).eps / 2
+        # each output and each gradient is off by half a step, and by the sums' share, which is below another half
+        tol = 2 * half * (((sides[0].abs() + sides[1].abs()) * dy.double().abs()).sum() + (grad.double().abs() * d.abs()).sum())
+        assert abs(float(want - got)) <= float(tol)
+
+
+def test_fp32_parameters():
+    """fp32 parameters are rounded to the activations' type; their gradients come in fp32."""
+    dt = torch.bfloat16
+    bank, x, base, dy = make(3, 50, 2, 8, 136, 264, dt, seed=4)
+    bank = bank.float().requires_grad_(True)
+    with torch.no_grad():
+        bank.lora_A.add_(torch.randn_like(bank.lora_A) * 1e-4)
+    ids = torch.tensor([0, 1, 0], device=DEV)
+    batch = L.AdapterBatch(ids, 2, 50)
+    y = bank(x, batch, base)
+    da, db = torch.autograd.grad(y, (bank.lora_A, bank.lora_B), dy)
+    assert da.dtype == db.dtype == torch.float32
+    a, b = bank.lora_A.detach().to(dt), bank.lora_B.detach().to(dt)
+    ry, _, ra, rb = reference(x, base, a, b, bank.scaling, owners(ids, 3, 50, 2), dy)
+    close(y.detach(), ry, 136 + 8)
+    close(da, ra, 264 + 100)
+    close(db, rb, 136 + 100)
+
+
+def test_subsets_of_gradients():
+    bank, x, base, dy = make(4, 33, 2, 16, 128, 256, torch.bfloat16, seed=6)
+    batch = L.AdapterBatch(some_ids(4, 2, 2, False), 2, 33)
+    bank.requires_grad_(True)
+    x.requires_grad_(True)
+    whole = torch.autograd.grad(bank(x, batch, base), (x, bank.lora_A, bank.lora_B), dy)
+    leaves = (x, bank.lora_A, bank.lora_B)
+    for i, t in enumerate(leaves):
+        for o in leaves:
+            o.requires_grad_(o is t)
+        got, = torch.autograd.grad(bank(x, batch, base), (t,), dy)
+        assert torch.equal(got, whole[i])
+
+
+def test_nothing_but_zeros_and_padding():
+    """Adapters without tokens get zeros; a batch without adapters passes base on; padding may hold anything."""
+    for dt in TYPES.values():
+        bank, x, base, dy = make(3, 70, 4, 16, 128, 136, dt, seed=7)
+        bank.requires_grad_(True)
+        ids = torch.tensor([1, 3, 1], dtype=torch.int32, device=DEV)
+        counts = torch.tensor([70, 0, 31], dtype=torch.int32, device=DEV)
+        clean = bank(x, L.AdapterBatch(ids, 4, 70, counts), base)
+        want = torch.autograd.grad(clean, (bank.lora_A, bank.lora_B), dy)
+        bad, bad_dy = x.view(3, 70, -1).clone(), dy.view(3, 70, -1).clone()
+        for t in (bad, bad_dy):
+            t[1], t[2, 31:] = float("nan"), float("inf")
+        bad = bad.view_as(x).requires_grad_(True)
+        y = bank(bad, L.AdapterBatch(ids, 4, 70, counts), base)
+        assert torch.equal(y, clean)
+        dx, da, db = torch.autograd.grad(y, (bad, bank.lora_A, bank.lora_B), bad_dy.view_as(dy))
+        assert torch.equal(da, want[0]) and torch.equal(db, want[1])
+        for i in (0, 2, 3):
+            assert not da[i].any() and not db[i].any()
+        assert not dx.view(3, 70, -1)[1].any() and not dx.view(3, 70, -1)[2, 31:].any()
+        none = L.AdapterBatch(torch.full((3,), -1, dtype=torch.int32, device=DEV), 4, 70)
+        assert torch.equal(bank(x, none, base), base) and not bank(x, none).any()
+        g = torch.autograd.grad(bank(x, none, base), (bank.lora_A, bank.lora_B), dy)
+        assert not g[0].any() and not g[1].any()
+
+
+def test_infinities_stay_in_their_rows():
+    for dt in TYPES.values():
+        bank, x, base, _ = make(1, 300, 1, 16, 128, 136, dt, seed=8)
+        batch = L.AdapterBatch(torch.zeros(1, dtype=torch.int32, device=DEV), 1, 300)
+        clean = bank(x, batch, base)
+        bad = x.clone()
+        bad[7, 3], bad[200, 64], bad[201, 127] = float("inf"), float("nan"), float("-inf")
+        y = bank(bad, batch, base)
+        rows = torch.ones(300, dtype=torch.bool, device=DEV)
+        rows[[7, 200, 201]] = False
+        assert torch.equal(y[rows], clean[rows])
+        assert y[200].isnan().all() and not y[[7, 201]].isfinite().any()
+
+
+@pytest.mark.parametrize("rows", [1, 40, 900])
+def test_values_over_the_range_of_the_type(rows):
+    """u may leave fp16's range in either direction; y does not."""
+    dt = torch.float16
+    K, N, R = 256, 136, 16
+    bank, x, _, dy = make(rows, 1, 2, R, K, N, dt, seed=10)
+    ids = some_ids(rows, 2, 3, False)
+    batch = L.AdapterBatch(ids, 2)
+    own = owners(ids, rows, 1, 2)
+    for grow in (2.0 ** 12, 2.0 ** -14):
+        with torch.no_grad():
+            x2 = (x.float() * 200).to(dt) if grow > 1 else (x.float() * 2.0 ** -8).to(dt)
+            bank.lora_A.copy_((torch.randn(2, R, K, device=DEV, generator=torch.Generator(DEV).manual_seed(1)) * min(grow, 600.0)).to(dt))
+            bank.lora_B.copy_((torch.randn(2, R, N, device=DEV, generator=torch.Generator(DEV).manual_seed(2)) * (2.0 ** -13 if grow > 1 else 16.0)).to(dt))
+            bank.scaling.fill_(1.0)
+        bank.requires_grad_(True)
+        y = bank(x2, batch)
+        (ry, _, _, rb) = reference(x2, None, bank.lora_A.detach(), bank.lora_B.detach(), bank.scaling, own, dy)
+        close(y.detach(), ry, K + R)
+        small = (dy.float() * 2.0 ** -8).to(dt) if grow > 1 else dy
+        db, = torch.autograd.grad(y, (bank.lora_B,), small)
+        rb = reference(x2, None, bank.lora_A.detach(), bank.lora_B.detach(), bank.scaling, own, small)[3]
+        if float(rb[0].abs().max()) < 60000:
+            close(db, rb, K + rows)
+
+
+def test_rows_of_other_strides():
+    dt = torch.bfloat16
+    bank, x, base, dy = make(3, 30, 2, 16, 128, 256, dt, seed=11)
+    ids = some_ids(3, 2, 4, True)
+    batch = L.AdapterBatch(ids, 2, 30)
+    want = bank(x, batch, base)
+    wide = torch.zeros(90, 400, dtype=dt, device=DEV)
+    wide[:, 8:136] = x
+    assert torch.equal(bank(wide[:, 8:136], batch, base), want)          # rows on 16 bytes: read as they are
+    wide[:, 3:131] = x
+    assert torch.equal(bank(wide[:, 3:131], batch, base), want)          # off them: copied
+    assert torch.equal(bank(x.view(3, 30, 128), batch, base.view(3, 30, 256)).view(90, 256), want)
+    assert torch.equal(bank(x.t().contiguous().t(), batch, base), want)
+    y = torch.zeros(90, 264, dtype=dt, device=DEV)
+    y[:, :256] = base
+    bank.add_(y[:, :256], x, batch)
+    assert torch.equal(y[:, :256], want) and not y[:, 256:].any()
+    one = x[:1].expand(90, 128)                                          # rows that are all the same memory
+    assert torch.equal(bank(one, batch, base), bank(one.contiguous(), batch, base))
+    bank.requires_grad_(True)
+    out = bank(x.clone().requires_grad_(True), batch, base)
+    a = torch.autograd.grad(out.sum(), (bank.lora_A,), retain_graph=True)[0]  # dy is one value, expanded
+    assert torch.equal(a, torch.autograd.grad(out, (bank.lora_A,), torch.ones_like(out))[0])
+    out = bank(x, batch, base)
+    turned = torch.autograd.grad(out, (bank.lora_A,), dy.t().contiguous().t(), retain_graph=True)[0]
+    assert torch.equal(turned, torch.autograd.grad(out, (bank.lora_A,), dy)[0])
+
+
+def test_no_tokens():
+    bank = L.AdapterBank(64, 128, 3, 8, dtype=torch.bfloat16, device=DEV)
+    batch = L.AdapterBatch(torch.zeros(0, dtype=torch.int32, device=DEV), 3)
+    x = torch.zeros(0, 64, dtype=torch.bfloat16, device=DEV, requires_grad=True)
+    y = bank(x, batch)
+    assert y.shape == (0, 128)
+    dx, da, db = torch.autograd.grad(y, (x, bank.lora_A, bank.lora_B), torch.zeros_like(y))
+    assert dx.shape == (0, 64) and not da.any() and not db.any()
+    batch = L.AdapterBatch(torch.zeros(4, dtype=torch.int32, device=DEV), 3, 0)
+    assert bank(torch.zeros(4, 0, 64, dtype=torch.bfloat16, device=DEV), batch).shape == (4, 0, 128)
+
+
+def test_captured_steps_and_new_requests():
+    """A captured plan, forward and backward pass, replayed for other requests and values."""
+    dt = torch.bfloat16
+    for n, seq in ((6, 1), (5, 90)):
+        bank, x, base, dy = make(n, seq, 3, 16, 256, 136, dt, seed=12)
+        bank.requires_grad_(True)
+        ids = some_ids(n, 3, 1, True)
+        batch = L.AdapterBatch(ids, 3, seq)
+        x.requires_grad_(True)
+
+        def step():
+            batch.update(ids)
+            y = bank(x, batch, base)
+            return [y.detach(), *torch.autograd.grad(y, (x, bank.lora_A, bank.lora_B), dy)]
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = step()
+        for seed in (2, 3):
+            with torch.no_grad():
+                ids.copy_(some_ids(n, 3, seed, True))
+                x.copy_(torch.randn(x.shape, device=DEV, generator=torch.Generator(DEV).manual_seed(seed)))
+            graph.replay()
+            got = [t.clone() for t in held]
+            for p, q in zip(got, step()):
+                assert torch.equal(p, q)
+
+
+def test_two_streams():
+    """Calls of one bank on two streams at once, each with its own batch."""
+    bank, x, base, _ = make(40, 20, 4, 16, 512, 520, torch.bfloat16, seed=13)
+    batches = [L.AdapterBatch(some_ids(40, 4, s, True), 4, 20) for s in range(2)]
+    want = [bank(x, b, base) for b in batches]
+    streams = [torch.cuda.Stream() for _ in batches]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(bank(x, batches[i], base))
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        assert all(torch.equal(w, y) for y in g)
+
+
+def test_changed_plan_is_noticed():
+    bank, x, base, dy = make(3, 5, 2, 8, 64, 64, torch.bfloat16)
+    bank.requires_grad_(True)
+    ids = some_ids(3, 2, 0, False)
+    batch = L.AdapterBatch(ids, 2, 5)
+    y = bank(x, batch, base)
+    batch.update(ids)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(dy)
+
+
+def test_layers_and_their_step():
+    """QLoRALinear with a bank: serving, a training step and the clipping of its
+    gradients; a bank made of layers gives what the layers give."""
+    torch.manual_seed(0)
+    dt = torch.bfloat16
+    K, N = 256, 384
+    w = (torch.randn(N, K, device=DEV) * 0.05).to(dt)
+    layers = []
+    for r in (4, 16):
+        ql = L.QLoRALinear(K, N, rank=r, alpha=2.0 * r).to(DEV)
+        ql.pack_base(w)
+        torch.nn.init.normal_(ql.lora_B, std=0.1)
+        torch.nn.init.normal_(ql.bias, std=0.1)
+        layers.append(ql)
+    layers[1].bias = layers[0].bias
+    bank = L.AdapterBank.from_layers(layers)
+    x = torch.randn(2, 17, K, device=DEV).to(dt)
+    batch = L.AdapterBatch(torch.tensor([1, 0], device=DEV), 2, 17)
+    with torch.no_grad():
+        y = layers[0](x, bank, batch)
+        wf = layers[0]._dequantize_base().double()
+        for i, owner in enumerate((1, 0)):
+            ql = layers[owner]
+            u = x[i].double() @ ql.lora_A.to(dt).double().T * ql.scaling
+            low = u @ ql.lora_B.to(dt).double().T
+            shared = x[i].double() @ wf.T + ql.bias.double()
+            # the base product is rounded before the adapter is added: two roundings
+            tol = 2.0 ** -8 * (shared.abs() + (shared + low).abs()) \
+                + (K + 32) * 2.0 ** -23 * (x[i].double().abs() @ wf.abs().T + ql.bias.abs().double()) \
+                + ((K + 32) * 2.0 ** -23 + 2.0 ** -16) * (2 * x[i].double().abs() @ ql.lora_A.to(dt).double().abs().T
+                                                         @ ql.lora_B.to(dt).double().abs().T)
+            assert bool(((y[i].double() - shared - low).abs() <= tol).all())
+    ql = layers[0]
+    ql.requires_grad_(False)
+    before = ql(x)
+    opt = torch.optim.SGD(bank.parameters(), lr=1e-2)
+    out = ql(x, bank, batch)
+    out.float().square().mean().backward()
+    pipeline = L.QLoRA()
+    grads = [p.grad.double().clone() for p in pipeline.trainable_params(bank)]
+    norm = pipeline.clip_gradients(bank, 1e-3)
+    want = torch.stack([g.square().sum() for g in grads]).sum().sqrt()
+    assert abs(float(norm) - float(want)) <= 2.0 ** -23 * float(want)
+    for p, g in zip(bank.parameters(), grads):
+        assert bool(((p.grad.double() - g * (1e-3 / (want + 1e-6))).abs() <= 2.0 ** -8 * 1.001 * g.abs() * (1e-3 / want) + 1e-40).all())
+    opt.step()
+    assert torch.equal(ql(x), before)  # the layer's own adapter and base are as they were
+
+
+def test_refusals_on_the_device():
+    bank = L.AdapterBank(64, 128, 3, 8, dtype=torch.bfloat16, device=DEV)
+    ids = torch.zeros(4, dtype=torch.int32, device=DEV)
+    batch = L.AdapterBatch(ids, 3)
+    x = torch.zeros(4, 64, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(TypeError, match="float32"):
+        bank(x.float(), batch)
+    with pytest.raises(RuntimeError, match="tokens"):
+        bank(x[:3], batch)
+    with pytest.raises(RuntimeError, match="features"):
+        bank(torch.zeros(4, 72, dtype=torch.bfloat16, device=DEV), batch)
+    with pytest.raises(RuntimeError, match="base"):
+        bank(x, batch, torch.zeros(4, 64, dtype=torch.bfloat16, device=DEV))
+    with pytest.raises(ValueError, match="adapters"):
+        bank(x, L.AdapterBatch(ids, 2))
+    with pytest.raises(RuntimeError, match="no gradient"):
+        bank.add_(torch.zeros(4, 128, dtype=torch.bfloat16, device=DEV), x, batch)
+    with torch.no_grad(), pytest.raises(ValueError, match="16 bytes"):
+        bank.add_(torch.zeros(4, 130, dtype=torch.bfloat16, device=DEV)[:, 1:129], x, batch)
+    with torch.no_grad(), pytest.raises(ValueError, match="16 bytes"):
+        bank.add_(torch.zeros(1, 128, dtype=torch.bfloat16, device=DEV).expand(4, 128), x, batch)
+    with pytest.raises(TypeError, match="int32 or int64"):
+        L.AdapterBatch(ids.float(), 3)
+    with pytest.raises(ValueError, match="counts"):
+        L.AdapterBatch(ids, 3, 2, ids.long())
+    with pytest.raises(ValueError, match="counts"):
+        L.AdapterBatch(ids, 3, 2, ids[:3])
+    with pytest.raises(ValueError, match="num_adapters"):
+        L.AdapterBatch(ids, 0)
+    with pytest.raises(ValueError, match="expected 4"):
+        batch.update(ids[:2])
+    with pytest.raises(RuntimeError, match="CUDA"):
+        L.AdapterBatch(ids.cpu(), 3)
+    ql = L.QLoRALinear(64, 64).to(DEV)
+    with pytest.raises(ValueError, match="together"):
+        ql(x, bank)
+    with pytest.raises(ValueError, match="beside"):
+        ql(x, bank, batch)
+
+
+def test_inference_mode():
+    bank, x, base, _ = make(4, 1, 2, 8, 64, 64, torch.bfloat16)
+    with torch.inference_mode():
+        batch = L.AdapterBatch(torch.zeros(4, dtype=torch.int32, device=DEV), 2)
+        y = base.clone()
+        batch.update(torch.zeros(4, dtype=torch.int32, device=DEV))
+        assert torch.equal(bank.add_(y, x, batch), bank(x, batch, base))
