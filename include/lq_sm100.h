@@ -484,20 +484,22 @@ typedef struct {
 /* Which tokens use which adapter, for n = n_ids * seq_len tokens: token t uses
  * ids[t / seq_len] (int32 or int64; outside [0, L): none), or none where t %
  * seq_len >= counts[t / seq_len] (counts may be NULL).  plan: 16-byte aligned,
- * of lq_adapter_plan_bytes; read by the calls below until it is built again. */
+ * of lq_adapter_plan_bytes; read by the calls below until it is built again.
+ * Its first word is an lq_status: LQ_ETIMEOUT if a wait on the device ran out in
+ * one of them, whose results are then incomplete. */
 size_t lq_adapter_plan_bytes(int64_t n, int64_t L);
 int lq_adapter_plan(const void* ids, int ids_dtype, int64_t n_ids, int64_t seq_len, const int32_t* counts,
                     int64_t L, void* plan, void* stream);
 /* out [n, N] = base [n, N] (NULL: 0; may be out itself) + the adapters' share of
  * x [n, K].  Strides are of rows, in elements, multiples of 8, as the addresses
  * are of 16 bytes.  u [n, R] fp32: scaling * A x of the tokens with an adapter. */
-int lq_adapter_forward(const lq_adapter_bank* host_bank, const void* plan, int64_t n, const void* x, int64_t x_stride,
+int lq_adapter_forward(const lq_adapter_bank* host_bank, void* plan, int64_t n, const void* x, int64_t x_stride,
                        const void* base, int64_t base_stride, void* out, int64_t out_stride, float* u, void* stream);
 /* Gradients for dy [n, N], the gradient of out (base's is dy itself): dx [n, K],
  * da [L, R, K], db [L, R, N] in grad_dtype (LQ_F32 or the bank's), all
  * contiguous; a NULL one is not computed.  u is what the forward call left. */
 size_t lq_adapter_backward_workspace_bytes(const lq_adapter_bank* host_bank, int64_t n);
-int lq_adapter_backward(const lq_adapter_bank* host_bank, const void* plan, int64_t n, const void* x, int64_t x_stride,
+int lq_adapter_backward(const lq_adapter_bank* host_bank, void* plan, int64_t n, const void* x, int64_t x_stride,
                         const void* dy, int64_t dy_stride, const float* u, void* dx, void* da, void* db,
                         int grad_dtype, void* workspace, size_t workspace_bytes, void* stream);
 

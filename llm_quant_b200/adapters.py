@@ -101,6 +101,14 @@ class AdapterBatch:
         _call(self.device, "lq_adapter_plan", ids.data_ptr(), _C.dt(ids), self.requests, self.seq_len, _C.ptr(counts),
               self.num_adapters, self._plan.data_ptr())
 
+    def check(self) -> None:
+        """Wait for the batch's work and raise LQError if a kernel gave up a
+        wait on the device since the last ``update`` (its results are
+        incomplete then)."""
+        status = int(self._plan[:4].view(torch.int32)) if self.tokens else _C.OK
+        if status:
+            raise _C.LQError("AdapterBatch", status, "a wait on the device ran out")
+
 
 def _rows(x: torch.Tensor, width: int):
     """x as rows of `width` values that the kernels can read, and their stride:
@@ -213,7 +221,7 @@ class AdapterBank(nn.Module):
         x2, xs = _rows(x, self.in_features)
         b2, bs = (None, 0) if base is None else _rows(base, self.out_features)
         y, ys = (x.new_empty(x.shape[:-1] + (self.out_features,)), self.out_features) if out is None else (out, out.stride(0))
-        u = torch.empty(n, self.rank, dtype=torch.float32, device=dev)
+        u = torch.empty(n, (self.rank + 7) // 8 * 8, dtype=torch.float32, device=dev)
         a, b = self._weights(x.dtype)
         if n:
             _call(dev, "lq_adapter_forward", self._struct(a, b, self.scaling), batch._plan.data_ptr(), n, x2.data_ptr(), xs,

@@ -5,6 +5,9 @@
 // products: rows times a factor (u = s A x, v = s B dy), a low-rank row times a
 // factor (y = B^T u, dx = A^T v) and sums of outer products over an adapter's
 // tokens (dA = v x^T, dB = u dy^T).  u and v are kept in fp32.
+//
+// This file: the plan and the entry points; the products are in
+// lq_adapters_mm.cu.
 #include "lq_adapters.cuh"
 
 namespace lq {
@@ -59,7 +62,7 @@ __global__ void __launch_bounds__(kPlanThreads) ad_plan_kernel(const I* __restri
   const int first = base[0], tile = base[1], n = hist[me], n_tiles = (n + kAdTile - 1) / kAdTile;
   if (tid == 0) {
     p.start[me] = first, p.tile_of[me] = tile;
-    if (me == L) p.start[L + 1] = first + n, p.tile_of[L + 1] = tile + n_tiles;
+    if (me == L) p.start[L + 1] = first + n, p.tile_of[L + 1] = tile + n_tiles, *p.status = LQ_OK;
   }
   int at = first;
   for (int t0 = 0; t0 < T && at < first + n; t0 += kPlanThreads) {
@@ -89,109 +92,6 @@ __global__ void __launch_bounds__(kPlanThreads) ad_plan_kernel(const I* __restri
   }
 }
 
-// ---------------------------------------------------------------------------
-// A block to a token: u[t][r] = s sum_k f[r][k] x[t][k], a warp to a rank row.
-// ---------------------------------------------------------------------------
-template <typename T>
-__global__ void __launch_bounds__(256) ad_down_kernel(const T* __restrict__ x, int64_t stride, const T* __restrict__ f,
-                                                      const float* __restrict__ scaling, int R, int K,
-                                                      const int* __restrict__ owner, float* __restrict__ u) {
-  const int64_t t = blockIdx.x;
-  const int o = owner[t];
-  if (o < 0) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int r = warp; r < R; r += 8) {
-    const T* row = f + ((int64_t)o * R + r) * K;
-    float s = 0.0f;
-    for (int k = lane * 8; k < K; k += 256) {
-      Vec16<T> a, b;
-      a.u = *reinterpret_cast<const uint4*>(row + k);
-      b.u = *reinterpret_cast<const uint4*>(x + t * stride + k);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s = fmaf(Ty<T>::to_f(a.v[i]), Ty<T>::to_f(b.v[i]), s);
-    }
-#pragma unroll
-    for (int m = 16; m; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
-    if (lane == 0) u[t * R + r] = s * scaling[o];
-  }
-}
-
-// A block to a token and 2048 columns: out[t][c] = base[t][c] + sum_r u[t][r] f[r][c].
-template <typename T>
-__global__ void __launch_bounds__(256) ad_up_kernel(const float* __restrict__ u, const T* __restrict__ f, int R, int N,
-                                                    const int* __restrict__ owner, const T* base, int64_t base_stride,
-                                                    T* out, int64_t out_stride) {
-  const int64_t t = blockIdx.x;
-  const int c = (blockIdx.y * 256 + threadIdx.x) * 8;
-  if (c >= N) return;
-  const int o = owner[t];
-  float s[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s[i] = 0.0f;
-  for (int r = 0; r < (o < 0 ? 0 : R); ++r) {
-    Vec16<T> a;
-    a.u = *reinterpret_cast<const uint4*>(f + ((int64_t)o * R + r) * N + c);
-    const float w = u[t * R + r];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s[i] = fmaf(w, Ty<T>::to_f(a.v[i]), s[i]);
-  }
-  Vec16<T> y;
-  y.u = base ? *reinterpret_cast<const uint4*>(base + t * base_stride + c) : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) y.v[i] = Ty<T>::from_f(Ty<T>::to_f(y.v[i]) + s[i]);
-  *reinterpret_cast<uint4*>(out + t * out_stride + c) = y.u;
-}
-
-// A block to an adapter, 256 columns and 16 ranks: g[l][r][c] = sum_t u[t][r] x[t][c].
-template <typename T, typename G>
-__global__ void __launch_bounds__(256) ad_outer_kernel(const float* __restrict__ u, const T* __restrict__ x, int64_t stride,
-                                                       int R, int K, AdPlan p, G* __restrict__ g) {
-  const int l = blockIdx.x, c = blockIdx.y * 256 + threadIdx.x, r0 = blockIdx.z * 16;
-  if (c >= K) return;
-  float s[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) s[i] = 0.0f;
-  for (int j = p.start[l]; j < p.start[l + 1]; ++j) {
-    const int64_t t = p.order[j];
-    const float v = Ty<T>::to_f(x[t * stride + c]);
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (r0 + i < R) s[i] = fmaf(u[t * R + r0 + i], v, s[i]);
-  }
-#pragma unroll
-  for (int i = 0; i < 16; ++i)
-    if (r0 + i < R) g[((int64_t)l * R + r0 + i) * K + c] = Ty<G>::from_f(s[i]);
-}
-
-template <typename T>
-int down(const lq_adapter_bank& b, const AdPlan& p, int64_t n, const void* x, int64_t stride, bool is_a, float* u,
-         cudaStream_t st) {
-  const int K = (int)(is_a ? b.K : b.N);
-  ad_down_kernel<T><<<(unsigned)n, 256, 0, st>>>(static_cast<const T*>(x), stride, static_cast<const T*>(is_a ? b.a : b.b),
-                                                 b.scaling, (int)b.R, K, p.owner, u);
-  return launched("ad_down_kernel");
-}
-template <typename T>
-int up(const lq_adapter_bank& b, const AdPlan& p, int64_t n, const float* u, bool is_a, const void* base, int64_t bs,
-       void* out, int64_t os, cudaStream_t st) {
-  const int N = (int)(is_a ? b.K : b.N);
-  ad_up_kernel<T><<<dim3((unsigned)n, (N + 2047) / 2048), 256, 0, st>>>(
-      u, static_cast<const T*>(is_a ? b.a : b.b), (int)b.R, N, p.owner, static_cast<const T*>(base), bs,
-      static_cast<T*>(out), os);
-  return launched("ad_up_kernel");
-}
-template <typename T>
-int outer(const lq_adapter_bank& b, const AdPlan& p, const float* u, const void* x, int64_t stride, bool is_a, void* g,
-          int grad_dtype, cudaStream_t st) {
-  const int K = (int)(is_a ? b.K : b.N);
-  const dim3 grid((unsigned)b.L, (K + 255) / 256, (unsigned)(b.R + 15) / 16);
-  if (grad_dtype == LQ_F32)
-    ad_outer_kernel<T, float><<<grid, 256, 0, st>>>(u, static_cast<const T*>(x), stride, (int)b.R, K, p, static_cast<float*>(g));
-  else
-    ad_outer_kernel<T, T><<<grid, 256, 0, st>>>(u, static_cast<const T*>(x), stride, (int)b.R, K, p, static_cast<T*>(g));
-  return launched("ad_outer_kernel");
-}
-
 int check_bank(const lq_adapter_bank* b, const void* plan, int64_t n) {
   LQ_REQUIRE(b && b->a && b->b && b->scaling, LQ_EINVAL, "adapters: NULL bank");
   LQ_REQUIRE(b->dtype == LQ_F16 || b->dtype == LQ_BF16, LQ_EDTYPE, "adapters: fp16 or bf16 (got dtype %d)", b->dtype);
@@ -210,6 +110,8 @@ int check_rows(const char* what, const void* p, int64_t stride, int64_t width, b
   LQ_REQUIRE(stride >= (wide ? width : 0), LQ_EINVAL, "adapters: rows of %s overlap", what);
   return LQ_OK;
 }
+
+size_t v_bytes(const lq_adapter_bank& b, int64_t n) { return 4 * (size_t)(n * ad_pitch(b.R)); }
 
 }  // namespace
 }  // namespace lq
@@ -240,7 +142,7 @@ extern "C" int lq_adapter_plan(const void* ids, int ids_dtype, int64_t n_ids, in
   return launched("ad_plan_kernel");
 }
 
-extern "C" int lq_adapter_forward(const lq_adapter_bank* bank, const void* plan, int64_t n, const void* x, int64_t x_stride,
+extern "C" int lq_adapter_forward(const lq_adapter_bank* bank, void* plan, int64_t n, const void* x, int64_t x_stride,
                                   const void* base, int64_t base_stride, void* out, int64_t out_stride, float* u,
                                   void* stream) {
   LQ_TRY(check_bank(bank, plan, n));
@@ -249,23 +151,18 @@ extern "C" int lq_adapter_forward(const lq_adapter_bank* bank, const void* plan,
   LQ_TRY(check_rows("out", out, out_stride, bank->N, n > 1));
   if (base) LQ_TRY(check_rows("base", base, base_stride, bank->N, false));
   LQ_REQUIRE(base != out || base_stride == out_stride, LQ_EINVAL, "adapters: out is base, with other rows");
-  LQ_REQUIRE(u, LQ_EINVAL, "adapters: NULL u");
-  const AdPlan p = ad_plan(const_cast<void*>(plan), n, bank->L);
-  cudaStream_t st = as_stream(stream);
-  if (bank->dtype == LQ_F16) {
-    LQ_TRY((down<__half>(*bank, p, n, x, x_stride, true, u, st)));
-    return up<__half>(*bank, p, n, u, false, base, base_stride, out, out_stride, st);
-  }
-  LQ_TRY((down<__nv_bfloat16>(*bank, p, n, x, x_stride, true, u, st)));
-  return up<__nv_bfloat16>(*bank, p, n, u, false, base, base_stride, out, out_stride, st);
+  LQ_REQUIRE(u && aligned16(u), LQ_EINVAL, "adapters: u is NULL or not on 16 bytes");
+  const AdCall a = {bank, ad_plan(plan, n, bank->L), n, as_stream(stream)};
+  LQ_TRY(ad_down(a, x, x_stride, true, u));
+  return ad_up(a, u, false, base, base_stride, out, out_stride);
 }
 
 extern "C" size_t lq_adapter_backward_workspace_bytes(const lq_adapter_bank* bank, int64_t n) {
-  if (!bank || n < 0 || n > (1 << 24)) return 0;
-  return 4 * (size_t)(n * bank->R);
+  if (!bank || n < 0 || n > (1 << 24) || bank->R < 1 || bank->R > kAdMaxRank || bank->K < 8 || bank->N < 8 || bank->L < 1) return 0;
+  return v_bytes(*bank, n) + ad_outer_part_bytes(*bank, n);
 }
 
-extern "C" int lq_adapter_backward(const lq_adapter_bank* bank, const void* plan, int64_t n, const void* x, int64_t x_stride,
+extern "C" int lq_adapter_backward(const lq_adapter_bank* bank, void* plan, int64_t n, const void* x, int64_t x_stride,
                                    const void* dy, int64_t dy_stride, const float* u, void* dx, void* da, void* db,
                                    int grad_dtype, void* workspace, size_t workspace_bytes, void* stream) {
   LQ_TRY(check_bank(bank, plan, n));
@@ -280,19 +177,14 @@ extern "C" int lq_adapter_backward(const lq_adapter_bank* bank, const void* plan
   LQ_TRY(check_rows("dy", dy, dy_stride, bank->N, false));
   if (da) LQ_TRY(check_rows("x", x, x_stride, bank->K, false));
   LQ_REQUIRE(!dx || aligned16(dx), LQ_EALIGN, "adapters: dx must be 16-byte aligned");
-  LQ_REQUIRE(!db || u, LQ_EINVAL, "adapters: NULL u");
+  LQ_REQUIRE(!db || (u && aligned16(u)), LQ_EINVAL, "adapters: u is NULL or not on 16 bytes");
   const size_t need = lq_adapter_backward_workspace_bytes(bank, n);
   LQ_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need, LQ_EINVAL, "adapters: %zu bytes of workspace needed", need);
-  const AdPlan p = ad_plan(const_cast<void*>(plan), n, bank->L);
+  const AdCall a = {bank, ad_plan(plan, n, bank->L), n, st};
   float* v = static_cast<float*>(workspace);
-  const bool half = bank->dtype == LQ_F16;
-  using H = __half;
-  using B = __nv_bfloat16;
-  if (dx || da) {
-    LQ_TRY((half ? down<H>(*bank, p, n, dy, dy_stride, false, v, st) : down<B>(*bank, p, n, dy, dy_stride, false, v, st)));
-  }
-  if (db) LQ_TRY((half ? outer<H>(*bank, p, u, dy, dy_stride, false, db, grad_dtype, st) : outer<B>(*bank, p, u, dy, dy_stride, false, db, grad_dtype, st)));
-  if (da) LQ_TRY((half ? outer<H>(*bank, p, v, x, x_stride, true, da, grad_dtype, st) : outer<B>(*bank, p, v, x, x_stride, true, da, grad_dtype, st)));
-  if (dx) LQ_TRY((half ? up<H>(*bank, p, n, v, true, nullptr, 0, dx, bank->K, st) : up<B>(*bank, p, n, v, true, nullptr, 0, dx, bank->K, st)));
+  float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + v_bytes(*bank, n));
+  if (dx || da) LQ_TRY(ad_down(a, dy, dy_stride, false, v));
+  if (da || db) LQ_TRY(ad_outer(a, {v, x, x_stride, da, u, dy, dy_stride, db, grad_dtype, part}));
+  if (dx) LQ_TRY(ad_up(a, v, true, nullptr, 0, dx, bank->K));
   return LQ_OK;
 }

@@ -27,6 +27,7 @@ struct AdPlan {
   int* start;    // [L + 2]
   int* tile_of;  // [L + 2]
   AdTile* tiles;
+  int* status;   // an lq_status: LQ_ETIMEOUT if a wait on the device ran out
 };
 
 __host__ __device__ inline int64_t ad_round4(int64_t n) { return (n + 3) / 4 * 4; }
@@ -38,16 +39,60 @@ __host__ __device__ inline int64_t ad_max_tiles(int64_t T, int64_t L) {
   return n < T ? n : T;
 }
 __host__ __device__ inline int64_t ad_plan_ints(int64_t T, int64_t L) {
-  return 2 * ad_round4(T) + 2 * ad_round4(L + 2) + 4 * ad_max_tiles(T, L);
+  return 4 + 2 * ad_round4(T) + 2 * ad_round4(L + 2) + 4 * ad_max_tiles(T, L);
 }
 __host__ __device__ inline AdPlan ad_plan(void* p, int64_t T, int64_t L) {
   AdPlan a;
-  a.owner = static_cast<int*>(p);
+  a.status = static_cast<int*>(p);
+  a.owner = a.status + 4;
   a.order = a.owner + ad_round4(T);
   a.start = a.order + ad_round4(T);
   a.tile_of = a.start + ad_round4(L + 2);
   a.tiles = reinterpret_cast<AdTile*>(a.tile_of + ad_round4(L + 2));
   return a;
 }
+
+// Columns of u and v: the rank, rounded up so that rows are on 32 bytes; zeros
+// behind the rank.
+inline int ad_pitch(int64_t R) { return (int)((R + 7) / 8 * 8); }
+
+// What every launch of a call has.
+struct AdCall {
+  const lq_adapter_bank* bank;
+  AdPlan plan;
+  int64_t n;
+  cudaStream_t st;
+};
+
+// The sums of outer products: da = sum v x^T and db = sum u dy^T, either NULL.
+struct AdOuter {
+  const float* v;
+  const void* x;
+  int64_t x_stride;
+  void* da;
+  const float* u;
+  const void* dy;
+  int64_t dy_stride;
+  void* db;
+  int grad_dtype;
+  float* part;  // two partial sums of each side's [R, K], [R, N] for each group
+};
+// Groups that the tiles of a call are dealt out to: with all column chunks of
+// both sides, one wave of resident blocks.  `blocks` to an SM go by the rank.
+inline int64_t ad_outer_groups(const lq_adapter_bank& b, int64_t n) {
+  const int64_t chunks = (b.K + 255) / 256 + (b.N + 255) / 256, tiles = ad_max_tiles(n, b.L);
+  int64_t g = (int64_t)num_sms() * (b.R <= 16 ? 2 : 1) / chunks;
+  g = g < tiles ? g : tiles;
+  return g > 1 ? g : 1;
+}
+inline size_t ad_outer_part_bytes(const lq_adapter_bank& b, int64_t n) {
+  return sizeof(float) * 2 * (size_t)ad_outer_groups(b, n) * b.R * (b.K + b.N);
+}
+
+// lq_adapters_mm.cu: u = s A x (is_a) or v = s B dy of the tokens with an
+// adapter; out = base + A^T u (is_a) or base + B^T u; ad_outer as above.
+int ad_down(const AdCall& a, const void* x, int64_t stride, bool is_a, float* u);
+int ad_up(const AdCall& a, const float* u, bool is_a, const void* base, int64_t base_stride, void* out, int64_t out_stride);
+int ad_outer(const AdCall& a, const AdOuter& o);
 
 }  // namespace lq
