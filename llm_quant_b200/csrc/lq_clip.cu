@@ -35,22 +35,28 @@ struct ClipTable {
   int count;
 };
 
-// Values of a unit: those before the first 16-byte boundary of `at` belong to
-// the tensor's first unit, what is left behind the last whole vector to its last.
+// Values of a unit.  The vectors begin at the first 16-byte boundary of `at`
+// (and one vector later, and end one earlier, where `wide`); what lies before
+// them belongs to the tensor's first unit, what is left behind them to its last.
 struct Span {
-  int64_t lo, hi;    // the vectors' values
-  int64_t head, end;  // head: values 0 .. head - 1 are this unit's too (0: none); end: values hi .. end - 1 too
+  int64_t lo;     // the first vector's first value
+  int vecs;
+  int64_t head;   // values 0 .. head - 1 are this unit's too (0: none)
+  int64_t tail, end;  // and values tail .. end - 1
 };
-__device__ __forceinline__ Span span_of(const void* at, int64_t n, int size, int unit, int units) {
-  const int per = kClipUnit / size, vec = 16 / size;
-  const int64_t head = min(n, (int64_t)((16 - ((reinterpret_cast<uintptr_t>(at)) & 15)) & 15) / size);
+template <typename T>
+__device__ __forceinline__ Span span_of(const void* at, int64_t n, int unit, int units, bool wide) {
+  constexpr int size = sizeof(T), per = kClipUnit / size, vec = 16 / size;
+  const int edge = wide ? vec : 0;
+  const int64_t head = min(n, (int64_t)((16 - ((reinterpret_cast<uintptr_t>(at)) & 15)) & 15) / size + edge);
+  const int64_t stop = head + (max(n - edge - head, (int64_t)0) & -(int64_t)vec);  // behind the last vector
   Span s;
-  s.lo = min(n, head + (int64_t)unit * per);
-  // the head moves the units on: the last but one may reach the end already
-  const bool last = unit == units - 1 || s.lo + per > n;
-  s.hi = last ? s.lo + (n - s.lo) / vec * vec : s.lo + per;
+  s.lo = min(stop, head + (int64_t)unit * per);
+  const int64_t hi = unit == units - 1 ? stop : min(stop, s.lo + per);
+  s.vecs = (int)((hi - s.lo) / vec);
   s.head = unit == 0 ? head : 0;
-  s.end = last ? n : s.hi;
+  s.tail = unit == units - 1 ? stop : n;
+  s.end = n;
   return s;
 }
 
@@ -113,9 +119,11 @@ __device__ __forceinline__ double squares(const uint32_t* w) {
 }
 
 template <typename T>
-__device__ __forceinline__ double unit_squares(const T* x, const Span& s) {
+__device__ __forceinline__ double unit_squares(const void* in, int64_t n, int unit, int units) {
+  const T* x = static_cast<const T*>(in);
+  const Span s = span_of<T>(in, n, unit, units, false);
+  const int vecs = s.vecs;
   double d = 0.0;
-  const int vecs = (int)((s.hi - s.lo) / Clip<T>::V);
   const uint4* v = reinterpret_cast<const uint4*>(x + s.lo);
   uint4 w[kClipVecs];
 #pragma unroll
@@ -132,7 +140,7 @@ __device__ __forceinline__ double unit_squares(const T* x, const Span& s) {
   // fewer than a vector's values on either side
   const int t = threadIdx.x;
   if (t < s.head) d += (double)Ty<T>::to_f(x[t]) * (double)Ty<T>::to_f(x[t]);
-  if (s.hi + t < s.end) d += (double)Ty<T>::to_f(x[s.hi + t]) * (double)Ty<T>::to_f(x[s.hi + t]);
+  if (s.tail + t < s.end) d += (double)Ty<T>::to_f(x[s.tail + t]) * (double)Ty<T>::to_f(x[s.tail + t]);
   return d;
 }
 
@@ -166,99 +174,88 @@ __global__ void __launch_bounds__(kClipThreads) clip_norm_kernel(const __grid_co
   pdl_wait();
   pdl_trigger();
   const int64_t units = t.unit0[t.count];
-  const int u0 = (int)(units * blockIdx.x / gridDim.x), u1 = (int)(units * (blockIdx.x + 1) / gridDim.x);
   double d = 0.0;
-  int i = u0 < u1 ? tensor_of(t, u0) : 0;
-  for (int u = u0; u < u1; ++u) {
-    while (t.unit0[i + 1] <= u) ++i;
-    const int size = t.dtype[i] == LQ_F32 ? 4 : 2;
-    const Span s = span_of(t.in[i], t.n[i], size, u - t.unit0[i], t.unit0[i + 1] - t.unit0[i]);
-    if (t.dtype[i] == LQ_F32) d += unit_squares(static_cast<const float*>(t.in[i]), s);
-    else if (t.dtype[i] == LQ_F16) d += unit_squares(static_cast<const __half*>(t.in[i]), s);
-    else d += unit_squares(static_cast<const __nv_bfloat16*>(t.in[i]), s);
+  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const int i = tensor_of(t, (int)u);
+    const int k = (int)u - t.unit0[i], units_i = t.unit0[i + 1] - t.unit0[i];
+    if (t.dtype[i] == LQ_F32) d += unit_squares<float>(t.in[i], t.n[i], k, units_i);
+    else if (t.dtype[i] == LQ_F16) d += unit_squares<__half>(t.in[i], t.n[i], k, units_i);
+    else d += unit_squares<__nv_bfloat16>(t.in[i], t.n[i], k, units_i);
   }
   d = block_sum(d, part);
   if (threadIdx.x == 0) sums[blockIdx.x] = d;
 }
 
-// 16 bytes of x from any address that its type can have: two aligned vectors,
-// shifted together.  Both are inside the tensor.
-__device__ __forceinline__ void load_shifted(const uint8_t* p, uint32_t* w) {
-  const int off = (int)(reinterpret_cast<uintptr_t>(p) & 15);
-  const uint4* v = reinterpret_cast<const uint4*>(p - off);
-  const uint4 a = __ldg(v), b = __ldg(v + 1);
-  const uint32_t x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+// 16 bytes from off bytes into two neighbouring vectors (off: not 0).
+__device__ __forceinline__ void shift(const uint4& a, const uint4& b, int off, uint32_t* w) {
   const int bits = (off & 3) * 8;
   uint32_t y[5];
-  switch (off >> 2) {  // the same for the whole unit
-    case 0:
-#pragma unroll
-      for (int i = 0; i < 5; ++i) y[i] = x[i];
-      break;
-    case 1:
-#pragma unroll
-      for (int i = 0; i < 5; ++i) y[i] = x[i + 1];
-      break;
-    case 2:
-#pragma unroll
-      for (int i = 0; i < 5; ++i) y[i] = x[i + 2];
-      break;
-    default:
-#pragma unroll
-      for (int i = 0; i < 5; ++i) y[i] = x[i + 3];
-      break;
+  switch (off >> 2) {
+    case 0: y[0] = a.x, y[1] = a.y, y[2] = a.z, y[3] = a.w, y[4] = b.x; break;
+    case 1: y[0] = a.y, y[1] = a.z, y[2] = a.w, y[3] = b.x, y[4] = b.y; break;
+    case 2: y[0] = a.z, y[1] = a.w, y[2] = b.x, y[3] = b.y, y[4] = b.z; break;
+    default: y[0] = a.w, y[1] = b.x, y[2] = b.y, y[3] = b.z, y[4] = b.w; break;
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(y[i], y[i + 1], bits);
 }
 
-template <typename T>
-__device__ __forceinline__ void unit_scale(const T* x, T* out, int64_t n, const Span& s, float c) {
+// SHIFTED: the result lies on 16 bytes where the source does not.  A lane loads
+// the aligned vector that its source begins in; the rest of it is the next lane's.
+template <typename T, bool SHIFTED>
+__device__ __forceinline__ void scale_vectors(const uint8_t* from, uint4* to, int vecs, int off, float c) {
   constexpr int V = Clip<T>::V;
-  const int vecs = (int)((s.hi - s.lo) / V);
-  const int t = threadIdx.x;
-  const uint8_t* from = reinterpret_cast<const uint8_t*>(x + s.lo);
-  uint4* to = reinterpret_cast<uint4*>(out + s.lo);
-  const bool aligned = (reinterpret_cast<uintptr_t>(from) & 15) == 0;
-  // shifted loads reach up to 15 bytes to either side of a vector
-  const uint8_t* first = reinterpret_cast<const uint8_t*>(x);
-  const uint8_t* last = reinterpret_cast<const uint8_t*>(x + n);
-  uint32_t w[kClipVecs][4];
+  const int lane = threadIdx.x & 31;
+  uint4 a[kClipVecs];
 #pragma unroll
   for (int k = 0; k < kClipVecs; ++k) {
-    const int i = k * kClipThreads + t;
-    if (i >= vecs) continue;
-    const uint8_t* p = from + 16 * (int64_t)i;
-    if (aligned) {
-      const uint4 a = *reinterpret_cast<const uint4*>(p);
-      w[k][0] = a.x, w[k][1] = a.y, w[k][2] = a.z, w[k][3] = a.w;
-    } else if (p - 15 >= first && p + 31 <= last) {
-      load_shifted(p, w[k]);
-    } else {
-      const T* q = reinterpret_cast<const T*>(p);
-      float f[V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) f[e] = Ty<T>::to_f(q[e]);
-      Clip<T>::put(f, w[k]);
-    }
+    const int i = k * kClipThreads + threadIdx.x;
+    a[k] = make_uint4(0u, 0u, 0u, 0u);
+    // the vector behind the last one is inside the tensor too
+    if (SHIFTED ? i <= vecs : i < vecs) a[k] = *reinterpret_cast<const uint4*>(from - off + 16 * (int64_t)i);
   }
 #pragma unroll
   for (int k = 0; k < kClipVecs; ++k) {
-    const int i = k * kClipThreads + t;
+    const int i = k * kClipThreads + threadIdx.x;
+    uint32_t w[4] = {a[k].x, a[k].y, a[k].z, a[k].w};
+    if (SHIFTED) {
+      uint4 b;
+      b.x = __shfl_down_sync(0xffffffffu, a[k].x, 1), b.y = __shfl_down_sync(0xffffffffu, a[k].y, 1);
+      b.z = __shfl_down_sync(0xffffffffu, a[k].z, 1), b.w = __shfl_down_sync(0xffffffffu, a[k].w, 1);
+      if (lane == 31 && i < vecs) b = *reinterpret_cast<const uint4*>(from - off + 16 * (int64_t)(i + 1));
+      shift(a[k], b, off, w);
+    }
     if (i >= vecs) continue;
     float f[V];
-    Clip<T>::get(w[k], f);
+    Clip<T>::get(w, f);
 #pragma unroll
     for (int e = 0; e < V; ++e) f[e] = __fmul_rn(f[e], c);
-    Clip<T>::put(f, w[k]);
-    to[i] = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+    Clip<T>::put(f, w);
+    __stcs(to + i, make_uint4(w[0], w[1], w[2], w[3]));
   }
+}
+
+template <typename T>
+__device__ __forceinline__ void unit_scale(const void* in, void* res, int64_t n, int unit, int units, float c) {
+  const T* x = static_cast<const T*>(in);
+  T* out = static_cast<T*>(res);
+  const int off = (int)((reinterpret_cast<uintptr_t>(in) - reinterpret_cast<uintptr_t>(res)) & 15);  // the same for all vectors
+  const Span s = span_of<T>(res, n, unit, units, off != 0);
+  const uint8_t* from = reinterpret_cast<const uint8_t*>(x + s.lo);
+  uint4* to = reinterpret_cast<uint4*>(out + s.lo);
+  // without a vector there may be no boundary either: the tensor may end before the first
+  if (s.vecs > 0) {
+    if (off) scale_vectors<T, true>(from, to, s.vecs, off, c);
+    else scale_vectors<T, false>(from, to, s.vecs, 0, c);
+  }
+  // fewer than three vectors' values on either side
+  const int t = threadIdx.x;
   if (t < s.head) out[t] = Ty<T>::from_f(__fmul_rn(Ty<T>::to_f(x[t]), c));
-  if (s.hi + t < s.end) out[s.hi + t] = Ty<T>::from_f(__fmul_rn(Ty<T>::to_f(x[s.hi + t]), c));
+  if (s.tail + t < s.end) out[s.tail + t] = Ty<T>::from_f(__fmul_rn(Ty<T>::to_f(x[s.tail + t]), c));
 }
 
 template <int N>
-__global__ void __launch_bounds__(kClipThreads) clip_scale_kernel(const __grid_constant__ ClipTable<N> t,
+__global__ void __launch_bounds__(kClipThreads, 4) clip_scale_kernel(const __grid_constant__ ClipTable<N> t,
                                                                   const double* __restrict__ sums, int n_sums,
                                                                   double max_norm, float* __restrict__ norm) {
   __shared__ double part[kClipThreads / 32];
@@ -276,16 +273,13 @@ __global__ void __launch_bounds__(kClipThreads) clip_scale_kernel(const __grid_c
   __syncthreads();
   const float c = coef;
   const int64_t units = t.unit0[t.count];
-  const int u0 = (int)(units * blockIdx.x / gridDim.x), u1 = (int)(units * (blockIdx.x + 1) / gridDim.x);
-  int i = u0 < u1 ? tensor_of(t, u1 - 1) : 0;
-  for (int u = u1 - 1; u >= u0; --u) {
-    while (t.unit0[i] > u || t.unit0[i] == t.unit0[i + 1]) --i;
+  for (int64_t u = units - 1 - blockIdx.x; u >= 0; u -= gridDim.x) {
+    const int i = tensor_of(t, (int)u);
     if (c == 1.0f && t.in[i] == t.out[i]) continue;  // nothing changes
-    const int size = t.dtype[i] == LQ_F32 ? 4 : 2;
-    const Span s = span_of(t.out[i], t.n[i], size, u - t.unit0[i], t.unit0[i + 1] - t.unit0[i]);
-    if (t.dtype[i] == LQ_F32) unit_scale(static_cast<const float*>(t.in[i]), static_cast<float*>(t.out[i]), t.n[i], s, c);
-    else if (t.dtype[i] == LQ_F16) unit_scale(static_cast<const __half*>(t.in[i]), static_cast<__half*>(t.out[i]), t.n[i], s, c);
-    else unit_scale(static_cast<const __nv_bfloat16*>(t.in[i]), static_cast<__nv_bfloat16*>(t.out[i]), t.n[i], s, c);
+    const int k = (int)u - t.unit0[i], units_i = t.unit0[i + 1] - t.unit0[i];
+    if (t.dtype[i] == LQ_F32) unit_scale<float>(t.in[i], t.out[i], t.n[i], k, units_i, c);
+    else if (t.dtype[i] == LQ_F16) unit_scale<__half>(t.in[i], t.out[i], t.n[i], k, units_i, c);
+    else unit_scale<__nv_bfloat16>(t.in[i], t.out[i], t.n[i], k, units_i, c);
   }
 }
 
