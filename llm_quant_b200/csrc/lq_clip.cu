@@ -17,8 +17,10 @@ namespace lq {
 namespace {
 
 constexpr int kClipThreads = 256;
-constexpr int kClipVecs = 8;                                  // 16-byte vectors of a thread in a unit
-constexpr int kClipUnit = kClipThreads * kClipVecs * 16;      // bytes of a unit
+constexpr int kClipVecs = 8;  // 16-byte vectors of a thread in a unit
+// Bytes of a unit; where results lie on other bytes of 16 than their source, a
+// warp's last lane only serves the one before it.
+__host__ __device__ constexpr int clip_unit(bool shifted) { return kClipThreads / 32 * (shifted ? 31 : 32) * kClipVecs * 16; }
 constexpr int kClipMost = 1024;                               // tensors of a launch
 constexpr int kClipBlocks = 148 * 4;
 
@@ -32,32 +34,36 @@ struct ClipTable {
   int64_t n[N];
   int unit0[N + 1];  // units before the tensor's
   uint8_t dtype[N];
+  uint16_t first[kClipBlocks + 1];  // the tensor that a block's units begin in (a search on the device cost 8 us of 1024)
   int count;
+  int moved;  // some result is not in its source's place
 };
 
-// Values of a unit.  The vectors begin at the first 16-byte boundary of `at`
-// (and one vector later, and end one earlier, where `wide`); what lies before
-// them belongs to the tensor's first unit, what is left behind them to its last.
-struct Span {
-  int64_t lo;     // the first vector's first value
-  int vecs;
-  int64_t head;   // values 0 .. head - 1 are this unit's too (0: none)
-  int64_t tail, end;  // and values tail .. end - 1
+// Units k0 .. k1 - 1 of a tensor, in bytes from its start.  Vectors lie on 16
+// bytes of the result; those of the source are loaded from `off` bytes before,
+// where it lies otherwise.  The tensor's first unit has what comes before the
+// first vector too, its last one what is left behind the last; with a shifted
+// source these edges are a vector wider, so that the vectors to either side of
+// a load are inside the tensor.
+struct Stretch {
+  int64_t lo;             // the first vector
+  int64_t vecs;
+  int head;               // bytes 0 .. head - 1 too
+  int64_t tail, end;      // and bytes tail .. end - 1
 };
-template <typename T>
-__device__ __forceinline__ Span span_of(const void* at, int64_t n, int unit, int units, bool wide) {
-  constexpr int size = sizeof(T), per = kClipUnit / size, vec = 16 / size;
-  const int edge = wide ? vec : 0;
-  const int64_t head = min(n, (int64_t)((16 - ((reinterpret_cast<uintptr_t>(at)) & 15)) & 15) / size + edge);
-  const int64_t stop = head + (max(n - edge - head, (int64_t)0) & -(int64_t)vec);  // behind the last vector
-  Span s;
-  s.lo = min(stop, head + (int64_t)unit * per);
-  const int64_t hi = unit == units - 1 ? stop : min(stop, s.lo + per);
-  s.vecs = (int)((hi - s.lo) / vec);
-  s.head = unit == 0 ? head : 0;
-  s.tail = unit == units - 1 ? stop : n;
-  s.end = n;
+__device__ __forceinline__ Stretch stretch_of(const void* at, int64_t bytes, int off, int unit, int k0, int k1, int units) {
+  const int wide = off ? 16 : 0;
+  const int64_t head = min(bytes, (int64_t)((16 - (reinterpret_cast<uintptr_t>(at) & 15)) & 15) + wide);
+  const int64_t stop = head + (max(bytes - wide - head, (int64_t)0) & -16);  // behind the last vector
+  Stretch s;
+  s.lo = min(stop, head + (int64_t)k0 * unit);
+  s.vecs = ((k1 == units ? stop : min(stop, head + (int64_t)k1 * unit)) - s.lo) >> 4;
+  s.head = k0 == 0 ? (int)head : 0;
+  s.tail = stop, s.end = k1 == units ? bytes : stop;
   return s;
+}
+__device__ __forceinline__ int shift_of(const void* in, const void* out) {
+  return (int)((reinterpret_cast<uintptr_t>(in) - reinterpret_cast<uintptr_t>(out)) & 15);
 }
 
 template <typename T> struct Clip;  // 16 bytes of T: sum of squares, and scaled
@@ -119,28 +125,32 @@ __device__ __forceinline__ double squares(const uint32_t* w) {
 }
 
 template <typename T>
-__device__ __forceinline__ double unit_squares(const void* in, int64_t n, int unit, int units) {
-  const T* x = static_cast<const T*>(in);
-  const Span s = span_of<T>(in, n, unit, units, false);
-  const int vecs = s.vecs;
+__device__ __forceinline__ double stretch_squares(const void* in, const Stretch& s) {
+  const uint4* v = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(in) + s.lo) + threadIdx.x;
   double d = 0.0;
-  const uint4* v = reinterpret_cast<const uint4*>(x + s.lo);
-  uint4 w[kClipVecs];
+  int64_t left = s.vecs - threadIdx.x;
+  for (; left > (kClipVecs - 1) * kClipThreads; left -= kClipVecs * kClipThreads, v += kClipVecs * kClipThreads) {
+    uint4 w[kClipVecs];
 #pragma unroll
-  for (int k = 0; k < kClipVecs; ++k) {
-    const int i = k * kClipThreads + threadIdx.x;
-    w[k] = i < vecs ? v[i] : make_uint4(0u, 0u, 0u, 0u);
-  }
+    for (int k = 0; k < kClipVecs; ++k) w[k] = v[k * kClipThreads];
 #pragma unroll
-  for (int k = 0; k < kClipVecs; ++k)
-    if (k * kClipThreads + (int)threadIdx.x < vecs) {
+    for (int k = 0; k < kClipVecs; ++k) {
       const uint32_t a[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
       d += squares<T>(a);
     }
+  }
+#pragma unroll 4
+  for (; left > 0; left -= kClipThreads, v += kClipThreads) {
+    const uint4 w = *v;
+    const uint32_t a[4] = {w.x, w.y, w.z, w.w};
+    d += squares<T>(a);
+  }
   // fewer than a vector's values on either side
+  const T* x = static_cast<const T*>(in);
   const int t = threadIdx.x;
-  if (t < s.head) d += (double)Ty<T>::to_f(x[t]) * (double)Ty<T>::to_f(x[t]);
-  if (s.tail + t < s.end) d += (double)Ty<T>::to_f(x[s.tail + t]) * (double)Ty<T>::to_f(x[s.tail + t]);
+  if (t * (int)sizeof(T) < s.head) d += (double)Ty<T>::to_f(x[t]) * (double)Ty<T>::to_f(x[t]);
+  const int64_t e = s.tail / (int)sizeof(T) + t;
+  if (e * (int)sizeof(T) < s.end) d += (double)Ty<T>::to_f(x[e]) * (double)Ty<T>::to_f(x[e]);
   return d;
 }
 
@@ -157,30 +167,23 @@ __device__ __forceinline__ double block_sum(double d, double* part) {
   return d;
 }
 
-// The block's stretch of units, and the tensor that unit u is of.
-template <int N>
-__device__ __forceinline__ int tensor_of(const ClipTable<N>& t, int u) {
-  int lo = 0, hi = t.count;  // unit0[lo] <= u < unit0[hi]
-  while (hi - lo > 1) {
-    const int m = (lo + hi) / 2;
-    if (t.unit0[m] <= u) lo = m; else hi = m;
-  }
-  return lo;
-}
-
 template <int N>
 __global__ void __launch_bounds__(kClipThreads) clip_norm_kernel(const __grid_constant__ ClipTable<N> t, double* __restrict__ sums) {
   __shared__ double part[kClipThreads / 32];
   pdl_wait();
   pdl_trigger();
   const int64_t units = t.unit0[t.count];
+  const int u0 = (int)(units * blockIdx.x / gridDim.x), u1 = (int)(units * (blockIdx.x + 1) / gridDim.x);
   double d = 0.0;
-  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-    const int i = tensor_of(t, (int)u);
-    const int k = (int)u - t.unit0[i], units_i = t.unit0[i + 1] - t.unit0[i];
-    if (t.dtype[i] == LQ_F32) d += unit_squares<float>(t.in[i], t.n[i], k, units_i);
-    else if (t.dtype[i] == LQ_F16) d += unit_squares<__half>(t.in[i], t.n[i], k, units_i);
-    else d += unit_squares<__nv_bfloat16>(t.in[i], t.n[i], k, units_i);
+  for (int u = u0, i = t.first[blockIdx.x]; u < u1; ++i) {
+    const int a = t.unit0[i], b = t.unit0[i + 1], k1 = min(b, u1);
+    if (k1 <= u) continue;  // an empty tensor
+    const int size = t.dtype[i] == LQ_F32 ? 4 : 2;
+    const Stretch s = stretch_of(t.in[i], t.n[i] * size, 0, clip_unit(shift_of(t.in[i], t.out[i]) != 0), u - a, k1 - a, b - a);
+    if (t.dtype[i] == LQ_F32) d += stretch_squares<float>(t.in[i], s);
+    else if (t.dtype[i] == LQ_F16) d += stretch_squares<__half>(t.in[i], s);
+    else d += stretch_squares<__nv_bfloat16>(t.in[i], s);
+    u = k1;
   }
   d = block_sum(d, part);
   if (threadIdx.x == 0) sums[blockIdx.x] = d;
@@ -200,58 +203,46 @@ __device__ __forceinline__ void shift(const uint4& a, const uint4& b, int off, u
   for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(y[i], y[i + 1], bits);
 }
 
-// SHIFTED: the result lies on 16 bytes where the source does not.  A lane loads
-// the aligned vector that its source begins in; the rest of it is the next lane's.
+// A stretch, from its end to its start.  A lane of a shifted one loads the
+// aligned vector that its source begins in; the rest of it is the next lane's.
 template <typename T, bool SHIFTED>
-__device__ __forceinline__ void scale_vectors(const uint8_t* from, uint4* to, int vecs, int off, float c) {
-  constexpr int V = Clip<T>::V;
-  const int lane = threadIdx.x & 31;
-  uint4 a[kClipVecs];
+__device__ __forceinline__ void stretch_scale(const void* in, void* out, const Stretch& s, int off, float c) {
+  constexpr int V = Clip<T>::V, W = SHIFTED ? 31 : 32, STEP = kClipThreads / 32 * W;
+  const int lane = threadIdx.x & 31, at = (threadIdx.x >> 5) * W + lane;
+  const uint4* from = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(in) + s.lo - off);
+  uint4* to = reinterpret_cast<uint4*>(static_cast<uint8_t*>(out) + s.lo);
+  const int64_t loads = s.vecs == 0 ? 0 : SHIFTED ? s.vecs + 1 : s.vecs;
+  const int64_t most = SHIFTED && lane == 31 ? 0 : s.vecs;  // what the lane writes ends here
+  float f[V];
+  for (int64_t b = (s.vecs - 1) / (STEP * kClipVecs) * (STEP * kClipVecs); b >= 0; b -= STEP * kClipVecs) {
+    uint4 a[kClipVecs];
+    const int64_t i0 = b + at;
 #pragma unroll
-  for (int k = 0; k < kClipVecs; ++k) {
-    const int i = k * kClipThreads + threadIdx.x;
-    a[k] = make_uint4(0u, 0u, 0u, 0u);
-    // the vector behind the last one is inside the tensor too
-    if (SHIFTED ? i <= vecs : i < vecs) a[k] = *reinterpret_cast<const uint4*>(from - off + 16 * (int64_t)i);
-  }
+    for (int k = 0; k < kClipVecs; ++k)
+      a[k] = i0 + k * STEP < loads ? from[i0 + k * STEP] : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-  for (int k = 0; k < kClipVecs; ++k) {
-    const int i = k * kClipThreads + threadIdx.x;
-    uint32_t w[4] = {a[k].x, a[k].y, a[k].z, a[k].w};
-    if (SHIFTED) {
-      uint4 b;
-      b.x = __shfl_down_sync(0xffffffffu, a[k].x, 1), b.y = __shfl_down_sync(0xffffffffu, a[k].y, 1);
-      b.z = __shfl_down_sync(0xffffffffu, a[k].z, 1), b.w = __shfl_down_sync(0xffffffffu, a[k].w, 1);
-      if (lane == 31 && i < vecs) b = *reinterpret_cast<const uint4*>(from - off + 16 * (int64_t)(i + 1));
-      shift(a[k], b, off, w);
+    for (int k = 0; k < kClipVecs; ++k) {
+      uint32_t x[4] = {a[k].x, a[k].y, a[k].z, a[k].w};
+      if (SHIFTED) {
+        uint4 n;
+        n.x = __shfl_down_sync(0xffffffffu, x[0], 1), n.y = __shfl_down_sync(0xffffffffu, x[1], 1);
+        n.z = __shfl_down_sync(0xffffffffu, x[2], 1), n.w = __shfl_down_sync(0xffffffffu, x[3], 1);
+        shift(a[k], n, off, x);
+      }
+      Clip<T>::get(x, f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[e] = __fmul_rn(f[e], c);
+      Clip<T>::put(f, x);
+      if (i0 + k * STEP < most) __stcs(to + i0 + k * STEP, make_uint4(x[0], x[1], x[2], x[3]));
     }
-    if (i >= vecs) continue;
-    float f[V];
-    Clip<T>::get(w, f);
-#pragma unroll
-    for (int e = 0; e < V; ++e) f[e] = __fmul_rn(f[e], c);
-    Clip<T>::put(f, w);
-    __stcs(to + i, make_uint4(w[0], w[1], w[2], w[3]));
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ void unit_scale(const void* in, void* res, int64_t n, int unit, int units, float c) {
-  const T* x = static_cast<const T*>(in);
-  T* out = static_cast<T*>(res);
-  const int off = (int)((reinterpret_cast<uintptr_t>(in) - reinterpret_cast<uintptr_t>(res)) & 15);  // the same for all vectors
-  const Span s = span_of<T>(res, n, unit, units, off != 0);
-  const uint8_t* from = reinterpret_cast<const uint8_t*>(x + s.lo);
-  uint4* to = reinterpret_cast<uint4*>(out + s.lo);
-  // without a vector there may be no boundary either: the tensor may end before the first
-  if (s.vecs > 0) {
-    if (off) scale_vectors<T, true>(from, to, s.vecs, off, c);
-    else scale_vectors<T, false>(from, to, s.vecs, 0, c);
   }
   // fewer than three vectors' values on either side
+  const T* x = static_cast<const T*>(in);
+  T* y = static_cast<T*>(out);
   const int t = threadIdx.x;
-  if (t < s.head) out[t] = Ty<T>::from_f(__fmul_rn(Ty<T>::to_f(x[t]), c));
-  if (s.tail + t < s.end) out[s.tail + t] = Ty<T>::from_f(__fmul_rn(Ty<T>::to_f(x[s.tail + t]), c));
+  if (t * (int)sizeof(T) < s.head) y[t] = Ty<T>::from_f(__fmul_rn(Ty<T>::to_f(x[t]), c));
+  const int64_t e = s.tail / (int)sizeof(T) + t;
+  if (e * (int)sizeof(T) < s.end) y[e] = Ty<T>::from_f(__fmul_rn(Ty<T>::to_f(x[e]), c));
 }
 
 template <int N>
@@ -272,20 +263,28 @@ __global__ void __launch_bounds__(kClipThreads, 4) clip_scale_kernel(const __gri
   }
   __syncthreads();
   const float c = coef;
+  if (c == 1.0f && !t.moved) return;  // nothing changes
   const int64_t units = t.unit0[t.count];
-  for (int64_t u = units - 1 - blockIdx.x; u >= 0; u -= gridDim.x) {
-    const int i = tensor_of(t, (int)u);
-    if (c == 1.0f && t.in[i] == t.out[i]) continue;  // nothing changes
-    const int k = (int)u - t.unit0[i], units_i = t.unit0[i + 1] - t.unit0[i];
-    if (t.dtype[i] == LQ_F32) unit_scale<float>(t.in[i], t.out[i], t.n[i], k, units_i, c);
-    else if (t.dtype[i] == LQ_F16) unit_scale<__half>(t.in[i], t.out[i], t.n[i], k, units_i, c);
-    else unit_scale<__nv_bfloat16>(t.in[i], t.out[i], t.n[i], k, units_i, c);
+  const int u0 = (int)(units * blockIdx.x / gridDim.x), u1 = (int)(units * (blockIdx.x + 1) / gridDim.x);
+  for (int u = u1, i = t.first[blockIdx.x + 1]; u > u0; --i) {
+    const int a = t.unit0[i], b = t.unit0[i + 1], k0 = max(a, u0);
+    if (k0 >= u) continue;  // an empty tensor
+    const int size = t.dtype[i] == LQ_F32 ? 4 : 2, off = shift_of(t.in[i], t.out[i]);
+    const Stretch s = stretch_of(t.out[i], t.n[i] * size, off, clip_unit(off != 0), k0 - a, u - a, b - a);
+    if (t.dtype[i] == LQ_F32)
+      off ? stretch_scale<float, true>(t.in[i], t.out[i], s, off, c) : stretch_scale<float, false>(t.in[i], t.out[i], s, 0, c);
+    else if (t.dtype[i] == LQ_F16)
+      off ? stretch_scale<__half, true>(t.in[i], t.out[i], s, off, c) : stretch_scale<__half, false>(t.in[i], t.out[i], s, 0, c);
+    else
+      off ? stretch_scale<__nv_bfloat16, true>(t.in[i], t.out[i], s, off, c) : stretch_scale<__nv_bfloat16, false>(t.in[i], t.out[i], s, 0, c);
+    u = k0;
   }
 }
 
-int64_t units_of(int64_t n, int dtype) {
+int64_t units_of(const void* in, const void* out, int64_t n, int dtype) {
   const int64_t bytes = n * dtype_size(dtype);
-  return (bytes + kClipUnit - 1) / kClipUnit;
+  const int unit = clip_unit(((reinterpret_cast<uintptr_t>(in) - reinterpret_cast<uintptr_t>(out)) & 15) != 0);
+  return (bytes + unit - 1) / unit;
 }
 
 template <int N>
@@ -296,10 +295,14 @@ int clip_launch(const void* const* in, void* const* out, const int64_t* n, const
   for (int i = 0; i < count; ++i) {
     t.in[i] = in[i], t.out[i] = out ? out[i] : const_cast<void*>(in[i]);
     t.n[i] = n[i], t.dtype[i] = (uint8_t)dtype[i], t.unit0[i] = (int)units;
-    units += units_of(n[i], dtype[i]);
+    units += units_of(t.in[i], t.out[i], n[i], dtype[i]);
   }
   LQ_REQUIRE(units < (1LL << 31), LQ_ERANGE, "clip: too many values");
-  t.unit0[count] = (int)units, t.count = count;
+  t.unit0[count] = (int)units, t.count = count, t.moved = out != nullptr;
+  for (int b = 0, i = 0; b <= blocks; ++b) {
+    while (i + 1 < count && t.unit0[i + 1] <= units * b / blocks) ++i;
+    t.first[b] = (uint16_t)i;
+  }
   const cudaError_t e = norm_pass ? launch_pdl(clip_norm_kernel<N>, dim3(blocks), dim3(kClipThreads), 0, st, t, sums)
                                   : launch_pdl(clip_scale_kernel<N>, dim3(blocks), dim3(kClipThreads), 0, st, t,
                                                (const double*)sums, n_sums, max_norm, norm);
@@ -342,7 +345,8 @@ extern "C" int lq_clip_grad_norm(const void* const* host_in, void* const* host_o
     for (int64_t i0 = 0; i0 < count || i0 == 0; i0 += kClipMost) {
       const int c = (int)(count - i0 < kClipMost ? count - i0 : kClipMost);
       int64_t units = 0;
-      for (int i = 0; i < c; ++i) units += units_of(host_n[i0 + i], host_dtype[i0 + i]);
+      for (int i = 0; i < c; ++i)
+        units += units_of(host_in[i0 + i], host_out ? host_out[i0 + i] : host_in[i0 + i], host_n[i0 + i], host_dtype[i0 + i]);
       const int blocks = (int)(units < 1 ? 1 : units < kClipBlocks ? units : kClipBlocks);
       const auto f = c <= 32 ? clip_launch<32> : c <= 256 ? clip_launch<256> : clip_launch<kClipMost>;
       LQ_TRY(f(host_in ? host_in + i0 : nullptr, host_out ? host_out + i0 : nullptr, host_n ? host_n + i0 : nullptr,

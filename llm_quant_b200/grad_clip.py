@@ -78,7 +78,9 @@ class GradClipper:
                       None if out is None else (ctypes.c_void_p * n)(*[o.data_ptr() for o in self._out]),
                       (ctypes.c_int64 * n)(*[g.numel() for g in self._in]),
                       (ctypes.c_int * n)(*[_C.dt(g) for g in self._in]), n)
-        self._versions = [o for o in self._out if not o.is_inference()]
+        # views of one buffer share its version
+        bases = {id(b): b for b in (o if o._base is None else o._base for o in outs)}
+        self._versions = [b for b in bases.values() if not b.is_inference()]
         self._bytes = _C.lib().lq_clip_workspace_bytes(n)
 
     def clip(self, max_norm: float) -> torch.Tensor:
