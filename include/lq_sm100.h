@@ -471,8 +471,9 @@ int lq_kv4_reset(const lq_kv4_cache* host_cache, void* stream);
  * A [R, K] and B [R, N] (lora_B transposed), scaling[l].  For token t with
  * adapter i:  out_t = base_t + scaling[i] B_i^T (A_i x_t), else out_t = base_t.
  * fp16 or bf16; K and N multiples of 8 up to 2^22, R up to 128, L up to 8192, up
- * to 2^24 tokens.  Products are summed in fp32 or more, u is kept in fp32 and
- * each output is rounded once. */
+ * to 2^24 tokens.  Products are summed in fp32; A x and B dy meet the next factor
+ * in fp32 or as two 16-bit parts (off by 2^-16 of themselves in bf16, 2^-22 in
+ * fp16), and each output is rounded once. */
 typedef struct {
   const void* a;        /* [L, R, K] */
   const void* b;        /* [L, R, N] */
@@ -490,18 +491,26 @@ typedef struct {
 size_t lq_adapter_plan_bytes(int64_t n, int64_t L);
 int lq_adapter_plan(const void* ids, int ids_dtype, int64_t n_ids, int64_t seq_len, const int32_t* counts,
                     int64_t L, void* plan, void* stream);
+/* The rows of a call: n tokens; strides from row to row in elements, multiples
+ * of 8, as the addresses are of 16 bytes.  keep: what the forward call leaves in
+ * `low` is for lq_adapter_backward (which takes the form too: out_stride is dy's). */
+typedef struct {
+  int64_t n, x_stride, base_stride, out_stride;
+  int keep;
+} lq_adapter_form;
 /* out [n, N] = base [n, N] (NULL: 0; may be out itself) + the adapters' share of
- * x [n, K].  Strides are of rows, in elements, multiples of 8, as the addresses
- * are of 16 bytes.  u [n, R] fp32: scaling * A x of the tokens with an adapter. */
-int lq_adapter_forward(const lq_adapter_bank* host_bank, void* plan, int64_t n, const void* x, int64_t x_stride,
-                       const void* base, int64_t base_stride, void* out, int64_t out_stride, float* u, void* stream);
+ * x [n, K].  low: lq_adapter_low_bytes (0: may be NULL) for this call alone, or
+ * until its backward call. */
+size_t lq_adapter_low_bytes(const lq_adapter_bank* host_bank, const lq_adapter_form* host_form);
+int lq_adapter_forward(const lq_adapter_bank* host_bank, const lq_adapter_form* host_form, void* plan, const void* x,
+                       const void* base, void* out, void* low, size_t low_bytes, void* stream);
 /* Gradients for dy [n, N], the gradient of out (base's is dy itself): dx [n, K],
  * da [L, R, K], db [L, R, N] in grad_dtype (LQ_F32 or the bank's), all
- * contiguous; a NULL one is not computed.  u is what the forward call left. */
+ * contiguous; a NULL one is not computed. */
 size_t lq_adapter_backward_workspace_bytes(const lq_adapter_bank* host_bank, int64_t n);
-int lq_adapter_backward(const lq_adapter_bank* host_bank, void* plan, int64_t n, const void* x, int64_t x_stride,
-                        const void* dy, int64_t dy_stride, const float* u, void* dx, void* da, void* db,
-                        int grad_dtype, void* workspace, size_t workspace_bytes, void* stream);
+int lq_adapter_backward(const lq_adapter_bank* host_bank, const lq_adapter_form* host_form, void* plan, const void* x,
+                        const void* dy, void* low, size_t low_bytes, void* dx, void* da, void* db, int grad_dtype,
+                        void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- gradients -----------------------------------------------------------------
  * norm = sqrt(sum of the squares of all values of `count` tensors together), out

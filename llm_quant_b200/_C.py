@@ -84,8 +84,8 @@ _SIGS = {
     "lq_kv4_attention": [_V, _V, _V, _V, _V, _V, _V, _V, ctypes.c_size_t, _V],
     "lq_kv4_reset": [_V, _V],
     "lq_adapter_plan": [_V, _I, _L, _L, _V, _L, _V, _V],
-    "lq_adapter_forward": [_V, _V, _L, _V, _L, _V, _L, _V, _L, _V, _V],
-    "lq_adapter_backward": [_V, _V, _L, _V, _L, _V, _L, _V, _V, _V, _V, _I, _V, ctypes.c_size_t, _V],
+    "lq_adapter_forward": [_V, _V, _V, _V, _V, _V, _V, ctypes.c_size_t, _V],
+    "lq_adapter_backward": [_V, _V, _V, _V, _V, _V, ctypes.c_size_t, _V, _V, _V, _I, _V, ctypes.c_size_t, _V],
     "lq_clip_grad_norm": [_V, _V, _V, _V, _L, ctypes.c_double, _V, _V, ctypes.c_size_t, _V],
 }
 _SIZE_SIGS = {
@@ -98,6 +98,7 @@ _SIZE_SIGS = {
     "lq_kv4_attention_workspace_bytes": [_V, _V],
     "lq_clip_workspace_bytes": [_L],
     "lq_adapter_plan_bytes": [_L, _L],
+    "lq_adapter_low_bytes": [_V, _V],
     "lq_adapter_backward_workspace_bytes": [_V, _L],
 }
 
@@ -118,6 +119,11 @@ class KV4Attn(ctypes.Structure):
 class AdapterBank(ctypes.Structure):
     """lq_adapter_bank"""
     _fields_ = [(n, _V) for n in ("a", "b", "scaling")] + [(n, _L) for n in ("L", "R", "K", "N")] + [("dtype", _I)]
+
+
+class AdapterForm(ctypes.Structure):
+    """lq_adapter_form"""
+    _fields_ = [(n, _L) for n in ("n", "x_stride", "base_stride", "out_stride")] + [("keep", _I)]
 
 
 _lib = None

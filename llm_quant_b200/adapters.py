@@ -42,7 +42,7 @@ MAX_RANK, MAX_ADAPTERS, MAX_TOKENS = 128, 8192, 1 << 24
 def _call(device: torch.device, name: str, *args) -> None:
     """Call an entry point on `device` and its current stream."""
     index = device.index
-    if index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():
         _C.call(name, *args, _C.raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -80,6 +80,7 @@ class AdapterBatch:
         self.num_adapters, self.seq_len, self.requests = num_adapters, seq_len, ids.numel()
         self.tokens = self.requests * seq_len
         self.device = ids.device
+        self._sig = (self.tokens, num_adapters, ids.device)
         self._plan = torch.empty(_C.lib().lq_adapter_plan_bytes(self.tokens, num_adapters), dtype=torch.uint8,
                                  device=ids.device)
         self.update(ids, counts)
@@ -110,14 +111,25 @@ class AdapterBatch:
             raise _C.LQError("AdapterBatch", status, "a wait on the device ran out")
 
 
-def _rows(x: torch.Tensor, width: int):
-    """x as rows of `width` values that the kernels can read, and their stride:
-    the values side by side, rows on 16 bytes."""
-    x2 = x if x.ndim == 2 else x.reshape(-1, width)
-    stride = x2.stride(0) if x2.shape[0] > 1 else width
-    if x2.stride(1) == 1 and stride >= 0 and stride % 8 == 0 and x2.data_ptr() % 16 == 0:
-        return x2, stride
-    return x2.contiguous() if not x2.is_contiguous() else x2.clone(), width
+def _row_stride(x: torch.Tensor) -> Optional[int]:
+    """Elements from row to row of x [..., width], or None where the kernels
+    cannot read its rows as they lie: side by side values, one stride over all
+    leading dimensions, rows on 16 bytes."""
+    width = x.shape[-1]
+    if x.numel() <= width or x.is_contiguous():
+        return width if x.numel() == 0 or x.stride(-1) == 1 else None
+    if x.stride(-1) != 1:
+        return None
+    rows, stride = 1, None
+    for n, st in zip(reversed(x.shape[:-1]), reversed(x.stride()[:-1])):
+        if n == 1:
+            continue
+        if stride is None:
+            stride = st
+        elif st != rows * stride:
+            return None
+        rows *= n
+    return stride if stride >= 0 and stride % 8 == 0 else None
 
 
 class AdapterBank(nn.Module):
@@ -148,7 +160,9 @@ class AdapterBank(nn.Module):
         self.register_buffer("scaling", torch.full((num_adapters,), alpha / rank, dtype=torch.float32, device=device))
         bound = 1.0 / math.sqrt(in_features)  # as QLoRALinear's
         nn.init.uniform_(self.lora_A, -bound, bound)
-        self._c = (None, None)  # the bank as the entry points take it, and its addresses
+        self._c = (None, None)  # the bank's addresses, and the bank as the entry points take it
+        self._shapes = (self.lora_A.shape, self.lora_B.shape)
+        self._forms: dict = {}  # calls' shapes and strides as the entry points take them
 
     @classmethod
     def from_layers(cls, layers: Iterable, *, dtype: torch.dtype = torch.bfloat16) -> "AdapterBank":
@@ -180,14 +194,37 @@ class AdapterBank(nn.Module):
 
     # -- calls -------------------------------------------------------------------
     def _struct(self, a: torch.Tensor, b: torch.Tensor, s: torch.Tensor):
+        """The bank as the entry points take it, by reference, with the weights
+        a, b in a call's dtype."""
         key = (a.data_ptr(), b.data_ptr(), s.data_ptr(), a.dtype)
-        at, c = self._c
-        if at != key:
-            c = _C.AdapterBank(*key[:3], self.num_adapters, self.rank, self.in_features, self.out_features, _C.dt(a))
-            self._c = (key, c)  # the struct itself is never changed
-        return ctypes.byref(c)
+        c = self._c
+        if c[0] != key:
+            form = _C.AdapterBank(*key[:3], self.num_adapters, self.rank, self.in_features, self.out_features, _C.dt(a))
+            self._c = c = (key, ctypes.byref(form))  # the struct itself is never changed
+        return c[1]
 
-    def _check(self, x: torch.Tensor, batch: AdapterBatch, base: Optional[torch.Tensor]) -> None:
+    def _weights(self, x: torch.Tensor):
+        """lora_A, lora_B in x's dtype, and scaling."""
+        p = self._parameters
+        a, b, s = p["lora_A"], p["lora_B"], self._buffers["scaling"]
+        dev = x.device
+        if a.device != dev or b.device != dev or s.device != dev:
+            raise RuntimeError(f"AdapterBank: x on {dev}, the bank on {a.device}")
+        if a.dtype != b.dtype or s.dtype != torch.float32:
+            raise TypeError(f"AdapterBank: lora_A is {a.dtype}, lora_B {b.dtype}, scaling {s.dtype} (expected float32)")
+        if a.shape != self._shapes[0] or b.shape != self._shapes[1] or s.numel() != self.num_adapters:
+            raise RuntimeError(f"AdapterBank: lora_A {list(a.shape)}, lora_B {list(b.shape)} are not the bank's")
+        if a.dtype != x.dtype:
+            a, b = a.detach().to(x.dtype), b.detach().to(x.dtype)
+        if not (a.is_contiguous() and b.is_contiguous() and s.is_contiguous()) or (a.data_ptr() | b.data_ptr()) & 15:
+            a, b, s = (t.detach().clone(memory_format=torch.contiguous_format) for t in (a, b, s))
+        return a, b, s
+
+    def _form(self, key, x: torch.Tensor, batch: AdapterBatch, base: Optional[torch.Tensor], keep: bool,
+              inplace: bool):
+        """What a call's shapes and strides come to, checked once for each such
+        form: (form, bytes of `low`, shape of the result, whether x / base are to be
+        laid out first, form struct)."""
         _C.require_cuda(x, what="AdapterBank")
         if x.dtype not in _HALF:
             raise TypeError(f"AdapterBank: unsupported dtype {x.dtype} (float16, bfloat16)")
@@ -195,65 +232,78 @@ class AdapterBank(nn.Module):
             raise RuntimeError(f"AdapterBank: x {list(x.shape)} is not {batch.tokens} tokens of {self.in_features} features")
         if batch.num_adapters != self.num_adapters:
             raise ValueError(f"AdapterBank: a batch for {batch.num_adapters} adapters, a bank of {self.num_adapters}")
-        dev = x.device
-        if self.lora_A.device != dev or self.lora_B.device != dev or self.scaling.device != dev or batch.device != dev:
-            raise RuntimeError(f"AdapterBank: x on {dev}, the bank on {self.lora_A.device}, the batch on {batch.device}")
-        if self.lora_A.dtype != self.lora_B.dtype:
-            raise TypeError(f"AdapterBank: lora_A is {self.lora_A.dtype}, lora_B {self.lora_B.dtype}")
-        if self.scaling.dtype != torch.float32:
-            raise TypeError(f"AdapterBank: scaling must stay float32, not {self.scaling.dtype}")
-        if base is not None and (base.dtype != x.dtype or base.device != dev
-                                 or base.shape != x.shape[:-1] + (self.out_features,)):
+        if batch.device != x.device:
+            raise RuntimeError(f"AdapterBank: x on {x.device}, the batch on {batch.device}")
+        shape = x.shape[:-1] + (self.out_features,)
+        if base is not None and (base.dtype != x.dtype or base.device != x.device or base.shape != shape):
             raise RuntimeError(f"AdapterBank: base {list(base.shape)} {base.dtype} on {base.device} for x {list(x.shape)} "
-                               f"{x.dtype} on {dev}")
+                               f"{x.dtype} on {x.device}")
+        xs = _row_stride(x)
+        bs = 0 if base is None else _row_stride(base)
+        if inplace and (bs is None or batch.tokens > 1 and bs < self.out_features):
+            raise ValueError(f"AdapterBank.add_: y {list(base.shape)} with strides {list(base.stride())} must be rows on 16 bytes")
+        c = _C.AdapterForm(batch.tokens, self.in_features if xs is None else xs, self.out_features if bs is None else bs,
+                           bs if inplace else self.out_features, keep)
+        ref = ctypes.byref(c)
+        bank = _C.AdapterBank(None, None, None, self.num_adapters, self.rank, self.in_features, self.out_features, _C.dt(x))
+        low = _C.lib().lq_adapter_low_bytes(ctypes.byref(bank), ref)
+        form = (ref, low, shape, xs is None, bs is None, c)
+        if len(self._forms) >= 256:
+            self._forms.clear()
+        self._forms[key] = form
+        return form
 
-    def _weights(self, dtype: torch.dtype):
-        a, b = self.lora_A, self.lora_B
-        if a.dtype != dtype:
-            a = a.detach().to(dtype)
-        if b.dtype != dtype:
-            b = b.detach().to(dtype)
-        return a.contiguous(), b.contiguous()
-
-    def _forward(self, x: torch.Tensor, batch: AdapterBatch, base: Optional[torch.Tensor], out: Optional[torch.Tensor] = None):
-        """(out, u, a, b): out [..., out_features] is made here unless given as rows."""
-        n, dev = batch.tokens, x.device
-        x2, xs = _rows(x, self.in_features)
-        b2, bs = (None, 0) if base is None else _rows(base, self.out_features)
-        y, ys = (x.new_empty(x.shape[:-1] + (self.out_features,)), self.out_features) if out is None else (out, out.stride(0))
-        u = torch.empty(n, (self.rank + 7) // 8 * 8, dtype=torch.float32, device=dev)
-        a, b = self._weights(x.dtype)
-        if n:
-            _call(dev, "lq_adapter_forward", self._struct(a, b, self.scaling), batch._plan.data_ptr(), n, x2.data_ptr(), xs,
-                  None if b2 is None else b2.data_ptr(), bs, y.data_ptr(), ys, u.data_ptr())
-        return y, u, a, b
+    def _run(self, x: torch.Tensor, batch: AdapterBatch, base: Optional[torch.Tensor], keep: bool, inplace: bool):
+        """(out, low, form, a, b, scaling)"""
+        key = (x.dtype, x.shape, x.stride(), x.device, batch._sig, keep, inplace,
+               None if base is None else (base.dtype, base.shape, base.stride(), base.device))
+        form = self._forms.get(key)
+        if form is None:
+            form = self._form(key, x, batch, base, keep, inplace)
+        ref, nbytes, shape, copy_x, copy_base, _ = form
+        a, b, s = self._weights(x)
+        dev = x.device
+        if copy_x:
+            x = x.contiguous() if not x.is_contiguous() else x.clone()
+        at = x.data_ptr()
+        if at & 15:
+            if not copy_x and not x.is_contiguous():  # the form's strides are x's
+                return self._run(x.contiguous(), batch, base, keep, inplace)
+            x = x.clone()
+            at = x.data_ptr()
+        base_at = None
+        if base is not None:
+            if copy_base:
+                base = base.contiguous() if not base.is_contiguous() else base.clone()
+            base_at = base.data_ptr()
+            if base_at & 15:
+                if inplace:
+                    raise ValueError("AdapterBank.add_: y must be rows on 16 bytes")
+                return self._run(x, batch, base.clone(memory_format=torch.contiguous_format), keep, inplace)
+        out = base if inplace else torch.empty(shape, dtype=x.dtype, device=dev)
+        low = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        if batch.tokens:
+            _call(dev, "lq_adapter_forward", self._struct(a, b, s), ref, batch._plan.data_ptr(), at, base_at,
+                  out.data_ptr(), None if low is None else low.data_ptr(), nbytes)
+        return out, low, form, a, b, s, x
 
     def forward(self, x: torch.Tensor, batch: AdapterBatch, base: Optional[torch.Tensor] = None) -> torch.Tensor:
         """base [..., out_features] (default zeros) plus each token's adapter of
         x [..., in_features], whose leading dimensions are the batch's tokens."""
-        self._check(x, batch, base)
-        if torch.is_grad_enabled() and (x.requires_grad or self.lora_A.requires_grad or self.lora_B.requires_grad
-                                        or base is not None and base.requires_grad):
-            return _Adapters.apply(x, self.lora_A, self.lora_B, base, self, batch)
-        return self._forward(x, batch, base)[0]
+        if torch.is_grad_enabled():
+            p = self._parameters
+            a, b = p["lora_A"], p["lora_B"]
+            if x.requires_grad or a.requires_grad or b.requires_grad or base is not None and base.requires_grad:
+                return _Adapters.apply(x, a, b, base, self, batch)
+        return self._run(x, batch, base, False, False)[0]
 
     def add_(self, y: torch.Tensor, x: torch.Tensor, batch: AdapterBatch) -> torch.Tensor:
         """y += each token's adapter of x, in place; no gradient (call it under
         ``torch.no_grad()``).  Rows of tokens without an adapter are not written."""
-        self._check(x, batch, y)
         if torch.is_grad_enabled() and (x.requires_grad or y.requires_grad or self.lora_A.requires_grad
                                         or self.lora_B.requires_grad):
             raise RuntimeError("AdapterBank.add_: no gradient is computed here (use forward, or torch.no_grad())")
-        try:
-            y2 = y.view(-1, self.out_features)
-        except RuntimeError:
-            y2 = None
-        if y2 is None or y2.stride(1) != 1 or y2.data_ptr() % 16 \
-                or y2.shape[0] > 1 and (y2.stride(0) % 8 or y2.stride(0) < self.out_features):
-            raise ValueError(f"AdapterBank.add_: y {list(y.shape)} with strides {list(y.stride())} must be rows on 16 bytes")
-        if y2.shape[0] == 1:
-            y2 = y2.as_strided(y2.shape, (self.out_features, 1))
-        self._forward(x, batch, y2, out=y2)
+        self._run(x, batch, y, False, True)
         _changed(y)
         return y
 
@@ -267,28 +317,38 @@ class _Adapters(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, lora_A, lora_B, base, bank, batch):
-        y, u, a, b = bank._forward(x, batch, base)
-        # the weights as the call rounded them; scaling and the plan raise if they were changed since
-        ctx.save_for_backward(x, a, b, u, bank.scaling, batch._plan)
-        ctx.bank, ctx.tokens = bank, batch.tokens
-        ctx.dtype = lora_A.dtype
+        y, low, form, a, b, s, rows = bank._run(x, batch, base, True, False)
+        # the weights as the call rounded them; all of these raise if they were changed since
+        ctx.save_for_backward(rows, a, b, low, s, batch._plan)
+        ctx.bank, ctx.form, ctx.shape, ctx.dtype = bank, form, x.shape, lora_A.dtype
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, a, b, u, scaling, plan = ctx.saved_tensors
-        bank, n, dev = ctx.bank, ctx.tokens, x.device
         want_x, want_a, want_b, want_base = ctx.needs_input_grad[:4]
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_x else None
-        da = torch.empty(a.shape, dtype=ctx.dtype, device=dev) if want_a else None
-        db = torch.empty(b.shape, dtype=ctx.dtype, device=dev) if want_b else None
+        dx = da = db = None
         if want_x or want_a or want_b:
-            x2, xs = _rows(x, bank.in_features)
-            d2, ds = _rows(dy, bank.out_features)
-            ref = bank._struct(a, b, scaling)
-            nbytes = _C.lib().lq_adapter_backward_workspace_bytes(ref, n)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            _call(dev, "lq_adapter_backward", ref, plan.data_ptr(), n, x2.data_ptr(), xs, d2.data_ptr(), ds, u.data_ptr(),
-                  _C.ptr(dx), _C.ptr(da), _C.ptr(db), _C.dt(ctx.dtype), ws.data_ptr(), nbytes)
+            x, a, b, low, s, plan = ctx.saved_tensors
+            dev = x.device
+            if want_x:
+                dx = torch.empty(ctx.shape, dtype=x.dtype, device=dev)
+            if want_a:
+                da = torch.empty(a.shape, dtype=ctx.dtype, device=dev)
+            if want_b:
+                db = torch.empty(b.shape, dtype=ctx.dtype, device=dev)
+            bank, (form, nbytes, _, _, _, c) = ctx.bank, ctx.form
+            d = dy
+            stride = _row_stride(d)
+            if stride is None or d.data_ptr() & 15:
+                d = d.clone(memory_format=torch.contiguous_format)
+                stride = bank.out_features
+            if stride != bank.out_features:
+                form = ctypes.byref(_C.AdapterForm(c.n, c.x_stride, 0, stride, 1))
+            ref = bank._struct(a, b, s)
+            ws_bytes = _C.lib().lq_adapter_backward_workspace_bytes(ref, c.n)
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+            _call(dev, "lq_adapter_backward", ref, form, plan.data_ptr(), x.data_ptr(), d.data_ptr(), _C.ptr(low), nbytes,
+                  _C.ptr(dx), _C.ptr(da), _C.ptr(db), _C.dt(ctx.dtype) if da is not None or db is not None else _C.dt(x),
+                  ws.data_ptr(), ws_bytes)
         return dx, da, db, dy if want_base else None, None, None

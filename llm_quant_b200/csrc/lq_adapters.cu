@@ -4,10 +4,10 @@
 // adapter's lora_B transposed), so that both directions are the same three
 // products: rows times a factor (u = s A x, v = s B dy), a low-rank row times a
 // factor (y = B^T u, dx = A^T v) and sums of outer products over an adapter's
-// tokens (dA = v x^T, dB = u dy^T).  u and v are kept in fp32.
+// tokens (dA = v x^T, dB = u dy^T).
 //
 // This file: the plan and the entry points; the products are in
-// lq_adapters_mm.cu.
+// lq_adapters_few.cu and lq_adapters_mm.cu.
 #include "lq_adapters.cuh"
 
 namespace lq {
@@ -111,7 +111,10 @@ int check_rows(const char* what, const void* p, int64_t stride, int64_t width, b
   return LQ_OK;
 }
 
-size_t v_bytes(const lq_adapter_bank& b, int64_t n) { return 4 * (size_t)(n * ad_pitch(b.R)); }
+bool sizes_ok(const lq_adapter_bank& b, int64_t n) {
+  return n >= 0 && n <= (1 << 24) && b.L >= 1 && b.L <= kAdMaxAdapters && b.R >= 1 && b.R <= kAdMaxRank && b.K >= 8 && b.N >= 8;
+}
+size_t v_bytes(const lq_adapter_bank& b, int64_t n) { return (ad_low_bytes(b, n, true) + 255) / 256 * 256; }
 
 }  // namespace
 }  // namespace lq
@@ -142,29 +145,43 @@ extern "C" int lq_adapter_plan(const void* ids, int ids_dtype, int64_t n_ids, in
   return launched("ad_plan_kernel");
 }
 
-extern "C" int lq_adapter_forward(const lq_adapter_bank* bank, void* plan, int64_t n, const void* x, int64_t x_stride,
-                                  const void* base, int64_t base_stride, void* out, int64_t out_stride, float* u,
-                                  void* stream) {
+// Up to here a cluster works at each token: one launch, and weights that tokens
+// share come from L2 again; above, tiles of tokens share them.
+static bool few_tokens(const lq_adapter_form* f) { return !f->keep && f->n <= kAdFewTokens; }
+
+extern "C" size_t lq_adapter_low_bytes(const lq_adapter_bank* bank, const lq_adapter_form* form) {
+  if (!bank || !form || !sizes_ok(*bank, form->n) || few_tokens(form)) return 0;
+  return ad_low_bytes(*bank, form->n, form->keep != 0);
+}
+
+extern "C" int lq_adapter_forward(const lq_adapter_bank* bank, const lq_adapter_form* form, void* plan, const void* x,
+                                  const void* base, void* out, void* low, size_t low_bytes, void* stream) {
+  LQ_REQUIRE(form, LQ_EINVAL, "adapters: NULL form");
+  const int64_t n = form->n;
   LQ_TRY(check_bank(bank, plan, n));
   if (n == 0) return LQ_OK;
-  LQ_TRY(check_rows("x", x, x_stride, bank->K, false));
-  LQ_TRY(check_rows("out", out, out_stride, bank->N, n > 1));
-  if (base) LQ_TRY(check_rows("base", base, base_stride, bank->N, false));
-  LQ_REQUIRE(base != out || base_stride == out_stride, LQ_EINVAL, "adapters: out is base, with other rows");
-  LQ_REQUIRE(u && aligned16(u), LQ_EINVAL, "adapters: u is NULL or not on 16 bytes");
+  LQ_TRY(check_rows("x", x, form->x_stride, bank->K, false));
+  LQ_TRY(check_rows("out", out, form->out_stride, bank->N, n > 1));
+  if (base) LQ_TRY(check_rows("base", base, form->base_stride, bank->N, false));
+  LQ_REQUIRE(base != out || form->base_stride == form->out_stride, LQ_EINVAL, "adapters: out is base, with other rows");
+  const size_t need = lq_adapter_low_bytes(bank, form);
+  LQ_REQUIRE(need == 0 || (low && aligned16(low) && low_bytes >= need), LQ_EINVAL, "adapters: low must have %zu bytes, on 16", need);
   const AdCall a = {bank, ad_plan(plan, n, bank->L), n, as_stream(stream)};
-  LQ_TRY(ad_down(a, x, x_stride, true, u));
-  return ad_up(a, u, false, base, base_stride, out, out_stride);
+  if (few_tokens(form)) return ad_few(a, x, form->x_stride, base, form->base_stride, out, form->out_stride);
+  LQ_TRY(ad_down(a, x, form->x_stride, true, low, form->keep != 0));
+  return ad_up(a, low, false, base, form->base_stride, out, form->out_stride);
 }
 
 extern "C" size_t lq_adapter_backward_workspace_bytes(const lq_adapter_bank* bank, int64_t n) {
-  if (!bank || n < 0 || n > (1 << 24) || bank->R < 1 || bank->R > kAdMaxRank || bank->K < 8 || bank->N < 8 || bank->L < 1) return 0;
+  if (!bank || !sizes_ok(*bank, n)) return 0;
   return v_bytes(*bank, n) + ad_outer_part_bytes(*bank, n);
 }
 
-extern "C" int lq_adapter_backward(const lq_adapter_bank* bank, void* plan, int64_t n, const void* x, int64_t x_stride,
-                                   const void* dy, int64_t dy_stride, const float* u, void* dx, void* da, void* db,
-                                   int grad_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+extern "C" int lq_adapter_backward(const lq_adapter_bank* bank, const lq_adapter_form* form, void* plan, const void* x,
+                                   const void* dy, void* low, size_t low_bytes, void* dx, void* da, void* db, int grad_dtype,
+                                   void* workspace, size_t workspace_bytes, void* stream) {
+  LQ_REQUIRE(form, LQ_EINVAL, "adapters: NULL form");
+  const int64_t n = form->n;
   LQ_TRY(check_bank(bank, plan, n));
   LQ_REQUIRE(grad_dtype == LQ_F32 || grad_dtype == bank->dtype, LQ_EDTYPE, "adapters: gradients in fp32 or the bank's type");
   cudaStream_t st = as_stream(stream);
@@ -174,17 +191,18 @@ extern "C" int lq_adapter_backward(const lq_adapter_bank* bank, void* plan, int6
     LQ_REQUIRE(!db || cudaMemsetAsync(db, 0, size * bank->N, st) == cudaSuccess, LQ_ECUDA, "adapters: memset failed");
     return LQ_OK;
   }
-  LQ_TRY(check_rows("dy", dy, dy_stride, bank->N, false));
-  if (da) LQ_TRY(check_rows("x", x, x_stride, bank->K, false));
+  LQ_TRY(check_rows("dy", dy, form->out_stride, bank->N, false));
+  if (da) LQ_TRY(check_rows("x", x, form->x_stride, bank->K, false));
   LQ_REQUIRE(!dx || aligned16(dx), LQ_EALIGN, "adapters: dx must be 16-byte aligned");
-  LQ_REQUIRE(!db || (u && aligned16(u)), LQ_EINVAL, "adapters: u is NULL or not on 16 bytes");
+  LQ_REQUIRE(!db || (form->keep && low && aligned16(low) && low_bytes >= ad_low_bytes(*bank, n, true)), LQ_EINVAL,
+             "adapters: low must be what a forward call with `keep` left");
   const size_t need = lq_adapter_backward_workspace_bytes(bank, n);
   LQ_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need, LQ_EINVAL, "adapters: %zu bytes of workspace needed", need);
   const AdCall a = {bank, ad_plan(plan, n, bank->L), n, st};
-  float* v = static_cast<float*>(workspace);
+  void* v = workspace;
   float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + v_bytes(*bank, n));
-  if (dx || da) LQ_TRY(ad_down(a, dy, dy_stride, false, v));
-  if (da || db) LQ_TRY(ad_outer(a, {v, x, x_stride, da, u, dy, dy_stride, db, grad_dtype, part}));
+  if (dx || da) LQ_TRY(ad_down(a, dy, form->out_stride, false, v, da != nullptr));
+  if (da || db) LQ_TRY(ad_outer(a, {v, x, form->x_stride, da, low, dy, form->out_stride, db, grad_dtype, part}));
   if (dx) LQ_TRY(ad_up(a, v, true, nullptr, 0, dx, bank->K));
   return LQ_OK;
 }

@@ -9,6 +9,7 @@ namespace lq {
 constexpr int kAdTile = 128;        // tokens of a tile
 constexpr int kAdMaxAdapters = 8192;
 constexpr int kAdMaxRank = 128;
+constexpr int kAdFewTokens = 64;    // up to here a call without gradients takes ad_few
 
 // A tile: up to 128 tokens of one adapter (owner -1: of none), at places first
 // .. first + rows - 1 of `order`; run is the first one's token if all follow
@@ -52,9 +53,8 @@ __host__ __device__ inline AdPlan ad_plan(void* p, int64_t T, int64_t L) {
   return a;
 }
 
-// Columns of u and v: the rank, rounded up so that rows are on 32 bytes; zeros
-// behind the rank.
-inline int ad_pitch(int64_t R) { return (int)((R + 7) / 8 * 8); }
+// The rank, rounded up to what the kernels are made for.
+inline int ad_padded(int64_t R) { return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128; }
 
 // What every launch of a call has.
 struct AdCall {
@@ -66,11 +66,11 @@ struct AdCall {
 
 // The sums of outer products: da = sum v x^T and db = sum u dy^T, either NULL.
 struct AdOuter {
-  const float* v;
+  void* v;
   const void* x;
   int64_t x_stride;
   void* da;
-  const float* u;
+  void* u;
   const void* dy;
   int64_t dy_stride;
   void* db;
@@ -89,10 +89,17 @@ inline size_t ad_outer_part_bytes(const lq_adapter_bank& b, int64_t n) {
   return sizeof(float) * 2 * (size_t)ad_outer_groups(b, n) * b.R * (b.K + b.N);
 }
 
-// lq_adapters_mm.cu: u = s A x (is_a) or v = s B dy of the tokens with an
-// adapter; out = base + A^T u (is_a) or base + B^T u; ad_outer as above.
-int ad_down(const AdCall& a, const void* x, int64_t stride, bool is_a, float* u);
-int ad_up(const AdCall& a, const float* u, bool is_a, const void* base, int64_t base_stride, void* out, int64_t out_stride);
+// lq_adapters_few.cu: out = base + B^T (s A x), in fp32, a cluster of blocks to a
+// token.
+int ad_few(const AdCall& a, const void* x, int64_t x_stride, const void* base, int64_t base_stride, void* out,
+           int64_t out_stride);
+
+// lq_adapters_mm.cu.  ad_down: low = s A x (is_a) or s B dy, of the tokens with
+// an adapter, ad_low_bytes in the forms that the others read (`turned`: ad_outer
+// too); ad_up: out = base + A^T low (is_a) or base + B^T low; ad_outer as above.
+size_t ad_low_bytes(const lq_adapter_bank& b, int64_t n, bool turned);
+int ad_down(const AdCall& a, const void* x, int64_t stride, bool is_a, void* low, bool turned);
+int ad_up(const AdCall& a, void* low, bool is_a, const void* base, int64_t base_stride, void* out, int64_t out_stride);
 int ad_outer(const AdCall& a, const AdOuter& o);
 
 }  // namespace lq

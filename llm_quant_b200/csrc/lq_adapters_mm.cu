@@ -55,7 +55,7 @@ constexpr float kInf = __builtin_huge_valf();
 
 // Two fp32 values as two 16-bit pairs that add up to them.
 template <typename T>
-__device__ __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& lo) {
+__device__ __forceinline__ void split16(float a, float b, uint32_t& hi, uint32_t& lo) {
   hi = Half16<T>::pack(a, b);
   const float2 h = Half16<T>::unpack(hi);
   // nothing is left of what went to infinity (infinity less itself is NaN)
@@ -88,8 +88,44 @@ __device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr, uint32_t rank) {
   return v;
 }
 
+__device__ __forceinline__ void bulk_load_at(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+               "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ int lane_id() { return threadIdx.x & 31; }
 __device__ __forceinline__ int token_of(const AdPlan& p, const AdTile& d, int row) {
   return d.run >= 0 ? d.run + row : p.order[d.first + row];
+}
+
+// ---------------------------------------------------------------------------
+// The low-rank rows of a call (u or v), as ad_down leaves them for each tile:
+//   image  the two 16-bit parts as the K-major operand that ad_up copies into
+//          shared memory as it is: rows of hi (NP) | lo (NP), in panels of 64 values
+//          with the 128-byte swizzle (NP = 16: 32 values, 64-byte swizzle)
+//   back   fp16: what each row of the image is to be multiplied with
+//   turned fp32 [NP][128 tokens], for ad_outer
+//   top    fp16: greatest magnitude in the tile, by parts
+// ---------------------------------------------------------------------------
+struct Low {
+  uint8_t* image;
+  float* back;
+  float* turned;  // NULL: nobody reads it
+  float* top;
+};
+template <int NP>
+__host__ __device__ inline Low low_at(void* p, int64_t tiles, bool turned) {
+  Low l;
+  l.image = static_cast<uint8_t*>(p);
+  l.back = reinterpret_cast<float*>(l.image + tiles * (128 * NP * 4));
+  l.top = l.back + tiles * 128;
+  l.turned = turned ? l.top + tiles * 8 : nullptr;
+  return l;
+}
+template <int NP>
+__device__ __forceinline__ uint32_t image_offset(int row, int k) {  // of value k (a multiple of 8) of a row
+  if (NP == 16) return row * 64 + (((k >> 3) ^ ((row >> 1) & 3)) << 4);
+  return (k >> 6) * 16384 + row * 128 + ((((k >> 3) & 7) ^ (row & 7)) << 4);
 }
 
 // ---------------------------------------------------------------------------
@@ -108,15 +144,16 @@ struct DownShared {
 
 template <typename T, int NP>
 __global__ void __launch_bounds__(160, 2) ad_down_kernel(const T* __restrict__ x, int64_t stride, const T* __restrict__ f,
-                                                         const float* __restrict__ scaling, int R, int pitch, int K, AdPlan p,
-                                                         int L, float* __restrict__ u, int split) {
+                                                         const float* __restrict__ scaling, int R, int K, AdPlan p, int L,
+                                                         Low low, int split) {
   using S = DownShared<NP>;
   constexpr int NS = S::stages, LAG = NS - 2;
   constexpr uint32_t kCols = NP < 32 ? 32 : NP;
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t full[NS], empty[NS], done;
   __shared__ uint32_t tmem_at;
-  __shared__ int failed;
+  __shared__ int failed, row_top[128];
+  using H = Half16<T>;
   pdl_wait();
   pdl_trigger();
   const int tile = blockIdx.x / split, rank = blockIdx.x - tile * split;
@@ -194,216 +231,320 @@ __global__ void __launch_bounds__(160, 2) ad_down_kernel(const T* __restrict__ x
   if (!ok) failed = 1;
   tc_fence_after();
   if (warp < 4) {
-    const int row = tid;
-    const bool mine = split == 1 && row < d.rows;
-    float* to = mine ? u + (int64_t)token_of(p, d, row) * pitch : nullptr;
 #pragma unroll
     for (int c = 0; c < NP; c += 16) {
       uint32_t v[16];
       tmem_ld16(tmem + ((uint32_t)warp << 21) + c, v);
       tmem_wait_ld16(v);
 #pragma unroll
-      for (int q = 0; q < 16; q += 4) {
-        float4 w = make_float4(__uint_as_float(v[q]), __uint_as_float(v[q + 1]), __uint_as_float(v[q + 2]), __uint_as_float(v[q + 3]));
-        if (split == 1) {
-          if (mine && c + q < pitch) {  // ranks behind R: rows of F that nobody loaded
-            w.x = c + q < R ? w.x * s : 0.0f, w.y = c + q + 1 < R ? w.y * s : 0.0f;
-            w.z = c + q + 2 < R ? w.z * s : 0.0f, w.w = c + q + 3 < R ? w.w * s : 0.0f;
-            *reinterpret_cast<float4*>(to + c + q) = w;
-          }
-        } else {
-          asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(base + (row * S::pitch + c + q) * 4), "f"(w.x), "f"(w.y), "f"(w.z), "f"(w.w) : "memory");
-        }
-      }
+      for (int q = 0; q < 16; q += 4)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(base + (tid * S::pitch + c + q) * 4), "r"(v[q]), "r"(v[q + 1]), "r"(v[q + 2]), "r"(v[q + 3]) : "memory");
     }
     tc_fence_before();
   }
-  if (split > 1) {
-    cluster_arrive();
-    cluster_wait();
-    if (warp < 4) {
-      const int rows = 128 / split;
-      for (int e = tid; e < rows * (NP / 4); e += 128) {
-        const int row = rank * rows + e / (NP / 4), r = e % (NP / 4) * 4;
-        if (row >= d.rows || r >= pitch) continue;
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int b = 0; b < split; ++b) {
-          const float4 w = ld_cluster_v4(base + (row * S::pitch + r) * 4, b);
-          v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
-        }
-        v.x = r < R ? v.x * s : 0.0f, v.y = r + 1 < R ? v.y * s : 0.0f;
-        v.z = r + 2 < R ? v.z * s : 0.0f, v.w = r + 3 < R ? v.w * s : 0.0f;
-        *reinterpret_cast<float4*>(u + (int64_t)token_of(p, d, row) * pitch + r) = v;
+  if (tid < 128) row_top[tid] = 0;
+  cluster_arrive();
+  cluster_wait();
+  // The block's share of the tile's rows, a lane to a row and 8 ranks.  fp16: once
+  // for the rows' greatest values, and again.
+  const int rows = 128 / split;
+#pragma unroll
+  for (int pass = H::scaled ? 0 : 1; pass < 2; ++pass) {
+    for (int e = tid; warp < 4 && e < rows * (NP / 8); e += 128) {
+      const int row = rank * rows + e % rows, r = e / rows * 8;
+      if (row >= d.rows) continue;
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+      for (int b = 0; b < split; ++b) {
+        const float4 a = ld_cluster_v4(base + (row * S::pitch + r) * 4, b), z = ld_cluster_v4(base + (row * S::pitch + r + 4) * 4, b);
+        v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w, v[4] += z.x, v[5] += z.y, v[6] += z.z, v[7] += z.w;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = r + k < R ? v[k] * s : 0.0f;  // behind R: rows of F that nobody loaded
+      if (pass == 0) {
+        float m = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) m = fmaxf(m, finite_mag(v[k]));
+        atomicMax(&row_top[row], __float_as_int(m));  // not negative: ordered as integers, whoever comes first
+        continue;
+      }
+      float f = 1.0f;
+      if (H::scaled) {
+        const int x2 = scale_exp(__int_as_float(row_top[row]));
+        f = exp2i(x2);
+        if (r == 0) low.back[(int64_t)tile * 128 + row] = exp2i(-x2);
+      }
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) split16<T>(v[2 * k] * f, v[2 * k + 1] * f, hi[k], lo[k]);
+      uint8_t* to = low.image + (int64_t)tile * (128 * NP * 4);
+      *reinterpret_cast<uint4*>(to + image_offset<NP>(row, r)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      *reinterpret_cast<uint4*>(to + image_offset<NP>(row, NP + r)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      if (low.turned) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) low.turned[((int64_t)tile * NP + r + k) * 128 + row] = v[k];
       }
     }
-    cluster_arrive();
-    cluster_wait();  // no block leaves while others read its sums
+    if (pass == 0) {
+      __syncthreads();
+      if (low.turned && warp == 0) {
+        int m = 0;
+        for (int i = lane_id(); i < rows; i += 32) m = max(m, row_top[rank * rows + i]);
+#pragma unroll
+        for (int i = 16; i; i >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, i));
+        if (tid == 0)
+          for (int i = rank; i < 8; i += split) low.top[(int64_t)tile * 8 + i] = __int_as_float(m);
+      }
+    }
   }
+  cluster_arrive();
+  cluster_wait();  // no block leaves while others read its sums
   __syncthreads();
   if (tid == 0 && failed) *p.status = LQ_ETIMEOUT;
   if (warp == 4) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols));
 }
 
 // ---------------------------------------------------------------------------
-// out = base + u f over one tile and 256 columns.  A warp has 32 columns: its
-// part of F stays in registers as B operands while the tile's 8 groups of 16
-// rows pass.  A lane's 8 values of an output row are neighbours: F's columns are
-// dealt out to the four 8-column operands so (column 8 p + 2 j + e goes to
-// operand j, place 2 p + e), so that base and out move in whole 16-byte pieces
-// between global memory and registers.
+// out = base + u f, a unit of one tile and 128 columns at a time: D [128 tokens
+// x 128] = (hi + lo) [128 x NP] F [NP x 128], F as its rows lie in memory.  A
+// block has a stretch of units.  Rows of base come by bulk copies of 256 bytes
+// into a ring, a row of D is added to the row of base by the thread that has it,
+// in place, and leaves by a bulk copy again: no load or store of base or out
+// passes a warp's load path but the one to and from shared memory, any rows will
+// do, and none that is not the tile's is touched.  Two groups of four warps take
+// turns with the units.
 // ---------------------------------------------------------------------------
+constexpr int kUpThreads = 384;
+constexpr int kUpRow = 256 + 16;  // bytes between rows of base in shared memory: 8 rows' pieces in all banks
 template <int NP>
 struct UpShared {
-  static constexpr int row = 512 + 16;  // bytes of a rank's 256 columns: 8 rows' pieces in all banks
-  static constexpr int off_u = NP * row;
-  static constexpr int bytes = off_u + NP * 512;
+  static constexpr int stages = NP <= 16 ? 5 : NP <= 32 ? 4 : NP <= 64 ? 3 : 2;
+  static constexpr int off_f = 128 * kUpRow;            // of a stage
+  static constexpr int stage = off_f + NP * 256;
+  static constexpr int image = 128 * NP * 4;
+  static constexpr int images = NP <= 64 ? 2 : 1;
+  static constexpr int off_image = stages * stage;
+  static constexpr int bytes = off_image + images * image + 1024;
 };
 
+__device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+}
+
 template <typename T, int NP>
-__global__ void __launch_bounds__(256, NP <= 64 ? 2 : 1)
-    ad_up_kernel(const float* __restrict__ u, int pitch, const T* __restrict__ f, int R, int N, AdPlan p, int L,
-                 const T* base, int64_t base_stride, T* out, int64_t out_stride, int chunks) {
+__global__ void __launch_bounds__(kUpThreads, 1)
+    ad_up_kernel(const Low low, const T* __restrict__ f, int R, int N, AdPlan p, int L, const T* base, int64_t base_stride,
+                 T* out, int64_t out_stride, int chunks) {
   using S = UpShared<NP>;
   using H = Half16<T>;
-  extern __shared__ __align__(16) uint8_t raw[];
-  __shared__ int64_t tok[kAdTile];
-  __shared__ float back[kAdTile];
+  constexpr int NS = S::stages, NI = S::images;
+  extern __shared__ uint8_t raw[];
+  // f_full: F is there; b_full: base is; empty: a stage was read out; i_full / i_empty: the images
+  __shared__ uint64_t f_full[NS], b_full[NS], empty[NS], i_full[NI], i_empty[NI], d_full[2], d_empty[2], drain;
+  __shared__ uint32_t tmem_at;
+  __shared__ int failed;
   pdl_wait();
   pdl_trigger();
-  const int tile = blockIdx.x / chunks, col0 = (blockIdx.x - tile * chunks) * 256;
-  if (tile >= p.tile_of[L + 1]) return;
-  const AdTile d = p.tiles[tile];
-  if (d.owner < 0 && base == out) return;  // nothing changes
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
-  if (tid < kAdTile) tok[tid] = tid < d.rows ? token_of(p, d, tid) : -1;
-  const uint32_t at = smem_u32(raw);
-  if (d.owner >= 0) {
-    // F: 64 bytes of a row at a time, as a 4 x 4 transpose of words
-    for (int e = tid; e < NP * 8; e += 256) {
-      const int r = e >> 3, q = e & 7;
-      uint32_t w[4][4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int col = col0 + q * 32 + i * 8;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (r < R && col < N) v = __ldg(reinterpret_cast<const uint4*>(f + ((int64_t)d.owner * R + r) * N + col));
-        w[i][0] = v.x, w[i][1] = v.y, w[i][2] = v.z, w[i][3] = v.w;
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + r * S::row + q * 64 + j * 16), "r"(w[0][j]), "r"(w[1][j]), "r"(w[2][j]), "r"(w[3][j]) : "memory");
-    }
+  // tokens without an adapter: nothing to do where out is base
+  const int64_t units = (int64_t)p.tile_of[base == out ? L : L + 1] * chunks;
+  const int64_t u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
+  const int n = (int)(u1 - u0);
+  if (n == 0) return;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t at = (smem_u32(raw) + 1023) & ~1023u;
+  if (tid == 0) {
+    for (int i = 0; i < NS; ++i) mbar_init(&f_full[i], 64), mbar_init(&b_full[i], 1), mbar_init(&empty[i], 128);
+    for (int i = 0; i < NI; ++i) mbar_init(&i_full[i], 1), mbar_init(&i_empty[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_empty[i], 128);
+    mbar_init(&drain, 1);
+    failed = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    proxy_fence();
   }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_at)), "r"(256u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
   __syncthreads();
-  if (d.owner >= 0) {
-    // u: warp w makes the A operands of rows 16 w .. 16 w + 15
-    const int64_t t0 = tok[16 * warp + g], t1 = tok[16 * warp + g + 8];
-    float v[NP / 16][8];
-    float m0 = 0.0f, m1 = 0.0f;
-#pragma unroll
-    for (int k = 0; k < NP / 16; ++k) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = 16 * k + 8 * h + 2 * c;
-        const float2 a = t0 >= 0 && r < pitch ? *reinterpret_cast<const float2*>(u + t0 * pitch + r) : make_float2(0.0f, 0.0f);
-        const float2 b = t1 >= 0 && r < pitch ? *reinterpret_cast<const float2*>(u + t1 * pitch + r) : make_float2(0.0f, 0.0f);
-        v[k][4 * h] = a.x, v[k][4 * h + 1] = a.y, v[k][4 * h + 2] = b.x, v[k][4 * h + 3] = b.y;
-        if (H::scaled) {
-          m0 = fmaxf(m0, fmaxf(finite_mag(a.x), finite_mag(a.y)));
-          m1 = fmaxf(m1, fmaxf(finite_mag(b.x), finite_mag(b.y)));
-        }
+  tc_fence_after();
+  const uint32_t tmem = tmem_at;
+  volatile int* fail = &failed;
+  int tile = (int)(u0 / chunks), chunk = (int)(u0 - (int64_t)tile * chunks);
+  if (warp < 8) {
+    // ---- add and send out: a thread to a row ----
+    const int e = warp >> 2, row = (warp & 3) * 32 + lane;
+    AdTile d = {};
+    T* to = nullptr;
+    float back = 1.0f;
+    int known = -1;
+    for (int i = 0; i < n; ++i, ++chunk) {
+      if (chunk == chunks) chunk = 0, ++tile;
+      if ((i & 1) != e) continue;
+      const int slot = i % NS;
+      if (tile != known) {
+        d = p.tiles[tile];
+        to = row < d.rows ? out + (int64_t)token_of(p, d, row) * out_stride : nullptr;
+        if (H::scaled) back = d.owner >= 0 && row < d.rows ? low.back[(int64_t)tile * 128 + row] : 1.0f;
+        known = tile;
       }
-    }
-    float f0 = 1.0f, f1 = 1.0f;
-    if (H::scaled) {
-#pragma unroll
-      for (int i = 1; i < 4; i <<= 1) {
-        m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, i));
-        m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, i));
-      }
-      const int e0 = scale_exp(m0), e1 = scale_exp(m1);
-      f0 = exp2i(e0), f1 = exp2i(e1);
-      if (c == 0) back[16 * warp + g] = exp2i(-e0), back[16 * warp + g + 8] = exp2i(-e1);
-    }
-#pragma unroll
-    for (int k = 0; k < NP / 16; ++k) {
-      uint4 hi, lo;
-      split<T>(v[k][0] * f0, v[k][1] * f0, hi.x, lo.x);
-      split<T>(v[k][2] * f1, v[k][3] * f1, hi.y, lo.y);
-      split<T>(v[k][4] * f0, v[k][5] * f0, hi.z, lo.z);
-      split<T>(v[k][6] * f1, v[k][7] * f1, hi.w, lo.w);
-      uint4* to = reinterpret_cast<uint4*>(raw + S::off_u) + ((warp * (NP / 16) + k) * 2) * 32 + lane;
-      to[0] = hi, to[32] = lo;
-    }
-  }
-  __syncthreads();
-  const int col = col0 + warp * 32 + c * 8;
-  if (col0 + warp * 32 >= N) return;
-  const bool in = col < N;
-  uint32_t b[NP / 16][8];
-  if (d.owner >= 0) {
-#pragma unroll
-    for (int k = 0; k < NP / 16; ++k)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        // lanes 0..15: the 16 ranks of operand 2 h, lanes 16..31: of operand 2 h + 1
-        const uint32_t a = at + (16 * k + (lane & 15)) * S::row + warp * 64 + (2 * h + (lane >> 4)) * 16;
-        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(b[k][4 * h]), "=r"(b[k][4 * h + 1]), "=r"(b[k][4 * h + 2]), "=r"(b[k][4 * h + 3])
-                     : "r"(a));
-      }
-  }
-  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-  constexpr int AHEAD = 4;  // groups of 16 rows whose base is on its way
-  uint4 y[AHEAD][2];
-  auto fetch = [&](int mt) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int64_t t = tok[16 * mt + 8 * h + g];
-      y[mt % AHEAD][h] = base && in && t >= 0 ? *reinterpret_cast<const uint4*>(base + t * base_stride + col) : zero;
-    }
-  };
-#pragma unroll
-  for (int mt = 0; mt < AHEAD; ++mt) fetch(mt);
-#pragma unroll
-  for (int mt = 0; mt < 8; ++mt) {
-    if (16 * mt >= d.rows) break;
-    float acc[4][4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[j][e] = 0.0f;
-    if (d.owner >= 0) {
-      const uint4* from = reinterpret_cast<const uint4*>(raw + S::off_u) + mt * (NP / 16) * 64 + lane;
-#pragma unroll
-      for (int k = 0; k < NP / 16; ++k) {
-        const uint4 hi = from[64 * k], lo = from[64 * k + 32];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          H::mma(acc[j], lo, b[k][2 * j], b[k][2 * j + 1]);
-          H::mma(acc[j], hi, b[k][2 * j], b[k][2 * j + 1]);
-        }
-      }
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int row = 16 * mt + 8 * h + g;
-      const int64_t t = tok[row];
-      const float w = H::scaled && d.owner >= 0 ? back[row] : 1.0f;
-      const uint4 z = y[mt % AHEAD][h];
-      uint32_t o[4] = {z.x, z.y, z.z, z.w};
+      if (!mbar_wait(&b_full[slot], (i / NS) & 1) || !mbar_wait(&d_full[e], (i >> 1) & 1)) *fail = 1;
+      if (*fail) break;
+      __syncwarp();
+      tc_fence_after();
+      const uint32_t mine = at + slot * S::stage + row * kUpRow;
+      const int width = min(128, N - chunk * 128);
       if (d.owner >= 0) {
+#pragma unroll 1
+        for (int c = 0; c < width; c += 32) {
+          uint32_t v[32];
+          tmem_ld32(tmem + ((uint32_t)(warp & 3) << 21) + e * 128 + c, v);
+          uint4 y[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 q = H::unpack(o[j]);
-          o[j] = H::scaled ? H::pack(fmaf(acc[j][2 * h], w, q.x), fmaf(acc[j][2 * h + 1], w, q.y))
-                           : H::pack(q.x + acc[j][2 * h], q.y + acc[j][2 * h + 1]);
+          for (int q = 0; q < 4; ++q) y[q] = base ? lds_v4(mine + (c + 8 * q) * 2) : make_uint4(0u, 0u, 0u, 0u);
+          tmem_wait_ld32(v);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t o[4] = {y[q].x, y[q].y, y[q].z, y[q].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 b = H::unpack(o[k]);
+              const float v0 = __uint_as_float(v[8 * q + 2 * k]), v1 = __uint_as_float(v[8 * q + 2 * k + 1]);
+              o[k] = H::scaled ? H::pack(fmaf(v0, back, b.x), fmaf(v1, back, b.y)) : H::pack(b.x + v0, b.y + v1);
+            }
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + (c + 8 * q) * 2), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
+          }
+        }
+      } else if (!base) {
+        for (int c = 0; c < width; c += 8)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(mine + c * 2), "r"(0u) : "memory");
+      }
+      tc_fence_before();
+      mbar_arrive(&d_empty[e]);
+      proxy_fence();
+      if (to) bulk_store(to + chunk * 128, mine, width * 2);
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      mbar_arrive(&empty[slot]);
+    }
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  } else if (warp == 8) {
+    // ---- rows of base, and images ----
+    AdTile d = {};
+    int known = -1, images = 0, done = 0;
+    int64_t tok[4];
+    for (int i = 0; i < n; ++i, ++chunk) {
+      if (chunk == chunks) chunk = 0, ++tile;
+      const int slot = i % NS;
+      const bool fresh = tile != known;
+      if (fresh) {
+        d = p.tiles[tile];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) tok[k] = lane + 32 * k < d.rows ? token_of(p, d, lane + 32 * k) : -1;
+        known = tile;
+      }
+      if (i >= NS && !wait_warp(&empty[slot], (i / NS - 1) & 1)) *fail = 1;
+      if (*fail) break;
+      const uint32_t bytes = min(128, N - chunk * 128) * 2;
+      if (lane == 0) {
+        if (base) mbar_expect_tx(&b_full[slot], bytes * d.rows);
+        else mbar_arrive(&b_full[slot]);
+      }
+      __syncwarp();
+      if (base) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (tok[k] >= 0)
+            bulk_load_at(at + slot * S::stage + (lane + 32 * k) * kUpRow, base + tok[k] * base_stride + chunk * 128, bytes, &b_full[slot]);
+      }
+      done = i + 1;
+      if (fresh && d.owner >= 0) {
+        const int b = images % NI;
+        if (images >= NI && !wait_warp(&i_empty[b], (images / NI - 1) & 1)) *fail = 1;
+        if (*fail) break;
+        if (lane == 0) {
+          mbar_expect_tx(&i_full[b], S::image);
+          bulk_load_at(at + S::off_image + b * S::image, low.image + (int64_t)tile * S::image, S::image, &i_full[b]);
+        }
+        ++images;
+      }
+    }
+    if (*fail) {  // what was sent for arrives before its memory goes
+      for (int i = max(0, done - NS); i < done; ++i) wait_warp(&b_full[i % NS], (i / NS) & 1);
+      for (int i = max(0, images - NI); i < images; ++i) wait_warp(&i_full[i % NI], (i / NI) & 1);
+    }
+  } else if (warp == 9) {
+    // ---- products ----
+    constexpr uint32_t idesc = make_idesc(H::fmt, 128) | kMajorB;
+    int known = -1, images = 0, b = 0;
+    bool some = false;
+    for (int i = 0; i < n; ++i, ++chunk) {
+      if (chunk == chunks) chunk = 0, ++tile;
+      const int slot = i % NS, e = i & 1;
+      if (tile != known) {
+        some = p.tiles[tile].owner >= 0;
+        known = tile;
+        if (some) {
+          b = images % NI;
+          if (!wait_warp(&i_full[b], (images / NI) & 1)) *fail = 1;
+          ++images;
         }
       }
-      if (in && t >= 0) *reinterpret_cast<uint4*>(out + t * out_stride + col) = make_uint4(o[0], o[1], o[2], o[3]);
+      if (!wait_warp(&f_full[slot], (i / NS) & 1) || (i >= 2 && !wait_warp(&d_empty[e], ((i >> 1) - 1) & 1))) *fail = 1;
+      if (*fail) break;
+      tc_fence_after();
+      if (some) {
+        const uint32_t im = at + S::off_image + b * S::image;
+        const uint64_t df = sw128_mn_desc(at + slot * S::stage + S::off_f, NP * 128);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int k = 0; k < NP / 16; ++k) {
+            const int v = h * NP + 16 * k;  // value of the image's row
+            const uint64_t da = NP == 16 ? sw64_desc(im + v * 2) : sw128_desc(im + (v >> 6) * 16384 + (v & 63) * 2);
+            mma_ss(tmem + e * 128, da, df + 128 * k, idesc, (h | k) > 0);
+          }
+        commit(&d_full[e]);
+        if (i + 1 == n || chunk + 1 == chunks) commit(&i_empty[b]);
+      } else if (lane == 0) {
+        mbar_arrive(&d_full[e]);
+      }
+      __syncwarp();
     }
-    if (mt + AHEAD < 8) fetch(mt + AHEAD);
+    if (*fail) {
+      commit(&drain);
+      wait_warp(&drain, 0);
+    }
+  } else {
+    // ---- F: 128 columns of the adapter's rows ----
+    const int t = tid - 320, c = t & 15, r0 = t >> 4;
+    int known = -1, owner = -1;
+    for (int i = 0; i < n; ++i, ++chunk) {
+      if (chunk == chunks) chunk = 0, ++tile;
+      const int slot = i % NS;
+      if (tile != known) owner = p.tiles[tile].owner, known = tile;
+      if (i >= NS && !mbar_wait(&empty[slot], (i / NS - 1) & 1)) *fail = 1;
+      if (*fail) break;
+      if (owner >= 0) {
+        const bool in = chunk * 128 + c * 8 < N;
+        const T* from = f + (int64_t)owner * R * N + (in ? chunk * 128 + c * 8 : 0);
+        const uint32_t to = at + slot * S::stage + S::off_f + (c >> 3) * (NP * 128);
+#pragma unroll 8
+        for (int r = r0; r < NP; r += 4)  // zeros behind the rank: they meet zeros of the image
+          cp16(to + r * 128 + (((c & 7) ^ (r & 7)) << 4), from + (int64_t)min(r, R - 1) * N, in && r < R);
+      }
+      cp_commit();
+      cp_wait<0>();
+      proxy_fence();
+      mbar_arrive(&f_full[slot]);
+    }
   }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (tid == 0 && failed) *p.status = LQ_ETIMEOUT;
+  if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u));
 }
 
 // ---------------------------------------------------------------------------
@@ -444,7 +585,7 @@ __device__ __forceinline__ bool any_loader(int fail) {
 // One of the two problems of a launch: (v, x, dA) and (u, dy, dB).
 template <typename T>
 struct OuterSide {
-  const float* v;
+  Low v;
   const T* x;
   int64_t stride;
   int K, chunks;
@@ -454,16 +595,15 @@ struct OuterSide {
 
 template <typename T, int NP, typename G>
 __global__ void __launch_bounds__(kOuterLoaders + 32, OuterShared<NP>::blocks)
-    ad_outer_kernel(const OuterSide<T> one, const OuterSide<T> two, int R, int pitch, AdPlan p, int L) {
+    ad_outer_kernel(const OuterSide<T> one, const OuterSide<T> two, int R, AdPlan p, int L) {
   using S = OuterShared<NP>;
   using H = Half16<T>;
-  constexpr int NS = S::stages, LAG = NS - 2, VI = NP * 8 / kOuterLoaders > 0 ? NP * 8 / kOuterLoaders : 1;
+  constexpr int NS = S::stages, LAG = NS - 2, VI = NP / 16;  // 8 tokens of a rank, of a lane that brings V
   constexpr uint32_t kCols = 4 * NP;  // two tiles of 128 columns, hi and lo
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t full[NS], empty[NS], done, free_, drain;
   __shared__ uint32_t tmem_at;
   __shared__ int failed;
-  __shared__ float top[kOuterLoaders / 32];
   pdl_wait();
   pdl_trigger();
   const bool first_side = (int)blockIdx.x < one.chunks;
@@ -494,78 +634,87 @@ __global__ void __launch_bounds__(kOuterLoaders + 32, OuterShared<NP>::blocks)
   volatile int* fail = &failed;
   int step = 0, run = 0;  // 64-token steps and runs so far: the barriers' phases
   if (warp < kOuterLoaders / 32) {
-    const int c = tid & 15, r0 = tid >> 4;
-    const int col = col0;
-    const uint32_t at = base + r0 * 128 + (((c & 7) ^ (r0 & 7)) << 4) + (c >> 3) * 8192;
-    const bool c0 = col + c * 8 < q.K, c1 = col + 128 + c * 8 < q.K;
+    // warps 0 .. 3 bring X, a row of 512 bytes at a time; warps 4 .. 7 V
+    const bool brings_x = warp < 4;
+    const uint32_t at = base + (lane >> 3) * 8192;
+    const bool in = col0 + lane * 8 < q.K;
     for (int t0 = t_lo; !any_loader(*fail) && t0 < t_hi; ++run) {
       const int owner = p.tiles[t0].owner;
       const int first = p.tiles[t0].first, last = min(p.tile_of[owner + 1], t_hi) - 1;
       const int rows = p.tiles[last].first + p.tiles[last].rows - first;  // of the whole run, one behind the other in `order`
       float f = 1.0f, back = 1.0f;
-      if (H::scaled) {
-        // fp16: the run's greatest value of v
+      if (H::scaled) {  // fp16: by the run's greatest value of v
         float m = 0.0f;
-        for (int e = tid; e < rows * (pitch / 4); e += kOuterLoaders) {
-          const int row = e / (pitch / 4);
-          const float4 w = *reinterpret_cast<const float4*>(q.v + (int64_t)p.order[first + row] * pitch + (e - row * (pitch / 4)) * 4);
-          m = fmaxf(m, fmaxf(fmaxf(finite_mag(w.x), finite_mag(w.y)), fmaxf(finite_mag(w.z), finite_mag(w.w))));
-        }
+        for (int e = lane; e < (last - t0 + 1) * 8; e += 32) m = fmaxf(m, q.v.top[(int64_t)t0 * 8 + e]);
 #pragma unroll
         for (int i = 16; i; i >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i));
-        if (lane == 0) top[warp] = m;
-        asm volatile("bar.sync 1, %0;" ::"n"(kOuterLoaders) : "memory");
-        for (int i = 0; i < kOuterLoaders / 32; ++i) m = fmaxf(m, top[i]);
-        asm volatile("bar.sync 1, %0;" ::"n"(kOuterLoaders) : "memory");
         const int e = scale_exp(m);
         f = exp2i(e), back = exp2i(-e);
       }
       const int n = (rows + 63) / 64;
-      float v[VI][8];
-      // the next step's part of V: 8 tokens of one rank to a lane
-      auto fetch = [&](int i) {
+      if (brings_x) {
+        // lane k has the token of the warp's k-th row of the next step
+        auto token = [&](int i) {
+          const int row = i * 64 + warp + 4 * lane;
+          return lane < 16 && row < rows ? p.order[first + row] : -1;
+        };
+        int next = token(0);
+        for (int i = 0; i < n + LAG; ++i) {
+          if (i < n) {
+            const int slot = (step + i) % NS, now = next;
+            if (i + 1 < n) next = token(i + 1);
+            if (step + i >= NS && !mbar_wait(&empty[slot], ((step + i) / NS - 1) & 1)) *fail = 1;
+            if (*fail) break;
+            __syncwarp();
+            const uint32_t to = at + slot * S::stage;
 #pragma unroll
-        for (int j = 0; j < VI; ++j) {
-          const int e = tid + j * kOuterLoaders, r = e % NP, tk = i * 64 + e / NP * 8;
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            v[j][k] = e < NP * 8 && r < R && tk + k < rows ? q.v[(int64_t)p.order[first + tk + k] * pitch + r] : 0.0f;
+            for (int j = 0; j < 16; ++j) {
+              const int row = warp + 4 * j, tok = __shfl_sync(0xffffffffu, now, j);
+              const bool some = in && tok >= 0;  // behind the run: zeros in both factors
+              cp16(to + row * 128 + (((lane & 7) ^ (row & 7)) << 4), some ? q.x + (int64_t)tok * q.stride + col0 + lane * 8 : q.x, some);
+            }
+          }
+          cp_commit();
+          if (i >= LAG) {
+            cp_wait<LAG>();
+            proxy_fence();
+            mbar_arrive(&full[(step + i - LAG) % NS]);
+          }
         }
-      };
-      fetch(0);
-      for (int i = 0; i < n + LAG; ++i) {
-        if (i < n) {
+      } else {
+        const int id = tid - 128, k8 = id & 7, r0 = id >> 3;
+        float v[VI][8];
+        auto fetch = [&](int i) {
+          const float* from = q.v.turned + (int64_t)(t0 + (i >> 1)) * NP * 128 + (i & 1) * 64 + k8 * 8;
+          const int left = rows - i * 64 - k8 * 8;  // of the 8 tokens; nobody wrote those behind the run
+#pragma unroll
+          for (int j = 0; j < VI; ++j) {
+            float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f), b = a;
+            if (left > 0) a = *reinterpret_cast<const float4*>(from + (r0 + 16 * j) * 128);
+            if (left > 4) b = *reinterpret_cast<const float4*>(from + (r0 + 16 * j) * 128 + 4);
+            v[j][0] = a.x, v[j][1] = left > 1 ? a.y : 0.0f, v[j][2] = left > 2 ? a.z : 0.0f, v[j][3] = left > 3 ? a.w : 0.0f;
+            v[j][4] = b.x, v[j][5] = left > 5 ? b.y : 0.0f, v[j][6] = left > 6 ? b.z : 0.0f, v[j][7] = left > 7 ? b.w : 0.0f;
+          }
+        };
+        fetch(0);
+        for (int i = 0; i < n; ++i) {
           const int slot = (step + i) % NS;
           if (step + i >= NS && !mbar_wait(&empty[slot], ((step + i) / NS - 1) & 1)) *fail = 1;
           if (*fail) break;
-          const uint32_t to = at + slot * S::stage;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int row = i * 64 + r0 + 16 * j;
-            const bool some = row < rows;  // behind the run: zeros in both factors
-            const T* from = q.x + (some ? (int64_t)p.order[first + row] * q.stride : 0);
-            cp16(to + j * 2048, c0 ? from + col + c * 8 : q.x, some && c0);
-            cp16(to + j * 2048 + 16384, c1 ? from + col + 128 + c * 8 : q.x, some && c1);
-          }
           const uint32_t vt = base + slot * S::stage + S::off_v;
 #pragma unroll
           for (int j = 0; j < VI; ++j) {
-            const int e = tid + j * kOuterLoaders, r = e % NP, k8 = e / NP;
-            if (e >= NP * 8) continue;
+            const int r = r0 + 16 * j;
             uint32_t hi[4], lo[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) split<T>(v[j][2 * k] * f, v[j][2 * k + 1] * f, hi[k], lo[k]);
+            for (int k = 0; k < 4; ++k) split16<T>(v[j][2 * k] * f, v[j][2 * k + 1] * f, hi[k], lo[k]);
             const uint32_t a = vt + r * 128 + ((k8 ^ (r & 7)) << 4);
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a + NP * 128), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
           }
           if (i + 1 < n) fetch(i + 1);
-        }
-        cp_commit();
-        if (i >= LAG) {
-          cp_wait<LAG>();
           proxy_fence();
-          mbar_arrive(&full[(step + i - LAG) % NS]);
+          mbar_arrive(&full[slot]);
         }
       }
       step += n;
@@ -685,7 +834,7 @@ int more_shared(int bytes) {
 }
 
 template <typename T, int NP>
-int down_np(const AdCall& a, const void* x, int64_t stride, bool is_a, float* u) {
+int down_np(const AdCall& a, const void* x, int64_t stride, bool is_a, void* low, bool turned) {
   using S = DownShared<NP>;
   const lq_adapter_bank& b = *a.bank;
   const int K = (int)(is_a ? b.K : b.N), steps = (K + 63) / 64;
@@ -708,23 +857,22 @@ int down_np(const AdCall& a, const void* x, int64_t stride, bool is_a, float* u)
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, static_cast<const T*>(x), stride, static_cast<const T*>(is_a ? b.a : b.b),
-                                           b.scaling, (int)b.R, ad_pitch(b.R), K, a.plan, (int)b.L, u, split);
+                                           b.scaling, (int)b.R, K, a.plan, (int)b.L, low_at<NP>(low, tiles, turned), split);
   LQ_REQUIRE(e == cudaSuccess, LQ_ECUDA, "ad_down_kernel launch: %s", cudaGetErrorString(e));
   return launched("ad_down_kernel");
 }
 
 template <typename T, int NP>
-int up_np(const AdCall& a, const float* u, bool is_a, const void* base, int64_t bs, void* out, int64_t os) {
+int up_np(const AdCall& a, void* low, bool is_a, const void* base, int64_t bs, void* out, int64_t os) {
   using S = UpShared<NP>;
   const lq_adapter_bank& b = *a.bank;
-  const int N = (int)(is_a ? b.K : b.N), chunks = (N + 255) / 256;
-  const int64_t grid = ad_max_tiles(a.n, b.L) * chunks;
-  LQ_REQUIRE(grid < (1LL << 31), LQ_ERANGE, "adapters: too many tokens for %d features", N);
+  const int N = (int)(is_a ? b.K : b.N), chunks = (N + 127) / 128;
+  const int64_t tiles = ad_max_tiles(a.n, b.L), units = tiles * chunks;
   constexpr auto kern = ad_up_kernel<T, NP>;
   LQ_TRY(more_shared<kern>(S::bytes));
-  const cudaError_t e = launch_pdl(kern, dim3((unsigned)grid), dim3(256), S::bytes, a.st, u, ad_pitch(b.R),
-                                   static_cast<const T*>(is_a ? b.a : b.b), (int)b.R, N, a.plan, (int)b.L,
-                                   static_cast<const T*>(base), bs, static_cast<T*>(out), os, chunks);
+  const cudaError_t e = launch_pdl(kern, dim3((unsigned)(units < num_sms() ? units : num_sms())), dim3(kUpThreads), S::bytes, a.st,
+                                   low_at<NP>(low, tiles, false), static_cast<const T*>(is_a ? b.a : b.b), (int)b.R, N, a.plan,
+                                   (int)b.L, static_cast<const T*>(base), bs, static_cast<T*>(out), os, chunks);
   LQ_REQUIRE(e == cudaSuccess, LQ_ECUDA, "ad_up_kernel launch: %s", cudaGetErrorString(e));
   return launched("ad_up_kernel");
 }
@@ -733,14 +881,15 @@ template <typename T, int NP, typename G>
 int outer_np(const AdCall& a, const AdOuter& o) {
   using S = OuterShared<NP>;
   const lq_adapter_bank& b = *a.bank;
-  const int64_t groups = ad_outer_groups(b, a.n);
+  const int64_t groups = ad_outer_groups(b, a.n), tiles = ad_max_tiles(a.n, b.L);
   OuterSide<T> one = {}, two = {};
-  if (o.da) one = {o.v, static_cast<const T*>(o.x), o.x_stride, (int)b.K, (int)(b.K + 255) / 256, o.da, o.part};
-  if (o.db) two = {o.u, static_cast<const T*>(o.dy), o.dy_stride, (int)b.N, (int)(b.N + 255) / 256, o.db, o.part + 2 * groups * b.R * b.K};
+  if (o.da) one = {low_at<NP>(o.v, tiles, true), static_cast<const T*>(o.x), o.x_stride, (int)b.K, (int)(b.K + 255) / 256, o.da, o.part};
+  if (o.db) two = {low_at<NP>(o.u, tiles, true), static_cast<const T*>(o.dy), o.dy_stride, (int)b.N, (int)(b.N + 255) / 256, o.db,
+                   o.part + 2 * groups * b.R * b.K};
   constexpr auto kern = ad_outer_kernel<T, NP, G>;
   LQ_TRY(more_shared<kern>(S::bytes));
   cudaError_t e = launch_pdl(kern, dim3((unsigned)(one.chunks + two.chunks), (unsigned)groups), dim3(kOuterLoaders + 32), S::bytes,
-                             a.st, one, two, (int)b.R, ad_pitch(b.R), a.plan, (int)b.L);
+                             a.st, one, two, (int)b.R, a.plan, (int)b.L);
   LQ_REQUIRE(e == cudaSuccess, LQ_ECUDA, "ad_outer_kernel launch: %s", cudaGetErrorString(e));
   LQ_TRY(launched("ad_outer_kernel"));
   const int64_t b1 = o.da ? (b.R * b.K + 2047) / 2048 : 0, b2 = o.db ? (b.R * b.N + 2047) / 2048 : 0;
@@ -751,47 +900,49 @@ int outer_np(const AdCall& a, const AdOuter& o) {
 }
 
 // NP: the rank, rounded up to what the kernels are made for
-#define AD_BY_RANK(call)                          \
-  const int64_t r = a.bank->R;                    \
-  if (r <= 16) return call(16);                   \
-  if (r <= 32) return call(32);                   \
-  if (r <= 64) return call(64);                   \
-  return call(128)
+#define AD_BY_RANK(rank, call)                  \
+  (ad_padded(rank) == 16   ? call(16)           \
+   : ad_padded(rank) == 32 ? call(32)           \
+   : ad_padded(rank) == 64 ? call(64)           \
+                           : call(128))
 
 template <typename T>
-int down_t(const AdCall& a, const void* x, int64_t stride, bool is_a, float* u) {
-#define AD_CALL(np) (down_np<T, np>(a, x, stride, is_a, u))
-  AD_BY_RANK(AD_CALL);
+int down_t(const AdCall& a, const void* x, int64_t stride, bool is_a, void* low, bool turned) {
+#define AD_CALL(np) (down_np<T, np>(a, x, stride, is_a, low, turned))
+  return AD_BY_RANK(a.bank->R, AD_CALL);
 #undef AD_CALL
 }
 template <typename T>
-int up_t(const AdCall& a, const float* u, bool is_a, const void* base, int64_t bs, void* out, int64_t os) {
-#define AD_CALL(np) (up_np<T, np>(a, u, is_a, base, bs, out, os))
-  AD_BY_RANK(AD_CALL);
+int up_t(const AdCall& a, void* low, bool is_a, const void* base, int64_t bs, void* out, int64_t os) {
+#define AD_CALL(np) (up_np<T, np>(a, low, is_a, base, bs, out, os))
+  return AD_BY_RANK(a.bank->R, AD_CALL);
 #undef AD_CALL
 }
-template <typename T>
+template <typename T, typename G>
 int outer_t(const AdCall& a, const AdOuter& o) {
-  if (o.grad_dtype == LQ_F32) {
-#define AD_CALL(np) (outer_np<T, np, float>(a, o))
-    AD_BY_RANK(AD_CALL);
-#undef AD_CALL
-  }
-#define AD_CALL(np) (outer_np<T, np, T>(a, o))
-  AD_BY_RANK(AD_CALL);
+#define AD_CALL(np) (outer_np<T, np, G>(a, o))
+  return AD_BY_RANK(a.bank->R, AD_CALL);
 #undef AD_CALL
 }
 
 }  // namespace
 
-int ad_down(const AdCall& a, const void* x, int64_t stride, bool is_a, float* u) {
-  return a.bank->dtype == LQ_F16 ? down_t<__half>(a, x, stride, is_a, u) : down_t<__nv_bfloat16>(a, x, stride, is_a, u);
+size_t ad_low_bytes(const lq_adapter_bank& b, int64_t n, bool turned) {
+  const int np = ad_padded(b.R);
+  return (size_t)ad_max_tiles(n, b.L) * (128 * np * 4 + 128 * 4 + 8 * 4 + (turned ? 128 * np * 4 : 0));
 }
-int ad_up(const AdCall& a, const float* u, bool is_a, const void* base, int64_t bs, void* out, int64_t os) {
-  return a.bank->dtype == LQ_F16 ? up_t<__half>(a, u, is_a, base, bs, out, os) : up_t<__nv_bfloat16>(a, u, is_a, base, bs, out, os);
+int ad_down(const AdCall& a, const void* x, int64_t stride, bool is_a, void* low, bool turned) {
+  return a.bank->dtype == LQ_F16 ? down_t<__half>(a, x, stride, is_a, low, turned)
+                                 : down_t<__nv_bfloat16>(a, x, stride, is_a, low, turned);
+}
+int ad_up(const AdCall& a, void* low, bool is_a, const void* base, int64_t bs, void* out, int64_t os) {
+  return a.bank->dtype == LQ_F16 ? up_t<__half>(a, low, is_a, base, bs, out, os)
+                                 : up_t<__nv_bfloat16>(a, low, is_a, base, bs, out, os);
 }
 int ad_outer(const AdCall& a, const AdOuter& o) {
-  return a.bank->dtype == LQ_F16 ? outer_t<__half>(a, o) : outer_t<__nv_bfloat16>(a, o);
+  if (o.grad_dtype == LQ_F32)
+    return a.bank->dtype == LQ_F16 ? outer_t<__half, float>(a, o) : outer_t<__nv_bfloat16, float>(a, o);
+  return a.bank->dtype == LQ_F16 ? outer_t<__half, __half>(a, o) : outer_t<__nv_bfloat16, __nv_bfloat16>(a, o);
 }
 
 }  // namespace lq

@@ -138,7 +138,17 @@ __device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t saddr, uint32_t panel
   d |= (uint64_t)2 << 61;
   return d;
 }
-constexpr uint32_t kMajorA = 1u << 15;  // instruction descriptor: A's tile is such a one
+constexpr uint32_t kMajorA = 1u << 15, kMajorB = 1u << 16;  // instruction descriptor: A's (B's) tile is such a one
+// A K-major tile with rows of 64 bytes and the 64-byte swizzle.
+__device__ __forceinline__ uint64_t sw64_desc(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr & 0x3FFFF) >> 4);
+  d |= (uint64_t)1 << 16;
+  d |= (uint64_t)(512 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)4 << 61;  // SWIZZLE_64B
+  return d;
+}
 
 // kind::f16 instruction descriptor: D fp32, A/B fp16 (fmt 0) or bf16 (fmt 1),
 // both K-major, M = 128, N = BT.

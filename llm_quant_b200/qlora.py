@@ -309,7 +309,8 @@ class QLoRALinear(nn.Module):
         if (adapters.in_features, adapters.out_features) != (self.in_features, self.out_features):
             raise ValueError(f"QLoRALinear.forward: adapters of {adapters.in_features} to {adapters.out_features} features "
                              f"beside {self.in_features} to {self.out_features}")
-        adapters._check(x, batch, None)
+        if x.dtype not in (torch.float16, torch.bfloat16):
+            raise TypeError(f"QLoRALinear.forward: adapters take float16 or bfloat16 activations, not {x.dtype}")
         if nf4_linear.eligible(self, x):
             base = nf4_linear.base_linear(self, x)
         else:

@@ -24,36 +24,48 @@ def _bank(**kw):
     return ctypes.byref(_C.AdapterBank(*[f[n] for n, _ in _C.AdapterBank._fields_]))
 
 
+def _form(n=4, x_stride=64, base_stride=0, out_stride=128, keep=0):
+    from llm_quant_b200 import _C
+    return ctypes.byref(_C.AdapterForm(n, x_stride, base_stride, out_stride, keep))
+
+
 BAD = [({"a": None}, -1, "NULL"), ({"scaling": None}, -1, "NULL"), ({"dtype": 0}, -2, "fp16 or bf16"), ({"L": 0}, -6, "adapters"),
        ({"L": 8193}, -6, "adapters"), ({"R": 0}, -6, "rank"), ({"R": 129}, -6, "rank"), ({"K": 68}, -5, "multiples of 8"),
        ({"N": 4}, -6, "features"), ({"N": (1 << 22) + 8}, -6, "features"), ({"a": 4104}, -5, "aligned")]
+HUGE = 1 << 40
 
 
 @pytest.mark.parametrize("kw,status,word", BAD)
 def test_bad_banks(lib, kw, status, word):
     b = _bank(**kw)
-    for call in (lambda: lib.lq_adapter_forward(b, 4096, 4, 4096, 128, None, 0, 4096, 128, 4096, None),
-                 lambda: lib.lq_adapter_backward(b, 4096, 4, 4096, 128, 4096, 128, 4096, 4096, 4096, 4096, 2, 4096, 1 << 40, None)):
+    for call in (lambda: lib.lq_adapter_forward(b, _form(), 4096, 4096, None, 4096, 4096, HUGE, None),
+                 lambda: lib.lq_adapter_backward(b, _form(keep=1), 4096, 4096, 4096, 4096, HUGE, 4096, 4096, 4096, 2, 4096, HUGE, None)):
         assert call() == status
         assert word.encode() in lib.lq_last_error()
 
 
 def test_bad_calls(lib):
-    def forward(bank=None, plan=4096, n=4, x=4096, xs=64, base=None, bs=0, out=4096, os=128, u=4096):
-        return lib.lq_adapter_forward(bank or _bank(), plan, n, x, xs, base, bs, out, os, u, None)
+    def forward(plan=4096, x=4096, base=None, out=4096, low=4096, nb=HUGE, **form):
+        return lib.lq_adapter_forward(_bank(), _form(**form), plan, x, base, out, low, nb, None)
 
     assert forward(plan=None) == -1 and forward(plan=4104) == -1 and forward(n=-1) == -6 and forward(n=(1 << 24) + 1) == -6
-    assert forward(x=None) == -5 and forward(x=4098) == -5 and forward(xs=68) == -5 and forward(xs=-64) == -1
-    assert forward(out=None) == -5 and forward(os=64) == -1 and forward(base=4104) == -5
-    assert forward(base=4096, bs=136) == -1 and forward(u=None) == -1
-    assert forward(n=0, plan=None, x=None, out=None, u=None) == 0
+    assert forward(x=None) == -5 and forward(x=4098) == -5 and forward(x_stride=68) == -5 and forward(x_stride=-64) == -1
+    assert forward(out=None) == -5 and forward(out_stride=64) == -1 and forward(base=4104) == -5
+    assert forward(base=4096, base_stride=136) == -1
+    for kw in (dict(n=1000), dict(keep=1)):  # calls that leave something in low
+        assert forward(low=None, **kw) == -1 and forward(low=4100, **kw) == -1 and forward(nb=64, **kw) == -1
+    assert forward(n=0, plan=None, x=None, out=None, low=None, nb=0) == 0
+    assert lib.lq_adapter_forward(_bank(), None, 4096, 4096, None, 4096, 4096, HUGE, None) == -1
 
-    def backward(x=4096, dy=4096, ds=128, u=4096, dx=4096, da=4096, db=4096, dt=2, ws=4096, nb=1 << 40):
-        return lib.lq_adapter_backward(_bank(), 4096, 4, x, 64, dy, ds, u, dx, da, db, dt, ws, nb, None)
+    def backward(x=4096, dy=4096, ds=128, low=4096, nl=HUGE, dx=4096, da=4096, db=4096, dt=2, ws=4096, nb=HUGE, keep=1):
+        return lib.lq_adapter_backward(_bank(), _form(out_stride=ds, keep=keep), 4096, x, dy, low, nl, dx, da, db, dt, ws, nb, None)
 
-    assert backward(dt=1) == -2 and backward(dy=None) == -5 and backward(ds=100) == -5 and backward(u=None) == -1
+    assert backward(dt=1) == -2 and backward(dy=None) == -5 and backward(ds=100) == -5 and backward(low=None) == -1
     assert backward(x=None) == -5 and backward(dx=4104) == -5 and backward(ws=None) == -1 and backward(nb=8) == -1
+    assert backward(nl=8) == -1 and backward(keep=0) == -1
     assert lib.lq_adapter_backward_workspace_bytes(None, 4) == 0 and lib.lq_adapter_backward_workspace_bytes(_bank(), -1) == 0
+    assert lib.lq_adapter_low_bytes(None, _form()) == 0 and lib.lq_adapter_low_bytes(_bank(), None) == 0
+    assert lib.lq_adapter_low_bytes(_bank(), _form(n=1000)) < lib.lq_adapter_low_bytes(_bank(), _form(n=1000, keep=1))
 
 
 def test_bad_plans(lib):
