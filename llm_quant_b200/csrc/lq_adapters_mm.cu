@@ -98,6 +98,22 @@ __device__ __forceinline__ int token_of(const AdPlan& p, const AdTile& d, int ro
   return d.run >= 0 ? d.run + row : p.order[d.first + row];
 }
 
+// Whether a wait ran out for any of the `threads` that meet at a named barrier:
+// they leave together, since such a barrier has no limit.
+template <int THREADS>
+__device__ __forceinline__ bool any_failed(int barrier, int fail) {
+  int r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.s32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, %3, %2, p;\n\t"
+      "selp.s32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(fail), "n"(THREADS), "r"(barrier)
+      : "memory");
+  return r != 0;
+}
+
 // ---------------------------------------------------------------------------
 // The low-rank rows of a call (u or v), as ad_down leaves them for each tile:
 //   image  the two 16-bit parts as the K-major operand that ad_up copies into
@@ -308,14 +324,15 @@ __global__ void __launch_bounds__(160, 2) ad_down_kernel(const T* __restrict__ x
 // ---------------------------------------------------------------------------
 // out = base + u f, a unit of one tile and 128 columns at a time: D [128 tokens
 // x 128] = (hi + lo) [128 x NP] F [NP x 128], F as its rows lie in memory.  A
-// block has a stretch of units.  Rows of base come by bulk copies of 256 bytes
-// into a ring, a row of D is added to the row of base by the thread that has it,
-// in place, and leaves by a bulk copy again: no load or store of base or out
-// passes a warp's load path but the one to and from shared memory, any rows will
-// do, and none that is not the tile's is touched.  Two groups of four warps take
-// turns with the units.
+// block has a stretch of units.  Base and F come by cp.async, whole rows of 256
+// bytes to half a warp; the thread that has a row of D adds it to the row of base
+// in shared memory, and half a warp takes each row out again.  (A lane that
+// loads its own part of base, as mma.sync deals D out, touches eight lines of
+// 64 bytes each at a time: L1 was busy 4 cycles of 5.  Bulk copies of a row
+// each took 30 cycles apiece.)  Two groups of four warps take turns with the
+// units, and two teams of two warps with bringing them.
 // ---------------------------------------------------------------------------
-constexpr int kUpThreads = 384;
+constexpr int kUpThreads = 416;
 constexpr int kUpRow = 256 + 16;  // bytes between rows of base in shared memory: 8 rows' pieces in all banks
 template <int NP>
 struct UpShared {
@@ -328,10 +345,6 @@ struct UpShared {
   static constexpr int bytes = off_image + images * image + 1024;
 };
 
-__device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t bytes) {
-  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
-}
-
 template <typename T, int NP>
 __global__ void __launch_bounds__(kUpThreads, 1)
     ad_up_kernel(const Low low, const T* __restrict__ f, int R, int N, AdPlan p, int L, const T* base, int64_t base_stride,
@@ -340,8 +353,8 @@ __global__ void __launch_bounds__(kUpThreads, 1)
   using H = Half16<T>;
   constexpr int NS = S::stages, NI = S::images;
   extern __shared__ uint8_t raw[];
-  // f_full: F is there; b_full: base is; empty: a stage was read out; i_full / i_empty: the images
-  __shared__ uint64_t f_full[NS], b_full[NS], empty[NS], i_full[NI], i_empty[NI], d_full[2], d_empty[2], drain;
+  // full: base and F are there; empty: the unit was taken out; i_full / i_empty: the images
+  __shared__ uint64_t full[NS], empty[NS], i_full[NI], i_empty[NI], d_full[2], d_empty[2], drain;
   __shared__ uint32_t tmem_at;
   __shared__ int failed;
   pdl_wait();
@@ -354,7 +367,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t at = (smem_u32(raw) + 1023) & ~1023u;
   if (tid == 0) {
-    for (int i = 0; i < NS; ++i) mbar_init(&f_full[i], 64), mbar_init(&b_full[i], 1), mbar_init(&empty[i], 128);
+    for (int i = 0; i < NS; ++i) mbar_init(&full[i], 64), mbar_init(&empty[i], 128);
     for (int i = 0; i < NI; ++i) mbar_init(&i_full[i], 1), mbar_init(&i_empty[i], 1);
     for (int i = 0; i < 2; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_empty[i], 128);
     mbar_init(&drain, 1);
@@ -362,7 +375,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     proxy_fence();
   }
-  if (warp == 9) {
+  if (warp == 12) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_at)), "r"(256u));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -373,10 +386,12 @@ __global__ void __launch_bounds__(kUpThreads, 1)
   volatile int* fail = &failed;
   int tile = (int)(u0 / chunks), chunk = (int)(u0 - (int64_t)tile * chunks);
   if (warp < 8) {
-    // ---- add and send out: a thread to a row ----
+    // ---- add and take out ----
     const int e = warp >> 2, row = (warp & 3) * 32 + lane;
+    const int c16 = lane & 15;                       // of a row going out: its 16 bytes
+    const int row0 = (warp & 3) * 2 + (lane >> 4);   // and the first of its 16 rows, 8 apart
     AdTile d = {};
-    T* to = nullptr;
+    int tok = -1;  // lane k: of row (warp & 3) * 2 + k / 16 + 8 (k % 16)
     float back = 1.0f;
     int known = -1;
     for (int i = 0; i < n; ++i, ++chunk) {
@@ -385,15 +400,15 @@ __global__ void __launch_bounds__(kUpThreads, 1)
       const int slot = i % NS;
       if (tile != known) {
         d = p.tiles[tile];
-        to = row < d.rows ? out + (int64_t)token_of(p, d, row) * out_stride : nullptr;
+        const int r = row0 + 8 * c16;
+        tok = r < d.rows ? token_of(p, d, r) : -1;
         if (H::scaled) back = d.owner >= 0 && row < d.rows ? low.back[(int64_t)tile * 128 + row] : 1.0f;
         known = tile;
       }
-      if (!mbar_wait(&b_full[slot], (i / NS) & 1) || !mbar_wait(&d_full[e], (i >> 1) & 1)) *fail = 1;
-      if (*fail) break;
+      if (!mbar_wait(&full[slot], (i / NS) & 1) || !mbar_wait(&d_full[e], (i >> 1) & 1)) *fail = 1;
       __syncwarp();
       tc_fence_after();
-      const uint32_t mine = at + slot * S::stage + row * kUpRow;
+      const uint32_t stage = at + slot * S::stage, mine = stage + row * kUpRow;
       const int width = min(128, N - chunk * 128);
       if (d.owner >= 0) {
 #pragma unroll 1
@@ -416,82 +431,104 @@ __global__ void __launch_bounds__(kUpThreads, 1)
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + (c + 8 * q) * 2), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
           }
         }
-      } else if (!base) {
-        for (int c = 0; c < width; c += 8)
-          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(mine + c * 2), "r"(0u) : "memory");
       }
       tc_fence_before();
       mbar_arrive(&d_empty[e]);
-      proxy_fence();
-      if (to) bulk_store(to + chunk * 128, mine, width * 2);
-      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-      asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      // the group's rows are done: they go out, half a warp to a row
+      if (any_failed<128>(1 + e, *fail)) break;
+      T* to = out + chunk * 128 + c16 * 8;
+      const bool in = c16 * 8 < width;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int t = __shfl_sync(0xffffffffu, tok, (lane & 16) + j);
+        if (!in || t < 0) continue;
+        const uint4 y = d.owner >= 0 || base ? lds_v4(stage + (row0 + 8 * j) * kUpRow + c16 * 16) : make_uint4(0u, 0u, 0u, 0u);
+        *reinterpret_cast<uint4*>(to + (int64_t)t * out_stride) = y;
+      }
       mbar_arrive(&empty[slot]);
     }
-    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-  } else if (warp == 8) {
-    // ---- rows of base, and images ----
+  } else if (warp < 12) {
+    // ---- base and F: a team brings every other unit ----
+    const int team = (warp - 8) >> 1, w2 = warp & 1, c16 = lane & 15, row0 = w2 * 2 + (lane >> 4);
     AdTile d = {};
-    int known = -1, images = 0, done = 0;
-    int64_t tok[4];
+    int tok[2] = {-1, -1};  // lane k: of rows row0(k) + 4 (k % 16), and 64 later
+    int known = -1;
     for (int i = 0; i < n; ++i, ++chunk) {
       if (chunk == chunks) chunk = 0, ++tile;
+      if ((i & 1) != team) continue;
       const int slot = i % NS;
-      const bool fresh = tile != known;
-      if (fresh) {
+      if (tile != known) {
         d = p.tiles[tile];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) tok[k] = lane + 32 * k < d.rows ? token_of(p, d, lane + 32 * k) : -1;
+        for (int k = 0; k < 2; ++k) {
+          const int r = row0 + 4 * c16 + 64 * k;
+          tok[k] = r < d.rows ? token_of(p, d, r) : -1;
+        }
         known = tile;
       }
-      if (i >= NS && !wait_warp(&empty[slot], (i / NS - 1) & 1)) *fail = 1;
-      if (*fail) break;
-      const uint32_t bytes = min(128, N - chunk * 128) * 2;
-      if (lane == 0) {
-        if (base) mbar_expect_tx(&b_full[slot], bytes * d.rows);
-        else mbar_arrive(&b_full[slot]);
-      }
+      if (i >= NS && !mbar_wait(&empty[slot], (i / NS - 1) & 1)) *fail = 1;
       __syncwarp();
+      if (*fail) break;
+      const uint32_t stage = at + slot * S::stage;
+      const int col = chunk * 128 + c16 * 8;
+      const bool in = col < N;
       if (base) {
+        const T* from = base + (in ? col : 0);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (tok[k] >= 0)
-            bulk_load_at(at + slot * S::stage + (lane + 32 * k) * kUpRow, base + tok[k] * base_stride + chunk * 128, bytes, &b_full[slot]);
-      }
-      done = i + 1;
-      if (fresh && d.owner >= 0) {
-        const int b = images % NI;
-        if (images >= NI && !wait_warp(&i_empty[b], (images / NI - 1) & 1)) *fail = 1;
-        if (*fail) break;
-        if (lane == 0) {
-          mbar_expect_tx(&i_full[b], S::image);
-          bulk_load_at(at + S::off_image + b * S::image, low.image + (int64_t)tile * S::image, S::image, &i_full[b]);
+        for (int j = 0; j < 32; ++j) {
+          const int t = __shfl_sync(0xffffffffu, tok[j >> 4], (lane & 16) + (j & 15));
+          if (in && t >= 0) cp16(stage + (row0 + 4 * j) * kUpRow + c16 * 16, from + (int64_t)t * base_stride, true);
         }
-        ++images;
       }
+      if (d.owner >= 0) {
+        const T* from = f + (int64_t)d.owner * R * N + (in ? col : 0);
+        const uint32_t to = stage + S::off_f + (c16 >> 3) * (NP * 128);
+#pragma unroll 8
+        for (int r = row0; r < NP; r += 4)  // zeros behind the rank: they meet zeros of the image
+          cp16(to + r * 128 + (((c16 & 7) ^ (r & 7)) << 4), from + (int64_t)min(r, R - 1) * N, in && r < R);
+      }
+      cp_commit();
+      cp_wait<0>();
+      proxy_fence();
+      mbar_arrive(&full[slot]);
     }
-    if (*fail) {  // what was sent for arrives before its memory goes
-      for (int i = max(0, done - NS); i < done; ++i) wait_warp(&b_full[i % NS], (i / NS) & 1);
-      for (int i = max(0, images - NI); i < images; ++i) wait_warp(&i_full[i % NI], (i / NI) & 1);
-    }
-  } else if (warp == 9) {
-    // ---- products ----
+    cp_wait<0>();
+  } else {
+    // ---- images and products ----
     constexpr uint32_t idesc = make_idesc(H::fmt, 128) | kMajorB;
-    int known = -1, images = 0, b = 0;
+    // the tile's image, and the next one where there is room for two
+    int known = -1, images = 0, sent = 0, b = 0;
+    int next = tile;  // the next tile whose image was not asked for
+    const int last = (int)((u1 - 1) / chunks);
     bool some = false;
-    for (int i = 0; i < n; ++i, ++chunk) {
+    for (int i = 0; i < n && !*fail; ++i, ++chunk) {
       if (chunk == chunks) chunk = 0, ++tile;
       const int slot = i % NS, e = i & 1;
       if (tile != known) {
         some = p.tiles[tile].owner >= 0;
         known = tile;
+        while (next <= last && (next <= tile || (NI > 1 && next == tile + 1))) {
+          if (p.tiles[next].owner >= 0) {
+            const int k = sent % NI;
+            if (sent >= NI && !wait_warp(&i_empty[k], (sent / NI - 1) & 1)) *fail = 1;
+            if (*fail) break;
+            if (lane == 0) {
+              mbar_expect_tx(&i_full[k], S::image);
+              bulk_load_at(at + S::off_image + k * S::image, low.image + (int64_t)next * S::image, S::image, &i_full[k]);
+            }
+            __syncwarp();
+            ++sent;
+          }
+          ++next;
+        }
+        if (*fail) break;
         if (some) {
           b = images % NI;
           if (!wait_warp(&i_full[b], (images / NI) & 1)) *fail = 1;
           ++images;
         }
       }
-      if (!wait_warp(&f_full[slot], (i / NS) & 1) || (i >= 2 && !wait_warp(&d_empty[e], ((i >> 1) - 1) & 1))) *fail = 1;
+      if (!wait_warp(&full[slot], (i / NS) & 1) || (i >= 2 && !wait_warp(&d_empty[e], ((i >> 1) - 1) & 1))) *fail = 1;
       if (*fail) break;
       tc_fence_after();
       if (some) {
@@ -512,39 +549,17 @@ __global__ void __launch_bounds__(kUpThreads, 1)
       }
       __syncwarp();
     }
-    if (*fail) {
+    if (*fail) {  // what was begun, or sent for, ends before its memory goes
       commit(&drain);
       wait_warp(&drain, 0);
-    }
-  } else {
-    // ---- F: 128 columns of the adapter's rows ----
-    const int t = tid - 320, c = t & 15, r0 = t >> 4;
-    int known = -1, owner = -1;
-    for (int i = 0; i < n; ++i, ++chunk) {
-      if (chunk == chunks) chunk = 0, ++tile;
-      const int slot = i % NS;
-      if (tile != known) owner = p.tiles[tile].owner, known = tile;
-      if (i >= NS && !mbar_wait(&empty[slot], (i / NS - 1) & 1)) *fail = 1;
-      if (*fail) break;
-      if (owner >= 0) {
-        const bool in = chunk * 128 + c * 8 < N;
-        const T* from = f + (int64_t)owner * R * N + (in ? chunk * 128 + c * 8 : 0);
-        const uint32_t to = at + slot * S::stage + S::off_f + (c >> 3) * (NP * 128);
-#pragma unroll 8
-        for (int r = r0; r < NP; r += 4)  // zeros behind the rank: they meet zeros of the image
-          cp16(to + r * 128 + (((c & 7) ^ (r & 7)) << 4), from + (int64_t)min(r, R - 1) * N, in && r < R);
-      }
-      cp_commit();
-      cp_wait<0>();
-      proxy_fence();
-      mbar_arrive(&f_full[slot]);
+      for (int k = max(images - 1, 0); k < sent; ++k) wait_warp(&i_full[k % NI], (k / NI) & 1);
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   if (tid == 0 && failed) *p.status = LQ_ETIMEOUT;
-  if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u));
+  if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u));
 }
 
 // ---------------------------------------------------------------------------
@@ -566,21 +581,6 @@ struct OuterShared {
   static constexpr int stage = off_v + 2 * NP * 128;
   static constexpr int bytes = stages * stage + 1024;
 };
-
-// Whether any loader found that a wait ran out: they leave together, at a run's
-// start, since they meet at barriers that have no limit.
-__device__ __forceinline__ bool any_loader(int fail) {
-  int r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.s32 p, %1, 0;\n\t"
-      "barrier.cta.red.or.pred q, 1, %2, p;\n\t"
-      "selp.s32 %0, 1, 0, q;\n\t}"
-      : "=r"(r)
-      : "r"(fail), "n"(kOuterLoaders)
-      : "memory");
-  return r != 0;
-}
 
 // One of the two problems of a launch: (v, x, dA) and (u, dy, dB).
 template <typename T>
@@ -638,7 +638,7 @@ __global__ void __launch_bounds__(kOuterLoaders + 32, OuterShared<NP>::blocks)
     const bool brings_x = warp < 4;
     const uint32_t at = base + (lane >> 3) * 8192;
     const bool in = col0 + lane * 8 < q.K;
-    for (int t0 = t_lo; !any_loader(*fail) && t0 < t_hi; ++run) {
+    for (int t0 = t_lo; !any_failed<kOuterLoaders>(1, *fail) && t0 < t_hi; ++run) {
       const int owner = p.tiles[t0].owner;
       const int first = p.tiles[t0].first, last = min(p.tile_of[owner + 1], t_hi) - 1;
       const int rows = p.tiles[last].first + p.tiles[last].rows - first;  // of the whole run, one behind the other in `order`
