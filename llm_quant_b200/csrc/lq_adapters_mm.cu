@@ -75,8 +75,12 @@ __device__ __forceinline__ float finite_mag(float v) {
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool some) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(some ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// Arrives at the barrier once all of the thread's copies so far are there.  The
+// proxy fence that the tensor cores' reads need is the reader's.
+__device__ __forceinline__ void cp_arrive(uint64_t* b) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(b)) : "memory");
+}
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
@@ -163,7 +167,7 @@ __global__ void __launch_bounds__(160, 2) ad_down_kernel(const T* __restrict__ x
                                                          const float* __restrict__ scaling, int R, int K, AdPlan p, int L,
                                                          Low low, int split) {
   using S = DownShared<NP>;
-  constexpr int NS = S::stages, LAG = NS - 2;
+  constexpr int NS = S::stages;
   constexpr uint32_t kCols = NP < 32 ? 32 : NP;
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t full[NS], empty[NS], done;
@@ -202,30 +206,23 @@ __global__ void __launch_bounds__(160, 2) ad_down_kernel(const T* __restrict__ x
 #pragma unroll
     for (int i = 0; i < NP / 16; ++i) fr[i] = r0 + 16 * i < R ? f + ((int64_t)d.owner * R + r0 + 16 * i) * K : nullptr;
     const uint32_t at = base + r0 * 128 + ((c ^ (r0 & 7)) << 4);
-    for (int i = 0; i < n + LAG; ++i) {
-      if (i < n) {
-        const int slot = i % NS;
-        if (i >= NS && !mbar_wait(&empty[slot], (i / NS - 1) & 1)) failed = 1;
-        if (*(volatile int*)&failed) break;
-        const int k = (s0 + i) * 64 + c * 8;
-        const bool some = k < K;  // behind K: zeros in both factors
-        const int kk = some ? k : 0;
-        const uint32_t to = at + slot * S::stage;
+    for (int i = 0; i < n; ++i) {
+      const int slot = i % NS;
+      if (i >= NS && !mbar_wait(&empty[slot], (i / NS - 1) & 1)) failed = 1;
+      if (*(volatile int*)&failed) break;
+      const int k = (s0 + i) * 64 + c * 8;
+      const bool some = k < K;  // behind K: zeros in both factors
+      const int kk = some ? k : 0;
+      const uint32_t to = at + slot * S::stage;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (xr[j]) cp16(to + j * 2048, xr[j] + kk, some);
+      for (int j = 0; j < 8; ++j)
+        if (xr[j]) cp16(to + j * 2048, xr[j] + kk, some);
 #pragma unroll
-        for (int j = 0; j < NP / 16; ++j)
-          if (fr[j]) cp16(to + 16384 + j * 2048, fr[j] + kk, some);
-      }
-      cp_commit();
-      if (i >= LAG) {
-        cp_wait<LAG>();
-        proxy_fence();
-        mbar_arrive(&full[(i - LAG) % NS]);
-      }
+      for (int j = 0; j < NP / 16; ++j)
+        if (fr[j]) cp16(to + 16384 + j * 2048, fr[j] + kk, some);
+      cp_arrive(&full[slot]);
     }
-    cp_wait<0>();
+    cp_wait_all();
   } else {
     constexpr uint32_t idesc = make_idesc(Half16<T>::fmt, NP);
     for (int i = 0; i < n; ++i) {
@@ -234,6 +231,7 @@ __global__ void __launch_bounds__(160, 2) ad_down_kernel(const T* __restrict__ x
         failed = 1;
         break;
       }
+      proxy_fence();
       tc_fence_after();
       const uint64_t da = sw128_desc(base + slot * S::stage), db = sw128_desc(base + slot * S::stage + 16384);
 #pragma unroll
@@ -487,12 +485,9 @@ __global__ void __launch_bounds__(kUpThreads, 1)
         for (int r = row0; r < NP; r += 4)  // zeros behind the rank: they meet zeros of the image
           cp16(to + r * 128 + (((c16 & 7) ^ (r & 7)) << 4), from + (int64_t)min(r, R - 1) * N, in && r < R);
       }
-      cp_commit();
-      cp_wait<0>();
-      proxy_fence();
-      mbar_arrive(&full[slot]);
+      cp_arrive(&full[slot]);
     }
-    cp_wait<0>();
+    cp_wait_all();
   } else {
     // ---- images and products ----
     constexpr uint32_t idesc = make_idesc(H::fmt, 128) | kMajorB;
@@ -530,6 +525,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
       }
       if (!wait_warp(&full[slot], (i / NS) & 1) || (i >= 2 && !wait_warp(&d_empty[e], ((i >> 1) - 1) & 1))) *fail = 1;
       if (*fail) break;
+      proxy_fence();
       tc_fence_after();
       if (some) {
         const uint32_t im = at + S::off_image + b * S::image;
@@ -598,7 +594,7 @@ __global__ void __launch_bounds__(kOuterLoaders + 32, OuterShared<NP>::blocks)
     ad_outer_kernel(const OuterSide<T> one, const OuterSide<T> two, int R, AdPlan p, int L) {
   using S = OuterShared<NP>;
   using H = Half16<T>;
-  constexpr int NS = S::stages, LAG = NS - 2, VI = NP / 16;  // 8 tokens of a rank, of a lane that brings V
+  constexpr int NS = S::stages, VI = NP / 16;  // 8 tokens of a rank, of a lane that brings V
   constexpr uint32_t kCols = 4 * NP;  // two tiles of 128 columns, hi and lo
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t full[NS], empty[NS], done, free_, drain;
@@ -659,42 +655,36 @@ __global__ void __launch_bounds__(kOuterLoaders + 32, OuterShared<NP>::blocks)
           return lane < 16 && row < rows ? p.order[first + row] : -1;
         };
         int next = token(0);
-        for (int i = 0; i < n + LAG; ++i) {
-          if (i < n) {
-            const int slot = (step + i) % NS, now = next;
-            if (i + 1 < n) next = token(i + 1);
-            if (step + i >= NS && !mbar_wait(&empty[slot], ((step + i) / NS - 1) & 1)) *fail = 1;
-            if (*fail) break;
-            __syncwarp();
-            const uint32_t to = at + slot * S::stage;
+        for (int i = 0; i < n; ++i) {
+          const int slot = (step + i) % NS, now = next;
+          if (i + 1 < n) next = token(i + 1);
+          if (step + i >= NS && !mbar_wait(&empty[slot], ((step + i) / NS - 1) & 1)) *fail = 1;
+          __syncwarp();
+          if (*fail) break;
+          const uint32_t to = at + slot * S::stage;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const int row = warp + 4 * j, tok = __shfl_sync(0xffffffffu, now, j);
-              const bool some = in && tok >= 0;  // behind the run: zeros in both factors
-              cp16(to + row * 128 + (((lane & 7) ^ (row & 7)) << 4), some ? q.x + (int64_t)tok * q.stride + col0 + lane * 8 : q.x, some);
-            }
+          for (int j = 0; j < 16; ++j) {
+            const int row = warp + 4 * j, tok = __shfl_sync(0xffffffffu, now, j);
+            const bool some = in && tok >= 0;  // behind the run: zeros in both factors
+            cp16(to + row * 128 + (((lane & 7) ^ (row & 7)) << 4), some ? q.x + (int64_t)tok * q.stride + col0 + lane * 8 : q.x, some);
           }
-          cp_commit();
-          if (i >= LAG) {
-            cp_wait<LAG>();
-            proxy_fence();
-            mbar_arrive(&full[(step + i - LAG) % NS]);
-          }
+          cp_arrive(&full[slot]);
         }
       } else {
         const int id = tid - 128, k8 = id & 7, r0 = id >> 3;
         float v[VI][8];
+        // whole pieces, the ones behind the run too (a tile's rows are all there, if
+        // nobody wrote them): a load under a condition, whose value is looked at
+        // before the next one, cost a trip to L2 each (370 us instead of 136)
         auto fetch = [&](int i) {
           const float* from = q.v.turned + (int64_t)(t0 + (i >> 1)) * NP * 128 + (i & 1) * 64 + k8 * 8;
-          const int left = rows - i * 64 - k8 * 8;  // of the 8 tokens; nobody wrote those behind the run
 #pragma unroll
-          for (int j = 0; j < VI; ++j) {
-            float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f), b = a;
-            if (left > 0) a = *reinterpret_cast<const float4*>(from + (r0 + 16 * j) * 128);
-            if (left > 4) b = *reinterpret_cast<const float4*>(from + (r0 + 16 * j) * 128 + 4);
-            v[j][0] = a.x, v[j][1] = left > 1 ? a.y : 0.0f, v[j][2] = left > 2 ? a.z : 0.0f, v[j][3] = left > 3 ? a.w : 0.0f;
-            v[j][4] = b.x, v[j][5] = left > 5 ? b.y : 0.0f, v[j][6] = left > 6 ? b.z : 0.0f, v[j][7] = left > 7 ? b.w : 0.0f;
-          }
+          for (int j = 0; j < VI; ++j)
+#pragma unroll
+            for (int k = 0; k < 8; k += 4) {
+              const float4 a = *reinterpret_cast<const float4*>(from + (r0 + 16 * j) * 128 + k);
+              v[j][k] = a.x, v[j][k + 1] = a.y, v[j][k + 2] = a.z, v[j][k + 3] = a.w;
+            }
         };
         fetch(0);
         for (int i = 0; i < n; ++i) {
@@ -702,6 +692,13 @@ __global__ void __launch_bounds__(kOuterLoaders + 32, OuterShared<NP>::blocks)
           if (step + i >= NS && !mbar_wait(&empty[slot], ((step + i) / NS - 1) & 1)) *fail = 1;
           if (*fail) break;
           const uint32_t vt = base + slot * S::stage + S::off_v;
+          const int left = rows - i * 64 - k8 * 8;  // tokens of the run from here on
+          if (left < 8) {
+#pragma unroll
+            for (int j = 0; j < VI; ++j)
+#pragma unroll
+              for (int k = 0; k < 8; ++k) v[j][k] = k < left ? v[j][k] : 0.0f;
+          }
 #pragma unroll
           for (int j = 0; j < VI; ++j) {
             const int r = r0 + 16 * j;
@@ -712,13 +709,13 @@ __global__ void __launch_bounds__(kOuterLoaders + 32, OuterShared<NP>::blocks)
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a + NP * 128), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
           }
-          if (i + 1 < n) fetch(i + 1);
           proxy_fence();
           mbar_arrive(&full[slot]);
+          if (i + 1 < n) fetch(i + 1);
         }
       }
       step += n;
-      cp_wait<0>();
+      cp_wait_all();
       if (!mbar_wait(&done, run & 1)) *fail = 1;
       __syncwarp();
       tc_fence_after();
@@ -745,7 +742,6 @@ __global__ void __launch_bounds__(kOuterLoaders + 32, OuterShared<NP>::blocks)
       mbar_arrive(&free_);
       t0 = last + 1;
     }
-    cp_wait<0>();
   } else {
     constexpr uint32_t idesc = make_idesc(H::fmt, 2 * NP) | kMajorA;
     for (int t0 = t_lo; t0 < t_hi && !*fail; ++run) {
@@ -760,6 +756,7 @@ __global__ void __launch_bounds__(kOuterLoaders + 32, OuterShared<NP>::blocks)
           *fail = 1;
           break;
         }
+        proxy_fence();
         tc_fence_after();
         const uint32_t s = base + slot * S::stage;
         const uint64_t db = sw128_desc(s + S::off_v);
