@@ -75,6 +75,13 @@ __device__ __forceinline__ float finite_mag(float v) {
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool some) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(some ? 16 : 0) : "memory");
 }
+// A bounded wait of a thread by itself (as wait_warp: no timer is read)
+__device__ __forceinline__ bool wait_lane(uint64_t* bar, uint32_t parity) {
+  bool ok = false;
+#pragma unroll 1
+  for (int i = 0; i < (1 << 20) && !ok; ++i) ok = mbar_try_sleep(bar, parity, 10000u);
+  return ok;
+}
 __device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 // Arrives at the barrier once all of the thread's copies so far are there.  The
 // proxy fence that the tensor cores' reads need is the reader's.
@@ -208,7 +215,7 @@ __global__ void __launch_bounds__(160, 2) ad_down_kernel(const T* __restrict__ x
     const uint32_t at = base + r0 * 128 + ((c ^ (r0 & 7)) << 4);
     for (int i = 0; i < n; ++i) {
       const int slot = i % NS;
-      if (i >= NS && !mbar_wait(&empty[slot], (i / NS - 1) & 1)) failed = 1;
+      if (i >= NS && !wait_lane(&empty[slot], (i / NS - 1) & 1)) failed = 1;
       if (*(volatile int*)&failed) break;
       const int k = (s0 + i) * 64 + c * 8;
       const bool some = k < K;  // behind K: zeros in both factors
@@ -241,7 +248,7 @@ __global__ void __launch_bounds__(160, 2) ad_down_kernel(const T* __restrict__ x
     commit(&done);
   }
   const float s = scaling[d.owner];
-  const bool ok = mbar_wait_warp(&done, 0);
+  const bool ok = wait_warp(&done, 0);
   if (!ok) failed = 1;
   tc_fence_after();
   if (warp < 4) {
@@ -324,23 +331,29 @@ __global__ void __launch_bounds__(160, 2) ad_down_kernel(const T* __restrict__ x
 // x 128] = (hi + lo) [128 x NP] F [NP x 128], F as its rows lie in memory.  A
 // block has a stretch of units.  Base and F come by cp.async, whole rows of 256
 // bytes to half a warp; the thread that has a row of D adds it to the row of base
-// in shared memory, and half a warp takes each row out again.  (A lane that
+// in shared memory, and half a warp of others takes each row out again.  (A lane that
 // loads its own part of base, as mma.sync deals D out, touches eight lines of
 // 64 bytes each at a time: L1 was busy 4 cycles of 5.  Bulk copies of a row
 // each took 30 cycles apiece.)  Two groups of four warps take turns with the
-// units, and two teams of two warps with bringing them.
+// units, and two teams of two warps with bringing base.
 // ---------------------------------------------------------------------------
-constexpr int kUpThreads = 416;
+constexpr int kUpBeside = 4;  // blocks that go along a tile's rows side by side, so that 1024 bytes of a row are asked for at a time
+constexpr int kUpThreads = 736;  // 8 warps add, 8 take out, 4 bring base, 2 bring F, 1 has the products
 constexpr int kUpRow = 256 + 16;  // bytes between rows of base in shared memory: 8 rows' pieces in all banks
 template <int NP>
 struct UpShared {
-  static constexpr int stages = NP <= 16 ? 5 : NP <= 32 ? 4 : NP <= 64 ? 3 : 2;
-  static constexpr int off_f = 128 * kUpRow;            // of a stage
-  static constexpr int stage = off_f + NP * 256;
+  // Two stages of base are being taken out, the others are on their way: with
+  // one (three in all, each with its F) the loads' latency was what counted, 226 us
+  // instead of FIGURE for 16384 tokens and 14336 columns
+  static constexpr int stages = NP <= 32 ? 5 : NP <= 64 ? 4 : 3;
+  static constexpr int stage = 128 * kUpRow;
+  static constexpr int fs = NP <= 64 ? 2 : 1;           // stages of F
+  static constexpr int f_bytes = NP * 256;
+  static constexpr int images = NP <= 32 ? 2 : 1;
   static constexpr int image = 128 * NP * 4;
-  static constexpr int images = NP <= 64 ? 2 : 1;
-  static constexpr int off_image = stages * stage;
+  static constexpr int off_f = stages * stage, off_image = off_f + fs * f_bytes;
   static constexpr int bytes = off_image + images * image + 1024;
+  static_assert(stage % 1024 == 0 && f_bytes % 1024 == 0, "operands are swizzled in pieces of 1024 bytes");
 };
 
 template <typename T, int NP>
@@ -349,23 +362,26 @@ __global__ void __launch_bounds__(kUpThreads, 1)
                  T* out, int64_t out_stride, int chunks) {
   using S = UpShared<NP>;
   using H = Half16<T>;
-  constexpr int NS = S::stages, NI = S::images;
+  constexpr int NS = S::stages, NF = S::fs, NI = S::images;
   extern __shared__ uint8_t raw[];
-  // full: base and F are there; empty: the unit was taken out; i_full / i_empty: the images
-  __shared__ uint64_t full[NS], empty[NS], i_full[NI], i_empty[NI], d_full[2], d_empty[2], drain;
+  // full: base is there; added: D too; empty: the unit was taken out; f_, i_, d_: the same of F, of images and of D
+  __shared__ uint64_t full[NS], added[NS], empty[NS], f_full[NF], f_empty[NF], i_full[NI], i_empty[NI], d_full[2], d_empty[2], drain;
   __shared__ uint32_t tmem_at;
   __shared__ int failed;
   pdl_wait();
   pdl_trigger();
   // tokens without an adapter: nothing to do where out is base
-  const int64_t units = (int64_t)p.tile_of[base == out ? L : L + 1] * chunks;
-  const int64_t u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
+  const int wide = (chunks + kUpBeside - 1) / kUpBeside * kUpBeside;  // of a tile; what is behind the columns is empty
+  const int64_t units = (int64_t)p.tile_of[base == out ? L : L + 1] * (wide / kUpBeside);  // of each block of a group
+  const int64_t group = blockIdx.x / kUpBeside, groups = gridDim.x / kUpBeside;
+  const int64_t u0 = units * group / groups, u1 = units * (group + 1) / groups;
   const int n = (int)(u1 - u0);
   if (n == 0) return;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t at = (smem_u32(raw) + 1023) & ~1023u;
   if (tid == 0) {
-    for (int i = 0; i < NS; ++i) mbar_init(&full[i], 64), mbar_init(&empty[i], 128);
+    for (int i = 0; i < NS; ++i) mbar_init(&full[i], 64), mbar_init(&added[i], 128), mbar_init(&empty[i], 128);
+    for (int i = 0; i < NF; ++i) mbar_init(&f_full[i], 64), mbar_init(&f_empty[i], 1);
     for (int i = 0; i < NI; ++i) mbar_init(&i_full[i], 1), mbar_init(&i_empty[i], 1);
     for (int i = 0; i < 2; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_empty[i], 128);
     mbar_init(&drain, 1);
@@ -373,7 +389,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     proxy_fence();
   }
-  if (warp == 12) {
+  if (warp == 22) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_at)), "r"(256u));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -382,77 +398,101 @@ __global__ void __launch_bounds__(kUpThreads, 1)
   tc_fence_after();
   const uint32_t tmem = tmem_at;
   volatile int* fail = &failed;
-  int tile = (int)(u0 / chunks), chunk = (int)(u0 - (int64_t)tile * chunks);
+  int tile = (int)(u0 * kUpBeside / wide), chunk = (int)(u0 * kUpBeside - (int64_t)tile * wide + blockIdx.x % kUpBeside);
   if (warp < 8) {
-    // ---- add and take out ----
+    // ---- add: a thread to a row ----
     const int e = warp >> 2, row = (warp & 3) * 32 + lane;
-    const int c16 = lane & 15;                       // of a row going out: its 16 bytes
-    const int row0 = (warp & 3) * 2 + (lane >> 4);   // and the first of its 16 rows, 8 apart
-    AdTile d = {};
-    int tok = -1;  // lane k: of row (warp & 3) * 2 + k / 16 + 8 (k % 16)
     float back = 1.0f;
+    bool some = false;
     int known = -1;
-    for (int i = 0; i < n; ++i, ++chunk) {
-      if (chunk == chunks) chunk = 0, ++tile;
+    for (int i = 0; i < n; ++i, chunk += kUpBeside) {
+      if (chunk >= wide) chunk -= wide, ++tile;
       if ((i & 1) != e) continue;
       const int slot = i % NS;
       if (tile != known) {
-        d = p.tiles[tile];
-        const int r = row0 + 8 * c16;
-        tok = r < d.rows ? token_of(p, d, r) : -1;
-        if (H::scaled) back = d.owner >= 0 && row < d.rows ? low.back[(int64_t)tile * 128 + row] : 1.0f;
+        const AdTile d = p.tiles[tile];
+        some = d.owner >= 0;
+        if (H::scaled) back = some && row < d.rows ? low.back[(int64_t)tile * 128 + row] : 1.0f;
         known = tile;
       }
-      if (!mbar_wait(&full[slot], (i / NS) & 1) || !mbar_wait(&d_full[e], (i >> 1) & 1)) *fail = 1;
+      if (!wait_lane(&full[slot], (i / NS) & 1) || !wait_lane(&d_full[e], (i >> 1) & 1)) *fail = 1;
       __syncwarp();
+      if (*fail) break;
       tc_fence_after();
-      const uint32_t stage = at + slot * S::stage, mine = stage + row * kUpRow;
-      const int width = min(128, N - chunk * 128);
-      if (d.owner >= 0) {
-#pragma unroll 1
-        for (int c = 0; c < width; c += 32) {
-          uint32_t v[32];
-          tmem_ld32(tmem + ((uint32_t)(warp & 3) << 21) + e * 128 + c, v);
+      const uint32_t mine = at + slot * S::stage + row * kUpRow, from = tmem + ((uint32_t)(warp & 3) << 21) + e * 128;
+      if (some) {
+        // the next 32 columns leave tensor memory while these are added
+        uint32_t v[2][32];
+        tmem_ld32(from, v[0]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t* w = v[c & 1];
           uint4 y[4];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) y[q] = base ? lds_v4(mine + (c + 8 * q) * 2) : make_uint4(0u, 0u, 0u, 0u);
-          tmem_wait_ld32(v);
+          for (int q = 0; q < 4; ++q) y[q] = base ? lds_v4(mine + c * 64 + q * 16) : make_uint4(0u, 0u, 0u, 0u);
+          tmem_wait_ld32(w);
+          if (c < 3) tmem_ld32(from + c * 32 + 32, v[(c + 1) & 1]);
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             uint32_t o[4] = {y[q].x, y[q].y, y[q].z, y[q].w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const float2 b = H::unpack(o[k]);
-              const float v0 = __uint_as_float(v[8 * q + 2 * k]), v1 = __uint_as_float(v[8 * q + 2 * k + 1]);
+              const float v0 = __uint_as_float(w[8 * q + 2 * k]), v1 = __uint_as_float(w[8 * q + 2 * k + 1]);
               o[k] = H::scaled ? H::pack(fmaf(v0, back, b.x), fmaf(v1, back, b.y)) : H::pack(b.x + v0, b.y + v1);
             }
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + (c + 8 * q) * 2), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + c * 64 + q * 16), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
           }
         }
       }
       tc_fence_before();
       mbar_arrive(&d_empty[e]);
-      // the group's rows are done: they go out, half a warp to a row
-      if (any_failed<128>(1 + e, *fail)) break;
+      mbar_arrive(&added[slot]);
+    }
+  } else if (warp < 16) {
+    // ---- take out: half a warp to a row, a team every other unit ----
+    const int team = (warp - 8) >> 2;
+    const int c16 = lane & 15, row0 = (warp & 3) * 2 + (lane >> 4);  // its 16 bytes, and the first of its rows, 8 apart
+    AdTile d = {};
+    int tok = -1;  // lane k: of row (warp & 3) * 2 + k / 16 + 8 (k % 16)
+    int known = -1;
+    for (int i = 0; i < n; ++i, chunk += kUpBeside) {
+      if (chunk >= wide) chunk -= wide, ++tile;
+      if ((i & 1) != team) continue;
+      const int slot = i % NS;
+      if (tile != known) {
+        d = p.tiles[tile];
+        const int r = row0 + 8 * c16;
+        tok = r < d.rows ? token_of(p, d, r) : -1;
+        known = tile;
+      }
+      if (!wait_lane(&added[slot], (i / NS) & 1)) *fail = 1;
+      __syncwarp();
+      if (*fail) break;
+      const uint32_t from = at + slot * S::stage + row0 * kUpRow + c16 * 16;
       T* to = out + chunk * 128 + c16 * 8;
-      const bool in = c16 * 8 < width;
+      const bool in = chunk * 128 + c16 * 8 < N, some = d.owner >= 0 || base;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const int t = __shfl_sync(0xffffffffu, tok, (lane & 16) + j);
-        if (!in || t < 0) continue;
-        const uint4 y = d.owner >= 0 || base ? lds_v4(stage + (row0 + 8 * j) * kUpRow + c16 * 16) : make_uint4(0u, 0u, 0u, 0u);
-        *reinterpret_cast<uint4*>(to + (int64_t)t * out_stride) = y;
+      for (int j0 = 0; j0 < 16; j0 += 8) {
+        uint4 y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = lds_v4(from + 8 * (j0 + j) * kUpRow);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int t = __shfl_sync(0xffffffffu, tok, (lane & 16) + j0 + j);
+          if (in && t >= 0) *reinterpret_cast<uint4*>(to + (int64_t)t * out_stride) = some ? y[j] : make_uint4(0u, 0u, 0u, 0u);
+        }
       }
       mbar_arrive(&empty[slot]);
     }
-  } else if (warp < 12) {
-    // ---- base and F: a team brings every other unit ----
-    const int team = (warp - 8) >> 1, w2 = warp & 1, c16 = lane & 15, row0 = w2 * 2 + (lane >> 4);
+  } else if (warp < 20) {
+    // ---- base: a team brings every other unit ----
+    const int team = (warp - 16) >> 1, w2 = warp & 1, c16 = lane & 15, row0 = w2 * 2 + (lane >> 4);
     AdTile d = {};
     int tok[2] = {-1, -1};  // lane k: of rows row0(k) + 4 (k % 16), and 64 later
     int known = -1;
-    for (int i = 0; i < n; ++i, ++chunk) {
-      if (chunk == chunks) chunk = 0, ++tile;
+    for (int i = 0; i < n; ++i, chunk += kUpBeside) {
+      if (chunk >= wide) chunk -= wide, ++tile;
       if ((i & 1) != team) continue;
       const int slot = i % NS;
       if (tile != known) {
@@ -464,7 +504,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
         }
         known = tile;
       }
-      if (i >= NS && !mbar_wait(&empty[slot], (i / NS - 1) & 1)) *fail = 1;
+      if (i >= NS && !wait_lane(&empty[slot], (i / NS - 1) & 1)) *fail = 1;
       __syncwarp();
       if (*fail) break;
       const uint32_t stage = at + slot * S::stage;
@@ -478,27 +518,43 @@ __global__ void __launch_bounds__(kUpThreads, 1)
           if (in && t >= 0) cp16(stage + (row0 + 4 * j) * kUpRow + c16 * 16, from + (int64_t)t * base_stride, true);
         }
       }
-      if (d.owner >= 0) {
-        const T* from = f + (int64_t)d.owner * R * N + (in ? col : 0);
-        const uint32_t to = stage + S::off_f + (c16 >> 3) * (NP * 128);
-#pragma unroll 8
-        for (int r = row0; r < NP; r += 4)  // zeros behind the rank: they meet zeros of the image
-          cp16(to + r * 128 + (((c16 & 7) ^ (r & 7)) << 4), from + (int64_t)min(r, R - 1) * N, in && r < R);
-      }
       cp_arrive(&full[slot]);
+    }
+    cp_wait_all();
+  } else if (warp < 22) {
+    // ---- F: 128 columns of the adapter's rows ----
+    const int c16 = lane & 15, row0 = (warp & 1) * 2 + (lane >> 4);
+    int known = -1, owner = -1, sent = 0;
+    for (int i = 0; i < n; ++i, chunk += kUpBeside) {
+      if (chunk >= wide) chunk -= wide, ++tile;
+      if (tile != known) owner = p.tiles[tile].owner, known = tile;
+      if (owner < 0) continue;
+      const int fs = sent % NF;
+      if (sent >= NF && !wait_lane(&f_empty[fs], (sent / NF - 1) & 1)) *fail = 1;
+      __syncwarp();
+      if (*fail) break;
+      const int col = chunk * 128 + c16 * 8;
+      const bool in = col < N;
+      const T* from = f + (int64_t)owner * R * N + (in ? col : 0);
+      const uint32_t to = at + S::off_f + fs * S::f_bytes + (c16 >> 3) * (NP * 128);
+#pragma unroll 16
+      for (int r = row0; r < NP; r += 4)  // zeros behind the rank: they meet zeros of the image
+        cp16(to + r * 128 + (((c16 & 7) ^ (r & 7)) << 4), from + (int64_t)min(r, R - 1) * N, in && r < R);
+      cp_arrive(&f_full[fs]);
+      ++sent;
     }
     cp_wait_all();
   } else {
     // ---- images and products ----
     constexpr uint32_t idesc = make_idesc(H::fmt, 128) | kMajorB;
     // the tile's image, and the next one where there is room for two
-    int known = -1, images = 0, sent = 0, b = 0;
+    int known = -1, images = 0, sent = 0, b = 0, used = 0;
     int next = tile;  // the next tile whose image was not asked for
-    const int last = (int)((u1 - 1) / chunks);
+    const int last = (int)((u1 - 1) * kUpBeside / wide);
     bool some = false;
-    for (int i = 0; i < n && !*fail; ++i, ++chunk) {
-      if (chunk == chunks) chunk = 0, ++tile;
-      const int slot = i % NS, e = i & 1;
+    for (int i = 0; i < n && !*fail; ++i, chunk += kUpBeside) {
+      if (chunk >= wide) chunk -= wide, ++tile;
+      const int fs = used % NF, e = i & 1;
       if (tile != known) {
         some = p.tiles[tile].owner >= 0;
         known = tile;
@@ -523,13 +579,13 @@ __global__ void __launch_bounds__(kUpThreads, 1)
           ++images;
         }
       }
-      if (!wait_warp(&full[slot], (i / NS) & 1) || (i >= 2 && !wait_warp(&d_empty[e], ((i >> 1) - 1) & 1))) *fail = 1;
+      if ((some && !wait_warp(&f_full[fs], (used / NF) & 1)) || (i >= 2 && !wait_warp(&d_empty[e], ((i >> 1) - 1) & 1))) *fail = 1;
       if (*fail) break;
       proxy_fence();
       tc_fence_after();
       if (some) {
         const uint32_t im = at + S::off_image + b * S::image;
-        const uint64_t df = sw128_mn_desc(at + slot * S::stage + S::off_f, NP * 128);
+        const uint64_t df = sw128_mn_desc(at + S::off_f + fs * S::f_bytes, NP * 128);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -539,7 +595,9 @@ __global__ void __launch_bounds__(kUpThreads, 1)
             mma_ss(tmem + e * 128, da, df + 128 * k, idesc, (h | k) > 0);
           }
         commit(&d_full[e]);
-        if (i + 1 == n || chunk + 1 == chunks) commit(&i_empty[b]);
+        commit(&f_empty[fs]);
+        ++used;
+        if (i + 1 == n || chunk + kUpBeside >= wide) commit(&i_empty[b]);
       } else if (lane == 0) {
         mbar_arrive(&d_full[e]);
       }
@@ -555,7 +613,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
   __syncthreads();
   tc_fence_after();
   if (tid == 0 && failed) *p.status = LQ_ETIMEOUT;
-  if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u));
+  if (warp == 22) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u));
 }
 
 // ---------------------------------------------------------------------------
@@ -658,7 +716,7 @@ __global__ void __launch_bounds__(kOuterLoaders + 32, OuterShared<NP>::blocks)
         for (int i = 0; i < n; ++i) {
           const int slot = (step + i) % NS, now = next;
           if (i + 1 < n) next = token(i + 1);
-          if (step + i >= NS && !mbar_wait(&empty[slot], ((step + i) / NS - 1) & 1)) *fail = 1;
+          if (step + i >= NS && !wait_lane(&empty[slot], ((step + i) / NS - 1) & 1)) *fail = 1;
           __syncwarp();
           if (*fail) break;
           const uint32_t to = at + slot * S::stage;
@@ -689,7 +747,7 @@ __global__ void __launch_bounds__(kOuterLoaders + 32, OuterShared<NP>::blocks)
         fetch(0);
         for (int i = 0; i < n; ++i) {
           const int slot = (step + i) % NS;
-          if (step + i >= NS && !mbar_wait(&empty[slot], ((step + i) / NS - 1) & 1)) *fail = 1;
+          if (step + i >= NS && !wait_lane(&empty[slot], ((step + i) / NS - 1) & 1)) *fail = 1;
           if (*fail) break;
           const uint32_t vt = base + slot * S::stage + S::off_v;
           const int left = rows - i * 64 - k8 * 8;  // tokens of the run from here on
@@ -716,7 +774,7 @@ __global__ void __launch_bounds__(kOuterLoaders + 32, OuterShared<NP>::blocks)
       }
       step += n;
       cp_wait_all();
-      if (!mbar_wait(&done, run & 1)) *fail = 1;
+      if (!wait_lane(&done, run & 1)) *fail = 1;
       __syncwarp();
       tc_fence_after();
       const int mt = warp >> 2, my = col0 + mt * 128 + (warp & 3) * 32 + lane;
@@ -864,10 +922,11 @@ int up_np(const AdCall& a, void* low, bool is_a, const void* base, int64_t bs, v
   using S = UpShared<NP>;
   const lq_adapter_bank& b = *a.bank;
   const int N = (int)(is_a ? b.K : b.N), chunks = (N + 127) / 128;
-  const int64_t tiles = ad_max_tiles(a.n, b.L), units = tiles * chunks;
+  const int64_t tiles = ad_max_tiles(a.n, b.L), units = tiles * ((chunks + kUpBeside - 1) / kUpBeside);
+  const int64_t groups = units < num_sms() / kUpBeside ? units : num_sms() / kUpBeside;
   constexpr auto kern = ad_up_kernel<T, NP>;
   LQ_TRY(more_shared<kern>(S::bytes));
-  const cudaError_t e = launch_pdl(kern, dim3((unsigned)(units < num_sms() ? units : num_sms())), dim3(kUpThreads), S::bytes, a.st,
+  const cudaError_t e = launch_pdl(kern, dim3((unsigned)(groups * kUpBeside)), dim3(kUpThreads), S::bytes, a.st,
                                    low_at<NP>(low, tiles, false), static_cast<const T*>(is_a ? b.a : b.b), (int)b.R, N, a.plan,
                                    (int)b.L, static_cast<const T*>(base), bs, static_cast<T*>(out), os, chunks);
   LQ_REQUIRE(e == cudaSuccess, LQ_ECUDA, "ad_up_kernel launch: %s", cudaGetErrorString(e));
