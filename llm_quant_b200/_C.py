@@ -162,7 +162,7 @@ def lib():
 
 def call(name: str, *args) -> None:
     """Call an entry point and turn a non-zero status into an exception."""
-    rc = getattr(lib(), name)(*args)
+    rc = getattr(_lib or lib(), name)(*args)
     if rc != OK:
         msg = lib().lq_last_error().decode(errors="replace")
         if rc in (EINVAL, ERANGE):

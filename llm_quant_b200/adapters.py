@@ -31,7 +31,6 @@ from typing import Iterable, Optional
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from . import _C
 
@@ -193,20 +192,15 @@ class AdapterBank(nn.Module):
         self.scaling[index] = scaling
 
     # -- calls -------------------------------------------------------------------
-    def _struct(self, a: torch.Tensor, b: torch.Tensor, s: torch.Tensor):
-        """The bank as the entry points take it, by reference, with the weights
-        a, b in a call's dtype."""
-        key = (a.data_ptr(), b.data_ptr(), s.data_ptr(), a.dtype)
-        c = self._c
-        if c[0] != key:
-            form = _C.AdapterBank(*key[:3], self.num_adapters, self.rank, self.in_features, self.out_features, _C.dt(a))
-            self._c = c = (key, ctypes.byref(form))  # the struct itself is never changed
-        return c[1]
-
     def _weights(self, x: torch.Tensor):
-        """lora_A, lora_B in x's dtype, and scaling."""
+        """(the bank as the entry points take it, by reference, and the tensors
+        that it points to: lora_A, lora_B in x's dtype, scaling)"""
         p = self._parameters
         a, b, s = p["lora_A"], p["lora_B"], self._buffers["scaling"]
+        key = (a.data_ptr(), b.data_ptr(), s.data_ptr(), a.dtype, a.numel(), b.numel(), a.is_contiguous(), x.dtype, x.device)
+        known, ref = self._c
+        if known == key:
+            return ref, a, b, s
         dev = x.device
         if a.device != dev or b.device != dev or s.device != dev:
             raise RuntimeError(f"AdapterBank: x on {dev}, the bank on {a.device}")
@@ -214,11 +208,20 @@ class AdapterBank(nn.Module):
             raise TypeError(f"AdapterBank: lora_A is {a.dtype}, lora_B {b.dtype}, scaling {s.dtype} (expected float32)")
         if a.shape != self._shapes[0] or b.shape != self._shapes[1] or s.numel() != self.num_adapters:
             raise RuntimeError(f"AdapterBank: lora_A {list(a.shape)}, lora_B {list(b.shape)} are not the bank's")
-        if a.dtype != x.dtype:
+        as_is = a.dtype == x.dtype
+        if not as_is:
             a, b = a.detach().to(x.dtype), b.detach().to(x.dtype)
         if not (a.is_contiguous() and b.is_contiguous() and s.is_contiguous()) or (a.data_ptr() | b.data_ptr()) & 15:
             a, b, s = (t.detach().clone(memory_format=torch.contiguous_format) for t in (a, b, s))
-        return a, b, s
+            as_is = False
+        ref = self._struct(a, b, s)
+        if as_is:
+            self._c = (key, ref)  # the struct itself is never changed
+        return ref, a, b, s
+
+    def _struct(self, a: torch.Tensor, b: torch.Tensor, s: torch.Tensor):
+        return ctypes.byref(_C.AdapterBank(a.data_ptr(), b.data_ptr(), s.data_ptr(), self.num_adapters, self.rank,
+                                           self.in_features, self.out_features, _C.dt(a)))
 
     def _form(self, key, x: torch.Tensor, batch: AdapterBatch, base: Optional[torch.Tensor], keep: bool,
               inplace: bool):
@@ -254,14 +257,17 @@ class AdapterBank(nn.Module):
         return form
 
     def _run(self, x: torch.Tensor, batch: AdapterBatch, base: Optional[torch.Tensor], keep: bool, inplace: bool):
-        """(out, low, form, a, b, scaling)"""
-        key = (x.dtype, x.shape, x.stride(), x.device, batch._sig, keep, inplace,
-               None if base is None else (base.dtype, base.shape, base.stride(), base.device))
+        """(out, low, form, bank by reference, a, b, scaling, x as it was read)"""
+        if base is None:
+            key = (x.dtype, x.shape, x.stride(), x.device, batch._sig, keep)
+        else:
+            key = (x.dtype, x.shape, x.stride(), x.device, batch._sig, keep, inplace, base.dtype, base.shape, base.stride(),
+                   base.device)
         form = self._forms.get(key)
         if form is None:
             form = self._form(key, x, batch, base, keep, inplace)
         ref, nbytes, shape, copy_x, copy_base, _ = form
-        a, b, s = self._weights(x)
+        bank, a, b, s = self._weights(x)
         dev = x.device
         if copy_x:
             x = x.contiguous() if not x.is_contiguous() else x.clone()
@@ -283,9 +289,9 @@ class AdapterBank(nn.Module):
         out = base if inplace else torch.empty(shape, dtype=x.dtype, device=dev)
         low = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         if batch.tokens:
-            _call(dev, "lq_adapter_forward", self._struct(a, b, s), ref, batch._plan.data_ptr(), at, base_at,
+            _call(dev, "lq_adapter_forward", bank, ref, batch._plan.data_ptr(), at, base_at,
                   out.data_ptr(), None if low is None else low.data_ptr(), nbytes)
-        return out, low, form, a, b, s, x
+        return out, low, form, bank, a, b, s, x
 
     def forward(self, x: torch.Tensor, batch: AdapterBatch, base: Optional[torch.Tensor] = None) -> torch.Tensor:
         """base [..., out_features] (default zeros) plus each token's adapter of
@@ -317,38 +323,45 @@ class _Adapters(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, lora_A, lora_B, base, bank, batch):
-        y, low, form, a, b, s, rows = bank._run(x, batch, base, True, False)
-        # the weights as the call rounded them; all of these raise if they were changed since
-        ctx.save_for_backward(rows, a, b, low, s, batch._plan)
-        ctx.bank, ctx.form, ctx.shape, ctx.dtype = bank, form, x.shape, lora_A.dtype
+        y, low, form, ref, a, b, s, rows = bank._run(x, batch, base, True, False)
+        ctx.save_for_backward(rows, a, b)  # the weights as the call rounded them
+        # low is nobody else's; scaling and the plan may be written to
+        ctx.call = (low, form, ref, s, s._version, batch._plan, batch._plan._version, x.shape, lora_A.dtype)
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        if torch.is_grad_enabled():
+            raise RuntimeError("AdapterBank: gradients of gradients are not computed")
         want_x, want_a, want_b, want_base = ctx.needs_input_grad[:4]
         dx = da = db = None
         if want_x or want_a or want_b:
-            x, a, b, low, s, plan = ctx.saved_tensors
+            x, a, b = ctx.saved_tensors
+            low, (form, nbytes, _, _, _, c), ref, s, s_version, plan, plan_version, shape, dtype = ctx.call
+            if s._version != s_version or plan._version != plan_version:
+                raise RuntimeError("AdapterBank: scaling or the batch's plan has been modified by an inplace operation "
+                                   "since the forward pass")
             dev = x.device
             if want_x:
-                dx = torch.empty(ctx.shape, dtype=x.dtype, device=dev)
+                dx = torch.empty(shape, dtype=x.dtype, device=dev)
             if want_a:
-                da = torch.empty(a.shape, dtype=ctx.dtype, device=dev)
+                da = torch.empty(a.shape, dtype=dtype, device=dev)
             if want_b:
-                db = torch.empty(b.shape, dtype=ctx.dtype, device=dev)
-            bank, (form, nbytes, _, _, _, c) = ctx.bank, ctx.form
+                db = torch.empty(b.shape, dtype=dtype, device=dev)
+            out_features = b.shape[2]
             d = dy
-            stride = _row_stride(d)
+            stride = out_features
+            if not d.is_contiguous():
+                stride = _row_stride(d)
             if stride is None or d.data_ptr() & 15:
                 d = d.clone(memory_format=torch.contiguous_format)
-                stride = bank.out_features
-            if stride != bank.out_features:
+                stride = out_features
+            if stride != c.out_stride:
                 form = ctypes.byref(_C.AdapterForm(c.n, c.x_stride, 0, stride, 1))
-            ref = bank._struct(a, b, s)
             ws_bytes = _C.lib().lq_adapter_backward_workspace_bytes(ref, c.n)
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-            _call(dev, "lq_adapter_backward", ref, form, plan.data_ptr(), x.data_ptr(), d.data_ptr(), _C.ptr(low), nbytes,
-                  _C.ptr(dx), _C.ptr(da), _C.ptr(db), _C.dt(ctx.dtype) if da is not None or db is not None else _C.dt(x),
+            _call(dev, "lq_adapter_backward", ref, form, plan.data_ptr(), x.data_ptr(), d.data_ptr(),
+                  None if low is None else low.data_ptr(), nbytes, None if dx is None else dx.data_ptr(),
+                  None if da is None else da.data_ptr(), None if db is None else db.data_ptr(), _C.TORCH_TO_LQ[dtype],
                   ws.data_ptr(), ws_bytes)
         return dx, da, db, dy if want_base else None, None, None
