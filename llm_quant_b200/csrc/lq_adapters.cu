@@ -145,12 +145,21 @@ extern "C" int lq_adapter_plan(const void* ids, int ids_dtype, int64_t n_ids, in
   return launched("ad_plan_kernel");
 }
 
-// Up to here a cluster works at each token: one launch, and weights that tokens
-// share come from L2 again; above, tiles of tokens share them.
-static bool few_tokens(const lq_adapter_form* f) { return !f->keep && f->n <= kAdFewTokens; }
+// Whether a call takes ad_few, where every token reads its adapter's weights,
+// through L2 where tokens share them, or the tiles, where an adapter's tokens
+// share a read but two launches and a tile's fixed costs stand against it.
+// Measured (us, ad_few / tiles, K, N = 4096, ranks 16 and 64): 64 tokens of 1
+// adapter 5.6 / 14, 11 / 16, of 64 adapters 8.4 / 31, 21 / 41; 256 of 1 10.5 / 16,
+// 31 / 20, of 64 13 / 31, 44 / 41.  14336 to 4096 features, rank 64: 64 of 1
+// 20 / 23, 128 of 1 34 / 26, 128 of 64 52 / 63, 256 of 64 77 / 63.
+static bool few_tokens(const lq_adapter_bank& b, const lq_adapter_form* f) {
+  if (f->keep || f->n > 1024) return false;
+  const int64_t weights = 2 * b.R * (b.K + b.N), users = f->n < b.L ? f->n : b.L;
+  return f->n <= 64 || f->n * weights <= (96 << 20) + 2 * users * weights;
+}
 
 extern "C" size_t lq_adapter_low_bytes(const lq_adapter_bank* bank, const lq_adapter_form* form) {
-  if (!bank || !form || !sizes_ok(*bank, form->n) || few_tokens(form)) return 0;
+  if (!bank || !form || !sizes_ok(*bank, form->n) || few_tokens(*bank, form)) return 0;
   return ad_low_bytes(*bank, form->n, form->keep != 0);
 }
 
@@ -167,7 +176,7 @@ extern "C" int lq_adapter_forward(const lq_adapter_bank* bank, const lq_adapter_
   const size_t need = lq_adapter_low_bytes(bank, form);
   LQ_REQUIRE(need == 0 || (low && aligned16(low) && low_bytes >= need), LQ_EINVAL, "adapters: low must have %zu bytes, on 16", need);
   const AdCall a = {bank, ad_plan(plan, n, bank->L), n, as_stream(stream)};
-  if (few_tokens(form)) return ad_few(a, x, form->x_stride, base, form->base_stride, out, form->out_stride);
+  if (few_tokens(*bank, form)) return ad_few(a, x, form->x_stride, base, form->base_stride, out, form->out_stride);
   LQ_TRY(ad_down(a, x, form->x_stride, true, low, form->keep != 0));
   return ad_up(a, low, false, base, form->base_stride, out, form->out_stride);
 }

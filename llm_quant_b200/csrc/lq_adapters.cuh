@@ -9,7 +9,6 @@ namespace lq {
 constexpr int kAdTile = 128;        // tokens of a tile
 constexpr int kAdMaxAdapters = 8192;
 constexpr int kAdMaxRank = 128;
-constexpr int kAdFewTokens = 64;    // up to here a call without gradients takes ad_few
 
 // A tile: up to 128 tokens of one adapter (owner -1: of none), at places first
 // .. first + rows - 1 of `order`; run is the first one's token if all follow

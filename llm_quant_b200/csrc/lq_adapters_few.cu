@@ -1,11 +1,11 @@
 // lq_adapters_few.cu -- the adapter bank for a few tokens: out = base + B^T (s A x)
-// for each token by a cluster of eight blocks, in one launch.
+// for each token by a cluster of one to eight blocks, in one launch.
 //
 // A decode step's product is its adapters' weights once through the SMs, and
 // its time the length of the chain: load A, sum over K, exchange, load B, add.
-// Each block takes an eighth of K for all ranks, then an eighth of the
-// columns; the eight partial sums of a rank meet in distributed shared memory
-// (added block by block, in order), and the loads of B and of base do not wait
+// Each block takes its part of K for all ranks, then its part of the
+// columns; the partial sums of a rank meet in distributed shared memory (added
+// block by block, in order), and the loads of B and of base do not wait
 // for that: they are on their way before the exchange.  Everything is fp32
 // with one rounding at the end.
 #include "lq_adapters.cuh"
@@ -13,7 +13,7 @@
 namespace lq {
 namespace {
 
-constexpr int kFewBlocks = 8, kFewThreads = 256, kFewWarps = kFewThreads / 32;
+constexpr int kFewThreads = 256, kFewWarps = kFewThreads / 32;
 constexpr int kFewAhead = 8;  // ranks of B that a thread has on their way before the exchange
 
 __device__ __forceinline__ float ld_peer(const float* p, uint32_t rank) {
@@ -38,8 +38,9 @@ __device__ __forceinline__ void unpack8(const uint4& w, float* f) {
   }
 }
 
-// RW: ranks of a warp (the rank, rounded up, over the block's eight warps)
-template <typename T, int RW>
+// RW: ranks of a warp (the rank, rounded up, over the block's eight warps); C: blocks
+// of a token
+template <typename T, int RW, int C>
 __global__ void __launch_bounds__(kFewThreads, 2)
     ad_few_kernel(const T* __restrict__ x, int64_t x_stride, const T* __restrict__ a, const T* __restrict__ b,
                   const float* __restrict__ scaling, int R, int K, int N, const int* __restrict__ owner, const T* base,
@@ -49,11 +50,11 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   __shared__ float more[kFewThreads * 8];  // sums of the threads that share columns
   pdl_wait();
   pdl_trigger();
-  const int64_t t = blockIdx.x / kFewBlocks;
-  const int blk = blockIdx.x % kFewBlocks, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t t = blockIdx.x / C;
+  const int blk = blockIdx.x % C, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int o = owner[t];
   const int units = N / 8;  // of 8 columns
-  const int c0 = units * blk / kFewBlocks, c1 = units * (blk + 1) / kFewBlocks;
+  const int c0 = units * blk / C, c1 = units * (blk + 1) / C;
   if (o < 0) {  // the whole cluster
     if (base == out) return;
     for (int c = c0 + tid; c < c1; c += kFewThreads) {
@@ -77,12 +78,13 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   }
   if (first && g == 0 && base) y = *reinterpret_cast<const uint4*>(base + t * base_stride + 8 * (c0 + at));
   // sums over this block's part of K
-  const int ku = K / 8, k0 = ku * blk / kFewBlocks, k1 = ku * (blk + 1) / kFewBlocks;
+  const int ku = K / 8, k0 = ku * blk / C, k1 = ku * (blk + 1) / C;
   float s[RW];
 #pragma unroll
   for (int j = 0; j < RW; ++j) s[j] = 0.0f;
   const T* xo = x + t * x_stride;
   const T* ao = a + ((int64_t)o * R + warp) * K;
+#pragma unroll (RW <= 2 ? 4 : RW <= 4 ? 2 : 1)
   for (int k = k0 + lane; k < k1; k += 32) {
     const uint4 xw = *reinterpret_cast<const uint4*>(xo + 8 * k);
     uint4 aw[RW];
@@ -106,14 +108,15 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   if (lane == 0)
 #pragma unroll
     for (int j = 0; j < RW; ++j) part[warp + j * kFewWarps] = s[j];
-  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+  if (C > 1) asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+  else __syncthreads();
   if (tid < R) {
     float v = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kFewBlocks; ++i) v += ld_peer(&part[tid], i);
+    for (int i = 0; i < C; ++i) v += C > 1 ? ld_peer(&part[tid], i) : part[tid];
     u[tid] = v * scaling[o];
   }
-  asm volatile("barrier.cluster.arrive.release;" ::: "memory");  // waited for at the end: others may still read part
+  if (C > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");  // waited for at the end: others may still read part
   __syncthreads();
   for (int c = c0; c < c1; c += per) {
     const bool some = c + at < c1;
@@ -135,7 +138,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
       } else if (g == 0 && base) {
         y = *reinterpret_cast<const uint4*>(base + t * base_stride + 8 * (c + at));
       }
-#pragma unroll 4
+#pragma unroll 8
       for (; r < R; r += G) {
         float f[8];
         unpack8<T>(__ldg(reinterpret_cast<const uint4*>(bo + (int64_t)r * N + 8 * (c + at))), f);
@@ -162,29 +165,38 @@ __global__ void __launch_bounds__(kFewThreads, 2)
       *reinterpret_cast<uint4*>(out + t * out_stride + 8 * (c + at)) = w.u;
     }
   }
-  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+  if (C > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 
-template <typename T, int RW>
-int few_rw(const AdCall& a, const void* x, int64_t xs, const void* base, int64_t bs, void* out, int64_t os) {
+template <typename T, int RW, int C>
+int few_c(const AdCall& a, const void* x, int64_t xs, const void* base, int64_t bs, void* out, int64_t os) {
   const lq_adapter_bank& b = *a.bank;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.n * kFewBlocks));
+  cfg.gridDim = dim3((unsigned)(a.n * C));
   cfg.blockDim = dim3(kFewThreads);
   cfg.stream = a.st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = kFewBlocks;
+  attr[1].val.clusterDim.x = C;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, ad_few_kernel<T, RW>, static_cast<const T*>(x), xs, static_cast<const T*>(b.a),
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, ad_few_kernel<T, RW, C>, static_cast<const T*>(x), xs, static_cast<const T*>(b.a),
                                            static_cast<const T*>(b.b), b.scaling, (int)b.R, (int)b.K, (int)b.N,
                                            (const int*)a.plan.owner, static_cast<const T*>(base), bs, static_cast<T*>(out), os);
   LQ_REQUIRE(e == cudaSuccess, LQ_ECUDA, "ad_few_kernel launch: %s", cudaGetErrorString(e));
   return launched("ad_few_kernel");
+}
+// As many blocks to a token as are resident at once
+template <typename T, int RW>
+int few_rw(const AdCall& a, const void* x, int64_t xs, const void* base, int64_t bs, void* out, int64_t os) {
+  const int64_t room = 2 * num_sms();
+  if (a.n * 8 <= room) return few_c<T, RW, 8>(a, x, xs, base, bs, out, os);
+  if (a.n * 4 <= room) return few_c<T, RW, 4>(a, x, xs, base, bs, out, os);
+  if (a.n * 2 <= room) return few_c<T, RW, 2>(a, x, xs, base, bs, out, os);
+  return few_c<T, RW, 1>(a, x, xs, base, bs, out, os);
 }
 template <typename T>
 int few_t(const AdCall& a, const void* x, int64_t xs, const void* base, int64_t bs, void* out, int64_t os) {
