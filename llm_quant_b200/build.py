@@ -1,4 +1,5 @@
-"""Build liblq_sm100.so in-tree with nvcc for sm_100a (B200).
+"""Build liblq_sm100.so in-tree with nvcc for sm_100a (B200), and lq_torch.so, the
+torch bindings in C++ of the calls whose host time counts, with the host compiler.
 
     python -m llm_quant_b200.build        # or: python llm_quant_b200/build.py
 
@@ -22,6 +23,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "_lib")
 OBJDIR = os.path.join(HERE, "_lib", "obj")
 LIB = os.path.join(LIBDIR, "liblq_sm100.so")
+EXT = os.path.join(LIBDIR, "lq_torch.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -69,18 +71,57 @@ def _compile(src: str, force: bool, verbose: bool) -> str:
     return obj
 
 
+def _compile_ext(force: bool) -> str:
+    """lq_torch.cpp against the installed torch's headers."""
+    src, obj = os.path.join(CSRC, "lq_torch.cpp"), os.path.join(OBJDIR, "lq_torch.o")
+    header = os.path.join(INCLUDE, "lq_sm100.h")
+    if not force and os.path.exists(obj) and os.path.getmtime(obj) >= max(os.path.getmtime(src), os.path.getmtime(header)):
+        return obj
+    import sysconfig
+    import torch
+    root = os.path.join(os.path.dirname(torch.__file__), "include")
+    cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-c", src, "-o", obj,
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", "-DTORCH_API_INCLUDE_EXTENSION_H"]
+    for d in (root, os.path.join(root, "torch", "csrc", "api", "include"), cuda, sysconfig.get_paths()["include"]):
+        cmd += ["-isystem", d]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"the host compiler failed for lq_torch.cpp:\n{r.stdout}\n{r.stderr}")
+    return obj
+
+
+def _link_ext(obj: str, force: bool) -> None:
+    if not force and os.path.exists(EXT) and os.path.getmtime(EXT) >= os.path.getmtime(obj):
+        return
+    import torch
+    tmp = EXT + ".tmp"
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    # torch's own libstdc++, never a static one: two copies in a process do not share
+    # their locales, and formatting a number in the second one ends it
+    cmd = [os.environ.get("CXX", "g++"), "-shared", "-o", tmp, obj, LIB, "-Wl,-rpath,$ORIGIN", f"-L{libs}", "-lc10", "-ltorch_cpu",
+           "-ltorch_python", "-lc10_cuda", "-ltorch_cuda", "-nostdlib++", "-l:libstdc++.so.6"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, EXT)
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(OBJDIR, exist_ok=True)
     srcs = _sources()
-    with ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
+    with ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as ex:
+        ext = ex.submit(_compile_ext, force)
         objs = list(ex.map(lambda s: _compile(s, force, verbose), srcs))
+        ext = ext.result()
     if force or not os.path.exists(LIB) or os.path.getmtime(LIB) < max(os.path.getmtime(o) for o in objs):
         tmp = LIB + ".tmp"
-        cmd = [nvcc()] + ARCH + ["-shared", "-o", tmp] + objs
+        cmd = [nvcc()] + ARCH + ["-shared", "-Xlinker", "-soname=liblq_sm100.so", "-o", tmp] + objs
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         os.replace(tmp, LIB)
+    _link_ext(ext, force)
     return LIB
 
 

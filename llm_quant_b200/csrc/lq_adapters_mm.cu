@@ -182,7 +182,6 @@ __global__ void __launch_bounds__(160, 2) ad_down_kernel(const T* __restrict__ x
   __shared__ int failed, row_top[128];
   using H = Half16<T>;
   pdl_wait();
-  pdl_trigger();
   const int tile = blockIdx.x / split, rank = blockIdx.x - tile * split;
   if (tile >= p.tile_of[L]) return;  // the whole cluster
   const AdTile d = p.tiles[tile];
@@ -202,6 +201,9 @@ __global__ void __launch_bounds__(160, 2) ad_down_kernel(const T* __restrict__ x
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // only now: a block of the next kernel that took its tensor memory on this SM
+  // first would wait for this one, and this one for it
+  pdl_trigger();
   const uint32_t tmem = tmem_at;
   const int all = (K + 63) / 64, s0 = (int)((int64_t)all * rank / split), n = (int)((int64_t)all * (rank + 1) / split) - s0;
   if (warp < 4) {
@@ -368,8 +370,9 @@ __global__ void __launch_bounds__(kUpThreads, 1)
   __shared__ uint64_t full[NS], added[NS], empty[NS], f_full[NF], f_empty[NF], i_full[NI], i_empty[NI], d_full[2], d_empty[2], drain;
   __shared__ uint32_t tmem_at;
   __shared__ int failed;
-  pdl_wait();
-  pdl_trigger();
+  // Started while ad_down (or ad_sum) still runs, which began only when all before
+  // it had ended: base, F and the plan are there, and only the low-rank rows are
+  // waited for, by the warps that read them.  Nothing is written before them.
   // tokens without an adapter: nothing to do where out is base
   const int wide = (chunks + kUpBeside - 1) / kUpBeside * kUpBeside;  // of a tile; what is behind the columns is empty
   const int64_t units = (int64_t)p.tile_of[base == out ? L : L + 1] * (wide / kUpBeside);  // of each block of a group
@@ -396,11 +399,13 @@ __global__ void __launch_bounds__(kUpThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_trigger();
   const uint32_t tmem = tmem_at;
   volatile int* fail = &failed;
   int tile = (int)(u0 * kUpBeside / wide), chunk = (int)(u0 * kUpBeside - (int64_t)tile * wide + blockIdx.x % kUpBeside);
   if (warp < 8) {
     // ---- add: a thread to a row ----
+    pdl_wait();
     const int e = warp >> 2, row = (warp & 3) * 32 + lane;
     float back = 1.0f;
     bool some = false;
@@ -451,6 +456,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
     }
   } else if (warp < 16) {
     // ---- take out: half a warp to a row, a team every other unit ----
+    pdl_wait();
     const int team = (warp - 8) >> 2;
     const int c16 = lane & 15, row0 = (warp & 3) * 2 + (lane >> 4);  // its 16 bytes, and the first of its rows, 8 apart
     AdTile d = {};
@@ -546,6 +552,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
     cp_wait_all();
   } else {
     // ---- images and products ----
+    pdl_wait();
     constexpr uint32_t idesc = make_idesc(H::fmt, 128) | kMajorB;
     // the tile's image, and the next one where there is room for two
     int known = -1, images = 0, sent = 0, b = 0, used = 0;
@@ -658,8 +665,7 @@ __global__ void __launch_bounds__(kOuterLoaders + 32, OuterShared<NP>::blocks)
   __shared__ uint64_t full[NS], empty[NS], done, free_, drain;
   __shared__ uint32_t tmem_at;
   __shared__ int failed;
-  pdl_wait();
-  pdl_trigger();
+  // as ad_up: x, dy, u and the plan are there, v is waited for by those who read it
   const bool first_side = (int)blockIdx.x < one.chunks;
   const OuterSide<T>& q = first_side ? one : two;
   const int col0 = ((int)blockIdx.x - (first_side ? 0 : one.chunks)) * 256;
@@ -684,12 +690,14 @@ __global__ void __launch_bounds__(kOuterLoaders + 32, OuterShared<NP>::blocks)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_trigger();
   const uint32_t tmem = tmem_at;
   volatile int* fail = &failed;
   int step = 0, run = 0;  // 64-token steps and runs so far: the barriers' phases
   if (warp < kOuterLoaders / 32) {
     // warps 0 .. 3 bring X, a row of 512 bytes at a time; warps 4 .. 7 V
     const bool brings_x = warp < 4;
+    if (H::scaled || !brings_x) pdl_wait();
     const uint32_t at = base + (lane >> 3) * 8192;
     const bool in = col0 + lane * 8 < q.K;
     for (int t0 = t_lo; !any_failed<kOuterLoaders>(1, *fail) && t0 < t_hi; ++run) {
@@ -835,6 +843,7 @@ __global__ void __launch_bounds__(kOuterLoaders + 32, OuterShared<NP>::blocks)
       wait_warp(&drain, 0);
     }
   }
+  pdl_wait();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();

@@ -1,0 +1,191 @@
+// lq_torch.cpp -- the calls whose host time counts, bound to torch in C++:
+// AdapterBank's forward and backward pass and GradClipper's call.  They check
+// their arguments, allocate and call the C entry points of lq_sm100.h, as the
+// other modules do from Python through ctypes.  A decode step's adapters take
+// some 5 us on the device; the same calls took 11 us in Python, and a training
+// step 50 us more, most of it in Python on the autograd engine's thread.
+#include <torch/extension.h>
+
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include "../../include/lq_sm100.h"
+
+namespace {
+
+using at::Tensor;
+using OptTensor = std::optional<Tensor>;
+
+std::string name_of(at::ScalarType t) {
+  switch (t) {
+    case at::kFloat: return "float32";
+    case at::kHalf: return "float16";
+    case at::kBFloat16: return "bfloat16";
+    default: return c10::toString(t);
+  }
+}
+int code_of(at::ScalarType t) { return t == at::kFloat ? LQ_F32 : t == at::kHalf ? LQ_F16 : LQ_BF16; }
+
+void check(int status) {
+  if (status == LQ_OK) return;
+  const std::string m = lq_last_error();
+  TORCH_CHECK_VALUE(status != LQ_EINVAL && status != LQ_ERANGE, m);
+  TORCH_CHECK_TYPE(status != LQ_EDTYPE, m);
+  TORCH_CHECK(false, m, " (status ", status, ")");
+}
+
+bool on16(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
+
+// Elements from row to row of x [..., width], or -1 where the kernels cannot
+// read its rows as they lie: values side by side, one stride over all leading
+// dimensions, rows on 16 bytes.
+int64_t row_stride(const Tensor& x) {
+  const int64_t width = x.size(-1);
+  if (x.is_contiguous()) return on16(x) || x.numel() == 0 ? width : -1;
+  if (x.numel() == 0 || x.stride(-1) != 1 || !on16(x)) return -1;
+  int64_t rows = 1, stride = -1;
+  for (int64_t d = x.dim() - 2; d >= 0; --d) {
+    if (x.size(d) == 1) continue;
+    if (stride < 0) stride = x.stride(d);
+    else if (x.stride(d) != rows * stride) return -1;
+    rows *= x.size(d);
+  }
+  return stride < 0 ? width : stride % 8 == 0 ? stride : -1;
+}
+// x as rows that the kernels can read, laid out anew if need be
+Tensor rows_of(const Tensor& x, int64_t& stride) {
+  stride = row_stride(x);
+  if (stride >= 0) return x;
+  stride = x.size(-1);
+  return x.clone(at::MemoryFormat::Contiguous);
+}
+
+struct Call {
+  lq_adapter_bank bank;
+  lq_adapter_form form;
+  Tensor a, b, s, x, low, out;
+};
+
+Call run(const Tensor& x, const Tensor& lora_a, const Tensor& lora_b, const Tensor& scaling, const OptTensor& base,
+         const Tensor& plan, int64_t tokens, int64_t num_adapters, bool keep, bool in_place) {
+  TORCH_CHECK(x.is_cuda(), "AdapterBank: expected a CUDA tensor, got device ", x.device(), " (llm_quant_b200 has no CPU implementation)");
+  const auto type = x.scalar_type();
+  TORCH_CHECK_TYPE(type == at::kHalf || type == at::kBFloat16, "AdapterBank: unsupported dtype ", name_of(type), " (float16, bfloat16)");
+  TORCH_CHECK(lora_a.dim() == 3 && lora_b.dim() == 3 && lora_a.size(0) == lora_b.size(0) && lora_a.size(1) == lora_b.size(1) &&
+                  scaling.dim() == 1 && scaling.size(0) == lora_a.size(0),
+              "AdapterBank: lora_A ", lora_a.sizes(), ", lora_B ", lora_b.sizes(), " and scaling ", scaling.sizes(), " do not go together");
+  const int64_t L = lora_a.size(0), R = lora_a.size(1), K = lora_a.size(2), N = lora_b.size(2);
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) == K && x.numel() == tokens * K, "AdapterBank: x ", x.sizes(), " is not ", tokens,
+              " tokens of ", K, " features");
+  TORCH_CHECK_VALUE(num_adapters == L, "AdapterBank: a batch for ", num_adapters, " adapters, a bank of ", L);
+  TORCH_CHECK(lora_a.device() == x.device() && lora_b.device() == x.device() && scaling.device() == x.device() &&
+                  plan.device() == x.device(),
+              "AdapterBank: x on ", x.device(), ", the bank on ", lora_a.device(), ", the batch on ", plan.device());
+  TORCH_CHECK_TYPE(lora_a.scalar_type() == lora_b.scalar_type() && scaling.scalar_type() == at::kFloat, "AdapterBank: lora_A is ",
+                   name_of(lora_a.scalar_type()), ", lora_B ", name_of(lora_b.scalar_type()), ", scaling ",
+                   name_of(scaling.scalar_type()), " (expected float32)");
+  at::DimVector shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = N;
+  if (base)
+    TORCH_CHECK(base->scalar_type() == type && base->device() == x.device() && base->sizes() == at::IntArrayRef(shape),
+                "AdapterBank: base ", base->sizes(), " ", name_of(base->scalar_type()), " on ", base->device(), " for x ", x.sizes(),
+                " ", name_of(type), " on ", x.device());
+  Call c;
+  c.form = {tokens, K, N, N, keep};
+  c.x = rows_of(x, c.form.x_stride);
+  Tensor from;
+  if (in_place) {
+    const int64_t stride = row_stride(*base);
+    TORCH_CHECK_VALUE(stride >= 0 && (tokens <= 1 || stride >= N), "AdapterBank.add_: y ", base->sizes(), " with strides ",
+                      base->strides(), " must be rows on 16 bytes");
+    c.form.base_stride = c.form.out_stride = stride;
+    from = c.out = *base;
+  } else {
+    if (base) from = rows_of(*base, c.form.base_stride);
+    c.out = at::empty(shape, x.options().requires_grad(false));
+  }
+  const auto ready = [&](const Tensor& t) {
+    const Tensor u = t.scalar_type() == type ? t : t.to(type);
+    return u.is_contiguous() && on16(u) ? u : u.clone(at::MemoryFormat::Contiguous);
+  };
+  c.a = ready(lora_a), c.b = ready(lora_b), c.s = scaling.contiguous();
+  c.bank = {c.a.data_ptr(), c.b.data_ptr(), c.s.data_ptr<float>(), L, R, K, N, code_of(type)};
+  if (tokens == 0) return c;
+  const size_t low = lq_adapter_low_bytes(&c.bank, &c.form);
+  if (low) c.low = at::empty({(int64_t)low}, plan.options());
+  check(lq_adapter_forward(&c.bank, &c.form, plan.data_ptr(), c.x.data_ptr(), from.defined() ? from.data_ptr() : nullptr,
+                           c.out.data_ptr(), low ? c.low.data_ptr() : nullptr, low, at::cuda::getCurrentCUDAStream()));
+  return c;
+}
+
+// base + each token's adapter of x, with the gradients of x, lora_A, lora_B and base
+struct Adapters : torch::autograd::Function<Adapters> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& lora_a, const Tensor& lora_b,
+                        const OptTensor& base, const Tensor& scaling, const Tensor& plan, int64_t tokens, int64_t num_adapters) {
+    Call c = run(x, lora_a, lora_b, scaling, base, plan, tokens, num_adapters, true, false);
+    // the weights as the call rounded them; all of these raise if they were changed since
+    ctx->save_for_backward({c.x, c.a, c.b, scaling, plan, c.low});
+    ctx->saved_data["shape"] = x.sizes().vec();
+    ctx->saved_data["type"] = static_cast<int64_t>(lora_a.scalar_type());
+    ctx->saved_data["stride"] = c.form.x_stride;
+    ctx->saved_data["base"] = base.has_value();
+    return c.out;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "AdapterBank: gradients of gradients are not computed");
+    torch::autograd::variable_list out(8);
+    Tensor dy = grads[0];
+    if (!dy.defined()) return out;
+    const bool want[3] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2)};
+    if (ctx->saved_data["base"].toBool()) out[3] = dy;
+    if (!want[0] && !want[1] && !want[2]) return out;
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &a = saved[1], &b = saved[2], &plan = saved[4], &low = saved[5];
+    const Tensor s = saved[3].contiguous();
+    const c10::cuda::CUDAGuard guard(x.device());
+    const auto type = static_cast<at::ScalarType>(ctx->saved_data["type"].toInt());
+    const auto shape = ctx->saved_data["shape"].toIntVector();
+    const lq_adapter_bank bank = {a.data_ptr(), b.data_ptr(), s.data_ptr<float>(), a.size(0), a.size(1), a.size(2), b.size(2),
+                                  code_of(x.scalar_type())};
+    const int64_t n = x.numel() / a.size(2);
+    lq_adapter_form form = {n, ctx->saved_data["stride"].toInt(), 0, 0, 1};
+    const Tensor d = rows_of(dy, form.out_stride);
+    if (want[0]) out[0] = at::empty(shape, x.options());
+    if (want[1]) out[1] = at::empty(a.sizes(), x.options().dtype(type));
+    if (want[2]) out[2] = at::empty(b.sizes(), x.options().dtype(type));
+    const size_t bytes = lq_adapter_backward_workspace_bytes(&bank, n);
+    const Tensor ws = at::empty({(int64_t)bytes}, plan.options());
+    const auto at = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+    check(lq_adapter_backward(&bank, &form, plan.data_ptr(), x.data_ptr(), d.data_ptr(), at(low), low.defined() ? low.numel() : 0,
+                              at(out[0]), at(out[1]), at(out[2]), code_of(type), ws.data_ptr(), bytes,
+                              at::cuda::getCurrentCUDAStream()));
+    return out;
+  }
+};
+
+Tensor adapters_forward(const Tensor& x, const Tensor& lora_a, const Tensor& lora_b, const Tensor& scaling, const OptTensor& base,
+                        const Tensor& plan, int64_t tokens, int64_t num_adapters) {
+  const c10::OptionalDeviceGuard guard(x.is_cuda() ? std::make_optional(x.device()) : std::nullopt);
+  if (at::GradMode::is_enabled() &&
+      (x.requires_grad() || lora_a.requires_grad() || lora_b.requires_grad() || (base && base->requires_grad())))
+    return Adapters::apply(x, lora_a, lora_b, base, scaling, plan, tokens, num_adapters);
+  return run(x, lora_a, lora_b, scaling, base, plan, tokens, num_adapters, false, false).out;
+}
+
+void adapters_add_(const Tensor& y, const Tensor& x, const Tensor& lora_a, const Tensor& lora_b, const Tensor& scaling,
+                   const Tensor& plan, int64_t tokens, int64_t num_adapters) {
+  TORCH_CHECK(!at::GradMode::is_enabled() ||
+                  !(x.requires_grad() || y.requires_grad() || lora_a.requires_grad() || lora_b.requires_grad()),
+              "AdapterBank.add_: no gradient is computed here (use forward, or torch.no_grad())");
+  const c10::OptionalDeviceGuard guard(x.is_cuda() ? std::make_optional(x.device()) : std::nullopt);
+  run(x, lora_a, lora_b, scaling, y, plan, tokens, num_adapters, false, true);
+  if (!y.is_inference()) y.unsafeGetTensorImpl()->bump_version();
+}
+
+}  // namespace
+
+PYBIND11_MODULE(lq_torch, m) {
+  m.def("adapters_forward", &adapters_forward);
+  m.def("adapters_add_", &adapters_add_);
+}
