@@ -104,6 +104,26 @@ __device__ __forceinline__ void bulk_load_at(uint32_t dst, const void* src, uint
                "r"(bytes), "r"(smem_u32(bar))
                : "memory");
 }
+// A box of a tensor map; what lies outside of the tensor reads as zeros.
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+// Rows of a call as tensor maps, where the rows lie one behind the other (ok:
+// else the rows are copied by threads); always 64 columns, 128 bytes, wide, on a
+// multiple of 64, with the 128-byte swizzle that the operands have.
+struct RowsMap {
+  CUtensorMap map;
+  int ok;
+};
 __device__ __forceinline__ int lane_id() { return threadIdx.x & 31; }
 __device__ __forceinline__ int token_of(const AdPlan& p, const AdTile& d, int row) {
   return d.run >= 0 ? d.run + row : p.order[d.first + row];
@@ -170,7 +190,8 @@ struct DownShared {
 };
 
 template <typename T, int NP>
-__global__ void __launch_bounds__(160, 2) ad_down_kernel(const T* __restrict__ x, int64_t stride, const T* __restrict__ f,
+__global__ void __launch_bounds__(160, 2) ad_down_kernel(const __grid_constant__ RowsMap xm, const __grid_constant__ CUtensorMap fm,
+                                                         const T* __restrict__ x, int64_t stride, const T* __restrict__ f,
                                                          const float* __restrict__ scaling, int R, int K, AdPlan p, int L,
                                                          Low low, int split) {
   using S = DownShared<NP>;
@@ -187,8 +208,11 @@ __global__ void __launch_bounds__(160, 2) ad_down_kernel(const T* __restrict__ x
   const AdTile d = p.tiles[tile];
   const int tid = threadIdx.x, warp = tid >> 5;
   const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
+  // a tile whose tokens follow each other comes by TMA (rows of others behind its
+  // own do no harm: each row of D is its own), any other by threads
+  const bool tma = xm.ok && d.run >= 0;
   if (tid == 0) {
-    for (int i = 0; i < NS; ++i) mbar_init(&full[i], 128), mbar_init(&empty[i], 1);
+    for (int i = 0; i < NS; ++i) mbar_init(&full[i], tma ? 1 : 128), mbar_init(&empty[i], 1);
     mbar_init(&done, 1);
     failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -206,7 +230,20 @@ __global__ void __launch_bounds__(160, 2) ad_down_kernel(const T* __restrict__ x
   pdl_trigger();
   const uint32_t tmem = tmem_at;
   const int all = (K + 63) / 64, s0 = (int)((int64_t)all * rank / split), n = (int)((int64_t)all * (rank + 1) / split) - s0;
-  if (warp < 4) {
+  if (warp < 4 && tma) {
+    for (int i = 0; i < n && warp == 0; ++i) {
+      const int slot = i % NS;
+      if (i >= NS && !wait_warp(&empty[slot], (i / NS - 1) & 1)) failed = 1;
+      if (*(volatile int*)&failed) break;
+      if (tid == 0) {
+        const uint32_t to = base + slot * S::stage;
+        mbar_expect_tx(&full[slot], S::stage);
+        tma_2d(to, &xm.map, (s0 + i) * 64, d.run, &full[slot]);
+        tma_3d(to + 16384, &fm, (s0 + i) * 64, 0, d.owner, &full[slot]);
+      }
+      __syncwarp();
+    }
+  } else if (warp < 4) {
     const int c = tid & 7, r0 = tid >> 3;
     const T* xr[8];
     const T* fr[NP / 16];
@@ -238,6 +275,8 @@ __global__ void __launch_bounds__(160, 2) ad_down_kernel(const T* __restrict__ x
       const int slot = i % NS;
       if (!wait_warp(&full[slot], (i / NS) & 1)) {
         failed = 1;
+        // what may still be on its way
+        for (int j = i + 1; j < min(n, i + NS); ++j) wait_warp(&full[j % NS], (j / NS) & 1);
         break;
       }
       proxy_fence();
@@ -340,28 +379,31 @@ __global__ void __launch_bounds__(160, 2) ad_down_kernel(const T* __restrict__ x
 // units, and two teams of two warps with bringing base.
 // ---------------------------------------------------------------------------
 constexpr int kUpBeside = 4;  // blocks that go along a tile's rows side by side, so that 1024 bytes of a row are asked for at a time
-constexpr int kUpThreads = 736;  // 8 warps add, 8 take out, 4 bring base, 2 bring F, 1 has the products
-constexpr int kUpRow = 256 + 16;  // bytes between rows of base in shared memory: 8 rows' pieces in all banks
+constexpr int kUpThreads = 704;  // 8 warps add, 8 take out, 4 bring base, 1 F, 1 has the products
 template <int NP>
 struct UpShared {
-  // Two stages of base are being taken out, the others are on their way: with
-  // one (three in all, each with its F) the loads' latency was what counted, 226 us
-  // instead of FIGURE for 16384 tokens and 14336 columns
-  static constexpr int stages = NP <= 32 ? 5 : NP <= 64 ? 4 : 3;
-  static constexpr int stage = 128 * kUpRow;
+  // Two stages of base are being added to, two taken out, the others on their way.
+  // An even number: a stage then is always the same team's and the same group's,
+  // who see each of its phases (a barrier's parity tells a phase from the next one
+  // only, and nothing else keeps the teams abreast).
+  static constexpr int stages = NP <= 32 ? 6 : 4;
+  static constexpr int stage = 32768;                   // two halves of 64 columns, rows of 128 bytes, swizzled
   static constexpr int fs = NP <= 64 ? 2 : 1;           // stages of F
   static constexpr int f_bytes = NP * 256;
-  static constexpr int images = NP <= 32 ? 2 : 1;
+  static constexpr int images = NP == 16 || NP == 64 ? 2 : 1;
   static constexpr int image = 128 * NP * 4;
   static constexpr int off_f = stages * stage, off_image = off_f + fs * f_bytes;
   static constexpr int bytes = off_image + images * image + 1024;
-  static_assert(stage % 1024 == 0 && f_bytes % 1024 == 0, "operands are swizzled in pieces of 1024 bytes");
+  static_assert(stages % 2 == 0, "a stage to a team");
+  static_assert(bytes <= 232448 && f_bytes % 1024 == 0, "shared memory; operands are swizzled in pieces of 1024 bytes");
 };
+// 16 bytes of a row of a stage
+__device__ __forceinline__ uint32_t up_at(int row, int c16) { return (c16 >> 3) * 16384 + row * 128 + (((c16 & 7) ^ (row & 7)) << 4); }
 
 template <typename T, int NP>
 __global__ void __launch_bounds__(kUpThreads, 1)
-    ad_up_kernel(const Low low, const T* __restrict__ f, int R, int N, AdPlan p, int L, const T* base, int64_t base_stride,
-                 T* out, int64_t out_stride, int chunks) {
+    ad_up_kernel(const __grid_constant__ RowsMap bm, const __grid_constant__ CUtensorMap fm, const Low low, int N, AdPlan p, int L,
+                 const T* base, int64_t base_stride, T* out, int64_t out_stride, int chunks) {
   using S = UpShared<NP>;
   using H = Half16<T>;
   constexpr int NS = S::stages, NF = S::fs, NI = S::images;
@@ -384,7 +426,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
   const uint32_t at = (smem_u32(raw) + 1023) & ~1023u;
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) mbar_init(&full[i], 64), mbar_init(&added[i], 128), mbar_init(&empty[i], 128);
-    for (int i = 0; i < NF; ++i) mbar_init(&f_full[i], 64), mbar_init(&f_empty[i], 1);
+    for (int i = 0; i < NF; ++i) mbar_init(&f_full[i], 1), mbar_init(&f_empty[i], 1);
     for (int i = 0; i < NI; ++i) mbar_init(&i_full[i], 1), mbar_init(&i_empty[i], 1);
     for (int i = 0; i < 2; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_empty[i], 128);
     mbar_init(&drain, 1);
@@ -392,7 +434,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     proxy_fence();
   }
-  if (warp == 22) {
+  if (warp == 21) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_at)), "r"(256u));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -424,7 +466,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
       __syncwarp();
       if (*fail) break;
       tc_fence_after();
-      const uint32_t mine = at + slot * S::stage + row * kUpRow, from = tmem + ((uint32_t)(warp & 3) << 21) + e * 128;
+      const uint32_t stage = at + slot * S::stage, from = tmem + ((uint32_t)(warp & 3) << 21) + e * 128;
       if (some) {
         // the next 32 columns leave tensor memory while these are added
         uint32_t v[2][32];
@@ -434,7 +476,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
           uint32_t* w = v[c & 1];
           uint4 y[4];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) y[q] = base ? lds_v4(mine + c * 64 + q * 16) : make_uint4(0u, 0u, 0u, 0u);
+          for (int q = 0; q < 4; ++q) y[q] = base ? lds_v4(stage + up_at(row, 4 * c + q)) : make_uint4(0u, 0u, 0u, 0u);
           tmem_wait_ld32(w);
           if (c < 3) tmem_ld32(from + c * 32 + 32, v[(c + 1) & 1]);
 #pragma unroll
@@ -446,7 +488,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
               const float v0 = __uint_as_float(w[8 * q + 2 * k]), v1 = __uint_as_float(w[8 * q + 2 * k + 1]);
               o[k] = H::scaled ? H::pack(fmaf(v0, back, b.x), fmaf(v1, back, b.y)) : H::pack(b.x + v0, b.y + v1);
             }
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + c * 64 + q * 16), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + up_at(row, 4 * c + q)), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
           }
         }
       }
@@ -475,14 +517,14 @@ __global__ void __launch_bounds__(kUpThreads, 1)
       if (!wait_lane(&added[slot], (i / NS) & 1)) *fail = 1;
       __syncwarp();
       if (*fail) break;
-      const uint32_t from = at + slot * S::stage + row0 * kUpRow + c16 * 16;
+      const uint32_t from = at + slot * S::stage + up_at(row0, c16);  // 8 rows on: the same place of the swizzle
       T* to = out + chunk * 128 + c16 * 8;
       const bool in = chunk * 128 + c16 * 8 < N, some = d.owner >= 0 || base;
 #pragma unroll
       for (int j0 = 0; j0 < 16; j0 += 8) {
         uint4 y[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = lds_v4(from + 8 * (j0 + j) * kUpRow);
+        for (int j = 0; j < 8; ++j) y[j] = lds_v4(from + (j0 + j) * 1024);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int t = __shfl_sync(0xffffffffu, tok, (lane & 16) + j0 + j);
@@ -496,7 +538,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
     const int team = (warp - 16) >> 1, w2 = warp & 1, c16 = lane & 15, row0 = w2 * 2 + (lane >> 4);
     AdTile d = {};
     int tok[2] = {-1, -1};  // lane k: of rows row0(k) + 4 (k % 16), and 64 later
-    int known = -1;
+    int known = -1, sent = 0;
     for (int i = 0; i < n; ++i, chunk += kUpBeside) {
       if (chunk >= wide) chunk -= wide, ++tile;
       if ((i & 1) != team) continue;
@@ -513,43 +555,57 @@ __global__ void __launch_bounds__(kUpThreads, 1)
       if (i >= NS && !wait_lane(&empty[slot], (i / NS - 1) & 1)) *fail = 1;
       __syncwarp();
       if (*fail) break;
+      sent = i + 1;
       const uint32_t stage = at + slot * S::stage;
       const int col = chunk * 128 + c16 * 8;
       const bool in = col < N;
+      if (base && bm.ok && d.run >= 0) {
+        // rows of other tiles behind the tile's own are not taken out
+        if (w2 == 0 && lane == 0) {
+          mbar_expect_tx(&full[slot], S::stage);
+          tma_2d(stage, &bm.map, chunk * 128, d.run, &full[slot]);
+          tma_2d(stage + 16384, &bm.map, chunk * 128 + 64, d.run, &full[slot]);
+        } else {
+          mbar_arrive(&full[slot]);
+        }
+        __syncwarp();
+        continue;
+      }
       if (base) {
         const T* from = base + (in ? col : 0);
 #pragma unroll
         for (int j = 0; j < 32; ++j) {
           const int t = __shfl_sync(0xffffffffu, tok[j >> 4], (lane & 16) + (j & 15));
-          if (in && t >= 0) cp16(stage + (row0 + 4 * j) * kUpRow + c16 * 16, from + (int64_t)t * base_stride, true);
+          if (in && t >= 0) cp16(stage + up_at(row0 + 4 * j, c16), from + (int64_t)t * base_stride, true);
         }
       }
       cp_arrive(&full[slot]);
     }
     cp_wait_all();
-  } else if (warp < 22) {
-    // ---- F: 128 columns of the adapter's rows ----
-    const int c16 = lane & 15, row0 = (warp & 1) * 2 + (lane >> 4);
+    if (*fail)  // boxes that were sent for arrive before their memory goes
+      for (int i = max(sent - NS, 0); i < sent; ++i)
+        if ((i & 1) == team) wait_lane(&full[i % NS], (i / NS) & 1);
+  } else if (warp == 20) {
+    // ---- F: 128 columns of the adapter's rows, zeros behind the rank (they meet zeros of the image) ----
     int known = -1, owner = -1, sent = 0;
     for (int i = 0; i < n; ++i, chunk += kUpBeside) {
       if (chunk >= wide) chunk -= wide, ++tile;
       if (tile != known) owner = p.tiles[tile].owner, known = tile;
       if (owner < 0) continue;
       const int fs = sent % NF;
-      if (sent >= NF && !wait_lane(&f_empty[fs], (sent / NF - 1) & 1)) *fail = 1;
-      __syncwarp();
+      if (sent >= NF && !wait_warp(&f_empty[fs], (sent / NF - 1) & 1)) *fail = 1;
       if (*fail) break;
-      const int col = chunk * 128 + c16 * 8;
-      const bool in = col < N;
-      const T* from = f + (int64_t)owner * R * N + (in ? col : 0);
-      const uint32_t to = at + S::off_f + fs * S::f_bytes + (c16 >> 3) * (NP * 128);
-#pragma unroll 16
-      for (int r = row0; r < NP; r += 4)  // zeros behind the rank: they meet zeros of the image
-        cp16(to + r * 128 + (((c16 & 7) ^ (r & 7)) << 4), from + (int64_t)min(r, R - 1) * N, in && r < R);
-      cp_arrive(&f_full[fs]);
+      if (lane == 0) {
+        const uint32_t to = at + S::off_f + fs * S::f_bytes;
+        mbar_expect_tx(&f_full[fs], S::f_bytes);
+        tma_3d(to, &fm, chunk * 128, 0, owner, &f_full[fs]);
+        tma_3d(to + NP * 128, &fm, chunk * 128 + 64, 0, owner, &f_full[fs]);
+      }
+      __syncwarp();
       ++sent;
     }
-    cp_wait_all();
+    if (*fail)  // what was sent for arrives before its memory goes
+      for (int k = max(sent - NF, 0); k < sent; ++k) wait_warp(&f_full[k % NF], (k / NF) & 1);
   } else {
     // ---- images and products ----
     pdl_wait();
@@ -620,7 +676,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
   __syncthreads();
   tc_fence_after();
   if (tid == 0 && failed) *p.status = LQ_ETIMEOUT;
-  if (warp == 22) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u));
+  if (warp == 21) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u));
 }
 
 // ---------------------------------------------------------------------------
@@ -656,7 +712,8 @@ struct OuterSide {
 
 template <typename T, int NP, typename G>
 __global__ void __launch_bounds__(kOuterLoaders + 32, OuterShared<NP>::blocks)
-    ad_outer_kernel(const OuterSide<T> one, const OuterSide<T> two, int R, AdPlan p, int L) {
+    ad_outer_kernel(const __grid_constant__ RowsMap one_m, const __grid_constant__ RowsMap two_m, const OuterSide<T> one,
+                    const OuterSide<T> two, int R, AdPlan p, int L) {
   using S = OuterShared<NP>;
   using H = Half16<T>;
   constexpr int NS = S::stages, VI = NP / 16;  // 8 tokens of a rank, of a lane that brings V
@@ -668,6 +725,7 @@ __global__ void __launch_bounds__(kOuterLoaders + 32, OuterShared<NP>::blocks)
   // as ad_up: x, dy, u and the plan are there, v is waited for by those who read it
   const bool first_side = (int)blockIdx.x < one.chunks;
   const OuterSide<T>& q = first_side ? one : two;
+  const RowsMap& xm = first_side ? one_m : two_m;
   const int col0 = ((int)blockIdx.x - (first_side ? 0 : one.chunks)) * 256;
   const int n_tiles = p.tile_of[L], per = (n_tiles + gridDim.y - 1) / gridDim.y;
   const int t_lo = blockIdx.y * per, t_hi = min(t_lo + per, n_tiles);
@@ -720,13 +778,30 @@ __global__ void __launch_bounds__(kOuterLoaders + 32, OuterShared<NP>::blocks)
           const int row = i * 64 + warp + 4 * lane;
           return lane < 16 && row < rows ? p.order[first + row] : -1;
         };
-        int next = token(0);
+        // the token of a step's first row if all its 64 rows are there and follow each other: it comes by TMA
+        auto whole = [&](int i) {
+          const AdTile d = p.tiles[t0 + (i >> 1)];
+          const int r = (i & 1) * 64;
+          return xm.ok && d.run >= 0 && r + 64 <= d.rows ? d.run + r : -1;
+        };
+        int next = token(0), next_box = whole(0);
         for (int i = 0; i < n; ++i) {
-          const int slot = (step + i) % NS, now = next;
-          if (i + 1 < n) next = token(i + 1);
+          const int slot = (step + i) % NS, now = next, box = next_box;
+          if (i + 1 < n) next = token(i + 1), next_box = whole(i + 1);
           if (step + i >= NS && !wait_lane(&empty[slot], ((step + i) / NS - 1) & 1)) *fail = 1;
           __syncwarp();
           if (*fail) break;
+          if (box >= 0) {
+            if (tid == 0) {
+              mbar_expect_tx(&full[slot], 32768);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) tma_2d(base + slot * S::stage + j * 8192, &xm.map, col0 + j * 64, box, &full[slot]);
+            } else {
+              mbar_arrive(&full[slot]);
+            }
+            __syncwarp();
+            continue;
+          }
           const uint32_t to = at + slot * S::stage;
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
@@ -838,9 +913,10 @@ __global__ void __launch_bounds__(kOuterLoaders + 32, OuterShared<NP>::blocks)
       step += n;
       t0 = last + 1;
     }
-    if (*fail) {  // the products that were begun end before their memory goes
+    if (*fail) {  // the products that were begun, and boxes on their way, end before their memory goes
       commit(&drain);
       wait_warp(&drain, 0);
+      for (int i = 0; i < NS; ++i) wait_warp(&full[i], 0), wait_warp(&full[i], 1);
     }
   }
   pdl_wait();
@@ -897,6 +973,49 @@ int more_shared(int bytes) {
   return LQ_OK;
 }
 
+// The encoder needs a current context, which a thread that made no call of the
+// runtime yet (autograd's, at its first backward pass) does not have.
+template <typename... Args>
+CUresult encode(Args... args) {
+  const EncodeTiledFn enc = encode_fn();
+  if (!enc) return CUDA_ERROR_NOT_FOUND;
+  CUresult r = enc(args...);
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = enc(args...);
+  }
+  return r;
+}
+
+// [rows, width] of 16-bit values as boxes of 64 columns and `box` rows
+template <typename T>
+int map_rows(RowsMap* m, const void* p, int64_t rows, int64_t width, int64_t stride, int box) {
+  m->ok = 0;
+  if (!p || (rows > 1 && stride < width)) return LQ_OK;  // rows that share memory: not a tensor map's
+  const cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)(rows > 1 ? stride : width) * 2};
+  const cuuint32_t boxes[2] = {64, (cuuint32_t)box}, ones[2] = {1, 1};
+  const CUresult r = encode(&m->map, Half16<T>::fmt ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                         const_cast<void*>(p), dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  LQ_REQUIRE(r == CUDA_SUCCESS, LQ_ECUDA, "adapters: a tensor map of %lld rows of %lld values failed (%d)", (long long)rows,
+             (long long)width, (int)r);
+  m->ok = 1;
+  return LQ_OK;
+}
+// A bank's factor [L, R, width], boxes of one adapter's ranks
+template <typename T, int NP>
+int map_factor(CUtensorMap* m, const lq_adapter_bank& b, bool is_a) {
+  const int64_t width = is_a ? b.K : b.N;
+  const cuuint64_t dims[3] = {(cuuint64_t)width, (cuuint64_t)b.R, (cuuint64_t)b.L};
+  const cuuint64_t strides[2] = {(cuuint64_t)width * 2, (cuuint64_t)(b.R * width) * 2};
+  const cuuint32_t boxes[3] = {64, NP, 1}, ones[3] = {1, 1, 1};
+  const CUresult r = encode(m, Half16<T>::fmt ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                         const_cast<void*>(is_a ? b.a : b.b), dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  LQ_REQUIRE(r == CUDA_SUCCESS, LQ_ECUDA, "adapters: a tensor map of the bank failed (%d)", (int)r);
+  return LQ_OK;
+}
+
 template <typename T, int NP>
 int down_np(const AdCall& a, const void* x, int64_t stride, bool is_a, void* low, bool turned) {
   using S = DownShared<NP>;
@@ -920,7 +1039,11 @@ int down_np(const AdCall& a, const void* x, int64_t stride, bool is_a, void* low
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, static_cast<const T*>(x), stride, static_cast<const T*>(is_a ? b.a : b.b),
+  RowsMap xm;
+  CUtensorMap fm;
+  LQ_TRY(map_rows<T>(&xm, x, a.n, K, stride, 128));
+  LQ_TRY((map_factor<T, NP>(&fm, b, is_a)));
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, xm, fm, static_cast<const T*>(x), stride, static_cast<const T*>(is_a ? b.a : b.b),
                                            b.scaling, (int)b.R, K, a.plan, (int)b.L, low_at<NP>(low, tiles, turned), split);
   LQ_REQUIRE(e == cudaSuccess, LQ_ECUDA, "ad_down_kernel launch: %s", cudaGetErrorString(e));
   return launched("ad_down_kernel");
@@ -935,9 +1058,12 @@ int up_np(const AdCall& a, void* low, bool is_a, const void* base, int64_t bs, v
   const int64_t groups = units < num_sms() / kUpBeside ? units : num_sms() / kUpBeside;
   constexpr auto kern = ad_up_kernel<T, NP>;
   LQ_TRY(more_shared<kern>(S::bytes));
-  const cudaError_t e = launch_pdl(kern, dim3((unsigned)(groups * kUpBeside)), dim3(kUpThreads), S::bytes, a.st,
-                                   low_at<NP>(low, tiles, false), static_cast<const T*>(is_a ? b.a : b.b), (int)b.R, N, a.plan,
-                                   (int)b.L, static_cast<const T*>(base), bs, static_cast<T*>(out), os, chunks);
+  RowsMap bm;
+  CUtensorMap fm;
+  LQ_TRY(map_rows<T>(&bm, base, a.n, N, bs, 128));
+  LQ_TRY((map_factor<T, NP>(&fm, b, is_a)));
+  const cudaError_t e = launch_pdl(kern, dim3((unsigned)(groups * kUpBeside)), dim3(kUpThreads), S::bytes, a.st, bm, fm,
+                                   low_at<NP>(low, tiles, false), N, a.plan, (int)b.L, static_cast<const T*>(base), bs, static_cast<T*>(out), os, chunks);
   LQ_REQUIRE(e == cudaSuccess, LQ_ECUDA, "ad_up_kernel launch: %s", cudaGetErrorString(e));
   return launched("ad_up_kernel");
 }
@@ -953,8 +1079,11 @@ int outer_np(const AdCall& a, const AdOuter& o) {
                    o.part + 2 * groups * b.R * b.K};
   constexpr auto kern = ad_outer_kernel<T, NP, G>;
   LQ_TRY(more_shared<kern>(S::bytes));
+  RowsMap one_m, two_m;
+  LQ_TRY(map_rows<T>(&one_m, one.x, a.n, b.K, one.stride, 64));
+  LQ_TRY(map_rows<T>(&two_m, two.x, a.n, b.N, two.stride, 64));
   cudaError_t e = launch_pdl(kern, dim3((unsigned)(one.chunks + two.chunks), (unsigned)groups), dim3(kOuterLoaders + 32), S::bytes,
-                             a.st, one, two, (int)b.R, a.plan, (int)b.L);
+                             a.st, one_m, two_m, one, two, (int)b.R, a.plan, (int)b.L);
   LQ_REQUIRE(e == cudaSuccess, LQ_ECUDA, "ad_outer_kernel launch: %s", cudaGetErrorString(e));
   LQ_TRY(launched("ad_outer_kernel"));
   const int64_t b1 = o.da ? (b.R * b.K + 2047) / 2048 : 0, b2 = o.db ? (b.R * b.N + 2047) / 2048 : 0;

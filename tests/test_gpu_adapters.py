@@ -144,6 +144,27 @@ def test_backward(shape, dt):
         assert torch.equal(p, q)
 
 
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("R", [16, 32, 64, 128])
+def test_many_tiles(R, dt):
+    """Many tiles and columns to a block, of sequences that follow each other and
+    of tokens in any order, with padding between them; calls that nothing waits between."""
+    n, seq, num, K, N = 9, 515, 3, 136, 4360
+    bank, x, base, dy = make(n, seq, num, R, K, N, TYPES[dt], seed=20)
+    counts = torch.tensor([515, 512, 1, 0, 300, 515, 514, 129, 515], dtype=torch.int32, device=DEV)
+    ids = torch.tensor([0, 1, 2, 0, -1, 1, 0, 2, 2], dtype=torch.int32, device=DEV)
+    mixed = torch.randint(-1, num, (n * seq,), generator=torch.Generator().manual_seed(1)).int().to(DEV)
+    batches = [(L.AdapterBatch(ids, num, seq, counts), owners(ids, n, seq, num, counts)),
+               (L.AdapterBatch(mixed, num), owners(mixed, n * seq, 1, num))]
+    for batch, own in batches:
+        want = reference(x, base, bank.lora_A, bank.lora_B, bank.scaling, own)[0]
+        got = [bank(x, batch, base) for _ in range(6)]
+        close(got[0], want, K + R)
+        kept = base.clone()
+        assert torch.equal(bank.add_(kept, x, batch), got[0])
+        assert all(torch.equal(got[0], y) for y in got)
+
+
 def test_gradients_against_differences():
     """y is linear in x, in A and in B: a difference over any step is the
     derivative, up to the rounding of the two outputs."""
