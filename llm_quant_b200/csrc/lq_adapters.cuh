@@ -77,10 +77,10 @@ struct AdOuter {
   float* part;  // two partial sums of each side's [R, K], [R, N] for each group
 };
 // Groups that the tiles of a call are dealt out to: with all column chunks of
-// both sides, one wave of resident blocks.  `blocks` to an SM go by the rank.
+// both sides, one wave of blocks, one to an SM.
 inline int64_t ad_outer_groups(const lq_adapter_bank& b, int64_t n) {
   const int64_t chunks = (b.K + 255) / 256 + (b.N + 255) / 256, tiles = ad_max_tiles(n, b.L);
-  int64_t g = (int64_t)num_sms() * (b.R <= 16 ? 2 : 1) / chunks;
+  int64_t g = (int64_t)num_sms() / chunks;
   g = g < tiles ? g : tiles;
   return g > 1 ? g : 1;
 }

@@ -689,11 +689,10 @@ __global__ void __launch_bounds__(kUpThreads, 1)
 // that goes on in another group leaves a partial sum (place 0 if it began
 // before the group, else 1), which ad_sum adds up in order.
 // ---------------------------------------------------------------------------
-constexpr int kOuterLoaders = 256;
+constexpr int kOuterX = 128, kOuterV = 256, kOuterLoaders = kOuterX + kOuterV;
 template <int NP>
 struct OuterShared {
-  static constexpr int stages = NP <= 16 ? 3 : NP <= 64 ? 4 : 3;
-  static constexpr int blocks = NP <= 16 ? 2 : 1;  // resident on an SM
+  static constexpr int stages = NP <= 16 ? 6 : NP <= 32 ? 5 : NP <= 64 ? 4 : 3;
   static constexpr int off_v = 32768;
   static constexpr int stage = off_v + 2 * NP * 128;
   static constexpr int bytes = stages * stage + 1024;
@@ -711,12 +710,12 @@ struct OuterSide {
 };
 
 template <typename T, int NP, typename G>
-__global__ void __launch_bounds__(kOuterLoaders + 32, OuterShared<NP>::blocks)
+__global__ void __launch_bounds__(kOuterLoaders + 32, 1)
     ad_outer_kernel(const __grid_constant__ RowsMap one_m, const __grid_constant__ RowsMap two_m, const OuterSide<T> one,
                     const OuterSide<T> two, int R, AdPlan p, int L) {
   using S = OuterShared<NP>;
   using H = Half16<T>;
-  constexpr int NS = S::stages, VI = NP / 16;  // 8 tokens of a rank, of a lane that brings V
+  constexpr int NS = S::stages, VI = NP <= 32 ? 1 : NP / 32;  // 8 tokens of a rank, of a lane that brings V
   constexpr uint32_t kCols = 4 * NP;  // two tiles of 128 columns, hi and lo
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t full[NS], empty[NS], done, free_, drain;
@@ -753,7 +752,7 @@ __global__ void __launch_bounds__(kOuterLoaders + 32, OuterShared<NP>::blocks)
   volatile int* fail = &failed;
   int step = 0, run = 0;  // 64-token steps and runs so far: the barriers' phases
   if (warp < kOuterLoaders / 32) {
-    // warps 0 .. 3 bring X, a row of 512 bytes at a time; warps 4 .. 7 V
+    // warps 0 .. 3 bring X, by TMA or a row of 512 bytes at a time; the others V
     const bool brings_x = warp < 4;
     if (H::scaled || !brings_x) pdl_wait();
     const uint32_t at = base + (lane >> 3) * 8192;
@@ -812,47 +811,57 @@ __global__ void __launch_bounds__(kOuterLoaders + 32, OuterShared<NP>::blocks)
           cp_arrive(&full[slot]);
         }
       } else {
-        const int id = tid - 128, k8 = id & 7, r0 = id >> 3;
-        float v[VI][8];
+        const int id = tid - kOuterX, k8 = id & 7, r0 = id >> 3;
+        float v[2][VI][8];
         // whole pieces, the ones behind the run too (a tile's rows are all there, if
         // nobody wrote them): a load under a condition, whose value is looked at
-        // before the next one, cost a trip to L2 each (370 us instead of 136)
-        auto fetch = [&](int i) {
+        // before the next one, cost a trip to L2 each (370 us instead of 136).  Two
+        // steps are on their way: with one the trip was the step's time (140 us)
+        auto fetch = [&](int i, float (&w)[VI][8]) {
           const float* from = q.v.turned + (int64_t)(t0 + (i >> 1)) * NP * 128 + (i & 1) * 64 + k8 * 8;
 #pragma unroll
-          for (int j = 0; j < VI; ++j)
+          for (int j = 0; j < VI; ++j) {
+            if (r0 + 32 * j >= NP) continue;  // (NP = 16: half of the warps)
 #pragma unroll
             for (int k = 0; k < 8; k += 4) {
-              const float4 a = *reinterpret_cast<const float4*>(from + (r0 + 16 * j) * 128 + k);
-              v[j][k] = a.x, v[j][k + 1] = a.y, v[j][k + 2] = a.z, v[j][k + 3] = a.w;
+              const float4 a = *reinterpret_cast<const float4*>(from + (r0 + 32 * j) * 128 + k);
+              w[j][k] = a.x, w[j][k + 1] = a.y, w[j][k + 2] = a.z, w[j][k + 3] = a.w;
             }
+          }
         };
-        fetch(0);
-        for (int i = 0; i < n; ++i) {
+        auto put = [&](int i, float (&w)[VI][8]) {
           const int slot = (step + i) % NS;
           if (step + i >= NS && !wait_lane(&empty[slot], ((step + i) / NS - 1) & 1)) *fail = 1;
-          if (*fail) break;
+          if (*fail) return false;
           const uint32_t vt = base + slot * S::stage + S::off_v;
           const int left = rows - i * 64 - k8 * 8;  // tokens of the run from here on
           if (left < 8) {
 #pragma unroll
             for (int j = 0; j < VI; ++j)
 #pragma unroll
-              for (int k = 0; k < 8; ++k) v[j][k] = k < left ? v[j][k] : 0.0f;
+              for (int k = 0; k < 8; ++k) w[j][k] = k < left ? w[j][k] : 0.0f;
           }
 #pragma unroll
           for (int j = 0; j < VI; ++j) {
-            const int r = r0 + 16 * j;
+            const int r = r0 + 32 * j;
+            if (r >= NP) continue;
             uint32_t hi[4], lo[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) split16<T>(v[j][2 * k] * f, v[j][2 * k + 1] * f, hi[k], lo[k]);
+            for (int k = 0; k < 4; ++k) split16<T>(w[j][2 * k] * f, w[j][2 * k + 1] * f, hi[k], lo[k]);
             const uint32_t a = vt + r * 128 + ((k8 ^ (r & 7)) << 4);
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a + NP * 128), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
           }
           proxy_fence();
           mbar_arrive(&full[slot]);
-          if (i + 1 < n) fetch(i + 1);
+          if (i + 2 < n) fetch(i + 2, w);
+          return true;
+        };
+        fetch(0, v[0]);
+        if (n > 1) fetch(1, v[1]);
+        for (int i = 0; i < n; i += 2) {
+          if (!put(i, v[0])) break;
+          if (i + 1 < n && !put(i + 1, v[1])) break;
         }
       }
       step += n;
@@ -860,6 +869,11 @@ __global__ void __launch_bounds__(kOuterLoaders + 32, OuterShared<NP>::blocks)
       if (!wait_lane(&done, run & 1)) *fail = 1;
       __syncwarp();
       tc_fence_after();
+      if (warp >= 8) {  // eight warps have the 256 columns
+        mbar_arrive(&free_);
+        t0 = last + 1;
+        continue;
+      }
       const int mt = warp >> 2, my = col0 + mt * 128 + (warp & 3) * 32 + lane;
       const uint32_t from = tmem + ((uint32_t)(warp & 3) << 21) + mt * 2 * NP;
       const bool starts = p.tile_of[owner] == t0, ends = p.tile_of[owner + 1] == last + 1;
