@@ -183,9 +183,43 @@ void adapters_add_(const Tensor& y, const Tensor& x, const Tensor& lora_a, const
   if (!y.is_inference()) y.unsafeGetTensorImpl()->bump_version();
 }
 
+// The tensors of a GradClipper, which has checked them, as the entry point takes them
+class Clipper {
+ public:
+  Clipper(std::vector<Tensor> in, std::optional<std::vector<Tensor>> out, std::vector<Tensor> written)
+      : in_(std::move(in)), out_(std::move(out)), written_(std::move(written)) {
+    for (const Tensor& t : in_) from_.push_back(t.data_ptr()), n_.push_back(t.numel()), type_.push_back(code_of(t.scalar_type()));
+    if (out_)
+      for (const Tensor& t : *out_) to_.push_back(t.data_ptr());
+    bytes_ = lq_clip_workspace_bytes(in_.size());
+  }
+  Tensor clip(double max_norm) const {
+    const c10::cuda::CUDAGuard guard(in_[0].device());
+    const auto options = at::TensorOptions().device(in_[0].device());
+    const Tensor norm = at::empty({}, options.dtype(at::kFloat)), ws = at::empty({(int64_t)bytes_}, options.dtype(at::kByte));
+    check(lq_clip_grad_norm(from_.data(), out_ ? to_.data() : nullptr, n_.data(), type_.data(), in_.size(), max_norm,
+                            norm.data_ptr<float>(), ws.data_ptr(), bytes_, at::cuda::getCurrentCUDAStream()));
+    for (const Tensor& t : written_) t.unsafeGetTensorImpl()->bump_version();
+    return norm;
+  }
+
+ private:
+  std::vector<Tensor> in_;
+  std::optional<std::vector<Tensor>> out_;
+  std::vector<Tensor> written_;  // whose versions go up: one of those that share a buffer
+  std::vector<const void*> from_;
+  std::vector<void*> to_;
+  std::vector<int64_t> n_;
+  std::vector<int> type_;
+  size_t bytes_ = 0;
+};
+
 }  // namespace
 
 PYBIND11_MODULE(lq_torch, m) {
   m.def("adapters_forward", &adapters_forward);
   m.def("adapters_add_", &adapters_add_);
+  pybind11::class_<Clipper>(m, "Clipper")
+      .def(pybind11::init<std::vector<Tensor>, std::optional<std::vector<Tensor>>, std::vector<Tensor>>())
+      .def("clip", &Clipper::clip);
 }

@@ -12,8 +12,6 @@ fp32 and each product is rounded once.  Nothing is read back on the host.
 
 from __future__ import annotations
 
-import ctypes
-import math
 from typing import Iterable, Optional, Sequence
 
 import torch
@@ -70,37 +68,20 @@ class GradClipper:
                 end = max(end, hi)
             else:
                 read_end = max(read_end, hi)
-        # aliases of their own: a tensor given other memory later leaves these as they are
-        self._in = [g.detach() for g in grads]
-        self._out = self._in if out is None else [o.detach() for o in outs]
-        n = len(grads)
-        self._args = ((ctypes.c_void_p * n)(*[g.data_ptr() for g in self._in]),
-                      None if out is None else (ctypes.c_void_p * n)(*[o.data_ptr() for o in self._out]),
-                      (ctypes.c_int64 * n)(*[g.numel() for g in self._in]),
-                      (ctypes.c_int * n)(*[_C.dt(g) for g in self._in]), n)
         # views of one buffer share its version
         bases = {id(b): b for b in (o if o._base is None else o._base for o in outs)}
-        self._versions = [b for b in bases.values() if not b.is_inference()]
-        self._bytes = _C.lib().lq_clip_workspace_bytes(n)
+        # aliases of their own: a tensor given other memory later leaves these as they are
+        self._clipper = _C.ext().Clipper([g.detach() for g in grads], None if out is None else [o.detach() for o in outs],
+                                         [b.detach() for b in bases.values() if not b.is_inference()])
 
     def clip(self, max_norm: float) -> torch.Tensor:
         """Clip to ``max_norm`` and return the norm before it (float32 scalar on
         the device; inf or NaN where the gradients are not finite, and the
         gradients are then what the formula makes of them)."""
         max_norm = float(max_norm)
-        if math.isnan(max_norm) or max_norm < 0:
+        if not max_norm >= 0:
             raise ValueError(f"GradClipper.clip: max_norm {max_norm} must not be negative")
-        norm = torch.empty((), dtype=torch.float32, device=self.device)
-        ws = torch.empty(self._bytes, dtype=torch.uint8, device=self.device)
-        index = self.device.index
-        args = (*self._args, max_norm, norm.data_ptr(), ws.data_ptr(), self._bytes)
-        if index == torch.cuda.current_device():
-            _C.call("lq_clip_grad_norm", *args, _C.raw_stream(index))
-        else:
-            with torch.cuda.device(index):
-                _C.call("lq_clip_grad_norm", *args, _C.raw_stream(index))
-        torch.autograd.graph.increment_version(self._versions)
-        return norm
+        return self._clipper.clip(max_norm)
 
 
 def clip_grad_norm_(parameters: Iterable[torch.Tensor] | torch.Tensor, max_norm: float) -> torch.Tensor:

@@ -201,3 +201,20 @@ def test_memory_stays():
     g.data = rand(10, torch.float32)
     before = kept.clone()
     check(clipper.clip(0.5), [kept], [before], 0.5)
+
+
+def test_versions():
+    """A graph that saved a clipped tensor raises; parts of one buffer count as the buffer."""
+    x = rand(100, torch.float32).requires_grad_(True)
+    g = rand(100, torch.float32)
+    y = (x * g).sum()
+    L.GradClipper([g]).clip(0.5)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    flat = rand(300, torch.bfloat16)
+    before = flat._version
+    L.GradClipper(list(flat.split(100))).clip(0.5)
+    assert flat._version == before + 1
+    with torch.inference_mode():
+        h = rand(50, torch.float32)
+        check(L.GradClipper([h]).clip(0.5), [h], [rand(50, torch.float32)], 0.5)
