@@ -15,33 +15,45 @@ namespace {
 
 // ---------------------------------------------------------------------------
 // The plan.  A block to an adapter (block L: the tokens without one) counts all
-// tokens by adapter in shared memory (integers: no order of atomics shows), adds
-// up the counts below its own, and writes its tokens, in order, by ballots.
-// Every block counts for itself: T reads from L2 each, and no second launch.
+// requests' tokens by adapter in shared memory (integers: no order of atomics
+// shows), adds up the counts below its own, and writes its tokens, in order, by
+// sums over the block.  Every block counts for itself: the requests are read
+// from L2 L + 1 times, and there is no second launch.  8 requests of 2048 tokens
+// with 8 adapters 5.1 us, 16384 tokens by themselves with 64 25 us, 64 requests of
+// 16384 with 64 108 us.
 // ---------------------------------------------------------------------------
 constexpr int kPlanThreads = 512;
+constexpr int kPlanShort = 32;  // requests of up to so many tokens are a thread's, four at a time; longer ones the block's
 
+struct Share {  // of a request's tokens, the ones that belong to a block
+  int from, n;
+};
+// Tokens 0 .. live - 1 of a request are its adapter's, the others nobody's.
 template <typename I>
-__device__ __forceinline__ int owner_of(const I* ids, const int* counts, int64_t seq, int L, int64_t t) {
-  const int64_t b = seq == 1 ? t : t / seq;
-  if (counts && t - b * seq >= counts[b]) return L;
-  const int64_t i = static_cast<int64_t>(ids[b]);
-  return i >= 0 && i < L ? static_cast<int>(i) : L;
+__device__ __forceinline__ Share share_of(const I* ids, const int* counts, int seq, int L, int r, int me) {
+  const int64_t id = static_cast<int64_t>(ids[r]);
+  const int live = id < 0 || id >= L ? 0 : counts ? min(max(counts[r], 0), seq) : seq;
+  Share s;
+  s.from = me == L ? live : 0;
+  s.n = me == L ? seq - live : id == me ? live : 0;
+  return s;
 }
 
 template <typename I>
 __global__ void __launch_bounds__(kPlanThreads) ad_plan_kernel(const I* __restrict__ ids, const int* __restrict__ counts,
-                                                               int64_t seq, int T, int L, AdPlan p) {
+                                                               int seq, int requests, int L, AdPlan p) {
   extern __shared__ int hist[];  // [L + 1]
   __shared__ int part[2][kPlanThreads / 32];
-  __shared__ int base[2];
+  __shared__ int base[2], listed;
+  __shared__ int4 list[kPlanThreads];  // requests of the block: first token, number, place
   const int me = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   for (int i = tid; i <= L; i += kPlanThreads) hist[i] = 0;
   __syncthreads();
-  for (int t = tid; t < T; t += kPlanThreads) {
-    const int o = owner_of(ids, counts, seq, L, t);
-    atomicAdd(&hist[o], 1);
-    if (me == L) p.owner[t] = o == L ? -1 : o;
+  for (int r = tid; r < requests; r += kPlanThreads) {
+    const int64_t id = static_cast<int64_t>(ids[r]);
+    const int live = id < 0 || id >= L ? 0 : counts ? min(max(counts[r], 0), seq) : seq;
+    if (live) atomicAdd(&hist[static_cast<int>(id)], live);
+    if (live < seq) atomicAdd(&hist[L], seq - live);
   }
   __syncthreads();
   int before = 0, tiles = 0;
@@ -64,26 +76,52 @@ __global__ void __launch_bounds__(kPlanThreads) ad_plan_kernel(const I* __restri
     p.start[me] = first, p.tile_of[me] = tile;
     if (me == L) p.start[L + 1] = first + n, p.tile_of[L + 1] = tile + n_tiles, *p.status = LQ_OK;
   }
+  const int owner = me == L ? -1 : me, each = seq <= kPlanShort ? 4 : 1;  // requests of a thread at a time
   int at = first;
-  for (int t0 = 0; t0 < T && at < first + n; t0 += kPlanThreads) {
-    const int t = t0 + tid;
-    const bool mine = t < T && owner_of(ids, counts, seq, L, t) == me;
-    const unsigned m = __ballot_sync(0xffffffffu, mine);
-    __syncthreads();  // part was read
-    if (lane == 0) part[0][warp] = __popc(m);
+  for (int r0 = 0; r0 < requests && at < first + n; r0 += each * kPlanThreads) {
+    Share s[4];
+    int mine = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int r = r0 + tid * each + k;
+      s[k] = k < each && r < requests ? share_of(ids, counts, seq, L, r, me) : Share{0, 0};
+      mine += s[k].n;
+    }
+    int upto = mine;  // of the warp's threads up to this one
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, m);
+      if (lane >= m) upto += x;
+    }
+    __syncthreads();  // part and list were read
+    if (lane == 31) part[0][warp] = upto;
+    if (tid == 0) listed = 0;
     __syncthreads();
-    int below = 0, all = 0;
+    int place = at + upto - mine, all = 0;
     for (int w = 0; w < kPlanThreads / 32; ++w) {
-      below += w < warp ? part[0][w] : 0;
+      place += w < warp ? part[0][w] : 0;
       all += part[0][w];
     }
-    if (mine) p.order[at + below + __popc(m & ((1u << lane) - 1))] = t;
+    if (each > 1) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int t = (r0 + tid * each + k) * seq + s[k].from;
+        for (int i = 0; i < s[k].n; ++i, ++place) p.order[place] = t + i, p.owner[t + i] = owner;
+      }
+    } else {
+      if (mine) list[atomicAdd(&listed, 1)] = make_int4((r0 + tid) * seq + s[0].from, mine, place, 0);
+      __syncthreads();
+      for (int e = 0; e < listed; ++e) {
+        const int4 q = list[e];
+        for (int i = tid; i < q.y; i += kPlanThreads) p.order[q.z + i] = q.x + i, p.owner[q.x + i] = owner;
+      }
+    }
     at += all;
   }
   __syncthreads();  // the block's own order, read back below
   for (int i = tid; i < n_tiles; i += kPlanThreads) {
     AdTile d;
-    d.owner = me == L ? -1 : me;
+    d.owner = owner;
     d.first = first + i * kAdTile;
     d.rows = min(kAdTile, n - i * kAdTile);
     const int a = p.order[d.first], z = p.order[d.first + d.rows - 1];
@@ -139,9 +177,9 @@ extern "C" int lq_adapter_plan(const void* ids, int ids_dtype, int64_t n_ids, in
   const size_t smem = 4 * (size_t)(L + 1);
   cudaStream_t st = as_stream(stream);
   if (ids_dtype == LQ_I32)
-    ad_plan_kernel<int32_t><<<(unsigned)L + 1, kPlanThreads, smem, st>>>(static_cast<const int32_t*>(ids), counts, seq_len, (int)n, (int)L, p);
+    ad_plan_kernel<int32_t><<<(unsigned)L + 1, kPlanThreads, smem, st>>>(static_cast<const int32_t*>(ids), counts, (int)seq_len, (int)n_ids, (int)L, p);
   else
-    ad_plan_kernel<int64_t><<<(unsigned)L + 1, kPlanThreads, smem, st>>>(static_cast<const int64_t*>(ids), counts, seq_len, (int)n, (int)L, p);
+    ad_plan_kernel<int64_t><<<(unsigned)L + 1, kPlanThreads, smem, st>>>(static_cast<const int64_t*>(ids), counts, (int)seq_len, (int)n_ids, (int)L, p);
   return launched("ad_plan_kernel");
 }
 
