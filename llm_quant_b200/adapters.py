@@ -136,6 +136,14 @@ class AdapterBank(nn.Module):
         bound = 1.0 / math.sqrt(in_features)  # as QLoRALinear's
         nn.init.uniform_(self.lora_A, -bound, bound)
 
+    def _apply(self, fn, recurse=True):
+        """``scaling`` goes where the parameters go, and stays float32."""
+        scaling = self.scaling
+        super()._apply(fn, recurse)
+        if self.scaling.dtype != torch.float32:
+            self.scaling = scaling.to(self.scaling.device)
+        return self
+
     @classmethod
     def from_layers(cls, layers: Iterable, *, dtype: torch.dtype = torch.bfloat16) -> "AdapterBank":
         """The adapters of several QLoRALinear of one shape, as one bank."""

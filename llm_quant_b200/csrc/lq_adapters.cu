@@ -249,7 +249,7 @@ extern "C" int lq_adapter_backward(const lq_adapter_bank* bank, const lq_adapter
   void* v = workspace;
   float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + v_bytes(*bank, n));
   if (dx || da) LQ_TRY(ad_down(a, dy, form->out_stride, false, v, da != nullptr));
-  if (da || db) LQ_TRY(ad_outer(a, {v, x, form->x_stride, da, low, dy, form->out_stride, db, grad_dtype, part}));
+  if (da || db) LQ_TRY(ad_outer(a, {v, x, form->x_stride, da, low, dy, form->out_stride, db, grad_dtype, part, dx || da}));
   if (dx) LQ_TRY(ad_up(a, v, true, nullptr, 0, dx, bank->K));
   return LQ_OK;
 }

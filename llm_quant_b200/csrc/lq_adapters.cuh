@@ -75,6 +75,7 @@ struct AdOuter {
   void* db;
   int grad_dtype;
   float* part;  // two partial sums of each side's [R, K], [R, N] for each group
+  bool behind_down;  // ad_down is the launch before
 };
 // Groups that the tiles of a call are dealt out to: with all column chunks of
 // both sides, one wave of blocks, one to an SM.

@@ -562,6 +562,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
       if (base && bm.ok && d.run >= 0) {
         // rows of other tiles behind the tile's own are not taken out
         if (w2 == 0 && lane == 0) {
+          proxy_fence();  // the sums that were written here come before the box
           mbar_expect_tx(&full[slot], S::stage);
           tma_2d(stage, &bm.map, chunk * 128, d.run, &full[slot]);
           tma_2d(stage + 16384, &bm.map, chunk * 128 + 64, d.run, &full[slot]);
@@ -712,7 +713,7 @@ struct OuterSide {
 template <typename T, int NP, typename G>
 __global__ void __launch_bounds__(kOuterLoaders + 32, 1)
     ad_outer_kernel(const __grid_constant__ RowsMap one_m, const __grid_constant__ RowsMap two_m, const OuterSide<T> one,
-                    const OuterSide<T> two, int R, AdPlan p, int L) {
+                    const OuterSide<T> two, int R, AdPlan p, int L, int early) {
   using S = OuterShared<NP>;
   using H = Half16<T>;
   constexpr int NS = S::stages, VI = NP <= 32 ? 1 : NP / 32;  // 8 tokens of a rank, of a lane that brings V
@@ -721,7 +722,9 @@ __global__ void __launch_bounds__(kOuterLoaders + 32, 1)
   __shared__ uint64_t full[NS], empty[NS], done, free_, drain;
   __shared__ uint32_t tmem_at;
   __shared__ int failed;
-  // as ad_up: x, dy, u and the plan are there, v is waited for by those who read it
+  // behind ad_down (early), as ad_up: x, dy, u and the plan are there, v is waited
+  // for by those who read it.  Behind any other kernel dy may be that one's.
+  if (!early) pdl_wait();
   const bool first_side = (int)blockIdx.x < one.chunks;
   const OuterSide<T>& q = first_side ? one : two;
   const RowsMap& xm = first_side ? one_m : two_m;
@@ -792,6 +795,7 @@ __global__ void __launch_bounds__(kOuterLoaders + 32, 1)
           if (*fail) break;
           if (box >= 0) {
             if (tid == 0) {
+              proxy_fence();  // rows that threads copied here come before the box
               mbar_expect_tx(&full[slot], 32768);
 #pragma unroll
               for (int j = 0; j < 4; ++j) tma_2d(base + slot * S::stage + j * 8192, &xm.map, col0 + j * 64, box, &full[slot]);
@@ -1097,7 +1101,7 @@ int outer_np(const AdCall& a, const AdOuter& o) {
   LQ_TRY(map_rows<T>(&one_m, one.x, a.n, b.K, one.stride, 64));
   LQ_TRY(map_rows<T>(&two_m, two.x, a.n, b.N, two.stride, 64));
   cudaError_t e = launch_pdl(kern, dim3((unsigned)(one.chunks + two.chunks), (unsigned)groups), dim3(kOuterLoaders + 32), S::bytes,
-                             a.st, one_m, two_m, one, two, (int)b.R, a.plan, (int)b.L);
+                             a.st, one_m, two_m, one, two, (int)b.R, a.plan, (int)b.L, (int)o.behind_down);
   LQ_REQUIRE(e == cudaSuccess, LQ_ECUDA, "ad_outer_kernel launch: %s", cudaGetErrorString(e));
   LQ_TRY(launched("ad_outer_kernel"));
   const int64_t b1 = o.da ? (b.R * b.K + 2047) / 2048 : 0, b2 = o.db ? (b.R * b.N + 2047) / 2048 : 0;

@@ -84,6 +84,8 @@ Call run(const Tensor& x, const Tensor& lora_a, const Tensor& lora_b, const Tens
   TORCH_CHECK_TYPE(lora_a.scalar_type() == lora_b.scalar_type() && scaling.scalar_type() == at::kFloat, "AdapterBank: lora_A is ",
                    name_of(lora_a.scalar_type()), ", lora_B ", name_of(lora_b.scalar_type()), ", scaling ",
                    name_of(scaling.scalar_type()), " (expected float32)");
+  TORCH_CHECK_TYPE(lora_a.scalar_type() == type || lora_a.scalar_type() == at::kFloat, "AdapterBank: parameters in ",
+                   name_of(lora_a.scalar_type()), " for activations in ", name_of(type), " (theirs or float32)");
   at::DimVector shape(x.sizes().begin(), x.sizes().end());
   shape.back() = N;
   if (base)

@@ -491,3 +491,118 @@ def test_inference_mode():
         y = base.clone()
         batch.update(torch.zeros(4, dtype=torch.int32, device=DEV))
         assert torch.equal(bank.add_(y, x, batch), bank(x, batch, base))
+
+
+def test_gradient_of_b_alone_behind_another_bank():
+    """The gradient of lora_B alone needs no product with dy first: its sums are the
+    first launch of the backward pass, right behind the kernel that makes dy."""
+    dt = torch.bfloat16
+    first, x, _, _ = make(4, 1000, 2, 64, 128, 2048, dt, seed=30)
+    second, _, _, dy = make(4, 1000, 2, 64, 2048, 1024, dt, seed=31)
+    batch = L.AdapterBatch(some_ids(4, 2, 5, False), 2, 1000)
+    first.lora_B.requires_grad_(True)
+    between = first(x, batch)
+    torch.cuda.synchronize()
+    leaf = between.detach().requires_grad_(True)
+    d, = torch.autograd.grad(second(leaf, batch), (leaf,), dy)
+    torch.cuda.synchronize()
+    want, = torch.autograd.grad(first(x, batch), (first.lora_B,), d)
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got, = torch.autograd.grad(second(first(x, batch), batch), (first.lora_B,), dy)
+        assert torch.equal(got, want)
+
+
+def test_types_of_a_module():
+    """A bank whose module was moved to another type keeps its scaling in fp32;
+    parameters in another 16-bit type than the activations are refused."""
+    bank, x, base, _ = make(3, 1, 2, 8, 64, 64, torch.bfloat16, seed=32)
+    bank.scaling.fill_(1.0 / 3.0)
+    batch = L.AdapterBatch(torch.zeros(3, dtype=torch.int32, device=DEV), 2)
+    want = bank(x, batch, base)
+    bank.bfloat16()
+    assert bank.scaling.dtype == torch.float32 and torch.equal(bank(x, batch, base), want)
+    bank.half()
+    with pytest.raises(TypeError, match="float16 for activations in bfloat16"):
+        bank(x, batch, base)
+    assert bank(x.half(), batch).dtype == torch.float16
+    import copy
+    assert torch.equal(copy.deepcopy(bank)(x.half(), batch), bank(x.half(), batch))
+
+
+def test_infinities_stay_in_their_rows_of_tiles():
+    """As above, where tokens share tiles (a call that keeps what its backward pass needs)."""
+    for dt in TYPES.values():
+        bank, x, base, _ = make(1, 300, 1, 16, 128, 136, dt, seed=8)
+        bank.requires_grad_(True)
+        batch = L.AdapterBatch(torch.zeros(1, dtype=torch.int32, device=DEV), 1, 300)
+        clean = bank(x, batch, base).detach()
+        bad = x.clone()
+        bad[7, 3], bad[200, 64], bad[201, 127] = float("inf"), float("nan"), float("-inf")
+        y = bank(bad, batch, base).detach()
+        rows = torch.ones(300, dtype=torch.bool, device=DEV)
+        rows[[7, 200, 201]] = False
+        assert torch.equal(y[rows], clean[rows])
+        assert y[200].isnan().all() and not y[[7, 201]].isfinite().any()
+
+
+def test_in_place_on_its_own_input():
+    """y may be x itself where the features agree."""
+    for n, seq in ((5, 1), (3, 700)):
+        bank, x, _, _ = make(n, seq, 2, 16, 256, 256, torch.bfloat16, seed=33)
+        batch = L.AdapterBatch(some_ids(n, 2, 6, True), 2, seq)
+        want = bank(x, batch, x)
+        y = x.clone()
+        assert torch.equal(bank.add_(y, y, batch), want)
+
+
+def test_second_derivatives_are_refused():
+    bank, x, base, dy = make(3, 5, 2, 8, 64, 64, torch.bfloat16)
+    x.requires_grad_(True)
+    y = bank(x, L.AdapterBatch(some_ids(3, 2, 0, False), 2, 5), base)
+    with pytest.raises(RuntimeError, match="gradients of gradients"):
+        torch.autograd.grad(y, (x,), dy, create_graph=True)
+
+
+def test_captured_decode_step():
+    """A captured call of few tokens, replayed for other requests."""
+    bank, x, base, _ = make(8, 1, 4, 16, 512, 264, torch.bfloat16, seed=34)
+    ids = some_ids(8, 4, 1, True)
+    batch = L.AdapterBatch(ids, 4)
+    bank(x, batch, base)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        batch.update(ids)
+        held = bank(x, batch, base)
+    for seed in (2, 3):
+        ids.copy_(some_ids(8, 4, seed, True))
+        x.copy_(torch.randn(x.shape, device=DEV, generator=torch.Generator(DEV).manual_seed(seed)))
+        graph.replay()
+        assert torch.equal(held, bank(x, L.AdapterBatch(ids, 4), base))
+
+
+def test_nothing_ran_out():
+    bank, x, base, _ = make(4, 300, 2, 16, 256, 256, torch.bfloat16)
+    bank.requires_grad_(True)
+    batch = L.AdapterBatch(some_ids(4, 2, 0, True), 2, 300)
+    bank(x, batch, base).sum().backward()
+    batch.check()
+
+
+@pytest.mark.parametrize("seq", [1, 7, 32, 33, 200])
+def test_plans(seq):
+    """The plan's groups: every token once, in order, with its adapter."""
+    for n, num in ((1, 1), (3, 2), (700, 5), (50, 200)):
+        g = torch.Generator().manual_seed(n + seq)
+        ids = torch.randint(-2, num + 2, (n,), generator=g)
+        counts = torch.randint(-1, seq + 3, (n,), generator=g).int()
+        for c in (None, counts):
+            own = owners(ids, n, seq, num, None if c is None else c.clamp(0, seq))
+            batch = L.AdapterBatch(ids.to(DEV), num, seq, None if c is None else c.to(DEV))
+            t = n * seq
+            plan = batch._plan.view(torch.int32).cpu()
+            up = lambda k: (k + 3) // 4 * 4
+            got_owner, order = plan[4:4 + t], plan[4 + up(t):4 + up(t) + t]
+            assert torch.equal(got_owner.long(), own)
+            key = torch.where(own < 0, num, own)
+            assert torch.equal(order.long(), torch.sort(key, stable=True).indices)
