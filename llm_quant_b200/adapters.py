@@ -12,8 +12,9 @@ and, in training, gives the gradients of x, of all lora_A and of all lora_B.
 The reference has no counterpart (its QLoRALinear.forward, qlora.py:306-312, is
 the case of one adapter).
 
-Activations are float16 or bfloat16.  Products are exact and summed in fp32,
-``scaling * lora_A x`` is kept in fp32, and each output is rounded once.
+Activations are float16 or bfloat16.  Products are exact and summed in fp32;
+``scaling * lora_A x`` meets lora_B in fp32 or as two 16-bit parts (off by 2^-16
+of itself in bfloat16, 2^-22 in float16), and each output is rounded once.
 Parameters may be float32 (a training run's master weights): they are rounded
 to the activations' dtype at each call and their gradients come in float32.
 Sums go in an order of their own: equal calls give equal bits.

@@ -4,7 +4,7 @@
 // first: a block's stretch of the values is summed and the block's sum left in
 // the workspace; then every block adds up all sums, in one order, and scales the
 // same stretch from its end to its start, so that what was read last is still
-// in L2.  Up to a megabyte one cluster of eight blocks does both.
+// in L2.  Little is done by one cluster of eight blocks, both at once.
 //
 // Squares of 8 (fp32: 4) neighbours are added in fp32, and those sums in fp64;
 // a sum that leaves [2^-100, 2^100] is taken again from fp64 squares, so that
@@ -23,9 +23,10 @@ constexpr int kClipVecs = 8;  // 16-byte vectors that a thread has on their way
 __host__ __device__ constexpr int clip_unit(bool shifted, int grain) { return kClipThreads / 32 * (shifted ? 31 : 32) * grain * 16; }
 constexpr int kClipMost = 1024;                               // tensors of a launch
 constexpr int kClipBlocks = 148 * 4;
-// Up to here (and 256 tensors) one cluster: 3 x 20 KB 6.0 us instead of FIGURE on
-// the device, and a launch less for the host; beyond, eight SMs read too slowly.
-constexpr int64_t kClipSmall = 1 << 20;
+// Up to here (and 256 tensors) one cluster: three fp32 tensors of 60 KB 5.4 us on
+// the device, of 200 KB 7.6, of 340 KB 9.5, where two kernels take 7.6 throughout
+// and the host another 3 for the second launch.
+constexpr int64_t kClipSmall = 640 << 10;
 constexpr int kClipCluster = 8;
 
 // The tensors of one launch, as a kernel's parameters (no copy to the device,
