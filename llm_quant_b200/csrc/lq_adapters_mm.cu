@@ -204,8 +204,9 @@ __global__ void __launch_bounds__(160, 2) ad_down_kernel(const __grid_constant__
   using H = Half16<T>;
   pdl_wait();
   const int tile = blockIdx.x / split, rank = blockIdx.x - tile * split;
+  const AdTile d = p.tiles[tile];  // (there is room for every tile of the grid: both loads at once)
   if (tile >= p.tile_of[L]) return;  // the whole cluster
-  const AdTile d = p.tiles[tile];
+  const float s = scaling[d.owner];
   const int tid = threadIdx.x, warp = tid >> 5;
   const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
   // a tile whose tokens follow each other comes by TMA (rows of others behind its
@@ -288,7 +289,6 @@ __global__ void __launch_bounds__(160, 2) ad_down_kernel(const __grid_constant__
     }
     commit(&done);
   }
-  const float s = scaling[d.owner];
   const bool ok = wait_warp(&done, 0);
   if (!ok) failed = 1;
   tc_fence_after();
