@@ -189,10 +189,14 @@ int few_c(const AdCall& a, const void* x, int64_t xs, const void* base, int64_t 
   LQ_REQUIRE(e == cudaSuccess, LQ_ECUDA, "ad_few_kernel launch: %s", cudaGetErrorString(e));
   return launched("ad_few_kernel");
 }
-// As many blocks to a token as are resident at once
+// As many blocks to a token as are resident at once, two to an SM; an eighth of
+// the room stays empty, since a cluster's blocks lie on one of the chip's groups
+// of SMs (37 tokens by 8 blocks 7.9 us, by 4 blocks 4.8; 32 tokens of 14336 columns
+// by 8 blocks 5.8, by 4 6.4).  (A third block to an SM,
+// with 80 registers, made 5.2 us of 64 tokens 6.9 and 11.7 of 777 13.8.)
 template <typename T, int RW>
 int few_rw(const AdCall& a, const void* x, int64_t xs, const void* base, int64_t bs, void* out, int64_t os) {
-  const int64_t room = 2 * num_sms();
+  const int64_t room = num_sms() * 7 / 4;
   if (a.n * 8 <= room) return few_c<T, RW, 8>(a, x, xs, base, bs, out, os);
   if (a.n * 4 <= room) return few_c<T, RW, 4>(a, x, xs, base, bs, out, os);
   if (a.n * 2 <= room) return few_c<T, RW, 2>(a, x, xs, base, bs, out, os);
