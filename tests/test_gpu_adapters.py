@@ -606,3 +606,60 @@ def test_plans(seq):
             assert torch.equal(got_owner.long(), own)
             key = torch.where(own < 0, num, own)
             assert torch.equal(order.long(), torch.sort(key, stable=True).indices)
+
+
+def test_rows_of_other_strides_in_tiles():
+    """Rows that are parts of wider ones, off 16 bytes, all the same memory, and
+    turned, where tokens share tiles; sequences and tokens in any order."""
+    dt = torch.float16
+    n, seq, K, N = 3, 400, 128, 256
+    bank, x, base, dy = make(n, seq, 2, 16, K, N, dt, seed=40)
+    bank.requires_grad_(True)
+    order = torch.randint(-1, 2, (n * seq,), generator=torch.Generator().manual_seed(3)).int().to(DEV)
+    for batch in (L.AdapterBatch(some_ids(n, 2, 4, True), 2, seq), L.AdapterBatch(order, 2)):
+
+        def step(x, base, dy):
+            x = x.detach().requires_grad_(True)
+            y = bank(x, batch, base)
+            return [y.detach(), *torch.autograd.grad(y, (x, bank.lora_A, bank.lora_B), dy)]
+
+        want = step(x, base, dy)
+        wide, wide_b, wide_d = (torch.zeros(n * seq, w + 72, dtype=dt, device=DEV) for w in (K, N, N))
+        for at in (8, 3):
+            wide[:, at:at + K], wide_b[:, at:at + N], wide_d[:, at:at + N] = x, base, dy
+            got = step(wide[:, at:at + K], wide_b[:, at:at + N], wide_d[:, at:at + N])
+            assert all(torch.equal(p, q) for p, q in zip(got, want))
+        got = step(x.t().contiguous().t(), base.t().contiguous().t(), dy.t().contiguous().t())
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+        same = [t[:1].expand_as(t) for t in (x, base, dy)]
+        got, want = step(*same), step(*(t.contiguous() for t in same))
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_offsets_over_32_bits():
+    """More than 2^31 values in base, out and dy."""
+    dt = torch.bfloat16
+    T, K, N, R = 151_000, 64, 14336, 8
+    bank, x, _, _ = make(1, T, 2, R, K, N, dt, seed=41, base=False)
+    bank.requires_grad_(True)
+    batch = L.AdapterBatch(torch.tensor([1], device=DEV), 2, T)
+    base = torch.empty(T, N, dtype=dt, device=DEV)
+    for i in range(0, T, 10_000):
+        base[i:i + 10_000].normal_(generator=torch.Generator(DEV).manual_seed(i))
+    x.requires_grad_(True)
+    y = bank(x, batch, base)
+    dx, db = torch.autograd.grad(y, (x, bank.lora_B), base)
+    y = y.detach()
+    a, b, s = bank.lora_A[1].detach().double(), bank.lora_B[1].detach().double(), float(bank.scaling[1])
+    sums, mags = torch.zeros(R, N, dtype=torch.float64, device=DEV), torch.zeros(R, N, dtype=torch.float64, device=DEV)
+    for i in range(0, T, 10_000):
+        xi, d = x.detach()[i:i + 10_000].double(), base[i:i + 10_000].double()
+        u, ua = s * xi @ a.T, abs(s) * xi.abs() @ a.abs().T
+        sums += u.T @ d
+        mags += ua.T @ d.abs()
+        close(y[i:i + 10_000], (d + u @ b, d.abs() + ua @ b.abs()), K + R)
+        close(dx[i:i + 10_000], (s * d @ b.T @ a, abs(s) * d.abs() @ b.abs().T @ a.abs()), N + R)
+    close(db[1], (sums, mags), K + T)
+    assert not db[0].any()
+    with torch.no_grad():
+        assert torch.equal(bank.add_(base, x, batch), y)

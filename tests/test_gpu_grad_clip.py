@@ -218,3 +218,20 @@ def test_versions():
     with torch.inference_mode():
         h = rand(50, torch.float32)
         check(L.GradClipper([h]).clip(0.5), [h], [rand(50, torch.float32)], 0.5)
+
+
+def test_offsets_over_32_bits():
+    """More than 2^31 values in a tensor, its result off 16 bytes."""
+    n = 2 ** 31 + 12345
+    g = torch.empty(n, dtype=torch.bfloat16, device=DEV)
+    step = 1 << 27
+    for i in range(0, n, step):
+        g[i:i + step].normal_(std=0.01, generator=torch.Generator(DEV).manual_seed(i))
+    out = torch.empty(n + 8, dtype=torch.bfloat16, device=DEV)[3:n + 3]
+    norm = L.GradClipper([g], [out]).clip(1.0)
+    total = math.sqrt(math.fsum(float(g[i:i + step].double().square().sum()) for i in range(0, n, step)))
+    assert abs(float(norm) - total) <= 5 * 2.0 ** -24 * total
+    c = 1.0 / (total + 1e-6)
+    for i in range(0, n, step):
+        want = g[i:i + step].double() * c
+        assert bool(((out[i:i + step].double() - want).abs() <= (2.0 ** -8 + 6 * 2.0 ** -24) * want.abs() + 2.0 ** -134).all())
