@@ -99,6 +99,21 @@ __device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr, uint32_t rank) {
   return v;
 }
 
+// Sums of 8 values over the blocks of a cluster, in order; all loads first.
+template <int BLOCKS>
+__device__ __forceinline__ void cluster_sum(uint32_t addr, float (&v)[8]) {
+  float4 a[BLOCKS], z[BLOCKS];
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b) a[b] = ld_cluster_v4(addr, b), z[b] = ld_cluster_v4(addr + 16, b);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b)
+    v[0] += a[b].x, v[1] += a[b].y, v[2] += a[b].z, v[3] += a[b].w, v[4] += z[b].x, v[5] += z[b].y, v[6] += z[b].z, v[7] += z[b].w;
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
 __device__ __forceinline__ void bulk_load_at(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
                "r"(bytes), "r"(smem_u32(bar))
@@ -202,6 +217,7 @@ __global__ void __launch_bounds__(160, 2) ad_down_kernel(const __grid_constant__
   __shared__ uint32_t tmem_at;
   __shared__ int failed, row_top[128];
   using H = Half16<T>;
+  if (threadIdx.x == 0 && xm.ok) prefetch_map(&xm.map), prefetch_map(&fm);
   pdl_wait();
   const int tile = blockIdx.x / split, rank = blockIdx.x - tile * split;
   const AdTile d = p.tiles[tile];  // (there is room for every tile of the grid: both loads at once)
@@ -316,12 +332,11 @@ __global__ void __launch_bounds__(160, 2) ad_down_kernel(const __grid_constant__
       const int row = rank * rows + e % rows, r = e / rows * 8;
       if (row >= d.rows) continue;
       float v[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = 0.0f;
-      for (int b = 0; b < split; ++b) {
-        const float4 a = ld_cluster_v4(base + (row * S::pitch + r) * 4, b), z = ld_cluster_v4(base + (row * S::pitch + r + 4) * 4, b);
-        v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w, v[4] += z.x, v[5] += z.y, v[6] += z.z, v[7] += z.w;
-      }
+      const uint32_t from = base + (row * S::pitch + r) * 4;
+      if (split == 8) cluster_sum<8>(from, v);
+      else if (split == 4) cluster_sum<4>(from, v);
+      else if (split == 2) cluster_sum<2>(from, v);
+      else cluster_sum<1>(from, v);
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] = r + k < R ? v[k] * s : 0.0f;  // behind R: rows of F that nobody loaded
       if (pass == 0) {
@@ -425,6 +440,8 @@ __global__ void __launch_bounds__(kUpThreads, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t at = (smem_u32(raw) + 1023) & ~1023u;
   if (tid == 0) {
+    prefetch_map(&fm);
+    if (bm.ok) prefetch_map(&bm.map);
     for (int i = 0; i < NS; ++i) mbar_init(&full[i], 64), mbar_init(&added[i], 128), mbar_init(&empty[i], 128);
     for (int i = 0; i < NF; ++i) mbar_init(&f_full[i], 1), mbar_init(&f_empty[i], 1);
     for (int i = 0; i < NI; ++i) mbar_init(&i_full[i], 1), mbar_init(&i_empty[i], 1);
@@ -735,6 +752,7 @@ __global__ void __launch_bounds__(kOuterLoaders + 32, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
   if (tid == 0) {
+    if (xm.ok) prefetch_map(&xm.map);
     for (int i = 0; i < NS; ++i) mbar_init(&full[i], kOuterLoaders), mbar_init(&empty[i], 1);
     mbar_init(&done, 1);
     mbar_init(&free_, kOuterLoaders);
