@@ -1,14 +1,17 @@
 // lq_adapters_mm.cu -- the three products of the adapter bank for batches of
-// many tokens, over tiles of up to 128 tokens of one adapter:
-//   ad_down    u = s A x      [128 tokens x K] by [K x rank], tcgen05
-//   ad_up      y = base + B^T u   [128 tokens x rank] by [rank x 256], mma.sync
-//   ad_outer   dA = sum v x^T  [256 columns x tokens] by [tokens x rank], tcgen05
+// many tokens, over tiles of up to 128 tokens of one adapter, on tcgen05:
+//   ad_down    u = s A x          [128 tokens x K] by [K x rank]
+//   ad_up      y = base + B^T u   [128 tokens x rank] by [rank x 128 columns]
+//   ad_outer   dA = sum v x^T     [256 columns x tokens] by [tokens x rank]
 // All three are bound by memory (2 R flops to 2 bytes of x): the point is to
-// read x, dy and base once, and to keep the loads coming.
+// read x, dy and base once, and to keep the loads coming.  With 16384 tokens,
+// 14336 columns and rank 64 in bf16: ad_down 80 us (470 MB, 5.9 TB/s), ad_up 157
+// (940 MB read and written, 6.0 TB/s), ad_outer of 4096 and 14336 columns 105
+// (604 MB, 5.8 TB/s); a copy reaches 6.4 TB/s.
 //
-// u and v are fp32.  Where they meet a 16-bit factor they go in as two 16-bit
-// values, hi = round(u) and lo = round(u - hi), and two products: u is then off
-// by 2^-16 of itself (bf16; 2^-22 in fp16), far below the rounding of the
+// u and v are fp32 sums.  Where they meet a 16-bit factor they go in as two
+// 16-bit values, hi = round(u) and lo = round(u - hi), and two products: u is then
+// off by 2^-16 of itself (bf16; 2^-22 in fp16), far below the rounding of the
 // output, where one 16-bit value would be off as much as that.  fp16 has too
 // small a range for values nobody scaled: a row of u (an adapter's rows of v)
 // goes in times a power of two that puts its greatest below 2^13, which is
@@ -385,20 +388,20 @@ __global__ void __launch_bounds__(160, 2) ad_down_kernel(const __grid_constant__
 // ---------------------------------------------------------------------------
 // out = base + u f, a unit of one tile and 128 columns at a time: D [128 tokens
 // x 128] = (hi + lo) [128 x NP] F [NP x 128], F as its rows lie in memory.  A
-// block has a stretch of units.  Base and F come by cp.async, whole rows of 256
-// bytes to half a warp; the thread that has a row of D adds it to the row of base
+// block has a stretch of units.  Base and F come by TMA (base whose tokens do not
+// follow each other by cp.async, a row of 256 bytes to half a warp); the thread that has a row of D adds it to the row of base
 // in shared memory, and half a warp of others takes each row out again.  (A lane that
 // loads its own part of base, as mma.sync deals D out, touches eight lines of
-// 64 bytes each at a time: L1 was busy 4 cycles of 5.  Bulk copies of a row
-// each took 30 cycles apiece.)  Two groups of four warps take turns with the
+// 64 bytes each at a time: L1 was busy 4 cycles of 5, 224 us of the 157 above.
+// Bulk copies of a row each took 30 cycles apiece, 440 us.)  Two groups of four warps take turns with the
 // units, and two teams of two warps with bringing base.
 // ---------------------------------------------------------------------------
 constexpr int kUpBeside = 4;  // blocks that go along a tile's rows side by side, so that 1024 bytes of a row are asked for at a time
 constexpr int kUpThreads = 704;  // 8 warps add, 8 take out, 4 bring base, 1 F, 1 has the products
 template <int NP>
 struct UpShared {
-  // Two stages of base are being added to, two taken out, the others on their way.
-  // An even number: a stage then is always the same team's and the same group's,
+  // Two stages of base are being added to, two taken out, the others on their way
+  // (with three in all, each with its F, 226 us of the 157 above).  An even number: a stage then is always the same team's and the same group's,
   // who see each of its phases (a barrier's parity tells a phase from the next one
   // only, and nothing else keeps the teams abreast).
   static constexpr int stages = NP <= 32 ? 6 : 4;
