@@ -392,18 +392,21 @@ __global__ void __launch_bounds__(160, 2) ad_down_kernel(const __grid_constant__
 // follow each other by cp.async, a row of 256 bytes to half a warp); the thread that has a row of D adds it to the row of base
 // in shared memory, and half a warp of others takes each row out again.  (A lane that
 // loads its own part of base, as mma.sync deals D out, touches eight lines of
-// 64 bytes each at a time: L1 was busy 4 cycles of 5, 224 us of the 157 above.
-// Bulk copies of a row each took 30 cycles apiece, 440 us.)  Two groups of four warps take turns with the
-// units, and two teams of two warps with bringing base.
+// 64 bytes each at a time: L1 was busy 4 cycles of 5, 224 us instead of the 157
+// above.  Bulk copies of a row each took 30 cycles apiece, 440 us.)  Two groups of
+// four warps take turns with the units, and two teams of two with bringing base.
 // ---------------------------------------------------------------------------
-constexpr int kUpBeside = 4;  // blocks that go along a tile's rows side by side, so that 1024 bytes of a row are asked for at a time
+// Blocks that go along a tile's rows side by side, so that 1024 bytes of a row are
+// asked for at a time: 162 us, by one 166 (16384 tokens, 14336 columns, rank 64)
+constexpr int kUpBeside = 4;
 constexpr int kUpThreads = 704;  // 8 warps add, 8 take out, 4 bring base, 1 F, 1 has the products
 template <int NP>
 struct UpShared {
   // Two stages of base are being added to, two taken out, the others on their way
-  // (with three in all, each with its F, 226 us of the 157 above).  An even number: a stage then is always the same team's and the same group's,
-  // who see each of its phases (a barrier's parity tells a phase from the next one
-  // only, and nothing else keeps the teams abreast).
+  // (with three in all, each with its F, 226 us instead of the 157 above).  An even
+  // number: a stage then is always the same team's and the same group's, who see
+  // each of its phases (a barrier's parity tells a phase from the next one only, and
+  // nothing else keeps the teams abreast).
   static constexpr int stages = NP <= 32 ? 6 : 4;
   static constexpr int stage = 32768;                   // two halves of 64 columns, rows of 128 bytes, swizzled
   static constexpr int fs = NP <= 64 ? 2 : 1;           // stages of F
