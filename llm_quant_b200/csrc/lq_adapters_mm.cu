@@ -397,7 +397,10 @@ __global__ void __launch_bounds__(160, 2) ad_down_kernel(const __grid_constant__
 // four warps take turns with the units, and two teams of two with bringing base.
 // ---------------------------------------------------------------------------
 // Blocks that go along a tile's rows side by side, so that 1024 bytes of a row are
-// asked for at a time: 162 us, by one 166 (16384 tokens, 14336 columns, rank 64)
+// asked for at a time.  It matters little: means of five runs were 166 us by one,
+// 164 by two, 163 by four, 162 by eight (16384 tokens, 14336 columns, rank 64), where
+// runs of one setting lay up to 8 us apart; eight prompts of up to 2048 tokens, and
+// one of 2048 tokens with 4096 columns and rank 16, showed no difference.
 constexpr int kUpBeside = 4;
 constexpr int kUpThreads = 704;  // 8 warps add, 8 take out, 4 bring base, 1 F, 1 has the products
 template <int NP>
