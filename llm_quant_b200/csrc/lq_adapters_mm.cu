@@ -389,12 +389,14 @@ __global__ void __launch_bounds__(160, 2) ad_down_kernel(const __grid_constant__
 // out = base + u f, a unit of one tile and 128 columns at a time: D [128 tokens
 // x 128] = (hi + lo) [128 x NP] F [NP x 128], F as its rows lie in memory.  A
 // block has a stretch of units.  Base and F come by TMA (base whose tokens do not
-// follow each other by cp.async, a row of 256 bytes to half a warp); the thread that has a row of D adds it to the row of base
-// in shared memory, and half a warp of others takes each row out again.  (A lane that
-// loads its own part of base, as mma.sync deals D out, touches eight lines of
-// 64 bytes each at a time: L1 was busy 4 cycles of 5, 224 us instead of the 157
-// above.  Bulk copies of a row each took 30 cycles apiece, 440 us.)  Two groups of
-// four warps take turns with the units, and two teams of two with bringing base.
+// follow each other by cp.async, a row of 256 bytes to half a warp); the thread that
+// has a row of D adds it to the row of base in shared memory, and half a warp of
+// others takes each row out again.  (A lane that loads its own part of base, as
+// mma.sync deals D out, touches eight lines of 64 bytes each at a time: L1 was busy
+// 4 cycles of 5, and a call of eight prompts of up to 2048 tokens, 4096 to 14336
+// features, rank 64, took 289 us where it takes 207 now.  With bulk copies of a row
+// each it took 484.)  Two groups of four warps take turns with the units, and two
+// teams of two with bringing base.
 // ---------------------------------------------------------------------------
 // Blocks that go along a tile's rows side by side, so that 1024 bytes of a row are
 // asked for at a time.  It matters little: means of five runs were 166 us by one,
