@@ -60,6 +60,9 @@ Tensor rows_of(const Tensor& x, int64_t& stride) {
   return x.clone(at::MemoryFormat::Contiguous);
 }
 
+// t side by side and on 16 bytes
+Tensor whole(const Tensor& t) { return t.is_contiguous() && on16(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
+
 struct Call {
   lq_adapter_bank bank;
   lq_adapter_form form;
@@ -106,10 +109,7 @@ Call run(const Tensor& x, const Tensor& lora_a, const Tensor& lora_b, const Tens
     if (base) from = rows_of(*base, c.form.base_stride);
     c.out = at::empty(shape, x.options().requires_grad(false));
   }
-  const auto ready = [&](const Tensor& t) {
-    const Tensor u = t.scalar_type() == type ? t : t.to(type);
-    return u.is_contiguous() && on16(u) ? u : u.clone(at::MemoryFormat::Contiguous);
-  };
+  const auto ready = [&](const Tensor& t) { return whole(t.scalar_type() == type ? t : t.to(type)); };
   c.a = ready(lora_a), c.b = ready(lora_b), c.s = scaling.contiguous();
   c.bank = {c.a.data_ptr(), c.b.data_ptr(), c.s.data_ptr<float>(), L, R, K, N, code_of(type)};
   if (tokens == 0) return c;
@@ -124,12 +124,16 @@ Call run(const Tensor& x, const Tensor& lora_a, const Tensor& lora_b, const Tens
 struct Adapters : torch::autograd::Function<Adapters> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& lora_a, const Tensor& lora_b,
                         const OptTensor& base, const Tensor& scaling, const Tensor& plan, int64_t tokens, int64_t num_adapters) {
+    TORCH_CHECK(!plan.is_inference(), "AdapterBank: a batch that was made in inference mode cannot be used with gradients");
     Call c = run(x, lora_a, lora_b, scaling, base, plan, tokens, num_adapters, true, false);
     // the weights as the call rounded them; all of these raise if they were changed since
-    ctx->save_for_backward({c.x, c.a, c.b, scaling, plan, c.low});
+    ctx->save_for_backward({c.x, c.a, c.b, scaling, c.low});
+    // not the plan: saved-tensor hooks may bring back copies, and its status word is read where it lies
+    ctx->saved_data["plan"] = plan;
+    ctx->saved_data["version"] = static_cast<int64_t>(plan._version());
     ctx->saved_data["shape"] = x.sizes().vec();
     ctx->saved_data["type"] = static_cast<int64_t>(lora_a.scalar_type());
-    ctx->saved_data["stride"] = c.form.x_stride;
+    ctx->saved_data["adapters"] = num_adapters;
     ctx->saved_data["base"] = base.has_value();
     return c.out;
   }
@@ -143,15 +147,32 @@ struct Adapters : torch::autograd::Function<Adapters> {
     if (ctx->saved_data["base"].toBool()) out[3] = dy;
     if (!want[0] && !want[1] && !want[2]) return out;
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &a = saved[1], &b = saved[2], &plan = saved[4], &low = saved[5];
-    const Tensor s = saved[3].contiguous();
-    const c10::cuda::CUDAGuard guard(x.device());
+    const Tensor plan = ctx->saved_data["plan"].toTensor();
+    TORCH_CHECK(static_cast<int64_t>(plan._version()) == ctx->saved_data["version"].toInt(),
+                "AdapterBank: the batch that gradients are computed for has been modified by an inplace operation "
+                "(AdapterBatch.update) since the forward call");
     const auto type = static_cast<at::ScalarType>(ctx->saved_data["type"].toInt());
     const auto shape = ctx->saved_data["shape"].toIntVector();
+    // A hook may have laid them out anew, but what they hold has to be the same.
+    const int64_t L = ctx->saved_data["adapters"].toInt(), R = saved[1].dim() == 3 ? saved[1].size(1) : 0;
+    const int64_t sizes[3][3] = {{L, R, shape.back()}, {L, R, dy.size(-1)}};
+    TORCH_CHECK(saved[0].sizes() == at::IntArrayRef(shape) && saved[1].sizes() == at::IntArrayRef(sizes[0], 3) &&
+                    saved[2].sizes() == at::IntArrayRef(sizes[1], 3) && saved[3].sizes() == at::IntArrayRef(L),
+                "AdapterBank: saved tensors came back with other shapes");
+    for (const Tensor& t : saved)
+      if (t.defined())
+        TORCH_CHECK(t.device() == plan.device(), "AdapterBank: a saved tensor came back on ", t.device(), ", not on ", plan.device());
+    for (int i = 0; i < 3; ++i)
+      TORCH_CHECK(saved[i].scalar_type() == dy.scalar_type(), "AdapterBank: a saved tensor came back in ", name_of(saved[i].scalar_type()));
+    TORCH_CHECK(saved[3].scalar_type() == at::kFloat && (!saved[4].defined() || saved[4].scalar_type() == at::kByte),
+                "AdapterBank: saved tensors came back in other types");
+    const c10::cuda::CUDAGuard guard(plan.device());
+    lq_adapter_form form = {saved[0].numel() / shape.back(), 0, 0, 0, 1};
+    const Tensor x = rows_of(saved[0], form.x_stride), a = whole(saved[1]), b = whole(saved[2]), s = saved[3].contiguous();
+    const Tensor low = saved[4].defined() ? whole(saved[4]) : Tensor();
     const lq_adapter_bank bank = {a.data_ptr(), b.data_ptr(), s.data_ptr<float>(), a.size(0), a.size(1), a.size(2), b.size(2),
                                   code_of(x.scalar_type())};
-    const int64_t n = x.numel() / a.size(2);
-    lq_adapter_form form = {n, ctx->saved_data["stride"].toInt(), 0, 0, 1};
+    const int64_t n = form.n;
     const Tensor d = rows_of(dy, form.out_stride);
     if (want[0]) out[0] = at::empty(shape, x.options());
     if (want[1]) out[1] = at::empty(a.sizes(), x.options().dtype(type));

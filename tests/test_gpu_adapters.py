@@ -663,3 +663,68 @@ def test_offsets_over_32_bits():
     assert not db[0].any()
     with torch.no_grad():
         assert torch.equal(bank.add_(base, x, batch), y)
+
+
+def _off16(t):
+    """A copy of t, side by side, whose address is off 16 bytes."""
+    memory = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+    memory[1:].copy_(t.detach().reshape(-1))
+    return memory[1:].view(t.shape)
+
+
+def _turned(t):
+    return t.detach().transpose(0, -1).contiguous().transpose(0, -1)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_saved_tensors_that_come_back_laid_out_anew(dt):
+    """Saved-tensor hooks may bring back copies: offloaded ones, dense ones of a
+    strided x, turned ones, ones off 16 bytes.  Gradients are the same."""
+    K, N = 128, 264
+    bank, x, base, dy = make(2, 150, 2, 16, K, N, TYPES[dt], seed=50)
+    bank.requires_grad_(True)
+    batch = L.AdapterBatch(some_ids(2, 2, 3, False), 2, 150)
+    wide = torch.zeros(300, 400, dtype=TYPES[dt], device=DEV)
+    wide[:, 8:8 + K] = x
+    rows = wide[:, 8:8 + K].requires_grad_(True)
+
+    def grads(y):
+        return torch.autograd.grad(y, (rows, bank.lora_A, bank.lora_B), dy)
+
+    want = grads(bank(rows, batch, base))
+    with torch.autograd.graph.save_on_cpu():
+        y = bank(rows, batch, base)
+    assert all(torch.equal(p, q) for p, q in zip(grads(y), want))
+    packed = []
+
+    def pack(t):
+        packed.append(t.data_ptr())
+        return t.detach()
+
+    for unpack in (lambda t: t.contiguous().clone(), _turned, _off16):
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            y = bank(rows, batch, base)
+        assert all(torch.equal(p, q) for p, q in zip(grads(y), want))
+    assert batch._plan.data_ptr() not in packed  # check() reads the plan that the kernels wrote to
+    batch.check()
+    for unpack, word in ((lambda t: t.cpu(), "came back on cpu"), (lambda t: t.double(), "came back in"),
+                         (lambda t: t[:1], "other shapes")):
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            y = bank(rows, batch, base)
+        with pytest.raises(RuntimeError, match=word):
+            grads(y)
+    with torch.autograd.graph.save_on_cpu():
+        y = bank(rows, batch, base)
+    batch.update(some_ids(2, 2, 3, False))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        grads(y)
+
+
+def test_a_batch_of_inference_mode_has_no_gradients():
+    bank, x, base, _ = make(4, 1, 2, 8, 64, 64, torch.bfloat16)
+    with torch.inference_mode():
+        batch = L.AdapterBatch(torch.zeros(4, dtype=torch.int32, device=DEV), 2)
+    assert torch.equal(bank(x, batch, base), bank(x, L.AdapterBatch(torch.zeros(4, dtype=torch.int32, device=DEV), 2), base))
+    bank.requires_grad_(True)
+    with pytest.raises(RuntimeError, match="inference mode"):
+        bank(x, batch, base)
