@@ -217,6 +217,10 @@ class Clipper {
     bytes_ = lq_clip_workspace_bytes(in_.size());
   }
   Tensor clip(double max_norm) const {
+    for (size_t i = 0; i < in_.size(); ++i) {
+      stays(in_[i], from_[i], i);
+      if (out_) stays((*out_)[i], to_[i], i);
+    }
     const c10::cuda::CUDAGuard guard(in_[0].device());
     const auto options = at::TensorOptions().device(in_[0].device());
     const Tensor norm = at::empty({}, options.dtype(at::kFloat)), ws = at::empty({(int64_t)bytes_}, options.dtype(at::kByte));
@@ -227,6 +231,11 @@ class Clipper {
   }
 
  private:
+  // A storage that was resized has other memory, for its aliases too.
+  static void stays(const Tensor& t, const void* at, size_t i) {
+    TORCH_CHECK(t.numel() == 0 || (t.const_data_ptr() == at && t.storage().nbytes() >= (t.storage_offset() + t.numel()) * t.itemsize()),
+                "GradClipper: the storage of tensor ", i, " was resized since the clipper was made");
+  }
   std::vector<Tensor> in_;
   std::optional<std::vector<Tensor>> out_;
   std::vector<Tensor> written_;  // whose versions go up: one of those that share a buffer

@@ -122,3 +122,16 @@ def test_a_bank_of_layers():
         bank.load_adapter(2, layers[0].lora_A, layers[0].lora_B, 1.0)
     with pytest.raises(ValueError):
         bank.load_adapter(0, layers[0].lora_A, layers[1].lora_B, 1.0)
+
+
+def test_a_clipper_whose_memory_went(lib):
+    """Addresses are taken once: a storage that was resized since is refused before any launch."""
+    from llm_quant_b200 import _C
+    for size in (0, 64, 1 << 20):
+        g = torch.zeros(100)
+        for clipper in (_C.ext().Clipper([torch.ones(8), g.detach()], None, []), _C.ext().Clipper([torch.ones(100)], [g.detach()], [])):
+            kept = g.untyped_storage().size()
+            g.untyped_storage().resize_(size)
+            with pytest.raises(RuntimeError, match="storage of tensor . was resized"):
+                clipper.clip(1.0)
+            g.untyped_storage().resize_(kept)

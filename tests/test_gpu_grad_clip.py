@@ -235,3 +235,16 @@ def test_offsets_over_32_bits():
     for i in range(0, n, step):
         want = g[i:i + step].double() * c
         assert bool(((out[i:i + step].double() - want).abs() <= (2.0 ** -8 + 6 * 2.0 ** -24) * want.abs() + 2.0 ** -134).all())
+
+
+def test_resized_storage():
+    """What a gradient's storage was resized to is not the clipper's memory any more."""
+    g = rand(1000, torch.float32)
+    clipper, into = L.GradClipper([g]), L.GradClipper([rand(1000, torch.float32)], [g])
+    g.untyped_storage().resize_(0)
+    for c in (clipper, into):
+        with pytest.raises(RuntimeError, match="resized"):
+            c.clip(1.0)
+    g.untyped_storage().resize_(4000)
+    g.fill_(1.0)
+    assert abs(float(L.GradClipper([g]).clip(1.0)) - 1000 ** 0.5) < 1e-4
