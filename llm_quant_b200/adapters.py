@@ -183,7 +183,9 @@ class AdapterBank(nn.Module):
 
     def add_(self, y: torch.Tensor, x: torch.Tensor, batch: AdapterBatch) -> torch.Tensor:
         """y += each token's adapter of x, in place; no gradient (call it under
-        ``torch.no_grad()``).  Rows of tokens without an adapter are not written."""
+        ``torch.no_grad()``).  Rows of tokens without an adapter are not written.  y
+        may be x, or share x's buffer, where no row of y overlaps another token's
+        row of x."""
         p = self._parameters
         _C.ext().adapters_add_(y, x, p["lora_A"], p["lora_B"], self._buffers["scaling"], batch._plan, batch.tokens,
                                batch.num_adapters)

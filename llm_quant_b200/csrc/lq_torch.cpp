@@ -63,6 +63,17 @@ Tensor rows_of(const Tensor& x, int64_t& stride) {
 // t side by side and on 16 bytes
 Tensor whole(const Tensor& t) { return t.is_contiguous() && on16(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
 
+// Whether the rows of y (ys apart, N wide) can be written where the rows of x are
+// read: none is another token's row of x.  A token's own row is read before it
+// is written.
+bool rows_apart(const Tensor& x, int64_t xs, int64_t K, const Tensor& y, int64_t ys, int64_t N, int64_t tokens) {
+  const int64_t at_x = reinterpret_cast<intptr_t>(x.data_ptr()) / 2, at_y = reinterpret_cast<intptr_t>(y.data_ptr()) / 2;
+  if (tokens <= 1 || at_x + (tokens - 1) * xs + K <= at_y || at_y + (tokens - 1) * ys + N <= at_x) return true;
+  if (xs != ys || xs < K) return false;
+  const int64_t d = at_y - at_x, c = (d % xs + xs) % xs;  // the columns of x's rows that y begins at
+  return c + N <= xs && (c >= K || c == d);
+}
+
 struct Call {
   lq_adapter_bank bank;
   lq_adapter_form form;
@@ -103,6 +114,8 @@ Call run(const Tensor& x, const Tensor& lora_a, const Tensor& lora_b, const Tens
     const int64_t stride = row_stride(*base);
     TORCH_CHECK_VALUE(stride >= 0 && (tokens <= 1 || stride >= N), "AdapterBank.add_: y ", base->sizes(), " with strides ",
                       base->strides(), " must be rows on 16 bytes");
+    TORCH_CHECK_VALUE(rows_apart(c.x, c.form.x_stride, K, *base, stride, N, tokens),
+                      "AdapterBank.add_: rows of y overlap other tokens' rows of x");
     c.form.base_stride = c.form.out_stride = stride;
     from = c.out = *base;
   } else {

@@ -728,3 +728,40 @@ def test_a_batch_of_inference_mode_has_no_gradients():
     bank.requires_grad_(True)
     with pytest.raises(RuntimeError, match="inference mode"):
         bank(x, batch, base)
+
+
+def test_in_place_in_the_buffer_of_x():
+    """Rows of y and of x in one buffer: columns beside each other, the same columns,
+    tokens behind each other; rows of y that overlap other tokens' rows of x are refused."""
+    for n, seq in ((5, 1), (3, 400)):
+        T, K, N = n * seq, 128, 64
+        bank, x, base, _ = make(n, seq, 2, 16, K, N, torch.bfloat16, seed=51)
+        batch = L.AdapterBatch(some_ids(n, 2, 6, True), 2, seq)
+        want = bank(x, batch, base)
+
+        def placed(cols, xs, ys):
+            buf = torch.zeros(2 * T + 2, cols, dtype=torch.bfloat16, device=DEV)
+            vx, vy = buf[xs[0]:xs[0] + T, xs[1]:xs[1] + K], buf[ys[0]:ys[0] + T, ys[1]:ys[1] + N]
+            vx.copy_(x)
+            vy.copy_(base)
+            return vx, vy
+
+        for at in (((0, 0), (0, 128)), ((0, 64), (0, 0)), ((0, 0), (1, 128)), ((1, 0), (0, 128)), ((0, 0), (T, 0)), ((T, 8), (0, 72))):
+            vx, vy = placed(192, *at)
+            assert torch.equal(bank.add_(vy, vx, batch), want)
+        for c in (0, 8, 64):  # columns of x itself
+            vx, vy = placed(K, (0, 0), (0, c))
+            mine = bank(vx, batch, vy)
+            assert torch.equal(bank.add_(vy, vx, batch), mine)
+        for cols, xs, ys in ((K, (0, 0), (1, 0)), (K, (1, 0), (0, 64)), (192, (0, 0), (1, 64)), (192, (1, 0), (0, 64))):
+            vx, vy = placed(cols, xs, ys)
+            with pytest.raises(ValueError, match="overlap other tokens"):
+                bank.add_(vy, vx, batch)
+        flat = torch.zeros(T * K, dtype=torch.bfloat16, device=DEV)  # other distances from row to row
+        with pytest.raises(ValueError, match="overlap other tokens"):
+            bank.add_(flat[:T * N].view(T, N), flat.view(T, K), batch)
+        with pytest.raises(ValueError, match="overlap other tokens"):  # windows of x that overlap each other
+            bank.add_(flat.as_strided((T, N), (64, 1), 0), flat.as_strided((T, K), (64, 1), 0), batch)
+        one, first = x[:1], L.AdapterBatch(torch.zeros(1, dtype=torch.int32, device=DEV), 2)
+        mine = bank(one, first, one[:, 8:72])
+        assert torch.equal(bank.add_(one[:, 8:72], one, first), mine)
