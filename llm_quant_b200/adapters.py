@@ -164,6 +164,8 @@ class AdapterBank(nn.Module):
         r = lora_A.shape[0]
         if not 0 <= index < self.num_adapters:
             raise IndexError(f"AdapterBank.load_adapter: {index} outside [0, {self.num_adapters})")
+        if nn.utils.parametrize.is_parametrized(self):
+            raise RuntimeError("AdapterBank.load_adapter: the bank's tensors are computed (nn.utils.parametrize)")
         if lora_A.shape != (r, self.in_features) or lora_B.shape != (self.out_features, r) or r > self.rank:
             raise ValueError(f"AdapterBank.load_adapter: lora_A {list(lora_A.shape)} and lora_B {list(lora_B.shape)} for "
                              f"a bank of {self.in_features} to {self.out_features} features, rank {self.rank}")
@@ -177,8 +179,7 @@ class AdapterBank(nn.Module):
     def forward(self, x: torch.Tensor, batch: AdapterBatch, base: Optional[torch.Tensor] = None) -> torch.Tensor:
         """base [..., out_features] (default zeros) plus each token's adapter of
         x [..., in_features], whose leading dimensions are the batch's tokens."""
-        p = self._parameters
-        return _C.ext().adapters_forward(x, p["lora_A"], p["lora_B"], self._buffers["scaling"], base, batch._plan, batch.tokens,
+        return _C.ext().adapters_forward(x, self.lora_A, self.lora_B, self.scaling, base, batch._plan, batch.tokens,
                                          batch.num_adapters)
 
     def add_(self, y: torch.Tensor, x: torch.Tensor, batch: AdapterBatch) -> torch.Tensor:
@@ -186,9 +187,7 @@ class AdapterBank(nn.Module):
         ``torch.no_grad()``).  Rows of tokens without an adapter are not written.  y
         may be x, or share x's buffer, where no row of y overlaps another token's
         row of x."""
-        p = self._parameters
-        _C.ext().adapters_add_(y, x, p["lora_A"], p["lora_B"], self._buffers["scaling"], batch._plan, batch.tokens,
-                               batch.num_adapters)
+        _C.ext().adapters_add_(y, x, self.lora_A, self.lora_B, self.scaling, batch._plan, batch.tokens, batch.num_adapters)
         return y
 
     def extra_repr(self) -> str:

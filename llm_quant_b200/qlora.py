@@ -319,6 +319,9 @@ class QLoRALinear(nn.Module):
         if torch.is_grad_enabled() and (base.requires_grad or x.requires_grad or adapters.lora_A.requires_grad
                                         or adapters.lora_B.requires_grad):
             return adapters(x, batch, base)
+        if type(adapters).forward is not AdapterBank.forward or nn.modules.module._has_any_global_hook() \
+                or adapters._forward_pre_hooks or adapters._forward_hooks:
+            return adapters(x, batch, base)  # what a wrapper or a hook does around the bank's call is done
         return adapters.add_(base, x, batch)
 
     def merge_lora(self) -> torch.Tensor:

@@ -135,3 +135,32 @@ def test_a_clipper_whose_memory_went(lib):
             with pytest.raises(RuntimeError, match="storage of tensor . was resized"):
                 clipper.clip(1.0)
             g.untyped_storage().resize_(kept)
+
+
+class _Twice(torch.nn.Module):
+    def forward(self, t):
+        return 2 * t
+
+
+def test_tensors_that_are_not_the_modules_parameters(lib):
+    """Parametrized ones and those of a replica are found as attributes; no call
+    fails before the device is asked for."""
+    from types import SimpleNamespace
+    batch = SimpleNamespace(_plan=torch.zeros(64, dtype=torch.uint8), tokens=4, num_adapters=2)
+    x = torch.zeros(4, 64, dtype=torch.bfloat16)
+    for change in ("parametrized", "replica"):
+        bank = L.AdapterBank(64, 128, 2, 8)
+        if change == "parametrized":
+            torch.nn.utils.parametrize.register_parametrization(bank, "lora_A", _Twice())
+        else:
+            copy = bank._replicate_for_data_parallel()
+            for name, t in (*bank._parameters.items(), *bank._buffers.items()):
+                setattr(copy, name, t.detach())
+            bank = copy
+        with torch.no_grad():
+            for call in (lambda: bank(x, batch), lambda: bank.add_(torch.zeros(4, 128, dtype=torch.bfloat16), x, batch)):
+                with pytest.raises(RuntimeError, match="CUDA"):
+                    call()
+        if change == "parametrized":
+            with pytest.raises(RuntimeError, match="computed"):
+                bank.load_adapter(0, torch.zeros(8, 64), torch.zeros(128, 8), 1.0)

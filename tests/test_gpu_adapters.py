@@ -765,3 +765,57 @@ def test_in_place_in_the_buffer_of_x():
         one, first = x[:1], L.AdapterBatch(torch.zeros(1, dtype=torch.int32, device=DEV), 2)
         mine = bank(one, first, one[:, 8:72])
         assert torch.equal(bank.add_(one[:, 8:72], one, first), mine)
+
+
+class _Twice(torch.nn.Module):
+    def forward(self, t):
+        return 2 * t
+
+
+def test_parametrized_banks_and_hooks():
+    """Tensors that are computed from others, and what hooks and wrappers do around a bank's call."""
+    dt = torch.bfloat16
+    bank, x, base, dy = make(3, 20, 2, 16, 128, 256, dt, seed=52)
+    batch = L.AdapterBatch(some_ids(3, 2, 4, True), 2, 20)
+    plain, _, _, _ = make(3, 20, 2, 16, 128, 256, dt, seed=52)
+    plain.lora_A.mul_(2)
+    for b in (bank, plain):
+        b.requires_grad_(True)
+    torch.nn.utils.parametrize.register_parametrization(bank, "lora_A", _Twice())
+    y, want = bank(x, batch, base), plain(x, batch, base)
+    assert torch.equal(y, want)
+    got = torch.autograd.grad(y, (bank.parametrizations.lora_A.original, bank.lora_B), dy)
+    ref = torch.autograd.grad(want, (plain.lora_A, plain.lora_B), dy)
+    assert torch.equal(got[0], 2 * ref[0]) and torch.equal(got[1], ref[1])
+
+    class Wrapped(torch.nn.Module):
+        in_features, out_features = 128, 256
+
+        def __init__(self):
+            super().__init__()
+            self.bank, self.calls = plain, 0
+
+        def __getattr__(self, name):
+            try:
+                return super().__getattr__(name)
+            except AttributeError:
+                return getattr(super().__getattr__("bank"), name)
+
+        def forward(self, *args):
+            self.calls += 1
+            return self.bank(*args)
+
+    ql = L.QLoRALinear(128, 256).to(DEV)
+    ql.pack_base((torch.randn(256, 128, device=DEV, generator=torch.Generator(DEV).manual_seed(0)) * 0.1).to(dt))
+    wrapped, seen = Wrapped(), []
+    with torch.no_grad():
+        want = ql(x, plain, batch)
+        assert torch.equal(ql(x, wrapped, batch), want) and wrapped.calls == 1
+        hooks = [plain.register_forward_pre_hook(lambda m, args: seen.append("before")),
+                 plain.register_forward_hook(lambda m, args, out: seen.append("behind"))]
+        assert torch.equal(ql(x, plain, batch), want) and seen == ["before", "behind"]
+        for h in hooks:
+            h.remove()
+        every = torch.nn.modules.module.register_module_forward_hook(lambda m, args, out: seen.append(type(m)))
+        assert torch.equal(ql(x, plain, batch), want) and L.AdapterBank in seen
+        every.remove()
