@@ -200,8 +200,16 @@ struct Adapters : torch::autograd::Function<Adapters> {
   }
 };
 
+// A tangent of forward mode would be lost without a word.
+void no_tangents(std::initializer_list<const Tensor*> tensors) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : tensors)
+    TORCH_CHECK(!t || !t->defined() || !t->_fw_grad(0).defined(), "AdapterBank: forward-mode derivatives are not computed");
+}
+
 Tensor adapters_forward(const Tensor& x, const Tensor& lora_a, const Tensor& lora_b, const Tensor& scaling, const OptTensor& base,
                         const Tensor& plan, int64_t tokens, int64_t num_adapters) {
+  no_tangents({&x, &lora_a, &lora_b, &scaling, base ? &*base : nullptr});
   const c10::OptionalDeviceGuard guard(x.is_cuda() ? std::make_optional(x.device()) : std::nullopt);
   if (at::GradMode::is_enabled() &&
       (x.requires_grad() || lora_a.requires_grad() || lora_b.requires_grad() || (base && base->requires_grad())))
@@ -211,6 +219,7 @@ Tensor adapters_forward(const Tensor& x, const Tensor& lora_a, const Tensor& lor
 
 void adapters_add_(const Tensor& y, const Tensor& x, const Tensor& lora_a, const Tensor& lora_b, const Tensor& scaling,
                    const Tensor& plan, int64_t tokens, int64_t num_adapters) {
+  no_tangents({&y, &x, &lora_a, &lora_b, &scaling});
   TORCH_CHECK(!at::GradMode::is_enabled() ||
                   !(x.requires_grad() || y.requires_grad() || lora_a.requires_grad() || lora_b.requires_grad()),
               "AdapterBank.add_: no gradient is computed here (use forward, or torch.no_grad())");

@@ -164,3 +164,24 @@ def test_tensors_that_are_not_the_modules_parameters(lib):
         if change == "parametrized":
             with pytest.raises(RuntimeError, match="computed"):
                 bank.load_adapter(0, torch.zeros(8, 64), torch.zeros(128, 8), 1.0)
+
+
+def test_forward_mode_is_refused(lib):
+    """A tangent would be lost without a word."""
+    import torch.autograd.forward_ad as fw
+    from types import SimpleNamespace
+    batch = SimpleNamespace(_plan=torch.zeros(64, dtype=torch.uint8), tokens=4, num_adapters=2)
+    bank = L.AdapterBank(64, 128, 2, 8).requires_grad_(False)
+    x, y = torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(4, 128, dtype=torch.bfloat16)
+    with fw.dual_level():
+        dual_x, dual_y = fw.make_dual(x, torch.ones_like(x)), fw.make_dual(y, torch.ones_like(y))
+        for call in (lambda: bank(dual_x, batch), lambda: bank(x, batch, dual_y), lambda: bank.add_(dual_y, x, batch),
+                     lambda: bank.add_(y, dual_x, batch)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        with pytest.raises(RuntimeError, match="CUDA"):  # nothing has a tangent
+            bank(x, batch, y)
+        del bank.lora_B
+        bank.lora_B = fw.make_dual(torch.zeros(2, 8, 128, dtype=torch.bfloat16), torch.ones(2, 8, 128, dtype=torch.bfloat16))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            bank(x, batch)
