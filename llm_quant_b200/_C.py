@@ -166,17 +166,20 @@ _ext = None
 def ext():
     """The calls that are bound in C++ (csrc/lq_torch.cpp); raise if they are not built."""
     global _ext
-    if _ext is None:
-        import importlib.machinery
-        import importlib.util
-        lib()  # lq_torch.so is linked against it
-        path = os.path.join(os.path.dirname(LIB_PATH), "lq_torch.so")
-        if not os.path.exists(path):
-            raise RuntimeError(f"{path} is not built; run `python -m llm_quant_b200.build`")
-        loader = importlib.machinery.ExtensionFileLoader("lq_torch", path)
-        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("lq_torch", loader))
-        loader.exec_module(module)
-        _ext = module
+    if _ext is not None:
+        return _ext
+    lib()  # lq_torch.so is linked against it
+    with _lock:
+        if _ext is None:
+            import importlib.machinery
+            import importlib.util
+            path = os.path.join(os.path.dirname(LIB_PATH), "lq_torch.so")
+            if not os.path.exists(path):
+                raise RuntimeError(f"{path} is not built; run `python -m llm_quant_b200.build`")
+            loader = importlib.machinery.ExtensionFileLoader("lq_torch", path)
+            module = importlib.util.module_from_spec(importlib.util.spec_from_loader("lq_torch", loader))
+            loader.exec_module(module)
+            _ext = module
     return _ext
 
 

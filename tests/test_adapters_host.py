@@ -185,3 +185,30 @@ def test_forward_mode_is_refused(lib):
         bank.lora_B = fw.make_dual(torch.zeros(2, 8, 128, dtype=torch.bfloat16), torch.ones(2, 8, 128, dtype=torch.bfloat16))
         with pytest.raises(RuntimeError, match="forward-mode"):
             bank(x, batch)
+
+
+def test_first_calls_of_many_threads(lib, monkeypatch):
+    """The bindings are loaded once, whoever comes first."""
+    import importlib.machinery
+    import threading
+    import time
+    from llm_quant_b200 import _C
+    loads = []
+
+    class Loader(importlib.machinery.ExtensionFileLoader):
+        def create_module(self, spec):
+            return None
+
+        def exec_module(self, module):
+            loads.append(module)
+            time.sleep(0.2)
+
+    monkeypatch.setattr(_C, "_ext", None)
+    monkeypatch.setattr(importlib.machinery, "ExtensionFileLoader", Loader)
+    got = []
+    threads = [threading.Thread(target=lambda: got.append(_C.ext())) for _ in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(loads) == 1 and len(got) == 8 and all(m is loads[0] for m in got)
