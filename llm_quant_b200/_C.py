@@ -179,6 +179,10 @@ def ext():
             loader = importlib.machinery.ExtensionFileLoader("lq_torch", path)
             module = importlib.util.module_from_spec(importlib.util.spec_from_loader("lq_torch", loader))
             loader.exec_module(module)
+            built = getattr(module, "torch_version", "")
+            if not torch.__version__.startswith(built):
+                raise RuntimeError(f"{path} was built for torch {built}, this is {torch.__version__}; run "
+                                   "`python -m llm_quant_b200.build`")
             _ext = module
     return _ext
 

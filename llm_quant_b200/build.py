@@ -12,6 +12,7 @@ may be contracted into one FMA.
 
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -71,23 +72,32 @@ def _compile(src: str, force: bool, verbose: bool) -> str:
     return obj
 
 
+def _cxx() -> str:
+    return os.environ.get("CXX") or "g++"
+
+
 def _compile_ext(force: bool) -> str:
-    """lq_torch.cpp against the installed torch's headers."""
-    src, obj = os.path.join(CSRC, "lq_torch.cpp"), os.path.join(OBJDIR, "lq_torch.o")
-    header = os.path.join(INCLUDE, "lq_sm100.h")
-    if not force and os.path.exists(obj) and os.path.getmtime(obj) >= max(os.path.getmtime(src), os.path.getmtime(header)):
-        return obj
+    """lq_torch.cpp against the installed torch's headers; again for another torch, Python or compiler."""
     import sysconfig
     import torch
+    src, obj, made = os.path.join(CSRC, "lq_torch.cpp"), os.path.join(OBJDIR, "lq_torch.o"), os.path.join(OBJDIR, "lq_torch.for")
+    key = f"torch {torch.__version__} python {sys.version} {_cxx()}"
+    if not force and os.path.exists(obj) and os.path.exists(made):
+        with open(made) as f:
+            same = f.read() == key
+        if same and os.path.getmtime(obj) >= max(os.path.getmtime(src), os.path.getmtime(os.path.join(INCLUDE, "lq_sm100.h"))):
+            return obj
     root = os.path.join(os.path.dirname(torch.__file__), "include")
     cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-c", src, "-o", obj,
+    cmd = [_cxx(), "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-c", src, "-o", obj,
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", "-DTORCH_API_INCLUDE_EXTENSION_H"]
     for d in (root, os.path.join(root, "torch", "csrc", "api", "include"), cuda, sysconfig.get_paths()["include"]):
         cmd += ["-isystem", d]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"the host compiler failed for lq_torch.cpp:\n{r.stdout}\n{r.stderr}")
+    with open(made, "w") as f:
+        f.write(key)
     return obj
 
 
@@ -99,8 +109,8 @@ def _link_ext(obj: str, force: bool) -> None:
     libs = os.path.join(os.path.dirname(torch.__file__), "lib")
     # torch's own libstdc++, never a static one: two copies in a process do not share
     # their locales, and formatting a number in the second one ends it
-    cmd = [os.environ.get("CXX", "g++"), "-shared", "-o", tmp, obj, LIB, "-Wl,-rpath,$ORIGIN", f"-L{libs}", "-lc10", "-ltorch_cpu",
-           "-ltorch_python", "-lc10_cuda", "-ltorch_cuda", "-nostdlib++", "-l:libstdc++.so.6"]
+    cmd = [_cxx(), "-shared", "-o", tmp, obj, LIB, "-Wl,-rpath,$ORIGIN", f"-L{libs}", "-lc10", "-ltorch_cpu", "-ltorch_python",
+           "-lc10_cuda", "-ltorch_cuda", "-nodefaultlibs", "-l:libstdc++.so.6", "-lm", "-lgcc_s", "-lgcc", "-lc"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
@@ -108,12 +118,13 @@ def _link_ext(obj: str, force: bool) -> None:
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
+    """The library, which needs nvcc alone, and then the bindings, which need torch and a host compiler."""
     os.makedirs(OBJDIR, exist_ok=True)
     srcs = _sources()
+    torch_there = importlib.util.find_spec("torch") is not None
     with ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as ex:
-        ext = ex.submit(_compile_ext, force)
+        ext = ex.submit(_compile_ext, force) if torch_there else None
         objs = list(ex.map(lambda s: _compile(s, force, verbose), srcs))
-        ext = ext.result()
     if force or not os.path.exists(LIB) or os.path.getmtime(LIB) < max(os.path.getmtime(o) for o in objs):
         tmp = LIB + ".tmp"
         cmd = [nvcc()] + ARCH + ["-shared", "-Xlinker", "-soname=liblq_sm100.so", "-o", tmp] + objs
@@ -121,7 +132,10 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         os.replace(tmp, LIB)
-    _link_ext(ext, force)
+    if ext is None:
+        sys.stderr.write("no torch here: lq_torch.so, its bindings, is not built\n")
+    else:
+        _link_ext(ext.result(), force)
     return LIB
 
 

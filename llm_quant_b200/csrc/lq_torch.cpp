@@ -271,6 +271,7 @@ class Clipper {
 }  // namespace
 
 PYBIND11_MODULE(lq_torch, m) {
+  m.attr("torch_version") = TORCH_VERSION;
   m.def("adapters_forward", &adapters_forward);
   m.def("adapters_add_", &adapters_add_);
   pybind11::class_<Clipper>(m, "Clipper")

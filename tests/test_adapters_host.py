@@ -212,3 +212,44 @@ def test_first_calls_of_many_threads(lib, monkeypatch):
     for t in threads:
         t.join()
     assert len(loads) == 1 and len(got) == 8 and all(m is loads[0] for m in got)
+
+
+def test_build_without_torch_or_a_host_compiler(lib, tmp_path, monkeypatch, capfd):
+    """The C library needs nvcc alone: it is linked whether or not its bindings can be."""
+    import os
+    import sys
+    from llm_quant_b200 import build
+    objects = {s: os.path.join(build.OBJDIR, s.replace(".cu", ".o")) for s in build._sources()}
+    monkeypatch.setattr(build, "_compile", lambda src, force, verbose: objects[src])
+    for name in ("LIBDIR", "OBJDIR", "LIB", "EXT"):
+        monkeypatch.setattr(build, name, str(tmp_path / os.path.basename(getattr(build, name))))
+    monkeypatch.setenv("CXX", str(tmp_path / "no_such_compiler"))
+    with pytest.raises((OSError, RuntimeError)):
+        build.build()
+    assert os.path.exists(build.LIB) and not os.path.exists(build.EXT)
+    os.remove(build.LIB)
+    monkeypatch.setitem(sys.modules, "torch", None)
+    assert build.build() == build.LIB and os.path.exists(build.LIB) and not os.path.exists(build.EXT)
+    assert "no torch" in capfd.readouterr().err
+
+
+def test_bindings_are_built_for_one_torch(lib, monkeypatch):
+    """Another torch: they are compiled again, and ones of another torch are not used."""
+    import subprocess
+    from llm_quant_b200 import _C, build
+    ran = []
+
+    def run(cmd, **kw):
+        ran.append(cmd)
+        return subprocess.CompletedProcess(cmd, 1, "", "stopped here")
+
+    monkeypatch.setattr(build.subprocess, "run", run)
+    build._compile_ext(False)
+    assert not ran
+    monkeypatch.setattr(torch, "__version__", "1.0.0")
+    with pytest.raises(RuntimeError, match="stopped here"):
+        build._compile_ext(False)
+    assert len(ran) == 1
+    monkeypatch.setattr(_C, "_ext", None)
+    with pytest.raises(RuntimeError, match="this is 1.0.0"):
+        _C.ext()
