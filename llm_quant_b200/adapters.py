@@ -100,9 +100,10 @@ class AdapterBatch:
               self.num_adapters, self._plan.data_ptr())
 
     def check(self) -> None:
-        """Wait for the batch's work and raise LQError if a kernel gave up a
-        wait on the device since the last ``update`` (its results are
-        incomplete then)."""
+        """Wait for the device, whichever streams the batch's work went to, and
+        raise LQError if a kernel gave up a wait there since the last ``update``
+        (its results are incomplete then)."""
+        torch.cuda.synchronize(self.device)
         status = int(self._plan[:4].view(torch.int32)) if self.tokens else _C.OK
         if status:
             raise _C.LQError("AdapterBatch", status, "a wait on the device ran out")

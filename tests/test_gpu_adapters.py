@@ -819,3 +819,18 @@ def test_parametrized_banks_and_hooks():
         every = torch.nn.modules.module.register_module_forward_hook(lambda m, args, out: seen.append(type(m)))
         assert torch.equal(ql(x, plain, batch), want) and L.AdapterBank in seen
         every.remove()
+
+
+def test_check_waits_for_other_streams():
+    """The status of work that is still on its way on a stream of its own (here a copy in its place) is waited for."""
+    batch = L.AdapterBatch(torch.zeros(4, dtype=torch.int32, device=DEV), 2)
+    batch.check()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)
+        batch._plan[:4].view(torch.int32).fill_(7)
+    with pytest.raises(RuntimeError, match="ran out"):
+        batch.check()
+    batch.update(torch.zeros(4, dtype=torch.int32, device=DEV))
+    batch.check()
