@@ -17,7 +17,9 @@ Activations are float16 or bfloat16.  Products are exact and summed in fp32;
 of itself in bfloat16, 2^-22 in float16), and each output is rounded once.
 Parameters may be float32 (a training run's master weights): they are rounded
 to the activations' dtype at each call and their gradients come in float32.
-Sums go in an order of their own: equal calls give equal bits.
+Sums go in an order of their own: equal calls give equal bits.  An infinite x or
+gradient gives what the formulas give; an infinite weight may give NaN where they
+give an infinity.
 
 Nothing here reads the device on the host, so plans, calls and their backward
 passes can be captured into a CUDA graph and replayed (as for any module, with

@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(kPlanThreads) ad_plan_kernel(const I* __restri
   const int first = base[0], tile = base[1], n = hist[me], n_tiles = (n + kAdTile - 1) / kAdTile;
   if (tid == 0) {
     p.start[me] = first, p.tile_of[me] = tile;
-    if (me == L) p.start[L + 1] = first + n, p.tile_of[L + 1] = tile + n_tiles, *p.status = LQ_OK;
+    if (me == L) p.start[L + 1] = first + n, p.tile_of[L + 1] = tile + n_tiles, *p.status = LQ_OK, *p.nan = 0;
   }
   const int owner = me == L ? -1 : me, each = seq <= kPlanShort ? 4 : 1;  // requests of a thread at a time
   int at = first;

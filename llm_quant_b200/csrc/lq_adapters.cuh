@@ -28,6 +28,7 @@ struct AdPlan {
   int* tile_of;  // [L + 2]
   AdTile* tiles;
   int* status;   // an lq_status: LQ_ETIMEOUT if a wait on the device ran out
+  int* nan;      // whether ad_outer left a sum that is no number, since the plan was made
 };
 
 __host__ __device__ inline int64_t ad_round4(int64_t n) { return (n + 3) / 4 * 4; }
@@ -44,6 +45,7 @@ __host__ __device__ inline int64_t ad_plan_ints(int64_t T, int64_t L) {
 __host__ __device__ inline AdPlan ad_plan(void* p, int64_t T, int64_t L) {
   AdPlan a;
   a.status = static_cast<int*>(p);
+  a.nan = a.status + 1;
   a.owner = a.status + 4;
   a.order = a.owner + ad_round4(T);
   a.start = a.order + ad_round4(T);

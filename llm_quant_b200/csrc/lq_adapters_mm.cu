@@ -911,6 +911,7 @@ __global__ void __launch_bounds__(kOuterLoaders + 32, 1)
       const uint32_t from = tmem + ((uint32_t)(warp & 3) << 21) + mt * 2 * NP;
       const bool starts = p.tile_of[owner] == t0, ends = p.tile_of[owner + 1] == last + 1;
       float* part = q.part + ((int64_t)blockIdx.y * 2 + (starts ? 1 : 0)) * R * q.K;
+      bool nan = false;
 #pragma unroll
       for (int r = 0; r < NP; r += 16) {
         uint32_t hi[16], lo[16];
@@ -922,10 +923,12 @@ __global__ void __launch_bounds__(kOuterLoaders + 32, 1)
         for (int k = 0; k < 16; ++k) {
           if (r + k >= R || my >= q.K) continue;
           const float w = (__uint_as_float(hi[k]) + __uint_as_float(lo[k])) * back;
+          nan |= w != w;
           if (starts && ends) static_cast<G*>(q.g)[((int64_t)owner * R + r + k) * q.K + my] = Ty<G>::from_f(w);
           else part[(int64_t)(r + k) * q.K + my] = w;
         }
       }
+      if (nan) *p.nan = 1;
       tc_fence_before();
       mbar_arrive(&free_);
       t0 = last + 1;
@@ -974,31 +977,73 @@ __global__ void __launch_bounds__(kOuterLoaders + 32, 1)
   if (warp == kOuterLoaders / 32) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols));
 }
 
+// Sums of one rank and 8 columns over an adapter's tokens in fp32, until all are no numbers.
+template <typename T>
+__device__ __forceinline__ void sum_again(const OuterSide<T>& q, const AdPlan& p, int l, int np, int r, int c, float (&s)[8]) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) s[k] = 0.0f;
+  const int first = p.start[l], rows = p.start[l + 1] - first;
+  const float* v = q.v.turned + ((int64_t)p.tile_of[l] * np + r) * 128;
+  for (int i0 = 0; i0 < rows; i0 += 128, v += (int64_t)np * 128) {
+#pragma unroll 4
+    for (int i = 0; i < min(128, rows - i0); ++i) {
+      Vec16<T> x;
+      x.u = *reinterpret_cast<const uint4*>(q.x + p.order[first + i0 + i] * q.stride + c);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s[k] = fmaf(v[i], Ty<T>::to_f(x.v[k]), s[k]);
+    }
+    bool some = false;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) some |= s[k] == s[k];
+    if (!some) return;
+  }
+}
+
 // What several groups left of an adapter, added in order, and zeros for
 // adapters without tokens.  A block to 2048 values of an adapter's [R, K].
+//
+// Where x is infinite, v's parts give no number although v itself may: 0 times it
+// where lo is 0, infinities of both signs where lo's sign is not hi's.  Sums that are
+// no numbers are taken again, then, from v as it is: some ms where all of a long
+// step's are, and one word to read in a call without any.
 template <typename T, typename G>
 __global__ void __launch_bounds__(256) ad_sum_kernel(const OuterSide<T> one, const OuterSide<T> two, int R, AdPlan p, int L,
-                                                     int groups, int blocks_one) {
+                                                     int groups, int blocks_one, int np) {
   pdl_wait();
   pdl_trigger();
-  const bool first_side = (int)blockIdx.x < blocks_one;
+  const bool first_side = (int)blockIdx.x < blocks_one, odd = *p.nan != 0;
   const OuterSide<T>& q = first_side ? one : two;
   const int l = blockIdx.y, a = p.tile_of[l], b = p.tile_of[l + 1];
   const int per = max(1, (p.tile_of[L] + groups - 1) / groups);
   const int ga = a / per, gb = (b - 1) / per;
-  if (a < b && ga == gb) return;
+  const bool there = a < b && ga == gb;  // in the gradient
+  if (there && !odd) return;
   const int64_t size = (int64_t)R * q.K;
   const int64_t i = ((int64_t)((int)blockIdx.x - (first_side ? 0 : blocks_one)) * 256 + threadIdx.x) * 8;
   if (i >= size) return;
+  G* g = static_cast<G*>(q.g) + (int64_t)l * size + i;
   float s[8];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) s[k] = 0.0f;
-  for (int j = ga; a < b && j <= gb; ++j) {
+  for (int k = 0; k < 8; ++k) s[k] = there ? Ty<G>::to_f(g[k]) : 0.0f;
+  for (int j = ga; !there && a < b && j <= gb; ++j) {
     const float4* w = reinterpret_cast<const float4*>(q.part + ((int64_t)j * 2 + (j == ga ? 1 : 0)) * size + i);
     const float4 x = w[0], y = w[1];
     s[0] += x.x, s[1] += x.y, s[2] += x.z, s[3] += x.w, s[4] += y.x, s[5] += y.y, s[6] += y.z, s[7] += y.w;
   }
-  G* g = static_cast<G*>(q.g) + (int64_t)l * size + i;
+  if (odd && a < b) {
+    bool nan = false;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) nan |= s[k] != s[k];
+    if (nan) {
+      float w[8];
+      const int r = (int)(i / q.K);
+      sum_again(q, p, l, np, r, (int)(i - (int64_t)r * q.K), w);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s[k] = s[k] != s[k] ? w[k] : s[k];
+    } else if (there) {
+      return;
+    }
+  }
 #pragma unroll
   for (int k = 0; k < 8; ++k) g[k] = Ty<G>::from_f(s[k]);
 }
@@ -1135,7 +1180,7 @@ int outer_np(const AdCall& a, const AdOuter& o) {
   LQ_TRY(launched("ad_outer_kernel"));
   const int64_t b1 = o.da ? (b.R * b.K + 2047) / 2048 : 0, b2 = o.db ? (b.R * b.N + 2047) / 2048 : 0;
   e = launch_pdl(ad_sum_kernel<T, G>, dim3((unsigned)(b1 + b2), (unsigned)b.L), dim3(256), 0, a.st, one, two, (int)b.R, a.plan,
-                 (int)b.L, (int)groups, (int)b1);
+                 (int)b.L, (int)groups, (int)b1, NP);
   LQ_REQUIRE(e == cudaSuccess, LQ_ECUDA, "ad_sum_kernel launch: %s", cudaGetErrorString(e));
   return launched("ad_sum_kernel");
 }

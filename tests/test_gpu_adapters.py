@@ -834,3 +834,50 @@ def test_check_waits_for_other_streams():
         batch.check()
     batch.update(torch.zeros(4, dtype=torch.int32, device=DEV))
     batch.check()
+
+
+def whole_numbers(n, seq, num, R, K, N, dt, seed, most=2):
+    """As make, in small whole numbers, whose products and sums fp32 holds exactly (scaling: powers of two)."""
+    g = torch.Generator(DEV).manual_seed(seed)
+
+    def rand(*shape):
+        return torch.randint(-most, most + 1, shape, generator=g, device=DEV).to(dt)
+
+    bank = L.AdapterBank(K, N, num, R, dtype=dt, device=DEV).requires_grad_(False)
+    bank.lora_A.copy_(rand(num, R, K))
+    bank.lora_B.copy_(rand(num, R, N))
+    bank.scaling.copy_(2.0 ** torch.randint(-1, 2, (num,), generator=g, device=DEV).float())
+    return bank, rand(n * seq, K), rand(n * seq, N), rand(n * seq, N)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("R", [5, 16, 64, 128])
+def test_infinities_in_gradients(R, dt):
+    """Infinite x and dy: gradients are infinite with the sign, and no numbers,
+    where the definition's are, in every form of a run; the others are as without
+    them.  (Whole numbers: sums are exact, signs and zeros certain.)"""
+    t = TYPES[dt]
+    n, seq, num, K, N = 6, 333, 3, 136, 264
+    bank, x, base, dy = whole_numbers(n, seq, num, R, K, N, t, seed=60)
+    bank.scaling.abs_()
+    bank = bank.float().requires_grad_(True)  # gradients in fp32: exact
+    inf = float("inf")
+    ids = torch.tensor([0, 2, 0, -1, 0, 2], dtype=torch.int32, device=DEV)
+    mixed = torch.randint(-1, num, (n * seq,), generator=torch.Generator().manual_seed(4)).int().to(DEV)
+    for batch, own in ((L.AdapterBatch(ids, num, seq), owners(ids, n, seq, num)),
+                       (L.AdapterBatch(mixed, num), owners(mixed, n * seq, 1, num))):
+        bad, bad_dy = x.clone(), dy.clone()
+        for row, column, value in ((7, 3, inf), (200, 64, -inf), (350, 100, inf), (1500, 100, -inf), (1700, 3, inf)):
+            bad[row, column] = value
+        for row, column, value in ((9, 17, -inf), (800, 33, inf), (801, 33, -inf), (1999 - 2, 263, inf)):
+            bad_dy[row, column] = value
+        for p, d in ((x, dy), (bad, dy), (x, bad_dy), (bad, bad_dy)):
+            y = bank(p, batch, base)
+            da, db = torch.autograd.grad(y, (bank.lora_A, bank.lora_B), d)
+            with torch.no_grad():
+                _, _, (ra, _), (rb, _) = reference(p, base, bank.lora_A, bank.lora_B, bank.scaling, own, d)
+            for got, want in ((da, ra), (db, rb)):
+                nan = want.isnan()
+                assert torch.equal(got.isnan(), nan)
+                assert torch.equal(got[~nan].double(), want[~nan])
+        batch.check()
