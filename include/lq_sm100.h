@@ -472,8 +472,9 @@ int lq_kv4_reset(const lq_kv4_cache* host_cache, void* stream);
  * adapter i:  out_t = base_t + scaling[i] B_i^T (A_i x_t), else out_t = base_t.
  * fp16 or bf16; K and N multiples of 8 up to 2^22, R up to 128, L up to 8192, up
  * to 2^24 tokens.  Products are summed in fp32; A x and B dy meet the next factor
- * in fp32 or as two 16-bit parts (off by 2^-16 of themselves in bf16, 2^-22 in
- * fp16), and each output is rounded once. */
+ * in fp32 or as two 16-bit parts (off by 2^-16 of themselves in bf16; in fp16 by
+ * 2^-22 of themselves, or by 2^-37 of the greatest beside them: of the token's
+ * values, or for da and db of the adapter's), and each output is rounded once. */
 typedef struct {
   const void* a;        /* [L, R, K] */
   const void* b;        /* [L, R, N] */

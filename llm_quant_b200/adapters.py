@@ -14,7 +14,9 @@ the case of one adapter).
 
 Activations are float16 or bfloat16.  Products are exact and summed in fp32;
 ``scaling * lora_A x`` meets lora_B in fp32 or as two 16-bit parts (off by 2^-16
-of itself in bfloat16, 2^-22 in float16), and each output is rounded once.
+of itself in bfloat16; in float16 2^-22, or 2^-37 of the greatest value beside it
+if that is more: of its token's or, in the sums of lora_A's and lora_B's gradients,
+of its adapter's), and each output is rounded once.
 Parameters may be float32 (a training run's master weights): they are rounded
 to the activations' dtype at each call and their gradients come in float32.
 Sums go in an order of their own: equal calls give equal bits.  An infinite x or

@@ -14,8 +14,10 @@
 // off by 2^-16 of itself (bf16; 2^-22 in fp16), far below the rounding of the
 // output, where one 16-bit value would be off as much as that.  fp16 has too
 // small a range for values nobody scaled: a row of u (an adapter's rows of v)
-// goes in times a power of two that puts its greatest below 2^13, which is
-// taken back from the fp32 sum.
+// goes in times a power of two that puts its greatest in [2^12, 2^13), which is
+// taken back from the fp32 sum.  A value 2^-15 of the greatest or less has a lo
+// below fp16's normal numbers, and is off by half of their step, 2^-25, which is
+// 2^-37 of the greatest at most (measured against 64 bits in the tests).
 #include "lq_adapters.cuh"
 #include "lq_tc.cuh"
 

@@ -881,3 +881,52 @@ def test_infinities_in_gradients(R, dt):
                 assert torch.equal(got.isnan(), nan)
                 assert torch.equal(got[~nan].double(), want[~nan])
         batch.check()
+
+
+def test_small_values_beside_great_ones():
+    """fp16: what meets a factor in two parts is off by 2^-22 of itself or, beside
+    much greater values, by 2^-37 of the greatest: of a token's ranks in y and dx,
+    of an adapter's tokens in the gradients.  Columns that are zero where the great
+    values are show the small ones alone."""
+    dt = torch.float16
+    n, seq, R, K, N = 2, 400, 16, 136, 264
+    bank, x, base, dy = make(n, seq, 2, R, K, N, dt, seed=61)
+    T = n * seq
+    own = owners(torch.tensor([1, 0]), n, seq, 2)
+    batch = L.AdapterBatch(torch.tensor([1, 0], device=DEV), 2, seq)
+    # tokens by 2^-18 to 2^8 of dy, ranks by 2^-20 to 1 of A and B (within fp16's normal numbers after their own sizes)
+    size = 2.0 ** -torch.randint(-8, 10, (T, 1), device=DEV, generator=torch.Generator(DEV).manual_seed(1)).double()
+    great = size.flatten() > 16
+    dy = (dy.double() * size).to(dt)
+    x = (x.double() * size.clamp(max=16)).to(dt)
+    x[great, :40] = 0
+    dy[great, :40] = 0
+    ranks = 2.0 ** -torch.arange(0, R, device=DEV).double()[None, :, None] / 4
+    with torch.no_grad():
+        bank.lora_A.copy_(bank.lora_A.double() * ranks * 8)
+        bank.lora_B.copy_(bank.lora_B.double() * ranks * 8)
+        bank.lora_A[:, :4, 60:90] = 0  # the great ranks have no part in these columns
+        bank.lora_B[:, :4, 60:90] = 0
+    bank = bank.float().requires_grad_(True)
+    x.requires_grad_(True)
+    y = bank(x, batch)
+    dx, da, db = torch.autograd.grad(y, (x, bank.lora_A, bank.lora_B), dy)
+    with torch.no_grad():
+        a, b, s = bank.lora_A.double(), bank.lora_B.double(), bank.scaling.double()
+        ry, rx, ra, rb = reference(x, None, a, b, bank.scaling, own, dy)
+        o = own.to(DEV)
+        u = torch.einsum("tk,trk->tr", x.double(), a[o]) * s[o][:, None]
+        v = torch.einsum("tn,trn->tr", dy.double(), b[o]) * s[o][:, None]
+
+        def check(got, want, terms, far):
+            half, tiny = (2.0 ** -11, 2.0 ** -25) if got.dtype == dt else (2.0 ** -24, 2.0 ** -133)
+            exact, mag = want
+            tol = half * exact.abs() + ((terms + 16) * 2.0 ** -23 + 2.0 ** -22) * mag + 2.0 ** -37 * far + tiny
+            err = (got.double() - exact).abs()
+            assert bool((err <= tol).all()), f"worst {float((err / tol).max())} of the tolerance"
+
+        check(y.detach(), ry, K + R, u.abs().amax(1, keepdim=True) * b.abs().sum(1)[o])
+        check(dx, rx, N + R, v.abs().amax(1, keepdim=True) * a.abs().sum(1)[o])
+        for got, want, terms, low, rows in ((da, ra, N, v, x), (db, rb, K, u, dy)):
+            far = torch.stack([low[o == i].abs().max() * rows.detach().double()[o == i].abs().sum(0) for i in range(2)])[:, None]
+            check(got, want, terms + seq, far)
