@@ -930,3 +930,55 @@ def test_small_values_beside_great_ones():
         for got, want, terms, low, rows in ((da, ra, N, v, x), (db, rb, K, u, dy)):
             far = torch.stack([low[o == i].abs().max() * rows.detach().double()[o == i].abs().sum(0) for i in range(2)])[:, None]
             check(got, want, terms + seq, far)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_whole_numbers(shape, dt):
+    """Small whole numbers: every product and every sum is exact in fp32 (and u and v
+    in two parts), in whatever order, so that y and dx are the definition's,
+    rounded once, and gradients in fp32 are the definition's."""
+    n, seq, num, R, K, N = shape
+    t = TYPES[dt]
+    bank, x, base, dy = whole_numbers(n, seq, num, R, K, N, t, seed=62)
+    bank = bank.float().requires_grad_(True)
+    ids = some_ids(n, num, n, n % 3 == 0)
+    counts = torch.randint(0, seq + 1, (n,), dtype=torch.int32, generator=torch.Generator().manual_seed(6)).to(DEV) if seq > 2 else None
+    batch = L.AdapterBatch(ids, num, seq, counts)
+    x.requires_grad_(True)
+    y = bank(x, batch, base)
+    dx, da, db = torch.autograd.grad(y, (x, bank.lora_A, bank.lora_B), dy)
+    with torch.no_grad():
+        served = bank(x, batch, base)
+        (ry, _), (rx, _), (ra, _), (rb, _) = reference(x, base, bank.lora_A, bank.lora_B, bank.scaling,
+                                                       owners(ids, n, seq, num, counts), dy)
+    for low, w in ((x.detach().float() @ bank.lora_A.detach().flatten(0, 1).T, "u"), (dy.float() @ bank.lora_B.detach().flatten(0, 1).T, "v")):
+        assert float(low.abs().max()) * 2 < 2 ** 14, w  # halves of up to twice that: 16 bits
+    assert max(float(g.abs().max()) for g in (ra, rb)) < 2 ** 22
+    for got, want in ((y, ry), (served, ry), (dx, rx)):
+        assert torch.equal(got.detach(), want.to(t))
+    assert torch.equal(da.double(), ra) and torch.equal(db.double(), rb)
+
+
+def test_whole_numbers_over_32_bits():
+    """As above, with more than 2^31 values in base, out and dy."""
+    dt = torch.bfloat16
+    T, K, N, R = 151_000, 64, 14336, 8
+    bank, x, base, _ = whole_numbers(1, T, 2, R, K, N, dt, seed=63)
+    bank = bank.float().requires_grad_(True)
+    batch = L.AdapterBatch(torch.tensor([1], device=DEV), 2, T)
+    x.requires_grad_(True)
+    y = bank(x, batch, base)
+    dx, da, db = torch.autograd.grad(y, (x, bank.lora_A, bank.lora_B), base)
+    y = y.detach()
+    a, b, s = bank.lora_A[1].detach().double(), bank.lora_B[1].detach().double(), float(bank.scaling[1])
+    ra, rb = torch.zeros(R, K, dtype=torch.float64, device=DEV), torch.zeros(R, N, dtype=torch.float64, device=DEV)
+    for i in range(0, T, 10_000):
+        xi, d = x.detach()[i:i + 10_000].double(), base[i:i + 10_000].double()
+        u, v = s * xi @ a.T, s * d @ b.T
+        ra += v.T @ xi
+        rb += u.T @ d
+        assert torch.equal(y[i:i + 10_000], (d + u @ b).to(dt))
+        assert torch.equal(dx[i:i + 10_000], (v @ a).to(dt))
+    assert torch.equal(da[1].double(), ra) and torch.equal(db[1].double(), rb)
+    assert not da[0].any() and not db[0].any()
