@@ -147,8 +147,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
         for (int i = 0; i < 8; ++i) v[i] = fmaf(w, f[i], v[i]);
       }
     }
-    if (G > 1) {
-      if (c != c0) __syncthreads();  // more was read
+    if (G > 1) {  // threads share columns where one pass has all of them
 #pragma unroll
       for (int i = 0; i < 8; ++i) more[i * kFewThreads + tid] = v[i];
       __syncthreads();
