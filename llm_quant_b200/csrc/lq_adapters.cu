@@ -185,15 +185,29 @@ extern "C" int lq_adapter_plan(const void* ids, int ids_dtype, int64_t n_ids, in
 
 // Whether a call takes ad_few, where every token reads its adapter's weights,
 // through L2 where tokens share them, or the tiles, where an adapter's tokens
-// share a read but two launches and a tile's fixed costs stand against it.
-// Measured (us, ad_few / tiles, K, N = 4096, ranks 16 and 64): 64 tokens of 1
-// adapter 5.6 / 14, 11 / 16, of 64 adapters 8.4 / 31, 21 / 41; 256 of 1 10.5 / 16,
-// 31 / 20, of 64 13 / 31, 44 / 41.  14336 to 4096 features, rank 64: 64 of 1
-// 20 / 23, 128 of 1 34 / 26, 128 of 64 52 / 63, 256 of 64 77 / 63.
+// share a read but two launches and a tile's fixed costs stand against it.  How
+// many adapters a call's tokens use is not known here: as many as there can be.
+// Measured (us on the device, ad_few / tiles, weights from memory, `users` adapters
+// in the bank and in use), over 420 shapes of ranks 16 to 128, 4096 to 14336 features
+// and 4 to 256 tokens, of which the choice below is over 5 % slower than the other in
+// 10, by 23 % at most.  B costs ad_few some three times what A does:
+//   rank  features     users  tokens
+//     16   4096  4096      1      64   4.5 / 10    256   7.9 / 11
+//     64   4096  4096      1      64   9.8 / 13     96    16 / 15    256    30 / 16
+//     64   4096  4096    all      64    16 / 30     96    25 / 42    256    50 / 91
+//     64   4096 14336      1      24    13 / 13     48    23 / 13     96    44 / 15
+//     64  14336  4096      1      48    18 / 20     64    18 / 20     96    32 / 22
+//    128  14336 14336      8      16    35 / 37     32    37 / 37     64    66 / 37
+//    128  14336 14336    all      16    40 / 49     64    88 / 139   256   312 / 534
+// and, where a block's columns of so many ranks are a longer chain than the tiles':
+//    128   4096 14336      1       1    25 / 13     16    22 / 15
+//    128   4096 14336      4       4    25 / 22
+//    128   4096 14336      8       8    26 / 28
 static bool few_tokens(const lq_adapter_bank& b, const lq_adapter_form* f) {
   if (f->keep || f->n > 1024) return false;
-  const int64_t weights = 2 * b.R * (b.K + b.N), users = f->n < b.L ? f->n : b.L;
-  return f->n <= 64 || f->n * weights <= (96 << 20) + 2 * users * weights;
+  const int64_t cost = b.R * (b.K + 3 * b.N), users = f->n < b.L ? f->n : b.L;
+  if (users <= 4 && 2 * b.R * b.N > (3 << 20)) return false;
+  return f->n * cost <= (112 << 20) + users * cost * 3 / 2;
 }
 
 extern "C" size_t lq_adapter_low_bytes(const lq_adapter_bank* bank, const lq_adapter_form* form) {
