@@ -391,11 +391,11 @@ __global__ void __launch_bounds__(160, 2) ad_down_kernel(const __grid_constant__
 // teams of two with bringing base.
 // ---------------------------------------------------------------------------
 // Blocks that go along a tile's rows side by side, so that 1024 bytes of a row are
-// asked for at a time.  It matters little: means of five runs were 166 us by one,
-// 164 by two, 163 by four, 162 by eight (16384 tokens, 14336 columns, rank 64), where
-// runs of one setting lay up to 8 us apart; eight prompts of up to 2048 tokens, and
-// one of 2048 tokens with 4096 columns and rank 16, showed no difference.
-constexpr int kUpBeside = 4;
+// asked for at a time: a call of 16384 tokens, rank 64, takes 194.7 us with four and
+// 198.1 with one at 14336 columns, 80.3 and 81.3 at 4096, 59.8 and 59.7 at 2048
+// (runs lie 0.3 us apart).  A group's share is rounded up to whole rounds of it, which
+// narrow rows are fewer than: 48.3 and 45.2 us at 1032 columns, 34.9 and 31.4 at 64.
+constexpr int kUpBeside = 2, kUpBesideFrom = 32;  // 1 << 2 blocks; chunks of 128 columns
 constexpr int kUpThreads = 704;  // 8 warps add, 8 take out, 4 bring base, 1 F, 1 has the products
 template <int NP>
 struct UpShared {
@@ -421,7 +421,7 @@ __device__ __forceinline__ uint32_t up_at(int row, int c16) { return (c16 >> 3) 
 template <typename T, int NP>
 __global__ void __launch_bounds__(kUpThreads, 1)
     ad_up_kernel(const __grid_constant__ RowsMap bm, const __grid_constant__ CUtensorMap fm, const Low low, int N, AdPlan p, int L,
-                 const T* base, int64_t base_stride, T* out, int64_t out_stride, int chunks) {
+                 const T* base, int64_t base_stride, T* out, int64_t out_stride, int chunks, int beside_log2) {
   using S = UpShared<NP>;
   using H = Half16<T>;
   constexpr int NS = S::stages, NF = S::fs, NI = S::images;
@@ -434,9 +434,9 @@ __global__ void __launch_bounds__(kUpThreads, 1)
   // it had ended: base, F and the plan are there, and only the low-rank rows are
   // waited for, by the warps that read them.  Nothing is written before them.
   // tokens without an adapter: nothing to do where out is base
-  const int wide = (chunks + kUpBeside - 1) / kUpBeside * kUpBeside;  // of a tile; what is behind the columns is empty
-  const int64_t units = (int64_t)p.tile_of[base == out ? L : L + 1] * (wide / kUpBeside);  // of each block of a group
-  const int64_t group = blockIdx.x / kUpBeside, groups = gridDim.x / kUpBeside;
+  const int beside = 1 << beside_log2, wide = (chunks + beside - 1) & -beside;  // of a tile; what is behind the columns is empty
+  const int64_t units = (int64_t)p.tile_of[base == out ? L : L + 1] * (wide >> beside_log2);  // of each block of a group
+  const int64_t group = blockIdx.x >> beside_log2, groups = gridDim.x >> beside_log2;
   const int64_t u0 = units * group / groups, u1 = units * (group + 1) / groups;
   const int n = (int)(u1 - u0);
   if (n == 0) return;
@@ -464,7 +464,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
   pdl_trigger();
   const uint32_t tmem = tmem_at;
   volatile int* fail = &failed;
-  int tile = (int)(u0 * kUpBeside / wide), chunk = (int)(u0 * kUpBeside - (int64_t)tile * wide + blockIdx.x % kUpBeside);
+  int tile = (int)(u0 * beside / wide), chunk = (int)(u0 * beside - (int64_t)tile * wide + (blockIdx.x & (beside - 1)));
   if (warp < 8) {
     // ---- add: a thread to a row ----
     pdl_wait();
@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
     float back = 1.0f;
     bool some = false;
     int known = -1;
-    for (int i = 0; i < n; ++i, chunk += kUpBeside) {
+    for (int i = 0; i < n; ++i, chunk += beside) {
       if (chunk >= wide) chunk -= wide, ++tile;
       if ((i & 1) != e) continue;
       const int slot = i % NS;
@@ -524,7 +524,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
     AdTile d = {};
     int tok = -1;  // lane k: of row (warp & 3) * 2 + k / 16 + 8 (k % 16)
     int known = -1;
-    for (int i = 0; i < n; ++i, chunk += kUpBeside) {
+    for (int i = 0; i < n; ++i, chunk += beside) {
       if (chunk >= wide) chunk -= wide, ++tile;
       if ((i & 1) != team) continue;
       const int slot = i % NS;
@@ -559,7 +559,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
     AdTile d = {};
     int tok[2] = {-1, -1};  // lane k: of rows row0(k) + 4 (k % 16), and 64 later
     int known = -1, sent = 0;
-    for (int i = 0; i < n; ++i, chunk += kUpBeside) {
+    for (int i = 0; i < n; ++i, chunk += beside) {
       if (chunk >= wide) chunk -= wide, ++tile;
       if ((i & 1) != team) continue;
       const int slot = i % NS;
@@ -609,7 +609,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
   } else if (warp == 20) {
     // ---- F: 128 columns of the adapter's rows, zeros behind the rank (they meet zeros of the image) ----
     int known = -1, owner = -1, sent = 0;
-    for (int i = 0; i < n; ++i, chunk += kUpBeside) {
+    for (int i = 0; i < n; ++i, chunk += beside) {
       if (chunk >= wide) chunk -= wide, ++tile;
       if (tile != known) owner = p.tiles[tile].owner, known = tile;
       if (owner < 0) continue;
@@ -634,9 +634,9 @@ __global__ void __launch_bounds__(kUpThreads, 1)
     // the tile's image, and the next one where there is room for two
     int known = -1, images = 0, sent = 0, b = 0, used = 0;
     int next = tile;  // the next tile whose image was not asked for
-    const int last = (int)((u1 - 1) * kUpBeside / wide);
+    const int last = (int)((u1 - 1) * beside / wide);
     bool some = false;
-    for (int i = 0; i < n && !*fail; ++i, chunk += kUpBeside) {
+    for (int i = 0; i < n && !*fail; ++i, chunk += beside) {
       if (chunk >= wide) chunk -= wide, ++tile;
       const int fs = used % NF, e = i & 1;
       if (tile != known) {
@@ -681,7 +681,7 @@ __global__ void __launch_bounds__(kUpThreads, 1)
         commit(&d_full[e]);
         commit(&f_empty[fs]);
         ++used;
-        if (i + 1 == n || chunk + kUpBeside >= wide) commit(&i_empty[b]);
+        if (i + 1 == n || chunk + beside >= wide) commit(&i_empty[b]);
       } else if (lane == 0) {
         mbar_arrive(&d_full[e]);
       }
@@ -1138,16 +1138,17 @@ int up_np(const AdCall& a, void* low, bool is_a, const void* base, int64_t bs, v
   using S = UpShared<NP>;
   const lq_adapter_bank& b = *a.bank;
   const int N = (int)(is_a ? b.K : b.N), chunks = (N + 127) / 128;
-  const int64_t tiles = ad_max_tiles(a.n, b.L), units = tiles * ((chunks + kUpBeside - 1) / kUpBeside);
-  const int64_t groups = units < num_sms() / kUpBeside ? units : num_sms() / kUpBeside;
+  const int beside_log2 = chunks < kUpBesideFrom ? 0 : kUpBeside, beside = 1 << beside_log2;
+  const int64_t tiles = ad_max_tiles(a.n, b.L), units = tiles * ((chunks + beside - 1) / beside);
+  const int64_t groups = units < num_sms() / beside ? units : num_sms() / beside;
   constexpr auto kern = ad_up_kernel<T, NP>;
   LQ_TRY(more_shared<kern>(S::bytes));
   RowsMap bm;
   CUtensorMap fm;
   LQ_TRY(map_rows<T>(&bm, base, a.n, N, bs, 128));
   LQ_TRY((map_factor<T, NP>(&fm, b, is_a)));
-  const cudaError_t e = launch_pdl(kern, dim3((unsigned)(groups * kUpBeside)), dim3(kUpThreads), S::bytes, a.st, bm, fm,
-                                   low_at<NP>(low, tiles, false), N, a.plan, (int)b.L, static_cast<const T*>(base), bs, static_cast<T*>(out), os, chunks);
+  const cudaError_t e = launch_pdl(kern, dim3((unsigned)(groups * beside)), dim3(kUpThreads), S::bytes, a.st, bm, fm,
+                                   low_at<NP>(low, tiles, false), N, a.plan, (int)b.L, static_cast<const T*>(base), bs, static_cast<T*>(out), os, chunks, beside_log2);
   LQ_REQUIRE(e == cudaSuccess, LQ_ECUDA, "ad_up_kernel launch: %s", cudaGetErrorString(e));
   return launched("ad_up_kernel");
 }
