@@ -5,9 +5,10 @@
 //   ad_outer   dA = sum v x^T     [256 columns x tokens] by [tokens x rank]
 // All three are bound by memory (2 R flops to 2 bytes of x): the point is to
 // read x, dy and base once, and to keep the loads coming.  With 16384 tokens,
-// 14336 columns and rank 64 in bf16: ad_down 80 us (470 MB, 5.9 TB/s), ad_up 157
-// (940 MB read and written, 6.0 TB/s), ad_outer of 4096 and 14336 columns 105
-// (604 MB, 5.8 TB/s); a copy reaches 6.4 TB/s.
+// 14336 columns and rank 64 in bf16, each launch by itself and nothing in L2 (events,
+// to 2 us): ad_down 82 us (470 MB, 5.7 TB/s), ad_up 160 (940 MB read and written,
+// 5.9 TB/s), ad_outer of 4096 and 14336 columns with ad_sum 117 (604 MB, 5.2 TB/s); a
+// copy reaches 6.4 TB/s.  In fp16 86, 158 and 119.
 //
 // u and v are fp32 sums.  Where they meet a 16-bit factor they go in as two
 // 16-bit values, hi = round(u) and lo = round(u - hi), and two products: u is then
@@ -400,7 +401,8 @@ constexpr int kUpThreads = 704;  // 8 warps add, 8 take out, 4 bring base, 1 F, 
 template <int NP>
 struct UpShared {
   // Two stages of base are being added to, two taken out, the others on their way
-  // (with three in all, each with its F, 226 us instead of the 157 above).  An even
+  // (with three in all, each with its F, the 16384 tokens above took 226 us where they
+  // took 157 with four and F by itself).  An even
   // number: a stage then is always the same team's and the same group's, who see
   // each of its phases (a barrier's parity tells a phase from the next one only, and
   // nothing else keeps the teams abreast).
@@ -839,9 +841,10 @@ __global__ void __launch_bounds__(kOuterLoaders + 32, 1)
         const int id = tid - kOuterX, k8 = id & 7, r0 = id >> 3;
         float v[2][VI][8];
         // whole pieces, the ones behind the run too (a tile's rows are all there, if
-        // nobody wrote them): a load under a condition, whose value is looked at
-        // before the next one, cost a trip to L2 each (370 us instead of 136).  Two
-        // steps are on their way: with one the trip was the step's time (140 us)
+        // nobody wrote them): loads under a condition, whose value is looked at before
+        // the next one, cost a trip to L2 each (a training step of 16384 tokens, rank 64,
+        // 741 us, without them 573).  Two steps are on their way: with one, and half of
+        // the warps, the trip was the step's time (the sums 140 us, with two 105)
         auto fetch = [&](int i, float (&w)[VI][8]) {
           const float* from = q.v.turned + (int64_t)(t0 + (i >> 1)) * NP * 128 + (i & 1) * 64 + k8 * 8;
 #pragma unroll

@@ -280,11 +280,12 @@ class QLoRALinear(nn.Module):
 
     def forward(self, x: torch.Tensor, adapters: Optional[AdapterBank] = None,
                 batch: Optional[AdapterBatch] = None) -> torch.Tensor:
-        """qlora.py:306-312.  With ``adapters`` and ``batch`` each token of x (fp16
-        or bf16) uses its own adapter of that bank in place of this layer's.  fp16 / bf16 activations of the base weight's dtype
+        """qlora.py:306-312.  fp16 / bf16 activations of the base weight's dtype
         take the fused NF4 kernel for the base product (the reference fails
         there: its bias and LoRA factors stay fp32), with the LoRA path in the
-        activations' dtype; other inputs follow the reference exactly."""
+        activations' dtype; other inputs follow the reference exactly.  With
+        ``adapters`` and ``batch`` each token of x (fp16 or bf16) uses its own
+        adapter of that bank in place of this layer's."""
         from . import nf4_linear
         if adapters is not None or batch is not None:
             return self._forward_adapters(x, adapters, batch)
