@@ -143,11 +143,10 @@ struct Adapters : torch::autograd::Function<Adapters> {
     ctx->save_for_backward({c.x, c.a, c.b, scaling, c.low});
     // not the plan: saved-tensor hooks may bring back copies, and its status word is read where it lies
     ctx->saved_data["plan"] = plan;
-    ctx->saved_data["version"] = static_cast<int64_t>(plan._version());
-    ctx->saved_data["shape"] = x.sizes().vec();
-    ctx->saved_data["type"] = static_cast<int64_t>(lora_a.scalar_type());
-    ctx->saved_data["adapters"] = num_adapters;
-    ctx->saved_data["base"] = base.has_value();
+    std::vector<int64_t> form = {static_cast<int64_t>(plan._version()), num_adapters, static_cast<int64_t>(lora_a.scalar_type()),
+                                 base.has_value()};
+    form.insert(form.end(), x.sizes().begin(), x.sizes().end());
+    ctx->saved_data["form"] = std::move(form);
     return c.out;
   }
 
@@ -157,19 +156,20 @@ struct Adapters : torch::autograd::Function<Adapters> {
     Tensor dy = grads[0];
     if (!dy.defined()) return out;
     const bool want[3] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2)};
-    if (ctx->saved_data["base"].toBool()) out[3] = dy;
+    const auto kept = ctx->saved_data["form"].toIntVector();  // the plan's version, adapters, the parameters' type, base, x's shape
+    const at::IntArrayRef shape = at::IntArrayRef(kept).slice(4);
+    if (kept[3]) out[3] = dy;
     if (!want[0] && !want[1] && !want[2]) return out;
     const auto saved = ctx->get_saved_variables();
     const Tensor plan = ctx->saved_data["plan"].toTensor();
-    TORCH_CHECK(static_cast<int64_t>(plan._version()) == ctx->saved_data["version"].toInt(),
+    TORCH_CHECK(static_cast<int64_t>(plan._version()) == kept[0],
                 "AdapterBank: the batch that gradients are computed for has been modified by an inplace operation "
                 "(AdapterBatch.update) since the forward call");
-    const auto type = static_cast<at::ScalarType>(ctx->saved_data["type"].toInt());
-    const auto shape = ctx->saved_data["shape"].toIntVector();
+    const auto type = static_cast<at::ScalarType>(kept[2]);
     // A hook may have laid them out anew, but what they hold has to be the same.
-    const int64_t L = ctx->saved_data["adapters"].toInt(), R = saved[1].dim() == 3 ? saved[1].size(1) : 0;
+    const int64_t L = kept[1], R = saved[1].dim() == 3 ? saved[1].size(1) : 0;
     const int64_t sizes[3][3] = {{L, R, shape.back()}, {L, R, dy.size(-1)}};
-    TORCH_CHECK(saved[0].sizes() == at::IntArrayRef(shape) && saved[1].sizes() == at::IntArrayRef(sizes[0], 3) &&
+    TORCH_CHECK(saved[0].sizes() == shape && saved[1].sizes() == at::IntArrayRef(sizes[0], 3) &&
                     saved[2].sizes() == at::IntArrayRef(sizes[1], 3) && saved[3].sizes() == at::IntArrayRef(L),
                 "AdapterBank: saved tensors came back with other shapes");
     for (const Tensor& t : saved)
