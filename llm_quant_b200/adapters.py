@@ -180,19 +180,28 @@ class AdapterBank(nn.Module):
         self.lora_B[index, r:] = 0
         self.scaling[index] = scaling
 
+    def _tensors(self):
+        """lora_A, lora_B and scaling: from the module's own tables (0.2 us less of a
+        call), and as attributes where they are not in these, as of a parametrized
+        bank or a replica."""
+        p = self._parameters
+        try:
+            return p["lora_A"], p["lora_B"], self._buffers["scaling"]
+        except KeyError:
+            return self.lora_A, self.lora_B, self.scaling
+
     # -- calls (checked, allocated for and differentiated in csrc/lq_torch.cpp) ------
     def forward(self, x: torch.Tensor, batch: AdapterBatch, base: Optional[torch.Tensor] = None) -> torch.Tensor:
         """base [..., out_features] (default zeros) plus each token's adapter of
         x [..., in_features], whose leading dimensions are the batch's tokens."""
-        return _C.ext().adapters_forward(x, self.lora_A, self.lora_B, self.scaling, base, batch._plan, batch.tokens,
-                                         batch.num_adapters)
+        return _C.ext().adapters_forward(x, *self._tensors(), base, batch._plan, batch.tokens, batch.num_adapters)
 
     def add_(self, y: torch.Tensor, x: torch.Tensor, batch: AdapterBatch) -> torch.Tensor:
         """y += each token's adapter of x, in place; no gradient (call it under
         ``torch.no_grad()``).  Rows of tokens without an adapter are not written.  y
         may be x, or share x's buffer, where no row of y overlaps another token's
         row of x."""
-        _C.ext().adapters_add_(y, x, self.lora_A, self.lora_B, self.scaling, batch._plan, batch.tokens, batch.num_adapters)
+        _C.ext().adapters_add_(y, x, *self._tensors(), batch._plan, batch.tokens, batch.num_adapters)
         return y
 
     def extra_repr(self) -> str:
