@@ -402,10 +402,9 @@ template <int NP>
 struct UpShared {
   // Two stages of base are being added to, two taken out, the others on their way
   // (with three in all, each with its F, the 16384 tokens above took 226 us where they
-  // took 157 with four and F by itself).  An even
-  // number: a stage then is always the same team's and the same group's, who see
-  // each of its phases (a barrier's parity tells a phase from the next one only, and
-  // nothing else keeps the teams abreast).
+  // took 157 with four and F by itself).  An even number: a stage then is always the
+  // same team's and the same group's, who see each of its phases (a barrier's parity
+  // tells a phase from the next one only, and nothing else keeps the teams abreast).
   static constexpr int stages = NP <= 32 ? 6 : 4;
   static constexpr int stage = 32768;                   // two halves of 64 columns, rows of 128 bytes, swizzled
   static constexpr int fs = NP <= 64 ? 2 : 1;           // stages of F
