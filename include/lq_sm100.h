@@ -500,8 +500,9 @@ typedef struct {
   int keep;
 } lq_adapter_form;
 /* out [n, N] = base [n, N] (NULL: 0; may be out itself) + the adapters' share of
- * x [n, K], whose rows out's may overlap only for the same token.  low: lq_adapter_low_bytes (0: may be NULL) for this call alone, or
- * until its backward call. */
+ * x [n, K], whose rows out's may overlap only for the same token.  low:
+ * lq_adapter_low_bytes (0: may be NULL) for this call alone, or until its backward
+ * call. */
 size_t lq_adapter_low_bytes(const lq_adapter_bank* host_bank, const lq_adapter_form* host_form);
 int lq_adapter_forward(const lq_adapter_bank* host_bank, const lq_adapter_form* host_form, void* plan, const void* x,
                        const void* base, void* out, void* low, size_t low_bytes, void* stream);

@@ -168,7 +168,7 @@ struct Adapters : torch::autograd::Function<Adapters> {
     const auto type = static_cast<at::ScalarType>(kept[2]);
     // A hook may have laid them out anew, but what they hold has to be the same.
     const int64_t L = kept[1], R = saved[1].dim() == 3 ? saved[1].size(1) : 0;
-    const int64_t sizes[3][3] = {{L, R, shape.back()}, {L, R, dy.size(-1)}};
+    const int64_t sizes[2][3] = {{L, R, shape.back()}, {L, R, dy.size(-1)}};
     TORCH_CHECK(saved[0].sizes() == shape && saved[1].sizes() == at::IntArrayRef(sizes[0], 3) &&
                     saved[2].sizes() == at::IntArrayRef(sizes[1], 3) && saved[3].sizes() == at::IntArrayRef(L),
                 "AdapterBank: saved tensors came back with other shapes");
