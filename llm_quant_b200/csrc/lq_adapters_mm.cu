@@ -971,24 +971,32 @@ __global__ void __launch_bounds__(kOuterLoaders + 32, 1)
   if (warp == kOuterLoaders / 32) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols));
 }
 
-// Sums of one rank and 8 columns over an adapter's tokens in fp32, until all are no numbers.
+// Sums of one rank and 8 columns over an adapter's tokens in fp32, or until all are no numbers.
 template <typename T>
 __device__ __forceinline__ void sum_again(const OuterSide<T>& q, const AdPlan& p, int l, int np, int r, int c, float (&s)[8]) {
+  constexpr int AHEAD = 8;  // tokens on their way
 #pragma unroll
   for (int k = 0; k < 8; ++k) s[k] = 0.0f;
   const int first = p.start[l], rows = p.start[l + 1] - first;
   const float* v = q.v.turned + ((int64_t)p.tile_of[l] * np + r) * 128;
-  for (int i0 = 0; i0 < rows; i0 += 128, v += (int64_t)np * 128) {
-#pragma unroll 4
-    for (int i = 0; i < min(128, rows - i0); ++i) {
-      Vec16<T> x;
-      x.u = *reinterpret_cast<const uint4*>(q.x + p.order[first + i0 + i] * q.stride + c);
+  for (int i0 = 0; i0 < rows; i0 += AHEAD) {
+    const float* u = v + (int64_t)(i0 >> 7) * np * 128 + (i0 & 127);
+    Vec16<T> x[AHEAD];
+    float w[AHEAD];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) s[k] = fmaf(v[i], Ty<T>::to_f(x.v[k]), s[k]);
+    for (int j = 0; j < AHEAD; ++j) {
+      const bool some = i0 + j < rows;
+      x[j].u = make_uint4(0u, 0u, 0u, 0u);
+      if (some) x[j].u = *reinterpret_cast<const uint4*>(q.x + p.order[first + i0 + j] * q.stride + c);
+      w[j] = some ? u[j] : 0.0f;
     }
-    bool some = false;
+    bool some = false;  // a sum that may still be one
 #pragma unroll
-    for (int k = 0; k < 8; ++k) some |= s[k] == s[k];
+    for (int k = 0; k < 8; ++k) {
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) s[k] = fmaf(w[j], Ty<T>::to_f(x[j].v[k]), s[k]);
+      some |= s[k] == s[k];
+    }
     if (!some) return;
   }
 }
@@ -998,8 +1006,10 @@ __device__ __forceinline__ void sum_again(const OuterSide<T>& q, const AdPlan& p
 //
 // Where x is infinite, v's parts give no number although v itself may: 0 times it
 // where lo is 0, infinities of both signs where lo's sign is not hi's.  Sums that are
-// no numbers are taken again, then, from v as it is: some ms where all of a long
-// step's are, and one word to read in a call without any.
+// no numbers are taken again, then, from v as it is; a call without any reads one word.
+// A backward pass of 16384 tokens, 4096 to 14336 features, rank 64, of 0.32 ms takes 1.6
+// with one infinite value in x and 2.1 with a token of dy infinite (by the number of
+// loads on their way: with a token at a time 3.8 and 4.0).
 template <typename T, typename G>
 __global__ void __launch_bounds__(256) ad_sum_kernel(const OuterSide<T> one, const OuterSide<T> two, int R, AdPlan p, int L,
                                                      int groups, int blocks_one, int np) {
