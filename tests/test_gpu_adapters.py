@@ -982,3 +982,34 @@ def test_whole_numbers_over_32_bits():
         assert torch.equal(dx[i:i + 10_000], (v @ a).to(dt))
     assert torch.equal(da[1].double(), ra) and torch.equal(db[1].double(), rb)
     assert not da[0].any() and not db[0].any()
+
+
+def test_checkpointed_calls():
+    """Activation checkpointing: what the forward call saved is computed again in the backward pass."""
+    from torch.utils.checkpoint import checkpoint
+    bank, x, base, dy = make(3, 70, 2, 16, 128, 256, torch.bfloat16, seed=64)
+    bank.requires_grad_(True)
+    x.requires_grad_(True)
+    batch = L.AdapterBatch(some_ids(3, 2, 4, True), 2, 70)
+    leaves = (x, bank.lora_A, bank.lora_B)
+    want = torch.autograd.grad(bank(x, batch, base), leaves, dy)
+    got = torch.autograd.grad(checkpoint(bank, x, batch, base, use_reentrant=False), leaves, dy)
+    checkpoint(bank, x, batch, base, use_reentrant=True).backward(dy)
+    for p, q, w in zip(got, leaves, want):
+        assert torch.equal(p, w) and torch.equal(q.grad, w)
+
+
+def test_a_flag_of_infinities_changes_nothing_later():
+    """A plan keeps that a call with it had sums that are no number; its later calls give what they give without."""
+    bank, x, base, dy = make(4, 300, 2, 24, 136, 264, torch.float16, seed=65)
+    bank.requires_grad_(True)
+    ids = some_ids(4, 2, 4, True)
+    leaves = (bank.lora_A, bank.lora_B)
+    want = torch.autograd.grad(bank(x, L.AdapterBatch(ids, 2, 300), base), leaves, dy)
+    batch = L.AdapterBatch(ids, 2, 300)
+    bad = x.clone()
+    bad[torch.arange(0, 1200, 7), 3] = float("inf")
+    assert not torch.autograd.grad(bank(bad, batch, base), leaves, dy)[0].isfinite().all()
+    for _ in range(2):
+        got = torch.autograd.grad(bank(x, batch, base), leaves, dy)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
